@@ -612,6 +612,35 @@ typedef struct m3s_gemv_fused_args {
 } m3s_gemv_fused_args;
 int32_t m3s_gemv_fused(const m3s_gemv_fused_args* args, void* stream);
 
+/* The LM's embedding: y[t] = scale table[ids[t]] (the lookup of model.py:194-232, with a
+ * scale), and its gradient dtable[v] = scale sum of dy[t] over the t with ids[t] = v, summed in
+ * float32 in position order and rounded once (bit-reproducible). Rows of ids that do not occur,
+ * and of padding_idx, are zeros. An id outside [0, vocab) gives a row of NaN in y and adds to no
+ * row. y, dy and dtable are dense, aligned to one element; vocab < 2^31 - 1, width < 2^22,
+ * tokens < 2^31 - 32. */
+typedef struct m3s_embed_args {
+  int32_t struct_size;   /* sizeof(m3s_embed_args) */
+  int32_t dtype;         /* M3S_DTYPE_* of table, y, dy and dtable */
+  int32_t id_bytes;      /* 4 or 8: int32 or int64 ids */
+  int32_t vocab, width;
+  float scale;
+  int64_t tokens;
+  int64_t padding_idx;   /* backward: the id whose row gets no gradient, or -1 */
+  const void* ids;       /* (tokens) */
+  const void* table;     /* forward in (vocab, width) */
+  int64_t table_stride;  /* elements from one table row to the next, >= 0 */
+  void* y;               /* forward out (tokens, width) */
+  const void* dy;        /* backward in (tokens, width) */
+  void* dtable;          /* backward out (vocab, width) */
+  void* workspace;       /* backward scratch, 16-byte aligned */
+  int64_t workspace_bytes; /* its size, at least m3s_embed_bwd_workspace_bytes() */
+} m3s_embed_args;
+/* The sorted ids and positions, digit counts, row spans and float32 partial sums. -1 on bad
+ * dimensions. No counterpart in the reference. */
+int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t width);
+int32_t m3s_embed_fwd(const m3s_embed_args* args, void* stream);
+int32_t m3s_embed_bwd(const m3s_embed_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,7 +16,7 @@ import torch  # noqa: F401  (must precede the C-ABI library load)
 
 from . import convert, kernels, layout  # noqa: F401
 from . import kernel_bwd, kernel_decode, kernel_fwd  # noqa: F401
-from . import checkpoint, model, train  # noqa: F401
+from . import checkpoint, model, tokens, train  # noqa: F401
 from .kernels import (  # noqa: F401
     ForwardResiduals, KernelGrads, SISOGrads, decode_loop, decode_scan, decode_step,
     siso_backward, siso_backward_kernel, siso_decode, siso_decode_folded, siso_forward,
@@ -31,3 +31,4 @@ from .scan_prep import (  # noqa: F401
     zero_state,
 )
 from .siso import SISOOutput, siso, siso_segment  # noqa: F401
+from .tokens import embed_tokens  # noqa: F401

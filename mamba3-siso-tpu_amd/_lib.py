@@ -224,6 +224,15 @@ class GemvFusedArgs(C.Structure):
     ]
 
 
+class EmbedArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", i32), ("dtype", i32), ("id_bytes", i32), ("vocab", i32), ("width", i32),
+        ("scale", C.c_float), ("tokens", i64), ("padding_idx", i64),
+        ("ids", vp), ("table", vp), ("table_stride", i64), ("y", vp), ("dy", vp), ("dtable", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
+    ]
+
+
 #: ``M3S_GEMV_*``
 GEMV_NORM, GEMV_GATE, GEMV_HEAD = 1, 2, 3
 
@@ -237,7 +246,7 @@ EXPORTS = ("m3s_abi_version", "m3s_last_error", "m3s_supported", "m3s_fwd_raw_su
            "m3s_norm_bwd", "m3s_decode_layer", "m3s_transpose", "m3s_swiglu_fwd",
            "m3s_swiglu_bwd", "m3s_rms_fwd", "m3s_rms_bwd", "m3s_rms_bwd_workspace_bytes",
            "m3s_norm_bwd_noalloc", "m3s_adamw", "m3s_wgrad", "m3s_wgrad_workspace_bytes", "m3s_gemv",
-           "m3s_gemv_fused")
+           "m3s_gemv_fused", "m3s_embed_bwd_workspace_bytes", "m3s_embed_fwd", "m3s_embed_bwd")
 
 _lib = None
 
@@ -329,6 +338,11 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     lib.m3s_gemv.argtypes = [C.POINTER(GemvArgs), vp]
     lib.m3s_gemv_fused.restype = i32
     lib.m3s_gemv_fused.argtypes = [C.POINTER(GemvFusedArgs), vp]
+    lib.m3s_embed_bwd_workspace_bytes.restype = i64
+    lib.m3s_embed_bwd_workspace_bytes.argtypes = [i64, i32, i32]
+    for fn in (lib.m3s_embed_fwd, lib.m3s_embed_bwd):
+        fn.restype = i32
+        fn.argtypes = [C.POINTER(EmbedArgs), vp]
     _lib = lib
     return lib
 

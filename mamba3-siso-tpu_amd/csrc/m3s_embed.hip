@@ -1,0 +1,566 @@
+// The language model's embedding on gfx950: the scaled lookup and the table's gradient.
+//
+//   forward:   y[t] = scale table[id_t]
+//   backward:  dtable[v] = scale sum_{t : id_t = v} dy[t], v != padding_idx
+//
+// The lookup is a gather of whole rows, bound by HBM (the output; a byte LM's table stays in L2).
+//
+// The gradient is a sum of rows by token id. Adding rows into the table with atomics would make
+// the result depend on the order of arrival and would serialise on the commonest ids (the first
+// of 256 Zipf-distributed bytes stands on a sixth of all positions). So the positions are sorted
+// by id, stably, and each id's rows stand together in position order:
+//
+//   1. least-significant-digit radix sort of (id, position), at most 9 bits a pass: one pass for
+//      bytes, two up to 2^18 ids. Ranks within a wave come from ballots (lanes with the same digit
+//      find each other bit by bit), across waves and workgroups from digit counts, so the order
+//      is that of the positions whatever runs first. Up to 4096 tokens one workgroup sorts in LDS.
+//   2. run_sum: a wave adds kRun sorted rows, 256 columns of them. A run of equal ids inside the
+//      piece is finished and written; one that crosses a border leaves a float32 partial.
+//   3. finish: a workgroup per table row adds the partials of a run that crosses pieces, in order,
+//      and writes zeros for ids that never occur.
+//
+// Every sum is float32 in a fixed order, rounded once. The gradient reads dy once and writes the
+// table once: bound by HBM from a few MB on, by the launches below that.
+#include <algorithm>
+
+#include "m3s_common.h"
+#include "m3s_internal.h"
+
+namespace m3s {
+
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kDigits = 512;          // counters of a pass: digits of up to 9 bits
+constexpr int kDigitBits = 9;
+constexpr int kSortOne = 4096;        // tokens that one workgroup sorts alone, in LDS
+constexpr int kSortRounds = kSortOne / kSortThreads;
+constexpr int kSortBlocks = 256;      // workgroups of a larger sort, at most
+constexpr int kRun = 32;              // sorted rows that a wave of run_sum adds
+
+// Four consecutive elements at any element alignment (gfx950 takes 16-byte accesses there).
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+__device__ __forceinline__ f32x4 ld4u(const float* p) { return *reinterpret_cast<const f32x4_u*>(p); }
+__device__ __forceinline__ f32x4 ld4u(const bf16* p) {
+  const bf16x4 r = *reinterpret_cast<const bf16x4_u*>(p);
+  return f32x4{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
+}
+__device__ __forceinline__ void st4u(float* p, f32x4 v) { *reinterpret_cast<f32x4_u*>(p) = v; }
+__device__ __forceinline__ void st4u(bf16* p, f32x4 v) {
+  *reinterpret_cast<bf16x4_u*>(p) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
+}
+// W = 4 columns of a row, or one of a row narrower than that. Lanes take 4 columns each and the
+// last one steps back to the row's end: it and its neighbour then hold some columns both, read,
+// add and write the same numbers for them, and no row needs a ragged edge.
+template <int W, typename T>
+__device__ __forceinline__ f32x4 ld_cols(const T* p) {
+  if constexpr (W == 4) return ld4u(p);
+  return f32x4{(float)p[0], 0.f, 0.f, 0.f};
+}
+template <int W, typename T>
+__device__ __forceinline__ void st_cols(T* p, f32x4 v) {
+  if constexpr (W == 4) st4u(p, v);
+  else p[0] = (T)v[0];
+}
+
+// ---- lookup -----------------------------------------------------------------------------
+// 2^lg lanes to a row. An id outside the table reads nothing and gives a row of NaN.
+template <int W, typename T, typename ID>
+__global__ void __launch_bounds__(256) embed_fwd_kernel(const T* __restrict__ table, int64_t ld,
+                                                        const ID* __restrict__ ids,
+                                                        T* __restrict__ y, int64_t n, int vocab,
+                                                        int D, float scale, int lg) {
+  const int step = W << lg, c0 = W * (threadIdx.x & ((1 << lg) - 1));
+  const int64_t hop = ((int64_t)gridDim.x * 256) >> lg;
+  for (int64_t t = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> lg; t < n; t += hop) {
+    const int64_t id = (int64_t)ids[t];
+    T* out = y + t * D;
+    int c = c0;
+    if (id < 0 || id >= vocab) {
+      const float nan = __builtin_nanf("");
+      for (; c < D; c += step) st_cols<W>(out + min(c, D - W), f32x4{nan, nan, nan, nan});
+      continue;
+    }
+    const T* row = table + id * ld;
+    for (; c + 3 * step + W <= D; c += 4 * step) {
+      f32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = ld_cols<W>(row + c + u * step);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) st_cols<W>(out + c + u * step, v[u] * scale);
+    }
+    for (; c < D; c += step) {
+      const int cc = min(c, D - W);
+      st_cols<W>(out + cc, ld_cols<W>(row + cc) * scale);
+    }
+  }
+}
+
+// ---- stable sort of positions by id --------------------------------------------------------
+// What sorts last and is never summed: the padding id, and ids outside the table.
+template <typename ID>
+__device__ __forceinline__ uint32_t sort_key(ID raw, int vocab, int64_t pad) {
+  const int64_t id = (int64_t)raw;
+  return id >= 0 && id < vocab && id != pad ? (uint32_t)id : (uint32_t)vocab;
+}
+
+// The lanes that hold this lane's digit, among those of `valid`.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits, uint64_t valid) {
+  uint64_t m = valid;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1;
+    const uint64_t bal = __ballot(one);
+    m &= one ? bal : ~bal;
+  }
+  return m;
+}
+
+// The place of one key of the wave's 64: next[] holds the wave's next free place of each digit.
+// Every lane of the wave calls it; an invalid lane's result means nothing.
+__device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t digit, int bits, bool ok) {
+  const uint64_t peers = same_digit(digit, bits, __ballot(ok));
+  const uint64_t below = peers & ((1ull << lane_id()) - 1);
+  uint32_t at = 0;
+  if (ok) at = next[digit];
+  __builtin_amdgcn_wave_barrier();   // every lane has read before a digit's first lane adds
+  if (ok && below == 0) next[digit] = at + (uint32_t)__popcll(peers);
+  __builtin_amdgcn_wave_barrier();
+  return at + (uint32_t)__popcll(below);
+}
+
+// cnt[wave][digit] -> the first place of that wave's keys of that digit: digits in order, then
+// waves; `before` (this thread's digit, threadIdx.x < kDigits) is what earlier workgroups hold and
+// `total` what all of them do. Uses scan[kDigits]; called by all kSortThreads.
+__device__ __forceinline__ void digit_places(uint32_t (*cnt)[kDigits], uint32_t* scan,
+                                             uint32_t before, uint32_t total) {
+  const int d = threadIdx.x;
+  if (d < kDigits) scan[d] = total;
+  __syncthreads();
+  for (int s = 1; s < kDigits; s <<= 1) {   // inclusive prefix sum over the digits
+    uint32_t add = 0;
+    if (d < kDigits && d >= s) add = scan[d - s];
+    __syncthreads();
+    if (d < kDigits) scan[d] += add;
+    __syncthreads();
+  }
+  if (d < kDigits) {
+    uint32_t at = scan[d] - total + before;
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = cnt[w][d];
+      cnt[w][d] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ void zero_counts(uint32_t (*cnt)[kDigits]) {
+  for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) cnt[i / kDigits][i % kDigits] = 0;
+}
+
+// Up to kSortOne tokens: block 0 sorts, the others clear start and stop (span = 2 vocab ints).
+// Wave w holds the kSortRounds * 64 keys from w * kSortRounds * 64 on.
+template <typename ID>
+__global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const ID* __restrict__ ids,
+                                                                uint32_t* __restrict__ keys,
+                                                                uint32_t* __restrict__ pos,
+                                                                int32_t* __restrict__ span,
+                                                                int64_t span_n, int n, int vocab,
+                                                                int64_t pad, int passes, int bits) {
+  if (blockIdx.x > 0) {
+    for (int64_t i = (int64_t)(blockIdx.x - 1) * kSortThreads + threadIdx.x; i < span_n;
+         i += (int64_t)(gridDim.x - 1) * kSortThreads) {
+      span[i] = 0;
+    }
+    return;
+  }
+  __shared__ uint32_t cnt[kSortWaves][kDigits];
+  __shared__ uint32_t scan[kDigits];
+  __shared__ uint32_t skey[kSortOne];
+  __shared__ uint16_t spos[kSortOne];
+  const int wave = threadIdx.x >> 6, lane = lane_id();
+  const int i0 = wave * kSortRounds * 64 + lane;
+  uint32_t key[kSortRounds], p[kSortRounds];
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const int i = i0 + 64 * r;
+    key[r] = i < n ? sort_key(ids[i], vocab, pad) : 0u;
+    p[r] = (uint32_t)i;
+  }
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * bits;
+    const uint32_t mask = (1u << bits) - 1;
+    zero_counts(cnt);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      if (i0 + 64 * r < n) atomicAdd(&cnt[wave][(key[r] >> shift) & mask], 1u);
+    }
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < kDigits) {
+      for (int w = 0; w < kSortWaves; ++w) total += cnt[w][threadIdx.x];
+    }
+    digit_places(cnt, scan, 0u, total);
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      const bool ok = i0 + 64 * r < n;
+      const uint32_t at = take_place(cnt[wave], (key[r] >> shift) & mask, bits, ok);
+      if (ok && at < (uint32_t)n) {
+        skey[at] = key[r];
+        spos[at] = (uint16_t)p[r];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r) {
+      const int i = i0 + 64 * r;
+      if (i < n) {
+        key[r] = skey[i];
+        p[r] = spos[i];
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int r = 0; r < kSortRounds; ++r) {
+    const int i = i0 + 64 * r;
+    if (i < n) {
+      keys[i] = key[r];
+      pos[i] = p[r];
+    }
+  }
+}
+
+// More tokens: workgroup b holds the `tile` keys from b tile on (tile a multiple of kSortThreads).
+// First the counts of each workgroup's digits ...
+template <typename ID, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const ID* __restrict__ ids,
+                                                                  const uint32_t* __restrict__ keys,
+                                                                  uint32_t* __restrict__ hist,
+                                                                  int32_t* __restrict__ span,
+                                                                  int64_t span_n, int64_t n,
+                                                                  int tile, int vocab, int64_t pad,
+                                                                  int shift, int bits) {
+  __shared__ uint32_t cnt[kDigits];
+  if (FIRST) {
+    for (int64_t i = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; i < span_n;
+         i += (int64_t)gridDim.x * kSortThreads) {
+      span[i] = 0;
+    }
+  }
+  if (threadIdx.x < kDigits) cnt[threadIdx.x] = 0;
+  __syncthreads();
+  const uint32_t mask = (1u << bits) - 1;
+  const int64_t lo = (int64_t)blockIdx.x * tile, hi = lo + tile < n ? lo + tile : n;
+  for (int64_t i = lo + threadIdx.x; i < hi; i += kSortThreads) {
+    const uint32_t k = FIRST ? sort_key(ids[i], vocab, pad) : keys[i];
+    atomicAdd(&cnt[(k >> shift) & mask], 1u);
+  }
+  __syncthreads();
+  if (threadIdx.x < kDigits) hist[(int64_t)blockIdx.x * kDigits + threadIdx.x] = cnt[threadIdx.x];
+}
+
+// ... then every key to its place. Wave w of a workgroup holds tile / kSortWaves keys in a row.
+template <typename ID, bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(
+    const ID* __restrict__ ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
+    uint32_t* __restrict__ okeys, uint32_t* __restrict__ opos, const uint32_t* __restrict__ hist,
+    int64_t n, int tile, int vocab, int64_t pad, int shift, int bits) {
+  __shared__ uint32_t cnt[kSortWaves][kDigits];
+  __shared__ uint32_t scan[kDigits];
+  const int wave = threadIdx.x >> 6, lane = lane_id();
+  const uint32_t mask = (1u << bits) - 1;
+  const int share = tile / kSortWaves;
+  const int64_t lo = (int64_t)blockIdx.x * tile + (int64_t)wave * share;
+  zero_counts(cnt);
+  __syncthreads();
+  for (int r = 0; r < share; r += 64) {
+    const int64_t i = lo + r + lane;
+    if (i < n) {
+      const uint32_t k = FIRST ? sort_key(ids[i], vocab, pad) : keys[i];
+      atomicAdd(&cnt[wave][(k >> shift) & mask], 1u);
+    }
+  }
+  uint32_t before = 0, total = 0;
+  if (threadIdx.x < kDigits) {
+#pragma unroll 8
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const uint32_t h = hist[(int64_t)b * kDigits + threadIdx.x];
+      total += h;
+      if (b < (int)blockIdx.x) before += h;
+    }
+  }
+  __syncthreads();
+  digit_places(cnt, scan, before, total);
+  for (int r = 0; r < share; r += 64) {
+    const int64_t i = lo + r + lane;
+    const bool ok = i < n;
+    uint32_t k = 0;
+    if (ok) k = FIRST ? sort_key(ids[i], vocab, pad) : keys[i];
+    const uint32_t at = take_place(cnt[wave], (k >> shift) & mask, bits, ok);
+    if (ok && at < (uint64_t)n) {   // always, unless the ids change under the sort
+      okeys[at] = k;
+      opos[at] = FIRST ? (uint32_t)i : pos[i];
+    }
+  }
+}
+
+// ---- sums by id ------------------------------------------------------------------------------
+// A wave adds the sorted rows kRun * piece .. of its 64 W columns. part (pieces, 2, D): slot 0 a
+// run that came from the piece before (and may go on), slot 1 one that starts here and goes on.
+template <int W, typename T>
+__global__ void __launch_bounds__(256) run_sum_kernel(const uint32_t* __restrict__ keys,
+                                                      const uint32_t* __restrict__ pos,
+                                                      const T* __restrict__ dy,
+                                                      T* __restrict__ dtable,
+                                                      float* __restrict__ part,
+                                                      int32_t* __restrict__ start,
+                                                      int32_t* __restrict__ stop, int64_t n,
+                                                      int vocab, int D, float scale, int tiles) {
+  const int lane = lane_id();
+  const uint32_t none = 0xffffffffu;
+  const int64_t work = (n + kRun - 1) / kRun * tiles;
+  for (int64_t g = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); g < work; g += (int64_t)gridDim.x * 4) {
+    const int64_t piece = g / tiles;
+    const int tile = (int)(g - piece * tiles);
+    const int64_t i0 = piece * kRun;
+    const int held = n - i0 < kRun ? (int)(n - i0) : kRun;
+    uint32_t key = none, p = 0;
+    if (lane < held) {
+      key = keys[i0 + lane];
+      p = (uint32_t)min((int64_t)pos[i0 + lane], n - 1);
+    }
+    const uint32_t kprev = i0 > 0 ? keys[i0 - 1] : none;
+    const uint32_t knext = i0 + held < n ? keys[i0 + held] : none;
+    const int rows = __popcll(__ballot(lane < held && key < (uint32_t)vocab));   // the rest sorts last
+    if (tile == 0) {
+      uint32_t l = __shfl_up(key, 1), r = __shfl_down(key, 1);
+      if (lane == 0) l = kprev;
+      if (lane == held - 1) r = knext;
+      if (lane < rows && l != key) start[key] = (int32_t)(i0 + lane);
+      if (lane < rows && r != key) stop[key] = (int32_t)(i0 + lane + 1);
+    }
+    const bool mine = W * (64 * tile + lane) < D;   // lanes past the row load its end and drop it
+    const int c = min(W * (64 * tile + lane), D - W);
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    int from = 0;
+    for (int j0 = 0; j0 < rows; j0 += 8) {
+      f32x4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int j = min(j0 + u, rows - 1);
+        const int64_t row = (int64_t)(uint32_t)__builtin_amdgcn_readlane((int)p, j);
+        v[u] = ld_cols<W>(dy + row * D + c);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int j = j0 + u;
+        if (j >= rows) break;
+        acc += v[u];
+        const uint32_t k = (uint32_t)__builtin_amdgcn_readlane((int)key, j);
+        const uint32_t kn = j + 1 < held ? (uint32_t)__builtin_amdgcn_readlane((int)key, j + 1) : knext;
+        if (j + 1 < rows && kn == k) continue;
+        if (mine) {
+          if (from == 0 && kprev == k) st_cols<W>(part + 2 * piece * D + c, acc);
+          else if (kn == k) st_cols<W>(part + (2 * piece + 1) * D + c, acc);
+          else st_cols<W>(dtable + (int64_t)k * D + c, acc * scale);
+        }
+        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        from = j + 1;
+      }
+    }
+  }
+}
+
+// The rest of the table: `each` rows to a workgroup, 64 W columns (blockIdx.y). Rows of a run
+// inside one piece are done. The four waves add a quarter of the partials each.
+template <int W, typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ part,
+                                                     const int32_t* __restrict__ start,
+                                                     const int32_t* __restrict__ stop,
+                                                     T* __restrict__ dtable, int vocab, int D,
+                                                     float scale, int each) {
+  __shared__ f32x4 sums[4][64];
+  const int lane = lane_id(), wave = threadIdx.x >> 6;
+  const bool mine = W * (64 * (int)blockIdx.y + lane) < D;
+  const int c = min(W * (64 * (int)blockIdx.y + lane), D - W);
+  const int64_t v0 = (int64_t)blockIdx.x * each;
+  const int64_t v1 = v0 + each < vocab ? v0 + each : vocab;
+  for (int64_t v = v0; v < v1; ++v) {
+    const int s = start[v], e = stop[v];
+    if (s == e) {   // an id that never occurs
+      if (wave == (int)(v & 3) && mine) st_cols<W>(dtable + v * D + c, f32x4{0.f, 0.f, 0.f, 0.f});
+      continue;
+    }
+    const int64_t p0 = s / kRun, p1 = (e - 1) / kRun;
+    if (p0 == p1) continue;
+    const int64_t count = p1 - p0 + 1, share = (count + 3) / 4;
+    const int64_t lo = wave * share, hi = lo + share < count ? lo + share : count;
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int64_t i = lo; i < hi; ++i) acc += ld_cols<W>(part + (2 * (p0 + i) + (i == 0)) * D + c);
+    sums[wave][lane] = acc;
+    __syncthreads();
+    if (wave == 0 && mine) {
+      st_cols<W>(dtable + v * D + c,
+                 (((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * scale);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------
+struct EmbedSpace {
+  int64_t keys[2], pos[2], hist, span, part, total;   // byte offsets
+};
+
+static EmbedSpace embed_space(int64_t n, int64_t vocab, int64_t D) {
+  EmbedSpace s;
+  int64_t at = 0;
+  const auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  for (int i = 0; i < 2; ++i) {
+    s.keys[i] = take(4 * n);
+    s.pos[i] = take(4 * n);
+  }
+  s.hist = take((int64_t)kSortBlocks * kDigits * 4);
+  s.span = take(8 * vocab);
+  s.part = take((n + kRun - 1) / kRun * 2 * D * 4);
+  s.total = at;
+  return s;
+}
+
+static bool embed_sizes_ok(int64_t n, int64_t vocab, int64_t D) {
+  return n >= 0 && n < (1ll << 31) - kRun && vocab > 0 && vocab < (1ll << 31) - 1 && D > 0 && D < (1 << 22);
+}
+
+constexpr int64_t kGridMax = 1 << 20;   // workgroups of a launch: the kernels step over the rest
+
+template <int W, typename T, typename ID>
+static void launch_embed_fwd(const m3s_embed_args* a, hipStream_t s) {
+  int lg = 0;
+  while (lg < 6 && (W << lg) < a->width) ++lg;   // lanes to a row, up to a wave
+  const int64_t blocks = std::min(kGridMax, (a->tokens + (256 >> lg) - 1) / (256 >> lg));
+  hipLaunchKernelGGL((embed_fwd_kernel<W, T, ID>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(a->table), a->table_stride,
+                     static_cast<const ID*>(a->ids), static_cast<T*>(a->y), a->tokens, a->vocab,
+                     a->width, a->scale, lg);
+}
+
+template <int W, typename T, typename ID>
+static void launch_embed_bwd(const m3s_embed_args* a, hipStream_t s) {
+  const int64_t n = a->tokens, span_n = 2 * (int64_t)a->vocab;
+  const EmbedSpace sp = embed_space(n, a->vocab, a->width);
+  char* w = static_cast<char*>(a->workspace);
+  const auto u32 = [&](int64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
+  int32_t* span = reinterpret_cast<int32_t*>(w + sp.span);
+  float* part = reinterpret_cast<float*>(w + sp.part);
+  const ID* ids = static_cast<const ID*>(a->ids);
+  int width = 1;   // bits of a key: 0 .. vocab
+  while ((uint64_t)a->vocab >> width) ++width;
+  const int passes = (width + kDigitBits - 1) / kDigitBits, bits = (width + passes - 1) / passes;
+  int last = 0;
+  if (n <= kSortOne) {
+    const int64_t clear = (span_n + 4 * kSortThreads - 1) / (4 * kSortThreads);
+    hipLaunchKernelGGL((sort_one_kernel<ID>), dim3(1 + (unsigned)std::min<int64_t>(clear, 255)),
+                       dim3(kSortThreads), 0, s, ids, u32(sp.keys[0]), u32(sp.pos[0]), span, span_n,
+                       (int)n, a->vocab, a->padding_idx, passes, bits);
+  } else {
+    // the fewest 1024-key rounds that leave at most kSortBlocks workgroups
+    const int64_t rounds = (n + (int64_t)kSortThreads * kSortBlocks - 1) / ((int64_t)kSortThreads * kSortBlocks);
+    const int tile = (int)(rounds * kSortThreads);
+    const unsigned nb = (unsigned)((n + tile - 1) / tile);
+    for (int p = 0; p < passes; ++p) {
+      const int from = (p + 1) & 1, to = p & 1;
+      uint32_t *ik = u32(sp.keys[from]), *ip = u32(sp.pos[from]), *ok = u32(sp.keys[to]), *op = u32(sp.pos[to]);
+      const auto go = [&](auto count, auto place) {
+        hipLaunchKernelGGL(count, dim3(nb), dim3(kSortThreads), 0, s, ids, ik, u32(sp.hist), span, span_n,
+                           n, tile, a->vocab, a->padding_idx, p * bits, bits);
+        hipLaunchKernelGGL(place, dim3(nb), dim3(kSortThreads), 0, s, ids, ik, ip, ok, op, u32(sp.hist),
+                           n, tile, a->vocab, a->padding_idx, p * bits, bits);
+      };
+      if (p == 0) go(sort_count_kernel<ID, true>, sort_place_kernel<ID, true>);
+      else go(sort_count_kernel<ID, false>, sort_place_kernel<ID, false>);
+      last = to;
+    }
+  }
+  const int tiles = (a->width + 64 * W - 1) / (64 * W);
+  const int64_t blocks = ((n + kRun - 1) / kRun * tiles + 3) / 4;
+  if (n > 0) {
+    hipLaunchKernelGGL((run_sum_kernel<W, T>), dim3((unsigned)std::min(kGridMax, blocks)), dim3(256), 0, s,
+                       u32(sp.keys[last]), u32(sp.pos[last]), static_cast<const T*>(a->dy),
+                       static_cast<T*>(a->dtable), part, span, span + a->vocab, n, a->vocab, a->width,
+                       a->scale, tiles);
+  }
+  const int each = (int)std::max<int64_t>(std::max(1, std::min(16, a->vocab / 2048)),
+                                          (a->vocab + kGridMax - 1) / kGridMax);
+  hipLaunchKernelGGL((finish_kernel<W, T>), dim3((unsigned)((a->vocab + each - 1) / each), (unsigned)tiles),
+                     dim3(256), 0, s, part, span, span + a->vocab, static_cast<T*>(a->dtable), a->vocab,
+                     a->width, a->scale, each);
+}
+
+template <typename T, typename ID>
+static void launch_embed(const m3s_embed_args* a, hipStream_t s, bool bwd) {
+  const bool narrow = a->width < 4;
+  if (bwd) narrow ? launch_embed_bwd<1, T, ID>(a, s) : launch_embed_bwd<4, T, ID>(a, s);
+  else narrow ? launch_embed_fwd<1, T, ID>(a, s) : launch_embed_fwd<4, T, ID>(a, s);
+}
+
+static void dispatch_embed(const m3s_embed_args* a, hipStream_t s, bool bwd) {
+  const bool wide = a->id_bytes == 8;
+  if (a->dtype == M3S_DTYPE_BF16) wide ? launch_embed<bf16, int64_t>(a, s, bwd) : launch_embed<bf16, int32_t>(a, s, bwd);
+  else wide ? launch_embed<float, int64_t>(a, s, bwd) : launch_embed<float, int32_t>(a, s, bwd);
+}
+
+static int32_t check_embed(const m3s_embed_args* a, const char* who, bool bwd) {
+  M3S_REQUIRE(a != nullptr, "%s: args is NULL", who);
+  M3S_REQUIRE(a->struct_size == (int32_t)sizeof(m3s_embed_args),
+              "%s: struct_size %d != %d (ABI mismatch)", who, a->struct_size,
+              (int)sizeof(m3s_embed_args));
+  M3S_REQUIRE(a->dtype == M3S_DTYPE_BF16 || a->dtype == M3S_DTYPE_F32, "%s: bad dtype", who);
+  M3S_REQUIRE(a->id_bytes == 4 || a->id_bytes == 8, "%s: ids of %d bytes, must be 4 or 8", who, a->id_bytes);
+  M3S_REQUIRE(embed_sizes_ok(a->tokens, a->vocab, a->width),
+              "%s: bad sizes (tokens %lld, vocab %d, width %d)", who, (long long)a->tokens, a->vocab, a->width);
+  const uintptr_t es = a->dtype == M3S_DTYPE_BF16 ? 2 : 4;
+  M3S_REQUIRE((uintptr_t)a->ids % a->id_bytes == 0, "%s: ids misaligned", who);
+  if (!bwd) {
+    if (a->tokens == 0) return 0;
+    M3S_REQUIRE(a->ids && a->table && a->y, "%s: NULL pointer", who);
+    M3S_REQUIRE((uintptr_t)a->table % es == 0 && (uintptr_t)a->y % es == 0, "%s: misaligned rows", who);
+    M3S_REQUIRE(a->table_stride >= 0, "%s: negative table stride", who);
+    return 0;
+  }
+  M3S_REQUIRE(a->dtable && a->workspace && (a->tokens == 0 || (a->ids && a->dy)), "%s: NULL pointer", who);
+  M3S_REQUIRE((uintptr_t)a->dy % es == 0 && (uintptr_t)a->dtable % es == 0, "%s: misaligned rows", who);
+  M3S_REQUIRE(aligned16(a->workspace), "%s: workspace must be 16-byte aligned", who);
+  const int64_t need = embed_space(a->tokens, a->vocab, a->width).total;
+  M3S_REQUIRE(a->workspace_bytes >= need, "%s: workspace of %lld bytes, needs %lld", who,
+              (long long)a->workspace_bytes, (long long)need);
+  return 0;
+}
+
+}  // namespace m3s
+
+using namespace m3s;
+
+extern "C" int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t width) {
+  if (!embed_sizes_ok(tokens, vocab, width)) return -1;
+  return embed_space(tokens, vocab, width).total;
+}
+
+extern "C" int32_t m3s_embed_fwd(const m3s_embed_args* a, void* stream) {
+  clear_error();
+  if (int32_t rc = check_embed(a, "m3s_embed_fwd", false)) return rc;
+  if (a->tokens == 0) return 0;
+  dispatch_embed(a, static_cast<hipStream_t>(stream), false);
+  return launch_status("m3s_embed_fwd");
+}
+
+extern "C" int32_t m3s_embed_bwd(const m3s_embed_args* a, void* stream) {
+  clear_error();
+  if (int32_t rc = check_embed(a, "m3s_embed_bwd", true)) return rc;
+  dispatch_embed(a, static_cast<hipStream_t>(stream), true);
+  return launch_status("m3s_embed_bwd");
+}

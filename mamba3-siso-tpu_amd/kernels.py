@@ -1362,3 +1362,74 @@ def transpose_pad(w: Tensor, dtype: torch.dtype, out_rows: int) -> Tensor:
     a.inp, a.in_stride, a.out = w.data_ptr(), w.stride(0), out.data_ptr()
     _lib.launch(_lib.load().m3s_transpose, a, dev, "m3s_transpose")
     return out
+
+
+#: The id and row types of the embedding and vocabulary kernels.
+ID_BYTES = {torch.int32: 4, torch.int64: 8}
+
+
+def _embed_args(tokens: Tensor, dtype: torch.dtype, vocab: int, width: int,
+                scale: float) -> "_lib.EmbedArgs":
+    if tokens.dtype not in ID_BYTES:
+        raise ValueError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
+    if vocab < 1 or width < 1:
+        raise ValueError(f"embedding: the table must not be empty, got {(vocab, width)}")
+    a = _lib.EmbedArgs()
+    a.struct_size = ctypes.sizeof(_lib.EmbedArgs)
+    a.dtype, a.id_bytes = _lib.dtype_code(dtype), ID_BYTES[tokens.dtype]
+    a.vocab, a.width, a.scale, a.tokens = vocab, width, scale, tokens.numel()
+    a.padding_idx = -1
+    return a
+
+
+def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
+    """``scale * table[tokens]`` (one ``m3s_embed_fwd`` launch; the lookup of
+    ``model.py:194-232``): ``table`` (V, D) float32 or bf16 with any row stride, ``tokens`` int32
+    or int64 of any shape. The result is in the table's dtype, the product formed in float32. An
+    id outside [0, V) gives a row of NaN (no host synchronisation checks it)."""
+    if table.dim() != 2:
+        raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
+    v, d = table.shape
+    a = _embed_args(tokens, table.dtype, v, d, float(scale))
+    dev = _device_of(table, tokens)
+    if table.stride(1) != 1 and d > 1:
+        table = table.contiguous()
+    tokens = tokens.contiguous()
+    y = empty(*tokens.shape, d, device=dev, dtype=table.dtype)
+    a.ids, a.table, a.table_stride, a.y = tokens.data_ptr(), table.data_ptr(), table.stride(0), y.data_ptr()
+    _lib.launch(_lib.load().m3s_embed_fwd, a, dev, "m3s_embed_fwd")
+    return y
+
+
+def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.0,
+                       padding_idx: Optional[int] = None) -> Tensor:
+    """The table's cotangent of `embedding_forward` (one ``m3s_embed_bwd`` call): ``dy``
+    (tokens.shape, D) -> dense (vocab, D) in dy's dtype, each row the float32 sum of its tokens'
+    rows in position order (a stable sort by id; bit-reproducible), times ``scale``.
+    ``padding_idx`` (negative: from the end) gets a row of zeros; ids outside [0, vocab) add to
+    no row."""
+    if dy.shape[:-1] != tokens.shape or dy.dim() == 0:
+        raise ValueError(f"embedding: dy must be (*tokens.shape, D), got {tuple(dy.shape)} for tokens "
+                         f"{tuple(tokens.shape)}")
+    a = _embed_args(tokens, dy.dtype, int(vocab), dy.shape[-1], float(scale))
+    if padding_idx is not None:
+        a.padding_idx = embedding_padding(padding_idx, a.vocab)
+    dev = _device_of(tokens, dy)
+    tokens, dy = tokens.contiguous(), dy.contiguous()
+    lib = _lib.load()
+    nbytes = lib.m3s_embed_bwd_workspace_bytes(a.tokens, a.vocab, a.width)
+    if nbytes < 0:
+        raise ValueError(f"embedding: bad sizes (tokens {a.tokens}, vocab {a.vocab}, width {a.width})")
+    dtable = empty(a.vocab, a.width, device=dev, dtype=dy.dtype)
+    ws = empty(nbytes, device=dev, dtype=torch.uint8)
+    a.ids, a.dy, a.dtable = tokens.data_ptr(), dy.data_ptr(), dtable.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _lib.launch(lib.m3s_embed_bwd, a, dev, "m3s_embed_bwd")
+    return dtable
+
+
+def embedding_padding(padding_idx: int, vocab: int) -> int:
+    """``padding_idx`` as an id in [0, vocab); negative ones count from the end."""
+    if not -vocab <= padding_idx < vocab:
+        raise ValueError(f"embedding: padding_idx {padding_idx} is outside a vocabulary of {vocab}")
+    return padding_idx % vocab

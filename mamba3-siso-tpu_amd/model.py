@@ -30,6 +30,7 @@ import torch.nn.functional as F
 from . import kernels as K
 from . import layer as LY
 from . import layout as L
+from . import tokens as TK
 from .scan_prep import SISOState, zero_state
 
 Tensor = torch.Tensor
@@ -323,9 +324,13 @@ def _norm(x: Tensor, gain: Tensor, eps: float, dt: torch.dtype) -> Tensor:
 
 
 def _embed(table: Tensor, tokens: Tensor) -> Tensor:
-    """``table[tokens]``. Through ``F.embedding``, whose backward reduces duplicate ids in
-    parallel partial segments; the plain-indexing backward sums each id's rows serially,
-    which for byte data (256 ids, Zipf-skewed) costs ~5 ms per training step."""
+    """``table[tokens]`` through `tokens.embed_tokens`, whose gradient sums each id's rows in
+    parallel pieces in a fixed order. What that does not take (other dtypes, a forward-mode
+    tangent, a trace) goes to ``F.embedding``."""
+    if (table.is_cuda and tokens.device == table.device and table.dim() == 2 and table.numel()
+            and table.dtype in (torch.float32, torch.bfloat16) and tokens.dtype in K.ID_BYTES
+            and not torch.jit.is_tracing() and not LY.has_tangent(table)):
+        return TK.embed_tokens(table, tokens)
     return F.embedding(tokens, table)
 
 

@@ -1,0 +1,208 @@
+"""GPU parity of the embedding lookup and its gradient (`m3s_embed_fwd` / `m3s_embed_bwd`)
+against float64 sums on the CPU.
+
+Tolerances:
+  * forward: the scale is a float32 (22.7 is not one: half a step), one float32 product (half a
+    step), and for bf16 one rounding to that type: 2 2^-24 relative in float32, and 2^-8 more in
+    bf16 (second-order terms are covered by a factor 1 + 2^-8); with scale 1 bit-identical.
+  * gradient: a row that sums n values of magnitude at most m in float32, in pieces, is off by at
+    most n 2^-24 times the sum of the magnitudes (n additions, each of a partial sum no larger),
+    then the scale's two roundings and the type's, as above.
+"""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EPS32 = 2.0 ** -24
+
+
+def scaled_step(dtype):
+    """The relative error of one product with the scale, rounded to ``dtype``."""
+    return 2 * EPS32 if dtype == torch.float32 else (2 * EPS32 + 2.0 ** -8) * (1 + 2.0 ** -8)
+
+
+def reference(tokens, dy, vocab, scale, pad):
+    """The gradient in float64 and the bound on the float32 sums' error, element by element."""
+    ids = tokens.reshape(-1).cpu().long()
+    rows = dy.reshape(-1, dy.shape[-1]).cpu().double()
+    ok = (ids >= 0) & (ids < vocab)
+    if pad is not None:
+        ok &= ids != pad % vocab
+    ids, rows = ids[ok], rows[ok]
+    want = torch.zeros(vocab, rows.shape[-1], dtype=torch.float64).index_add_(0, ids, rows)
+    mag = torch.zeros_like(want).index_add_(0, ids, rows.abs())
+    n = torch.bincount(ids, minlength=vocab).double().unsqueeze(1)
+    return want * scale, n * EPS32 * mag * abs(scale)
+
+
+def check_grad(got, tokens, dy, scale, pad):
+    want, err = reference(tokens, dy, got.shape[0], scale, pad)
+    tol = err * (1 + 2.0 ** -7) + want.abs() * scaled_step(got.dtype) + 1e-38
+    over = ((got.cpu().double() - want).abs() / tol).max().item()
+    assert over <= 1.0
+
+
+def skewed(vocab, shape, gen, dtype=torch.int64):
+    u = torch.rand(shape, generator=gen, dtype=torch.float64)
+    return ((vocab + 1.0) ** u - 1).floor().clamp(0, vocab - 1).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ids", [torch.int32, torch.int64])
+@pytest.mark.parametrize("vocab,d,shape,scale", [
+    (1, 1, (1,), 1.0), (7, 3, (5, 2), 1.0), (40, 5, (64,), 2.5), (256, 768, (3, 700), 1.0),
+    (257, 260, (4097,), 0.5), (511, 64, (2, 2500), 1.0), (512, 17, (33, 3), 1.0),
+    (5003, 515, (4, 1025), 22.7), (70001, 36, (9000,), 6.0), (300007, 8, (3001,), 1.0)])
+def test_lookup_and_gradient(m3, dev, dtype, ids, vocab, d, shape, scale):
+    gen = torch.Generator().manual_seed(vocab + d)
+    table = torch.randn(vocab, d, generator=gen).to(dtype)
+    tokens = skewed(vocab, shape, gen, ids)
+    dy = torch.randn(*shape, d, generator=gen).to(dtype)
+    w = table.to(dev).requires_grad_(True)
+    y = m3.embed_tokens(w, tokens.to(dev), scale=scale)
+    want = table[tokens.long()].double() * scale
+    assert y.dtype == dtype and y.shape == (*shape, d)
+    if scale == 1.0:
+        assert torch.equal(y.detach().cpu(), table[tokens.long()])
+    over = (y.detach().cpu().double() - want).abs() / (want.abs() * scaled_step(dtype) + 1e-38)
+    assert over.max().item() <= 1.0
+    (dw,) = torch.autograd.grad(y, w, dy.to(dev))
+    assert dw.dtype == dtype and dw.shape == (vocab, d)
+    check_grad(dw, tokens, dy, scale, None)
+    with torch.no_grad():
+        assert torch.equal(m3.embed_tokens(w, tokens.to(dev), scale=scale), y)
+
+
+@pytest.mark.parametrize("n", [0, 1, 31, 32, 33, 64, 1023, 1024, 1025, 4095, 4096, 4097, 8192, 40000])
+def test_sort_sizes_and_single_ids(m3, dev, n):
+    """Lengths around the pieces, the workgroups and the switch of the sort; every token the same
+    id, ids in order, and ids against the order."""
+    gen = torch.Generator().manual_seed(n)
+    d, vocab = 12, 1000
+    dy = torch.randn(n, d, generator=gen)
+    for tokens in (torch.full((n,), 999), torch.arange(n) % vocab, (n - 1 - torch.arange(n)) * vocab // max(n, 1),
+                   skewed(vocab, (n,), gen)):
+        got = m3.kernels.embedding_backward(tokens.to(dev), dy.to(dev), vocab)
+        check_grad(got, tokens, dy, 1.0, None)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_padding_and_ids_outside_the_table(m3, dev, dtype):
+    """The padding id's row is looked up and gets zeros back; an id outside the table gives NaN and
+    adds to no row, whatever its cotangent holds."""
+    gen = torch.Generator().manual_seed(3)
+    vocab, d = 300, 96
+    table = torch.randn(vocab, d, generator=gen).to(dtype)
+    tokens = skewed(vocab, (5, 400), gen)
+    tokens[1, 100:] = vocab - 1
+    dy = torch.randn(5, 400, d, generator=gen).to(dtype)
+    for pad in (vocab - 1, -1, 0, None):
+        w = table.to(dev).requires_grad_(True)
+        y = m3.embed_tokens(w, tokens.to(dev), padding_idx=pad)
+        assert torch.equal(y.detach().cpu(), table[tokens])
+        (dw,) = torch.autograd.grad(y, w, dy.to(dev))
+        check_grad(dw, tokens, dy, 1.0, pad)
+    bad = tokens.clone()
+    outside = torch.rand(bad.shape, generator=gen) < 0.1
+    bad[outside] = torch.tensor([-1, -100, vocab, 1 << 40])[torch.arange(int(outside.sum())) % 4]
+    w = table.to(dev).requires_grad_(True)
+    y = m3.embed_tokens(w, bad.to(dev))
+    assert y[outside.to(dev)].isnan().all() and not y[~outside.to(dev)].isnan().any()
+    dy[outside] = float("nan")
+    (dw,) = torch.autograd.grad(y, w, dy.to(dev))
+    check_grad(dw, bad, dy, 1.0, None)
+
+
+def test_gradient_is_bit_reproducible_and_matches_differences(m3, dev):
+    gen = torch.Generator().manual_seed(8)
+    tokens = skewed(256, (6, 2048), gen).to(dev)
+    dy = torch.randn(6, 2048, 100, generator=gen).to(dev)
+    first = m3.kernels.embedding_backward(tokens, dy, 256)
+    for _ in range(3):
+        assert torch.equal(m3.kernels.embedding_backward(tokens, dy, 256), first)
+    # the lookup is linear: a step h of one entry moves <y, dy> by h times that gradient entry
+    table = torch.randn(256, 100, generator=gen).to(dev)
+    step = torch.zeros_like(table)
+    step[0, 7] = 0.5
+    f = lambda t: (m3.embed_tokens(t, tokens, scale=3.0).double() * dy.double()).sum()  # noqa: E731
+    slope = (f(table + step) - f(table - step)).item()
+    want = m3.kernels.embedding_backward(tokens, dy, 256, 3.0)[0, 7].item()
+    assert abs(slope - want) <= 1e-4 * abs(want) + 1e-3
+
+
+def test_strides_broadcast_cotangents_and_views(m3, dev):
+    """A table that is a slice of a wider one, tokens that are a strided view, and a cotangent
+    that is broadcast."""
+    gen = torch.Generator().manual_seed(4)
+    wide = torch.randn(90, 48, generator=gen).to(dev)
+    table = wide[:, 7:40]
+    tokens = torch.randint(0, 90, (6, 50), generator=gen).to(dev).t()[::2]
+    assert torch.equal(m3.embed_tokens(table, tokens), table[tokens])
+    assert torch.equal(m3.embed_tokens(wide.t(), tokens % 48), wide.t()[tokens % 48])
+    dy = torch.randn(33, generator=gen).to(dev).expand(*tokens.shape, 33)
+    check_grad(m3.kernels.embedding_backward(tokens, dy, 90), tokens.cpu(), dy.cpu(), 1.0, None)
+    w = table.detach().requires_grad_(True)
+    m3.embed_tokens(w, tokens).sum().backward()
+    check_grad(w.grad, tokens.cpu(), torch.ones(*tokens.shape, 33), 1.0, None)
+    one = m3.embed_tokens(table, tokens[0, 0])   # a single id without axes
+    assert one.shape == (33,) and torch.equal(one, table[tokens[0, 0]])
+
+
+def test_captured_calls_replay_on_new_inputs(m3, dev):
+    """Lookup and gradient inside a recorded graph, replayed on changed ids and cotangents with
+    other work between the replays."""
+    gen = torch.Generator().manual_seed(6)
+    vocab, d = 700, 64
+    table = torch.randn(vocab, d, generator=gen).to(dev)
+    for n in (50, 6000):
+        tokens = torch.zeros(n, dtype=torch.int64, device=dev)
+        dy = torch.zeros(n, d, device=dev)
+        side = torch.cuda.Stream(dev)
+        with torch.cuda.stream(side):
+            m3.kernels.embedding_forward(table, tokens), m3.kernels.embedding_backward(tokens, dy, vocab)
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = m3.kernels.embedding_forward(table, tokens, 2.0)
+            dw = m3.kernels.embedding_backward(tokens, dy, vocab, 2.0, padding_idx=3)
+        for _ in range(3):
+            tokens.copy_(skewed(vocab, (n,), gen))
+            dy.copy_(torch.randn(n, d, generator=gen))
+            graph.replay()
+            assert torch.equal(y, m3.kernels.embedding_forward(table, tokens, 2.0))
+            assert torch.equal(dw, m3.kernels.embedding_backward(tokens, dy, vocab, 2.0, padding_idx=3))
+            torch.cuda.synchronize()
+
+
+def test_calls_on_another_stream_and_two_at_once(m3, dev):
+    gen = torch.Generator().manual_seed(9)
+    a, b = (skewed(400, (5000,), gen).to(dev) for _ in range(2))
+    dy = torch.randn(5000, 32, generator=gen).to(dev)
+    want = [m3.kernels.embedding_backward(t, dy, 400) for t in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(dev) for _ in range(2)]
+    got = []
+    for s, t in zip(streams, (a, b)):
+        with torch.cuda.stream(s):
+            got.append(m3.kernels.embedding_backward(t, dy, 400))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_model_lookup_keeps_what_it_took(m3, dev):
+    """`model._embed` still takes tables and modes that the kernels do not."""
+    table = torch.randn(11, 6, device=dev, dtype=torch.float64, requires_grad=True)
+    tokens = torch.tensor([[1, 2], [10, 0]], device=dev)
+    y = m3.model._embed(table, tokens)
+    assert torch.equal(y, table[tokens])
+    y.sum().backward()
+    assert table.grad[1, 0] == 1 and table.grad[3, 0] == 0
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level():
+        dual = fwad.make_dual(table.detach().float(), torch.ones(11, 6, device=dev))
+        assert (fwad.unpack_dual(m3.model._embed(dual, tokens)).tangent == 1).all()
+        with pytest.raises((NotImplementedError, RuntimeError)):
+            m3.embed_tokens(dual, tokens)
