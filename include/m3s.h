@@ -641,6 +641,71 @@ int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t wid
 int32_t m3s_embed_fwd(const m3s_embed_args* args, void* stream);
 int32_t m3s_embed_bwd(const m3s_embed_args* args, void* stream);
 
+/* Log-probabilities read off the LM's logits, beside the cross-entropy of train.py:414-416. Per row
+ * x of `vocab` logits at `temperature` T: logp = log softmax(x / T) at the target, the entropy of
+ * softmax(x / T), and with top > 0 the log-probabilities and ids of the `top` largest logits (ties:
+ * the lower id). Float32 out. stats holds what the backward needs of a row. Backward: dlogits
+ * (dense, in dtype) of dlogp, dentropy and dtop_logp, each NULL for none. Logit rows may start at
+ * any element.
+ * A row whose target is ignore_index is not read: logp and entropy 0, ids -1, top_logp -inf, no
+ * gradient. Another target outside [0, vocab): logp NaN, a gradient of NaN if dlogp is given. A row
+ * of nothing but -inf: logp and top_logp -inf, entropy 0, no gradient. A row with NaN or +inf: NaN
+ * throughout, ids -1. */
+typedef struct m3s_logprob_args {
+  int32_t struct_size;   /* sizeof(m3s_logprob_args) */
+  int32_t dtype;         /* M3S_DTYPE_* of logits and dlogits */
+  int32_t batch, seqlen; /* rows = batch * seqlen < 2^31 */
+  int32_t vocab;         /* < 2^30 */
+  int32_t top;           /* 0 .. 64, at most vocab */
+  float temperature;
+  int64_t ignore_index;
+  m3s_blx logits;        /* (batch, seqlen, vocab), strides >= 0 */
+  const int64_t* targets; /* (rows), or NULL: no logp */
+  float* logp;           /* forward out (rows) with targets */
+  float* entropy;        /* forward out (rows) */
+  float* stats;          /* forward out, backward in (rows, 3) */
+  float* top_logp;       /* forward out (rows, top) */
+  int64_t* top_ids;      /* forward out (rows, top); backward in with dtop_logp */
+  const float* dlogp;    /* backward in (rows) or NULL */
+  const float* dentropy; /* backward in (rows) or NULL */
+  const float* dtop_logp; /* backward in (rows, top) or NULL */
+  void* dlogits;         /* backward out (rows, vocab) */
+} m3s_logprob_args;
+int32_t m3s_logprob_fwd(const m3s_logprob_args* args, void* stream);
+int32_t m3s_logprob_bwd(const m3s_logprob_args* args, void* stream);
+
+/* The distillation loss of a student's logits from a teacher's best tokens, no counterpart in the
+ * reference. Per row, w = softmax(teacher_logits / T) over the teacher_k entries (an id < 0: no
+ * entry; a logit of -inf: weight 0; a repeated id adds up) and q = softmax(logits / T):
+ * kd = T^2 sum w (log w - log q[id]). With targets also nll = -log softmax(logits)[target], in the
+ * same pass. Float32 out. Backward: dlogits (dense, in dtype) of dkd and dnll, each NULL for none.
+ * A row without an entry has kd 0 and no gradient from it; one with target ignore_index likewise
+ * nll 0; with neither it is not read. An id >= vocab, or another target outside [0, vocab), gives
+ * NaN and a gradient of NaN. A student row of nothing but -inf: +inf and no gradient. */
+typedef struct m3s_distill_args {
+  int32_t struct_size;   /* sizeof(m3s_distill_args) */
+  int32_t dtype;         /* M3S_DTYPE_* of logits and dlogits */
+  int32_t batch, seqlen; /* rows = batch * seqlen < 2^31 */
+  int32_t vocab;         /* < 2^30 */
+  int32_t teacher_k;     /* 1 .. 256 */
+  int32_t teacher_dtype; /* M3S_DTYPE_* of teacher_logits */
+  int32_t id_bytes;      /* 4 or 8: int32 or int64 teacher_ids */
+  float temperature;
+  int64_t ignore_index;
+  m3s_blx logits;        /* (batch, seqlen, vocab), strides >= 0 */
+  const void* teacher_ids;    /* (rows, teacher_k) */
+  const void* teacher_logits; /* (rows, teacher_k) */
+  const int64_t* targets;     /* (rows), or NULL */
+  float* kd;             /* forward out (rows) */
+  float* nll;            /* forward out (rows) iff targets */
+  float* stats;          /* forward out, backward in (rows, 5) */
+  const float* dkd;      /* backward in (rows) or NULL */
+  const float* dnll;     /* backward in (rows) or NULL */
+  void* dlogits;         /* backward out (rows, vocab) */
+} m3s_distill_args;
+int32_t m3s_distill_fwd(const m3s_distill_args* args, void* stream);
+int32_t m3s_distill_bwd(const m3s_distill_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

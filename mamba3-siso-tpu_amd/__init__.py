@@ -31,4 +31,6 @@ from .scan_prep import (  # noqa: F401
     zero_state,
 )
 from .siso import SISOOutput, siso, siso_segment  # noqa: F401
-from .tokens import embed_tokens  # noqa: F401
+from .tokens import (  # noqa: F401
+    DistillLoss, TokenLogprobs, distill_loss, embed_tokens, token_logprobs,
+)

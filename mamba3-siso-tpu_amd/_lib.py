@@ -233,6 +233,25 @@ class EmbedArgs(C.Structure):
     ]
 
 
+class LogprobArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", i32), ("dtype", i32), ("batch", i32), ("seqlen", i32), ("vocab", i32),
+        ("top", i32), ("temperature", C.c_float), ("ignore_index", i64), ("logits", Blx),
+        ("targets", vp), ("logp", vp), ("entropy", vp), ("stats", vp), ("top_logp", vp),
+        ("top_ids", vp), ("dlogp", vp), ("dentropy", vp), ("dtop_logp", vp), ("dlogits", vp),
+    ]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", i32), ("dtype", i32), ("batch", i32), ("seqlen", i32), ("vocab", i32),
+        ("teacher_k", i32), ("teacher_dtype", i32), ("id_bytes", i32), ("temperature", C.c_float),
+        ("ignore_index", i64), ("logits", Blx), ("teacher_ids", vp), ("teacher_logits", vp),
+        ("targets", vp), ("kd", vp), ("nll", vp), ("stats", vp), ("dkd", vp), ("dnll", vp),
+        ("dlogits", vp),
+    ]
+
+
 #: ``M3S_GEMV_*``
 GEMV_NORM, GEMV_GATE, GEMV_HEAD = 1, 2, 3
 
@@ -246,7 +265,8 @@ EXPORTS = ("m3s_abi_version", "m3s_last_error", "m3s_supported", "m3s_fwd_raw_su
            "m3s_norm_bwd", "m3s_decode_layer", "m3s_transpose", "m3s_swiglu_fwd",
            "m3s_swiglu_bwd", "m3s_rms_fwd", "m3s_rms_bwd", "m3s_rms_bwd_workspace_bytes",
            "m3s_norm_bwd_noalloc", "m3s_adamw", "m3s_wgrad", "m3s_wgrad_workspace_bytes", "m3s_gemv",
-           "m3s_gemv_fused", "m3s_embed_bwd_workspace_bytes", "m3s_embed_fwd", "m3s_embed_bwd")
+           "m3s_gemv_fused", "m3s_embed_bwd_workspace_bytes", "m3s_embed_fwd", "m3s_embed_bwd",
+           "m3s_logprob_fwd", "m3s_logprob_bwd", "m3s_distill_fwd", "m3s_distill_bwd")
 
 _lib = None
 
@@ -343,6 +363,12 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     for fn in (lib.m3s_embed_fwd, lib.m3s_embed_bwd):
         fn.restype = i32
         fn.argtypes = [C.POINTER(EmbedArgs), vp]
+    for fn in (lib.m3s_logprob_fwd, lib.m3s_logprob_bwd):
+        fn.restype = i32
+        fn.argtypes = [C.POINTER(LogprobArgs), vp]
+    for fn in (lib.m3s_distill_fwd, lib.m3s_distill_bwd):
+        fn.restype = i32
+        fn.argtypes = [C.POINTER(DistillArgs), vp]
     _lib = lib
     return lib
 

@@ -36,7 +36,7 @@ def empty(*size, device=None, dtype=None) -> Tensor:
     """``torch.empty`` for kernel outputs and workspaces (see `POISON_OUTPUTS`)."""
     t = torch.empty(*size, device=device, dtype=dtype)
     if POISON_OUTPUTS:
-        t.view(torch.uint8).fill_(255) if t.numel() else None
+        t.reshape(-1).view(torch.uint8).fill_(255) if t.numel() else None
     return t
 
 
@@ -1433,3 +1433,188 @@ def embedding_padding(padding_idx: int, vocab: int) -> int:
     if not -vocab <= padding_idx < vocab:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside a vocabulary of {vocab}")
     return padding_idx % vocab
+
+
+#: Alternatives of `logprob_forward` and teacher tokens of `distill_forward`, at most.
+TOP_MAX, TEACHER_MAX = 64, 256
+
+
+def _logit_rows(logits: Tensor, what: str) -> Tensor:
+    """``logits`` (..., V) as the (B, L, V) view that the kernels read in place; a copy only where
+    the rows are not contiguous or more than two leading axes do not fold."""
+    if logits.dim() == 0 or logits.shape[-1] == 0:
+        raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
+    v = logits.shape[-1]
+    if logits.stride(-1) != 1 and v > 1:
+        logits = logits.contiguous()
+    if logits.dim() == 3:
+        return logits
+    if logits.dim() > 3:
+        return logits.reshape(-1, logits.shape[-2], v)
+    return logits.reshape(1, -1, v)
+
+
+def _row_args(a, rows3: Tensor, temperature: float, ignore_index: int) -> None:
+    """The fields that ``m3s_logprob_args`` and ``m3s_distill_args`` share."""
+    a.struct_size = ctypes.sizeof(a)
+    a.dtype = _lib.dtype_code(rows3.dtype)
+    a.batch, a.seqlen, a.vocab = rows3.shape
+    a.temperature, a.ignore_index = temperature, ignore_index
+    a.logits = _lib.blx(rows3)
+
+
+def _row_values(t: Optional[Tensor], shape, dtype: torch.dtype, what: str) -> Optional[Tensor]:
+    """A dense per-row operand of the given shape and dtype, or None."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
+    return t.to(dtype).contiguous()
+
+
+def _row_targets(targets: Optional[Tensor], shape, what: str) -> Optional[Tensor]:
+    if targets is not None and targets.dtype not in ID_BYTES:
+        raise ValueError(f"{what}: targets must be int32 or int64, got {targets.dtype}")
+    return _row_values(targets, shape, torch.int64, f"{what}: targets")
+
+
+def _check_temperature(temperature: float, what: str) -> float:
+    temperature = float(temperature)
+    if not 1e-30 <= temperature <= 1e30:
+        raise ValueError(f"{what}: the temperature must be positive and finite, got {temperature}")
+    return temperature
+
+
+def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int = 0,
+                    temperature: float = 1.0, ignore_index: int = -100):
+    """Log-probabilities read off ``logits`` (..., V), float32 or bf16 (``m3s_logprob_fwd``):
+    ``(logp, entropy, top_logp, top_ids, stats)``. ``logp`` (...,) is ``log softmax(logits / T)``
+    at ``targets`` (...,), ``entropy`` that distribution's, ``top_logp`` / ``top_ids`` (..., top)
+    its best ids in falling order (equal logits: the lower id first). ``logp`` is None without
+    targets, the two last None with ``top`` 0; ``stats`` (..., 3) is `logprob_backward`'s.
+
+    Rows whose target is ``ignore_index`` are not read: logp and entropy 0, ids -1, top_logp -inf.
+    Another target outside [0, V) gives NaN. A row of nothing but -inf has logp -inf, entropy 0; a
+    row with NaN or +inf is NaN throughout, with ids -1."""
+    rows = _logit_rows(logits, "logprob")
+    top = int(top)
+    if not 0 <= top <= min(TOP_MAX, rows.shape[-1]):
+        raise ValueError(f"logprob: top must be in [0, {min(TOP_MAX, rows.shape[-1])}], got {top}")
+    shape = logits.shape[:-1]
+    targets = _row_targets(targets, shape, "logprob")
+    a = _lib.LogprobArgs()
+    _row_args(a, rows, _check_temperature(temperature, "logprob"), int(ignore_index))
+    dev = _device_of(logits, targets)
+    # tensors of their own, not views of one: autograd refuses in-place work on a node's views
+    entropy = empty(shape, device=dev, dtype=torch.float32)
+    stats = empty(*shape, 3, device=dev, dtype=torch.float32)
+    logp = top_logp = top_ids = None
+    a.top = top
+    a.entropy, a.stats = entropy.data_ptr(), stats.data_ptr()
+    if targets is not None:
+        logp = empty(shape, device=dev, dtype=torch.float32)
+        a.targets, a.logp = targets.data_ptr(), logp.data_ptr()
+    if top:
+        top_logp = empty(*shape, top, device=dev, dtype=torch.float32)
+        top_ids = empty(*shape, top, device=dev, dtype=torch.int64)
+        a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
+    _lib.launch(_lib.load().m3s_logprob_fwd, a, dev, "m3s_logprob_fwd")
+    return logp, entropy, top_logp, top_ids, stats
+
+
+def logprob_backward(logits: Tensor, targets: Optional[Tensor], stats: Tensor,
+                     top_ids: Optional[Tensor] = None, dlogp: Optional[Tensor] = None,
+                     dentropy: Optional[Tensor] = None, dtop_logp: Optional[Tensor] = None,
+                     temperature: float = 1.0, ignore_index: int = -100) -> Tensor:
+    """The logits' cotangent of `logprob_forward` (one ``m3s_logprob_bwd`` launch), dense and in
+    their dtype, from any of the three outputs' cotangents."""
+    rows = _logit_rows(logits, "logprob")
+    shape = logits.shape[:-1]
+    targets = _row_targets(targets, shape, "logprob")
+    if dlogp is not None and targets is None:
+        raise ValueError("logprob: dlogp needs the targets")
+    f32 = torch.float32
+    dlogp = _row_values(dlogp, shape, f32, "logprob: dlogp")
+    dentropy = _row_values(dentropy, shape, f32, "logprob: dentropy")
+    stats = _row_values(stats, (*shape, 3), f32, "logprob: stats")
+    top = 0
+    if dtop_logp is not None:
+        if top_ids is None:
+            raise ValueError("logprob: dtop_logp needs top_ids")
+        top = top_ids.shape[-1]
+        top_ids = _row_values(top_ids, (*shape, top), torch.int64, "logprob: top_ids")
+        dtop_logp = _row_values(dtop_logp, (*shape, top), f32, "logprob: dtop_logp")
+    a = _lib.LogprobArgs()
+    _row_args(a, rows, _check_temperature(temperature, "logprob"), int(ignore_index))
+    dev = _device_of(logits, targets, stats, dlogp, dentropy, dtop_logp, top_ids if top else None)
+    dx = empty(logits.shape, device=dev, dtype=logits.dtype)
+    a.top = top
+    a.targets, a.stats, a.dlogits = _lib.ptr(targets), stats.data_ptr(), dx.data_ptr()
+    a.dlogp, a.dentropy = _lib.ptr(dlogp), _lib.ptr(dentropy)
+    if top:
+        a.top_ids, a.dtop_logp = top_ids.data_ptr(), dtop_logp.data_ptr()
+    _lib.launch(_lib.load().m3s_logprob_bwd, a, dev, "m3s_logprob_bwd")
+    return dx
+
+
+def _distill_args(logits: Tensor, ids: Tensor, teacher: Tensor, targets: Optional[Tensor],
+                  temperature: float, ignore_index: int):
+    rows = _logit_rows(logits, "distill")
+    shape = logits.shape[:-1]
+    k = ids.shape[-1] if ids.dim() else 0
+    if not 1 <= k <= TEACHER_MAX:
+        raise ValueError(f"distill: between 1 and {TEACHER_MAX} teacher tokens a row, got {k}")
+    if ids.dtype not in ID_BYTES:
+        raise ValueError(f"distill: teacher_ids must be int32 or int64, got {ids.dtype}")
+    a = _lib.DistillArgs()
+    a.teacher_k, a.id_bytes, a.teacher_dtype = k, ID_BYTES[ids.dtype], _lib.dtype_code(teacher.dtype)
+    ids = _row_values(ids, (*shape, k), ids.dtype, "distill: teacher_ids")
+    teacher = _row_values(teacher, (*shape, k), teacher.dtype, "distill: teacher_logits")
+    targets = _row_targets(targets, shape, "distill")
+    _row_args(a, rows, _check_temperature(temperature, "distill"), int(ignore_index))
+    dev = _device_of(logits, ids, teacher, targets)
+    a.teacher_ids, a.teacher_logits, a.targets = ids.data_ptr(), teacher.data_ptr(), _lib.ptr(targets)
+    return a, dev, (rows, ids, teacher, targets)   # the tensors stay alive until the launch
+
+
+def distill_forward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
+                    targets: Optional[Tensor] = None, temperature: float = 1.0,
+                    ignore_index: int = -100):
+    """The distillation loss of ``logits`` (..., V) from a teacher's best tokens
+    (``m3s_distill_fwd``): ``(kd, nll, stats)``. With ``w = softmax(teacher_logits / T)`` over the
+    (..., K) entries and ``q = softmax(logits / T)``, ``kd = T^2 sum w (log w - log q[ids])``;
+    ``nll = -log softmax(logits)[targets]`` in the same pass, None without targets.
+
+    An entry with an id < 0 does not count, one with logit -inf has weight 0, a repeated id adds
+    up. A row without entries has kd 0, one with target ``ignore_index`` nll 0; with neither it is
+    not read. An id >= V and another target outside [0, V) give NaN."""
+    a, dev, keep = _distill_args(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)
+    shape = logits.shape[:-1]
+    kd = empty(shape, device=dev, dtype=torch.float32)
+    stats = empty(*shape, 5, device=dev, dtype=torch.float32)
+    nll = None
+    a.kd, a.stats = kd.data_ptr(), stats.data_ptr()
+    if targets is not None:
+        nll = empty(shape, device=dev, dtype=torch.float32)
+        a.nll = nll.data_ptr()
+    _lib.launch(_lib.load().m3s_distill_fwd, a, dev, "m3s_distill_fwd")
+    return kd, nll, stats
+
+
+def distill_backward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
+                     targets: Optional[Tensor], stats: Tensor, dkd: Optional[Tensor] = None,
+                     dnll: Optional[Tensor] = None, temperature: float = 1.0,
+                     ignore_index: int = -100) -> Tensor:
+    """The logits' cotangent of `distill_forward` (one ``m3s_distill_bwd`` launch), dense and in
+    their dtype: ``T dkd (q - w)`` plus ``dnll (softmax(logits) - onehot)``."""
+    a, dev, keep = _distill_args(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)
+    if dnll is not None and targets is None:
+        raise ValueError("distill: dnll needs the targets")
+    shape, f32 = logits.shape[:-1], torch.float32
+    stats = _row_values(stats, (*shape, 5), f32, "distill: stats")
+    dkd, dnll = _row_values(dkd, shape, f32, "distill: dkd"), _row_values(dnll, shape, f32, "distill: dnll")
+    _device_of(logits, stats, dkd, dnll)
+    dx = empty(logits.shape, device=dev, dtype=logits.dtype)
+    a.stats, a.dkd, a.dnll, a.dlogits = stats.data_ptr(), _lib.ptr(dkd), _lib.ptr(dnll), dx.data_ptr()
+    _lib.launch(_lib.load().m3s_distill_bwd, a, dev, "m3s_distill_bwd")
+    return dx

@@ -369,6 +369,26 @@ def lm_loss(params: LMParams, xs: Tensor, ys: Tensor, cfg: LMConfig) -> Tensor:
     return F.cross_entropy(logits.reshape(-1, logits.shape[-1]), ys.reshape(-1))
 
 
+def lm_logprobs(params: LMParams, xs: Tensor, ys: Optional[Tensor], cfg: LMConfig, top: int = 0,
+                temperature: float = 1.0, ignore_index: int = -100) -> TK.TokenLogprobs:
+    """`tokens.token_logprobs` of `lm_forward`'s logits: what the model says about ``ys`` (B, L)
+    after ``xs`` (B, L), with the entropy and the ``top`` best tokens at each position (scoring text,
+    a teacher's pass, the log-probabilities of policy-gradient training)."""
+    return TK.token_logprobs(lm_forward(params, xs, cfg), ys, top, temperature, ignore_index)
+
+
+def lm_distill_loss(params: LMParams, xs: Tensor, ys: Tensor, teacher_ids: Tensor,
+                    teacher_logits: Tensor, cfg: LMConfig, temperature: float = 1.0,
+                    hard_weight: float = 0.0, ignore_index: int = -100) -> Tensor:
+    """Mean of ``(1 - hard_weight) kd + hard_weight nll`` (`tokens.distill_loss` of `lm_forward`'s
+    logits) over the positions whose ``ys`` is not ``ignore_index``: `lm_loss` with a teacher's best
+    tokens ``teacher_ids`` / ``teacher_logits`` (B, L, K) beside the text."""
+    live = ys != ignore_index
+    ids = teacher_ids.masked_fill(~live.unsqueeze(-1), -1)
+    out = TK.distill_loss(lm_forward(params, xs, cfg), ids, teacher_logits, temperature, ys, ignore_index)
+    return ((1.0 - hard_weight) * out.kd.sum() + hard_weight * out.nll.sum()) / live.sum()
+
+
 def zero_states(cfg: LMConfig, batch: int, dtype=torch.float32, device=None) -> list:
     """A fresh per-layer carry (``model.py:235-241``)."""
     c = cfg.siso

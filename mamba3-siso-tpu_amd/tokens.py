@@ -8,7 +8,7 @@ forward-mode rule and are differentiable once.
 
 from __future__ import annotations
 
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -22,7 +22,7 @@ Tensor = torch.Tensor
 def _needs_node(*tensors) -> bool:
     """Whether a call goes through its autograd node: a gradient is taken, or the node has to
     refuse what a bare launch would drop (a forward-mode tangent) or record wrongly (a trace)."""
-    return ((torch.is_grad_enabled() and any(t.requires_grad for t in tensors))
+    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
             or torch.jit.is_tracing() or LY.has_tangent(*tensors))
 
 
@@ -55,3 +55,108 @@ def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
     if _needs_node(table):
         return _EmbedFn.apply(table, tokens, float(scale), padding_idx)
     return K.embedding_forward(table, tokens, scale)
+
+
+class TokenLogprobs(NamedTuple):
+    """`token_logprobs`' results; see there. ``logp`` is None without targets, ``top_logp`` and
+    ``top_ids`` without ``top``."""
+
+    logp: Optional[Tensor]
+    entropy: Tensor
+    top_logp: Optional[Tensor]
+    top_ids: Optional[Tensor]
+
+
+class _LogprobFn(torch.autograd.Function):
+    """`kernels.logprob_forward` / `kernels.logprob_backward` as one node."""
+
+    @staticmethod
+    def forward(ctx, logits, targets, top, temperature, ignore_index):
+        logp, entropy, top_logp, top_ids, stats = K.logprob_forward(logits, targets, top, temperature,
+                                                                    ignore_index)
+        ctx.save_for_backward(logits, targets, stats, top_ids)
+        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.set_materialize_grads(False)
+        if top_ids is not None:
+            ctx.mark_non_differentiable(top_ids)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dlogp, dentropy, dtop_logp, _):
+        if dlogp is None and dentropy is None and dtop_logp is None:
+            return None, None, None, None, None
+        logits, targets, stats, top_ids = ctx.saved_tensors
+        dx = K.logprob_backward(logits, targets, stats, top_ids, dlogp, dentropy, dtop_logp,
+                                ctx.temperature, ctx.ignore_index)
+        return dx, None, None, None, None
+
+
+def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, top: int = 0,
+                   temperature: float = 1.0, ignore_index: int = -100) -> TokenLogprobs:
+    """What a row of ``logits`` (..., V), float32 or bf16, says about tokens: `TokenLogprobs` of
+    float32 ``logp`` (...,), ``log softmax(logits / temperature)`` at ``targets`` (...,);
+    ``entropy`` (...,) of that distribution; ``top_logp`` and int64 ``top_ids`` (..., top), its
+    ``top`` (at most 64) best ids in falling order, of equal logits the lower id first.
+
+    ``logp``, ``entropy`` and ``top_logp`` are differentiable in ``logits``. ``logits`` may be a
+    strided view (``logits[:, :-1]`` against ``tokens[:, 1:]`` makes no copy). Positions whose
+    target is ``ignore_index`` are padding: their logits are not read, logp and entropy are 0, ids
+    -1 (which `distill_loss` takes for no entry) and their gradient is 0. Any other target outside
+    [0, V) gives NaN; a row of nothing but -inf has logp -inf, entropy 0 and no gradient; a row with
+    a NaN or +inf is NaN, with ids -1."""
+    if _needs_node(logits):
+        return TokenLogprobs(*_LogprobFn.apply(logits, targets, int(top), float(temperature),
+                                               int(ignore_index)))
+    return TokenLogprobs(*K.logprob_forward(logits, targets, top, temperature, ignore_index)[:4])
+
+
+class DistillLoss(NamedTuple):
+    """`distill_loss`' per-row results; ``nll`` is None without targets."""
+
+    kd: Tensor
+    nll: Optional[Tensor]
+
+
+class _DistillFn(torch.autograd.Function):
+    """`kernels.distill_forward` / `kernels.distill_backward` as one node."""
+
+    @staticmethod
+    def forward(ctx, logits, ids, teacher, targets, temperature, ignore_index):
+        kd, nll, stats = K.distill_forward(logits, ids, teacher, targets, temperature, ignore_index)
+        ctx.save_for_backward(logits, ids, teacher, targets, stats)
+        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.set_materialize_grads(False)
+        return kd, nll
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dkd, dnll):
+        if dkd is None and dnll is None:
+            return None, None, None, None, None, None
+        logits, ids, teacher, targets, stats = ctx.saved_tensors
+        dx = K.distill_backward(logits, ids, teacher, targets, stats, dkd, dnll, ctx.temperature,
+                                ctx.ignore_index)
+        return dx, None, None, None, None, None
+
+
+def distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
+                 temperature: float = 1.0, targets: Optional[Tensor] = None,
+                 ignore_index: int = -100) -> DistillLoss:
+    """The loss of a student's ``logits`` (..., V) against a teacher's best K (at most 256) tokens,
+    per row in float32, differentiable in ``logits``: `DistillLoss` of ``kd = T^2 sum_i w_i (log w_i
+    - log softmax(logits / T)[id_i])`` with ``w = softmax(teacher_logits / T)`` over the K entries
+    (log-probabilities as `token_logprobs` gives them serve as well), and with ``targets``
+    ``nll = -log softmax(logits)[target]``, the cross-entropy, from the same pass.
+
+    Entries with an id < 0 do not count; a row without any has kd 0, one whose target is
+    ``ignore_index`` nll 0, and neither sends a gradient (nor is a row without both read). A
+    repeated id adds up. An id >= V, or another target outside [0, V), gives NaN. The teacher is a
+    constant: logits of it that require a gradient are refused."""
+    if torch.is_grad_enabled() and teacher_logits.requires_grad:
+        raise ValueError("distill_loss: the teacher's logits must not require a gradient (detach them)")
+    if _needs_node(logits, teacher_logits):
+        return DistillLoss(*_DistillFn.apply(logits, teacher_ids, teacher_logits, targets,
+                                             float(temperature), int(ignore_index)))
+    return DistillLoss(*K.distill_forward(logits, teacher_ids, teacher_logits, targets, temperature,
+                                          ignore_index)[:2])

@@ -7,6 +7,7 @@
   multi-tensor (``torch._foreach_*``) launches with no host synchronisation.
 * `make_step` is ``train.py:382-451``'s one-device step: loss and gradients through
   `model.lm_forward` (the fused HIP layer), then the optimizer, params updated in place.
+* `make_distill_step` is that step with a teacher model's best tokens in the loss.
 * `_pick_token`, `generate` and `sample` are ``train.py:454-624``: chunked prefill, then
   `model.lm_decode_step` per token, sampling with repetition penalty, temperature and
   nucleus (top-p) filtering. `DecodeGraph` records one decode step of the whole stack as
@@ -194,6 +195,30 @@ def make_step(cfg: M.LMConfig, opt: AdamW, interpret: Any = False):
 
     def step(params: M.LMParams, opt_state: AdamW, xs: Tensor, ys: Tensor):
         loss = M.lm_loss(params, xs, ys, cfg)
+        loss.backward()
+        opt_state.step()
+        opt_state.zero_grad()
+        return loss.detach(), params, opt_state
+
+    return step
+
+
+def make_distill_step(cfg: M.LMConfig, opt: AdamW, teacher: M.LMParams, teacher_cfg: M.LMConfig,
+                      k: int = 32, temperature: float = 2.0, hard_weight: float = 0.5,
+                      ignore_index: int = -100):
+    """`make_step` with a teacher: each step scores the batch with the ``teacher`` model (no
+    gradient), keeps its ``k`` best tokens at each position and trains on `model.lm_distill_loss`.
+    Targets equal to ``ignore_index`` are padding. The two models share a vocabulary."""
+    if teacher_cfg.vocab_size != cfg.vocab_size:
+        raise ValueError(f"make_distill_step: the teacher's vocabulary of {teacher_cfg.vocab_size} is not "
+                         f"the student's of {cfg.vocab_size}")
+    k = min(k, cfg.vocab_size)
+
+    def step(params: M.LMParams, opt_state: AdamW, xs: Tensor, ys: Tensor):
+        with torch.no_grad():
+            best = M.lm_logprobs(teacher, xs, ys, teacher_cfg, top=k, ignore_index=ignore_index)
+        loss = M.lm_distill_loss(params, xs, ys, best.top_ids, best.top_logp, cfg, temperature,
+                                 hard_weight, ignore_index)
         loss.backward()
         opt_state.step()
         opt_state.zero_grad()

@@ -62,7 +62,7 @@ def test_embed_abi_refuses_bad_structs(m3):
         assert h.m3s_embed_bwd_workspace_bytes(*sizes) == -1
 
 
-def test_embed_struct_matches_the_header(m3, tmp_path):
+def test_structs_match_the_header(m3, tmp_path):
     import os
     import subprocess
 
@@ -70,7 +70,8 @@ def test_embed_struct_matches_the_header(m3, tmp_path):
 
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     src, exe = tmp_path / "t.c", tmp_path / "t"
-    pairs = [("m3s_embed_args", lib.EmbedArgs)]
+    pairs = [("m3s_embed_args", lib.EmbedArgs), ("m3s_logprob_args", lib.LogprobArgs),
+             ("m3s_distill_args", lib.DistillArgs)]
     lines = []
     for name, cls in pairs:
         lines.append(f'printf("%zu\\n", sizeof({name}));')
@@ -84,3 +85,85 @@ def test_embed_struct_matches_the_header(m3, tmp_path):
         want.append(ctypes.sizeof(cls))
         want += [getattr(cls, f[0]).offset for f in cls._fields_]
     assert got == want
+
+
+def test_logprobs_and_distillation_refuse_bad_arguments(m3):
+    x, t = torch.zeros(3, 10), torch.zeros(3, dtype=torch.int64)
+    ids, u = torch.zeros(3, 4, dtype=torch.int64), torch.zeros(3, 4)
+    T, D = m3.token_logprobs, m3.distill_loss
+    for call in (lambda: T(x, t), lambda: D(x, ids, u)):
+        with pytest.raises(ValueError, match="ROCm device only"):
+            call()
+    for top in (-1, 11, 65):
+        with pytest.raises(ValueError, match="top must be"):
+            T(torch.zeros(3, 100) if top == 65 else x, t, top=top)
+    for temp in (0.0, -1.0, float("nan"), float("inf")):
+        for call in (lambda: T(x, t, temperature=temp), lambda: D(x, ids, u, temperature=temp)):
+            with pytest.raises(ValueError, match="temperature"):
+                call()
+    bad = [lambda: T(x.double(), t), lambda: T(x, t.float()), lambda: T(x, t[:2]), lambda: T(x[:, :0], t),
+           lambda: T(torch.tensor(1.0), t), lambda: T(x, t[:, None]),
+           lambda: D(x.half(), ids, u), lambda: D(x, ids[:2], u), lambda: D(x, ids, u[:, :3]),
+           lambda: D(x, ids.short(), u), lambda: D(x, ids, u.double()), lambda: D(x, ids[:, :0], u[:, :0]),
+           lambda: D(x, ids.repeat(1, 65), u.repeat(1, 65)), lambda: D(x, ids, u, targets=t[:1]),
+           lambda: D(x, ids, u, targets=t.bool()), lambda: D(x, ids[0], u[0])]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+    with pytest.raises(ValueError, match="must not require a gradient"):
+        D(x, ids, u.requires_grad_(True))
+    K, stats3, stats5 = m3.kernels, torch.zeros(3, 3), torch.zeros(3, 5)
+    with pytest.raises(ValueError, match="needs the targets"):
+        K.logprob_backward(x, None, stats3, dlogp=torch.zeros(3))
+    with pytest.raises(ValueError, match="needs top_ids"):
+        K.logprob_backward(x, t, stats3, dtop_logp=torch.zeros(3, 2))
+    with pytest.raises(ValueError, match="stats"):
+        K.logprob_backward(x, t, stats5, dlogp=torch.zeros(3))
+
+
+def test_vocab_abi_refuses_bad_structs(m3):
+    from mamba3_siso_tpu_amd import _lib as lib
+
+    h = lib.load()
+    entries = ((h.m3s_logprob_fwd, lib.LogprobArgs), (h.m3s_logprob_bwd, lib.LogprobArgs),
+               (h.m3s_distill_fwd, lib.DistillArgs), (h.m3s_distill_bwd, lib.DistillArgs))
+
+    def args(cls, **kw):
+        a = cls()
+        a.struct_size, a.dtype = ctypes.sizeof(cls), lib.DTYPE_F32
+        a.batch, a.seqlen, a.vocab, a.temperature, a.ignore_index = 2, 3, 10, 1.0, -100
+        a.logits = lib.Blx(4096, 30, 10)   # addresses are never read: every call is refused
+        for name in ("targets", "stats", "dlogits"):
+            setattr(a, name, 4096)
+        if cls is lib.LogprobArgs:
+            a.top = 2
+            for name in ("logp", "entropy", "top_logp", "top_ids", "dlogp", "dtop_logp"):
+                setattr(a, name, 4096)
+        else:
+            a.teacher_k, a.id_bytes, a.teacher_dtype = 4, 8, lib.DTYPE_BF16
+            for name in ("teacher_ids", "teacher_logits", "kd", "nll", "dkd", "dnll"):
+                setattr(a, name, 4096)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return a
+
+    common = [dict(dtype=5), dict(batch=-1), dict(seqlen=-1), dict(vocab=0), dict(vocab=1 << 30),
+              dict(batch=1 << 16, seqlen=1 << 16), dict(temperature=0.0), dict(temperature=-2.0),
+              dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-39),
+              dict(stats=None), dict(logits=lib.Blx(None, 30, 10)), dict(logits=lib.Blx(4098, 30, 10)),
+              dict(logits=lib.Blx(4096, -30, 10)), dict(logits=lib.Blx(4096, 30, -10))]
+    own = [[dict(top=-1), dict(top=65, vocab=100), dict(top=11), dict(logp=None), dict(entropy=None),
+            dict(top_logp=None), dict(top_ids=None)],
+           [dict(top=65, vocab=100), dict(dlogits=None), dict(dlogits=4098), dict(targets=None),
+            dict(top_ids=None)],
+           [dict(teacher_k=0), dict(teacher_k=257), dict(id_bytes=2), dict(teacher_dtype=9), dict(kd=None),
+            dict(nll=None), dict(targets=None), dict(teacher_ids=None), dict(teacher_logits=None)],
+           [dict(teacher_k=0), dict(dlogits=None), dict(dlogits=4098), dict(targets=None),
+            dict(teacher_ids=None)]]
+    for (entry, cls), extra in zip(entries, own):
+        assert entry(None, None) == lib.ERR_INVALID and b"NULL" in h.m3s_last_error()
+        assert entry(ctypes.byref(args(cls, struct_size=3)), None) == lib.ERR_INVALID
+        assert b"ABI mismatch" in h.m3s_last_error()
+        for bad in common + extra:
+            assert entry(ctypes.byref(args(cls, **bad)), None) == lib.ERR_INVALID, (cls, bad)
+        assert entry(ctypes.byref(args(cls, batch=0)), None) == lib.OK   # nothing to launch
