@@ -670,7 +670,12 @@ typedef struct m3s_logprob_args {
   const float* dentropy; /* backward in (rows) or NULL */
   const float* dtop_logp; /* backward in (rows, top) or NULL */
   void* dlogits;         /* backward out (rows, vocab) */
+  void* workspace;       /* forward scratch, 16-byte aligned, or NULL: every row stays whole */
+  int64_t workspace_bytes; /* its size: rows are cut with m3s_logprob_workspace_bytes() */
 } m3s_logprob_args;
+/* The scratch of the few long rows that are cut into pieces: their sums and best tokens. 0 where
+ * none is, -1 on bad dimensions. */
+int64_t m3s_logprob_workspace_bytes(int64_t rows, int32_t vocab, int32_t top);
 int32_t m3s_logprob_fwd(const m3s_logprob_args* args, void* stream);
 int32_t m3s_logprob_bwd(const m3s_logprob_args* args, void* stream);
 
@@ -702,7 +707,11 @@ typedef struct m3s_distill_args {
   const float* dkd;      /* backward in (rows) or NULL */
   const float* dnll;     /* backward in (rows) or NULL */
   void* dlogits;         /* backward out (rows, vocab) */
+  void* workspace;       /* forward scratch, 16-byte aligned, or NULL: every row stays whole */
+  int64_t workspace_bytes; /* its size: rows are cut with m3s_distill_workspace_bytes() */
 } m3s_distill_args;
+/* As m3s_logprob_workspace_bytes. */
+int64_t m3s_distill_workspace_bytes(int64_t rows, int32_t vocab);
 int32_t m3s_distill_fwd(const m3s_distill_args* args, void* stream);
 int32_t m3s_distill_bwd(const m3s_distill_args* args, void* stream);
 

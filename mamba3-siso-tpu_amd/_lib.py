@@ -239,6 +239,7 @@ class LogprobArgs(C.Structure):
         ("top", i32), ("temperature", C.c_float), ("ignore_index", i64), ("logits", Blx),
         ("targets", vp), ("logp", vp), ("entropy", vp), ("stats", vp), ("top_logp", vp),
         ("top_ids", vp), ("dlogp", vp), ("dentropy", vp), ("dtop_logp", vp), ("dlogits", vp),
+        ("workspace", vp), ("workspace_bytes", i64),
     ]
 
 
@@ -248,7 +249,7 @@ class DistillArgs(C.Structure):
         ("teacher_k", i32), ("teacher_dtype", i32), ("id_bytes", i32), ("temperature", C.c_float),
         ("ignore_index", i64), ("logits", Blx), ("teacher_ids", vp), ("teacher_logits", vp),
         ("targets", vp), ("kd", vp), ("nll", vp), ("stats", vp), ("dkd", vp), ("dnll", vp),
-        ("dlogits", vp),
+        ("dlogits", vp), ("workspace", vp), ("workspace_bytes", i64),
     ]
 
 
@@ -266,7 +267,8 @@ EXPORTS = ("m3s_abi_version", "m3s_last_error", "m3s_supported", "m3s_fwd_raw_su
            "m3s_swiglu_bwd", "m3s_rms_fwd", "m3s_rms_bwd", "m3s_rms_bwd_workspace_bytes",
            "m3s_norm_bwd_noalloc", "m3s_adamw", "m3s_wgrad", "m3s_wgrad_workspace_bytes", "m3s_gemv",
            "m3s_gemv_fused", "m3s_embed_bwd_workspace_bytes", "m3s_embed_fwd", "m3s_embed_bwd",
-           "m3s_logprob_fwd", "m3s_logprob_bwd", "m3s_distill_fwd", "m3s_distill_bwd")
+           "m3s_logprob_fwd", "m3s_logprob_bwd", "m3s_distill_fwd", "m3s_distill_bwd",
+           "m3s_logprob_workspace_bytes", "m3s_distill_workspace_bytes")
 
 _lib = None
 
@@ -363,6 +365,10 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     for fn in (lib.m3s_embed_fwd, lib.m3s_embed_bwd):
         fn.restype = i32
         fn.argtypes = [C.POINTER(EmbedArgs), vp]
+    lib.m3s_logprob_workspace_bytes.restype = i64
+    lib.m3s_logprob_workspace_bytes.argtypes = [i64, i32, i32]
+    lib.m3s_distill_workspace_bytes.restype = i64
+    lib.m3s_distill_workspace_bytes.argtypes = [i64, i32]
     for fn in (lib.m3s_logprob_fwd, lib.m3s_logprob_bwd):
         fn.restype = i32
         fn.argtypes = [C.POINTER(LogprobArgs), vp]
@@ -406,6 +412,12 @@ def supported(which: int, dtype: int, chunk: int, state_dim: int, headdim: int) 
 def raw_supported(dtype: int, chunk: int, state_dim: int, headdim: int, n_angles: int) -> bool:
     """Whether ``m3s_fwd`` takes this shape in raw mode (`m3s_fwd_raw_supported`)."""
     return bool(load().m3s_fwd_raw_supported(dtype, chunk, state_dim, headdim, n_angles))
+
+
+@functools.lru_cache(maxsize=4096)
+def scratch_bytes(entry: str, *sizes: int) -> int:
+    """What the library's ``entry`` (an ``m3s_*_workspace_bytes``) answers; it depends on the sizes alone."""
+    return getattr(load(), entry)(*sizes)
 
 
 def dtype_code(dt: torch.dtype) -> int:

@@ -21,6 +21,7 @@
 //
 // Rows may start at any element: 16-byte accesses need no alignment on gfx950.
 #include <algorithm>
+#include <type_traits>
 
 #include "m3s_common.h"
 #include "m3s_internal.h"
@@ -29,7 +30,8 @@ namespace m3s {
 
 constexpr int kRowThreads = 256;
 constexpr int kTopMax = 64;        // alternatives of a row
-constexpr int kTeacherMax = 256;   // teacher tokens of a row: one a thread
+constexpr int kTeacherMax = 256;   // teacher tokens of a row
+constexpr int kWaveVocab = 1024;   // rows up to this long go to a single wave
 constexpr float kNegInf = -__builtin_inff();
 
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
@@ -62,34 +64,57 @@ template <> struct Piece<bf16> {
   }
 };
 
-// ---- reductions over a workgroup of four waves ----------------------------------------------
-__device__ __forceinline__ float wave_max(float v) {
+// ---- a row's group of waves -------------------------------------------------------------------
+// NW = 4: the workgroup shares a row. NW = 1: each wave has its own, and nothing waits for others.
+template <int NW>
+struct Group {
+  static constexpr int NT = 64 * NW;        // threads to a row
+  static constexpr int ROWS = 4 / NW;       // rows to a workgroup
+  static __device__ __forceinline__ int tid() { return NW == 1 ? lane_id() : (int)threadIdx.x; }
+  static __device__ __forceinline__ int slot() { return NW == 1 ? (int)threadIdx.x >> 6 : 0; }
+  // what the group wrote to LDS or memory before is seen by it after
+  static __device__ __forceinline__ void sync() {
+    if constexpr (NW == 1) {
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+    } else {
+      __syncthreads();
+    }
+  }
+  // Reductions: the same value to every thread; `tmp` holds four floats and is free afterwards.
+  static __device__ __forceinline__ float max(float v, float* tmp) {
 #pragma unroll
-  for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-  return v;
-}
-// Each returns the same value to every thread; `tmp` holds four floats and is free afterwards.
-__device__ __forceinline__ float block_max(float v, float* tmp) {
-  v = wave_max(v);
-  if (lane_id() == 0) tmp[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
-  __syncthreads();
-  return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* tmp) {
-  v = wave_total(v);
-  if (lane_id() == 0) tmp[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
-  __syncthreads();
-  return v;
-}
+    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    if constexpr (NW == 4) {
+      if (lane_id() == 0) tmp[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = fmaxf(fmaxf(tmp[0], tmp[1]), fmaxf(tmp[2], tmp[3]));
+      __syncthreads();
+    }
+    return v;
+  }
+  static __device__ __forceinline__ float sum(float v, float* tmp) {
+    v = wave_total(v);
+    if constexpr (NW == 4) {
+      if (lane_id() == 0) tmp[threadIdx.x >> 6] = v;
+      __syncthreads();
+      v = (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
+      __syncthreads();
+    }
+    return v;
+  }
+};
 
 // ---- running sums of a row ------------------------------------------------------------------
 // s = sum 2^{c (x - m)}, t = sum of the same times (x - m), s1 = sum 2^{c1 (x - m)}. A row of -inf
 // keeps m = -inf and zeros; a NaN or +inf makes the sums NaN (fmaxf drops the NaN, s does not).
-enum { kPlain = 0, kEntropy = 1, kDual = 2 };
+enum { kEntropy = 1, kDual = 2 };
+// 2^{a b} with the product's rounding made good: a factor on a whole sum, so its error does not
+// average out as the terms' do (one row of 131072 in pieces: log-probability off by 1e-7, not 5e-7).
+__device__ __forceinline__ float exp2_product(float a, float b) {
+  const float hi = a * b;
+  return __builtin_amdgcn_exp2f(hi) * fmaf(fmaf(a, b, -hi), kLn2, 1.f);
+}
 template <int MODE>
 struct RowSums {
   float m = kNegInf, s = 0.f, t = 0.f, s1 = 0.f;
@@ -99,17 +124,15 @@ struct RowSums {
     const float mn = fmaxf(m, to);
     const float ref = mn == kNegInf ? 0.f : mn;
     const float gap = fmaxf(m - ref, -1e30f);   // 0 * -1e30, not 0 * -inf, while s = 0
-    const float f = __builtin_amdgcn_exp2f(gap * c);
+    const float f = exp2_product(gap, c);
     if constexpr (MODE == kEntropy) t = (t + s * gap) * f;
     s *= f;
-    if constexpr (MODE == kDual) s1 *= __builtin_amdgcn_exp2f(gap * c1);
+    if constexpr (MODE == kDual) s1 *= exp2_product(gap, c1);
     m = mn;
   }
+  // N more logits, the largest of them `top`
   template <int N>
-  __device__ __forceinline__ void add(const float* x, float c, float c1) {
-    float top = x[0];
-#pragma unroll
-    for (int i = 1; i < N; ++i) top = fmaxf(top, x[i]);
+  __device__ __forceinline__ void add(const float* x, float top, float c, float c1) {
     raise(top, c, c1);
     const float ref = m == kNegInf ? 0.f : m;
 #pragma unroll
@@ -121,42 +144,79 @@ struct RowSums {
       if constexpr (MODE == kDual) s1 += __builtin_amdgcn_exp2f(d * c1);
     }
   }
-  __device__ __forceinline__ void join_block(float c, float c1, float* tmp) {
-    raise(block_max(m, tmp), c, c1);
-    s = block_sum(s, tmp);
-    if constexpr (MODE == kEntropy) t = block_sum(t, tmp);
-    if constexpr (MODE == kDual) s1 = block_sum(s1, tmp);
+  template <typename G>
+  __device__ __forceinline__ void join(float c, float c1, float* tmp) {
+    raise(G::max(m, tmp), c, c1);
+    s = G::sum(s, tmp);
+    if constexpr (MODE == kEntropy) t = G::sum(t, tmp);
+    if constexpr (MODE == kDual) s1 = G::sum(s1, tmp);
   }
 };
 
-// One pass over n logits by the workgroup.
-template <int MODE, typename T>
-__device__ __forceinline__ void row_pass(RowSums<MODE>& r, const T* __restrict__ x, int n, float c,
-                                         float c1) {
-  constexpr int N = Piece<T>::N, U = 16 / N, HOP = kRowThreads * U;
-  const int full = n / N, tail = n - full * N, tid = threadIdx.x;
-  for (int p = 0; p < full; p += HOP) {
-    float v[U * N];
+// Where a thread's best logits lie: the largest maxima of its batches (U pieces of 16 bytes), the
+// first two with their batch, so that the alternatives are found without reading the row again.
+struct Best {
+  float m1 = kNegInf, m2 = kNegInf, m3 = kNegInf;
+  int b1 = -1, b2 = -1;   // -1: none seen, or none above -inf
+  __device__ __forceinline__ void see(float v, int batch) {
+    const bool first = v > m1, second = v > m2;
+    m3 = fmaxf(m3, fminf(m2, v));
+    b2 = first ? b1 : second ? batch : b2;
+    m2 = first ? m1 : fmaxf(m2, v);
+    b1 = first ? batch : b1;
+    m1 = fmaxf(m1, v);
+  }
+};
+
+// A thread's batch of a row of n logits: pieces batch U NT + u NT + tid, u < U; past the last whole
+// batch come the logits that fill no piece, one a thread. Missing ones are -inf.
+template <typename G, int U, typename T>
+struct Rows {
+  static constexpr int N = Piece<T>::N, HOP = G::NT * U, LEN = U * N;
+  static __device__ __forceinline__ int whole(int n) { return (n / N + HOP - 1) / HOP; }   // batches
+  static __device__ __forceinline__ int place(int batch, int i) {   // index of its i-th logit
+    return (batch * HOP + i / N * G::NT + G::tid()) * N + i % N;
+  }
+  static __device__ __forceinline__ void load(const T* __restrict__ x, int n, int batch, float* v) {
+    const int full = n / N, p = batch * HOP;
     if (p + HOP <= full) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) Piece<T>::load(x + (int64_t)(p + u * kRowThreads + tid) * N, v + u * N);
-    } else {
+      for (int u = 0; u < U; ++u) Piece<T>::load(x + (int64_t)(p + u * G::NT + G::tid()) * N, v + u * N);
+      return;
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int at = p + u * kRowThreads + tid;
-        if (at < full) {
-          Piece<T>::load(x + (int64_t)at * N, v + u * N);
-        } else {
+    for (int u = 0; u < U; ++u) {
+      const int at = p + u * G::NT + G::tid();
+      if (at < full) {
+        Piece<T>::load(x + (int64_t)at * N, v + u * N);
+      } else {
 #pragma unroll
-          for (int i = 0; i < N; ++i) v[u * N + i] = kNegInf;
-        }
+        for (int i = 0; i < N; ++i) v[u * N + i] = kNegInf;
       }
     }
-    r.template add<U * N>(v, c, c1);
   }
-  if (tid < tail) {
-    const float v = (float)x[(int64_t)full * N + tid];
-    r.template add<1>(&v, c, c1);
+};
+
+// One pass over n logits by the group.
+template <typename G, int U, bool TOP, int MODE, typename T>
+__device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* __restrict__ x, int n,
+                                         float c, float c1) {
+  using R = Rows<G, U, T>;
+  const int batches = R::whole(n);
+  for (int b = 0; b < batches; ++b) {
+    float v[R::LEN];
+    R::load(x, n, b, v);
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < R::LEN; ++i) top = fmaxf(top, v[i]);
+    if constexpr (TOP) best.see(top, b);
+    r.template add<R::LEN>(v, top, c, c1);
+  }
+  const int at = n / R::N * R::N + G::tid();
+  if (at < n) {
+    const float v = (float)x[at];
+    if constexpr (TOP) best.see(v, batches);
+    r.template add<1>(&v, v, c, c1);
   }
 }
 
@@ -166,35 +226,192 @@ __device__ __forceinline__ const T* row_at(const m3s_blx& b, int64_t r, int seql
   return static_cast<const T*>(b.ptr) + i * b.stride_b + (r - i * seqlen) * b.stride_t;
 }
 
-// The k best of a row, one round of (largest value, lowest index) each. For rows without NaN.
-template <typename T, typename OUT>
-__device__ __forceinline__ void pick_rounds(const T* __restrict__ x, int n, int k, float* tmp,
-                                            int* itmp, OUT&& out) {
-  float last = __builtin_inff();
-  int last_i = -1;
-  for (int j = 0; j < k; ++j) {
-    float best = kNegInf;
-    int best_i = 0x7fffffff;
-    for (int i = threadIdx.x; i < n; i += kRowThreads) {
-      const float v = (float)x[i];
-      const bool left = v < last || (v == last && i > last_i);
-      if (left && (v > best || (v == best && i < best_i))) {
-        best = v;
-        best_i = i;
+// ---- the k largest of a row --------------------------------------------------------------------
+// Unsigned keys in the floats' order (-0 counts as 0).
+__device__ __forceinline__ uint32_t float_key(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.f);
+  return b ^ ((b >> 31) ? 0xffffffffu : 0x80000000u);
+}
+__device__ __forceinline__ float key_float(uint32_t k) {
+  return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
+}
+// A bound that at least k of the wave's 64 N values reach, and as few more as ties allow: bit by
+// bit from the top, by ballots.
+template <int N>
+__device__ __forceinline__ float kth_bound(const float* v, int k) {
+  uint32_t key[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) key[i] = float_key(v[i]);
+  uint32_t at = 0;
+  for (int bit = 31; bit >= 0; --bit) {
+    const uint32_t trial = at | (1u << bit);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= trial));
+    if (n >= k) at = trial;
+    if (n == k) break;
+  }
+  return key_float(at < 0x007fffffu ? 0x007fffffu : at);   // not below the key of -inf
+}
+
+template <int NW>
+struct PickSpace {
+  static constexpr int CAP = NW == 4 ? 1024 : 512;
+  float best[64 * NW];
+  float v[CAP];
+  int i[CAP];
+  int count;
+  int itmp[4];
+  float tmp[4];
+};
+
+// Appends this thread's logit to the candidates if `hit`; a full list only counts.
+template <int CAP>
+__device__ __forceinline__ void append(bool hit, float v, int i, float* lv, int* li, int* count) {
+  const uint64_t m = __ballot(hit);
+  if (m == 0) return;
+  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+  int base = 0;
+  if (hit && before == 0) base = atomicAdd(count, (int)__popcll(m));
+  base = __builtin_amdgcn_readlane(base, __ffsll((unsigned long long)m) - 1);
+  if (hit && base + before < CAP) {
+    lv[base + before] = v;
+    li[base + before] = i;
+  }
+}
+
+// The candidates: every logit that reaches `bar` (STRICT: exceeds it), from the batches that hold
+// one. Returns their number, which may be more than the list holds.
+template <typename G, int U, bool STRICT, int NW, typename T>
+__device__ __forceinline__ int gather(const T* __restrict__ x, int n, const Best& best, float bar,
+                                      PickSpace<NW>& sp) {
+  using R = Rows<G, U, T>;
+  constexpr int CAP = PickSpace<NW>::CAP;
+  const auto in = [&](float v) { return STRICT ? v > bar : v >= bar; };
+  const int batches = R::whole(n);
+  if (G::tid() == 0) sp.count = 0;
+  G::sync();
+  const auto take = [&](int b) {
+    if (b == batches) {
+      const int at = n / R::N * R::N + G::tid();
+      const float v = at < n ? (float)x[at] : kNegInf;
+      append<CAP>(at < n && in(v), v, at, sp.v, sp.i, &sp.count);
+      return;
+    }
+    float v[R::LEN];
+    R::load(x, n, b, v);
+#pragma unroll
+    for (int i = 0; i < R::LEN; ++i) {
+      const int at = R::place(b, i);
+      append<CAP>(at < n / R::N * R::N && in(v[i]), v[i], at, sp.v, sp.i, &sp.count);
+    }
+  };
+  if (in(best.m1)) {
+    if (best.b1 >= 0) take(best.b1);
+    if (in(best.m2) && best.b2 >= 0) take(best.b2);
+    if (in(best.m3)) {
+      for (int b = 0; b <= batches; ++b) {
+        if (b != best.b1 && b != best.b2 && *(volatile int*)&sp.count <= CAP) take(b);
       }
     }
-    const float v = block_max(best, tmp);
-    int i = best == v ? best_i : 0x7fffffff;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) i = min(i, __shfl_xor(i, o));
-    if (lane_id() == 0) itmp[threadIdx.x >> 6] = i;
-    __syncthreads();
-    i = min(min(itmp[0], itmp[1]), min(itmp[2], itmp[3]));
-    __syncthreads();
-    if (threadIdx.x == 0) out(j, v, i);
-    last = v;
-    last_i = i;
   }
+  G::sync();
+  const int count = sp.count;
+  G::sync();
+  return count;
+}
+
+// Ranks the `count` candidates; those under k go out.
+template <typename G, int NW, typename OUT>
+__device__ __forceinline__ void rank_out(int count, int k, const PickSpace<NW>& sp, OUT&& out) {
+  for (int c = G::tid(); c < count; c += G::NT) {
+    const float v = sp.v[c];
+    const int i = sp.i[c];
+    int rank = 0;
+    for (int j = 0; j < count; ++j) rank += sp.v[j] > v || (sp.v[j] == v && sp.i[j] < i);
+    if (rank < k) out(rank, v, i);
+  }
+}
+
+// Logits equal to `v`, in the order of their index, to the places from `from` up to k.
+template <typename G, int NW, typename T, typename OUT>
+__device__ __forceinline__ void equal_out(const T* __restrict__ x, int n, float v, int from, int k,
+                                          PickSpace<NW>& sp, OUT&& out) {
+  const int lane = lane_id();
+  for (int p = 0; p < n && from < k; p += G::NT) {
+    const int at = p + G::tid();
+    const bool eq = at < n && (float)x[at] == v;
+    const uint64_t m = __ballot(eq);
+    int before = __popcll(m & ((1ull << lane) - 1)), all = __popcll(m);
+    if constexpr (NW == 4) {
+      const int wave = threadIdx.x >> 6;
+      if (lane == 0) sp.itmp[wave] = all;
+      __syncthreads();
+      all = 0;
+      for (int w = 0; w < 4; ++w) {
+        if (w < wave) before += sp.itmp[w];
+        all += sp.itmp[w];
+      }
+      __syncthreads();
+    }
+    if (eq && from + before < k) out(from + before, v, at);
+    from += all;
+  }
+}
+
+// One value after another, for rows whose best logits all fell to few threads: the largest value
+// below the last, then all that equal it.
+template <typename G, int NW, typename T, typename OUT>
+__device__ __forceinline__ void values_out(const T* __restrict__ x, int n, int k, PickSpace<NW>& sp,
+                                           OUT&& out) {
+  float last = __builtin_inff();
+  for (int done = 0; done < k;) {
+    float v = kNegInf;
+    int same = 0;
+    for (int i = G::tid(); i < n; i += G::NT) {
+      const float e = (float)x[i];
+      if (e < last) {
+        same = e > v ? 1 : same + (e == v);
+        v = fmaxf(v, e);
+      }
+    }
+    const float top = G::max(v, sp.tmp);
+    same = (int)G::sum(v == top ? (float)same : 0.f, sp.tmp);   // exact below 2^24, and k is 64
+    equal_out<G>(x, n, top, done, k, sp, out);
+    done += same;
+    last = top;
+    if (same == 0) break;
+  }
+}
+
+// out(rank, value, index) for the k largest of n logits (k <= n, no NaN, no +inf), equal ones by
+// index. The k-th largest of the threads' maxima is reached by at least k logits, and by hardly
+// more: those are collected from the few batches that hold them and ranked against each other.
+template <typename G, int U, int NW, typename T, typename OUT>
+__device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, const Best& best,
+                                     PickSpace<NW>& sp, OUT&& out) {
+  constexpr int CAP = PickSpace<NW>::CAP;
+  float m[NW];
+  if constexpr (NW == 1) {
+    m[0] = best.m1;
+  } else {
+    sp.best[threadIdx.x] = best.m1;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NW; ++i) m[i] = sp.best[64 * i + lane_id()];
+  }
+  const float bar = kth_bound<NW>(m, k);
+  int count = gather<G, U, false>(x, n, best, bar, sp);
+  if (count > CAP) {   // many ties, as in masked rows: what exceeds them, then the first of them
+    count = gather<G, U, true>(x, n, best, bar, sp);
+    if (count > CAP) {
+      values_out<G>(x, n, k, sp, out);
+      return;
+    }
+    equal_out<G>(x, n, bar, count, k, sp, out);
+  }
+  rank_out<G>(count, k, sp, out);
+  G::sync();   // the space is free again
 }
 
 // ---- log-probabilities ----------------------------------------------------------------------
@@ -205,75 +422,197 @@ struct LogprobParams {
   int64_t* top_ids;
   const float *dlogp, *dentropy, *dtop;
   void* dlogits;
+  float* part;       // a split row's pieces: (rows, split, 3) sums, (rows, split, top) values and ids
   int64_t ignore, rows;
-  int seqlen, vocab, top, chunks;
+  int seqlen, vocab, top, chunks, split, share;   // share: logits to a piece
   float temp, inv_t, c;
 };
 
-template <typename T>
+struct LogprobParts {
+  float *sums, *v;
+  int* i;
+  __device__ LogprobParts(const LogprobParams& p, int64_t r) {
+    const int64_t all = p.rows * p.split;
+    sums = p.part + 3 * r * p.split;
+    v = p.part + 3 * all + r * p.split * p.top;
+    i = reinterpret_cast<int*>(p.part + (3 + p.top) * all) + r * p.split * p.top;
+  }
+};
+
+// A row without a token at it: the logits are not read.
+template <typename G>
+__device__ __forceinline__ void logprob_skip(const LogprobParams& p, int64_t r) {
+  if (G::tid() == 0) {
+    p.logp[r] = p.entropy[r] = 0.f;
+    p.stats[3 * r] = p.stats[3 * r + 1] = p.stats[3 * r + 2] = 0.f;
+  }
+  for (int j = G::tid(); j < p.top; j += G::NT) {
+    p.top_logp[r * p.top + j] = kNegInf;
+    p.top_ids[r * p.top + j] = -1;
+  }
+}
+
+struct LogprobRow {   // from finished sums
+  float m, logs, temp;
+  bool empty;
+  __device__ LogprobRow(const RowSums<kEntropy>& s, float temp_)
+      : m(s.m), logs(logf(s.s)), temp(temp_), empty(s.m == kNegInf && s.s == 0.f) {}
+  __device__ float operator()(float v) const { return empty ? kNegInf : (v - m) / temp - logs; }
+};
+
+template <typename G, typename T>
+__device__ __forceinline__ void logprob_store(const LogprobParams& p, int64_t r, int64_t tgt, const T* x,
+                                              const RowSums<kEntropy>& sum, const LogprobRow& logp) {
+  if (G::tid() != 0) return;
+  const float h = logp.empty ? 0.f : logp.logs - sum.t / (p.temp * sum.s);
+  p.entropy[r] = h;
+  p.stats[3 * r] = sum.m;
+  p.stats[3 * r + 1] = sum.s;
+  p.stats[3 * r + 2] = h;
+  if (p.targets) p.logp[r] = tgt >= 0 && tgt < p.vocab ? logp((float)x[tgt]) : __builtin_nanf("");
+}
+
+// NaN or +inf among the logits: no order to report.
+template <typename G>
+__device__ __forceinline__ void logprob_unordered(const LogprobParams& p, int64_t r) {
+  for (int j = G::tid(); j < p.top; j += G::NT) {
+    p.top_logp[r * p.top + j] = __builtin_nanf("");
+    p.top_ids[r * p.top + j] = -1;
+  }
+}
+
+template <bool TOP, int NW, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobParams p) {
+  using G = Group<NW>;
   __shared__ float tmp[4];
-  __shared__ int itmp[4];
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+  __shared__ PickSpace<NW> space[TOP ? G::ROWS : 1];
+  for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
     const int64_t tgt = p.targets ? p.targets[r] : 0;
-    if (p.targets && tgt == p.ignore) {   // no token here: the logits are not read
-      if (threadIdx.x == 0) {
-        p.logp[r] = p.entropy[r] = 0.f;
-        p.stats[3 * r] = p.stats[3 * r + 1] = p.stats[3 * r + 2] = 0.f;
-      }
-      for (int j = threadIdx.x; j < p.top; j += kRowThreads) {
-        p.top_logp[r * p.top + j] = kNegInf;
-        p.top_ids[r * p.top + j] = -1;
-      }
+    if (p.targets && tgt == p.ignore) {
+      logprob_skip<G>(p, r);
       continue;
     }
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     RowSums<kEntropy> sum;
-    row_pass<kEntropy>(sum, x, p.vocab, p.c, 0.f);
-    sum.join_block(p.c, 0.f, tmp);
-    const bool empty = sum.m == kNegInf && sum.s == 0.f;
-    const float logs = logf(sum.s);
-    const auto logp = [&](float v) { return empty ? kNegInf : (v - sum.m) / p.temp - logs; };
-    if (threadIdx.x == 0) {
-      const float h = empty ? 0.f : logs - sum.t / (p.temp * sum.s);
-      p.entropy[r] = h;
-      p.stats[3 * r] = sum.m;
-      p.stats[3 * r + 1] = sum.s;
-      p.stats[3 * r + 2] = h;
-      if (p.targets) p.logp[r] = tgt >= 0 && tgt < p.vocab ? logp((float)x[tgt]) : __builtin_nanf("");
-    }
-    if (p.top == 0) continue;
-    if (sum.s != sum.s) {   // NaN or +inf among the logits: no order to report
-      for (int j = threadIdx.x; j < p.top; j += kRowThreads) {
-        p.top_logp[r * p.top + j] = __builtin_nanf("");
-        p.top_ids[r * p.top + j] = -1;
+    Best best;
+    row_pass<G, U, TOP>(sum, best, x, p.vocab, p.c, 0.f);
+    sum.template join<G>(p.c, 0.f, tmp);
+    const LogprobRow logp(sum, p.temp);
+    logprob_store<G>(p, r, tgt, x, sum, logp);
+    if constexpr (TOP) {
+      if (sum.s != sum.s) {
+        logprob_unordered<G>(p, r);
+        continue;
       }
-      continue;
+      pick<G, U>(x, p.vocab, p.top, best, space[G::slot()], [&](int j, float v, int i) {
+        p.top_logp[r * p.top + j] = logp(v);
+        p.top_ids[r * p.top + j] = i;
+      });
     }
-    pick_rounds(x, p.vocab, p.top, tmp, itmp, [&](int j, float v, int i) {
+  }
+}
+
+// Few long rows: a workgroup to each of a row's `split` pieces ...
+template <bool TOP, int U, typename T>
+__global__ void __launch_bounds__(kRowThreads) logprob_piece_kernel(const LogprobParams p) {
+  using G = Group<4>;
+  __shared__ float tmp[4];
+  __shared__ PickSpace<4> space[1];
+  const int64_t r = blockIdx.x / p.split;
+  const int g = (int)(blockIdx.x - r * p.split);
+  if (p.targets && p.targets[r] == p.ignore) return;
+  const int lo = g * p.share, n = min(p.share, p.vocab - lo);
+  const T* x = row_at<T>(p.logits, r, p.seqlen) + lo;
+  const LogprobParts part(p, r);
+  RowSums<kEntropy> sum;
+  Best best;
+  row_pass<G, U, TOP>(sum, best, x, n, p.c, 0.f);
+  sum.template join<G>(p.c, 0.f, tmp);
+  if (threadIdx.x == 0) {
+    part.sums[3 * g] = sum.m;
+    part.sums[3 * g + 1] = sum.s;
+    part.sums[3 * g + 2] = sum.t;
+  }
+  if constexpr (TOP) {
+    float* pv = part.v + g * p.top;
+    int* pi = part.i + g * p.top;
+    const int k = sum.s != sum.s ? 0 : min(p.top, n);
+    for (int j = k + threadIdx.x; j < p.top; j += kRowThreads) {   // never among the best of the row
+      pv[j] = kNegInf;
+      pi[j] = -1;
+    }
+    if (k) {
+      pick<G, U>(x, n, k, best, space[0], [&](int j, float v, int i) {
+        pv[j] = v;
+        pi[j] = lo + i;
+      });
+    }
+  }
+}
+
+// ... and one to join them. Pieces stand in the order of the row and hold their best in order, so
+// equal values are in the order of their index here too.
+template <bool TOP, typename T>
+__global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const LogprobParams p) {
+  using G = Group<4>;
+  __shared__ float tmp[4];
+  __shared__ PickSpace<4> space[1];
+  const int64_t r = blockIdx.x;
+  const int64_t tgt = p.targets ? p.targets[r] : 0;
+  if (p.targets && tgt == p.ignore) {
+    logprob_skip<G>(p, r);
+    return;
+  }
+  const LogprobParts part(p, r);
+  RowSums<kEntropy> sum;
+  if ((int)threadIdx.x < p.split) {
+    sum.m = part.sums[3 * threadIdx.x];
+    sum.s = part.sums[3 * threadIdx.x + 1];
+    sum.t = part.sums[3 * threadIdx.x + 2];
+  }
+  sum.template join<G>(p.c, 0.f, tmp);
+  const LogprobRow logp(sum, p.temp);
+  logprob_store<G>(p, r, tgt, row_at<T>(p.logits, r, p.seqlen), sum, logp);
+  if constexpr (TOP) {
+    if (sum.s != sum.s) {
+      logprob_unordered<G>(p, r);
+      return;
+    }
+    const int n = p.split * p.top;
+    Best best;
+    const int batches = Rows<G, 1, float>::whole(n);
+    for (int b = 0; b < batches; ++b) {
+      float v[4];
+      Rows<G, 1, float>::load(part.v, n, b, v);
+      best.see(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), b);
+    }
+    const int at = n / 4 * 4 + threadIdx.x;
+    if (at < n) best.see(part.v[at], batches);
+    pick<G, 1>(part.v, n, p.top, best, space[0], [&](int j, float v, int i) {
       p.top_logp[r * p.top + j] = logp(v);
-      p.top_ids[r * p.top + j] = i;
+      p.top_ids[r * p.top + j] = part.i[i];
     });
   }
 }
 
-// The dense part of a gradient: f(d) for every logit of a chunk (blockIdx.x = row * chunks + chunk),
-// d = x - m. Returns nothing to the caller but the chunk's bounds.
+// ---- gradients ---------------------------------------------------------------------------------
+// The dense part: f(x) for every logit of lo .. hi - 1, at most kBwdPieces pieces a thread.
 constexpr int kBwdPieces = 4;
-template <typename T, typename F>
+template <typename G, typename T> constexpr int kChunk = G::NT* kBwdPieces* Piece<T>::N;
+template <typename G, typename T, typename F>
 __device__ __forceinline__ void chunk_map(const T* __restrict__ x, T* __restrict__ dx, int lo, int hi,
                                           F&& f) {
   constexpr int N = Piece<T>::N;
-  const int n = hi - lo, full = n / N, tid = threadIdx.x;
+  const int n = hi - lo, full = n / N;
   float v[kBwdPieces * N];
 #pragma unroll
   for (int u = 0; u < kBwdPieces; ++u) {
-    const int at = u * kRowThreads + tid;
+    const int at = u * G::NT + G::tid();
     if (at < full) Piece<T>::load(x + lo + at * N, v + u * N);
   }
 #pragma unroll
   for (int u = 0; u < kBwdPieces; ++u) {
-    const int at = u * kRowThreads + tid;
+    const int at = u * G::NT + G::tid();
     if (at < full) {
       float o[N];
 #pragma unroll
@@ -281,25 +620,37 @@ __device__ __forceinline__ void chunk_map(const T* __restrict__ x, T* __restrict
       Piece<T>::store(dx + lo + at * N, o);
     }
   }
-  const int at = full * N + tid;
+  const int at = full * N + G::tid();
   if (at < n) dx[lo + at] = (T)f((float)x[lo + at]);
 }
+template <typename G, typename T>
+__device__ __forceinline__ void chunk_zero(T* __restrict__ dx, int lo, int hi) {
+  constexpr int N = Piece<T>::N;
+  const float zero[N] = {};
+  const int full = (hi - lo) / N;
+  for (int at = G::tid(); at < full; at += G::NT) Piece<T>::store(dx + lo + at * N, zero);
+  const int at = lo + full * N + G::tid();
+  if (at < hi) dx[at] = (T)0.f;
+}
 
-template <typename T>
+template <int NW, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_bwd_kernel(const LogprobParams p) {
-  constexpr int CHUNK = kRowThreads * kBwdPieces * Piece<T>::N;
-  __shared__ int ids[kTopMax];
-  __shared__ float gtop[kTopMax];
-  for (int64_t w = blockIdx.x; w < p.rows * p.chunks; w += gridDim.x) {
+  using G = Group<NW>;
+  __shared__ int sids[G::ROWS][kTopMax];
+  __shared__ float sgrad[G::ROWS][kTopMax];
+  int* ids = sids[G::slot()];
+  float* gtop = sgrad[G::slot()];
+  const int64_t work = p.rows * p.chunks;
+  for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
     const int64_t r = w / p.chunks;
-    const int lo = (int)(w - r * p.chunks) * CHUNK, hi = min(lo + CHUNK, p.vocab);
+    const int lo = (int)(w - r * p.chunks) * kChunk<G, T>, hi = min(lo + kChunk<G, T>, p.vocab);
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
     const int64_t tgt = p.targets ? p.targets[r] : -1;
     const float m = p.stats[3 * r], s = p.stats[3 * r + 1], h = p.stats[3 * r + 2];
     // an ignored row, and one of nothing but -inf, has s = 0 and no gradient
     if (s == 0.f) {
-      for (int i = lo + threadIdx.x; i < hi; i += kRowThreads) dx[i] = (T)0.f;
+      chunk_zero<G>(dx, lo, hi);
       continue;
     }
     float gl = p.dlogp ? p.dlogp[r] * p.inv_t : 0.f;
@@ -315,23 +666,23 @@ __global__ void __launch_bounds__(kRowThreads) logprob_bwd_kernel(const LogprobP
       const float lq = fmaxf(d * p.inv_t - logs, -1e30f);
       return -q * (g + gh * (lq + h));
     };
-    chunk_map(x, dx, lo, hi, f);
+    chunk_map<G>(x, dx, lo, hi, f);
     // then the entries that a token or an alternative adds to, whole
-    for (int j = threadIdx.x; j < top; j += kRowThreads) {
+    for (int j = G::tid(); j < top; j += G::NT) {
       ids[j] = (int)p.top_ids[r * top + j];
       gtop[j] = p.dtop[r * top + j] * p.inv_t;
     }
-    __syncthreads();
-    for (int j = threadIdx.x; j < top; j += kRowThreads) {
+    G::sync();
+    for (int j = G::tid(); j < top; j += G::NT) {
       const int i = ids[j];
       if (i >= lo && i < hi) dx[i] = (T)(f((float)x[i]) + gtop[j] + (i == tgt ? gl : 0.f));
     }
-    if (threadIdx.x == 0 && p.dlogp && tgt >= lo && tgt < hi) {
+    if (G::tid() == 0 && p.dlogp && tgt >= lo && tgt < hi) {
       bool alone = true;
       for (int j = 0; j < top; ++j) alone = alone && ids[j] != tgt;
       if (alone) dx[tgt] = (T)(f((float)x[tgt]) + gl);
     }
-    __syncthreads();
+    G::sync();
   }
 }
 
@@ -343,8 +694,9 @@ struct DistillParams {
   float *kd, *nll, *stats;
   const float *dkd, *dnll;
   void* dlogits;
+  float* part;       // a split row's pieces: (rows, split, 3) sums
   int64_t ignore, rows;
-  int seqlen, vocab, k, chunks, id_bytes, teacher_bf16;
+  int seqlen, vocab, k, chunks, id_bytes, teacher_bf16, split, share;
   float temp, inv_t, c, c1;
 };
 
@@ -355,78 +707,151 @@ __device__ __forceinline__ float teacher_logit(const DistillParams& p, int64_t a
   return p.teacher_bf16 ? (float)static_cast<const bf16*>(p.teacher)[at] : static_cast<const float*>(p.teacher)[at];
 }
 
-// stats (rows, 5): m, sum e^{d / T}, sum e^d, the teacher's maximum and its sum (0: no entry; NaN: an
-// id outside the vocabulary, or a NaN).
-template <typename T>
+// A row's teacher tokens, kTeacherMax / NT to a thread: ids (-1: none), logits, and e^{(u - ref) / T}.
+// ts = 0 says that there is no entry, NaN that one is a NaN or an id outside the vocabulary.
+template <typename G>
+struct Teacher {
+  static constexpr int N = kTeacherMax / G::NT;
+  int64_t id[N];
+  float u[N], e[N], ref, ts;
+  __device__ __forceinline__ Teacher(const DistillParams& p, int64_t r, float* tmp) {
+    float top = kNegInf, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = i * G::NT + G::tid();
+      id[i] = -1;
+      u[i] = kNegInf;
+      if (at < p.k) {
+        id[i] = teacher_id(p, r * p.k + at);
+        if (id[i] >= 0) u[i] = teacher_logit(p, r * p.k + at);
+        if (id[i] >= p.vocab) u[i] = __builtin_nanf("");
+      }
+      top = fmaxf(top, u[i]);
+    }
+    top = G::max(top, tmp);
+    ref = top == kNegInf ? 0.f : top;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      e[i] = __builtin_amdgcn_exp2f((u[i] - ref) * p.c);
+      sum += e[i];
+    }
+    ts = G::sum(sum, tmp);
+  }
+};
+
+// From a row's finished sums: its losses and stats (rows, 5): m, sum e^{d / T}, sum e^d, the
+// teacher's maximum and sum. A row with nothing to learn (its logits were not read) has zeros.
+template <typename G, typename T>
+__device__ __forceinline__ void distill_store(const DistillParams& p, int64_t r, const T* x,
+                                              const Teacher<G>& t, bool hard, int64_t tgt,
+                                              const RowSums<kDual>& sum, float* tmp) {
+  const bool soft = t.ts != 0.f, empty = sum.m == kNegInf && sum.s == 0.f;
+  const float logs = logf(sum.s), logts = logf(t.ts);
+  float term = 0.f;
+#pragma unroll
+  for (int i = 0; i < Teacher<G>::N; ++i) {
+    if (t.e[i] == 0.f || !soft) continue;   // weight 0; NaN goes on
+    const float lw = (t.u[i] - t.ref) / p.temp - logts;
+    const float xi = t.id[i] >= 0 && t.id[i] < p.vocab ? (float)x[t.id[i]] : __builtin_nanf("");
+    const float lq = empty ? kNegInf : (xi - sum.m) / p.temp - logs;
+    term += t.e[i] / t.ts * (lw - lq);
+  }
+  const float kd = G::sum(term, tmp);
+  if (G::tid() != 0) return;
+  float* stats = p.stats + 5 * r;
+  p.kd[r] = soft ? p.temp * p.temp * kd : 0.f;
+  stats[0] = soft || hard ? sum.m : 0.f;
+  stats[1] = sum.s;
+  stats[2] = sum.s1;
+  stats[3] = t.ref;
+  stats[4] = t.ts;
+  if (p.nll) {
+    float v = 0.f;
+    if (hard) {
+      v = tgt < 0 || tgt >= p.vocab ? __builtin_nanf("")
+          : empty                   ? __builtin_inff()
+                                    : logf(sum.s1) - ((float)x[tgt] - sum.m);
+    }
+    p.nll[r] = v;
+  }
+}
+
+template <int NW, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_fwd_kernel(const DistillParams p) {
+  using G = Group<NW>;
   __shared__ float tmp[4];
-  const int tid = threadIdx.x;
-  for (int64_t r = blockIdx.x; r < p.rows; r += gridDim.x) {
+  for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
     const T* x = row_at<T>(p.logits, r, p.seqlen);
-    float u = kNegInf;
-    int64_t id = -1;
-    if (tid < p.k) {
-      id = teacher_id(p, r * p.k + tid);
-      if (id >= 0) u = teacher_logit(p, r * p.k + tid);
-      if (id >= p.vocab) u = __builtin_nanf("");
-    }
-    const float tm = block_max(u, tmp);
-    const float ref = tm == kNegInf ? 0.f : tm;
-    const float e = __builtin_amdgcn_exp2f((u - ref) * p.c);
-    const float ts = block_sum(e, tmp);
+    const Teacher<G> t(p, r, tmp);
     const int64_t tgt = p.targets ? p.targets[r] : 0;
-    const bool soft = ts != 0.f, hard = p.targets && tgt != p.ignore;
-    float* stats = p.stats + 5 * r;
-    if (!soft && !hard) {   // nothing to learn here: the logits are not read
-      if (tid == 0) {
-        p.kd[r] = 0.f;
-        if (p.nll) p.nll[r] = 0.f;
-        stats[0] = stats[1] = stats[2] = stats[3] = stats[4] = 0.f;
-      }
-      continue;
-    }
+    const bool hard = p.targets && tgt != p.ignore;
     RowSums<kDual> sum;
-    row_pass<kDual>(sum, x, p.vocab, p.c, p.c1);
-    sum.join_block(p.c, p.c1, tmp);
-    const bool empty = sum.m == kNegInf && sum.s == 0.f;
-    float term = 0.f;
-    if (e != 0.f) {   // w (log w - log q)
-      const float w = e / ts;
-      const float lw = (u - ref) / p.temp - logf(ts);
-      const float xi = id >= 0 && id < p.vocab ? (float)x[id] : __builtin_nanf("");
-      const float lq = empty ? kNegInf : (xi - sum.m) / p.temp - logf(sum.s);
-      term = w * (lw - lq);
+    if (t.ts != 0.f || hard) {
+      Best unused;
+      row_pass<G, U, false>(sum, unused, x, p.vocab, p.c, p.c1);
+      sum.template join<G>(p.c, p.c1, tmp);
     }
-    const float kd = block_sum(term, tmp);
-    if (tid == 0) {
-      p.kd[r] = soft ? p.temp * p.temp * kd : 0.f;
-      stats[0] = sum.m;
-      stats[1] = sum.s;
-      stats[2] = sum.s1;
-      stats[3] = ref;
-      stats[4] = ts;
-      if (p.nll) {
-        float v = 0.f;
-        if (hard) {
-          v = tgt < 0 || tgt >= p.vocab ? __builtin_nanf("")
-              : empty                   ? __builtin_inff()
-                                        : logf(sum.s1) - ((float)x[tgt] - sum.m);
-        }
-        p.nll[r] = v;
-      }
-    }
+    distill_store(p, r, x, t, hard, tgt, sum, tmp);
+  }
+}
+
+// Few long rows: a workgroup to each of a row's pieces, then one to join them.
+template <int U, typename T>
+__global__ void __launch_bounds__(kRowThreads) distill_piece_kernel(const DistillParams p) {
+  using G = Group<4>;
+  __shared__ float tmp[4];
+  const int64_t r = blockIdx.x / p.split;
+  const int g = (int)(blockIdx.x - r * p.split);
+  const int lo = g * p.share, n = min(p.share, p.vocab - lo);
+  if (!p.targets || p.targets[r] == p.ignore) {   // without a teacher token either: not read
+    bool any = false;
+    for (int j = threadIdx.x; j < p.k; j += kRowThreads) any = any || teacher_id(p, r * p.k + j) >= 0;
+    if (!__syncthreads_or(any)) return;
+  }
+  RowSums<kDual> sum;
+  Best unused;
+  row_pass<G, U, false>(sum, unused, row_at<T>(p.logits, r, p.seqlen) + lo, n, p.c, p.c1);
+  sum.template join<G>(p.c, p.c1, tmp);
+  if (threadIdx.x == 0) {
+    float* out = p.part + 3 * (r * p.split + g);
+    out[0] = sum.m;
+    out[1] = sum.s;
+    out[2] = sum.s1;
   }
 }
 
 template <typename T>
+__global__ void __launch_bounds__(kRowThreads) distill_join_kernel(const DistillParams p) {
+  using G = Group<4>;
+  __shared__ float tmp[4];
+  const int64_t r = blockIdx.x;
+  const Teacher<G> t(p, r, tmp);
+  const int64_t tgt = p.targets ? p.targets[r] : 0;
+  const bool hard = p.targets && tgt != p.ignore;
+  RowSums<kDual> sum;
+  if (t.ts != 0.f || hard) {
+    if ((int)threadIdx.x < p.split) {
+      const float* in = p.part + 3 * (r * p.split + threadIdx.x);
+      sum.m = in[0];
+      sum.s = in[1];
+      sum.s1 = in[2];
+    }
+    sum.template join<G>(p.c, p.c1, tmp);
+  }
+  distill_store(p, r, row_at<T>(p.logits, r, p.seqlen), t, hard, tgt, sum, tmp);
+}
+
+template <int NW, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillParams p) {
-  constexpr int CHUNK = kRowThreads * kBwdPieces * Piece<T>::N;
-  __shared__ int ids[kTeacherMax];
-  __shared__ float wt[kTeacherMax];
-  const int tid = threadIdx.x;
-  for (int64_t w = blockIdx.x; w < p.rows * p.chunks; w += gridDim.x) {
+  using G = Group<NW>;
+  __shared__ int sids[G::ROWS][kTeacherMax];
+  __shared__ float sweight[G::ROWS][kTeacherMax];
+  int* ids = sids[G::slot()];
+  float* wt = sweight[G::slot()];
+  const int64_t work = p.rows * p.chunks;
+  for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
     const int64_t r = w / p.chunks;
-    const int lo = (int)(w - r * p.chunks) * CHUNK, hi = min(lo + CHUNK, p.vocab);
+    const int lo = (int)(w - r * p.chunks) * kChunk<G, T>, hi = min(lo + kChunk<G, T>, p.vocab);
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
     const float* stats = p.stats + 5 * r;
@@ -434,7 +859,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
     const int64_t tgt = p.targets ? p.targets[r] : p.ignore;
     const bool soft = p.dkd && ts != 0.f, hard = p.dnll && tgt != p.ignore;
     if (s == 0.f || (!soft && !hard)) {   // no loss, or no distribution
-      for (int i = lo + tid; i < hi; i += kRowThreads) dx[i] = (T)0.f;
+      chunk_zero<G>(dx, lo, hi);
       continue;
     }
     const float a = soft ? p.dkd[r] * p.temp : 0.f, as = ts != ts ? ts : a / s;
@@ -448,35 +873,36 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
       if (hard) o += bs * __builtin_amdgcn_exp2f(d * p.c1);
       return o;
     };
-    chunk_map(x, dx, lo, hi, f);
+    chunk_map<G>(x, dx, lo, hi, f);
     const int k = soft ? p.k : 0;
-    if (tid < k) {
-      const int64_t id = teacher_id(p, r * k + tid);
+    for (int j = G::tid(); j < k; j += G::NT) {
+      const int64_t id = teacher_id(p, r * k + j);
       const bool there = id >= 0 && id < p.vocab;
-      ids[tid] = there ? (int)id : -1;
-      wt[tid] = there ? a * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + tid) - ref) * p.c) / ts : 0.f;
+      ids[j] = there ? (int)id : -1;
+      wt[j] = there ? a * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + j) - ref) * p.c) / ts : 0.f;
     }
-    __syncthreads();
+    G::sync();
     // entries that the teacher's tokens or the true one take from, whole: a token named twice
     // is written by its first mention
-    if (tid < k && ids[tid] >= lo && ids[tid] < hi) {
-      const int i = ids[tid];
+    for (int j = G::tid(); j < k; j += G::NT) {
+      const int i = ids[j];
+      if (i < lo || i >= hi) continue;
       bool first = true;
       float take = 0.f;
-      for (int j = 0; j < k; ++j) {
-        if (ids[j] == i) {
-          first = first && j >= tid;
-          take += wt[j];
+      for (int l = 0; l < k; ++l) {
+        if (ids[l] == i) {
+          first = first && l >= j;
+          take += wt[l];
         }
       }
       if (first) dx[i] = (T)(f((float)x[i]) - take - (hard && i == tgt ? b : 0.f));
     }
-    if (tid == 0 && hard && tgt >= lo && tgt < hi) {
+    if (G::tid() == 0 && hard && tgt >= lo && tgt < hi) {
       bool alone = true;
-      for (int j = 0; j < k; ++j) alone = alone && ids[j] != tgt;
+      for (int l = 0; l < k; ++l) alone = alone && ids[l] != tgt;
       if (alone) dx[tgt] = (T)(f((float)x[tgt]) - b);
     }
-    __syncthreads();
+    G::sync();
   }
 }
 
@@ -504,8 +930,23 @@ static int32_t check_logits(const A* a, const char* who) {
   return 0;
 }
 static int vocab_chunks(int vocab, int dtype) {
-  const int chunk = kRowThreads * kBwdPieces * (dtype == M3S_DTYPE_BF16 ? 8 : 4);
+  const bool b = dtype == M3S_DTYPE_BF16;
+  const int chunk = vocab <= kWaveVocab ? (b ? kChunk<Group<1>, bf16> : kChunk<Group<1>, float>)
+                                        : (b ? kChunk<Group<4>, bf16> : kChunk<Group<4>, float>);
   return (vocab + chunk - 1) / chunk;
+}
+// Logits to a piece: whole 16-byte pieces.
+static int row_share(int vocab, int split) { return ((vocab + split - 1) / split + 7) / 8 * 8; }
+// Pieces to a row: where the rows alone leave most of the 256 CUs idle, enough for two workgroups
+// to each, of at least kPieceMin logits; with alternatives the pieces' best together stay within
+// what the joining workgroup ranks. 1: whole rows.
+constexpr int kPieceMin = 4096, kSplitMax = 64;
+static int row_split(int64_t rows, int vocab, int top) {
+  int64_t split = std::min<int64_t>({512 / std::max<int64_t>(rows, 1), vocab / kPieceMin, kSplitMax});
+  if (top) split = std::min<int64_t>(split, 1024 / top);
+  if (split < 2) return 1;
+  const int share = row_share(vocab, (int)split);
+  return (vocab + share - 1) / share;
 }
 
 static LogprobParams logprob_params(const m3s_logprob_args* a) {
@@ -527,6 +968,7 @@ static LogprobParams logprob_params(const m3s_logprob_args* a) {
   p.vocab = a->vocab;
   p.top = a->top;
   p.chunks = vocab_chunks(a->vocab, a->dtype);
+  p.part = static_cast<float*>(a->workspace);
   p.temp = a->temperature;
   p.inv_t = (float)(1.0 / a->temperature);
   p.c = (float)(1.4426950408889634 / a->temperature);
@@ -551,6 +993,7 @@ static DistillParams distill_params(const m3s_distill_args* a) {
   p.vocab = a->vocab;
   p.k = a->teacher_k;
   p.chunks = vocab_chunks(a->vocab, a->dtype);
+  p.part = static_cast<float*>(a->workspace);
   p.id_bytes = a->id_bytes;
   p.teacher_bf16 = a->teacher_dtype == M3S_DTYPE_BF16;
   p.temp = a->temperature;
@@ -561,15 +1004,84 @@ static DistillParams distill_params(const m3s_distill_args* a) {
 }
 
 template <typename P>
-static void launch_rows(void (*fb)(P), void (*ff)(P), const P& p, int dtype, int64_t blocks, hipStream_t s) {
-  const dim3 grid((unsigned)std::min(kRowGrid, blocks));
-  if (dtype == M3S_DTYPE_BF16) hipLaunchKernelGGL(fb, grid, dim3(kRowThreads), 0, s, p);
-  else hipLaunchKernelGGL(ff, grid, dim3(kRowThreads), 0, s, p);
+static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t s) {
+  hipLaunchKernelGGL(f, dim3((unsigned)std::min(kRowGrid, blocks)), dim3(kRowThreads), 0, s, p);
+}
+// f(group, U): the waves to a row and the 16-byte pieces of a batch, by the row's length
+template <typename T, typename F>
+static void with_group(int vocab, F&& f) {
+  constexpr int N = Piece<T>::N;
+  if (vocab > kWaveVocab) f(Group<4>(), std::integral_constant<int, 16 / N>());
+  else if (vocab > 64 * N) f(Group<1>(), std::integral_constant<int, 16 / N>());
+  else f(Group<1>(), std::integral_constant<int, 1>());
+}
+
+template <bool TOP, typename T>
+static void launch_logprob_fwd(const LogprobParams& p, hipStream_t s) {
+  if (p.split > 1) {
+    launch_kernel(logprob_piece_kernel<TOP, 16 / Piece<T>::N, T>, p.rows * p.split, p, s);
+    launch_kernel(logprob_join_kernel<TOP, T>, p.rows, p, s);
+    return;
+  }
+  with_group<T>(p.vocab, [&](auto g, auto u) {
+    constexpr int NW = decltype(g)::NT / 64;
+    launch_kernel(logprob_fwd_kernel<TOP, NW, decltype(u)::value, T>, (p.rows + 4 / NW - 1) / (4 / NW), p, s);
+  });
+}
+template <typename T>
+static void launch_distill_fwd(const DistillParams& p, hipStream_t s) {
+  if (p.split > 1) {
+    launch_kernel(distill_piece_kernel<16 / Piece<T>::N, T>, p.rows * p.split, p, s);
+    launch_kernel(distill_join_kernel<T>, p.rows, p, s);
+    return;
+  }
+  with_group<T>(p.vocab, [&](auto g, auto u) {
+    constexpr int NW = decltype(g)::NT / 64;
+    launch_kernel(distill_fwd_kernel<NW, decltype(u)::value, T>, (p.rows + 4 / NW - 1) / (4 / NW), p, s);
+  });
+}
+template <typename P>
+static void launch_bwd(void (*wave)(P), void (*block)(P), const P& p, hipStream_t s) {
+  const int64_t work = p.rows * p.chunks;
+  if (p.vocab <= kWaveVocab) launch_kernel(wave, (work + 3) / 4, p, s);
+  else launch_kernel(block, work, p, s);
+}
+
+static int64_t logprob_scratch(int64_t rows, int vocab, int top) {
+  const int split = row_split(rows, vocab, top);
+  return split == 1 ? 0 : rows * split * (3 + 2 * top) * 4;
+}
+static int64_t distill_scratch(int64_t rows, int vocab) {
+  const int split = row_split(rows, vocab, 0);
+  return split == 1 ? 0 : rows * split * 3 * 4;
+}
+// Rows are cut where the call brings the scratch for it, and stay whole (the same results to
+// rounding, later) where it does not.
+template <typename P>
+static void set_split(P& p, int64_t need, int64_t given, int top) {
+  p.split = need > 0 && p.part && given >= need ? row_split(p.rows, p.vocab, top) : 1;
+  p.share = row_share(p.vocab, p.split);
+}
+template <typename A>
+static int32_t check_scratch(const A* a, const char* who) {
+  M3S_REQUIRE(a->workspace_bytes >= 0 && (uintptr_t)a->workspace % 16 == 0,
+              "%s: workspace must be 16-byte aligned", who);
+  return 0;
 }
 
 }  // namespace m3s
 
 using namespace m3s;
+
+extern "C" int64_t m3s_logprob_workspace_bytes(int64_t rows, int32_t vocab, int32_t top) {
+  if (rows < 0 || rows >= (1ll << 31) || vocab <= 0 || vocab >= (1 << 30) || top < 0 || top > kTopMax) return -1;
+  return logprob_scratch(rows, vocab, top);
+}
+
+extern "C" int64_t m3s_distill_workspace_bytes(int64_t rows, int32_t vocab) {
+  if (rows < 0 || rows >= (1ll << 31) || vocab <= 0 || vocab >= (1 << 30)) return -1;
+  return distill_scratch(rows, vocab);
+}
 
 extern "C" int32_t m3s_logprob_fwd(const m3s_logprob_args* a, void* stream) {
   clear_error();
@@ -580,9 +1092,13 @@ extern "C" int32_t m3s_logprob_fwd(const m3s_logprob_args* a, void* stream) {
   if (int32_t rc = check_logits(a, "m3s_logprob_fwd")) return rc;
   M3S_REQUIRE(a->entropy && a->stats && (!a->targets || a->logp) && (!a->top || (a->top_logp && a->top_ids)),
               "m3s_logprob_fwd: NULL pointer");
-  const LogprobParams p = logprob_params(a);
-  launch_rows(logprob_fwd_kernel<bf16>, logprob_fwd_kernel<float>, p, a->dtype, p.rows,
-              static_cast<hipStream_t>(stream));
+  if (int32_t rc = check_scratch(a, "m3s_logprob_fwd")) return rc;
+  LogprobParams p = logprob_params(a);
+  set_split(p, logprob_scratch(p.rows, p.vocab, p.top), a->workspace_bytes, p.top);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool b = a->dtype == M3S_DTYPE_BF16;
+  if (p.top) b ? launch_logprob_fwd<true, bf16>(p, s) : launch_logprob_fwd<true, float>(p, s);
+  else b ? launch_logprob_fwd<false, bf16>(p, s) : launch_logprob_fwd<false, float>(p, s);
   return launch_status("m3s_logprob_fwd");
 }
 
@@ -598,8 +1114,9 @@ extern "C" int32_t m3s_logprob_bwd(const m3s_logprob_args* a, void* stream) {
                   (!a->dtop_logp || !a->top || a->top_ids),
               "m3s_logprob_bwd: NULL or misaligned pointer");
   const LogprobParams p = logprob_params(a);
-  launch_rows(logprob_bwd_kernel<bf16>, logprob_bwd_kernel<float>, p, a->dtype, p.rows * p.chunks,
-              static_cast<hipStream_t>(stream));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->dtype == M3S_DTYPE_BF16) launch_bwd(logprob_bwd_kernel<1, bf16>, logprob_bwd_kernel<4, bf16>, p, s);
+  else launch_bwd(logprob_bwd_kernel<1, float>, logprob_bwd_kernel<4, float>, p, s);
   return launch_status("m3s_logprob_bwd");
 }
 
@@ -621,9 +1138,11 @@ extern "C" int32_t m3s_distill_fwd(const m3s_distill_args* a, void* stream) {
   if (int32_t rc = check_distill(a, "m3s_distill_fwd")) return rc;
   if (a->batch == 0 || a->seqlen == 0) return 0;
   M3S_REQUIRE(a->kd && (a->targets == nullptr) == (a->nll == nullptr), "m3s_distill_fwd: NULL pointer");
-  const DistillParams p = distill_params(a);
-  launch_rows(distill_fwd_kernel<bf16>, distill_fwd_kernel<float>, p, a->dtype, p.rows,
-              static_cast<hipStream_t>(stream));
+  if (int32_t rc = check_scratch(a, "m3s_distill_fwd")) return rc;
+  DistillParams p = distill_params(a);
+  set_split(p, distill_scratch(p.rows, p.vocab), a->workspace_bytes, 0);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  a->dtype == M3S_DTYPE_BF16 ? launch_distill_fwd<bf16>(p, s) : launch_distill_fwd<float>(p, s);
   return launch_status("m3s_distill_fwd");
 }
 
@@ -635,7 +1154,8 @@ extern "C" int32_t m3s_distill_bwd(const m3s_distill_args* a, void* stream) {
   M3S_REQUIRE(a->dlogits && (uintptr_t)a->dlogits % es == 0 && (!a->dnll || a->targets),
               "m3s_distill_bwd: NULL or misaligned pointer");
   const DistillParams p = distill_params(a);
-  launch_rows(distill_bwd_kernel<bf16>, distill_bwd_kernel<float>, p, a->dtype, p.rows * p.chunks,
-              static_cast<hipStream_t>(stream));
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a->dtype == M3S_DTYPE_BF16) launch_bwd(distill_bwd_kernel<1, bf16>, distill_bwd_kernel<4, bf16>, p, s);
+  else launch_bwd(distill_bwd_kernel<1, float>, distill_bwd_kernel<4, float>, p, s);
   return launch_status("m3s_distill_bwd");
 }

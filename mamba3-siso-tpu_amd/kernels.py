@@ -1417,7 +1417,7 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
     dev = _device_of(tokens, dy)
     tokens, dy = tokens.contiguous(), dy.contiguous()
     lib = _lib.load()
-    nbytes = lib.m3s_embed_bwd_workspace_bytes(a.tokens, a.vocab, a.width)
+    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", a.tokens, a.vocab, a.width)
     if nbytes < 0:
         raise ValueError(f"embedding: bad sizes (tokens {a.tokens}, vocab {a.vocab}, width {a.width})")
     dtable = empty(a.vocab, a.width, device=dev, dtype=dy.dtype)
@@ -1478,6 +1478,16 @@ def _row_targets(targets: Optional[Tensor], shape, what: str) -> Optional[Tensor
     return _row_values(targets, shape, torch.int64, f"{what}: targets")
 
 
+def _row_scratch(a, dev, entry: str, *sizes: int) -> Optional[Tensor]:
+    """The scratch for cutting few long rows into pieces, set in ``a``; None where none is cut."""
+    nbytes = _lib.scratch_bytes(entry, *sizes)
+    if nbytes <= 0:
+        return None
+    ws = empty(nbytes, device=dev, dtype=torch.uint8)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    return ws
+
+
 def _check_temperature(temperature: float, what: str) -> float:
     temperature = float(temperature)
     if not 1e-30 <= temperature <= 1e30:
@@ -1518,6 +1528,7 @@ def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int =
         top_logp = empty(*shape, top, device=dev, dtype=torch.float32)
         top_ids = empty(*shape, top, device=dev, dtype=torch.int64)
         a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
+    ws = _row_scratch(a, dev, "m3s_logprob_workspace_bytes", shape.numel(), a.vocab, top)  # noqa: F841
     _lib.launch(_lib.load().m3s_logprob_fwd, a, dev, "m3s_logprob_fwd")
     return logp, entropy, top_logp, top_ids, stats
 
@@ -1597,6 +1608,7 @@ def distill_forward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
     if targets is not None:
         nll = empty(shape, device=dev, dtype=torch.float32)
         a.nll = nll.data_ptr()
+    ws = _row_scratch(a, dev, "m3s_distill_workspace_bytes", shape.numel(), a.vocab)  # noqa: F841
     _lib.launch(_lib.load().m3s_distill_fwd, a, dev, "m3s_distill_fwd")
     return kd, nll, stats
 

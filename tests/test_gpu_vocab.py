@@ -192,6 +192,24 @@ def test_logprobs_of_hard_rows(m3, dev, dtype, kind, vocab):
         check_logprob(m3, dev, x, targets, top, 1.0, ("l", "lht"))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(600, 9001), (130, 20003), (2100, 700), (10, 260)])
+def test_whole_rows_of_hard_kinds(m3, dev, dtype, rows, vocab):
+    """Enough rows that none is cut: masks, ties, flat rows, empty ones and ordinary ones together,
+    and rows whose best logits all lie at the places of few threads."""
+    gen = torch.Generator().manual_seed(rows)
+    kinds = ("model", "masked", "flat", "ties", "wide")
+    x = torch.cat([make_logits((rows // 5, vocab), dtype, gen, k) for k in kinds])
+    x[3], x[5] = -INF, torch.finfo(dtype).min
+    place = torch.arange(vocab) // (4 if dtype == torch.float32 else 8) % 256
+    x[7] = (10 * (place < 40) + torch.rand(vocab, generator=gen)).to(dtype)
+    x[8] = torch.where(place == 3, 5.0, -INF)
+    targets = torch.randint(0, vocab, (len(x),), generator=gen)
+    targets[::11] = -100
+    for top in (1, 20, 64):
+        check_logprob(m3, dev, x, targets, top, 1.0, ("lht",) if top == 20 else ())
+
+
 def test_one_thread_holds_the_best(m3, dev):
     """The best tokens all at one stride, equal or falling, so that one part of the workgroup has
     them all."""
