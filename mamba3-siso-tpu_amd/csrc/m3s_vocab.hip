@@ -31,7 +31,12 @@ namespace m3s {
 constexpr int kRowThreads = 256;
 constexpr int kTopMax = 64;        // alternatives of a row
 constexpr int kTeacherMax = 256;   // teacher tokens of a row
-constexpr int kWaveVocab = 1024;   // rows up to this long go to a single wave
+// Rows up to kPartVocab long go to 16 lanes each, up to kWaveVocab to a wave, longer ones to a
+// workgroup.
+constexpr int kPartVocab = 512, kWaveVocab = 1024;
+constexpr int kPartTop = 8;         // alternatives that 16 lanes pick, of rows up to kPartPick long
+constexpr int kPartPick = 256;
+constexpr int kPartTeacher = 64;    // teacher tokens of a row of 16 lanes
 constexpr float kNegInf = -__builtin_inff();
 
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
@@ -64,27 +69,42 @@ template <> struct Piece<bf16> {
   }
 };
 
-// ---- a row's group of waves -------------------------------------------------------------------
-// NW = 4: the workgroup shares a row. NW = 1: each wave has its own, and nothing waits for others.
-template <int NW>
+// ---- a row's group of lanes -------------------------------------------------------------------
+// NT threads share a row: the workgroup, a wave, or 16 lanes (a row of the DPP moves) of a wave,
+// which then handles four rows at once: what is done once a row (sums over lanes, logarithms,
+// divisions) is what a short row costs.
+template <int NT_>
 struct Group {
-  static constexpr int NT = 64 * NW;        // threads to a row
-  static constexpr int ROWS = 4 / NW;       // rows to a workgroup
-  static __device__ __forceinline__ int tid() { return NW == 1 ? lane_id() : (int)threadIdx.x; }
-  static __device__ __forceinline__ int slot() { return NW == 1 ? (int)threadIdx.x >> 6 : 0; }
+  static constexpr int NT = NT_;
+  static constexpr int NW = NT / 64;                    // waves; 0 for a part of one
+  static constexpr int ROWS = kRowThreads / NT;         // rows to a workgroup
+  static constexpr int TMP = NW == 4 ? 8 : 1;           // floats that the reductions need in LDS
+  static __device__ __forceinline__ int tid() { return (int)threadIdx.x & (NT - 1); }
+  // the group's place in the workgroup: wave-uniform for a wave, so that a row's scalars are scalar loads
+  static __device__ __forceinline__ int slot() {
+    if constexpr (NW == 4) return 0;
+    const int s = (int)threadIdx.x / NT;
+    return NW == 1 ? __builtin_amdgcn_readfirstlane(s) : s;
+  }
   // what the group wrote to LDS or memory before is seen by it after
   static __device__ __forceinline__ void sync() {
-    if constexpr (NW == 1) {
+    if constexpr (NW == 4) {
+      __syncthreads();
+    } else {
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       __builtin_amdgcn_wave_barrier();
-    } else {
-      __syncthreads();
     }
   }
-  // Reductions: the same value to every thread; `tmp` holds four floats and is free afterwards.
+  // Reductions: the same value to every thread; `tmp` (TMP floats) is free afterwards.
   static __device__ __forceinline__ float max(float v, float* tmp) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    v = fmaxf(v, dpp_mov<kDppQuadSwap1>(v));
+    v = fmaxf(v, dpp_mov<kDppQuadSwap2>(v));
+    v = fmaxf(v, dpp_mov<kDppHalfMirror>(v));
+    v = fmaxf(v, dpp_mov<kDppRowMirror>(v));
+    if constexpr (NW == 0) return v;
+    const int i = __builtin_bit_cast(int, v);
+    const auto row = [&](int l) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(i, l)); };
+    v = fmaxf(fmaxf(row(0), row(16)), fmaxf(row(32), row(48)));
     if constexpr (NW == 4) {
       if (lane_id() == 0) tmp[threadIdx.x >> 6] = v;
       __syncthreads();
@@ -93,7 +113,27 @@ struct Group {
     }
     return v;
   }
+  static __device__ __forceinline__ void sum2(float& a, float& b, float* tmp) {
+    if constexpr (NW == 0) {
+      a = group_sum<16>(a);
+      b = group_sum<16>(b);
+      return;
+    }
+    a = wave_total(a);
+    b = wave_total(b);
+    if constexpr (NW == 4) {
+      if (lane_id() == 0) {
+        tmp[threadIdx.x >> 6] = a;
+        tmp[4 + (threadIdx.x >> 6)] = b;
+      }
+      __syncthreads();
+      a = (tmp[0] + tmp[1]) + (tmp[2] + tmp[3]);
+      b = (tmp[4] + tmp[5]) + (tmp[6] + tmp[7]);
+      __syncthreads();
+    }
+  }
   static __device__ __forceinline__ float sum(float v, float* tmp) {
+    if constexpr (NW == 0) return group_sum<16>(v);
     v = wave_total(v);
     if constexpr (NW == 4) {
       if (lane_id() == 0) tmp[threadIdx.x >> 6] = v;
@@ -108,7 +148,7 @@ struct Group {
 // ---- running sums of a row ------------------------------------------------------------------
 // s = sum 2^{c (x - m)}, t = sum of the same times (x - m), s1 = sum 2^{c1 (x - m)}. A row of -inf
 // keeps m = -inf and zeros; a NaN or +inf makes the sums NaN (fmaxf drops the NaN, s does not).
-enum { kEntropy = 1, kDual = 2 };
+enum { kSingle = 0, kEntropy = 1, kDual = 2 };
 // 2^{a b} with the product's rounding made good: a factor on a whole sum, so its error does not
 // average out as the terms' do (one row of 131072 in pieces: log-probability off by 1e-7, not 5e-7).
 __device__ __forceinline__ float exp2_product(float a, float b) {
@@ -147,11 +187,16 @@ struct RowSums {
   template <typename G>
   __device__ __forceinline__ void join(float c, float c1, float* tmp) {
     raise(G::max(m, tmp), c, c1);
-    s = G::sum(s, tmp);
-    if constexpr (MODE == kEntropy) t = G::sum(t, tmp);
-    if constexpr (MODE == kDual) s1 = G::sum(s1, tmp);
+    if constexpr (MODE == kEntropy) G::sum2(s, t, tmp);
+    else if constexpr (MODE == kDual) G::sum2(s, s1, tmp);
+    else s = G::sum(s, tmp);
   }
 };
+
+template <int ctrl>
+__device__ __forceinline__ int dpp_int(int v) {
+  return __builtin_amdgcn_mov_dpp(v, ctrl, 0xF, 0xF, false);
+}
 
 // Where a thread's best logits lie: the largest maxima of its batches (U pieces of 16 bytes), the
 // first two with their batch, so that the alternatives are found without reading the row again.
@@ -220,9 +265,16 @@ __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* 
   }
 }
 
+// a / b for a >= 0 and b > 0, without the 64-bit division's hundred instructions where it can be.
+__device__ __forceinline__ int64_t quotient(int64_t a, int b) {
+  if (a < b) return 0;
+  if (a >> 32 == 0) return (uint32_t)a / (uint32_t)b;
+  return a / b;
+}
+
 template <typename T>
 __device__ __forceinline__ const T* row_at(const m3s_blx& b, int64_t r, int seqlen) {
-  const int64_t i = r / seqlen;
+  const int64_t i = quotient(r, seqlen);
   return static_cast<const T*>(b.ptr) + i * b.stride_b + (r - i * seqlen) * b.stride_t;
 }
 
@@ -262,7 +314,7 @@ struct PickSpace {
   int i[CAP];
   int count;
   int itmp[4];
-  float tmp[4];
+  float tmp[8];
 };
 
 // Appends this thread's logit to the candidates if `hit`; a full list only counts.
@@ -414,6 +466,37 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, cons
   G::sync();   // the space is free again
 }
 
+// The same by 16 lanes that hold the row's at most kPartPick logits, one round for each of few.
+template <typename G, typename T, typename OUT>
+__device__ __forceinline__ void pick_few(const T* __restrict__ x, int n, int k, OUT&& out) {
+  constexpr int N = Piece<T>::N, U = kPartPick / (G::NT * N), LEN = U * N;
+  using R = Rows<G, U, T>;
+  const float gone = __builtin_nanf("");   // no logit, or one that is out already
+  const int tail = n / N * N + G::tid();
+  float v[LEN + 1];
+  R::load(x, n, 0, v);
+#pragma unroll
+  for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) < n / N * N ? v[i] : gone;
+  v[LEN] = tail < n ? (float)x[tail] : gone;
+  for (int j = 0; j < k; ++j) {
+    float top = v[LEN];
+#pragma unroll
+    for (int i = 0; i < LEN; ++i) top = fmaxf(top, v[i]);
+    top = G::max(top, nullptr);
+    int at = v[LEN] == top ? tail : 0x7fffffff;
+#pragma unroll
+    for (int i = LEN - 1; i >= 0; --i) at = v[i] == top ? R::place(0, i) : at;
+    at = min(at, dpp_int<kDppQuadSwap1>(at));
+    at = min(at, dpp_int<kDppQuadSwap2>(at));
+    at = min(at, dpp_int<kDppHalfMirror>(at));
+    at = min(at, dpp_int<kDppRowMirror>(at));
+#pragma unroll
+    for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) == at ? gone : v[i];
+    v[LEN] = tail == at ? gone : v[LEN];
+    if (G::tid() == j) out(j, top, at);
+  }
+}
+
 // ---- log-probabilities ----------------------------------------------------------------------
 struct LogprobParams {
   m3s_blx logits;
@@ -453,18 +536,18 @@ __device__ __forceinline__ void logprob_skip(const LogprobParams& p, int64_t r) 
 }
 
 struct LogprobRow {   // from finished sums
-  float m, logs, temp;
+  float m, logs, inv_t;
   bool empty;
-  __device__ LogprobRow(const RowSums<kEntropy>& s, float temp_)
-      : m(s.m), logs(logf(s.s)), temp(temp_), empty(s.m == kNegInf && s.s == 0.f) {}
-  __device__ float operator()(float v) const { return empty ? kNegInf : (v - m) / temp - logs; }
+  __device__ LogprobRow(const RowSums<kEntropy>& s, float inv_t_)
+      : m(s.m), logs(logf(s.s)), inv_t(inv_t_), empty(s.m == kNegInf && s.s == 0.f) {}
+  __device__ float operator()(float v) const { return empty ? kNegInf : (v - m) * inv_t - logs; }
 };
 
 template <typename G, typename T>
 __device__ __forceinline__ void logprob_store(const LogprobParams& p, int64_t r, int64_t tgt, const T* x,
                                               const RowSums<kEntropy>& sum, const LogprobRow& logp) {
   if (G::tid() != 0) return;
-  const float h = logp.empty ? 0.f : logp.logs - sum.t / (p.temp * sum.s);
+  const float h = logp.empty ? 0.f : logp.logs - sum.t * p.inv_t / sum.s;
   p.entropy[r] = h;
   p.stats[3 * r] = sum.m;
   p.stats[3 * r + 1] = sum.s;
@@ -481,11 +564,12 @@ __device__ __forceinline__ void logprob_unordered(const LogprobParams& p, int64_
   }
 }
 
-template <bool TOP, int NW, int U, typename T>
+template <bool TOP, int NT, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobParams p) {
-  using G = Group<NW>;
-  __shared__ float tmp[4];
-  __shared__ PickSpace<NW> space[TOP ? G::ROWS : 1];
+  using G = Group<NT>;
+  constexpr bool PICK = TOP && NT > 16;
+  __shared__ float tmp[G::TMP];
+  __shared__ PickSpace<NT == 256 ? 4 : 1> space[PICK ? G::ROWS : 1];
   for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
     const int64_t tgt = p.targets ? p.targets[r] : 0;
     if (p.targets && tgt == p.ignore) {
@@ -495,19 +579,21 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     RowSums<kEntropy> sum;
     Best best;
-    row_pass<G, U, TOP>(sum, best, x, p.vocab, p.c, 0.f);
+    row_pass<G, U, PICK>(sum, best, x, p.vocab, p.c, 0.f);
     sum.template join<G>(p.c, 0.f, tmp);
-    const LogprobRow logp(sum, p.temp);
+    const LogprobRow logp(sum, p.inv_t);
     logprob_store<G>(p, r, tgt, x, sum, logp);
     if constexpr (TOP) {
       if (sum.s != sum.s) {
         logprob_unordered<G>(p, r);
         continue;
       }
-      pick<G, U>(x, p.vocab, p.top, best, space[G::slot()], [&](int j, float v, int i) {
+      const auto out = [&](int j, float v, int i) {
         p.top_logp[r * p.top + j] = logp(v);
         p.top_ids[r * p.top + j] = i;
-      });
+      };
+      if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, best, space[G::slot()], out);
+      else pick_few<G>(x, p.vocab, p.top, out);
     }
   }
 }
@@ -515,8 +601,8 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
 // Few long rows: a workgroup to each of a row's `split` pieces ...
 template <bool TOP, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_piece_kernel(const LogprobParams p) {
-  using G = Group<4>;
-  __shared__ float tmp[4];
+  using G = Group<256>;
+  __shared__ float tmp[G::TMP];
   __shared__ PickSpace<4> space[1];
   const int64_t r = blockIdx.x / p.split;
   const int g = (int)(blockIdx.x - r * p.split);
@@ -554,8 +640,8 @@ __global__ void __launch_bounds__(kRowThreads) logprob_piece_kernel(const Logpro
 // equal values are in the order of their index here too.
 template <bool TOP, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const LogprobParams p) {
-  using G = Group<4>;
-  __shared__ float tmp[4];
+  using G = Group<256>;
+  __shared__ float tmp[G::TMP];
   __shared__ PickSpace<4> space[1];
   const int64_t r = blockIdx.x;
   const int64_t tgt = p.targets ? p.targets[r] : 0;
@@ -571,7 +657,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
     sum.t = part.sums[3 * threadIdx.x + 2];
   }
   sum.template join<G>(p.c, 0.f, tmp);
-  const LogprobRow logp(sum, p.temp);
+  const LogprobRow logp(sum, p.inv_t);
   logprob_store<G>(p, r, tgt, row_at<T>(p.logits, r, p.seqlen), sum, logp);
   if constexpr (TOP) {
     if (sum.s != sum.s) {
@@ -633,16 +719,16 @@ __device__ __forceinline__ void chunk_zero(T* __restrict__ dx, int lo, int hi) {
   if (at < hi) dx[at] = (T)0.f;
 }
 
-template <int NW, typename T>
+template <int NT, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_bwd_kernel(const LogprobParams p) {
-  using G = Group<NW>;
-  __shared__ int sids[G::ROWS][kTopMax];
-  __shared__ float sgrad[G::ROWS][kTopMax];
+  using G = Group<NT>;
+  __shared__ int sids[G::ROWS][kTopMax + 1];   // odd: the groups of a wave on different banks
+  __shared__ float sgrad[G::ROWS][kTopMax + 1];
   int* ids = sids[G::slot()];
   float* gtop = sgrad[G::slot()];
   const int64_t work = p.rows * p.chunks;
   for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
-    const int64_t r = w / p.chunks;
+    const int64_t r = quotient(w, p.chunks);
     const int lo = (int)(w - r * p.chunks) * kChunk<G, T>, hi = min(lo + kChunk<G, T>, p.vocab);
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
@@ -707,12 +793,13 @@ __device__ __forceinline__ float teacher_logit(const DistillParams& p, int64_t a
   return p.teacher_bf16 ? (float)static_cast<const bf16*>(p.teacher)[at] : static_cast<const float*>(p.teacher)[at];
 }
 
-// A row's teacher tokens, kTeacherMax / NT to a thread: ids (-1: none), logits, and e^{(u - ref) / T}.
+// A row's teacher tokens, kTeacherMax / NT to a thread: ids (-1: none, or outside the vocabulary),
+// logits, and e^{(u - ref) / T}.
 // ts = 0 says that there is no entry, NaN that one is a NaN or an id outside the vocabulary.
 template <typename G>
 struct Teacher {
-  static constexpr int N = kTeacherMax / G::NT;
-  int64_t id[N];
+  static constexpr int N = (G::NT == 16 ? kPartTeacher : kTeacherMax) / G::NT;
+  int id[N];
   float u[N], e[N], ref, ts;
   __device__ __forceinline__ Teacher(const DistillParams& p, int64_t r, float* tmp) {
     float top = kNegInf, sum = 0.f;
@@ -722,9 +809,9 @@ struct Teacher {
       id[i] = -1;
       u[i] = kNegInf;
       if (at < p.k) {
-        id[i] = teacher_id(p, r * p.k + at);
-        if (id[i] >= 0) u[i] = teacher_logit(p, r * p.k + at);
-        if (id[i] >= p.vocab) u[i] = __builtin_nanf("");
+        const int64_t v = teacher_id(p, r * p.k + at);
+        if (v >= 0) u[i] = v < p.vocab ? teacher_logit(p, r * p.k + at) : __builtin_nanf("");
+        if (v >= 0 && v < p.vocab) id[i] = (int)v;
       }
       top = fmaxf(top, u[i]);
     }
@@ -741,20 +828,20 @@ struct Teacher {
 
 // From a row's finished sums: its losses and stats (rows, 5): m, sum e^{d / T}, sum e^d, the
 // teacher's maximum and sum. A row with nothing to learn (its logits were not read) has zeros.
-template <typename G, typename T>
+template <typename G, int MODE, typename T>
 __device__ __forceinline__ void distill_store(const DistillParams& p, int64_t r, const T* x,
                                               const Teacher<G>& t, bool hard, int64_t tgt,
-                                              const RowSums<kDual>& sum, float* tmp) {
+                                              const RowSums<MODE>& sum, float* tmp) {
   const bool soft = t.ts != 0.f, empty = sum.m == kNegInf && sum.s == 0.f;
-  const float logs = logf(sum.s), logts = logf(t.ts);
+  const float logs = logf(sum.s), logts = logf(t.ts), inv_ts = 1.f / t.ts;
   float term = 0.f;
 #pragma unroll
   for (int i = 0; i < Teacher<G>::N; ++i) {
     if (t.e[i] == 0.f || !soft) continue;   // weight 0; NaN goes on
-    const float lw = (t.u[i] - t.ref) / p.temp - logts;
-    const float xi = t.id[i] >= 0 && t.id[i] < p.vocab ? (float)x[t.id[i]] : __builtin_nanf("");
-    const float lq = empty ? kNegInf : (xi - sum.m) / p.temp - logs;
-    term += t.e[i] / t.ts * (lw - lq);
+    const float lw = (t.u[i] - t.ref) * p.inv_t - logts;
+    const float xi = t.id[i] >= 0 ? (float)x[t.id[i]] : __builtin_nanf("");
+    const float lq = empty ? kNegInf : (xi - sum.m) * p.inv_t - logs;
+    term += t.e[i] * inv_ts * (lw - lq);
   }
   const float kd = G::sum(term, tmp);
   if (G::tid() != 0) return;
@@ -762,7 +849,8 @@ __device__ __forceinline__ void distill_store(const DistillParams& p, int64_t r,
   p.kd[r] = soft ? p.temp * p.temp * kd : 0.f;
   stats[0] = soft || hard ? sum.m : 0.f;
   stats[1] = sum.s;
-  stats[2] = sum.s1;
+  const float s1 = MODE == kDual ? sum.s1 : sum.s;
+  stats[2] = s1;
   stats[3] = t.ref;
   stats[4] = t.ts;
   if (p.nll) {
@@ -770,36 +858,37 @@ __device__ __forceinline__ void distill_store(const DistillParams& p, int64_t r,
     if (hard) {
       v = tgt < 0 || tgt >= p.vocab ? __builtin_nanf("")
           : empty                   ? __builtin_inff()
-                                    : logf(sum.s1) - ((float)x[tgt] - sum.m);
+                                    : logf(s1) - ((float)x[tgt] - sum.m);
     }
     p.nll[r] = v;
   }
 }
 
-template <int NW, int U, typename T>
+// MODE kDual where the cross-entropy's sum is another than the teacher's, else kSingle.
+template <int MODE, int NT, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_fwd_kernel(const DistillParams p) {
-  using G = Group<NW>;
-  __shared__ float tmp[4];
+  using G = Group<NT>;
+  __shared__ float tmp[G::TMP];
   for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     const Teacher<G> t(p, r, tmp);
     const int64_t tgt = p.targets ? p.targets[r] : 0;
     const bool hard = p.targets && tgt != p.ignore;
-    RowSums<kDual> sum;
+    RowSums<MODE> sum;
     if (t.ts != 0.f || hard) {
       Best unused;
       row_pass<G, U, false>(sum, unused, x, p.vocab, p.c, p.c1);
       sum.template join<G>(p.c, p.c1, tmp);
     }
-    distill_store(p, r, x, t, hard, tgt, sum, tmp);
+    distill_store<G>(p, r, x, t, hard, tgt, sum, tmp);
   }
 }
 
 // Few long rows: a workgroup to each of a row's pieces, then one to join them.
-template <int U, typename T>
+template <int MODE, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_piece_kernel(const DistillParams p) {
-  using G = Group<4>;
-  __shared__ float tmp[4];
+  using G = Group<256>;
+  __shared__ float tmp[G::TMP];
   const int64_t r = blockIdx.x / p.split;
   const int g = (int)(blockIdx.x - r * p.split);
   const int lo = g * p.share, n = min(p.share, p.vocab - lo);
@@ -808,7 +897,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_piece_kernel(const Distil
     for (int j = threadIdx.x; j < p.k; j += kRowThreads) any = any || teacher_id(p, r * p.k + j) >= 0;
     if (!__syncthreads_or(any)) return;
   }
-  RowSums<kDual> sum;
+  RowSums<MODE> sum;
   Best unused;
   row_pass<G, U, false>(sum, unused, row_at<T>(p.logits, r, p.seqlen) + lo, n, p.c, p.c1);
   sum.template join<G>(p.c, p.c1, tmp);
@@ -816,41 +905,42 @@ __global__ void __launch_bounds__(kRowThreads) distill_piece_kernel(const Distil
     float* out = p.part + 3 * (r * p.split + g);
     out[0] = sum.m;
     out[1] = sum.s;
-    out[2] = sum.s1;
+    if (MODE == kDual) out[2] = sum.s1;
   }
 }
 
-template <typename T>
+template <int MODE, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_join_kernel(const DistillParams p) {
-  using G = Group<4>;
-  __shared__ float tmp[4];
+  using G = Group<256>;
+  __shared__ float tmp[G::TMP];
   const int64_t r = blockIdx.x;
   const Teacher<G> t(p, r, tmp);
   const int64_t tgt = p.targets ? p.targets[r] : 0;
   const bool hard = p.targets && tgt != p.ignore;
-  RowSums<kDual> sum;
+  RowSums<MODE> sum;
   if (t.ts != 0.f || hard) {
     if ((int)threadIdx.x < p.split) {
       const float* in = p.part + 3 * (r * p.split + threadIdx.x);
       sum.m = in[0];
       sum.s = in[1];
-      sum.s1 = in[2];
+      if (MODE == kDual) sum.s1 = in[2];
     }
     sum.template join<G>(p.c, p.c1, tmp);
   }
-  distill_store(p, r, row_at<T>(p.logits, r, p.seqlen), t, hard, tgt, sum, tmp);
+  distill_store<G>(p, r, row_at<T>(p.logits, r, p.seqlen), t, hard, tgt, sum, tmp);
 }
 
-template <int NW, typename T>
+// DUAL: both losses, at two temperatures; else one exponential serves (kd alone or the
+// cross-entropy alone at its own c, or both at temperature 1).
+template <bool DUAL, int NT, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillParams p) {
-  using G = Group<NW>;
-  __shared__ int sids[G::ROWS][kTeacherMax];
-  __shared__ float sweight[G::ROWS][kTeacherMax];
-  int* ids = sids[G::slot()];
-  float* wt = sweight[G::slot()];
+  using G = Group<NT>;
+  constexpr int KMAX = NT == 16 ? kPartTeacher : kTeacherMax;
+  __shared__ int sids[G::ROWS][KMAX + 1];   // odd: the groups of a wave on different banks
+  __shared__ float sweight[G::ROWS][KMAX + 1];
   const int64_t work = p.rows * p.chunks;
   for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
-    const int64_t r = w / p.chunks;
+    const int64_t r = quotient(w, p.chunks);
     const int lo = (int)(w - r * p.chunks) * kChunk<G, T>, hi = min(lo + kChunk<G, T>, p.vocab);
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
@@ -866,8 +956,11 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
     float b = hard ? p.dnll[r] : 0.f;
     if (hard && (tgt < 0 || tgt >= p.vocab)) b = __builtin_nanf("");
     const float bs = b / s1;
+    // one exponential: of the teacher's temperature, or of the cross-entropy's if it is alone
+    const float ec = soft ? p.c : p.c1, es = soft ? (hard ? as + bs : as) : bs;
     const auto f = [&](float v) {
       const float d = v - m;
+      if constexpr (!DUAL) return es * __builtin_amdgcn_exp2f(d * ec);
       float o = 0.f;
       if (soft) o = as * __builtin_amdgcn_exp2f(d * p.c);
       if (hard) o += bs * __builtin_amdgcn_exp2f(d * p.c1);
@@ -875,15 +968,42 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
     };
     chunk_map<G>(x, dx, lo, hi, f);
     const int k = soft ? p.k : 0;
+    const float at = a / ts;
+    const auto weight = [&](int64_t id, int j) {   // what an entry takes
+      if (id < 0 || id >= p.vocab) return 0.f;
+      return at * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + j) - ref) * p.c);
+    };
+    // Entries that the teacher's tokens or the true one take from, whole: a token named twice is
+    // written by its first mention.
+    G::sync();
+    if (NT >= 64 && k <= 64) {   // one a lane of the first wave
+      if (NT == 256 && threadIdx.x >= 64) continue;
+      const int lane = lane_id();
+      const int64_t id = lane < k ? teacher_id(p, r * k + lane) : -1;
+      const int i = id >= lo && id < hi ? (int)id : -1;
+      if (__ballot(i >= 0)) {
+        const float mine = lane < k ? weight(id, lane) : 0.f;
+        float take = 0.f;
+        bool first = true;
+        for (int l = 0; l < k; ++l) {
+          const bool same = __builtin_amdgcn_readlane(i, l) == i;
+          const float wl = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), l));
+          take += same ? wl : 0.f;
+          first = first && !(same && l < lane);
+        }
+        if (i >= 0 && first) dx[i] = (T)(f((float)x[i]) - take - (hard && i == tgt ? b : 0.f));
+      }
+      if (hard && tgt >= lo && tgt < hi && !__ballot(i == (int)tgt) && lane == 0) dx[tgt] = (T)(f((float)x[tgt]) - b);
+      continue;
+    }
+    int* ids = sids[G::slot()];
+    float* wt = sweight[G::slot()];
     for (int j = G::tid(); j < k; j += G::NT) {
       const int64_t id = teacher_id(p, r * k + j);
-      const bool there = id >= 0 && id < p.vocab;
-      ids[j] = there ? (int)id : -1;
-      wt[j] = there ? a * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + j) - ref) * p.c) / ts : 0.f;
+      ids[j] = id >= 0 && id < p.vocab ? (int)id : -1;
+      wt[j] = weight(id, j);
     }
     G::sync();
-    // entries that the teacher's tokens or the true one take from, whole: a token named twice
-    // is written by its first mention
     for (int j = G::tid(); j < k; j += G::NT) {
       const int i = ids[j];
       if (i < lo || i >= hi) continue;
@@ -929,11 +1049,19 @@ static int32_t check_logits(const A* a, const char* who) {
   M3S_REQUIRE(a->logits.stride_b >= 0 && a->logits.stride_t >= 0, "%s: negative logits stride", who);
   return 0;
 }
-static int vocab_chunks(int vocab, int dtype) {
-  const bool b = dtype == M3S_DTYPE_BF16;
-  const int chunk = vocab <= kWaveVocab ? (b ? kChunk<Group<1>, bf16> : kChunk<Group<1>, float>)
-                                        : (b ? kChunk<Group<4>, bf16> : kChunk<Group<4>, float>);
+// The threads to a row: `part` says that 16 lanes can do the call at all.
+static int row_threads(int vocab, bool part) {
+  return part && vocab <= kPartVocab ? 16 : vocab <= kWaveVocab ? 64 : 256;
+}
+static int vocab_chunks(int vocab, int dtype, int nt) {
+  const int chunk = nt * kBwdPieces * (dtype == M3S_DTYPE_BF16 ? Piece<bf16>::N : Piece<float>::N);
   return (vocab + chunk - 1) / chunk;
+}
+// Rows from one stride_b to the next: all of them where the batch axis continues the other.
+template <typename A>
+static int row_period(const A* a) {
+  const bool one = a->batch == 1 || a->logits.stride_b == (int64_t)a->seqlen * a->logits.stride_t;
+  return one ? a->batch * a->seqlen : a->seqlen;
 }
 // Logits to a piece: whole 16-byte pieces.
 static int row_share(int vocab, int split) { return ((vocab + split - 1) / split + 7) / 8 * 8; }
@@ -964,10 +1092,9 @@ static LogprobParams logprob_params(const m3s_logprob_args* a) {
   p.dlogits = a->dlogits;
   p.ignore = a->ignore_index;
   p.rows = (int64_t)a->batch * a->seqlen;
-  p.seqlen = a->seqlen;
+  p.seqlen = row_period(a);
   p.vocab = a->vocab;
   p.top = a->top;
-  p.chunks = vocab_chunks(a->vocab, a->dtype);
   p.part = static_cast<float*>(a->workspace);
   p.temp = a->temperature;
   p.inv_t = (float)(1.0 / a->temperature);
@@ -989,10 +1116,9 @@ static DistillParams distill_params(const m3s_distill_args* a) {
   p.dlogits = a->dlogits;
   p.ignore = a->ignore_index;
   p.rows = (int64_t)a->batch * a->seqlen;
-  p.seqlen = a->seqlen;
+  p.seqlen = row_period(a);
   p.vocab = a->vocab;
   p.k = a->teacher_k;
-  p.chunks = vocab_chunks(a->vocab, a->dtype);
   p.part = static_cast<float*>(a->workspace);
   p.id_bytes = a->id_bytes;
   p.teacher_bf16 = a->teacher_dtype == M3S_DTYPE_BF16;
@@ -1007,44 +1133,63 @@ template <typename P>
 static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t s) {
   hipLaunchKernelGGL(f, dim3((unsigned)std::min(kRowGrid, blocks)), dim3(kRowThreads), 0, s, p);
 }
-// f(group, U): the waves to a row and the 16-byte pieces of a batch, by the row's length
-template <typename T, typename F>
-static void with_group(int vocab, F&& f) {
-  constexpr int N = Piece<T>::N;
-  if (vocab > kWaveVocab) f(Group<4>(), std::integral_constant<int, 16 / N>());
-  else if (vocab > 64 * N) f(Group<1>(), std::integral_constant<int, 16 / N>());
-  else f(Group<1>(), std::integral_constant<int, 1>());
+// f(group): the threads to a row
+template <typename F>
+static void with_group(int nt, F&& f) {
+  if (nt == 16) f(Group<16>());
+  else if (nt == 64) f(Group<64>());
+  else f(Group<256>());
 }
+// Pieces of a thread's batch: 16 logits, or one piece where a wave holds the whole row so.
+template <typename T>
+constexpr int kBatch = 16 / Piece<T>::N;
 
 template <bool TOP, typename T>
 static void launch_logprob_fwd(const LogprobParams& p, hipStream_t s) {
+  constexpr int U = kBatch<T>;
   if (p.split > 1) {
-    launch_kernel(logprob_piece_kernel<TOP, 16 / Piece<T>::N, T>, p.rows * p.split, p, s);
+    launch_kernel(logprob_piece_kernel<TOP, U, T>, p.rows * p.split, p, s);
     launch_kernel(logprob_join_kernel<TOP, T>, p.rows, p, s);
     return;
   }
-  with_group<T>(p.vocab, [&](auto g, auto u) {
-    constexpr int NW = decltype(g)::NT / 64;
-    launch_kernel(logprob_fwd_kernel<TOP, NW, decltype(u)::value, T>, (p.rows + 4 / NW - 1) / (4 / NW), p, s);
+  const int nt = row_threads(p.vocab, !TOP || (p.top <= kPartTop && p.vocab <= kPartPick));
+  with_group(nt, [&](auto g) {
+    constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
+    const int64_t blocks = (p.rows + ROWS - 1) / ROWS;
+    if (NT == 64 && p.vocab <= 64 * Piece<T>::N) launch_kernel(logprob_fwd_kernel<TOP, NT, 1, T>, blocks, p, s);
+    else launch_kernel(logprob_fwd_kernel<TOP, NT, U, T>, blocks, p, s);
+  });
+}
+template <int MODE, typename T>
+static void launch_distill_fwd(const DistillParams& p, hipStream_t s) {
+  constexpr int U = kBatch<T>;
+  if (p.split > 1) {
+    launch_kernel(distill_piece_kernel<MODE, U, T>, p.rows * p.split, p, s);
+    launch_kernel(distill_join_kernel<MODE, T>, p.rows, p, s);
+    return;
+  }
+  with_group(row_threads(p.vocab, p.k <= kPartTeacher), [&](auto g) {
+    constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
+    launch_kernel(distill_fwd_kernel<MODE, NT, U, T>, (p.rows + ROWS - 1) / ROWS, p, s);
   });
 }
 template <typename T>
-static void launch_distill_fwd(const DistillParams& p, hipStream_t s) {
-  if (p.split > 1) {
-    launch_kernel(distill_piece_kernel<16 / Piece<T>::N, T>, p.rows * p.split, p, s);
-    launch_kernel(distill_join_kernel<T>, p.rows, p, s);
-    return;
-  }
-  with_group<T>(p.vocab, [&](auto g, auto u) {
-    constexpr int NW = decltype(g)::NT / 64;
-    launch_kernel(distill_fwd_kernel<NW, decltype(u)::value, T>, (p.rows + 4 / NW - 1) / (4 / NW), p, s);
+static void launch_logprob_bwd(LogprobParams& p, int dtype, hipStream_t s) {
+  const int nt = row_threads(p.vocab, true);
+  p.chunks = vocab_chunks(p.vocab, dtype, nt);
+  with_group(nt, [&](auto g) {
+    constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
+    launch_kernel(logprob_bwd_kernel<NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s);
   });
 }
-template <typename P>
-static void launch_bwd(void (*wave)(P), void (*block)(P), const P& p, hipStream_t s) {
-  const int64_t work = p.rows * p.chunks;
-  if (p.vocab <= kWaveVocab) launch_kernel(wave, (work + 3) / 4, p, s);
-  else launch_kernel(block, work, p, s);
+template <bool DUAL, typename T>
+static void launch_distill_bwd(DistillParams& p, int dtype, hipStream_t s) {
+  const int nt = row_threads(p.vocab, p.k <= kPartTeacher);
+  p.chunks = vocab_chunks(p.vocab, dtype, nt);
+  with_group(nt, [&](auto g) {
+    constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
+    launch_kernel(distill_bwd_kernel<DUAL, NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s);
+  });
 }
 
 static int64_t logprob_scratch(int64_t rows, int vocab, int top) {
@@ -1113,10 +1258,10 @@ extern "C" int32_t m3s_logprob_bwd(const m3s_logprob_args* a, void* stream) {
   M3S_REQUIRE(a->stats && a->dlogits && (uintptr_t)a->dlogits % es == 0 && (!a->dlogp || a->targets) &&
                   (!a->dtop_logp || !a->top || a->top_ids),
               "m3s_logprob_bwd: NULL or misaligned pointer");
-  const LogprobParams p = logprob_params(a);
+  LogprobParams p = logprob_params(a);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == M3S_DTYPE_BF16) launch_bwd(logprob_bwd_kernel<1, bf16>, logprob_bwd_kernel<4, bf16>, p, s);
-  else launch_bwd(logprob_bwd_kernel<1, float>, logprob_bwd_kernel<4, float>, p, s);
+  if (a->dtype == M3S_DTYPE_BF16) launch_logprob_bwd<bf16>(p, a->dtype, s);
+  else launch_logprob_bwd<float>(p, a->dtype, s);
   return launch_status("m3s_logprob_bwd");
 }
 
@@ -1142,7 +1287,9 @@ extern "C" int32_t m3s_distill_fwd(const m3s_distill_args* a, void* stream) {
   DistillParams p = distill_params(a);
   set_split(p, distill_scratch(p.rows, p.vocab), a->workspace_bytes, 0);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  a->dtype == M3S_DTYPE_BF16 ? launch_distill_fwd<bf16>(p, s) : launch_distill_fwd<float>(p, s);
+  const bool b = a->dtype == M3S_DTYPE_BF16, dual = p.targets && p.temp != 1.f;
+  if (dual) b ? launch_distill_fwd<kDual, bf16>(p, s) : launch_distill_fwd<kDual, float>(p, s);
+  else b ? launch_distill_fwd<kSingle, bf16>(p, s) : launch_distill_fwd<kSingle, float>(p, s);
   return launch_status("m3s_distill_fwd");
 }
 
@@ -1153,9 +1300,10 @@ extern "C" int32_t m3s_distill_bwd(const m3s_distill_args* a, void* stream) {
   const uintptr_t es = a->dtype == M3S_DTYPE_BF16 ? 2 : 4;
   M3S_REQUIRE(a->dlogits && (uintptr_t)a->dlogits % es == 0 && (!a->dnll || a->targets),
               "m3s_distill_bwd: NULL or misaligned pointer");
-  const DistillParams p = distill_params(a);
+  DistillParams p = distill_params(a);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == M3S_DTYPE_BF16) launch_bwd(distill_bwd_kernel<1, bf16>, distill_bwd_kernel<4, bf16>, p, s);
-  else launch_bwd(distill_bwd_kernel<1, float>, distill_bwd_kernel<4, float>, p, s);
+  const bool b = a->dtype == M3S_DTYPE_BF16, dual = p.dkd && p.dnll && p.temp != 1.f;
+  if (dual) b ? launch_distill_bwd<true, bf16>(p, a->dtype, s) : launch_distill_bwd<true, float>(p, a->dtype, s);
+  else b ? launch_distill_bwd<false, bf16>(p, a->dtype, s) : launch_distill_bwd<false, float>(p, a->dtype, s);
   return launch_status("m3s_distill_bwd");
 }
