@@ -34,7 +34,7 @@ constexpr int kTeacherMax = 256;   // teacher tokens of a row
 // Rows up to kPartVocab long go to 16 lanes each, up to kWaveVocab to a wave, longer ones to a
 // workgroup.
 constexpr int kPartVocab = 512, kWaveVocab = 1024;
-constexpr int kPartTop = 8;         // alternatives that 16 lanes pick, of rows up to kPartPick long
+constexpr int kPartTop = 16;        // alternatives that 16 lanes pick, of rows up to kPartPick long
 constexpr int kPartPick = 256;
 constexpr int kPartTeacher = 64;    // teacher tokens of a row of 16 lanes
 constexpr float kNegInf = -__builtin_inff();
@@ -200,6 +200,7 @@ __device__ __forceinline__ int dpp_int(int v) {
 
 // Where a thread's best logits lie: the largest maxima of its batches (U pieces of 16 bytes), the
 // first two with their batch, so that the alternatives are found without reading the row again.
+// The rest that fills no piece is not among them.
 struct Best {
   float m1 = kNegInf, m2 = kNegInf, m3 = kNegInf;
   int b1 = -1, b2 = -1;   // -1: none seen, or none above -inf
@@ -260,7 +261,6 @@ __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* 
   const int at = n / R::N * R::N + G::tid();
   if (at < n) {
     const float v = (float)x[at];
-    if constexpr (TOP) best.see(v, batches);
     r.template add<1>(&v, v, c, c1);
   }
 }
@@ -287,101 +287,127 @@ __device__ __forceinline__ uint32_t float_key(float v) {
 __device__ __forceinline__ float key_float(uint32_t k) {
   return __builtin_bit_cast(float, k ^ ((k >> 31) ? 0x80000000u : 0xffffffffu));
 }
-// A bound that at least k of the wave's 64 N values reach, and as few more as ties allow: bit by
-// bit from the top, by ballots.
+constexpr uint32_t kKeyMin = 0x007fffffu;   // the key of -inf
+
+// A bound that at least k of the wave's 64 N values reach and no more than `most` >= k do, if ties
+// allow it: found by ballots, first in doubling steps down from the largest value's key `top`,
+// which the logits worth listing lie close to, then by halving. Of ties, the bound is the k-th value.
 template <int N>
-__device__ __forceinline__ float kth_bound(const float* v, int k) {
+__device__ __forceinline__ float kth_bound(const float* v, float top, int k, int most) {
   uint32_t key[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) key[i] = float_key(v[i]);
-  uint32_t at = 0;
-  for (int bit = 31; bit >= 0; --bit) {
-    const uint32_t trial = at | (1u << bit);
+  const auto reach = [&](uint32_t bar) {
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= trial));
-    if (n >= k) at = trial;
-    if (n == k) break;
+    for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= bar));
+    return n;
+  };
+  const uint32_t kt = __builtin_amdgcn_readfirstlane(float_key(top));
+  uint32_t lo = kKeyMin, hi = kt + 1;   // at least k reach lo, fewer than k reach hi
+  for (int j = 20; j < 32; ++j) {
+    const uint32_t bar = kt - kKeyMin > (1u << j) ? kt - (1u << j) : kKeyMin;
+    const int n = reach(bar);
+    if (n >= k) {
+      lo = bar;
+      if (n <= most) return key_float(lo);
+      break;
+    }
+    hi = bar;
   }
-  return key_float(at < 0x007fffffu ? 0x007fffffu : at);   // not below the key of -inf
+  while (hi - lo > 1) {
+    const uint32_t bar = lo + (hi - lo) / 2;
+    const int n = reach(bar);
+    if (n >= k) {
+      lo = bar;
+      if (n <= most) break;
+    } else {
+      hi = bar;
+    }
+  }
+  return key_float(lo);
 }
 
+// Candidates: (value, index) as one number, the better ones larger.
+__device__ __forceinline__ uint64_t candidate(float v, int i) {
+  return (uint64_t)float_key(v) << 32 | (uint32_t)~i;
+}
 template <int NW>
 struct PickSpace {
-  static constexpr int CAP = NW == 4 ? 1024 : 512;
+  static constexpr int CAP = NW == 4 ? 1024 : 512, ITEMS = NW == 4 ? 512 : 1, WIDE = NW == 4 ? 256 : 1;
+  uint64_t list[CAP + 4];
   float best[64 * NW];
-  float v[CAP];
-  int i[CAP];
-  int count;
-  int itmp[4];
-  float tmp[8];
+  uint32_t item[ITEMS];   // thread and batch of a thread's best logits
+  int wide[WIDE];         // threads whose other batches hold some too
+  int count, items, wides, counts[4];
+  float bar, tmp[8];
 };
+template <bool STRICT>
+__device__ __forceinline__ bool reaches(float v, float bar) { return STRICT ? v > bar : v >= bar; }
 
-// Appends this thread's logit to the candidates if `hit`; a full list only counts.
-template <int CAP>
-__device__ __forceinline__ void append(bool hit, float v, int i, float* lv, int* li, int* count) {
-  const uint64_t m = __ballot(hit);
-  if (m == 0) return;
-  const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
-  int base = 0;
-  if (hit && before == 0) base = atomicAdd(count, (int)__popcll(m));
-  base = __builtin_amdgcn_readlane(base, __ffsll((unsigned long long)m) - 1);
-  if (hit && base + before < CAP) {
-    lv[base + before] = v;
-    li[base + before] = i;
-  }
+template <int NW>
+__device__ __forceinline__ void append(PickSpace<NW>& sp, float v, int i) {
+  const int at = atomicAdd(&sp.count, 1);
+  if (at < PickSpace<NW>::CAP) sp.list[at] = candidate(v, i);
 }
 
-// The candidates: every logit that reaches `bar` (STRICT: exceeds it), from the batches that hold
-// one. Returns their number, which may be more than the list holds.
-template <typename G, int U, bool STRICT, int NW, typename T>
+// By a workgroup: lists every logit that reaches `bar`. The threads name the batches that hold one,
+// then all of them read those, a piece of 16 bytes each. Returns the number, which may be more than
+// the list holds (it is then cut short).
+template <typename G, int U, bool STRICT, typename T>
 __device__ __forceinline__ int gather(const T* __restrict__ x, int n, const Best& best, float bar,
-                                      PickSpace<NW>& sp) {
+                                      PickSpace<4>& sp) {
   using R = Rows<G, U, T>;
-  constexpr int CAP = PickSpace<NW>::CAP;
-  const auto in = [&](float v) { return STRICT ? v > bar : v >= bar; };
-  const int batches = R::whole(n);
-  if (G::tid() == 0) sp.count = 0;
-  G::sync();
-  const auto take = [&](int b) {
-    if (b == batches) {
-      const int at = n / R::N * R::N + G::tid();
-      const float v = at < n ? (float)x[at] : kNegInf;
-      append<CAP>(at < n && in(v), v, at, sp.v, sp.i, &sp.count);
-      return;
-    }
-    float v[R::LEN];
-    R::load(x, n, b, v);
+  constexpr int N = R::N;
+  const int tid = G::tid(), full = n / N;
+  if (tid == 0) sp.count = sp.items = sp.wides = 0;
+  __syncthreads();
+  if (reaches<STRICT>(best.m3, bar)) {
+    sp.wide[atomicAdd(&sp.wides, 1)] = tid;
+  } else if (reaches<STRICT>(best.m1, bar)) {   // above m3, so b1, and below b2, name a batch
+    sp.item[atomicAdd(&sp.items, 1)] = (uint32_t)best.b1 << 8 | tid;
+    if (reaches<STRICT>(best.m2, bar)) sp.item[atomicAdd(&sp.items, 1)] = (uint32_t)best.b2 << 8 | tid;
+  }
+  const int tail = full * N + tid;
+  if (tail < n) {
+    const float v = (float)x[tail];
+    if (reaches<STRICT>(v, bar)) append(sp, v, tail);
+  }
+  __syncthreads();
+  const auto piece = [&](int at) {
+    float v[N];
+    Piece<T>::load(x + (int64_t)at * N, v);
 #pragma unroll
-    for (int i = 0; i < R::LEN; ++i) {
-      const int at = R::place(b, i);
-      append<CAP>(at < n / R::N * R::N && in(v[i]), v[i], at, sp.v, sp.i, &sp.count);
+    for (int i = 0; i < N; ++i) {
+      if (reaches<STRICT>(v[i], bar)) append(sp, v[i], at * N + i);
     }
   };
-  if (in(best.m1)) {
-    if (best.b1 >= 0) take(best.b1);
-    if (in(best.m2) && best.b2 >= 0) take(best.b2);
-    if (in(best.m3)) {
-      for (int b = 0; b <= batches; ++b) {
-        if (b != best.b1 && b != best.b2 && *(volatile int*)&sp.count <= CAP) take(b);
-      }
-    }
+  const int items = sp.items * U, wides = sp.wides;
+  for (int q = tid; q < items; q += G::NT) {
+    const uint32_t it = sp.item[q / U];
+    const int at = (int)(it >> 8) * R::HOP + q % U * G::NT + (int)(it & 255);
+    if (at < full) piece(at);
   }
-  G::sync();
-  const int count = sp.count;
-  G::sync();
-  return count;
+  for (int w = 0; w < wides && *(volatile int*)&sp.count <= PickSpace<4>::CAP; ++w) {
+    for (int at = sp.wide[w] + tid * G::NT; at < full; at += G::NT * G::NT) piece(at);
+  }
+  __syncthreads();
+  return sp.count;
 }
 
-// Ranks the `count` candidates; those under k go out.
+// Ranks the `count` listed candidates; those under k go out.
 template <typename G, int NW, typename OUT>
-__device__ __forceinline__ void rank_out(int count, int k, const PickSpace<NW>& sp, OUT&& out) {
+__device__ __forceinline__ void rank_out(int count, int k, PickSpace<NW>& sp, OUT&& out) {
+  if (G::tid() < 4) sp.list[count + G::tid()] = 0;   // below every candidate
+  G::sync();
   for (int c = G::tid(); c < count; c += G::NT) {
-    const float v = sp.v[c];
-    const int i = sp.i[c];
+    const uint64_t me = sp.list[c];
     int rank = 0;
-    for (int j = 0; j < count; ++j) rank += sp.v[j] > v || (sp.v[j] == v && sp.i[j] < i);
-    if (rank < k) out(rank, v, i);
+    for (int j = 0; j < count; j += 4) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) rank += sp.list[j + u] > me;
+    }
+    if (rank < k) out(rank, key_float((uint32_t)(me >> 32)), (int)~(uint32_t)me);
   }
 }
 
@@ -397,12 +423,12 @@ __device__ __forceinline__ void equal_out(const T* __restrict__ x, int n, float 
     int before = __popcll(m & ((1ull << lane) - 1)), all = __popcll(m);
     if constexpr (NW == 4) {
       const int wave = threadIdx.x >> 6;
-      if (lane == 0) sp.itmp[wave] = all;
+      if (lane == 0) sp.counts[wave] = all;
       __syncthreads();
       all = 0;
       for (int w = 0; w < 4; ++w) {
-        if (w < wave) before += sp.itmp[w];
-        all += sp.itmp[w];
+        if (w < wave) before += sp.counts[w];
+        all += sp.counts[w];
       }
       __syncthreads();
     }
@@ -436,25 +462,28 @@ __device__ __forceinline__ void values_out(const T* __restrict__ x, int n, int k
   }
 }
 
-// out(rank, value, index) for the k largest of n logits (k <= n, no NaN, no +inf), equal ones by
-// index. The k-th largest of the threads' maxima is reached by at least k logits, and by hardly
-// more: those are collected from the few batches that hold them and ranked against each other.
-template <typename G, int U, int NW, typename T, typename OUT>
-__device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, const Best& best,
-                                     PickSpace<NW>& sp, OUT&& out) {
-  constexpr int CAP = PickSpace<NW>::CAP;
-  float m[NW];
-  if constexpr (NW == 1) {
-    m[0] = best.m1;
-  } else {
-    sp.best[threadIdx.x] = best.m1;
-    __syncthreads();
+// out(rank, value, index) for the k largest of n logits (k <= n, no NaN, no +inf, the largest
+// `top`), equal ones by index. By a workgroup: a bound that k of the threads' maxima reach is
+// reached by at least k logits, and by hardly more; those are collected from the few batches that
+// hold them and ranked against each other.
+template <typename G, int U, typename T, typename OUT>
+__device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, float top, const Best& best,
+                                     PickSpace<4>& sp, OUT&& out) {
+  constexpr int CAP = PickSpace<4>::CAP;
+  sp.best[threadIdx.x] = best.m1;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    float m[4];
 #pragma unroll
-    for (int i = 0; i < NW; ++i) m[i] = sp.best[64 * i + lane_id()];
+    for (int i = 0; i < 4; ++i) m[i] = sp.best[64 * i + threadIdx.x];
+    const float bar = kth_bound<4>(m, top, k, min(k + 12, 64));
+    if (threadIdx.x == 0) sp.bar = bar;
   }
-  const float bar = kth_bound<NW>(m, k);
+  __syncthreads();
+  const float bar = sp.bar;
   int count = gather<G, U, false>(x, n, best, bar, sp);
   if (count > CAP) {   // many ties, as in masked rows: what exceeds them, then the first of them
+    __syncthreads();
     count = gather<G, U, true>(x, n, best, bar, sp);
     if (count > CAP) {
       values_out<G>(x, n, k, sp, out);
@@ -463,7 +492,51 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, cons
     equal_out<G>(x, n, bar, count, k, sp, out);
   }
   rank_out<G>(count, k, sp, out);
-  G::sync();   // the space is free again
+  __syncthreads();   // the space is free again
+}
+
+constexpr int kLaneTop = 24;   // kLaneTop * 17 logits fit the list
+// The same by a wave that holds the whole row, one batch and a rest. The bound is on the lanes'
+// maxima for few alternatives (one value a lane to count), on the logits themselves for more, of
+// which the lanes' maxima would let most of the row through.
+template <typename G, int U, typename T, typename OUT>
+__device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, float top, const Best&,
+                                     PickSpace<1>& sp, OUT&& out) {
+  using R = Rows<G, U, T>;
+  constexpr int LEN = R::LEN;
+  const int whole = n / R::N * R::N, tail = whole + G::tid();
+  float v[LEN + 1];
+  R::load(x, n, 0, v);
+  v[LEN] = tail < n ? (float)x[tail] : kNegInf;
+  float bar;
+  if (k <= kLaneTop) {
+    float most = v[0];
+#pragma unroll
+    for (int i = 1; i <= LEN; ++i) most = fmaxf(most, v[i]);
+    bar = kth_bound<1>(&most, top, k, min(k + 12, 64));
+  } else {
+    bar = kth_bound<LEN + 1>(v, top, k, 64);
+  }
+  const auto gather = [&](auto strict) {
+    constexpr bool STRICT = decltype(strict)::value;
+    if (G::tid() == 0) sp.count = 0;
+    G::sync();
+#pragma unroll
+    for (int i = 0; i < LEN; ++i) {
+      if (reaches<STRICT>(v[i], bar) && R::place(0, i) < whole) append(sp, v[i], R::place(0, i));
+    }
+    if (reaches<STRICT>(v[LEN], bar) && tail < n) append(sp, v[LEN], tail);
+    G::sync();
+    return __builtin_amdgcn_readfirstlane(sp.count);
+  };
+  int count = gather(std::false_type());
+  if (count > PickSpace<1>::CAP) {
+    G::sync();
+    count = gather(std::true_type());   // fewer than kLaneTop (LEN + 1), or than k
+    equal_out<G>(x, n, bar, count, k, sp, out);
+  }
+  rank_out<G>(count, k, sp, out);
+  G::sync();
 }
 
 // The same by 16 lanes that hold the row's at most kPartPick logits, one round for each of few.
@@ -579,7 +652,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     RowSums<kEntropy> sum;
     Best best;
-    row_pass<G, U, PICK>(sum, best, x, p.vocab, p.c, 0.f);
+    row_pass<G, U, PICK && NT == 256>(sum, best, x, p.vocab, p.c, 0.f);
     sum.template join<G>(p.c, 0.f, tmp);
     const LogprobRow logp(sum, p.inv_t);
     logprob_store<G>(p, r, tgt, x, sum, logp);
@@ -592,7 +665,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
         p.top_logp[r * p.top + j] = logp(v);
         p.top_ids[r * p.top + j] = i;
       };
-      if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, best, space[G::slot()], out);
+      if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
       else pick_few<G>(x, p.vocab, p.top, out);
     }
   }
@@ -628,7 +701,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_piece_kernel(const Logpro
       pi[j] = -1;
     }
     if (k) {
-      pick<G, U>(x, n, k, best, space[0], [&](int j, float v, int i) {
+      pick<G, U>(x, n, k, sum.m, best, space[0], [&](int j, float v, int i) {
         pv[j] = v;
         pi[j] = lo + i;
       });
@@ -672,9 +745,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
       Rows<G, 1, float>::load(part.v, n, b, v);
       best.see(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), b);
     }
-    const int at = n / 4 * 4 + threadIdx.x;
-    if (at < n) best.see(part.v[at], batches);
-    pick<G, 1>(part.v, n, p.top, best, space[0], [&](int j, float v, int i) {
+    pick<G, 1>(part.v, n, p.top, sum.m, best, space[0], [&](int j, float v, int i) {
       p.top_logp[r * p.top + j] = logp(v);
       p.top_ids[r * p.top + j] = part.i[i];
     });
