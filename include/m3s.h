@@ -616,8 +616,8 @@ int32_t m3s_gemv_fused(const m3s_gemv_fused_args* args, void* stream);
  * scale), and its gradient dtable[v] = scale sum of dy[t] over the t with ids[t] = v, summed in
  * float32 in position order and rounded once (bit-reproducible). Rows of ids that do not occur,
  * and of padding_idx, are zeros. An id outside [0, vocab) gives a row of NaN in y and adds to no
- * row. y, dy and dtable are dense, aligned to one element; vocab < 2^31 - 1, width < 2^22,
- * tokens < 2^31 - 32. */
+ * row. y, dy and dtable are dense, y and dy aligned to one element, dtable to 16 bytes;
+ * vocab < 2^31 - 1, width < 2^22, tokens < 2^31 - 64. */
 typedef struct m3s_embed_args {
   int32_t struct_size;   /* sizeof(m3s_embed_args) */
   int32_t dtype;         /* M3S_DTYPE_* of table, y, dy and dtable */
@@ -635,7 +635,7 @@ typedef struct m3s_embed_args {
   void* workspace;       /* backward scratch, 16-byte aligned */
   int64_t workspace_bytes; /* its size, at least m3s_embed_bwd_workspace_bytes() */
 } m3s_embed_args;
-/* The sorted ids and positions, digit counts, row spans and float32 partial sums. -1 on bad
+/* The sorted ids and positions, digit counts and float32 partial sums. -1 on bad
  * dimensions. No counterpart in the reference. */
 int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t width);
 int32_t m3s_embed_fwd(const m3s_embed_args* args, void* stream);

@@ -395,12 +395,14 @@ def launch(fn, args: C.Structure, dev: torch.device, what: str) -> None:
     a launch together; a layer forward makes five launches and its backward twelve, so the
     guard is entered only for a device that is not the current one and the stream's handle
     is read directly (the host's share of a B=1, L=2048 layer forward: 189 -> 160 us)."""
-    if torch.cuda.current_device() == dev.index:
-        rc = fn(C.byref(args), stream_handle(dev))
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:   # the tensors at hand have initialised the runtime
+        rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(dev):
             rc = fn(C.byref(args), stream_handle(dev))
-    check(rc, what)
+    if rc:
+        check(rc, what)
 
 
 @functools.lru_cache(maxsize=None, typed=True)

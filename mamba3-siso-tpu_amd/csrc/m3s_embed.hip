@@ -14,13 +14,14 @@
 //      bytes, two up to 2^18 ids. Ranks within a wave come from ballots (lanes with the same digit
 //      find each other bit by bit), across waves and workgroups from digit counts, so the order
 //      is that of the positions whatever runs first. Up to 4096 tokens one workgroup sorts in LDS.
-//   2. run_sum: a wave adds kRun sorted rows, 256 columns of them. A run of equal ids inside the
-//      piece is finished and written; one that crosses a border leaves a float32 partial.
-//   3. finish: a workgroup per table row adds the partials of a run that crosses pieces, in order,
-//      and writes zeros for ids that never occur.
+//      The sort waits more than it works and fills few CUs: workgroups beside it clear the table.
+//   2. run_sum: a wave adds a piece of 8 to 32 sorted rows, 256 columns of them. A run of equal
+//      ids inside the piece is finished and written; one that crosses a border leaves a float32
+//      partial sum.
+//   3. finish: the workgroup of the piece that a crossing run starts in adds its partials, in order.
 //
 // Every sum is float32 in a fixed order, rounded once. The gradient reads dy once and writes the
-// table once: bound by HBM from a few MB on, by the launches below that.
+// table once (a row that occurs twice): bound by HBM from a few MB on, by the launches below that.
 #include <algorithm>
 
 #include "m3s_common.h"
@@ -33,33 +34,56 @@ constexpr int kDigits = 512;          // counters of a pass: digits of up to 9 b
 constexpr int kDigitBits = 9;
 constexpr int kSortOne = 4096;        // tokens that one workgroup sorts alone, in LDS
 constexpr int kSortRounds = kSortOne / kSortThreads;
-constexpr int kSortBlocks = 256;      // workgroups of a larger sort, at most
-constexpr int kRun = 32;              // sorted rows that a wave of run_sum adds
+constexpr int kSortBlocks = 64;       // workgroups of a larger sort, at most
+constexpr int64_t kRunWaves = 2048;   // waves of run_sum that make its pieces longer
 
-// Four consecutive elements at any element alignment (gfx950 takes 16-byte accesses there).
+// W columns of a row, at any element alignment (gfx950 takes wide accesses there): 8 or 4 of bf16, 4
+// of float32, or one of a row narrower than that. Lanes take W columns each and the last one steps back to the
+// row's end: it and its neighbour then hold some columns both, read, add and write the same numbers
+// for them, and no row needs a ragged edge.
+template <int W> struct Cols { typedef float type __attribute__((ext_vector_type(W))); };
+template <int W> using cols = typename Cols<W>::type;
 typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
 typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
-__device__ __forceinline__ f32x4 ld4u(const float* p) { return *reinterpret_cast<const f32x4_u*>(p); }
-__device__ __forceinline__ f32x4 ld4u(const bf16* p) {
-  const bf16x4 r = *reinterpret_cast<const bf16x4_u*>(p);
-  return f32x4{(float)r[0], (float)r[1], (float)r[2], (float)r[3]};
-}
-__device__ __forceinline__ void st4u(float* p, f32x4 v) { *reinterpret_cast<f32x4_u*>(p) = v; }
-__device__ __forceinline__ void st4u(bf16* p, f32x4 v) {
-  *reinterpret_cast<bf16x4_u*>(p) = bf16x4{(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3]};
-}
-// W = 4 columns of a row, or one of a row narrower than that. Lanes take 4 columns each and the
-// last one steps back to the row's end: it and its neighbour then hold some columns both, read,
-// add and write the same numbers for them, and no row needs a ragged edge.
+template <int W> struct Halves { typedef bf16x8_u type; };
+template <> struct Halves<4> { typedef bf16x4_u type; };
+template <typename T> constexpr int kCols = 16 / sizeof(T);
+
 template <int W, typename T>
-__device__ __forceinline__ f32x4 ld_cols(const T* p) {
-  if constexpr (W == 4) return ld4u(p);
-  return f32x4{(float)p[0], 0.f, 0.f, 0.f};
+__device__ __forceinline__ cols<W> ld_cols(const T* p) {
+  cols<W> v;
+  if constexpr (W == 1) {
+    v[0] = (float)p[0];
+  } else if constexpr (sizeof(T) == 2) {
+    const typename Halves<W>::type r = *reinterpret_cast<const typename Halves<W>::type*>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) v[i] = (float)r[i];
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      const f32x4 r = *reinterpret_cast<const f32x4_u*>(p + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[j + i] = r[i];
+    }
+  }
+  return v;
 }
 template <int W, typename T>
-__device__ __forceinline__ void st_cols(T* p, f32x4 v) {
-  if constexpr (W == 4) st4u(p, v);
-  else p[0] = (T)v[0];
+__device__ __forceinline__ void st_cols(T* p, cols<W> v) {
+  if constexpr (W == 1) {
+    p[0] = (T)v[0];
+  } else if constexpr (sizeof(T) == 2) {
+    typename Halves<W>::type r;
+#pragma unroll
+    for (int i = 0; i < W; ++i) r[i] = (bf16)v[i];
+    *reinterpret_cast<typename Halves<W>::type*>(p) = r;
+  } else {
+#pragma unroll
+    for (int j = 0; j < W; j += 4) {
+      *reinterpret_cast<f32x4_u*>(p + j) = f32x4{v[j], v[j + 1], v[j + 2], v[j + 3]};
+    }
+  }
 }
 
 // ---- lookup -----------------------------------------------------------------------------
@@ -77,12 +101,12 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const T* __restrict__ ta
     int c = c0;
     if (id < 0 || id >= vocab) {
       const float nan = __builtin_nanf("");
-      for (; c < D; c += step) st_cols<W>(out + min(c, D - W), f32x4{nan, nan, nan, nan});
+      for (; c < D; c += step) st_cols<W>(out + min(c, D - W), cols<W>(nan));
       continue;
     }
     const T* row = table + id * ld;
     for (; c + 3 * step + W <= D; c += 4 * step) {
-      f32x4 v[4];
+      cols<W> v[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) v[u] = ld_cols<W>(row + c + u * step);
 #pragma unroll
@@ -127,27 +151,40 @@ __device__ __forceinline__ uint32_t take_place(uint32_t* next, uint32_t digit, i
   return at + (uint32_t)__popcll(below);
 }
 
+// Inclusive prefix sum over a wave's lanes: within the rows of 16, then their totals carried over.
+template <int ctrl, int rows>
+__device__ __forceinline__ uint32_t dpp_add(uint32_t v) {
+  return v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, rows, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t v) {
+  v = dpp_add<0x111, 0xF>(v);   // row_shr 1, 2, 4, 8
+  v = dpp_add<0x112, 0xF>(v);
+  v = dpp_add<0x114, 0xF>(v);
+  v = dpp_add<0x118, 0xF>(v);
+  v = dpp_add<0x142, 0xA>(v);   // lane 15 of each row to the next: rows 1 and 3
+  v = dpp_add<0x143, 0xC>(v);   // lane 31 to rows 2 and 3
+  return v;
+}
+
 // cnt[wave][digit] -> the first place of that wave's keys of that digit: digits in order, then
 // waves; `before` (this thread's digit, threadIdx.x < kDigits) is what earlier workgroups hold and
-// `total` what all of them do. Uses scan[kDigits]; called by all kSortThreads.
-__device__ __forceinline__ void digit_places(uint32_t (*cnt)[kDigits], uint32_t* scan,
+// `total` what all of them do. Uses sums[kDigits / 64]; called by all kSortThreads.
+__device__ __forceinline__ void digit_places(uint32_t (*cnt)[kDigits], uint32_t* sums,
                                              uint32_t before, uint32_t total) {
-  const int d = threadIdx.x;
-  if (d < kDigits) scan[d] = total;
+  const int d = threadIdx.x, wave = d >> 6;
+  const uint32_t upto = wave_prefix(total);
+  if (d < kDigits && (d & 63) == 63) sums[wave] = upto;
   __syncthreads();
-  for (int s = 1; s < kDigits; s <<= 1) {   // inclusive prefix sum over the digits
-    uint32_t add = 0;
-    if (d < kDigits && d >= s) add = scan[d - s];
-    __syncthreads();
-    if (d < kDigits) scan[d] += add;
-    __syncthreads();
-  }
   if (d < kDigits) {
-    uint32_t at = scan[d] - total + before;
+    uint32_t at = upto - total + before;
+    for (int w = 0; w < wave; ++w) at += sums[w];
+    uint32_t c[kSortWaves];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) c[w] = cnt[w][d];
+#pragma unroll
     for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = cnt[w][d];
       cnt[w][d] = at;
-      at += c;
+      at += c[w];
     }
   }
   __syncthreads();
@@ -157,33 +194,44 @@ __device__ __forceinline__ void zero_counts(uint32_t (*cnt)[kDigits]) {
   for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) cnt[i / kDigits][i % kDigits] = 0;
 }
 
-// Up to kSortOne tokens: block 0 sorts, the others clear start and stop (span = 2 vocab ints).
-// Wave w holds the kSortRounds * 64 keys from w * kSortRounds * 64 on.
+// The share of the table that the workgroups behind the `sorters` first ones clear: 16-byte pieces
+// lo .. hi - 1 of it, and with the last of them the few elements after the last piece.
+struct Clear {
+  f32x4* table;
+  uint16_t* rest;
+  int64_t lo, hi;
+  int nrest;
+  __device__ __forceinline__ bool operator()(int sorters) const {
+    if ((int)blockIdx.x < sorters) return false;
+    const int64_t hop = (int64_t)(gridDim.x - sorters) * kSortThreads;
+    for (int64_t i = lo + (int64_t)(blockIdx.x - sorters) * kSortThreads + threadIdx.x; i < hi; i += hop) {
+      table[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    if ((int)blockIdx.x == sorters && (int)threadIdx.x < nrest) rest[threadIdx.x] = 0;
+    return true;
+  }
+};
+
+// Up to kSortOne tokens, by the first workgroup. Wave w holds the 64 `rounds` keys from 64 rounds w on.
 template <typename ID>
 __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const ID* __restrict__ ids,
                                                                 uint32_t* __restrict__ keys,
                                                                 uint32_t* __restrict__ pos,
-                                                                int32_t* __restrict__ span,
-                                                                int64_t span_n, int n, int vocab,
+                                                                const Clear clear, int n, int vocab,
                                                                 int64_t pad, int passes, int bits) {
-  if (blockIdx.x > 0) {
-    for (int64_t i = (int64_t)(blockIdx.x - 1) * kSortThreads + threadIdx.x; i < span_n;
-         i += (int64_t)(gridDim.x - 1) * kSortThreads) {
-      span[i] = 0;
-    }
-    return;
-  }
   __shared__ uint32_t cnt[kSortWaves][kDigits];
-  __shared__ uint32_t scan[kDigits];
+  __shared__ uint32_t sums[kDigits / 64];
   __shared__ uint32_t skey[kSortOne];
   __shared__ uint16_t spos[kSortOne];
+  if (clear(1)) return;
   const int wave = threadIdx.x >> 6, lane = lane_id();
-  const int i0 = wave * kSortRounds * 64 + lane;
+  const int rounds = (n + kSortThreads - 1) / kSortThreads;
+  const int i0 = wave * rounds * 64 + lane;
   uint32_t key[kSortRounds], p[kSortRounds];
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
     const int i = i0 + 64 * r;
-    key[r] = i < n ? sort_key(ids[i], vocab, pad) : 0u;
+    key[r] = r < rounds && i < n ? sort_key(ids[i], vocab, pad) : 0u;
     p[r] = (uint32_t)i;
   }
   for (int pass = 0; pass < passes; ++pass) {
@@ -193,16 +241,18 @@ __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const ID* __rest
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
-      if (i0 + 64 * r < n) atomicAdd(&cnt[wave][(key[r] >> shift) & mask], 1u);
+      if (r < rounds && i0 + 64 * r < n) atomicAdd(&cnt[wave][(key[r] >> shift) & mask], 1u);
     }
     __syncthreads();
     uint32_t total = 0;
     if (threadIdx.x < kDigits) {
+#pragma unroll
       for (int w = 0; w < kSortWaves; ++w) total += cnt[w][threadIdx.x];
     }
-    digit_places(cnt, scan, 0u, total);
+    digit_places(cnt, sums, 0u, total);
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
+      if (r >= rounds) break;
       const bool ok = i0 + 64 * r < n;
       const uint32_t at = take_place(cnt[wave], (key[r] >> shift) & mask, bits, ok);
       if (ok && at < (uint32_t)n) {
@@ -214,7 +264,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const ID* __rest
 #pragma unroll
     for (int r = 0; r < kSortRounds; ++r) {
       const int i = i0 + 64 * r;
-      if (i < n) {
+      if (r < rounds && i < n) {
         key[r] = skey[i];
         p[r] = spos[i];
       }
@@ -224,30 +274,24 @@ __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const ID* __rest
 #pragma unroll
   for (int r = 0; r < kSortRounds; ++r) {
     const int i = i0 + 64 * r;
-    if (i < n) {
+    if (r < rounds && i < n) {
       keys[i] = key[r];
       pos[i] = p[r];
     }
   }
 }
 
-// More tokens: workgroup b holds the `tile` keys from b tile on (tile a multiple of kSortThreads).
-// First the counts of each workgroup's digits ...
+// More tokens: workgroup b of nb holds the `tile` keys from b tile on (tile a multiple of
+// kSortThreads). First the counts of each workgroup's digits ...
 template <typename ID, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(const ID* __restrict__ ids,
                                                                   const uint32_t* __restrict__ keys,
                                                                   uint32_t* __restrict__ hist,
-                                                                  int32_t* __restrict__ span,
-                                                                  int64_t span_n, int64_t n,
+                                                                  const Clear clear, int nb, int64_t n,
                                                                   int tile, int vocab, int64_t pad,
                                                                   int shift, int bits) {
   __shared__ uint32_t cnt[kDigits];
-  if (FIRST) {
-    for (int64_t i = (int64_t)blockIdx.x * kSortThreads + threadIdx.x; i < span_n;
-         i += (int64_t)gridDim.x * kSortThreads) {
-      span[i] = 0;
-    }
-  }
+  if (clear(nb)) return;
   if (threadIdx.x < kDigits) cnt[threadIdx.x] = 0;
   __syncthreads();
   const uint32_t mask = (1u << bits) - 1;
@@ -265,9 +309,10 @@ template <typename ID, bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(
     const ID* __restrict__ ids, const uint32_t* __restrict__ keys, const uint32_t* __restrict__ pos,
     uint32_t* __restrict__ okeys, uint32_t* __restrict__ opos, const uint32_t* __restrict__ hist,
-    int64_t n, int tile, int vocab, int64_t pad, int shift, int bits) {
+    const Clear clear, int nb, int64_t n, int tile, int vocab, int64_t pad, int shift, int bits) {
   __shared__ uint32_t cnt[kSortWaves][kDigits];
-  __shared__ uint32_t scan[kDigits];
+  __shared__ uint32_t sums[kDigits / 64];
+  if (clear(nb)) return;
   const int wave = threadIdx.x >> 6, lane = lane_id();
   const uint32_t mask = (1u << bits) - 1;
   const int share = tile / kSortWaves;
@@ -283,15 +328,15 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(
   }
   uint32_t before = 0, total = 0;
   if (threadIdx.x < kDigits) {
-#pragma unroll 8
-    for (int b = 0; b < (int)gridDim.x; ++b) {
+#pragma unroll 16
+    for (int b = 0; b < nb; ++b) {
       const uint32_t h = hist[(int64_t)b * kDigits + threadIdx.x];
       total += h;
       if (b < (int)blockIdx.x) before += h;
     }
   }
   __syncthreads();
-  digit_places(cnt, scan, before, total);
+  digit_places(cnt, sums, before, total);
   for (int r = 0; r < share; r += 64) {
     const int64_t i = lo + r + lane;
     const bool ok = i < n;
@@ -306,25 +351,23 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(
 }
 
 // ---- sums by id ------------------------------------------------------------------------------
-// A wave adds the sorted rows kRun * piece .. of its 64 W columns. part (pieces, 2, D): slot 0 a
+// A wave adds the RUN sorted rows of a piece, 64 W columns of them. part (pieces, 2, D): slot 0 a
 // run that came from the piece before (and may go on), slot 1 one that starts here and goes on.
-template <int W, typename T>
+template <int RUN, int W, typename T>
 __global__ void __launch_bounds__(256) run_sum_kernel(const uint32_t* __restrict__ keys,
                                                       const uint32_t* __restrict__ pos,
                                                       const T* __restrict__ dy,
                                                       T* __restrict__ dtable,
-                                                      float* __restrict__ part,
-                                                      int32_t* __restrict__ start,
-                                                      int32_t* __restrict__ stop, int64_t n,
-                                                      int vocab, int D, float scale, int tiles) {
+                                                      float* __restrict__ part, int64_t n, int vocab,
+                                                      int D, float scale, int tiles) {
   const int lane = lane_id();
   const uint32_t none = 0xffffffffu;
-  const int64_t work = (n + kRun - 1) / kRun * tiles;
+  const int64_t work = (n + RUN - 1) / RUN * tiles;
   for (int64_t g = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); g < work; g += (int64_t)gridDim.x * 4) {
     const int64_t piece = g / tiles;
     const int tile = (int)(g - piece * tiles);
-    const int64_t i0 = piece * kRun;
-    const int held = n - i0 < kRun ? (int)(n - i0) : kRun;
+    const int64_t i0 = piece * RUN;
+    const int held = n - i0 < RUN ? (int)(n - i0) : RUN;
     uint32_t key = none, p = 0;
     if (lane < held) {
       key = keys[i0 + lane];
@@ -333,19 +376,12 @@ __global__ void __launch_bounds__(256) run_sum_kernel(const uint32_t* __restrict
     const uint32_t kprev = i0 > 0 ? keys[i0 - 1] : none;
     const uint32_t knext = i0 + held < n ? keys[i0 + held] : none;
     const int rows = __popcll(__ballot(lane < held && key < (uint32_t)vocab));   // the rest sorts last
-    if (tile == 0) {
-      uint32_t l = __shfl_up(key, 1), r = __shfl_down(key, 1);
-      if (lane == 0) l = kprev;
-      if (lane == held - 1) r = knext;
-      if (lane < rows && l != key) start[key] = (int32_t)(i0 + lane);
-      if (lane < rows && r != key) stop[key] = (int32_t)(i0 + lane + 1);
-    }
     const bool mine = W * (64 * tile + lane) < D;   // lanes past the row load its end and drop it
     const int c = min(W * (64 * tile + lane), D - W);
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    cols<W> acc = 0.f;
     int from = 0;
     for (int j0 = 0; j0 < rows; j0 += 8) {
-      f32x4 v[8];
+      cols<W> v[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const int j = min(j0 + u, rows - 1);
@@ -365,45 +401,49 @@ __global__ void __launch_bounds__(256) run_sum_kernel(const uint32_t* __restrict
           else if (kn == k) st_cols<W>(part + (2 * piece + 1) * D + c, acc);
           else st_cols<W>(dtable + (int64_t)k * D + c, acc * scale);
         }
-        acc = f32x4{0.f, 0.f, 0.f, 0.f};
+        acc = 0.f;
         from = j + 1;
       }
     }
   }
 }
 
-// The rest of the table: `each` rows to a workgroup, 64 W columns (blockIdx.y). Rows of a run
-// inside one piece are done. The four waves add a quarter of the partials each.
-template <int W, typename T>
-__global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ part,
-                                                     const int32_t* __restrict__ start,
-                                                     const int32_t* __restrict__ stop,
-                                                     T* __restrict__ dtable, int vocab, int D,
-                                                     float scale, int each) {
-  __shared__ f32x4 sums[4][64];
+// The runs that cross pieces, each by the workgroup of the piece it starts in, 64 W columns
+// (blockIdx.y): its slot 1, then slot 0 of the pieces that begin with its id. The four waves add a
+// quarter of them each. Most workgroups find no such run: all that decides it is loaded at once.
+template <int RUN, int W, typename T>
+__global__ void __launch_bounds__(256) finish_kernel(const uint32_t* __restrict__ keys,
+                                                     const float* __restrict__ part,
+                                                     T* __restrict__ dtable, int64_t n, int vocab,
+                                                     int D, float scale) {
+  __shared__ cols<W> sums[4][64];
   const int lane = lane_id(), wave = threadIdx.x >> 6;
   const bool mine = W * (64 * (int)blockIdx.y + lane) < D;
   const int c = min(W * (64 * (int)blockIdx.y + lane), D - W);
-  const int64_t v0 = (int64_t)blockIdx.x * each;
-  const int64_t v1 = v0 + each < vocab ? v0 + each : vocab;
-  for (int64_t v = v0; v < v1; ++v) {
-    const int s = start[v], e = stop[v];
-    if (s == e) {   // an id that never occurs
-      if (wave == (int)(v & 3) && mine) st_cols<W>(dtable + v * D + c, f32x4{0.f, 0.f, 0.f, 0.f});
-      continue;
+  for (int64_t p = blockIdx.x; (p + 1) * RUN < n; p += gridDim.x) {
+    // the ids before the piece, at its end, and at the start of each piece behind it
+    const uint32_t before = keys[p > 0 ? p * RUN - 1 : 0], k = keys[(p + 1) * RUN - 1];
+    const int64_t next = (p + 1 + lane) * RUN;
+    uint32_t head = keys[next < n ? next : n - 1];
+    uint64_t m = __ballot(next < n && head == k);
+    if (k >= (uint32_t)vocab || !(m & 1) || (p > 0 && before == k)) continue;
+    int64_t count = 1 + __popcll(m);
+    while (m == ~0ull) {
+      const int64_t at = (p + count + lane) * RUN;
+      head = keys[at < n ? at : n - 1];
+      m = __ballot(at < n && head == k);
+      count += __popcll(m);
     }
-    const int64_t p0 = s / kRun, p1 = (e - 1) / kRun;
-    if (p0 == p1) continue;
-    const int64_t count = p1 - p0 + 1, share = (count + 3) / 4;
+    const int64_t share = (count + 3) / 4;
     const int64_t lo = wave * share, hi = lo + share < count ? lo + share : count;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    cols<W> acc = 0.f;
 #pragma unroll 8
-    for (int64_t i = lo; i < hi; ++i) acc += ld_cols<W>(part + (2 * (p0 + i) + (i == 0)) * D + c);
+    for (int64_t i = lo; i < hi; ++i) acc += ld_cols<W>(part + (2 * (p + i) + (i == 0)) * D + c);
     sums[wave][lane] = acc;
     __syncthreads();
     if (wave == 0 && mine) {
-      st_cols<W>(dtable + v * D + c,
-                 (((sums[0][lane] + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * scale);
+      st_cols<W>(dtable + (int64_t)k * D + c,
+                 (((acc + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * scale);
     }
     __syncthreads();
   }
@@ -411,10 +451,11 @@ __global__ void __launch_bounds__(256) finish_kernel(const float* __restrict__ p
 
 // ---- host ------------------------------------------------------------------------------------
 struct EmbedSpace {
-  int64_t keys[2], pos[2], hist, span, part, total;   // byte offsets
+  int64_t keys[2], pos[2], hist, part, total;   // byte offsets
+  int run;                                      // sorted rows to a piece
 };
 
-static EmbedSpace embed_space(int64_t n, int64_t vocab, int64_t D) {
+static EmbedSpace embed_space(int64_t n, int64_t D) {   // for the wider of the two types, float32
   EmbedSpace s;
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
@@ -427,14 +468,16 @@ static EmbedSpace embed_space(int64_t n, int64_t vocab, int64_t D) {
     s.pos[i] = take(4 * n);
   }
   s.hist = take((int64_t)kSortBlocks * kDigits * 4);
-  s.span = take(8 * vocab);
-  s.part = take((n + kRun - 1) / kRun * 2 * D * 4);
+  // the longest pieces that leave enough waves to keep HBM busy
+  const int64_t tiles = D < 4 ? 1 : (D + 255) / 256;
+  s.run = n * tiles >= 32 * kRunWaves ? 32 : n * tiles >= 16 * kRunWaves ? 16 : 8;
+  s.part = take((n + s.run - 1) / s.run * 2 * D * 4);
   s.total = at;
   return s;
 }
 
 static bool embed_sizes_ok(int64_t n, int64_t vocab, int64_t D) {
-  return n >= 0 && n < (1ll << 31) - kRun && vocab > 0 && vocab < (1ll << 31) - 1 && D > 0 && D < (1 << 22);
+  return n >= 0 && n < (1ll << 31) - 64 && vocab > 0 && vocab < (1ll << 31) - 1 && D > 0 && D < (1 << 22);
 }
 
 constexpr int64_t kGridMax = 1 << 20;   // workgroups of a launch: the kernels step over the rest
@@ -449,63 +492,86 @@ static void launch_embed_fwd(const m3s_embed_args* a, hipStream_t s) {
                      a->width, a->scale, lg);
 }
 
+template <int RUN, int W, typename T>
+static void launch_sums(const m3s_embed_args* a, const uint32_t* keys, const uint32_t* pos, float* part,
+                        hipStream_t s) {
+  const int tiles = (a->width + 64 * W - 1) / (64 * W);
+  const int64_t pieces = (a->tokens + RUN - 1) / RUN;
+  T* dtable = static_cast<T*>(a->dtable);
+  hipLaunchKernelGGL((run_sum_kernel<RUN, W, T>), dim3((unsigned)std::min(kGridMax, (pieces * tiles + 3) / 4)),
+                     dim3(256), 0, s, keys, pos, static_cast<const T*>(a->dy), dtable, part, a->tokens,
+                     a->vocab, a->width, a->scale, tiles);
+  if (pieces < 2) return;   // nothing to cross
+  hipLaunchKernelGGL((finish_kernel<RUN, W, T>), dim3((unsigned)std::min(kGridMax, pieces - 1), (unsigned)tiles),
+                     dim3(256), 0, s, keys, part, dtable, a->tokens, a->vocab, a->width,
+                     a->scale);
+}
+
 template <int W, typename T, typename ID>
 static void launch_embed_bwd(const m3s_embed_args* a, hipStream_t s) {
-  const int64_t n = a->tokens, span_n = 2 * (int64_t)a->vocab;
-  const EmbedSpace sp = embed_space(n, a->vocab, a->width);
+  const int64_t n = a->tokens;
+  const EmbedSpace sp = embed_space(n, a->width);
   char* w = static_cast<char*>(a->workspace);
   const auto u32 = [&](int64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
-  int32_t* span = reinterpret_cast<int32_t*>(w + sp.span);
-  float* part = reinterpret_cast<float*>(w + sp.part);
   const ID* ids = static_cast<const ID*>(a->ids);
   int width = 1;   // bits of a key: 0 .. vocab
   while ((uint64_t)a->vocab >> width) ++width;
   const int passes = (width + kDigitBits - 1) / kDigitBits, bits = (width + passes - 1) / passes;
+  // each launch of the sort clears an equal share of the table
+  const int64_t bytes = (int64_t)a->vocab * a->width * sizeof(T), pieces = bytes / 16;
+  const int shares = n <= kSortOne ? 1 : 2 * passes;
+  const auto clear = [&](int share) {
+    Clear c;
+    c.table = static_cast<f32x4*>(a->dtable);
+    c.rest = reinterpret_cast<uint16_t*>(static_cast<char*>(a->dtable) + pieces * 16);
+    c.lo = pieces * share / shares;
+    c.hi = pieces * (share + 1) / shares;
+    c.nrest = share + 1 == shares ? (int)((bytes - pieces * 16) / 2) : 0;
+    return c;
+  };
+  const auto cleaners = [&](const Clear& c) {   // workgroups: 8 pieces to a thread, or more
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(1024, (c.hi - c.lo) / (8 * kSortThreads)));
+  };
   int last = 0;
   if (n <= kSortOne) {
-    const int64_t clear = (span_n + 4 * kSortThreads - 1) / (4 * kSortThreads);
-    hipLaunchKernelGGL((sort_one_kernel<ID>), dim3(1 + (unsigned)std::min<int64_t>(clear, 255)),
-                       dim3(kSortThreads), 0, s, ids, u32(sp.keys[0]), u32(sp.pos[0]), span, span_n,
-                       (int)n, a->vocab, a->padding_idx, passes, bits);
+    const Clear c = clear(0);
+    hipLaunchKernelGGL((sort_one_kernel<ID>), dim3(1 + cleaners(c)), dim3(kSortThreads), 0, s, ids,
+                       u32(sp.keys[0]), u32(sp.pos[0]), c, (int)n, a->vocab, a->padding_idx, passes, bits);
   } else {
     // the fewest 1024-key rounds that leave at most kSortBlocks workgroups
     const int64_t rounds = (n + (int64_t)kSortThreads * kSortBlocks - 1) / ((int64_t)kSortThreads * kSortBlocks);
     const int tile = (int)(rounds * kSortThreads);
-    const unsigned nb = (unsigned)((n + tile - 1) / tile);
+    const int nb = (int)((n + tile - 1) / tile);
     for (int p = 0; p < passes; ++p) {
       const int from = (p + 1) & 1, to = p & 1;
       uint32_t *ik = u32(sp.keys[from]), *ip = u32(sp.pos[from]), *ok = u32(sp.keys[to]), *op = u32(sp.pos[to]);
+      const Clear c0 = clear(2 * p), c1 = clear(2 * p + 1);
       const auto go = [&](auto count, auto place) {
-        hipLaunchKernelGGL(count, dim3(nb), dim3(kSortThreads), 0, s, ids, ik, u32(sp.hist), span, span_n,
-                           n, tile, a->vocab, a->padding_idx, p * bits, bits);
-        hipLaunchKernelGGL(place, dim3(nb), dim3(kSortThreads), 0, s, ids, ik, ip, ok, op, u32(sp.hist),
-                           n, tile, a->vocab, a->padding_idx, p * bits, bits);
+        hipLaunchKernelGGL(count, dim3(nb + cleaners(c0)), dim3(kSortThreads), 0, s, ids, ik, u32(sp.hist), c0,
+                           nb, n, tile, a->vocab, a->padding_idx, p * bits, bits);
+        hipLaunchKernelGGL(place, dim3(nb + cleaners(c1)), dim3(kSortThreads), 0, s, ids, ik, ip, ok, op,
+                           u32(sp.hist), c1, nb, n, tile, a->vocab, a->padding_idx, p * bits, bits);
       };
       if (p == 0) go(sort_count_kernel<ID, true>, sort_place_kernel<ID, true>);
       else go(sort_count_kernel<ID, false>, sort_place_kernel<ID, false>);
       last = to;
     }
   }
-  const int tiles = (a->width + 64 * W - 1) / (64 * W);
-  const int64_t blocks = ((n + kRun - 1) / kRun * tiles + 3) / 4;
-  if (n > 0) {
-    hipLaunchKernelGGL((run_sum_kernel<W, T>), dim3((unsigned)std::min(kGridMax, blocks)), dim3(256), 0, s,
-                       u32(sp.keys[last]), u32(sp.pos[last]), static_cast<const T*>(a->dy),
-                       static_cast<T*>(a->dtable), part, span, span + a->vocab, n, a->vocab, a->width,
-                       a->scale, tiles);
-  }
-  const int each = (int)std::max<int64_t>(std::max(1, std::min(16, a->vocab / 2048)),
-                                          (a->vocab + kGridMax - 1) / kGridMax);
-  hipLaunchKernelGGL((finish_kernel<W, T>), dim3((unsigned)((a->vocab + each - 1) / each), (unsigned)tiles),
-                     dim3(256), 0, s, part, span, span + a->vocab, static_cast<T*>(a->dtable), a->vocab,
-                     a->width, a->scale, each);
+  if (n == 0) return;
+  const uint32_t *keys = u32(sp.keys[last]), *pos = u32(sp.pos[last]);
+  float* part = reinterpret_cast<float*>(w + sp.part);
+  if (sp.run == 32) launch_sums<32, W, T>(a, keys, pos, part, s);
+  else if (sp.run == 16) launch_sums<16, W, T>(a, keys, pos, part, s);
+  else launch_sums<8, W, T>(a, keys, pos, part, s);
 }
 
 template <typename T, typename ID>
 static void launch_embed(const m3s_embed_args* a, hipStream_t s, bool bwd) {
-  const bool narrow = a->width < 4;
-  if (bwd) narrow ? launch_embed_bwd<1, T, ID>(a, s) : launch_embed_bwd<4, T, ID>(a, s);
-  else narrow ? launch_embed_fwd<1, T, ID>(a, s) : launch_embed_fwd<4, T, ID>(a, s);
+  const bool narrow = a->width < kCols<T>;
+  // sums of rows up to 256 wide: four columns of bf16 a lane, or half the lanes of a wave would idle
+  if (bwd && !narrow && a->width <= 256) launch_embed_bwd<4, T, ID>(a, s);
+  else if (bwd) narrow ? launch_embed_bwd<1, T, ID>(a, s) : launch_embed_bwd<kCols<T>, T, ID>(a, s);
+  else narrow ? launch_embed_fwd<1, T, ID>(a, s) : launch_embed_fwd<kCols<T>, T, ID>(a, s);
 }
 
 static void dispatch_embed(const m3s_embed_args* a, hipStream_t s, bool bwd) {
@@ -533,9 +599,9 @@ static int32_t check_embed(const m3s_embed_args* a, const char* who, bool bwd) {
     return 0;
   }
   M3S_REQUIRE(a->dtable && a->workspace && (a->tokens == 0 || (a->ids && a->dy)), "%s: NULL pointer", who);
-  M3S_REQUIRE((uintptr_t)a->dy % es == 0 && (uintptr_t)a->dtable % es == 0, "%s: misaligned rows", who);
-  M3S_REQUIRE(aligned16(a->workspace), "%s: workspace must be 16-byte aligned", who);
-  const int64_t need = embed_space(a->tokens, a->vocab, a->width).total;
+  M3S_REQUIRE((uintptr_t)a->dy % es == 0, "%s: misaligned rows", who);
+  M3S_REQUIRE(aligned16(a->workspace) && aligned16(a->dtable), "%s: dtable and workspace must be 16-byte aligned", who);
+  const int64_t need = embed_space(a->tokens, a->width).total;
   M3S_REQUIRE(a->workspace_bytes >= need, "%s: workspace of %lld bytes, needs %lld", who,
               (long long)a->workspace_bytes, (long long)need);
   return 0;
@@ -547,7 +613,7 @@ using namespace m3s;
 
 extern "C" int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t width) {
   if (!embed_sizes_ok(tokens, vocab, width)) return -1;
-  return embed_space(tokens, vocab, width).total;
+  return embed_space(tokens, width).total;
 }
 
 extern "C" int32_t m3s_embed_fwd(const m3s_embed_args* a, void* stream) {

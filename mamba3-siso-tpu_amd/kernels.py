@@ -1366,20 +1366,18 @@ def transpose_pad(w: Tensor, dtype: torch.dtype, out_rows: int) -> Tensor:
 
 #: The id and row types of the embedding and vocabulary kernels.
 ID_BYTES = {torch.int32: 4, torch.int64: 8}
+_EMBED_SIZE = ctypes.sizeof(_lib.EmbedArgs)
 
 
-def _embed_args(tokens: Tensor, dtype: torch.dtype, vocab: int, width: int,
-                scale: float) -> "_lib.EmbedArgs":
-    if tokens.dtype not in ID_BYTES:
+def _embed_args(tokens: Tensor, dtype: torch.dtype, vocab: int, width: int, scale: float,
+                padding_idx: int = -1) -> "_lib.EmbedArgs":
+    id_bytes = ID_BYTES.get(tokens.dtype)
+    if id_bytes is None:
         raise ValueError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
     if vocab < 1 or width < 1:
         raise ValueError(f"embedding: the table must not be empty, got {(vocab, width)}")
-    a = _lib.EmbedArgs()
-    a.struct_size = ctypes.sizeof(_lib.EmbedArgs)
-    a.dtype, a.id_bytes = _lib.dtype_code(dtype), ID_BYTES[tokens.dtype]
-    a.vocab, a.width, a.scale, a.tokens = vocab, width, scale, tokens.numel()
-    a.padding_idx = -1
-    return a
+    return _lib.EmbedArgs(_EMBED_SIZE, _lib.dtype_code(dtype), id_bytes, vocab, width, scale,
+                          tokens.numel(), padding_idx)
 
 
 def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
@@ -1390,7 +1388,7 @@ def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tens
     if table.dim() != 2:
         raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
     v, d = table.shape
-    a = _embed_args(tokens, table.dtype, v, d, float(scale))
+    a = _embed_args(tokens, table.dtype, v, d, scale)
     dev = _device_of(table, tokens)
     if table.stride(1) != 1 and d > 1:
         table = table.contiguous()
@@ -1411,16 +1409,15 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
     if dy.shape[:-1] != tokens.shape or dy.dim() == 0:
         raise ValueError(f"embedding: dy must be (*tokens.shape, D), got {tuple(dy.shape)} for tokens "
                          f"{tuple(tokens.shape)}")
-    a = _embed_args(tokens, dy.dtype, int(vocab), dy.shape[-1], float(scale))
-    if padding_idx is not None:
-        a.padding_idx = embedding_padding(padding_idx, a.vocab)
+    d, pad = dy.shape[-1], -1 if padding_idx is None else embedding_padding(padding_idx, vocab)
+    a = _embed_args(tokens, dy.dtype, vocab, d, scale, pad)
     dev = _device_of(tokens, dy)
     tokens, dy = tokens.contiguous(), dy.contiguous()
     lib = _lib.load()
-    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", a.tokens, a.vocab, a.width)
+    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", tokens.numel(), vocab, d)
     if nbytes < 0:
-        raise ValueError(f"embedding: bad sizes (tokens {a.tokens}, vocab {a.vocab}, width {a.width})")
-    dtable = empty(a.vocab, a.width, device=dev, dtype=dy.dtype)
+        raise ValueError(f"embedding: bad sizes (tokens {tokens.numel()}, vocab {vocab}, width {d})")
+    dtable = empty(vocab, d, device=dev, dtype=dy.dtype)
     ws = empty(nbytes, device=dev, dtype=torch.uint8)
     a.ids, a.dy, a.dtable = tokens.data_ptr(), dy.data_ptr(), dtable.data_ptr()
     a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
@@ -1430,9 +1427,9 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
 
 def embedding_padding(padding_idx: int, vocab: int) -> int:
     """``padding_idx`` as an id in [0, vocab); negative ones count from the end."""
-    if not -vocab <= padding_idx < vocab:
+    if vocab > 0 and not -vocab <= padding_idx < vocab:
         raise ValueError(f"embedding: padding_idx {padding_idx} is outside a vocabulary of {vocab}")
-    return padding_idx % vocab
+    return padding_idx % max(vocab, 1)
 
 
 #: Alternatives of `logprob_forward` and teacher tokens of `distill_forward`, at most.

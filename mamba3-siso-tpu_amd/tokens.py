@@ -22,8 +22,11 @@ Tensor = torch.Tensor
 def _needs_node(*tensors) -> bool:
     """Whether a call goes through its autograd node: a gradient is taken, or the node has to
     refuse what a bare launch would drop (a forward-mode tangent) or record wrongly (a trace)."""
-    return ((torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors))
-            or torch.jit.is_tracing() or LY.has_tangent(*tensors))
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                return True
+    return torch.jit.is_tracing() or LY.has_tangent(*tensors)
 
 
 class _EmbedFn(torch.autograd.Function):
