@@ -1037,61 +1037,103 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
       if (hard) o += bs * __builtin_amdgcn_exp2f(d * p.c1);
       return o;
     };
-    chunk_map<G>(x, dx, lo, hi, f);
     const int k = soft ? p.k : 0;
     const float at = a / ts;
     const auto weight = [&](int64_t id, int j) {   // what an entry takes
       if (id < 0 || id >= p.vocab) return 0.f;
       return at * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + j) - ref) * p.c);
     };
-    // Entries that the teacher's tokens or the true one take from, whole: a token named twice is
-    // written by its first mention.
-    G::sync();
-    if (NT >= 64 && k <= 64) {   // one a lane of the first wave
-      if (NT == 256 && threadIdx.x >= 64) continue;
-      const int lane = lane_id();
-      const int64_t id = lane < k ? teacher_id(p, r * k + lane) : -1;
-      const int i = id >= lo && id < hi ? (int)id : -1;
-      if (__ballot(i >= 0)) {
-        const float mine = lane < k ? weight(id, lane) : 0.f;
-        float take = 0.f;
-        bool first = true;
-        for (int l = 0; l < k; ++l) {
-          const bool same = __builtin_amdgcn_readlane(i, l) == i;
-          const float wl = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), l));
-          take += same ? wl : 0.f;
-          first = first && !(same && l < lane);
-        }
-        if (i >= 0 && first) dx[i] = (T)(f((float)x[i]) - take - (hard && i == tgt ? b : 0.f));
+    // The entries that the teacher's tokens or the true one take from are written again, whole; a
+    // token named twice by its first mention. Up to 64 of them lie one to a lane of the group's first
+    // wave, or four to each of 16 lanes, which load them ahead of the dense pass (22.9 -> 20.7 us at
+    // 32768 x 256; ahead of a workgroup's pass 107 -> 138 us at 2048 x 65536 bf16, all of which waits for them).
+    constexpr int LANES = NT == 16 ? 16 : 64, E = 64 / LANES;
+    const bool few = k <= 64, mine = few && G::tid() < LANES, truth = hard && tgt >= lo && tgt < hi;
+    int eid[E];
+    float ew[E], ex[E], tx = 0.f;
+    const auto load_entries = [&] {
+      if (!mine) return;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int j = e * LANES + G::tid();
+        const int64_t id = j < k ? teacher_id(p, r * k + j) : -1;
+        eid[e] = id >= lo && id < hi ? (int)id : -1;
+        ew[e] = eid[e] >= 0 ? weight(id, j) : 0.f;
+        ex[e] = eid[e] >= 0 ? (float)x[eid[e]] : 0.f;
       }
-      if (hard && tgt >= lo && tgt < hi && !__ballot(i == (int)tgt) && lane == 0) dx[tgt] = (T)(f((float)x[tgt]) - b);
-      continue;
-    }
+      if (truth) tx = (float)x[tgt];
+    };
+    if (NT == 16) load_entries();
+    chunk_map<G>(x, dx, lo, hi, f);
     int* ids = sids[G::slot()];
     float* wt = sweight[G::slot()];
-    for (int j = G::tid(); j < k; j += G::NT) {
-      const int64_t id = teacher_id(p, r * k + j);
-      ids[j] = id >= 0 && id < p.vocab ? (int)id : -1;
-      wt[j] = weight(id, j);
-    }
-    G::sync();
-    for (int j = G::tid(); j < k; j += G::NT) {
-      const int i = ids[j];
-      if (i < lo || i >= hi) continue;
-      bool first = true;
-      float take = 0.f;
-      for (int l = 0; l < k; ++l) {
-        if (ids[l] == i) {
-          first = first && l >= j;
-          take += wt[l];
+    if (NT == 16 || !few) {
+      if (few) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          ids[e * LANES + G::tid()] = eid[e];
+          wt[e * LANES + G::tid()] = ew[e];
+        }
+      } else {
+        for (int j = G::tid(); j < k; j += G::NT) {
+          const int64_t id = teacher_id(p, r * k + j);
+          ids[j] = id >= lo && id < hi ? (int)id : -1;
+          wt[j] = weight(id, j);
         }
       }
-      if (first) dx[i] = (T)(f((float)x[i]) - take - (hard && i == tgt ? b : 0.f));
     }
-    if (G::tid() == 0 && hard && tgt >= lo && tgt < hi) {
-      bool alone = true;
-      for (int l = 0; l < k; ++l) alone = alone && ids[l] != tgt;
-      if (alone) dx[tgt] = (T)(f((float)x[tgt]) - b);
+    G::sync();
+    if (few && !mine) continue;   // only now: waves that are done make room for the next workgroup's
+    if (NT > 16) load_entries();
+    const auto whole = [&](int i, float xi, float take) {
+      dx[i] = (T)(f(xi) - take - (hard && i == tgt ? b : 0.f));
+    };
+    const auto mentions = [&](int i, int j, float& take) {   // in LDS, of the j-th entry; first one?
+      bool first = true;
+      for (int l = 0; l < k; ++l) {
+        const bool same = ids[l] == i;
+        take += same ? wt[l] : 0.f;
+        first = first && !(same && l < j);
+      }
+      return first;
+    };
+    bool named = false;   // the true token is among the entries, some thread knows
+    if (few) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int j = e * LANES + G::tid();
+        if (NT == 16 ? e * LANES >= k : !__ballot(eid[e] >= 0)) break;
+        float take = 0.f;
+        bool first = true;
+        if constexpr (NT == 16) {
+          if (eid[e] >= 0) first = mentions(eid[e], j, take);
+        } else {
+          for (int l = 0; l < k; ++l) {
+            const bool same = __builtin_amdgcn_readlane(eid[0], l) == eid[0];
+            const float wl = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ew[0]), l));
+            take += same ? wl : 0.f;
+            first = first && !(same && l < j);
+          }
+        }
+        if (eid[e] >= 0 && first) whole(eid[e], ex[e], take);
+        named = named || (truth && eid[e] == (int)tgt);
+      }
+      if (truth) {
+        if constexpr (NT == 16) named = G::max(named ? 1.f : 0.f, nullptr) != 0.f;
+        else named = __ballot(named) != 0;
+        if (!named && G::tid() == 0) whole((int)tgt, tx, 0.f);
+      }
+      continue;
+    }
+    for (int j = G::tid(); j < k; j += G::NT) {
+      const int i = ids[j];
+      if (i < 0) continue;
+      float take = 0.f;
+      if (mentions(i, j, take)) whole(i, (float)x[i], take);
+    }
+    if (G::tid() == 0 && truth) {
+      for (int l = 0; l < k; ++l) named = named || ids[l] == tgt;
+      if (!named) whole((int)tgt, (float)x[tgt], 0.f);
     }
     G::sync();
   }
