@@ -1434,6 +1434,7 @@ def embedding_padding(padding_idx: int, vocab: int) -> int:
 
 #: Alternatives of `logprob_forward` and teacher tokens of `distill_forward`, at most.
 TOP_MAX, TEACHER_MAX = 64, 256
+_LOGPROB_SIZE, _DISTILL_SIZE = ctypes.sizeof(_lib.LogprobArgs), ctypes.sizeof(_lib.DistillArgs)
 
 
 def _logit_rows(logits: Tensor, what: str) -> Tensor:
@@ -1451,22 +1452,15 @@ def _logit_rows(logits: Tensor, what: str) -> Tensor:
     return logits.reshape(1, -1, v)
 
 
-def _row_args(a, rows3: Tensor, temperature: float, ignore_index: int) -> None:
-    """The fields that ``m3s_logprob_args`` and ``m3s_distill_args`` share."""
-    a.struct_size = ctypes.sizeof(a)
-    a.dtype = _lib.dtype_code(rows3.dtype)
-    a.batch, a.seqlen, a.vocab = rows3.shape
-    a.temperature, a.ignore_index = temperature, ignore_index
-    a.logits = _lib.blx(rows3)
-
-
 def _row_values(t: Optional[Tensor], shape, dtype: torch.dtype, what: str) -> Optional[Tensor]:
     """A dense per-row operand of the given shape and dtype, or None."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{what} must be {tuple(shape)}, got {tuple(t.shape)}")
-    return t.to(dtype).contiguous()
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
 
 
 def _row_targets(targets: Optional[Tensor], shape, what: str) -> Optional[Tensor]:
@@ -1509,14 +1503,14 @@ def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int =
         raise ValueError(f"logprob: top must be in [0, {min(TOP_MAX, rows.shape[-1])}], got {top}")
     shape = logits.shape[:-1]
     targets = _row_targets(targets, shape, "logprob")
-    a = _lib.LogprobArgs()
-    _row_args(a, rows, _check_temperature(temperature, "logprob"), int(ignore_index))
+    b, l, v = rows.shape
+    a = _lib.LogprobArgs(_LOGPROB_SIZE, _lib.dtype_code(rows.dtype), b, l, v, top,
+                         _check_temperature(temperature, "logprob"), ignore_index, _lib.blx(rows))
     dev = _device_of(logits, targets)
     # tensors of their own, not views of one: autograd refuses in-place work on a node's views
     entropy = empty(shape, device=dev, dtype=torch.float32)
     stats = empty(*shape, 3, device=dev, dtype=torch.float32)
     logp = top_logp = top_ids = None
-    a.top = top
     a.entropy, a.stats = entropy.data_ptr(), stats.data_ptr()
     if targets is not None:
         logp = empty(shape, device=dev, dtype=torch.float32)
@@ -1552,11 +1546,11 @@ def logprob_backward(logits: Tensor, targets: Optional[Tensor], stats: Tensor,
         top = top_ids.shape[-1]
         top_ids = _row_values(top_ids, (*shape, top), torch.int64, "logprob: top_ids")
         dtop_logp = _row_values(dtop_logp, (*shape, top), f32, "logprob: dtop_logp")
-    a = _lib.LogprobArgs()
-    _row_args(a, rows, _check_temperature(temperature, "logprob"), int(ignore_index))
+    b, l, v = rows.shape
+    a = _lib.LogprobArgs(_LOGPROB_SIZE, _lib.dtype_code(rows.dtype), b, l, v, top,
+                         _check_temperature(temperature, "logprob"), ignore_index, _lib.blx(rows))
     dev = _device_of(logits, targets, stats, dlogp, dentropy, dtop_logp, top_ids if top else None)
     dx = empty(logits.shape, device=dev, dtype=logits.dtype)
-    a.top = top
     a.targets, a.stats, a.dlogits = _lib.ptr(targets), stats.data_ptr(), dx.data_ptr()
     a.dlogp, a.dentropy = _lib.ptr(dlogp), _lib.ptr(dentropy)
     if top:
@@ -1574,12 +1568,13 @@ def _distill_args(logits: Tensor, ids: Tensor, teacher: Tensor, targets: Optiona
         raise ValueError(f"distill: between 1 and {TEACHER_MAX} teacher tokens a row, got {k}")
     if ids.dtype not in ID_BYTES:
         raise ValueError(f"distill: teacher_ids must be int32 or int64, got {ids.dtype}")
-    a = _lib.DistillArgs()
-    a.teacher_k, a.id_bytes, a.teacher_dtype = k, ID_BYTES[ids.dtype], _lib.dtype_code(teacher.dtype)
     ids = _row_values(ids, (*shape, k), ids.dtype, "distill: teacher_ids")
     teacher = _row_values(teacher, (*shape, k), teacher.dtype, "distill: teacher_logits")
     targets = _row_targets(targets, shape, "distill")
-    _row_args(a, rows, _check_temperature(temperature, "distill"), int(ignore_index))
+    b, l, v = rows.shape
+    a = _lib.DistillArgs(_DISTILL_SIZE, _lib.dtype_code(rows.dtype), b, l, v, k,
+                         _lib.dtype_code(teacher.dtype), ID_BYTES[ids.dtype],
+                         _check_temperature(temperature, "distill"), ignore_index, _lib.blx(rows))
     dev = _device_of(logits, ids, teacher, targets)
     a.teacher_ids, a.teacher_logits, a.targets = ids.data_ptr(), teacher.data_ptr(), _lib.ptr(targets)
     return a, dev, (rows, ids, teacher, targets)   # the tensors stay alive until the launch
