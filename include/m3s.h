@@ -657,7 +657,7 @@ typedef struct m3s_logprob_args {
   int32_t batch, seqlen; /* rows = batch * seqlen < 2^31 */
   int32_t vocab;         /* < 2^30 */
   int32_t top;           /* 0 .. 64, at most vocab */
-  float temperature;
+  float temperature;     /* in [1e-6, 1e6] */
   int64_t ignore_index;
   m3s_blx logits;        /* (batch, seqlen, vocab), strides >= 0 */
   const int64_t* targets; /* (rows), or NULL: no logp */
@@ -695,7 +695,7 @@ typedef struct m3s_distill_args {
   int32_t teacher_k;     /* 1 .. 256 */
   int32_t teacher_dtype; /* M3S_DTYPE_* of teacher_logits */
   int32_t id_bytes;      /* 4 or 8: int32 or int64 teacher_ids */
-  float temperature;
+  float temperature;     /* in [1e-6, 1e6] */
   int64_t ignore_index;
   m3s_blx logits;        /* (batch, seqlen, vocab), strides >= 0 */
   const void* teacher_ids;    /* (rows, teacher_k) */

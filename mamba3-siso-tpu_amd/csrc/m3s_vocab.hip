@@ -1151,8 +1151,9 @@ static int32_t check_rows(const A* a, const char* who) {
   M3S_REQUIRE(a->batch >= 0 && a->seqlen >= 0 && (int64_t)a->batch * a->seqlen < (1ll << 31),
               "%s: bad row count (%d x %d)", who, a->batch, a->seqlen);
   M3S_REQUIRE(a->vocab > 0 && a->vocab < (1 << 30), "%s: vocab %d must be in [1, 2^30)", who, a->vocab);
-  M3S_REQUIRE(a->temperature > 0.f && a->temperature <= 3.4e38f && 1.f / a->temperature <= 3.4e38f,
-              "%s: temperature must be positive and finite", who);
+  // 1 / T, log2(e) / T and T^2 stay far from float32's ends
+  M3S_REQUIRE(a->temperature >= 0.99e-6f && a->temperature <= 1.01e6f,
+              "%s: temperature must be in [1e-6, 1e6]", who);
   return 0;
 }
 template <typename A>

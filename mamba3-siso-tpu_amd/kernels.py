@@ -1369,15 +1369,14 @@ ID_BYTES = {torch.int32: 4, torch.int64: 8}
 _EMBED_SIZE = ctypes.sizeof(_lib.EmbedArgs)
 
 
-def _embed_args(tokens: Tensor, dtype: torch.dtype, vocab: int, width: int, scale: float,
-                padding_idx: int = -1) -> "_lib.EmbedArgs":
+def _embed_checks(tokens: Tensor, vocab: int, width: int) -> int:
+    """The bytes of an id; the checks that the lookup and its backward share."""
     id_bytes = ID_BYTES.get(tokens.dtype)
     if id_bytes is None:
         raise ValueError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
     if vocab < 1 or width < 1:
         raise ValueError(f"embedding: the table must not be empty, got {(vocab, width)}")
-    return _lib.EmbedArgs(_EMBED_SIZE, _lib.dtype_code(dtype), id_bytes, vocab, width, scale,
-                          tokens.numel(), padding_idx)
+    return id_bytes
 
 
 def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
@@ -1388,13 +1387,17 @@ def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tens
     if table.dim() != 2:
         raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
     v, d = table.shape
-    a = _embed_args(tokens, table.dtype, v, d, scale)
+    id_bytes, code = _embed_checks(tokens, v, d), _lib.dtype_code(table.dtype)
     dev = _device_of(table, tokens)
-    if table.stride(1) != 1 and d > 1:
+    row, col = table.stride()
+    if col != 1 and d > 1:
         table = table.contiguous()
-    tokens = tokens.contiguous()
+        row = d
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
     y = empty(*tokens.shape, d, device=dev, dtype=table.dtype)
-    a.ids, a.table, a.table_stride, a.y = tokens.data_ptr(), table.data_ptr(), table.stride(0), y.data_ptr()
+    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, v, d, scale, tokens.numel(), -1,
+                       tokens.data_ptr(), table.data_ptr(), row, y.data_ptr())
     _lib.launch(_lib.load().m3s_embed_fwd, a, dev, "m3s_embed_fwd")
     return y
 
@@ -1410,18 +1413,18 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
         raise ValueError(f"embedding: dy must be (*tokens.shape, D), got {tuple(dy.shape)} for tokens "
                          f"{tuple(tokens.shape)}")
     d, pad = dy.shape[-1], -1 if padding_idx is None else embedding_padding(padding_idx, vocab)
-    a = _embed_args(tokens, dy.dtype, vocab, d, scale, pad)
+    id_bytes, code = _embed_checks(tokens, vocab, d), _lib.dtype_code(dy.dtype)
     dev = _device_of(tokens, dy)
     tokens, dy = tokens.contiguous(), dy.contiguous()
-    lib = _lib.load()
-    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", tokens.numel(), vocab, d)
+    n = tokens.numel()
+    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", n, vocab, d)
     if nbytes < 0:
-        raise ValueError(f"embedding: bad sizes (tokens {tokens.numel()}, vocab {vocab}, width {d})")
+        raise ValueError(f"embedding: bad sizes (tokens {n}, vocab {vocab}, width {d})")
     dtable = empty(vocab, d, device=dev, dtype=dy.dtype)
     ws = empty(nbytes, device=dev, dtype=torch.uint8)
-    a.ids, a.dy, a.dtable = tokens.data_ptr(), dy.data_ptr(), dtable.data_ptr()
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.launch(lib.m3s_embed_bwd, a, dev, "m3s_embed_bwd")
+    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, vocab, d, scale, n, pad, tokens.data_ptr(), None, 0,
+                       None, dy.data_ptr(), dtable.data_ptr(), ws.data_ptr(), nbytes)
+    _lib.launch(_lib.load().m3s_embed_bwd, a, dev, "m3s_embed_bwd")
     return dtable
 
 
@@ -1448,8 +1451,8 @@ def _logit_rows(logits: Tensor, what: str) -> Tensor:
     if logits.dim() == 3:
         return logits
     if logits.dim() > 3:
-        return logits.reshape(-1, logits.shape[-2], v)
-    return logits.reshape(1, -1, v)
+        return logits.flatten(0, -3)
+    return logits.unsqueeze(0) if logits.dim() == 2 else logits.view(1, 1, v)
 
 
 def _row_values(t: Optional[Tensor], shape, dtype: torch.dtype, what: str) -> Optional[Tensor]:
@@ -1481,8 +1484,8 @@ def _row_scratch(a, dev, entry: str, *sizes: int) -> Optional[Tensor]:
 
 def _check_temperature(temperature: float, what: str) -> float:
     temperature = float(temperature)
-    if not 1e-30 <= temperature <= 1e30:
-        raise ValueError(f"{what}: the temperature must be positive and finite, got {temperature}")
+    if not 1e-6 <= temperature <= 1e6:
+        raise ValueError(f"{what}: the temperature must be in [1e-6, 1e6], got {temperature}")
     return temperature
 
 

@@ -328,9 +328,11 @@ def _embed(table: Tensor, tokens: Tensor) -> Tensor:
     parallel pieces in a fixed order. What that does not take (other dtypes, a forward-mode
     tangent, a trace) goes to ``F.embedding``."""
     if (table.is_cuda and tokens.device == table.device and table.dim() == 2 and table.numel()
-            and table.dtype in (torch.float32, torch.bfloat16) and tokens.dtype in K.ID_BYTES
-            and not torch.jit.is_tracing() and not LY.has_tangent(table)):
-        return TK.embed_tokens(table, tokens)
+            and (table.dtype == torch.float32 or table.dtype == torch.bfloat16)
+            and tokens.dtype in K.ID_BYTES and not torch.jit.is_tracing() and not LY.has_tangent(table)):
+        if torch.is_grad_enabled() and table.requires_grad:
+            return TK.embed_tokens(table, tokens)
+        return K.embedding_forward(table, tokens)
     return F.embedding(tokens, table)
 
 
@@ -385,8 +387,13 @@ def lm_distill_loss(params: LMParams, xs: Tensor, ys: Tensor, teacher_ids: Tenso
     tokens ``teacher_ids`` / ``teacher_logits`` (B, L, K) beside the text."""
     live = ys != ignore_index
     ids = teacher_ids.masked_fill(~live.unsqueeze(-1), -1)
-    out = TK.distill_loss(lm_forward(params, xs, cfg), ids, teacher_logits, temperature, ys, ignore_index)
-    return ((1.0 - hard_weight) * out.kd.sum() + hard_weight * out.nll.sum()) / live.sum()
+    # a part of weight 0 is left out, not multiplied: it may be infinite
+    out = TK.distill_loss(lm_forward(params, xs, cfg), ids, teacher_logits, temperature,
+                          ys if hard_weight != 0.0 else None, ignore_index)
+    total = out.nll.sum() * hard_weight if hard_weight != 0.0 else 0.0
+    if hard_weight != 1.0:
+        total = out.kd.sum() * (1.0 - hard_weight) + total
+    return total / live.sum()
 
 
 def zero_states(cfg: LMConfig, batch: int, dtype=torch.float32, device=None) -> list:

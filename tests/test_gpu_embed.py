@@ -132,6 +132,26 @@ def test_gradient_is_bit_reproducible_and_matches_differences(m3, dev):
     assert abs(slope - want) <= 1e-4 * abs(want) + 1e-3
 
 
+def test_offsets_past_31_bits(m3, dev):
+    """The last rows of a table, and the last tokens, with more than 2^31 entries before them."""
+    gen = torch.Generator().manual_seed(2)
+    vocab, d = 2200000, 1024
+    table = torch.zeros(vocab, d, device=dev, dtype=torch.bfloat16)
+    last = torch.randn(16, d, generator=gen).to(torch.bfloat16).to(dev)
+    table[-16:] = last
+    tokens = (vocab - 16 + torch.arange(16)).to(dev)
+    assert torch.equal(m3.embed_tokens(table, tokens), last)
+    dw = m3.kernels.embedding_backward(tokens, last, vocab)
+    assert torch.equal(dw[-16:], last) and not dw[:1000].any() and not dw[-1000:-16].any()
+    del table, dw
+    tokens = torch.zeros(vocab, dtype=torch.int32, device=dev)
+    tokens[-16:] = 1 + torch.arange(16, device=dev)
+    y = m3.embed_tokens(last.repeat(2, 1)[:17].contiguous(), tokens)
+    assert torch.equal(y[-16:], last.repeat(2, 1)[1:17]) and torch.equal(y[0], last[0])
+    dw = m3.kernels.embedding_backward(tokens, y, 17, padding_idx=0)
+    assert not dw[0].any() and torch.equal(dw[1:], y[-16:])
+
+
 def test_strides_broadcast_cotangents_and_views(m3, dev):
     """A table that is a slice of a wider one, tokens that are a strided view, and a cotangent
     that is broadcast."""

@@ -243,8 +243,14 @@ def test_shapes_strides_and_types(m3, dev):
         ref = T(xc, t, top=3)
         (dc,) = torch.autograd.grad(ref.logp.sum() + ref.top_logp.sum(), xc)
         assert torch.equal(dx, dc)
-    e = T(full[:0], targets[:0], top=2)
-    assert e.logp.shape == (0, 7) and e.top_ids.shape == (0, 7, 2)
+    for shape in ((0, 7, 301), (3, 0, 301), (0, 301), (2, 3, 0, 301), (0, 2, 3, 301)):
+        x = full.new_zeros(shape).requires_grad_(True)
+        t = targets.new_zeros(shape[:-1])
+        e = T(x, t, top=2)
+        assert e.logp.shape == shape[:-1] and e.top_ids.shape == (*shape[:-1], 2)
+        d = m3.distill_loss(x, e.top_ids, e.top_logp.detach(), targets=t)
+        (dx,) = torch.autograd.grad(e.logp.sum() + d.kd.sum() + d.nll.sum(), x)
+        assert dx.shape == shape
     only = T(full, top=4)
     assert only.logp is None and torch.equal(only.top_ids, T(full, targets, top=4).top_ids)
     out = T(full.requires_grad_(True), targets)
@@ -387,6 +393,33 @@ def test_distillation_of_hard_rows(m3, dev, vocab):
     for temp in (1.0, 3.0):
         check_distill(m3, dev, x, ids, teacher, targets, temp)
         check_distill(m3, dev, x, ids, teacher, None, temp)
+
+
+def test_offsets_past_31_bits(m3, dev):
+    """The last rows of logits with more than 2^31 entries equal the same rows on their own."""
+    gen = torch.Generator().manual_seed(3)
+    rows, v = 68000, 32000
+    x = torch.zeros(rows, v, device=dev, dtype=torch.bfloat16)
+    last = make_logits((8, v), torch.bfloat16, gen).to(dev)
+    x[-8:] = last
+    t = torch.randint(0, v, (rows,), generator=gen).to(dev)
+    t[:-8] = -100
+    ids = torch.randint(0, v, (rows, 4), generator=gen).to(dev)
+    ids[:-8] = -1
+    u = torch.randn(rows, 4, generator=gen).to(dev)
+    g = torch.randn(rows, generator=gen).to(dev)
+    K = m3.kernels
+    for part, whole in zip(K.logprob_forward(last, t[-8:], top=5), K.logprob_forward(x, t, top=5)):
+        # whole rows and cut ones sum in another order
+        assert (part.double() - whole[-8:].double()).abs().max().item() <= 1e-4 * part.double().abs().max().item()
+    stats = K.logprob_forward(x, t)[4]
+    dx = K.logprob_backward(x, t, stats, dlogp=g, dentropy=g)
+    assert torch.equal(dx[-8:], K.logprob_backward(last, t[-8:], stats[-8:], dlogp=g[-8:], dentropy=g[-8:]))
+    assert not dx[:64].any()
+    kd, nll, stats = K.distill_forward(x, ids, u, t, 2.0)
+    assert kd[-8:].isfinite().all() and (kd[-8:] != 0).all() and not kd[:-8].any()
+    dx = K.distill_backward(x, ids, u, t, stats, g, g, 2.0)
+    assert torch.equal(dx[-8:], K.distill_backward(last, ids[-8:], u[-8:], t[-8:], stats[-8:], g[-8:], g[-8:], 2.0))
 
 
 def test_gradients_match_differences(m3, dev):
@@ -555,5 +588,9 @@ def test_model_scores_and_distillation_step(m3, dev):
     assert torch.equal(got_loss, ref_loss)
     assert all(torch.equal(a, b) for a, b in zip(M.lm_leaves(p), M.lm_leaves(q)))
     assert any(not torch.equal(a, b) for a, b in zip(M.lm_leaves(p), first))
+    # a part of weight 0 is not there at all, as where the student rules a teacher's token out
+    for weight, part in ((0.0, kd.mean()), (1.0, torch.nn.functional.cross_entropy(x[live], ys[live]))):
+        only = M.lm_distill_loss(TR.train_params(student), xs, ys, best.top_ids, best.top_logp, cfg, 2.0, weight)
+        assert abs(only.item() - part.item()) <= 1e-5 * abs(part.item())
     with pytest.raises(ValueError, match="vocabulary"):
         TR.make_distill_step(cfg, opt, teacher, M.LMConfig(vocab_size=41, n_layers=1, siso=siso))
