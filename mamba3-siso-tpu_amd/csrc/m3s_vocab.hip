@@ -616,8 +616,14 @@ struct LogprobRow {   // from finished sums
   __device__ float operator()(float v) const { return empty ? kNegInf : (v - m) * inv_t - logs; }
 };
 
-template <typename G, typename T>
-__device__ __forceinline__ void logprob_store(const LogprobParams& p, int64_t r, int64_t tgt, const T* x,
+// The target's logit (NaN where there is none), loaded ahead of the row.
+template <typename T>
+__device__ __forceinline__ float target_logit(const LogprobParams& p, int64_t tgt, const T* x) {
+  return p.targets && tgt >= 0 && tgt < p.vocab ? (float)x[tgt] : __builtin_nanf("");
+}
+
+template <typename G>
+__device__ __forceinline__ void logprob_store(const LogprobParams& p, int64_t r, int64_t tgt, float xt,
                                               const RowSums<kEntropy>& sum, const LogprobRow& logp) {
   if (G::tid() != 0) return;
   const float h = logp.empty ? 0.f : logp.logs - sum.t * p.inv_t / sum.s;
@@ -625,7 +631,7 @@ __device__ __forceinline__ void logprob_store(const LogprobParams& p, int64_t r,
   p.stats[3 * r] = sum.m;
   p.stats[3 * r + 1] = sum.s;
   p.stats[3 * r + 2] = h;
-  if (p.targets) p.logp[r] = tgt >= 0 && tgt < p.vocab ? logp((float)x[tgt]) : __builtin_nanf("");
+  if (p.targets) p.logp[r] = tgt >= 0 && tgt < p.vocab ? logp(xt) : __builtin_nanf("");
 }
 
 // NaN or +inf among the logits: no order to report.
@@ -650,12 +656,13 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
       continue;
     }
     const T* x = row_at<T>(p.logits, r, p.seqlen);
+    const float xt = target_logit(p, tgt, x);
     RowSums<kEntropy> sum;
     Best best;
     row_pass<G, U, PICK && NT == 256>(sum, best, x, p.vocab, p.c, 0.f);
     sum.template join<G>(p.c, 0.f, tmp);
     const LogprobRow logp(sum, p.inv_t);
-    logprob_store<G>(p, r, tgt, x, sum, logp);
+    logprob_store<G>(p, r, tgt, xt, sum, logp);
     if constexpr (TOP) {
       if (sum.s != sum.s) {
         logprob_unordered<G>(p, r);
@@ -722,6 +729,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
     logprob_skip<G>(p, r);
     return;
   }
+  const float xt = target_logit(p, tgt, row_at<T>(p.logits, r, p.seqlen));
   const LogprobParts part(p, r);
   RowSums<kEntropy> sum;
   if ((int)threadIdx.x < p.split) {
@@ -731,7 +739,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
   }
   sum.template join<G>(p.c, 0.f, tmp);
   const LogprobRow logp(sum, p.inv_t);
-  logprob_store<G>(p, r, tgt, row_at<T>(p.logits, r, p.seqlen), sum, logp);
+  logprob_store<G>(p, r, tgt, xt, sum, logp);
   if constexpr (TOP) {
     if (sum.s != sum.s) {
       logprob_unordered<G>(p, r);
