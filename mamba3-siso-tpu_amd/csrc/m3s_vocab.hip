@@ -31,9 +31,14 @@ namespace m3s {
 constexpr int kRowThreads = 256;
 constexpr int kTopMax = 64;        // alternatives of a row
 constexpr int kTeacherMax = 256;   // teacher tokens of a row
-// Rows up to kPartVocab long go to 16 lanes each, up to kWaveVocab to a wave, longer ones to a
-// workgroup.
-constexpr int kPartVocab = 512, kWaveVocab = 1024;
+// The threads to a row, by measurement (us, forward / backward of the distillation with 16 teacher
+// tokens and a target, float32): many short rows go to 16 lanes each, as what is done once a row
+// then costs a quarter (20971 x 400: 9.9 / 20 against 21 / 23 by a wave, 8192 x 1000: 8.9 / 17
+// against 10.5 / 16.5; but 2048 x 1000: 5.1 / 7.1 against 4.4 / 6.6); rows up to 1024, and many up to
+// 4096, to a wave (2048 x 1000: 4.4 / 6.6 against 8.7 / 8.1 by a workgroup, 4096 x 2000: 8.8 / 16
+// against 15.6 / 16; but 512 x 4000: 5.2 / 6.0 against 4.9 / 6.0); the rest to a workgroup.
+constexpr int kPartVocab = 1024, kPartRows = 4096, kWaveVocab = 4096, kWaveRows = 1024;
+constexpr int kWaveHeld = 1024;     // one batch of a wave holds the row: it goes to one whatever the rows
 constexpr int kPartTop = 16;        // alternatives that 16 lanes pick, of rows up to kPartPick long
 constexpr int kPartPick = 256;
 constexpr int kPartTeacher = 64;    // teacher tokens of a row of 16 lanes
@@ -1172,8 +1177,9 @@ static int32_t check_logits(const A* a, const char* who) {
   return 0;
 }
 // The threads to a row: `part` says that 16 lanes can do the call at all.
-static int row_threads(int vocab, bool part) {
-  return part && vocab <= kPartVocab ? 16 : vocab <= kWaveVocab ? 64 : 256;
+static int row_threads(int64_t rows, int vocab, bool part) {
+  if (part && vocab <= kPartVocab && rows >= kPartRows) return 16;
+  return vocab <= kWaveHeld || (vocab <= kWaveVocab && rows >= kWaveRows) ? 64 : 256;
 }
 static int vocab_chunks(int vocab, int dtype, int nt) {
   const int chunk = nt * kBwdPieces * (dtype == M3S_DTYPE_BF16 ? Piece<bf16>::N : Piece<float>::N);
@@ -1274,7 +1280,8 @@ static void launch_logprob_fwd(const LogprobParams& p, hipStream_t s) {
     launch_kernel(logprob_join_kernel<TOP, T>, p.rows, p, s);
     return;
   }
-  const int nt = row_threads(p.vocab, !TOP || (p.top <= kPartTop && p.vocab <= kPartPick));
+  int nt = row_threads(p.rows, p.vocab, !TOP || (p.top <= kPartTop && p.vocab <= kPartPick));
+  if (TOP && p.vocab > kWaveHeld) nt = 256;   // a wave picks alternatives of a row that it holds
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
     const int64_t blocks = (p.rows + ROWS - 1) / ROWS;
@@ -1290,14 +1297,14 @@ static void launch_distill_fwd(const DistillParams& p, hipStream_t s) {
     launch_kernel(distill_join_kernel<MODE, T>, p.rows, p, s);
     return;
   }
-  with_group(row_threads(p.vocab, p.k <= kPartTeacher), [&](auto g) {
+  with_group(row_threads(p.rows, p.vocab, p.k <= kPartTeacher), [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
     launch_kernel(distill_fwd_kernel<MODE, NT, U, T>, (p.rows + ROWS - 1) / ROWS, p, s);
   });
 }
 template <typename T>
 static void launch_logprob_bwd(LogprobParams& p, int dtype, hipStream_t s) {
-  const int nt = row_threads(p.vocab, true);
+  const int nt = row_threads(p.rows, p.vocab, true);
   p.chunks = vocab_chunks(p.vocab, dtype, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
@@ -1306,7 +1313,7 @@ static void launch_logprob_bwd(LogprobParams& p, int dtype, hipStream_t s) {
 }
 template <bool DUAL, typename T>
 static void launch_distill_bwd(DistillParams& p, int dtype, hipStream_t s) {
-  const int nt = row_threads(p.vocab, p.k <= kPartTeacher);
+  const int nt = row_threads(p.rows, p.vocab, p.k <= kPartTeacher);
   p.chunks = vocab_chunks(p.vocab, dtype, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;

@@ -193,7 +193,8 @@ def test_logprobs_of_hard_rows(m3, dev, dtype, kind, vocab):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("rows,vocab", [(600, 9001), (130, 20003), (2100, 700), (10, 260)])
+@pytest.mark.parametrize("rows,vocab", [(600, 9001), (130, 20003), (2100, 700), (10, 260), (4200, 250), (4500, 1001),
+                                        (1100, 2049)])
 def test_whole_rows_of_hard_kinds(m3, dev, dtype, rows, vocab):
     """Enough rows that none is cut: masks, ties, flat rows, empty ones and ordinary ones together,
     and rows whose best logits all lie at the places of few threads."""
@@ -206,8 +207,8 @@ def test_whole_rows_of_hard_kinds(m3, dev, dtype, rows, vocab):
     x[8] = torch.where(place == 3, 5.0, -INF)
     targets = torch.randint(0, vocab, (len(x),), generator=gen)
     targets[::11] = -100
-    for top in (1, 20, 64):
-        check_logprob(m3, dev, x, targets, top, 1.0, ("lht",) if top == 20 else ())
+    for top in (0, 1, 16, 20, 64):
+        check_logprob(m3, dev, x, targets, top, 1.0, ("lht",) if top in (0, 20) else ())
 
 
 def test_one_thread_holds_the_best(m3, dev):
@@ -353,7 +354,9 @@ def teacher_of(x, k, gen, dtype):
     (3, 1, 1, 1.0, torch.float32, torch.int64), (5, 9, 3, 2.0, torch.float32, torch.int32),
     (40, 256, 16, 2.0, torch.float32, torch.int64), (7, 257, 64, 1.0, torch.bfloat16, torch.int64),
     (4, 1000, 100, 0.5, torch.float32, torch.int32), (3, 5003, 256, 4.0, torch.float32, torch.int64),
-    (2, 50001, 32, 2.0, torch.bfloat16, torch.int32), (300, 130, 7, 1.0, torch.float32, torch.int64)])
+    (2, 50001, 32, 2.0, torch.bfloat16, torch.int32), (300, 130, 7, 1.0, torch.float32, torch.int64),
+    (4500, 131, 16, 2.0, torch.float32, torch.int64), (4100, 999, 64, 1.0, torch.bfloat16, torch.int32),
+    (4100, 300, 65, 2.0, torch.float32, torch.int64), (1200, 2050, 9, 3.0, torch.float32, torch.int64)])
 def test_distillation_and_gradients(m3, dev, dtype, rows, vocab, k, temp, tdt, idt):
     gen = torch.Generator().manual_seed(rows * 31 + vocab)
     x = make_logits((rows, vocab), dtype, gen)
@@ -363,8 +366,8 @@ def test_distillation_and_gradients(m3, dev, dtype, rows, vocab, k, temp, tdt, i
     check_distill(m3, dev, x, ids.to(idt), teacher, None, temp)
 
 
-@pytest.mark.parametrize("vocab", [50, 3001, 20011])
-def test_distillation_of_hard_rows(m3, dev, vocab):
+@pytest.mark.parametrize("vocab,repeat", [(50, 1), (3001, 1), (20011, 1), (61, 300), (1003, 260), (2055, 70)])
+def test_distillation_of_hard_rows(m3, dev, vocab, repeat):
     """Rows without entries, entries of weight zero, ids named twice, ids and targets outside the
     vocabulary, ignored targets, empty student rows, NaN and infinities on either side, and garbage
     logits where there is nothing to learn."""
@@ -390,6 +393,8 @@ def test_distillation_of_hard_rows(m3, dev, vocab):
     teacher[13, 1] = INF
     x[14, ids[14, 0]] = -INF                      # the student rules the teacher's best out
     x[15, 0] = INF
+    # as often as it takes for the calls of many rows
+    x, ids, teacher, targets = (t.repeat(repeat, *[1] * (t.dim() - 1)) for t in (x, ids, teacher, targets))
     for temp in (1.0, 3.0):
         check_distill(m3, dev, x, ids, teacher, targets, temp)
         check_distill(m3, dev, x, ids, teacher, None, temp)
