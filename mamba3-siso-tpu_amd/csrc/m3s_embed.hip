@@ -22,6 +22,12 @@
 //
 // Every sum is float32 in a fixed order, rounded once. The gradient reads dy once and writes the
 // table once (a row that occurs twice): bound by HBM from a few MB on, by the launches below that.
+//
+// Measured: 32768 byte tokens (Zipf), D 768, float32: lookup 17.9 us (5.6 TB/s of output), gradient
+// 33 us, of which run_sum 18 (5.6 TB/s of dy), the sort 8 and finish 6. 16384 tokens of 50001, D 1024:
+// gradient 61 us, of which clearing 205 MB beside the four sort launches takes 36 (5.7 TB/s) and
+// run_sum 20 to 25; cleared by a pass of its own behind the sort it took 96 in all. 777 tokens of
+// 32003, D 515, bf16: 16 us, three launches.
 #include <algorithm>
 
 #include "m3s_common.h"
@@ -35,7 +41,10 @@ constexpr int kDigitBits = 9;
 constexpr int kSortOne = 4096;        // tokens that one workgroup sorts alone, in LDS
 constexpr int kSortRounds = kSortOne / kSortThreads;
 constexpr int kSortBlocks = 64;       // workgroups of a larger sort, at most
-constexpr int64_t kRunWaves = 2048;   // waves of run_sum that make its pieces longer
+// Waves of run_sum that make its pieces longer: longer pieces leave fewer partials, shorter ones more
+// waves. The whole gradient at 32768 x 768 (3072 waves of 32 rows) 39 us so, 45 and 56 with pieces of
+// 16 and 8; at 16384 x 1024 (2048 waves) 65 against 68 and 78.
+constexpr int64_t kRunWaves = 2048;
 
 // W columns of a row, at any element alignment (gfx950 takes wide accesses there): 8 or 4 of bf16, 4
 // of float32, or one of a row narrower than that. Lanes take W columns each and the last one steps back to the

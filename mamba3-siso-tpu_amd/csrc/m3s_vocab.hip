@@ -20,6 +20,13 @@
 // m + log s, whose rounding would shift a whole row of p).
 //
 // Rows may start at any element: 16-byte accesses need no alignment on gfx950.
+//
+// Measured (us; TB/s of logits read and gradients written): log-probability and entropy of 8192 x
+// 32000 float32, a tenth of it padding, forward 191 (4.9), backward 330 (6.0); distillation of 8192 x
+// 50001 float32 with 32 teacher tokens and the cross-entropy, forward 253 (5.8), backward 490 (6.4);
+// of 2048 x 65536 bf16, 59 (4.5) and 105 (5.1): there the exponentials take as long as the bytes. A
+// large copy moves 5.0 TB/s. 32768 x 256 float32, 16 teacher tokens: 11.3 and 18.2, what is done once
+// a row (sums over lanes, logarithms, the entries) taking half of it.
 #include <algorithm>
 #include <type_traits>
 
@@ -468,7 +475,9 @@ __device__ __forceinline__ void values_out(const T* __restrict__ x, int n, int k
 }
 
 // out(rank, value, index) for the k largest of n logits (k <= n, no NaN, no +inf, the largest
-// `top`), equal ones by index. By a workgroup: a bound that k of the threads' maxima reach is
+// `top`), equal ones by index. Measured, on top of the pass over the row: 999 rows of 50001 bf16 21 us,
+// with 1, 20 and 64 alternatives 25, 26 and 31 (by a bound's ties in a list built with one atomic a
+// logit, and ranked value by value, 27, 43 and 53; by rounds of arg-max, 64 took 5 ms). By a workgroup: a bound that k of the threads' maxima reach is
 // reached by at least k logits, and by hardly more; those are collected from the few batches that
 // hold them and ranked against each other.
 template <typename G, int U, typename T, typename OUT>
@@ -544,7 +553,9 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
   G::sync();
 }
 
-// The same by 16 lanes that hold the row's at most kPartPick logits, one round for each of few.
+// The same by 16 lanes that hold the row's at most kPartPick logits, one round for each of few:
+// 32768 x 256 with 1, 5 and 8 alternatives 9.7, 15 and 19 us, and 6.9 without; a wave's bound and list
+// take 29 for 20.
 template <typename G, typename T, typename OUT>
 __device__ __forceinline__ void pick_few(const T* __restrict__ x, int n, int k, OUT&& out) {
   constexpr int N = Piece<T>::N, U = kPartPick / (G::NT * N), LEN = U * N;
@@ -1195,7 +1206,8 @@ static int row_period(const A* a) {
 static int row_share(int vocab, int split) { return ((vocab + split - 1) / split + 7) / 8 * 8; }
 // Pieces to a row: where the rows alone leave most of the 256 CUs idle, enough for two workgroups
 // to each, of at least kPieceMin logits; with alternatives the pieces' best together stay within
-// what the joining workgroup ranks. 1: whole rows.
+// what the joining workgroup ranks. 1: whole rows. 37 rows of 50001: distillation forward 17 us whole,
+// 8 cut; one row of 131072 with 20 alternatives 10 us cut, in two launches of 3 to 6.
 constexpr int kPieceMin = 4096, kSplitMax = 64;
 static int row_split(int64_t rows, int vocab, int top) {
   int64_t split = std::min<int64_t>({512 / std::max<int64_t>(rows, 1), vocab / kPieceMin, kSplitMax});
