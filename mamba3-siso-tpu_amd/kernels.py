@@ -1379,11 +1379,32 @@ def _embed_checks(tokens: Tensor, vocab: int, width: int) -> int:
     return id_bytes
 
 
-def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
-    """``scale * table[tokens]`` (one ``m3s_embed_fwd`` launch; the lookup of
-    ``model.py:194-232``): ``table`` (V, D) float32 or bf16 with any row stride, ``tokens`` int32
-    or int64 of any shape. The result is in the table's dtype, the product formed in float32. An
-    id outside [0, V) gives a row of NaN (no host synchronisation checks it)."""
+def _row_grad(t: Optional[Tensor]) -> Optional[Tensor]:
+    """A cotangent that autograd hands a node, dense."""
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+class Call(NamedTuple):
+    """A launched forward call as its autograd node keeps it: the args struct, the device, and the
+    addresses of the operands that the node saves. The backward runs on a thread of its own, whose
+    core finds every Python object in another's cache (a forward and backward of 64 rows: 120 us
+    with the operands checked anew, 90 so), so it fills in a copy of the struct instead."""
+
+    args: ctypes.Structure
+    device: torch.device
+    addresses: tuple
+
+    def again(self, tensors):
+        """A copy of the struct, or None where a saved tensor came back at another address (hooks
+        on saved tensors may do that) or the call had read a copy of it."""
+        for t, at in zip(tensors, self.addresses):
+            if (t.data_ptr() or None if t is not None else None) != at:
+                return None
+        return type(self.args).from_buffer_copy(self.args)
+
+
+def embedding_call(table: Tensor, tokens: Tensor, scale: float, padding_idx: int = -1):
+    """`embedding_forward` with its `Call` and the dense tokens that the call read."""
     if table.dim() != 2:
         raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
     v, d = table.shape
@@ -1396,10 +1417,33 @@ def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tens
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     y = empty(*tokens.shape, d, device=dev, dtype=table.dtype)
-    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, v, d, scale, tokens.numel(), -1,
+    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, v, d, scale, tokens.numel(), padding_idx,
                        tokens.data_ptr(), table.data_ptr(), row, y.data_ptr())
     _lib.launch(_lib.load().m3s_embed_fwd, a, dev, "m3s_embed_fwd")
-    return y
+    return y, tokens, Call(a, dev, (a.ids,))
+
+
+def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
+    """``scale * table[tokens]`` (one ``m3s_embed_fwd`` launch; the lookup of
+    ``model.py:194-232``): ``table`` (V, D) float32 or bf16 with any row stride, ``tokens`` int32
+    or int64 of any shape. The result is in the table's dtype, the product formed in float32. An
+    id outside [0, V) gives a row of NaN (no host synchronisation checks it)."""
+    return embedding_call(table, tokens, scale)[0]
+
+
+def embedding_call_backward(a: "_lib.EmbedArgs", dev: torch.device, dy: Tensor) -> Tensor:
+    """`embedding_backward` by a copy of the forward's struct (`Call.again`)."""
+    dy = _row_grad(dy)
+    v, d, n = a.vocab, a.width, a.tokens
+    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", n, v, d)
+    if nbytes < 0:
+        raise ValueError(f"embedding: bad sizes (tokens {n}, vocab {v}, width {d})")
+    dtable = empty(v, d, device=dev, dtype=dy.dtype)
+    ws = empty(nbytes, device=dev, dtype=torch.uint8)
+    a.dy, a.dtable = dy.data_ptr(), dtable.data_ptr()
+    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _lib.launch(_lib.load().m3s_embed_bwd, a, dev, "m3s_embed_bwd")
+    return dtable
 
 
 def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.0,
@@ -1415,17 +1459,9 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
     d, pad = dy.shape[-1], -1 if padding_idx is None else embedding_padding(padding_idx, vocab)
     id_bytes, code = _embed_checks(tokens, vocab, d), _lib.dtype_code(dy.dtype)
     dev = _device_of(tokens, dy)
-    tokens, dy = tokens.contiguous(), dy.contiguous()
-    n = tokens.numel()
-    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", n, vocab, d)
-    if nbytes < 0:
-        raise ValueError(f"embedding: bad sizes (tokens {n}, vocab {vocab}, width {d})")
-    dtable = empty(vocab, d, device=dev, dtype=dy.dtype)
-    ws = empty(nbytes, device=dev, dtype=torch.uint8)
-    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, vocab, d, scale, n, pad, tokens.data_ptr(), None, 0,
-                       None, dy.data_ptr(), dtable.data_ptr(), ws.data_ptr(), nbytes)
-    _lib.launch(_lib.load().m3s_embed_bwd, a, dev, "m3s_embed_bwd")
-    return dtable
+    tokens = tokens.contiguous()
+    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, vocab, d, scale, tokens.numel(), pad, tokens.data_ptr())
+    return embedding_call_backward(a, dev, dy)
 
 
 def embedding_padding(padding_idx: int, vocab: int) -> int:
@@ -1489,24 +1525,17 @@ def _check_temperature(temperature: float, what: str) -> float:
     return temperature
 
 
-def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int = 0,
-                    temperature: float = 1.0, ignore_index: int = -100):
-    """Log-probabilities read off ``logits`` (..., V), float32 or bf16 (``m3s_logprob_fwd``):
-    ``(logp, entropy, top_logp, top_ids, stats)``. ``logp`` (...,) is ``log softmax(logits / T)``
-    at ``targets`` (...,), ``entropy`` that distribution's, ``top_logp`` / ``top_ids`` (..., top)
-    its best ids in falling order (equal logits: the lower id first). ``logp`` is None without
-    targets, the two last None with ``top`` 0; ``stats`` (..., 3) is `logprob_backward`'s.
-
-    Rows whose target is ``ignore_index`` are not read: logp and entropy 0, ids -1, top_logp -inf.
-    Another target outside [0, V) gives NaN. A row of nothing but -inf has logp -inf, entropy 0; a
-    row with NaN or +inf is NaN throughout, with ids -1."""
+def logprob_call(logits: Tensor, targets: Optional[Tensor], top: int, temperature: float,
+                 ignore_index: int):
+    """`logprob_forward` with its `Call`, on ``(logits, targets, stats, top_ids)``, and the targets
+    that the call read."""
     rows = _logit_rows(logits, "logprob")
+    b, l, v = rows.shape
     top = int(top)
-    if not 0 <= top <= min(TOP_MAX, rows.shape[-1]):
-        raise ValueError(f"logprob: top must be in [0, {min(TOP_MAX, rows.shape[-1])}], got {top}")
+    if not 0 <= top <= min(TOP_MAX, v):
+        raise ValueError(f"logprob: top must be in [0, {min(TOP_MAX, v)}], got {top}")
     shape = logits.shape[:-1]
     targets = _row_targets(targets, shape, "logprob")
-    b, l, v = rows.shape
     a = _lib.LogprobArgs(_LOGPROB_SIZE, _lib.dtype_code(rows.dtype), b, l, v, top,
                          _check_temperature(temperature, "logprob"), ignore_index, _lib.blx(rows))
     dev = _device_of(logits, targets)
@@ -1522,9 +1551,35 @@ def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int =
         top_logp = empty(*shape, top, device=dev, dtype=torch.float32)
         top_ids = empty(*shape, top, device=dev, dtype=torch.int64)
         a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
-    ws = _row_scratch(a, dev, "m3s_logprob_workspace_bytes", shape.numel(), a.vocab, top)  # noqa: F841
+    ws = _row_scratch(a, dev, "m3s_logprob_workspace_bytes", b * l, v, top)  # noqa: F841
     _lib.launch(_lib.load().m3s_logprob_fwd, a, dev, "m3s_logprob_fwd")
-    return logp, entropy, top_logp, top_ids, stats
+    return ((logp, entropy, top_logp, top_ids, stats), targets,
+            Call(a, dev, (a.logits.ptr, a.targets, a.stats, a.top_ids)))
+
+
+def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int = 0,
+                    temperature: float = 1.0, ignore_index: int = -100):
+    """Log-probabilities read off ``logits`` (..., V), float32 or bf16 (``m3s_logprob_fwd``):
+    ``(logp, entropy, top_logp, top_ids, stats)``. ``logp`` (...,) is ``log softmax(logits / T)``
+    at ``targets`` (...,), ``entropy`` that distribution's, ``top_logp`` / ``top_ids`` (..., top)
+    its best ids in falling order (equal logits: the lower id first). ``logp`` is None without
+    targets, the two last None with ``top`` 0; ``stats`` (..., 3) is `logprob_backward`'s.
+
+    Rows whose target is ``ignore_index`` are not read: logp and entropy 0, ids -1, top_logp -inf.
+    Another target outside [0, V) gives NaN. A row of nothing but -inf has logp -inf, entropy 0; a
+    row with NaN or +inf is NaN throughout, with ids -1."""
+    return logprob_call(logits, targets, top, temperature, ignore_index)[0]
+
+
+def logprob_call_backward(a: "_lib.LogprobArgs", dev: torch.device, logits: Tensor, dlogp, dentropy,
+                          dtop_logp) -> Tensor:
+    """`logprob_backward` by a copy of the forward's struct (`Call.again`)."""
+    dlogp, dentropy, dtop_logp = _row_grad(dlogp), _row_grad(dentropy), _row_grad(dtop_logp)
+    dx = empty(logits.shape, device=dev, dtype=logits.dtype)
+    a.dlogp, a.dentropy, a.dtop_logp = _lib.ptr(dlogp), _lib.ptr(dentropy), _lib.ptr(dtop_logp)
+    a.dlogits = dx.data_ptr()
+    _lib.launch(_lib.load().m3s_logprob_bwd, a, dev, "m3s_logprob_bwd")
+    return dx
 
 
 def logprob_backward(logits: Tensor, targets: Optional[Tensor], stats: Tensor,
@@ -1583,6 +1638,25 @@ def _distill_args(logits: Tensor, ids: Tensor, teacher: Tensor, targets: Optiona
     return a, dev, (rows, ids, teacher, targets)   # the tensors stay alive until the launch
 
 
+def distill_call(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
+                 targets: Optional[Tensor], temperature: float, ignore_index: int):
+    """`distill_forward` with its `Call`, on ``(logits, ids, teacher, targets, stats)``, and the
+    three operands between as the call read them."""
+    a, dev, ops = _distill_args(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)
+    shape = logits.shape[:-1]
+    kd = empty(shape, device=dev, dtype=torch.float32)
+    stats = empty(*shape, 5, device=dev, dtype=torch.float32)
+    nll = None
+    a.kd, a.stats = kd.data_ptr(), stats.data_ptr()
+    if targets is not None:
+        nll = empty(shape, device=dev, dtype=torch.float32)
+        a.nll = nll.data_ptr()
+    ws = _row_scratch(a, dev, "m3s_distill_workspace_bytes", a.batch * a.seqlen, a.vocab)  # noqa: F841
+    _lib.launch(_lib.load().m3s_distill_fwd, a, dev, "m3s_distill_fwd")
+    return ((kd, nll, stats), ops[1:],
+            Call(a, dev, (a.logits.ptr, a.teacher_ids, a.teacher_logits, a.targets, a.stats)))
+
+
 def distill_forward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
                     targets: Optional[Tensor] = None, temperature: float = 1.0,
                     ignore_index: int = -100):
@@ -1594,18 +1668,16 @@ def distill_forward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
     An entry with an id < 0 does not count, one with logit -inf has weight 0, a repeated id adds
     up. A row without entries has kd 0, one with target ``ignore_index`` nll 0; with neither it is
     not read. An id >= V and another target outside [0, V) give NaN."""
-    a, dev, keep = _distill_args(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)
-    shape = logits.shape[:-1]
-    kd = empty(shape, device=dev, dtype=torch.float32)
-    stats = empty(*shape, 5, device=dev, dtype=torch.float32)
-    nll = None
-    a.kd, a.stats = kd.data_ptr(), stats.data_ptr()
-    if targets is not None:
-        nll = empty(shape, device=dev, dtype=torch.float32)
-        a.nll = nll.data_ptr()
-    ws = _row_scratch(a, dev, "m3s_distill_workspace_bytes", shape.numel(), a.vocab)  # noqa: F841
-    _lib.launch(_lib.load().m3s_distill_fwd, a, dev, "m3s_distill_fwd")
-    return kd, nll, stats
+    return distill_call(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)[0]
+
+
+def distill_call_backward(a: "_lib.DistillArgs", dev: torch.device, logits: Tensor, dkd, dnll) -> Tensor:
+    """`distill_backward` by a copy of the forward's struct (`Call.again`)."""
+    dkd, dnll = _row_grad(dkd), _row_grad(dnll)
+    dx = empty(logits.shape, device=dev, dtype=logits.dtype)
+    a.dkd, a.dnll, a.dlogits = _lib.ptr(dkd), _lib.ptr(dnll), dx.data_ptr()
+    _lib.launch(_lib.load().m3s_distill_bwd, a, dev, "m3s_distill_bwd")
+    return dx
 
 
 def distill_backward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,

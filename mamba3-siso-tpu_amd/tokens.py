@@ -34,15 +34,20 @@ class _EmbedFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, table, tokens, scale, padding_idx):
+        y, tokens, ctx.call = K.embedding_call(table, tokens, scale, padding_idx)
         ctx.save_for_backward(tokens)
-        ctx.vocab, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
-        return K.embedding_forward(table, tokens, scale)
+        return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         (tokens,) = ctx.saved_tensors
-        return K.embedding_backward(tokens, dy, ctx.vocab, ctx.scale, ctx.padding_idx), None, None, None
+        a = ctx.call.again((tokens,))
+        if a is None:
+            a = ctx.call.args
+            return K.embedding_backward(tokens, dy, a.vocab, a.scale,
+                                        a.padding_idx if a.padding_idx >= 0 else None), None, None, None
+        return K.embedding_call_backward(a, ctx.call.device, dy), None, None, None
 
 
 def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
@@ -53,10 +58,9 @@ def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
     The gradient is dense, summed in float32 in position order and so bit-reproducible.
     ``padding_idx`` names an id (negative: from the end) whose row is looked up but gets no
     gradient. An id outside [0, V) gives a row of NaN, and no gradient."""
-    if padding_idx is not None:
-        padding_idx = K.embedding_padding(int(padding_idx), table.shape[0])
+    pad = -1 if padding_idx is None else K.embedding_padding(int(padding_idx), table.shape[0])
     if _needs_node(table):
-        return _EmbedFn.apply(table, tokens, float(scale), padding_idx)
+        return _EmbedFn.apply(table, tokens, float(scale), pad)
     return K.embedding_forward(table, tokens, scale)
 
 
@@ -75,10 +79,10 @@ class _LogprobFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, targets, top, temperature, ignore_index):
-        logp, entropy, top_logp, top_ids, stats = K.logprob_forward(logits, targets, top, temperature,
-                                                                    ignore_index)
+        out, targets, ctx.call = K.logprob_call(logits, targets, top, temperature, ignore_index)
+        logp, entropy, top_logp, top_ids, stats = out
         ctx.save_for_backward(logits, targets, stats, top_ids)
-        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         if top_ids is not None:
             ctx.mark_non_differentiable(top_ids)
@@ -89,9 +93,13 @@ class _LogprobFn(torch.autograd.Function):
     def backward(ctx, dlogp, dentropy, dtop_logp, _):
         if dlogp is None and dentropy is None and dtop_logp is None:
             return None, None, None, None, None
-        logits, targets, stats, top_ids = ctx.saved_tensors
-        dx = K.logprob_backward(logits, targets, stats, top_ids, dlogp, dentropy, dtop_logp,
-                                ctx.temperature, ctx.ignore_index)
+        saved = logits, targets, stats, top_ids = ctx.saved_tensors
+        a = ctx.call.again(saved)
+        if a is not None:
+            dx = K.logprob_call_backward(a, ctx.call.device, logits, dlogp, dentropy, dtop_logp)
+        else:
+            dx = K.logprob_backward(logits, targets, stats, top_ids, dlogp, dentropy, dtop_logp,
+                                    ctx.temperature, ctx.call.args.ignore_index)
         return dx, None, None, None, None
 
 
@@ -126,9 +134,10 @@ class _DistillFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, targets, temperature, ignore_index):
-        kd, nll, stats = K.distill_forward(logits, ids, teacher, targets, temperature, ignore_index)
-        ctx.save_for_backward(logits, ids, teacher, targets, stats)
-        ctx.temperature, ctx.ignore_index = temperature, ignore_index
+        (kd, nll, stats), ops, ctx.call = K.distill_call(logits, ids, teacher, targets, temperature,
+                                                         ignore_index)
+        ctx.save_for_backward(logits, *ops, stats)
+        ctx.temperature = temperature
         ctx.set_materialize_grads(False)
         return kd, nll
 
@@ -137,9 +146,13 @@ class _DistillFn(torch.autograd.Function):
     def backward(ctx, dkd, dnll):
         if dkd is None and dnll is None:
             return None, None, None, None, None, None
-        logits, ids, teacher, targets, stats = ctx.saved_tensors
-        dx = K.distill_backward(logits, ids, teacher, targets, stats, dkd, dnll, ctx.temperature,
-                                ctx.ignore_index)
+        saved = logits, ids, teacher, targets, stats = ctx.saved_tensors
+        a = ctx.call.again(saved)
+        if a is not None:
+            dx = K.distill_call_backward(a, ctx.call.device, logits, dkd, dnll)
+        else:
+            dx = K.distill_backward(logits, ids, teacher, targets, stats, dkd, dnll, ctx.temperature,
+                                    ctx.call.args.ignore_index)
         return dx, None, None, None, None, None
 
 

@@ -528,6 +528,53 @@ def test_runs_are_bit_reproducible(m3, dev):
         assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
+def test_backward_of_saved_tensors_elsewhere_and_twice(m3, dev):
+    """Saved operands that come back at other addresses (kept in host memory meanwhile), operands
+    that the forward read as copies, a graph kept for a second backward, and broadcast cotangents:
+    the same gradients as the bare calls."""
+    gen = torch.Generator().manual_seed(21)
+    x = make_logits((6, 300), torch.float32, gen).to(dev)
+    t = torch.randint(0, 300, (6,), generator=gen).to(dev)
+    ids, u = (a.to(dev) for a in teacher_of(x.cpu(), 8, gen, torch.float32))
+    table = torch.randn(40, 16, generator=gen).to(dev)
+    tokens = torch.randint(0, 40, (30, 6), generator=gen).to(dev)
+    K = m3.kernels
+    one = torch.ones(6, device=dev)
+    stats, kstats = K.logprob_forward(x, t, top=4), K.distill_forward(x, ids, u, t, 2.0)[2]
+    want = (K.logprob_backward(x, t, stats[4], stats[3], one, one, torch.ones(6, 4, device=dev)),
+            K.distill_backward(x, ids, u, t, kstats, one, one, 2.0),
+            K.embedding_backward(tokens, torch.ones(30, 6, 16, device=dev), 40, 3.0))
+
+    def sums(x, w, ids=ids, u=u, t=t, tokens=tokens):
+        lp = m3.token_logprobs(x, t, top=4)
+        kd = m3.distill_loss(x, ids, u, temperature=2.0, targets=t)
+        return (lp.logp.sum() + lp.entropy.sum() + lp.top_logp.sum(), kd.kd.sum() + kd.nll.sum(),
+                m3.embed_tokens(w, tokens, scale=3.0).sum())
+
+    def check(outs, xg, wg, **kw):
+        grads = [torch.autograd.grad(o, v, **kw)[0] for o, v in zip(outs, (xg, xg, wg))]
+        assert all(torch.equal(a, b) for a, b in zip(grads, want))
+
+    xg, wg = x.clone().requires_grad_(True), table.clone().requires_grad_(True)
+    outs = sums(xg, wg)
+    check(outs, xg, wg, retain_graph=True)
+    check(outs, xg, wg)
+    with torch.autograd.graph.save_on_cpu():
+        outs = sums(xg, wg)
+    check(outs, xg, wg)
+    # read as copies: another axis order, int32 targets, strided teacher and tokens
+    xt = x.t().contiguous().requires_grad_(True)
+    outs = sums(xt.t(), wg, ids.t().contiguous().t(), u.t().contiguous().t(), t.int(), tokens.t().contiguous().t())
+    for o, v, w in zip(outs, (xt, xt, wg), want):
+        g = torch.autograd.grad(o, v, retain_graph=True)[0]
+        assert torch.equal(g.t() if v is xt else g, w)
+    outs = sums(xg, wg)
+    with torch.no_grad():
+        xg.mul_(1.0)   # autograd sees that the saved logits changed
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(outs[0], xg)
+
+
 def test_nodes_refuse_what_they_cannot_do(m3, dev):
     x = torch.randn(3, 10, device=dev, requires_grad=True)
     t = torch.tensor([1, 2, 3], device=dev)
