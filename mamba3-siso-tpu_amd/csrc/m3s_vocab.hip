@@ -475,11 +475,11 @@ __device__ __forceinline__ void values_out(const T* __restrict__ x, int n, int k
 }
 
 // out(rank, value, index) for the k largest of n logits (k <= n, no NaN, no +inf, the largest
-// `top`), equal ones by index. Measured, on top of the pass over the row: 999 rows of 50001 bf16 21 us,
-// with 1, 20 and 64 alternatives 25, 26 and 31 (by a bound's ties in a list built with one atomic a
-// logit, and ranked value by value, 27, 43 and 53; by rounds of arg-max, 64 took 5 ms). By a workgroup: a bound that k of the threads' maxima reach is
-// reached by at least k logits, and by hardly more; those are collected from the few batches that
-// hold them and ranked against each other.
+// `top`), equal ones by index. By a workgroup: a bound that k of the threads' maxima reach is reached
+// by at least k logits, and by hardly more; those are collected from the few batches that hold them
+// and ranked against each other. 999 rows of 50001 bf16 take 21 us, with 1, 20 and 64 alternatives
+// 25, 26 and 31 (27, 43 and 53 with the exact k-th maximum, found bit by bit, and each thread reading
+// its own batches; 5 ms by rounds of arg-max for 64).
 template <typename G, int U, typename T, typename OUT>
 __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, float top, const Best& best,
                                      PickSpace<4>& sp, OUT&& out) {
@@ -509,7 +509,6 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
   __syncthreads();   // the space is free again
 }
 
-constexpr int kLaneTop = 24;   // kLaneTop * 17 logits fit the list
 // The same by a wave that holds the whole row, one batch and a rest. The bound is on the lanes'
 // maxima for few alternatives (one value a lane to count), on the logits themselves for more, of
 // which the lanes' maxima would let most of the row through.
@@ -518,16 +517,19 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
                                      PickSpace<1>& sp, OUT&& out) {
   using R = Rows<G, U, T>;
   constexpr int LEN = R::LEN;
+  // so many lanes' logits all fit the list: no bound lets more of them through but by ties, and
+  // what exceeds the tied value then comes from fewer than k lanes
+  constexpr int LANES = std::min(64, PickSpace<1>::CAP / (LEN + 1)), FEW = std::min(24, LANES);
   const int whole = n / R::N * R::N, tail = whole + G::tid();
   float v[LEN + 1];
   R::load(x, n, 0, v);
   v[LEN] = tail < n ? (float)x[tail] : kNegInf;
   float bar;
-  if (k <= kLaneTop) {
+  if (k <= FEW) {
     float most = v[0];
 #pragma unroll
     for (int i = 1; i <= LEN; ++i) most = fmaxf(most, v[i]);
-    bar = kth_bound<1>(&most, top, k, min(k + 12, 64));
+    bar = kth_bound<1>(&most, top, k, min(k + 12, LANES));
   } else {
     bar = kth_bound<LEN + 1>(v, top, k, 64);
   }
@@ -546,7 +548,7 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
   int count = gather(std::false_type());
   if (count > PickSpace<1>::CAP) {
     G::sync();
-    count = gather(std::true_type());   // fewer than kLaneTop (LEN + 1), or than k
+    count = gather(std::true_type());   // fewer than FEW (LEN + 1), or than k
     equal_out<G>(x, n, bar, count, k, sp, out);
   }
   rank_out<G>(count, k, sp, out);

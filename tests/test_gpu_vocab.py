@@ -211,6 +211,21 @@ def test_whole_rows_of_hard_kinds(m3, dev, dtype, rows, vocab):
         check_logprob(m3, dev, x, targets, top, 1.0, ("lht",) if top in (0, 20) else ())
 
 
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1000), (torch.float32, 1024), (torch.bfloat16, 1023),
+                                         (torch.float32, 250), (torch.bfloat16, 500)])
+def test_few_lanes_hold_more_than_the_list(m3, dev, dtype, vocab):
+    """Rows of a wave whose lanes hold falling blocks of logits: the lanes that reach a bound on their
+    maxima reach it with all they hold."""
+    gen = torch.Generator().manual_seed(vocab)
+    lane = torch.arange(vocab) // (4 if dtype == torch.float32 else 8) % 64
+    rows = [(100 - slope * lane + 0.1 * torch.rand(vocab, generator=gen)) for slope in (0.25, 0.5, 0.9, 1.5)]
+    rows += [100 - 0.9 * lane, 50.0 + 0 * lane, torch.where(lane < 40, 7.0, -INF)]
+    x = torch.stack([r.float() for r in rows]).to(dtype)
+    targets = torch.arange(len(rows))
+    for top in (1, 5, 20, 24, 25, 30, 31, 64):
+        check_logprob(m3, dev, x, targets, top, 1.0, ())
+
+
 def test_one_thread_holds_the_best(m3, dev):
     """The best tokens all at one stride, equal or falling, so that one part of the workgroup has
     them all."""
