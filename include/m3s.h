@@ -663,7 +663,7 @@ typedef struct m3s_logprob_args {
   const int64_t* targets; /* (rows), or NULL: no logp */
   float* logp;           /* forward out (rows) with targets */
   float* entropy;        /* forward out (rows) */
-  float* stats;          /* forward out, backward in (rows, 3) */
+  float* stats;          /* forward out or NULL, backward in (rows, 3) */
   float* top_logp;       /* forward out (rows, top) */
   int64_t* top_ids;      /* forward out (rows, top); backward in with dtop_logp */
   const float* dlogp;    /* backward in (rows) or NULL */
@@ -703,7 +703,7 @@ typedef struct m3s_distill_args {
   const int64_t* targets;     /* (rows), or NULL */
   float* kd;             /* forward out (rows) */
   float* nll;            /* forward out (rows) iff targets */
-  float* stats;          /* forward out, backward in (rows, 5) */
+  float* stats;          /* forward out or NULL, backward in (rows, 5) */
   const float* dkd;      /* backward in (rows) or NULL */
   const float* dnll;     /* backward in (rows) or NULL */
   void* dlogits;         /* backward out (rows, vocab) */

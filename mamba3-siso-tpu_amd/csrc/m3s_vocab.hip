@@ -618,7 +618,7 @@ template <typename G>
 __device__ __forceinline__ void logprob_skip(const LogprobParams& p, int64_t r) {
   if (G::tid() == 0) {
     p.logp[r] = p.entropy[r] = 0.f;
-    p.stats[3 * r] = p.stats[3 * r + 1] = p.stats[3 * r + 2] = 0.f;
+    if (p.stats) p.stats[3 * r] = p.stats[3 * r + 1] = p.stats[3 * r + 2] = 0.f;
   }
   for (int j = G::tid(); j < p.top; j += G::NT) {
     p.top_logp[r * p.top + j] = kNegInf;
@@ -646,9 +646,11 @@ __device__ __forceinline__ void logprob_store(const LogprobParams& p, int64_t r,
   if (G::tid() != 0) return;
   const float h = logp.empty ? 0.f : logp.logs - sum.t * p.inv_t / sum.s;
   p.entropy[r] = h;
-  p.stats[3 * r] = sum.m;
-  p.stats[3 * r + 1] = sum.s;
-  p.stats[3 * r + 2] = h;
+  if (p.stats) {
+    p.stats[3 * r] = sum.m;
+    p.stats[3 * r + 1] = sum.s;
+    p.stats[3 * r + 2] = h;
+  }
   if (p.targets) p.logp[r] = tgt >= 0 && tgt < p.vocab ? logp(xt) : __builtin_nanf("");
 }
 
@@ -942,14 +944,16 @@ __device__ __forceinline__ void distill_store(const DistillParams& p, int64_t r,
   }
   const float kd = G::sum(term, tmp);
   if (G::tid() != 0) return;
-  float* stats = p.stats + 5 * r;
   p.kd[r] = soft ? p.temp * p.temp * kd : 0.f;
-  stats[0] = soft || hard ? sum.m : 0.f;
-  stats[1] = sum.s;
   const float s1 = MODE == kDual ? sum.s1 : sum.s;
-  stats[2] = s1;
-  stats[3] = t.ref;
-  stats[4] = t.ts;
+  if (p.stats) {
+    float* stats = p.stats + 5 * r;
+    stats[0] = soft || hard ? sum.m : 0.f;
+    stats[1] = sum.s;
+    stats[2] = s1;
+    stats[3] = t.ref;
+    stats[4] = t.ts;
+  }
   if (p.nll) {
     float v = 0.f;
     if (hard) {
@@ -1378,7 +1382,7 @@ extern "C" int32_t m3s_logprob_fwd(const m3s_logprob_args* a, void* stream) {
               "m3s_logprob_fwd: top %d must be in [0, %d] and at most the vocabulary", a->top, kTopMax);
   if (a->batch == 0 || a->seqlen == 0) return 0;
   if (int32_t rc = check_logits(a, "m3s_logprob_fwd")) return rc;
-  M3S_REQUIRE(a->entropy && a->stats && (!a->targets || a->logp) && (!a->top || (a->top_logp && a->top_ids)),
+  M3S_REQUIRE(a->entropy && (!a->targets || a->logp) && (!a->top || (a->top_logp && a->top_ids)),
               "m3s_logprob_fwd: NULL pointer");
   if (int32_t rc = check_scratch(a, "m3s_logprob_fwd")) return rc;
   LogprobParams p = logprob_params(a);
@@ -1417,7 +1421,7 @@ static int32_t check_distill(const m3s_distill_args* a, const char* who) {
               who);
   if (a->batch == 0 || a->seqlen == 0) return 0;
   if (int32_t rc = check_logits(a, who)) return rc;
-  M3S_REQUIRE(a->teacher_ids && a->teacher_logits && a->stats, "%s: NULL pointer", who);
+  M3S_REQUIRE(a->teacher_ids && a->teacher_logits, "%s: NULL pointer", who);
   return 0;
 }
 
@@ -1441,7 +1445,7 @@ extern "C" int32_t m3s_distill_bwd(const m3s_distill_args* a, void* stream) {
   if (int32_t rc = check_distill(a, "m3s_distill_bwd")) return rc;
   if (a->batch == 0 || a->seqlen == 0) return 0;
   const uintptr_t es = a->dtype == M3S_DTYPE_BF16 ? 2 : 4;
-  M3S_REQUIRE(a->dlogits && (uintptr_t)a->dlogits % es == 0 && (!a->dnll || a->targets),
+  M3S_REQUIRE(a->stats && a->dlogits && (uintptr_t)a->dlogits % es == 0 && (!a->dnll || a->targets),
               "m3s_distill_bwd: NULL or misaligned pointer");
   DistillParams p = distill_params(a);
   const hipStream_t s = static_cast<hipStream_t>(stream);

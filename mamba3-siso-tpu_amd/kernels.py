@@ -1476,19 +1476,20 @@ TOP_MAX, TEACHER_MAX = 64, 256
 _LOGPROB_SIZE, _DISTILL_SIZE = ctypes.sizeof(_lib.LogprobArgs), ctypes.sizeof(_lib.DistillArgs)
 
 
-def _logit_rows(logits: Tensor, what: str) -> Tensor:
-    """``logits`` (..., V) as the (B, L, V) view that the kernels read in place; a copy only where
-    the rows are not contiguous or more than two leading axes do not fold."""
-    if logits.dim() == 0 or logits.shape[-1] == 0:
+def _logit_rows(logits: Tensor, what: str):
+    """``logits`` (..., V) as the (B, L, V) view that the kernels read in place, and its ``m3s_blx``;
+    a copy only where the rows are not contiguous or more than two leading axes do not fold."""
+    dim = logits.dim()
+    if dim == 0 or logits.shape[-1] == 0:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
-    v = logits.shape[-1]
-    if logits.stride(-1) != 1 and v > 1:
+    if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
-    if logits.dim() == 3:
-        return logits
-    if logits.dim() > 3:
-        return logits.flatten(0, -3)
-    return logits.unsqueeze(0) if logits.dim() == 2 else logits.view(1, 1, v)
+    if dim > 3:
+        logits = logits.flatten(0, -3)
+    elif dim < 3:
+        logits = logits.unsqueeze(0) if dim == 2 else logits.view(1, 1, -1)
+    sb, st, _ = logits.stride()
+    return logits, _lib.Blx(logits.data_ptr(), sb, st)
 
 
 def _row_values(t: Optional[Tensor], shape, dtype: torch.dtype, what: str) -> Optional[Tensor]:
@@ -1526,35 +1527,37 @@ def _check_temperature(temperature: float, what: str) -> float:
 
 
 def logprob_call(logits: Tensor, targets: Optional[Tensor], top: int, temperature: float,
-                 ignore_index: int):
-    """`logprob_forward` with its `Call`, on ``(logits, targets, stats, top_ids)``, and the targets
-    that the call read."""
-    rows = _logit_rows(logits, "logprob")
+                 ignore_index: int, keep: bool = True):
+    """`logprob_forward` with the targets that the call read and its `Call`, on ``(logits, targets,
+    stats, top_ids)``. Without ``keep`` there are no stats and no `Call` (a backward needs both)."""
+    rows, blx = _logit_rows(logits, "logprob")
     b, l, v = rows.shape
-    top = int(top)
     if not 0 <= top <= min(TOP_MAX, v):
         raise ValueError(f"logprob: top must be in [0, {min(TOP_MAX, v)}], got {top}")
     shape = logits.shape[:-1]
     targets = _row_targets(targets, shape, "logprob")
     a = _lib.LogprobArgs(_LOGPROB_SIZE, _lib.dtype_code(rows.dtype), b, l, v, top,
-                         _check_temperature(temperature, "logprob"), ignore_index, _lib.blx(rows))
+                         _check_temperature(temperature, "logprob"), ignore_index, blx)
     dev = _device_of(logits, targets)
     # tensors of their own, not views of one: autograd refuses in-place work on a node's views
-    entropy = empty(shape, device=dev, dtype=torch.float32)
-    stats = empty(*shape, 3, device=dev, dtype=torch.float32)
-    logp = top_logp = top_ids = None
-    a.entropy, a.stats = entropy.data_ptr(), stats.data_ptr()
+    f32 = torch.float32
+    entropy = empty(shape, device=dev, dtype=f32)
+    logp = top_logp = top_ids = stats = None
+    a.entropy = entropy.data_ptr()
     if targets is not None:
-        logp = empty(shape, device=dev, dtype=torch.float32)
+        logp = empty(shape, device=dev, dtype=f32)
         a.targets, a.logp = targets.data_ptr(), logp.data_ptr()
+    if keep:
+        stats = empty(*shape, 3, device=dev, dtype=f32)
+        a.stats = stats.data_ptr()
     if top:
-        top_logp = empty(*shape, top, device=dev, dtype=torch.float32)
+        top_logp = empty(*shape, top, device=dev, dtype=f32)
         top_ids = empty(*shape, top, device=dev, dtype=torch.int64)
         a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
     ws = _row_scratch(a, dev, "m3s_logprob_workspace_bytes", b * l, v, top)  # noqa: F841
     _lib.launch(_lib.load().m3s_logprob_fwd, a, dev, "m3s_logprob_fwd")
-    return ((logp, entropy, top_logp, top_ids, stats), targets,
-            Call(a, dev, (a.logits.ptr, a.targets, a.stats, a.top_ids)))
+    call = Call(a, dev, (a.logits.ptr, a.targets, a.stats, a.top_ids)) if keep else None
+    return (logp, entropy, top_logp, top_ids, stats), targets, call
 
 
 def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int = 0,
@@ -1568,7 +1571,7 @@ def logprob_forward(logits: Tensor, targets: Optional[Tensor] = None, top: int =
     Rows whose target is ``ignore_index`` are not read: logp and entropy 0, ids -1, top_logp -inf.
     Another target outside [0, V) gives NaN. A row of nothing but -inf has logp -inf, entropy 0; a
     row with NaN or +inf is NaN throughout, with ids -1."""
-    return logprob_call(logits, targets, top, temperature, ignore_index)[0]
+    return logprob_call(logits, targets, int(top), temperature, int(ignore_index))[0]
 
 
 def logprob_call_backward(a: "_lib.LogprobArgs", dev: torch.device, logits: Tensor, dlogp, dentropy,
@@ -1588,7 +1591,7 @@ def logprob_backward(logits: Tensor, targets: Optional[Tensor], stats: Tensor,
                      temperature: float = 1.0, ignore_index: int = -100) -> Tensor:
     """The logits' cotangent of `logprob_forward` (one ``m3s_logprob_bwd`` launch), dense and in
     their dtype, from any of the three outputs' cotangents."""
-    rows = _logit_rows(logits, "logprob")
+    rows, blx = _logit_rows(logits, "logprob")
     shape = logits.shape[:-1]
     targets = _row_targets(targets, shape, "logprob")
     if dlogp is not None and targets is None:
@@ -1606,7 +1609,7 @@ def logprob_backward(logits: Tensor, targets: Optional[Tensor], stats: Tensor,
         dtop_logp = _row_values(dtop_logp, (*shape, top), f32, "logprob: dtop_logp")
     b, l, v = rows.shape
     a = _lib.LogprobArgs(_LOGPROB_SIZE, _lib.dtype_code(rows.dtype), b, l, v, top,
-                         _check_temperature(temperature, "logprob"), ignore_index, _lib.blx(rows))
+                         _check_temperature(temperature, "logprob"), ignore_index, blx)
     dev = _device_of(logits, targets, stats, dlogp, dentropy, dtop_logp, top_ids if top else None)
     dx = empty(logits.shape, device=dev, dtype=logits.dtype)
     a.targets, a.stats, a.dlogits = _lib.ptr(targets), stats.data_ptr(), dx.data_ptr()
@@ -1619,7 +1622,7 @@ def logprob_backward(logits: Tensor, targets: Optional[Tensor], stats: Tensor,
 
 def _distill_args(logits: Tensor, ids: Tensor, teacher: Tensor, targets: Optional[Tensor],
                   temperature: float, ignore_index: int):
-    rows = _logit_rows(logits, "distill")
+    rows, blx = _logit_rows(logits, "distill")
     shape = logits.shape[:-1]
     k = ids.shape[-1] if ids.dim() else 0
     if not 1 <= k <= TEACHER_MAX:
@@ -1632,29 +1635,32 @@ def _distill_args(logits: Tensor, ids: Tensor, teacher: Tensor, targets: Optiona
     b, l, v = rows.shape
     a = _lib.DistillArgs(_DISTILL_SIZE, _lib.dtype_code(rows.dtype), b, l, v, k,
                          _lib.dtype_code(teacher.dtype), ID_BYTES[ids.dtype],
-                         _check_temperature(temperature, "distill"), ignore_index, _lib.blx(rows))
+                         _check_temperature(temperature, "distill"), ignore_index, blx)
     dev = _device_of(logits, ids, teacher, targets)
     a.teacher_ids, a.teacher_logits, a.targets = ids.data_ptr(), teacher.data_ptr(), _lib.ptr(targets)
     return a, dev, (rows, ids, teacher, targets)   # the tensors stay alive until the launch
 
 
 def distill_call(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
-                 targets: Optional[Tensor], temperature: float, ignore_index: int):
-    """`distill_forward` with its `Call`, on ``(logits, ids, teacher, targets, stats)``, and the
-    three operands between as the call read them."""
+                 targets: Optional[Tensor], temperature: float, ignore_index: int, keep: bool = True):
+    """`distill_forward` with the ids, teacher's logits and targets as the call read them and its
+    `Call`, on ``(logits, ids, teacher, targets, stats)``. Without ``keep`` there are no stats and no
+    `Call` (a backward needs both)."""
     a, dev, ops = _distill_args(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)
     shape = logits.shape[:-1]
     kd = empty(shape, device=dev, dtype=torch.float32)
-    stats = empty(*shape, 5, device=dev, dtype=torch.float32)
-    nll = None
-    a.kd, a.stats = kd.data_ptr(), stats.data_ptr()
+    nll = stats = None
+    a.kd = kd.data_ptr()
     if targets is not None:
         nll = empty(shape, device=dev, dtype=torch.float32)
         a.nll = nll.data_ptr()
+    if keep:
+        stats = empty(*shape, 5, device=dev, dtype=torch.float32)
+        a.stats = stats.data_ptr()
     ws = _row_scratch(a, dev, "m3s_distill_workspace_bytes", a.batch * a.seqlen, a.vocab)  # noqa: F841
     _lib.launch(_lib.load().m3s_distill_fwd, a, dev, "m3s_distill_fwd")
-    return ((kd, nll, stats), ops[1:],
-            Call(a, dev, (a.logits.ptr, a.teacher_ids, a.teacher_logits, a.targets, a.stats)))
+    call = Call(a, dev, (a.logits.ptr, a.teacher_ids, a.teacher_logits, a.targets, a.stats)) if keep else None
+    return (kd, nll, stats), ops[1:], call
 
 
 def distill_forward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
@@ -1668,7 +1674,7 @@ def distill_forward(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
     An entry with an id < 0 does not count, one with logit -inf has weight 0, a repeated id adds
     up. A row without entries has kd 0, one with target ``ignore_index`` nll 0; with neither it is
     not read. An id >= V and another target outside [0, V) give NaN."""
-    return distill_call(logits, teacher_ids, teacher_logits, targets, temperature, ignore_index)[0]
+    return distill_call(logits, teacher_ids, teacher_logits, targets, temperature, int(ignore_index))[0]
 
 
 def distill_call_backward(a: "_lib.DistillArgs", dev: torch.device, logits: Tensor, dkd, dnll) -> Tensor:

@@ -58,6 +58,8 @@ def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
     The gradient is dense, summed in float32 in position order and so bit-reproducible.
     ``padding_idx`` names an id (negative: from the end) whose row is looked up but gets no
     gradient. An id outside [0, V) gives a row of NaN, and no gradient."""
+    if table.dim() != 2:
+        raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
     pad = -1 if padding_idx is None else K.embedding_padding(int(padding_idx), table.shape[0])
     if _needs_node(table):
         return _EmbedFn.apply(table, tokens, float(scale), pad)
@@ -119,7 +121,7 @@ def token_logprobs(logits: Tensor, targets: Optional[Tensor] = None, top: int = 
     if _needs_node(logits):
         return TokenLogprobs(*_LogprobFn.apply(logits, targets, int(top), float(temperature),
                                                int(ignore_index)))
-    return TokenLogprobs(*K.logprob_forward(logits, targets, top, temperature, ignore_index)[:4])
+    return TokenLogprobs(*K.logprob_call(logits, targets, int(top), temperature, int(ignore_index), False)[0][:4])
 
 
 class DistillLoss(NamedTuple):
@@ -174,5 +176,5 @@ def distill_loss(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
     if _needs_node(logits, teacher_logits):
         return DistillLoss(*_DistillFn.apply(logits, teacher_ids, teacher_logits, targets,
                                              float(temperature), int(ignore_index)))
-    return DistillLoss(*K.distill_forward(logits, teacher_ids, teacher_logits, targets, temperature,
-                                          ignore_index)[:2])
+    return DistillLoss(*K.distill_call(logits, teacher_ids, teacher_logits, targets, temperature,
+                                       int(ignore_index), False)[0][:2])

@@ -15,8 +15,9 @@ def test_embedding_refuses_bad_arguments(m3):
         m3.embed_tokens(table, tokens.float())
     with pytest.raises(ValueError, match="bf16 or f32"):
         m3.embed_tokens(table.double(), tokens)
-    with pytest.raises(ValueError, match="must be \\(V, D\\)"):
-        m3.embed_tokens(table[0], tokens)
+    for bad in (table[0], table[0, 0]):
+        with pytest.raises(ValueError, match="must be \\(V, D\\)"):
+            m3.embed_tokens(bad, tokens, padding_idx=0)
     with pytest.raises(ValueError, match="must not be empty"):
         m3.embed_tokens(table[:0], tokens)
     for pad in (5, -6):
@@ -150,15 +151,15 @@ def test_vocab_abi_refuses_bad_structs(m3):
     common = [dict(dtype=5), dict(batch=-1), dict(seqlen=-1), dict(vocab=0), dict(vocab=1 << 30),
               dict(batch=1 << 16, seqlen=1 << 16), dict(temperature=0.0), dict(temperature=-2.0),
               dict(temperature=float("nan")), dict(temperature=float("inf")), dict(temperature=1e-39),
-              dict(stats=None), dict(logits=lib.Blx(None, 30, 10)), dict(logits=lib.Blx(4098, 30, 10)),
+              dict(logits=lib.Blx(None, 30, 10)), dict(logits=lib.Blx(4098, 30, 10)),
               dict(logits=lib.Blx(4096, -30, 10)), dict(logits=lib.Blx(4096, 30, -10))]
     own = [[dict(top=-1), dict(top=65, vocab=100), dict(top=11), dict(logp=None), dict(entropy=None),
             dict(top_logp=None), dict(top_ids=None)],
-           [dict(top=65, vocab=100), dict(dlogits=None), dict(dlogits=4098), dict(targets=None),
+           [dict(stats=None), dict(top=65, vocab=100), dict(dlogits=None), dict(dlogits=4098), dict(targets=None),
             dict(top_ids=None)],
            [dict(teacher_k=0), dict(teacher_k=257), dict(id_bytes=2), dict(teacher_dtype=9), dict(kd=None),
             dict(nll=None), dict(targets=None), dict(teacher_ids=None), dict(teacher_logits=None)],
-           [dict(teacher_k=0), dict(dlogits=None), dict(dlogits=4098), dict(targets=None),
+           [dict(stats=None), dict(teacher_k=0), dict(dlogits=None), dict(dlogits=4098), dict(targets=None),
             dict(teacher_ids=None)]]
     for (entry, cls), extra in zip(entries, own):
         assert entry(None, None) == lib.ERR_INVALID and b"NULL" in h.m3s_last_error()
