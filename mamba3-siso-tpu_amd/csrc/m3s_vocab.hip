@@ -46,7 +46,7 @@ constexpr int kTeacherMax = 256;   // teacher tokens of a row
 // against 15.6 / 16; but 512 x 4000: 5.2 / 6.0 against 4.9 / 6.0); the rest to a workgroup.
 constexpr int kPartVocab = 1024, kPartRows = 4096, kWaveVocab = 4096, kWaveRows = 1024;
 constexpr int kWaveHeld = 1024;     // one batch of a wave holds the row: it goes to one whatever the rows
-constexpr int kPartTop = 16;        // alternatives that 16 lanes pick, of rows up to kPartPick long
+constexpr int kPartTop = 14;        // alternatives that 16 lanes pick, of rows up to kPartPick long
 constexpr int kPartPick = 256;
 constexpr int kPartTeacher = 64;    // teacher tokens of a row of 16 lanes
 constexpr float kNegInf = -__builtin_inff();
@@ -555,20 +555,69 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
   G::sync();
 }
 
-// The same by 16 lanes that hold the row's at most kPartPick logits, one round for each of few:
-// 32768 x 256 with 1, 5 and 8 alternatives 9.7, 15 and 19 us, and 6.9 without; a wave's bound and list
-// take 29 for 20.
+// The same by 16 lanes that hold the row's at most kPartPick logits, for k < 16: the bound on the
+// lanes' maxima by comparing each with the others, the logits that reach it in a list, ranked. One or
+// two, and a list too long (ties, masked rows), go by rounds of (largest value, lowest index).
+// 32768 x 256 float32 takes 7 us, with 1, 5, 8 and 14 alternatives 10.9, 13.4, 14.4 and 23 (15, 18.7 and
+// 27 for the last three by rounds); with 20, by a wave, 30.
+struct PartSpace {
+  static constexpr int CAP = 64;
+  uint64_t list[CAP + 5];   // four zeros behind it; odd, so that the groups use different banks
+};
+template <int n>
+__device__ __forceinline__ float row_turned(float v) {   // lane i of 16 reads another, n places on
+  return dpp_mov<0x120 + n>(v);
+}
 template <typename G, typename T, typename OUT>
-__device__ __forceinline__ void pick_few(const T* __restrict__ x, int n, int k, OUT&& out) {
+__device__ __forceinline__ void pick_part(const T* __restrict__ x, int n, int k, PartSpace& sp, OUT&& out) {
   constexpr int N = Piece<T>::N, U = kPartPick / (G::NT * N), LEN = U * N;
   using R = Rows<G, U, T>;
   const float gone = __builtin_nanf("");   // no logit, or one that is out already
-  const int tail = n / N * N + G::tid();
+  const int whole = n / N * N, tail = whole + G::tid();
   float v[LEN + 1];
   R::load(x, n, 0, v);
 #pragma unroll
-  for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) < n / N * N ? v[i] : gone;
+  for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) < whole ? v[i] : gone;
   v[LEN] = tail < n ? (float)x[tail] : gone;
+  if (k > 2) {
+    float most = kNegInf;
+#pragma unroll
+    for (int i = 0; i <= LEN; ++i) most = fmaxf(most, v[i]);
+    // the k-th largest of the lanes' maxima: the largest that k of them reach
+    int reach = 1;
+    const auto against = [&](float other) { reach += other >= most; };
+    against(row_turned<1>(most)), against(row_turned<2>(most)), against(row_turned<3>(most));
+    against(row_turned<4>(most)), against(row_turned<5>(most)), against(row_turned<6>(most));
+    against(row_turned<7>(most)), against(row_turned<8>(most)), against(row_turned<9>(most));
+    against(row_turned<10>(most)), against(row_turned<11>(most)), against(row_turned<12>(most));
+    against(row_turned<13>(most)), against(row_turned<14>(most)), against(row_turned<15>(most));
+    const float bar = G::max(reach >= k ? most : kNegInf, nullptr);
+    int mine = 0;
+#pragma unroll
+    for (int i = 0; i <= LEN; ++i) mine += v[i] >= bar;
+    const float upto = row_prefix16((float)mine);
+    const int total = (int)G::max(upto, nullptr);
+    if (total <= PartSpace::CAP) {
+      int at = (int)upto - mine;
+#pragma unroll
+      for (int i = 0; i <= LEN; ++i) {
+        if (v[i] >= bar) sp.list[at++] = candidate(v[i], i < LEN ? R::place(0, i) : tail);
+      }
+      if (G::tid() < 4) sp.list[total + G::tid()] = 0;   // below every candidate
+      G::sync();
+      for (int c = G::tid(); c < total; c += G::NT) {
+        const uint64_t me = sp.list[c];
+        int rank = 0;
+        for (int j = 0; j < total; j += 4) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u) rank += sp.list[j + u] > me;
+        }
+        if (rank < k) out(rank, key_float((uint32_t)(me >> 32)), (int)~(uint32_t)me);
+      }
+      G::sync();
+      return;
+    }
+  }
   for (int j = 0; j < k; ++j) {
     float top = v[LEN];
 #pragma unroll
@@ -668,7 +717,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
   using G = Group<NT>;
   constexpr bool PICK = TOP && NT > 16;
   __shared__ float tmp[G::TMP];
-  __shared__ PickSpace<NT == 256 ? 4 : 1> space[PICK ? G::ROWS : 1];
+  __shared__ std::conditional_t<NT == 16, PartSpace, PickSpace<NT == 256 ? 4 : 1>> space[TOP ? G::ROWS : 1];
   for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
     const int64_t tgt = p.targets ? p.targets[r] : 0;
     if (p.targets && tgt == p.ignore) {
@@ -693,7 +742,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
         p.top_ids[r * p.top + j] = i;
       };
       if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
-      else pick_few<G>(x, p.vocab, p.top, out);
+      else pick_part<G>(x, p.vocab, p.top, space[G::slot()], out);
     }
   }
 }
