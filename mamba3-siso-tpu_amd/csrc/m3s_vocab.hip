@@ -260,7 +260,7 @@ template <typename G, int U, bool TOP, int MODE, typename T>
 __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* __restrict__ x, int n,
                                          float c, float c1) {
   using R = Rows<G, U, T>;
-  const int batches = R::whole(n);
+  const int full = n / R::N, batches = full / R::HOP;   // whole ones
   for (int b = 0; b < batches; ++b) {
     float v[R::LEN];
     R::load(x, n, b, v);
@@ -269,6 +269,20 @@ __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* 
     for (int i = 1; i < R::LEN; ++i) top = fmaxf(top, v[i]);
     if constexpr (TOP) best.see(top, b);
     r.template add<R::LEN>(v, top, c, c1);
+  }
+  if (batches * R::HOP < full) {   // the last batch, only the pieces that it has
+    float v[R::LEN], most = kNegInf;
+    R::load(x, n, batches, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (batches * R::HOP + u * G::NT >= full) break;
+      float top = v[u * R::N];
+#pragma unroll
+      for (int i = 1; i < R::N; ++i) top = fmaxf(top, v[u * R::N + i]);
+      most = fmaxf(most, top);
+      r.template add<R::N>(v + u * R::N, top, c, c1);
+    }
+    if constexpr (TOP) best.see(most, batches);
   }
   const int at = n / R::N * R::N + G::tid();
   if (at < n) {
@@ -647,7 +661,7 @@ struct LogprobParams {
   void* dlogits;
   float* part;       // a split row's pieces: (rows, split, 3) sums, (rows, split, top) values and ids
   int64_t ignore, rows;
-  int seqlen, vocab, top, chunks, split, share;   // share: logits to a piece
+  int seqlen, vocab, top, chunks, chunk, split, share;   // chunk, share: logits to one of chunks, to a piece
   float temp, inv_t, c;
 };
 
@@ -831,21 +845,20 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
 
 // ---- gradients ---------------------------------------------------------------------------------
 // The dense part: f(x) for every logit of lo .. hi - 1, at most kBwdPieces pieces a thread.
-constexpr int kBwdPieces = 4;
-template <typename G, typename T> constexpr int kChunk = G::NT* kBwdPieces* Piece<T>::N;
+template <typename T> constexpr int kBwdPieces = 4;
 template <typename G, typename T, typename F>
 __device__ __forceinline__ void chunk_map(const T* __restrict__ x, T* __restrict__ dx, int lo, int hi,
                                           F&& f) {
   constexpr int N = Piece<T>::N;
   const int n = hi - lo, full = n / N;
-  float v[kBwdPieces * N];
+  float v[kBwdPieces<T> * N];
 #pragma unroll
-  for (int u = 0; u < kBwdPieces; ++u) {
+  for (int u = 0; u < kBwdPieces<T>; ++u) {
     const int at = u * G::NT + G::tid();
     if (at < full) Piece<T>::load(x + lo + at * N, v + u * N);
   }
 #pragma unroll
-  for (int u = 0; u < kBwdPieces; ++u) {
+  for (int u = 0; u < kBwdPieces<T>; ++u) {
     const int at = u * G::NT + G::tid();
     if (at < full) {
       float o[N];
@@ -877,7 +890,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_bwd_kernel(const LogprobP
   const int64_t work = p.rows * p.chunks;
   for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
     const int64_t r = quotient(w, p.chunks);
-    const int lo = (int)(w - r * p.chunks) * kChunk<G, T>, hi = min(lo + kChunk<G, T>, p.vocab);
+    const int lo = (int)(w - r * p.chunks) * p.chunk, hi = min(lo + p.chunk, p.vocab);
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
     const int64_t tgt = p.targets ? p.targets[r] : -1;
@@ -930,7 +943,7 @@ struct DistillParams {
   void* dlogits;
   float* part;       // a split row's pieces: (rows, split, 3) sums
   int64_t ignore, rows;
-  int seqlen, vocab, k, chunks, id_bytes, teacher_bf16, split, share;
+  int seqlen, vocab, k, chunks, chunk, id_bytes, teacher_bf16, split, share;
   float temp, inv_t, c, c1;
 };
 
@@ -1091,7 +1104,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
   const int64_t work = p.rows * p.chunks;
   for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
     const int64_t r = quotient(w, p.chunks);
-    const int lo = (int)(w - r * p.chunks) * kChunk<G, T>, hi = min(lo + kChunk<G, T>, p.vocab);
+    const int lo = (int)(w - r * p.chunks) * p.chunk, hi = min(lo + p.chunk, p.vocab);
     const T* x = row_at<T>(p.logits, r, p.seqlen);
     T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
     const float* stats = p.stats + 5 * r;
@@ -1247,9 +1260,13 @@ static int row_threads(int64_t rows, int vocab, bool part) {
   if (part && vocab <= kPartVocab && rows >= kPartRows) return 16;
   return vocab <= kWaveHeld || (vocab <= kWaveVocab && rows >= kWaveRows) ? 64 : 256;
 }
-static int vocab_chunks(int vocab, int dtype, int nt) {
-  const int chunk = nt * kBwdPieces * (dtype == M3S_DTYPE_BF16 ? Piece<bf16>::N : Piece<float>::N);
-  return (vocab + chunk - 1) / chunk;
+// The backward's equal chunks of a row, at most kBwdPieces pieces to a thread, whole 16-byte pieces.
+template <typename T, typename P>
+static void set_chunks(P& p, int nt) {
+  constexpr int N = Piece<T>::N;
+  const int most = nt * kBwdPieces<T> * N;
+  p.chunks = (p.vocab + most - 1) / most;
+  p.chunk = ((p.vocab + p.chunks - 1) / p.chunks + N - 1) / N * N;
 }
 // Rows from one stride_b to the next: all of them where the batch axis continues the other.
 template <typename A>
@@ -1370,18 +1387,18 @@ static void launch_distill_fwd(const DistillParams& p, hipStream_t s) {
   });
 }
 template <typename T>
-static void launch_logprob_bwd(LogprobParams& p, int dtype, hipStream_t s) {
+static void launch_logprob_bwd(LogprobParams& p, hipStream_t s) {
   const int nt = row_threads(p.rows, p.vocab, true);
-  p.chunks = vocab_chunks(p.vocab, dtype, nt);
+  set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
     launch_kernel(logprob_bwd_kernel<NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s);
   });
 }
 template <bool DUAL, typename T>
-static void launch_distill_bwd(DistillParams& p, int dtype, hipStream_t s) {
+static void launch_distill_bwd(DistillParams& p, hipStream_t s) {
   const int nt = row_threads(p.rows, p.vocab, p.k <= kPartTeacher);
-  p.chunks = vocab_chunks(p.vocab, dtype, nt);
+  set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
     launch_kernel(distill_bwd_kernel<DUAL, NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s);
@@ -1456,8 +1473,8 @@ extern "C" int32_t m3s_logprob_bwd(const m3s_logprob_args* a, void* stream) {
               "m3s_logprob_bwd: NULL or misaligned pointer");
   LogprobParams p = logprob_params(a);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->dtype == M3S_DTYPE_BF16) launch_logprob_bwd<bf16>(p, a->dtype, s);
-  else launch_logprob_bwd<float>(p, a->dtype, s);
+  if (a->dtype == M3S_DTYPE_BF16) launch_logprob_bwd<bf16>(p, s);
+  else launch_logprob_bwd<float>(p, s);
   return launch_status("m3s_logprob_bwd");
 }
 
@@ -1499,7 +1516,7 @@ extern "C" int32_t m3s_distill_bwd(const m3s_distill_args* a, void* stream) {
   DistillParams p = distill_params(a);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const bool b = a->dtype == M3S_DTYPE_BF16, dual = p.dkd && p.dnll && p.temp != 1.f;
-  if (dual) b ? launch_distill_bwd<true, bf16>(p, a->dtype, s) : launch_distill_bwd<true, float>(p, a->dtype, s);
-  else b ? launch_distill_bwd<false, bf16>(p, a->dtype, s) : launch_distill_bwd<false, float>(p, a->dtype, s);
+  if (dual) b ? launch_distill_bwd<true, bf16>(p, s) : launch_distill_bwd<true, float>(p, s);
+  else b ? launch_distill_bwd<false, bf16>(p, s) : launch_distill_bwd<false, float>(p, s);
   return launch_status("m3s_distill_bwd");
 }

@@ -54,7 +54,7 @@ def skewed(vocab, shape, gen, dtype=torch.int64):
 @pytest.mark.parametrize("vocab,d,shape,scale", [
     (1, 1, (1,), 1.0), (7, 3, (5, 2), 1.0), (40, 5, (64,), 2.5), (256, 768, (3, 700), 1.0),
     (257, 260, (4097,), 0.5), (511, 64, (2, 2500), 1.0), (512, 17, (33, 3), 1.0),
-    (5003, 515, (4, 1025), 22.7), (70001, 36, (9000,), 6.0), (300007, 8, (3001,), 1.0)])
+    (5003, 515, (4, 1025), 22.7), (300, 1100, (2000,), 1.0), (70001, 36, (9000,), 6.0), (300007, 8, (3001,), 1.0)])
 def test_lookup_and_gradient(m3, dev, dtype, ids, vocab, d, shape, scale):
     gen = torch.Generator().manual_seed(vocab + d)
     table = torch.randn(vocab, d, generator=gen).to(dtype)
