@@ -20,6 +20,8 @@
 //      partial sum.
 //   3. finish: the workgroup of the piece that a crossing run starts in adds its partials, in order.
 //
+// Up to 1024 tokens a single launch does without the sort: each workgroup lists its own rows' tokens.
+//
 // Every sum is float32 in a fixed order, rounded once. The gradient reads dy once and writes the
 // table once (a row that occurs twice): bound by HBM from a few MB on, by the launches below that.
 //
@@ -27,7 +29,7 @@
 // 33 us, of which run_sum 18 (5.6 TB/s of dy), the sort 8 and finish 6. 16384 tokens of 50001, D 1024:
 // gradient 61 us, of which clearing 205 MB beside the four sort launches takes 36 (5.7 TB/s) and
 // run_sum 20 to 25; cleared by a pass of its own behind the sort it took 96 in all. 777 tokens of
-// 32003, D 515, bf16: 16 us, three launches.
+// 32003, D 515, bf16: 12.3 us in one launch (2.7 TB/s, the table's 33 MB), 16.4 sorted.
 #include <algorithm>
 
 #include "m3s_common.h"
@@ -458,6 +460,132 @@ __global__ void __launch_bounds__(256) finish_kernel(const uint32_t* __restrict_
   }
 }
 
+// ---- sums by id, few tokens --------------------------------------------------------------------
+// One launch without a sort: every workgroup reads all ids and lists the tokens of its own rows. Beside
+// the sort (three launches and a workspace) Zipf-distributed ids of 256, D 768, float32, take 3.6 us
+// against 9.7 at 64 tokens and 6.7 against 11.4 at 1024; 1024 of 50001 ids, D 1024, 29.9 against 34.6
+// (7.0 TB/s). What it is slower at is a single id on all of the tokens, whose rows one workgroup of
+// each slice then adds: 16.6 against 10.6 at 512, 29.6 against 12.3 at 1024. There it ends: at 2048
+// Zipf's ids would gain a sixth, and the single id lose 50 us.
+constexpr int kGatherTokens = 1024, kGatherRounds = kGatherTokens / 256;
+constexpr int kGatherRows = 1024;   // rows of a workgroup's, at most
+constexpr int kAlone = 16;          // tokens of a row that one wave adds alone: two rounds of loads
+
+// The rows of dy of those of hit[lo .. hi - 1] that belong to row j of the workgroup's, added in order.
+template <int W, typename T>
+__device__ __forceinline__ cols<W> sum_hits(const uint32_t* hit, int lo, int hi, uint32_t j,
+                                            const T* __restrict__ dy, int D, int c) {
+  cols<W> acc = 0.f;
+  for (int i0 = lo; i0 < hi; i0 += 64) {
+    const int i = i0 + lane_id();
+    const uint32_t e = hit[min(i, hi - 1)];
+    uint64_t m = __ballot(i < hi && e / kGatherTokens == j);
+    while (m) {
+      cols<W> v[8];
+      int held = 0, at = 0;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {   // past the last one its row again, not added
+        if (m) {
+          at = __builtin_ctzll(m);
+          m &= m - 1;
+          held = u + 1;
+        }
+        const int64_t row = (uint32_t)__builtin_amdgcn_readlane((int)e, at) % kGatherTokens;
+        v[u] = ld_cols<W>(dy + row * D + c);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (u < held) acc += v[u];
+      }
+    }
+  }
+  return acc;
+}
+
+// Workgroup (b, y) owns a row of each 2^lg of the table, 64 W columns of them: its row j is row
+// (b ^ j) mod 2^lg of the j-th 2^lg, so that neither neighbours (frequent ids often are) nor every 2^lg-th
+// row meet in one workgroup. It lists its rows' tokens in order and clears the rows without any; a row
+// of up to kAlone tokens is added by one wave, a longer one by all four, a quarter of the list each.
+template <int W, typename T, typename ID>
+__global__ void __launch_bounds__(256) gather_kernel(const ID* __restrict__ ids,
+                                                     const T* __restrict__ dy, T* __restrict__ dtable,
+                                                     int n, int vocab, int64_t pad, int D, float scale,
+                                                     int lg) {
+  __shared__ uint32_t hit[kGatherTokens];   // j, token
+  __shared__ uint32_t count[kGatherRows];   // tokens of row j
+  __shared__ int held[4];
+  __shared__ cols<W> sums[4][64];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t b = blockIdx.x, mask = (1u << lg) - 1;
+  const int rows = (int)(((int64_t)vocab + mask) >> lg);   // the last may lie past the table
+  const bool mine = W * (64 * (int)blockIdx.y + lane) < D;
+  const int c = min(W * (64 * (int)blockIdx.y + lane), D - W);
+  const auto store = [&](int j, cols<W> v) {
+    const int64_t id = ((int64_t)j << lg) + ((b ^ (uint32_t)j) & mask);
+    if (mine && id < vocab) st_cols<W>(dtable + id * D + c, v);
+  };
+  for (int j = threadIdx.x; j < rows; j += 256) count[j] = 0;
+  // wave w looks at kGatherTokens / 4 of the tokens from there on
+  const int t0 = wave * (kGatherTokens / 4) + lane;
+  uint32_t key[kGatherRounds];
+  uint64_t m[kGatherRounds];
+  int found = 0;
+#pragma unroll
+  for (int r = 0; r < kGatherRounds; ++r) {
+    key[r] = t0 + 64 * r < n ? sort_key(ids[t0 + 64 * r], vocab, pad) : (uint32_t)vocab;
+  }
+#pragma unroll
+  for (int r = 0; r < kGatherRounds; ++r) {
+    m[r] = __ballot(key[r] < (uint32_t)vocab && ((key[r] ^ (key[r] >> lg)) & mask) == b);
+    found += __popcll(m[r]);
+  }
+  if (lane == 0) held[wave] = found;
+  __syncthreads();
+  int at = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    at += w < wave ? held[w] : 0;
+    all += held[w];
+  }
+  all = __builtin_amdgcn_readfirstlane(all);
+#pragma unroll
+  for (int r = 0; r < kGatherRounds; ++r) {
+    if ((m[r] >> lane) & 1) {
+      const uint32_t j = key[r] >> lg;
+      hit[at + __popcll(m[r] & ((1ull << lane) - 1))] = j * kGatherTokens + t0 + 64 * r;
+      atomicAdd(&count[j], 1u);
+    }
+    at += __popcll(m[r]);
+  }
+  __syncthreads();
+  for (int j = wave; j < rows; j += 4) {
+    if (count[j] == 0) store(j, cols<W>(0.f));
+  }
+  if (all == 0) return;
+  int k = 0;
+  for (int j0 = 0; j0 < rows; j0 += 64) {
+    const uint32_t tokens = j0 + lane < rows ? count[j0 + lane] : 0;
+    for (uint64_t few = __ballot(tokens > 0 && tokens <= kAlone); few; few &= few - 1, ++k) {
+      if ((k & 3) != wave) continue;
+      const int j = j0 + __builtin_ctzll(few);
+      store(j, sum_hits<W>(hit, 0, all, j, dy, D, c) * scale);
+    }
+  }
+  if (all <= kAlone) return;
+  const int share = (all + 3) / 4, lo = wave * share, hi = min(lo + share, all);
+  for (int j0 = 0; j0 < rows; j0 += 64) {
+    const uint32_t tokens = j0 + lane < rows ? count[j0 + lane] : 0;
+    for (uint64_t many = __ballot(tokens > kAlone); many; many &= many - 1) {
+      const int j = j0 + __builtin_ctzll(many);
+      const cols<W> acc = sum_hits<W>(hit, lo, hi, j, dy, D, c);
+      sums[wave][lane] = acc;
+      __syncthreads();
+      if (wave == 0) store(j, (((acc + sums[1][lane]) + sums[2][lane]) + sums[3][lane]) * scale);
+      __syncthreads();
+    }
+  }
+}
+
 // ---- host ------------------------------------------------------------------------------------
 struct EmbedSpace {
   int64_t keys[2], pos[2], hist, part, total;   // byte offsets
@@ -465,7 +593,8 @@ struct EmbedSpace {
 };
 
 static EmbedSpace embed_space(int64_t n, int64_t D) {   // for the wider of the two types, float32
-  EmbedSpace s;
+  EmbedSpace s = {};
+  if (n <= kGatherTokens) return s;   // no sort
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -519,10 +648,20 @@ static void launch_sums(const m3s_embed_args* a, const uint32_t* keys, const uin
 template <int W, typename T, typename ID>
 static void launch_embed_bwd(const m3s_embed_args* a, hipStream_t s) {
   const int64_t n = a->tokens;
+  const ID* ids = static_cast<const ID*>(a->ids);
+  const T* dy = static_cast<const T*>(a->dy);
+  T* dtable = static_cast<T*>(a->dtable);
   const EmbedSpace sp = embed_space(n, a->width);
+  if (sp.total == 0) {
+    int lg = 0;   // 1024 workgroups to a slice, four to a CU: more would each read the ids again
+    while (lg < 10 && (1 << lg) < a->vocab) ++lg;
+    while (((int64_t)kGatherRows << lg) < a->vocab) ++lg;
+    hipLaunchKernelGGL((gather_kernel<W, T, ID>), dim3(1u << lg, (a->width + 64 * W - 1) / (64 * W)), dim3(256), 0, s,
+                       ids, dy, dtable, (int)n, a->vocab, a->padding_idx, a->width, a->scale, lg);
+    return;
+  }
   char* w = static_cast<char*>(a->workspace);
   const auto u32 = [&](int64_t off) { return reinterpret_cast<uint32_t*>(w + off); };
-  const ID* ids = static_cast<const ID*>(a->ids);
   int width = 1;   // bits of a key: 0 .. vocab
   while ((uint64_t)a->vocab >> width) ++width;
   const int passes = (width + kDigitBits - 1) / kDigitBits, bits = (width + passes - 1) / passes;
@@ -607,10 +746,11 @@ static int32_t check_embed(const m3s_embed_args* a, const char* who, bool bwd) {
     M3S_REQUIRE(a->table_stride >= 0, "%s: negative table stride", who);
     return 0;
   }
-  M3S_REQUIRE(a->dtable && a->workspace && (a->tokens == 0 || (a->ids && a->dy)), "%s: NULL pointer", who);
+  M3S_REQUIRE(a->dtable && (a->tokens == 0 || (a->ids && a->dy)), "%s: NULL pointer", who);
   M3S_REQUIRE((uintptr_t)a->dy % es == 0, "%s: misaligned rows", who);
   M3S_REQUIRE(aligned16(a->workspace) && aligned16(a->dtable), "%s: dtable and workspace must be 16-byte aligned", who);
-  const int64_t need = embed_space(a->tokens, a->width).total;
+  const int64_t need = embed_space(a->tokens, a->width).total;   // none for few tokens
+  M3S_REQUIRE(need == 0 || a->workspace, "%s: NULL pointer", who);
   M3S_REQUIRE(a->workspace_bytes >= need, "%s: workspace of %lld bytes, needs %lld", who,
               (long long)a->workspace_bytes, (long long)need);
   return 0;

@@ -1439,9 +1439,10 @@ def embedding_call_backward(a: "_lib.EmbedArgs", dev: torch.device, dy: Tensor) 
     if nbytes < 0:
         raise ValueError(f"embedding: bad sizes (tokens {n}, vocab {v}, width {d})")
     dtable = empty(v, d, device=dev, dtype=dy.dtype)
-    ws = empty(nbytes, device=dev, dtype=torch.uint8)
     a.dy, a.dtable = dy.data_ptr(), dtable.data_ptr()
-    a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    if nbytes:
+        ws = empty(nbytes, device=dev, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
     _lib.launch(_lib.load().m3s_embed_bwd, a, dev, "m3s_embed_bwd")
     return dtable
 
@@ -1450,7 +1451,7 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
                        padding_idx: Optional[int] = None) -> Tensor:
     """The table's cotangent of `embedding_forward` (one ``m3s_embed_bwd`` call): ``dy``
     (tokens.shape, D) -> dense (vocab, D) in dy's dtype, each row the float32 sum of its tokens'
-    rows in position order (a stable sort by id; bit-reproducible), times ``scale``.
+    rows in a fixed order (bit-reproducible), times ``scale``.
     ``padding_idx`` (negative: from the end) gets a row of zeros; ids outside [0, vocab) add to
     no row."""
     if dy.shape[:-1] != tokens.shape or dy.dim() == 0:

@@ -89,6 +89,30 @@ def test_sort_sizes_and_single_ids(m3, dev, n):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab,d", [(1, 6), (3, 700), (1023, 40), (1024, 515), (1025, 260), (2049, 9), (70001, 300),
+                                     (1100003, 8)])
+def test_few_tokens(m3, dev, dtype, vocab, d):
+    """Up to 1024 tokens, which are listed and not sorted: rows of one token, of the most that one wave
+    adds, of more, and of all; tables whose rows end inside a stride; ids one stride apart."""
+    gen = torch.Generator().manual_seed(vocab + d)
+    for n in (1, 16, 17, 63, 65, 500, 1000, 1024):
+        dy = torch.randn(n, d, generator=gen).to(dtype)
+        hot = skewed(vocab, (n,), gen)
+        hot[torch.rand(n, generator=gen) < 0.3] = vocab - 1
+        pairs = torch.arange(n) // 16 % vocab
+        strides = torch.arange(n) * 1024 % vocab
+        for tokens in (torch.full((n,), vocab // 2), hot, pairs, strides, torch.randperm(n, generator=gen) % vocab):
+            got = m3.kernels.embedding_backward(tokens.to(dev), dy.to(dev), vocab, 0.5)
+            check_grad(got, tokens, dy, 0.5, None)
+        holes = hot.clone()
+        holes[::3] = torch.tensor([-1, vocab, 1 << 40])[torch.arange(len(holes[::3])) % 3]
+        dy[::3] = float("nan")   # read by nobody
+        for pad in (None, vocab - 1):
+            got = m3.kernels.embedding_backward(holes.to(dev), dy.to(dev), vocab, 0.5, padding_idx=pad)
+            check_grad(got, holes, dy, 0.5, pad)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_padding_and_ids_outside_the_table(m3, dev, dtype):
     """The padding id's row is looked up and gets zeros back; an id outside the table gives NaN and
     adds to no row, whatever its cotangent holds."""

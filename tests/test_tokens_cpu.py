@@ -44,9 +44,9 @@ def test_embed_abi_refuses_bad_structs(m3):
     def args(**kw):
         a = lib.EmbedArgs()
         a.struct_size, a.dtype, a.id_bytes = ctypes.sizeof(lib.EmbedArgs), lib.DTYPE_F32, 8
-        a.vocab, a.width, a.tokens, a.padding_idx, a.table_stride = 10, 4, 6, -1, 4
+        a.vocab, a.width, a.tokens, a.padding_idx, a.table_stride = 10, 4, 2000, -1, 4
         a.ids = a.table = a.y = a.dy = a.dtable = a.workspace = 4096   # never read: every call is refused
-        a.workspace_bytes = h.m3s_embed_bwd_workspace_bytes(6, 10, 4)
+        a.workspace_bytes = h.m3s_embed_bwd_workspace_bytes(2000, 10, 4)
         for k, v in kw.items():
             setattr(a, k, v)
         return a
@@ -61,6 +61,8 @@ def test_embed_abi_refuses_bad_structs(m3):
     assert h.m3s_embed_fwd(ctypes.byref(args(tokens=0)), None) == lib.OK   # nothing to launch
     for sizes in ((-1, 10, 4), (6, 0, 4), (6, 10, 0), (1 << 31, 10, 4)):
         assert h.m3s_embed_bwd_workspace_bytes(*sizes) == -1
+    assert h.m3s_embed_bwd_workspace_bytes(1024, 10, 4) == 0   # few tokens are not sorted
+    assert h.m3s_embed_bwd_workspace_bytes(1025, 10, 4) > 0
 
 
 def test_structs_match_the_header(m3, tmp_path):
