@@ -1385,18 +1385,23 @@ def _row_grad(t: Optional[Tensor]) -> Optional[Tensor]:
 
 
 class Call(NamedTuple):
-    """A launched forward call as its autograd node keeps it: the args struct, the device, and the
-    addresses of the operands that the node saves. The backward runs on a thread of its own, whose
+    """A launched forward call as its autograd node keeps it: the args struct, the device, the
+    addresses of the operands that the node saves, and the strides of the first of them (the others
+    are dense). The backward runs on a thread of its own, whose
     core finds every Python object in another's cache (a forward and backward of 64 rows: 120 us
     with the operands checked anew, 90 so), so it fills in a copy of the struct instead."""
 
     args: ctypes.Structure
     device: torch.device
     addresses: tuple
+    strides: Optional[tuple]
 
     def again(self, tensors):
-        """A copy of the struct, or None where a saved tensor came back at another address (hooks
-        on saved tensors may do that) or the call had read a copy of it."""
+        """A copy of the struct, or None where a saved tensor came back at another address or with
+        other strides (hooks on saved tensors may do that; a compact copy may well stand where the
+        view stood) or the call had read a copy of it (``strides`` is None then)."""
+        if tensors[0].stride() != self.strides:
+            return None
         for t, at in zip(tensors, self.addresses):
             if (t.data_ptr() or None if t is not None else None) != at:
                 return None
@@ -1420,7 +1425,7 @@ def embedding_call(table: Tensor, tokens: Tensor, scale: float, padding_idx: int
     a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, v, d, scale, tokens.numel(), padding_idx,
                        tokens.data_ptr(), table.data_ptr(), row, y.data_ptr())
     _lib.launch(_lib.load().m3s_embed_fwd, a, dev, "m3s_embed_fwd")
-    return y, tokens, Call(a, dev, (a.ids,))
+    return y, tokens, Call(a, dev, (a.ids,), tokens.stride())
 
 
 def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
@@ -1493,6 +1498,11 @@ def _logit_rows(logits: Tensor, what: str):
     return logits, _lib.Blx(logits.data_ptr(), sb, st)
 
 
+def _read_strides(logits: Tensor, rows: Tensor) -> Optional[tuple]:
+    """The strides by which a call read ``logits`` itself; None where ``rows`` is a copy of it."""
+    return logits.stride() if rows.data_ptr() == logits.data_ptr() else None
+
+
 def _row_values(t: Optional[Tensor], shape, dtype: torch.dtype, what: str) -> Optional[Tensor]:
     """A dense per-row operand of the given shape and dtype, or None."""
     if t is None:
@@ -1557,7 +1567,7 @@ def logprob_call(logits: Tensor, targets: Optional[Tensor], top: int, temperatur
         a.top_logp, a.top_ids = top_logp.data_ptr(), top_ids.data_ptr()
     ws = _row_scratch(a, dev, "m3s_logprob_workspace_bytes", b * l, v, top)  # noqa: F841
     _lib.launch(_lib.load().m3s_logprob_fwd, a, dev, "m3s_logprob_fwd")
-    call = Call(a, dev, (a.logits.ptr, a.targets, a.stats, a.top_ids)) if keep else None
+    call = Call(a, dev, (a.logits.ptr, a.targets, a.stats, a.top_ids), _read_strides(logits, rows)) if keep else None
     return (logp, entropy, top_logp, top_ids, stats), targets, call
 
 
@@ -1660,7 +1670,10 @@ def distill_call(logits: Tensor, teacher_ids: Tensor, teacher_logits: Tensor,
         a.stats = stats.data_ptr()
     ws = _row_scratch(a, dev, "m3s_distill_workspace_bytes", a.batch * a.seqlen, a.vocab)  # noqa: F841
     _lib.launch(_lib.load().m3s_distill_fwd, a, dev, "m3s_distill_fwd")
-    call = Call(a, dev, (a.logits.ptr, a.teacher_ids, a.teacher_logits, a.targets, a.stats)) if keep else None
+    call = None
+    if keep:
+        call = Call(a, dev, (a.logits.ptr, a.teacher_ids, a.teacher_logits, a.targets, a.stats),
+                    _read_strides(logits, ops[0]))
     return (kd, nll, stats), ops[1:], call
 
 

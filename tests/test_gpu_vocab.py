@@ -590,6 +590,38 @@ def test_backward_of_saved_tensors_elsewhere_and_twice(m3, dev):
         torch.autograd.grad(outs[0], xg)
 
 
+def test_backward_of_saved_logits_with_other_strides(m3, dev):
+    """A view's logits that come back from a hook as a compact copy, at the address that the view had:
+    the same gradients as without the hook."""
+    gen = torch.Generator().manual_seed(23)
+    leaf = make_logits((2, 6, 300), torch.float32, gen).to(dev).requires_grad_(True)
+    t = torch.randint(0, 300, (2, 5), generator=gen).to(dev)
+    ids, u = (a.to(dev) for a in teacher_of(leaf.detach().cpu()[:, :-1], 8, gen, torch.float32))
+
+    def losses(full):
+        lp = m3.token_logprobs(full[:, :-1], t, top=4)
+        kd = m3.distill_loss(full[:, :-1], ids, u, temperature=2.0, targets=t)
+        return lp.logp.sum() + lp.entropy.sum() + lp.top_logp.sum(), kd.kd.sum() + kd.nll.sum()
+
+    want = [torch.autograd.grad(losses(leaf * 1.0)[i], leaf)[0] for i in (0, 1)]
+    for i in (0, 1):
+        full = leaf * 1.0
+
+        def unpack(held):
+            if held.shape != (2, 5, 300):
+                return held
+            place = full.detach().reshape(-1)[:held.numel()].view(held.shape)
+            assert place.data_ptr() == full.data_ptr()
+            return place.copy_(held)
+
+        def pack(saved):   # the small operands stay where they are
+            return saved.detach().cpu().contiguous() if saved.shape == (2, 5, 300) else saved.detach()
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = losses(full)[i]
+        assert torch.equal(torch.autograd.grad(out, leaf)[0], want[i])
+
+
 def test_nodes_refuse_what_they_cannot_do(m3, dev):
     x = torch.randn(3, 10, device=dev, requires_grad=True)
     t = torch.tensor([1, 2, 3], device=dev)
