@@ -22,9 +22,9 @@
 // Rows may start at any element: 16-byte accesses need no alignment on gfx950.
 //
 // Measured (us; TB/s of logits read and gradients written): log-probability and entropy of 8192 x
-// 32000 float32, a tenth of it padding, forward 191 (4.9), backward 330 (6.0); distillation of 8192 x
-// 50001 float32 with 32 teacher tokens and the cross-entropy, forward 253 (5.8), backward 490 (6.4);
-// of 2048 x 65536 bf16, 59 (4.5) and 105 (5.1): there the exponentials take as long as the bytes. A
+// 32000 float32, a tenth of it padding, forward 166 (5.7), backward 345 (5.8); distillation of 8192 x
+// 50001 float32 with 32 teacher tokens and the cross-entropy, forward 253 (5.8), backward 515 (6.1);
+// of 2048 x 65536 bf16, 58 (4.6) and 106 (5.1): there the exponentials take as long as the bytes. A
 // large copy moves 5.0 TB/s. 32768 x 256 float32, 16 teacher tokens: 11.3 and 18.2, what is done once
 // a row (sums over lanes, logarithms, the entries) taking half of it.
 #include <algorithm>
