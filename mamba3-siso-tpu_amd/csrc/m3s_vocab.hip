@@ -255,6 +255,25 @@ struct Rows {
   }
 };
 
+// The sums of a batch that may be the row's last, only of the pieces that it has; its largest logit.
+template <typename G, int U, int MODE, typename T>
+__device__ __forceinline__ float last_batch(RowSums<MODE>& r, const float* v, int n, int batch, float c,
+                                            float c1) {
+  using R = Rows<G, U, T>;
+  const int full = n / R::N;
+  float most = kNegInf;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (batch * R::HOP + u * G::NT >= full) break;
+    float top = v[u * R::N];
+#pragma unroll
+    for (int i = 1; i < R::N; ++i) top = fmaxf(top, v[u * R::N + i]);
+    most = fmaxf(most, top);
+    r.template add<R::N>(v + u * R::N, top, c, c1);
+  }
+  return most;
+}
+
 // One pass over n logits by the group.
 template <typename G, int U, bool TOP, int MODE, typename T>
 __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* __restrict__ x, int n,
@@ -270,18 +289,10 @@ __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* 
     if constexpr (TOP) best.see(top, b);
     r.template add<R::LEN>(v, top, c, c1);
   }
-  if (batches * R::HOP < full) {   // the last batch, only the pieces that it has
-    float v[R::LEN], most = kNegInf;
+  if (batches * R::HOP < full) {
+    float v[R::LEN];
     R::load(x, n, batches, v);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (batches * R::HOP + u * G::NT >= full) break;
-      float top = v[u * R::N];
-#pragma unroll
-      for (int i = 1; i < R::N; ++i) top = fmaxf(top, v[u * R::N + i]);
-      most = fmaxf(most, top);
-      r.template add<R::N>(v + u * R::N, top, c, c1);
-    }
+    const float most = last_batch<G, U, MODE, T>(r, v, n, batches, c, c1);
     if constexpr (TOP) best.see(most, batches);
   }
   const int at = n / R::N * R::N + G::tid();
@@ -582,17 +593,28 @@ template <int n>
 __device__ __forceinline__ float row_turned(float v) {   // lane i of 16 reads another, n places on
   return dpp_mov<0x120 + n>(v);
 }
+template <typename T> constexpr int kPartPieces = kPartPick / (16 * Piece<T>::N);
+template <typename T> constexpr int kPartHeld = kPartPieces<T> * Piece<T>::N;
+// The row, held: v[kPartHeld] is what fills no piece. Missing ones are -inf. Its sums.
+template <typename G, int MODE, typename T>
+__device__ __forceinline__ void hold_part(RowSums<MODE>& r, float* v, const T* __restrict__ x, int n, float c,
+                                          float c1) {
+  using R = Rows<G, kPartPieces<T>, T>;
+  const int tail = n / R::N * R::N + G::tid();
+  R::load(x, n, 0, v);
+  v[R::LEN] = tail < n ? (float)x[tail] : kNegInf;
+  last_batch<G, kPartPieces<T>, MODE, T>(r, v, n, 0, c, c1);
+  if (tail < n) r.template add<1>(v + R::LEN, v[R::LEN], c, c1);
+}
 template <typename G, typename T, typename OUT>
-__device__ __forceinline__ void pick_part(const T* __restrict__ x, int n, int k, PartSpace& sp, OUT&& out) {
-  constexpr int N = Piece<T>::N, U = kPartPick / (G::NT * N), LEN = U * N;
-  using R = Rows<G, U, T>;
+__device__ __forceinline__ void pick_part(float* v, int n, int k, PartSpace& sp, OUT&& out) {
+  constexpr int N = Piece<T>::N, LEN = kPartHeld<T>;
+  using R = Rows<G, kPartPieces<T>, T>;
   const float gone = __builtin_nanf("");   // no logit, or one that is out already
   const int whole = n / N * N, tail = whole + G::tid();
-  float v[LEN + 1];
-  R::load(x, n, 0, v);
 #pragma unroll
   for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) < whole ? v[i] : gone;
-  v[LEN] = tail < n ? (float)x[tail] : gone;
+  v[LEN] = tail < n ? v[LEN] : gone;
   if (k > 2) {
     float most = kNegInf;
 #pragma unroll
@@ -742,7 +764,9 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
     const float xt = target_logit(p, tgt, x);
     RowSums<kEntropy> sum;
     Best best;
-    row_pass<G, U, PICK && NT == 256>(sum, best, x, p.vocab, p.c, 0.f);
+    float held[TOP && NT == 16 ? kPartHeld<T> + 1 : 1];
+    if constexpr (TOP && NT == 16) hold_part<G>(sum, held, x, p.vocab, p.c, 0.f);
+    else row_pass<G, U, PICK && NT == 256>(sum, best, x, p.vocab, p.c, 0.f);
     sum.template join<G>(p.c, 0.f, tmp);
     const LogprobRow logp(sum, p.inv_t);
     logprob_store<G>(p, r, tgt, xt, sum, logp);
@@ -756,7 +780,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
         p.top_ids[r * p.top + j] = i;
       };
       if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
-      else pick_part<G>(x, p.vocab, p.top, space[G::slot()], out);
+      else pick_part<G, T>(held, p.vocab, p.top, space[G::slot()], out);
     }
   }
 }
