@@ -607,15 +607,12 @@ __device__ __forceinline__ void hold_part(RowSums<MODE>& r, float* v, const T* _
   if (tail < n) r.template add<1>(v + R::LEN, v[R::LEN], c, c1);
 }
 template <typename G, typename T, typename OUT>
-__device__ __forceinline__ void pick_part(float* v, int n, int k, PartSpace& sp, OUT&& out) {
+__device__ __forceinline__ void pick_part(const T* __restrict__ x, float* v, int n, int k, PartSpace& sp,
+                                          OUT&& out) {
   constexpr int N = Piece<T>::N, LEN = kPartHeld<T>;
   using R = Rows<G, kPartPieces<T>, T>;
-  const float gone = __builtin_nanf("");   // no logit, or one that is out already
   const int whole = n / N * N, tail = whole + G::tid();
-#pragma unroll
-  for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) < whole ? v[i] : gone;
-  v[LEN] = tail < n ? v[LEN] : gone;
-  if (k > 2) {
+  if (k > 1) {
     float most = kNegInf;
 #pragma unroll
     for (int i = 0; i <= LEN; ++i) most = fmaxf(most, v[i]);
@@ -628,16 +625,16 @@ __device__ __forceinline__ void pick_part(float* v, int n, int k, PartSpace& sp,
     against(row_turned<10>(most)), against(row_turned<11>(most)), against(row_turned<12>(most));
     against(row_turned<13>(most)), against(row_turned<14>(most)), against(row_turned<15>(most));
     const float bar = G::max(reach >= k ? most : kNegInf, nullptr);
-    int mine = 0;
+    uint32_t hits = 0;
 #pragma unroll
-    for (int i = 0; i <= LEN; ++i) mine += v[i] >= bar;
-    const float upto = row_prefix16((float)mine);
+    for (int i = 0; i <= LEN; ++i) hits |= v[i] >= bar ? 1u << i : 0u;
+    const float upto = row_prefix16((float)__popc(hits));
     const int total = (int)G::max(upto, nullptr);
-    if (total <= PartSpace::CAP) {
-      int at = (int)upto - mine;
-#pragma unroll
-      for (int i = 0; i <= LEN; ++i) {
-        if (v[i] >= bar) sp.list[at++] = candidate(v[i], i < LEN ? R::place(0, i) : tail);
+    if (bar > kNegInf && total <= PartSpace::CAP) {   // -inf may be a logit or none
+      int at = (int)upto - __popc(hits);
+      for (; hits; hits &= hits - 1) {   // read again: few, and no register has a running index
+        const int i = __builtin_ctz(hits), where = i < LEN ? R::place(0, i) : tail;
+        sp.list[at++] = candidate((float)x[where], where);
       }
       if (G::tid() < 4) sp.list[total + G::tid()] = 0;   // below every candidate
       G::sync();
@@ -654,21 +651,27 @@ __device__ __forceinline__ void pick_part(float* v, int n, int k, PartSpace& sp,
       return;
     }
   }
+  const float gone = __builtin_nanf("");   // no logit, or one that is out already
+#pragma unroll
+  for (int i = 0; i < LEN; ++i) v[i] = i / N * G::NT + G::tid() < n / N ? v[i] : gone;
+  v[LEN] = tail < n ? v[LEN] : gone;
   for (int j = 0; j < k; ++j) {
     float top = v[LEN];
 #pragma unroll
     for (int i = 0; i < LEN; ++i) top = fmaxf(top, v[i]);
     top = G::max(top, nullptr);
-    int at = v[LEN] == top ? tail : 0x7fffffff;
+    int own = LEN + 1;   // a lane's places rise with i
 #pragma unroll
-    for (int i = LEN - 1; i >= 0; --i) at = v[i] == top ? R::place(0, i) : at;
+    for (int i = LEN; i >= 0; --i) own = v[i] == top ? i : own;
+    const int mine = own > LEN ? 0x7fffffff : own < LEN ? R::place(0, own) : tail;
+    int at = mine;
     at = min(at, dpp_int<kDppQuadSwap1>(at));
     at = min(at, dpp_int<kDppQuadSwap2>(at));
     at = min(at, dpp_int<kDppHalfMirror>(at));
     at = min(at, dpp_int<kDppRowMirror>(at));
+    own = mine == at ? own : -1;
 #pragma unroll
-    for (int i = 0; i < LEN; ++i) v[i] = R::place(0, i) == at ? gone : v[i];
-    v[LEN] = tail == at ? gone : v[LEN];
+    for (int i = 0; i <= LEN; ++i) v[i] = i == own ? gone : v[i];
     if (G::tid() == j) out(j, top, at);
   }
 }
@@ -780,7 +783,7 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
         p.top_ids[r * p.top + j] = i;
       };
       if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
-      else pick_part<G, T>(held, p.vocab, p.top, space[G::slot()], out);
+      else pick_part<G>(x, held, p.vocab, p.top, space[G::slot()], out);
     }
   }
 }
@@ -1398,8 +1401,10 @@ static void launch_logprob_fwd(const LogprobParams& p, hipStream_t s) {
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
     const int64_t blocks = (p.rows + ROWS - 1) / ROWS;
-    if (NT == 64 && p.vocab <= 64 * Piece<T>::N) launch_kernel(logprob_fwd_kernel<TOP, NT, 1, T>, blocks, p, s);
-    else launch_kernel(logprob_fwd_kernel<TOP, NT, U, T>, blocks, p, s);
+    if constexpr (NT == 64) {
+      if (p.vocab <= 64 * Piece<T>::N) return launch_kernel(logprob_fwd_kernel<TOP, NT, 1, T>, blocks, p, s);
+    }
+    launch_kernel(logprob_fwd_kernel<TOP, NT, U, T>, blocks, p, s);
   });
 }
 template <int MODE, typename T>
