@@ -46,7 +46,7 @@ constexpr int kTeacherMax = 256;   // teacher tokens of a row
 // against 15.6 / 16; but 512 x 4000: 5.2 / 6.0 against 4.9 / 6.0); the rest to a workgroup.
 constexpr int kPartVocab = 1024, kPartRows = 4096, kWaveVocab = 4096, kWaveRows = 1024;
 constexpr int kWaveHeld = 1024;     // one batch of a wave holds the row: it goes to one whatever the rows
-constexpr int kPartTop = 14;        // alternatives that 16 lanes pick, of rows up to kPartPick long
+constexpr int kPartTop = 24, kPartLanes = 8;        // alternatives that 16 lanes pick, of rows up to kPartPick long
 constexpr int kPartPick = 256;
 constexpr int kPartTeacher = 64;    // teacher tokens of a row of 16 lanes
 constexpr float kNegInf = -__builtin_inff();
@@ -580,18 +580,23 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
   G::sync();
 }
 
-// The same by 16 lanes that hold the row's at most kPartPick logits, for k < 16: the bound on the
-// lanes' maxima by comparing each with the others, the logits that reach it in a list, ranked. One or
-// two, and a list too long (ties, masked rows), go by rounds of (largest value, lowest index).
-// 32768 x 256 float32 takes 7 us, with 1, 5, 8 and 14 alternatives 10.9, 13.4, 14.4 and 23 (15, 18.7 and
-// 27 for the last three by rounds); with 20, by a wave, 30.
+// The same by 16 lanes that hold the row's at most kPartPick logits: the bound on the lanes' maxima by
+// comparing each with the others, beyond kPartLanes alternatives on two maxima of each (of 16 values
+// a k-th near the last lets most of the row through); the logits that reach it in a list, ranked. One,
+// and a list too long or a bound of -inf (ties, masked rows, fewer maxima than alternatives), go by
+// rounds of (largest value, lowest index). 32768 x 256 float32 takes 7 us, with 1, 5, 8, 14, 20 and 24
+// alternatives 9.6, 11.5, 12.6, 15.6, 19.5 and 24.8; by rounds 5 and 8 took 15 and 18.7, on one maximum
+// of each lane 14 took 22, and by a wave 20 and 24 took 29 and 30 (in bf16 42 and 46, here 18.6 and 24).
 struct PartSpace {
-  static constexpr int CAP = 64;
-  uint64_t list[CAP + 5];   // four zeros behind it; odd, so that the groups use different banks
+  static constexpr int CAP = 96;
+  uint64_t list[CAP + 5];   // four zeros behind it; odd: the groups use different banks
 };
-template <int n>
-__device__ __forceinline__ float row_turned(float v) {   // lane i of 16 reads another, n places on
-  return dpp_mov<0x120 + n>(v);
+// f(turned) for each of a lane's 15 neighbours in 16: turned(v) is that lane's v.
+template <int n = 1, typename F>
+__device__ __forceinline__ void others(F&& f) {
+  f([](float v) { return dpp_mov<0x120 + n>(v); });
+  __builtin_amdgcn_sched_barrier(0);
+  if constexpr (n < 15) others<n + 1>(f);
 }
 template <typename T> constexpr int kPartPieces = kPartPick / (16 * Piece<T>::N);
 template <typename T> constexpr int kPartHeld = kPartPieces<T> * Piece<T>::N;
@@ -613,18 +618,28 @@ __device__ __forceinline__ void pick_part(const T* __restrict__ x, float* v, int
   using R = Rows<G, kPartPieces<T>, T>;
   const int whole = n / N * N, tail = whole + G::tid();
   if (k > 1) {
-    float most = kNegInf;
+    float even = v[LEN], odd = kNegInf;   // a lane's largest of each kind
 #pragma unroll
-    for (int i = 0; i <= LEN; ++i) most = fmaxf(most, v[i]);
-    // the k-th largest of the lanes' maxima: the largest that k of them reach
-    int reach = 1;
-    const auto against = [&](float other) { reach += other >= most; };
-    against(row_turned<1>(most)), against(row_turned<2>(most)), against(row_turned<3>(most));
-    against(row_turned<4>(most)), against(row_turned<5>(most)), against(row_turned<6>(most));
-    against(row_turned<7>(most)), against(row_turned<8>(most)), against(row_turned<9>(most));
-    against(row_turned<10>(most)), against(row_turned<11>(most)), against(row_turned<12>(most));
-    against(row_turned<13>(most)), against(row_turned<14>(most)), against(row_turned<15>(most));
-    const float bar = G::max(reach >= k ? most : kNegInf, nullptr);
+    for (int i = 0; i < LEN; i += 2) {
+      even = fmaxf(even, v[i]);
+      odd = fmaxf(odd, v[i + 1]);
+    }
+    float bar;   // the k-th largest of the lanes' maxima, or of both of each: the largest that k of them reach
+    if (k <= kPartLanes) {
+      const float most = fmaxf(even, odd);
+      int reach = 1;
+      others([&](auto turned) { reach += turned(most) >= most; });
+      bar = reach >= k ? most : kNegInf;
+    } else {
+      int reach0 = 1 + (odd >= even), reach1 = 1 + (even >= odd);
+      others([&](auto turned) {
+        const float a = turned(even), b = turned(odd);
+        reach0 += (a >= even) + (b >= even);
+        reach1 += (a >= odd) + (b >= odd);
+      });
+      bar = fmaxf(reach0 >= k ? even : kNegInf, reach1 >= k ? odd : kNegInf);
+    }
+    bar = G::max(bar, nullptr);
     uint32_t hits = 0;
 #pragma unroll
     for (int i = 0; i <= LEN; ++i) hits |= v[i] >= bar ? 1u << i : 0u;
@@ -672,7 +687,7 @@ __device__ __forceinline__ void pick_part(const T* __restrict__ x, float* v, int
     own = mine == at ? own : -1;
 #pragma unroll
     for (int i = 0; i <= LEN; ++i) v[i] = i == own ? gone : v[i];
-    if (G::tid() == j) out(j, top, at);
+    if (G::tid() == (j & 15)) out(j, top, at);
   }
 }
 

@@ -211,6 +211,26 @@ def test_whole_rows_of_hard_kinds(m3, dev, dtype, rows, vocab):
         check_logprob(m3, dev, x, targets, top, 1.0, ("lht",) if top in (0, 20) else ())
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [24, 31, 64, 130, 251, 256])
+def test_many_short_rows(m3, dev, dtype, vocab):
+    """As many rows as make 16 lanes pick the alternatives of each, around the numbers at which they
+    do it another way: ordinary rows, masks, ties and flat rows, and rows that rise or fall throughout."""
+    gen = torch.Generator().manual_seed(vocab)
+    kinds = ("model", "masked", "flat", "ties", "wide")
+    x = torch.cat([make_logits((830, vocab), dtype, gen, k) for k in kinds])
+    x[3], x[5] = -INF, torch.finfo(dtype).min
+    x[7], x[8] = torch.arange(vocab).to(dtype), -torch.arange(vocab).to(dtype)
+    x[9, : vocab - 3], x[10, 5:] = -INF, -INF
+    x[11, ::16], x[12, 1::2] = 9.0, 9.0
+    targets = torch.randint(0, vocab, (len(x),), generator=gen)
+    targets[::11] = -100
+    for top in (1, 2, 7, 8, 9, 16, 17, 23, 24):
+        check_logprob(m3, dev, x, targets, top, 1.0, ())
+    if vocab > 24:
+        check_logprob(m3, dev, x, targets, 25, 1.0, ("lht",))
+
+
 @pytest.mark.parametrize("dtype,vocab", [(torch.float32, 1000), (torch.float32, 1024), (torch.bfloat16, 1023),
                                          (torch.float32, 250), (torch.bfloat16, 500)])
 def test_few_lanes_hold_more_than_the_list(m3, dev, dtype, vocab):
