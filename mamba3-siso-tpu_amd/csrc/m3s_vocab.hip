@@ -302,6 +302,18 @@ __device__ __forceinline__ void row_pass(RowSums<MODE>& r, Best& best, const T* 
   }
 }
 
+// A row of one batch and a rest, held: v[U N] is what fills no piece. Missing ones are -inf. Its sums.
+template <typename G, int U, int MODE, typename T>
+__device__ __forceinline__ void hold_row(RowSums<MODE>& r, float* v, const T* __restrict__ x, int n, float c,
+                                         float c1) {
+  using R = Rows<G, U, T>;
+  const int tail = n / R::N * R::N + G::tid();
+  R::load(x, n, 0, v);
+  v[R::LEN] = tail < n ? (float)x[tail] : kNegInf;
+  last_batch<G, U, MODE, T>(r, v, n, 0, c, c1);
+  if (tail < n) r.template add<1>(v + R::LEN, v[R::LEN], c, c1);
+}
+
 // a / b for a >= 0 and b > 0, without the 64-bit division's hundred instructions where it can be.
 __device__ __forceinline__ int64_t quotient(int64_t a, int b) {
   if (a < b) return 0;
@@ -363,6 +375,14 @@ __device__ __forceinline__ float kth_bound(const float* v, float top, int k, int
     }
   }
   return key_float(lo);
+}
+
+// Inclusive prefix sum over a wave's lanes: within the rows of 16, then their totals.
+__device__ __forceinline__ int wave_prefix(int v) {
+  const int p = (int)row_prefix16((float)v);   // exact: small
+  const int a = __builtin_amdgcn_readlane(p, 15), b = __builtin_amdgcn_readlane(p, 31);
+  const int c = __builtin_amdgcn_readlane(p, 47), row = lane_id() >> 4;
+  return p + (row > 0 ? a : 0) + (row > 1 ? b : 0) + (row > 2 ? c : 0);
 }
 
 // Candidates: (value, index) as one number, the better ones larger.
@@ -538,17 +558,14 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
 // maxima for few alternatives (one value a lane to count), on the logits themselves for more, of
 // which the lanes' maxima would let most of the row through.
 template <typename G, int U, typename T, typename OUT>
-__device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, float top, const Best&,
-                                     PickSpace<1>& sp, OUT&& out) {
+__device__ __forceinline__ void pick_held(const T* __restrict__ x, const float* v, int n, int k, float top,
+                                          PickSpace<1>& sp, OUT&& out) {
   using R = Rows<G, U, T>;
   constexpr int LEN = R::LEN;
   // so many lanes' logits all fit the list: no bound lets more of them through but by ties, and
   // what exceeds the tied value then comes from fewer than k lanes
   constexpr int LANES = std::min(64, PickSpace<1>::CAP / (LEN + 1)), FEW = std::min(24, LANES);
   const int whole = n / R::N * R::N, tail = whole + G::tid();
-  float v[LEN + 1];
-  R::load(x, n, 0, v);
-  v[LEN] = tail < n ? (float)x[tail] : kNegInf;
   float bar;
   if (k <= FEW) {
     float most = v[0];
@@ -560,15 +577,24 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
   }
   const auto gather = [&](auto strict) {
     constexpr bool STRICT = decltype(strict)::value;
-    if (G::tid() == 0) sp.count = 0;
-    G::sync();
+    uint32_t hits = 0;
 #pragma unroll
-    for (int i = 0; i < LEN; ++i) {
-      if (reaches<STRICT>(v[i], bar) && R::place(0, i) < whole) append(sp, v[i], R::place(0, i));
+    for (int i = 0; i <= LEN; ++i) hits |= reaches<STRICT>(v[i], bar) ? 1u << i : 0u;
+    if (bar == kNegInf) {   // where there is no logit stands -inf too
+#pragma unroll
+      for (int i = 0; i < LEN; ++i) hits &= R::place(0, i) < whole ? ~0u : ~(1u << i);
+      hits &= tail < n ? ~0u : ~(1u << LEN);
     }
-    if (reaches<STRICT>(v[LEN], bar) && tail < n) append(sp, v[LEN], tail);
+    const int mine = __popc(hits), upto = wave_prefix(mine), all = __builtin_amdgcn_readlane(upto, 63);
+    int at = upto - mine;
+    if (all <= PickSpace<1>::CAP) {
+      for (; hits; hits &= hits - 1) {   // read again: few, and no register has a running index
+        const int i = __builtin_ctz(hits), where = i < LEN ? R::place(0, i) : tail;
+        sp.list[at++] = candidate((float)x[where], where);
+      }
+    }
     G::sync();
-    return __builtin_amdgcn_readfirstlane(sp.count);
+    return all;
   };
   int count = gather(std::false_type());
   if (count > PickSpace<1>::CAP) {
@@ -598,24 +624,11 @@ __device__ __forceinline__ void others(F&& f) {
   __builtin_amdgcn_sched_barrier(0);
   if constexpr (n < 15) others<n + 1>(f);
 }
-template <typename T> constexpr int kPartPieces = kPartPick / (16 * Piece<T>::N);
-template <typename T> constexpr int kPartHeld = kPartPieces<T> * Piece<T>::N;
-// The row, held: v[kPartHeld] is what fills no piece. Missing ones are -inf. Its sums.
-template <typename G, int MODE, typename T>
-__device__ __forceinline__ void hold_part(RowSums<MODE>& r, float* v, const T* __restrict__ x, int n, float c,
-                                          float c1) {
-  using R = Rows<G, kPartPieces<T>, T>;
-  const int tail = n / R::N * R::N + G::tid();
-  R::load(x, n, 0, v);
-  v[R::LEN] = tail < n ? (float)x[tail] : kNegInf;
-  last_batch<G, kPartPieces<T>, MODE, T>(r, v, n, 0, c, c1);
-  if (tail < n) r.template add<1>(v + R::LEN, v[R::LEN], c, c1);
-}
-template <typename G, typename T, typename OUT>
+template <typename G, int U, typename T, typename OUT>
 __device__ __forceinline__ void pick_part(const T* __restrict__ x, float* v, int n, int k, PartSpace& sp,
                                           OUT&& out) {
-  constexpr int N = Piece<T>::N, LEN = kPartHeld<T>;
-  using R = Rows<G, kPartPieces<T>, T>;
+  using R = Rows<G, U, T>;
+  constexpr int N = R::N, LEN = R::LEN;
   const int whole = n / N * N, tail = whole + G::tid();
   if (k > 1) {
     float even = v[LEN], odd = kNegInf;   // a lane's largest of each kind
@@ -769,7 +782,7 @@ __device__ __forceinline__ void logprob_unordered(const LogprobParams& p, int64_
 template <bool TOP, int NT, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobParams p) {
   using G = Group<NT>;
-  constexpr bool PICK = TOP && NT > 16;
+  constexpr bool HELD = TOP && NT < 256;   // the row stays in registers between its sums and the pick
   __shared__ float tmp[G::TMP];
   __shared__ std::conditional_t<NT == 16, PartSpace, PickSpace<NT == 256 ? 4 : 1>> space[TOP ? G::ROWS : 1];
   for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
@@ -782,9 +795,9 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
     const float xt = target_logit(p, tgt, x);
     RowSums<kEntropy> sum;
     Best best;
-    float held[TOP && NT == 16 ? kPartHeld<T> + 1 : 1];
-    if constexpr (TOP && NT == 16) hold_part<G>(sum, held, x, p.vocab, p.c, 0.f);
-    else row_pass<G, U, PICK && NT == 256>(sum, best, x, p.vocab, p.c, 0.f);
+    float held[HELD ? U * Piece<T>::N + 1 : 1];
+    if constexpr (HELD) hold_row<G, U>(sum, held, x, p.vocab, p.c, 0.f);
+    else row_pass<G, U, TOP>(sum, best, x, p.vocab, p.c, 0.f);
     sum.template join<G>(p.c, 0.f, tmp);
     const LogprobRow logp(sum, p.inv_t);
     logprob_store<G>(p, r, tgt, xt, sum, logp);
@@ -797,8 +810,9 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
         p.top_logp[r * p.top + j] = logp(v);
         p.top_ids[r * p.top + j] = i;
       };
-      if constexpr (PICK) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
-      else pick_part<G>(x, held, p.vocab, p.top, space[G::slot()], out);
+      if constexpr (NT == 256) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
+      else if constexpr (NT == 64) pick_held<G, U>(x, held, p.vocab, p.top, sum.m, space[G::slot()], out);
+      else pick_part<G, U>(x, held, p.vocab, p.top, space[G::slot()], out);
     }
   }
 }
