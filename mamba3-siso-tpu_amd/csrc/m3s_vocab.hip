@@ -341,25 +341,32 @@ constexpr uint32_t kKeyMin = 0x007fffffu;   // the key of -inf
 // A bound that at least k of the wave's 64 N values reach and no more than `most` >= k do, if ties
 // allow it: found by ballots, first in doubling steps down from the largest value's key `top`,
 // which the logits worth listing lie close to, then by halving. Of ties, the bound is the k-th value.
-template <int N>
+// Keys lose the bits that all of them share: bf16's lower 16, zeros or, below zero, ones.
+template <typename T, int N>
 __device__ __forceinline__ float kth_bound(const float* v, float top, int k, int most) {
+  constexpr int SHIFT = sizeof(T) == 2 ? 16 : 0;
+  constexpr uint32_t FIRST = kKeyMin >> SHIFT;
+  const auto value = [](uint32_t key) {
+    const bool below = !(key >> (31 - SHIFT));
+    return key_float(key << SHIFT | (SHIFT && below ? 0xffffu : 0u));
+  };
   uint32_t key[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) key[i] = float_key(v[i]);
+  for (int i = 0; i < N; ++i) key[i] = float_key(v[i]) >> SHIFT;
   const auto reach = [&](uint32_t bar) {
     int n = 0;
 #pragma unroll
     for (int i = 0; i < N; ++i) n += __popcll(__ballot(key[i] >= bar));
     return n;
   };
-  const uint32_t kt = __builtin_amdgcn_readfirstlane(float_key(top));
-  uint32_t lo = kKeyMin, hi = kt + 1;   // at least k reach lo, fewer than k reach hi
-  for (int j = 20; j < 32; ++j) {
-    const uint32_t bar = kt - kKeyMin > (1u << j) ? kt - (1u << j) : kKeyMin;
+  const uint32_t kt = __builtin_amdgcn_readfirstlane(float_key(top) >> SHIFT);
+  uint32_t lo = FIRST, hi = kt + 1;   // at least k reach lo, fewer than k reach hi
+  for (int j = 20 - SHIFT; j < 32 - SHIFT; ++j) {
+    const uint32_t bar = kt - FIRST > (1u << j) ? kt - (1u << j) : FIRST;
     const int n = reach(bar);
     if (n >= k) {
       lo = bar;
-      if (n <= most) return key_float(lo);
+      if (n <= most) return value(lo);
       break;
     }
     hi = bar;
@@ -374,7 +381,7 @@ __device__ __forceinline__ float kth_bound(const float* v, float top, int k, int
       hi = bar;
     }
   }
-  return key_float(lo);
+  return value(lo);
 }
 
 // Inclusive prefix sum over a wave's lanes: within the rows of 16, then their totals.
@@ -535,7 +542,7 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
     float m[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = sp.best[64 * i + threadIdx.x];
-    const float bar = kth_bound<4>(m, top, k, min(k + 12, 64));
+    const float bar = kth_bound<T, 4>(m, top, k, min(k + 12, 64));
     if (threadIdx.x == 0) sp.bar = bar;
   }
   __syncthreads();
@@ -571,9 +578,9 @@ __device__ __forceinline__ void pick_held(const T* __restrict__ x, const float* 
     float most = v[0];
 #pragma unroll
     for (int i = 1; i <= LEN; ++i) most = fmaxf(most, v[i]);
-    bar = kth_bound<1>(&most, top, k, min(k + 12, LANES));
+    bar = kth_bound<T, 1>(&most, top, k, min(k + 12, LANES));
   } else {
-    bar = kth_bound<LEN + 1>(v, top, k, 64);
+    bar = kth_bound<T, LEN + 1>(v, top, k, 64);
   }
   const auto gather = [&](auto strict) {
     constexpr bool STRICT = decltype(strict)::value;
