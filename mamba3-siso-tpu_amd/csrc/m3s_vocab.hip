@@ -314,6 +314,10 @@ __device__ __forceinline__ void hold_row(RowSums<MODE>& r, float* v, const T* __
   if (tail < n) r.template add<1>(v + R::LEN, v[R::LEN], c, c1);
 }
 
+// The workgroup's number. One row, or chunk of it, to each group and no loop over rows: a loop costs
+// the kernels with alternatives 25 to 45 registers (46 without, eight waves a SIMD, 82 with, five).
+__device__ __forceinline__ int64_t row_block() { return (int64_t)blockIdx.y * gridDim.x + blockIdx.x; }
+
 // a / b for a >= 0 and b > 0, without the 64-bit division's hundred instructions where it can be.
 __device__ __forceinline__ int64_t quotient(int64_t a, int b) {
   if (a < b) return 0;
@@ -438,14 +442,18 @@ __device__ __forceinline__ int gather(const T* __restrict__ x, int n, const Best
     if (reaches<STRICT>(v, bar)) append(sp, v, tail);
   }
   __syncthreads();
-  const auto piece = [&](int at) {
+  const auto piece = [&](int at) {   // by all lanes of the wave, past the row with nothing
     float v[N];
-    Piece<T>::load(x + (int64_t)at * N, v);
     uint32_t hits = 0;
+    if (at < full) {
+      Piece<T>::load(x + (int64_t)at * N, v);
 #pragma unroll
-    for (int i = 0; i < N; ++i) hits |= reaches<STRICT>(v[i], bar) ? 1u << i : 0u;
-    if (!hits) return;
-    int to = atomicAdd(&sp.count, __popc(hits));
+      for (int i = 0; i < N; ++i) hits |= reaches<STRICT>(v[i], bar) ? 1u << i : 0u;
+    }
+    const int mine = __popc(hits), upto = wave_prefix(mine), all = __builtin_amdgcn_readlane(upto, 63);
+    if (all == 0) return;
+    int to = lane_id() == 0 ? atomicAdd(&sp.count, all) : 0;
+    to = __builtin_amdgcn_readfirstlane(to) + upto - mine;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (!(hits >> i & 1)) continue;
@@ -454,13 +462,13 @@ __device__ __forceinline__ int gather(const T* __restrict__ x, int n, const Best
     }
   };
   const int items = sp.items * U, wides = sp.wides;
-  for (int q = tid; q < items; q += G::NT) {
-    const uint32_t it = sp.item[q / U];
-    const int at = (int)(it >> 8) * R::HOP + q % U * G::NT + (int)(it & 255);
-    if (at < full) piece(at);
+  for (int q0 = 0; q0 < items; q0 += G::NT) {
+    const int q = q0 + tid;
+    const uint32_t it = q < items ? sp.item[q / U] : 0;
+    piece(q < items ? (int)(it >> 8) * R::HOP + q % U * G::NT + (int)(it & 255) : full);
   }
   for (int w = 0; w < wides && *(volatile int*)&sp.count <= PickSpace<4>::CAP; ++w) {
-    for (int at = sp.wide[w] + tid * G::NT; at < full; at += G::NT * G::NT) piece(at);
+    for (int at = sp.wide[w]; at < full; at += G::NT * G::NT) piece(at + tid * G::NT);
   }
   __syncthreads();
   return sp.count;
@@ -801,35 +809,35 @@ __global__ void __launch_bounds__(kRowThreads) logprob_fwd_kernel(const LogprobP
   constexpr bool HELD = TOP && NT < 256;   // the row stays in registers between its sums and the pick
   __shared__ float tmp[G::TMP];
   __shared__ std::conditional_t<NT == 16, PartSpace, PickSpace<NT == 256 ? 4 : 1>> space[TOP ? G::ROWS : 1];
-  for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
-    const int64_t tgt = p.targets ? p.targets[r] : 0;
-    if (p.targets && tgt == p.ignore) {
-      logprob_skip<G>(p, r);
-      continue;
+  const int64_t r = row_block() * G::ROWS + G::slot();
+  if (r >= p.rows) return;
+  const int64_t tgt = p.targets ? p.targets[r] : 0;
+  if (p.targets && tgt == p.ignore) {
+    logprob_skip<G>(p, r);
+    return;
+  }
+  const T* x = row_at<T>(p.logits, r, p.seqlen);
+  const float xt = target_logit(p, tgt, x);
+  RowSums<kEntropy> sum;
+  Best best;
+  float held[HELD ? U * Piece<T>::N + 1 : 1];
+  if constexpr (HELD) hold_row<G, U>(sum, held, x, p.vocab, p.c, 0.f);
+  else row_pass<G, U, TOP>(sum, best, x, p.vocab, p.c, 0.f);
+  sum.template join<G>(p.c, 0.f, tmp);
+  const LogprobRow logp(sum, p.inv_t);
+  logprob_store<G>(p, r, tgt, xt, sum, logp);
+  if constexpr (TOP) {
+    if (sum.s != sum.s) {
+      logprob_unordered<G>(p, r);
+      return;
     }
-    const T* x = row_at<T>(p.logits, r, p.seqlen);
-    const float xt = target_logit(p, tgt, x);
-    RowSums<kEntropy> sum;
-    Best best;
-    float held[HELD ? U * Piece<T>::N + 1 : 1];
-    if constexpr (HELD) hold_row<G, U>(sum, held, x, p.vocab, p.c, 0.f);
-    else row_pass<G, U, TOP>(sum, best, x, p.vocab, p.c, 0.f);
-    sum.template join<G>(p.c, 0.f, tmp);
-    const LogprobRow logp(sum, p.inv_t);
-    logprob_store<G>(p, r, tgt, xt, sum, logp);
-    if constexpr (TOP) {
-      if (sum.s != sum.s) {
-        logprob_unordered<G>(p, r);
-        continue;
-      }
-      const auto out = [&](int j, float v, int i) {
-        p.top_logp[r * p.top + j] = logp(v);
-        p.top_ids[r * p.top + j] = i;
-      };
-      if constexpr (NT == 256) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
-      else if constexpr (NT == 64) pick_held<G, U>(x, held, p.vocab, p.top, sum.m, space[G::slot()], out);
-      else pick_part<G, U>(x, held, p.vocab, p.top, space[G::slot()], out);
-    }
+    const auto out = [&](int j, float v, int i) {
+      p.top_logp[r * p.top + j] = logp(v);
+      p.top_ids[r * p.top + j] = i;
+    };
+    if constexpr (NT == 256) pick<G, U>(x, p.vocab, p.top, sum.m, best, space[G::slot()], out);
+    else if constexpr (NT == 64) pick_held<G, U>(x, held, p.vocab, p.top, sum.m, space[G::slot()], out);
+    else pick_part<G, U>(x, held, p.vocab, p.top, space[G::slot()], out);
   }
 }
 
@@ -962,49 +970,47 @@ __global__ void __launch_bounds__(kRowThreads) logprob_bwd_kernel(const LogprobP
   __shared__ float sgrad[G::ROWS][kTopMax + 1];
   int* ids = sids[G::slot()];
   float* gtop = sgrad[G::slot()];
-  const int64_t work = p.rows * p.chunks;
-  for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
-    const int64_t r = quotient(w, p.chunks);
-    const int lo = (int)(w - r * p.chunks) * p.chunk, hi = min(lo + p.chunk, p.vocab);
-    const T* x = row_at<T>(p.logits, r, p.seqlen);
-    T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
-    const int64_t tgt = p.targets ? p.targets[r] : -1;
-    const float m = p.stats[3 * r], s = p.stats[3 * r + 1], h = p.stats[3 * r + 2];
-    // an ignored row, and one of nothing but -inf, has s = 0 and no gradient
-    if (s == 0.f) {
-      chunk_zero<G>(dx, lo, hi);
-      continue;
-    }
-    float gl = p.dlogp ? p.dlogp[r] * p.inv_t : 0.f;
-    if (p.dlogp && (tgt < 0 || tgt >= p.vocab)) gl = __builtin_nanf("");
-    const float gh = p.dentropy ? p.dentropy[r] * p.inv_t : 0.f;
-    float g = gl;
-    const int top = p.dtop ? p.top : 0;
-    for (int j = 0; j < top; ++j) g += p.dtop[r * top + j] * p.inv_t;
-    const float inv_s = 1.f / s, logs = logf(s);
-    const auto f = [&](float v) {
-      const float d = v - m;
-      const float q = __builtin_amdgcn_exp2f(d * p.c) * inv_s;
-      const float lq = fmaxf(d * p.inv_t - logs, -1e30f);
-      return -q * (g + gh * (lq + h));
-    };
-    chunk_map<G>(x, dx, lo, hi, f);
-    // then the entries that a token or an alternative adds to, whole
-    for (int j = G::tid(); j < top; j += G::NT) {
-      ids[j] = (int)p.top_ids[r * top + j];
-      gtop[j] = p.dtop[r * top + j] * p.inv_t;
-    }
-    G::sync();
-    for (int j = G::tid(); j < top; j += G::NT) {
-      const int i = ids[j];
-      if (i >= lo && i < hi) dx[i] = (T)(f((float)x[i]) + gtop[j] + (i == tgt ? gl : 0.f));
-    }
-    if (G::tid() == 0 && p.dlogp && tgt >= lo && tgt < hi) {
-      bool alone = true;
-      for (int j = 0; j < top; ++j) alone = alone && ids[j] != tgt;
-      if (alone) dx[tgt] = (T)(f((float)x[tgt]) + gl);
-    }
-    G::sync();
+  const int64_t w = row_block() * G::ROWS + G::slot();
+  if (w >= p.rows * p.chunks) return;
+  const int64_t r = quotient(w, p.chunks);
+  const int lo = (int)(w - r * p.chunks) * p.chunk, hi = min(lo + p.chunk, p.vocab);
+  const T* x = row_at<T>(p.logits, r, p.seqlen);
+  T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
+  const int64_t tgt = p.targets ? p.targets[r] : -1;
+  const float m = p.stats[3 * r], s = p.stats[3 * r + 1], h = p.stats[3 * r + 2];
+  // an ignored row, and one of nothing but -inf, has s = 0 and no gradient
+  if (s == 0.f) {
+    chunk_zero<G>(dx, lo, hi);
+    return;
+  }
+  float gl = p.dlogp ? p.dlogp[r] * p.inv_t : 0.f;
+  if (p.dlogp && (tgt < 0 || tgt >= p.vocab)) gl = __builtin_nanf("");
+  const float gh = p.dentropy ? p.dentropy[r] * p.inv_t : 0.f;
+  float g = gl;
+  const int top = p.dtop ? p.top : 0;
+  for (int j = 0; j < top; ++j) g += p.dtop[r * top + j] * p.inv_t;
+  const float inv_s = 1.f / s, logs = logf(s);
+  const auto f = [&](float v) {
+    const float d = v - m;
+    const float q = __builtin_amdgcn_exp2f(d * p.c) * inv_s;
+    const float lq = fmaxf(d * p.inv_t - logs, -1e30f);
+    return -q * (g + gh * (lq + h));
+  };
+  chunk_map<G>(x, dx, lo, hi, f);
+  // then the entries that a token or an alternative adds to, whole
+  for (int j = G::tid(); j < top; j += G::NT) {
+    ids[j] = (int)p.top_ids[r * top + j];
+    gtop[j] = p.dtop[r * top + j] * p.inv_t;
+  }
+  G::sync();
+  for (int j = G::tid(); j < top; j += G::NT) {
+    const int i = ids[j];
+    if (i >= lo && i < hi) dx[i] = (T)(f((float)x[i]) + gtop[j] + (i == tgt ? gl : 0.f));
+  }
+  if (G::tid() == 0 && p.dlogp && tgt >= lo && tgt < hi) {
+    bool alone = true;
+    for (int j = 0; j < top; ++j) alone = alone && ids[j] != tgt;
+    if (alone) dx[tgt] = (T)(f((float)x[tgt]) + gl);
   }
 }
 
@@ -1107,19 +1113,19 @@ template <int MODE, int NT, int U, typename T>
 __global__ void __launch_bounds__(kRowThreads) distill_fwd_kernel(const DistillParams p) {
   using G = Group<NT>;
   __shared__ float tmp[G::TMP];
-  for (int64_t r = (int64_t)blockIdx.x * G::ROWS + G::slot(); r < p.rows; r += (int64_t)gridDim.x * G::ROWS) {
-    const T* x = row_at<T>(p.logits, r, p.seqlen);
-    const Teacher<G> t(p, r, tmp);
-    const int64_t tgt = p.targets ? p.targets[r] : 0;
-    const bool hard = p.targets && tgt != p.ignore;
-    RowSums<MODE> sum;
-    if (t.ts != 0.f || hard) {
-      Best unused;
-      row_pass<G, U, false>(sum, unused, x, p.vocab, p.c, p.c1);
-      sum.template join<G>(p.c, p.c1, tmp);
-    }
-    distill_store<G>(p, r, x, t, hard, tgt, sum, tmp);
+  const int64_t r = row_block() * G::ROWS + G::slot();
+  if (r >= p.rows) return;
+  const T* x = row_at<T>(p.logits, r, p.seqlen);
+  const Teacher<G> t(p, r, tmp);
+  const int64_t tgt = p.targets ? p.targets[r] : 0;
+  const bool hard = p.targets && tgt != p.ignore;
+  RowSums<MODE> sum;
+  if (t.ts != 0.f || hard) {
+    Best unused;
+    row_pass<G, U, false>(sum, unused, x, p.vocab, p.c, p.c1);
+    sum.template join<G>(p.c, p.c1, tmp);
   }
+  distill_store<G>(p, r, x, t, hard, tgt, sum, tmp);
 }
 
 // Few long rows: a workgroup to each of a row's pieces, then one to join them.
@@ -1176,138 +1182,136 @@ __global__ void __launch_bounds__(kRowThreads) distill_bwd_kernel(const DistillP
   constexpr int KMAX = NT == 16 ? kPartTeacher : kTeacherMax;
   __shared__ int sids[G::ROWS][KMAX + 1];   // odd: the groups of a wave on different banks
   __shared__ float sweight[G::ROWS][KMAX + 1];
-  const int64_t work = p.rows * p.chunks;
-  for (int64_t w = (int64_t)blockIdx.x * G::ROWS + G::slot(); w < work; w += (int64_t)gridDim.x * G::ROWS) {
-    const int64_t r = quotient(w, p.chunks);
-    const int lo = (int)(w - r * p.chunks) * p.chunk, hi = min(lo + p.chunk, p.vocab);
-    const T* x = row_at<T>(p.logits, r, p.seqlen);
-    T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
-    const float* stats = p.stats + 5 * r;
-    const float m = stats[0], s = stats[1], s1 = stats[2], ref = stats[3], ts = stats[4];
-    const int64_t tgt = p.targets ? p.targets[r] : p.ignore;
-    const bool soft = p.dkd && ts != 0.f, hard = p.dnll && tgt != p.ignore;
-    if (s == 0.f || (!soft && !hard)) {   // no loss, or no distribution
-      chunk_zero<G>(dx, lo, hi);
-      continue;
-    }
-    const float a = soft ? p.dkd[r] * p.temp : 0.f, as = ts != ts ? ts : a / s;
-    float b = hard ? p.dnll[r] : 0.f;
-    if (hard && (tgt < 0 || tgt >= p.vocab)) b = __builtin_nanf("");
-    const float bs = b / s1;
-    // one exponential: of the teacher's temperature, or of the cross-entropy's if it is alone
-    const float ec = soft ? p.c : p.c1, es = soft ? (hard ? as + bs : as) : bs;
-    const auto f = [&](float v) {
-      const float d = v - m;
-      if constexpr (!DUAL) return es * __builtin_amdgcn_exp2f(d * ec);
-      float o = 0.f;
-      if (soft) o = as * __builtin_amdgcn_exp2f(d * p.c);
-      if (hard) o += bs * __builtin_amdgcn_exp2f(d * p.c1);
-      return o;
-    };
-    const int k = soft ? p.k : 0;
-    const float at = a / ts;
-    const auto weight = [&](int64_t id, int j) {   // what an entry takes
-      if (id < 0 || id >= p.vocab) return 0.f;
-      return at * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + j) - ref) * p.c);
-    };
-    // The entries that the teacher's tokens or the true one take from are written again, whole; a
-    // token named twice by its first mention. Up to 64 of them lie one to a lane of the group's first
-    // wave, or four to each of 16 lanes, which load them ahead of the dense pass (22.9 -> 20.7 us at
-    // 32768 x 256; ahead of a workgroup's pass 107 -> 138 us at 2048 x 65536 bf16, all of which waits for them).
-    constexpr int LANES = NT == 16 ? 16 : 64, E = 64 / LANES;
-    const bool few = k <= 64, mine = few && G::tid() < LANES, truth = hard && tgt >= lo && tgt < hi;
-    int eid[E];
-    float ew[E], ex[E], tx = 0.f;
-    const auto load_entries = [&] {
-      if (!mine) return;
+  const int64_t w = row_block() * G::ROWS + G::slot();
+  if (w >= p.rows * p.chunks) return;
+  const int64_t r = quotient(w, p.chunks);
+  const int lo = (int)(w - r * p.chunks) * p.chunk, hi = min(lo + p.chunk, p.vocab);
+  const T* x = row_at<T>(p.logits, r, p.seqlen);
+  T* dx = static_cast<T*>(p.dlogits) + r * p.vocab;
+  const float* stats = p.stats + 5 * r;
+  const float m = stats[0], s = stats[1], s1 = stats[2], ref = stats[3], ts = stats[4];
+  const int64_t tgt = p.targets ? p.targets[r] : p.ignore;
+  const bool soft = p.dkd && ts != 0.f, hard = p.dnll && tgt != p.ignore;
+  if (s == 0.f || (!soft && !hard)) {   // no loss, or no distribution
+    chunk_zero<G>(dx, lo, hi);
+    return;
+  }
+  const float a = soft ? p.dkd[r] * p.temp : 0.f, as = ts != ts ? ts : a / s;
+  float b = hard ? p.dnll[r] : 0.f;
+  if (hard && (tgt < 0 || tgt >= p.vocab)) b = __builtin_nanf("");
+  const float bs = b / s1;
+  // one exponential: of the teacher's temperature, or of the cross-entropy's if it is alone
+  const float ec = soft ? p.c : p.c1, es = soft ? (hard ? as + bs : as) : bs;
+  const auto f = [&](float v) {
+    const float d = v - m;
+    if constexpr (!DUAL) return es * __builtin_amdgcn_exp2f(d * ec);
+    float o = 0.f;
+    if (soft) o = as * __builtin_amdgcn_exp2f(d * p.c);
+    if (hard) o += bs * __builtin_amdgcn_exp2f(d * p.c1);
+    return o;
+  };
+  const int k = soft ? p.k : 0;
+  const float at = a / ts;
+  const auto weight = [&](int64_t id, int j) {   // what an entry takes
+    if (id < 0 || id >= p.vocab) return 0.f;
+    return at * __builtin_amdgcn_exp2f((teacher_logit(p, r * k + j) - ref) * p.c);
+  };
+  // The entries that the teacher's tokens or the true one take from are written again, whole; a
+  // token named twice by its first mention. Up to 64 of them lie one to a lane of the group's first
+  // wave, or four to each of 16 lanes, which load them ahead of the dense pass (22.9 -> 20.7 us at
+  // 32768 x 256; ahead of a workgroup's pass 107 -> 138 us at 2048 x 65536 bf16, all of which waits for them).
+  constexpr int LANES = NT == 16 ? 16 : 64, E = 64 / LANES;
+  const bool few = k <= 64, mine = few && G::tid() < LANES, truth = hard && tgt >= lo && tgt < hi;
+  int eid[E];
+  float ew[E], ex[E], tx = 0.f;
+  const auto load_entries = [&] {
+    if (!mine) return;
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int j = e * LANES + G::tid();
-        const int64_t id = j < k ? teacher_id(p, r * k + j) : -1;
-        eid[e] = id >= lo && id < hi ? (int)id : -1;
-        ew[e] = eid[e] >= 0 ? weight(id, j) : 0.f;
-        ex[e] = eid[e] >= 0 ? (float)x[eid[e]] : 0.f;
-      }
-      if (truth) tx = (float)x[tgt];
-    };
-    if (NT == 16) load_entries();
-    chunk_map<G>(x, dx, lo, hi, f);
-    int* ids = sids[G::slot()];
-    float* wt = sweight[G::slot()];
-    if (NT == 16 || !few) {
-      if (few) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          ids[e * LANES + G::tid()] = eid[e];
-          wt[e * LANES + G::tid()] = ew[e];
-        }
-      } else {
-        for (int j = G::tid(); j < k; j += G::NT) {
-          const int64_t id = teacher_id(p, r * k + j);
-          ids[j] = id >= lo && id < hi ? (int)id : -1;
-          wt[j] = weight(id, j);
-        }
-      }
+    for (int e = 0; e < E; ++e) {
+      const int j = e * LANES + G::tid();
+      const int64_t id = j < k ? teacher_id(p, r * k + j) : -1;
+      eid[e] = id >= lo && id < hi ? (int)id : -1;
+      ew[e] = eid[e] >= 0 ? weight(id, j) : 0.f;
+      ex[e] = eid[e] >= 0 ? (float)x[eid[e]] : 0.f;
     }
-    G::sync();
-    if (few && !mine) continue;   // only now: waves that are done make room for the next workgroup's
-    if (NT > 16) load_entries();
-    const auto whole = [&](int i, float xi, float take) {
-      dx[i] = (T)(f(xi) - take - (hard && i == tgt ? b : 0.f));
-    };
-    const auto mentions = [&](int i, int j, float& take) {   // in LDS, of the j-th entry; first one?
-      bool first = true;
-      for (int l = 0; l < k; ++l) {
-        const bool same = ids[l] == i;
-        take += same ? wt[l] : 0.f;
-        first = first && !(same && l < j);
-      }
-      return first;
-    };
-    bool named = false;   // the true token is among the entries, some thread knows
+    if (truth) tx = (float)x[tgt];
+  };
+  if (NT == 16) load_entries();
+  chunk_map<G>(x, dx, lo, hi, f);
+  int* ids = sids[G::slot()];
+  float* wt = sweight[G::slot()];
+  if (NT == 16 || !few) {
     if (few) {
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const int j = e * LANES + G::tid();
-        if (NT == 16 ? e * LANES >= k : !__ballot(eid[e] >= 0)) break;
-        float take = 0.f;
-        bool first = true;
-        if constexpr (NT == 16) {
-          if (eid[e] >= 0) first = mentions(eid[e], j, take);
-        } else {
-          for (int l = 0; l < k; ++l) {
-            const bool same = __builtin_amdgcn_readlane(eid[0], l) == eid[0];
-            const float wl = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ew[0]), l));
-            take += same ? wl : 0.f;
-            first = first && !(same && l < j);
-          }
-        }
-        if (eid[e] >= 0 && first) whole(eid[e], ex[e], take);
-        named = named || (truth && eid[e] == (int)tgt);
+        ids[e * LANES + G::tid()] = eid[e];
+        wt[e * LANES + G::tid()] = ew[e];
       }
-      if (truth) {
-        if constexpr (NT == 16) named = G::max(named ? 1.f : 0.f, nullptr) != 0.f;
-        else named = __ballot(named) != 0;
-        if (!named && G::tid() == 0) whole((int)tgt, tx, 0.f);
+    } else {
+      for (int j = G::tid(); j < k; j += G::NT) {
+        const int64_t id = teacher_id(p, r * k + j);
+        ids[j] = id >= lo && id < hi ? (int)id : -1;
+        wt[j] = weight(id, j);
       }
-      continue;
     }
-    for (int j = G::tid(); j < k; j += G::NT) {
-      const int i = ids[j];
-      if (i < 0) continue;
+  }
+  G::sync();
+  if (few && !mine) return;   // only now: waves that are done make room for the next workgroup's
+  if (NT > 16) load_entries();
+  const auto whole = [&](int i, float xi, float take) {
+    dx[i] = (T)(f(xi) - take - (hard && i == tgt ? b : 0.f));
+  };
+  const auto mentions = [&](int i, int j, float& take) {   // in LDS, of the j-th entry; first one?
+    bool first = true;
+    for (int l = 0; l < k; ++l) {
+      const bool same = ids[l] == i;
+      take += same ? wt[l] : 0.f;
+      first = first && !(same && l < j);
+    }
+    return first;
+  };
+  bool named = false;   // the true token is among the entries, some thread knows
+  if (few) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int j = e * LANES + G::tid();
+      if (NT == 16 ? e * LANES >= k : !__ballot(eid[e] >= 0)) break;
       float take = 0.f;
-      if (mentions(i, j, take)) whole(i, (float)x[i], take);
+      bool first = true;
+      if constexpr (NT == 16) {
+        if (eid[e] >= 0) first = mentions(eid[e], j, take);
+      } else {
+        for (int l = 0; l < k; ++l) {
+          const bool same = __builtin_amdgcn_readlane(eid[0], l) == eid[0];
+          const float wl = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ew[0]), l));
+          take += same ? wl : 0.f;
+          first = first && !(same && l < j);
+        }
+      }
+      if (eid[e] >= 0 && first) whole(eid[e], ex[e], take);
+      named = named || (truth && eid[e] == (int)tgt);
     }
-    if (G::tid() == 0 && truth) {
-      for (int l = 0; l < k; ++l) named = named || ids[l] == tgt;
-      if (!named) whole((int)tgt, (float)x[tgt], 0.f);
+    if (truth) {
+      if constexpr (NT == 16) named = G::max(named ? 1.f : 0.f, nullptr) != 0.f;
+      else named = __ballot(named) != 0;
+      if (!named && G::tid() == 0) whole((int)tgt, tx, 0.f);
     }
-    G::sync();
+    return;
+  }
+  for (int j = G::tid(); j < k; j += G::NT) {
+    const int i = ids[j];
+    if (i < 0) continue;
+    float take = 0.f;
+    if (mentions(i, j, take)) whole(i, (float)x[i], take);
+  }
+  if (G::tid() == 0 && truth) {
+    for (int l = 0; l < k; ++l) named = named || ids[l] == tgt;
+    if (!named) whole((int)tgt, (float)x[tgt], 0.f);
   }
 }
 
 // ---- host -----------------------------------------------------------------------------------
-constexpr int64_t kRowGrid = 1 << 20;
+constexpr int64_t kRowGrid = 1 << 23;   // workgroups of a grid's first axis: 2^31 threads
 
 template <typename A>
 static int32_t check_rows(const A* a, const char* who) {
@@ -1420,7 +1424,8 @@ static DistillParams distill_params(const m3s_distill_args* a) {
 
 template <typename P>
 static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t s) {
-  hipLaunchKernelGGL(f, dim3((unsigned)std::min(kRowGrid, blocks)), dim3(kRowThreads), 0, s, p);
+  const int64_t x = std::min(kRowGrid, blocks), y = (blocks + x - 1) / x;   // 2^39: more than memory holds
+  hipLaunchKernelGGL(f, dim3((unsigned)x, (unsigned)y), dim3(kRowThreads), 0, s, p);
 }
 // f(group): the threads to a row
 template <typename F>
