@@ -929,27 +929,33 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
 // 357 with 6 and 396 with 8 (registers cost waves); at bf16 ones of 8192 x 50001 it takes 328 with 4,
 // 376 with 2 (too few loads in flight), 334 with 6 and 383 with 8.
 template <typename T> constexpr int kBwdPieces = 4;
+// P pieces a thread, without a branch between them: past the last piece a thread takes that one again,
+// and writes what its owner writes. (A wait behind a branch is for everything, stores too: one for each
+// piece would wait for the piece before to reach memory.)
+template <typename G, int P, typename T, typename F>
+__device__ __forceinline__ void pieces_map(const T* __restrict__ x, T* __restrict__ dx, int full, F&& f) {
+  constexpr int N = Piece<T>::N;
+  float v[P * N];
+#pragma unroll
+  for (int u = 0; u < P; ++u) Piece<T>::load(x + min(u * G::NT + G::tid(), full - 1) * N, v + u * N);
+#pragma unroll
+  for (int u = 0; u < P; ++u) {
+    float o[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) o[i] = f(v[u * N + i]);
+    Piece<T>::store(dx + min(u * G::NT + G::tid(), full - 1) * N, o);
+  }
+}
 template <typename G, typename T, typename F>
 __device__ __forceinline__ void chunk_map(const T* __restrict__ x, T* __restrict__ dx, int lo, int hi,
                                           F&& f) {
   constexpr int N = Piece<T>::N;
   const int n = hi - lo, full = n / N;
-  float v[kBwdPieces<T> * N];
-#pragma unroll
-  for (int u = 0; u < kBwdPieces<T>; ++u) {
-    const int at = u * G::NT + G::tid();
-    if (at < full) Piece<T>::load(x + lo + at * N, v + u * N);
-  }
-#pragma unroll
-  for (int u = 0; u < kBwdPieces<T>; ++u) {
-    const int at = u * G::NT + G::tid();
-    if (at < full) {
-      float o[N];
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[i] = f(v[u * N + i]);
-      Piece<T>::store(dx + lo + at * N, o);
-    }
-  }
+  static_assert(kBwdPieces<T> == 4);
+  if (full > 3 * G::NT) pieces_map<G, 4>(x + lo, dx + lo, full, f);
+  else if (full > 2 * G::NT) pieces_map<G, 3>(x + lo, dx + lo, full, f);
+  else if (full > G::NT) pieces_map<G, 2>(x + lo, dx + lo, full, f);
+  else if (full > 0) pieces_map<G, 1>(x + lo, dx + lo, full, f);
   const int at = full * N + G::tid();
   if (at < n) dx[lo + at] = (T)f((float)x[lo + at]);
 }
@@ -1423,10 +1429,21 @@ static DistillParams distill_params(const m3s_distill_args* a) {
 }
 
 template <typename P>
-static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t s) {
+static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t s, int lds = 0) {
   const int64_t x = std::min(kRowGrid, blocks), y = (blocks + x - 1) / x;   // 2^39: more than memory holds
-  hipLaunchKernelGGL(f, dim3((unsigned)x, (unsigned)y), dim3(kRowThreads), 0, s, p);
+  hipLaunchKernelGGL(f, dim3((unsigned)x, (unsigned)y), dim3(kRowThreads), lds, s, p);
 }
+// The LDS that leaves room for n workgroups on a CU: the middle of what does, less the kernel's own.
+static int lds_for(int n, int own) { return 80 * 1024 / n + 80 * 1024 / (n + 1) - own; }
+// The workgroups on a CU of a backward whose rows take a workgroup. Eight fit, but then the loads and
+// stores of so many rows meet in HBM: the log-probabilities' at 8192 x 32000 and 8192 x 50001 float32
+// take 338 and 521 us with four, 398 and 607 with five, 406 and 613 with six, 417 and 602 with eight; in
+// bf16 172 and 300 with four, 174 and 292 with five, 185 and 299 with eight. The distillation's, which
+// waits for its entries behind the dense pass, at float32 350 and 538 with five, 341 and 527 with six,
+// 346 and 584 with seven, 430 and 620 with eight; in bf16 190 and 343 with six, 185 and 328 with seven,
+// 208 and 319 with eight.
+template <typename T> constexpr int kLogprobGroups = sizeof(T) == 2 ? 5 : 4;
+template <typename T> constexpr int kDistillGroups = sizeof(T) == 2 ? 7 : 6;
 // f(group): the threads to a row
 template <typename F>
 static void with_group(int nt, F&& f) {
@@ -1476,7 +1493,8 @@ static void launch_logprob_bwd(LogprobParams& p, hipStream_t s) {
   set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
-    launch_kernel(logprob_bwd_kernel<NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s);
+    const int lds = NT == 256 ? lds_for(kLogprobGroups<T>, 8 * (kTopMax + 1)) : 0;
+    launch_kernel(logprob_bwd_kernel<NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s, lds);
   });
 }
 template <bool DUAL, typename T>
@@ -1485,7 +1503,8 @@ static void launch_distill_bwd(DistillParams& p, hipStream_t s) {
   set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
-    launch_kernel(distill_bwd_kernel<DUAL, NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s);
+    const int lds = NT == 256 ? lds_for(kDistillGroups<T>, 8 * (kTeacherMax + 1)) : 0;
+    launch_kernel(distill_bwd_kernel<DUAL, NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s, lds);
   });
 }
 
