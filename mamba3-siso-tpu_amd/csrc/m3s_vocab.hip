@@ -1433,17 +1433,20 @@ static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t 
   const int64_t x = std::min(kRowGrid, blocks), y = (blocks + x - 1) / x;   // 2^39: more than memory holds
   hipLaunchKernelGGL(f, dim3((unsigned)x, (unsigned)y), dim3(kRowThreads), lds, s, p);
 }
-// The LDS that leaves room for n workgroups on a CU: the middle of what does, less the kernel's own.
-static int lds_for(int n, int own) { return 80 * 1024 / n + 80 * 1024 / (n + 1) - own; }
-// The workgroups on a CU of a backward whose rows take a workgroup. Eight fit, but then the loads and
-// stores of so many rows meet in HBM: the log-probabilities' at 8192 x 32000 and 8192 x 50001 float32
-// take 338 and 521 us with four, 398 and 607 with five, 406 and 613 with six, 417 and 602 with eight; in
-// bf16 172 and 300 with four, 174 and 292 with five, 185 and 299 with eight. The distillation's, which
-// waits for its entries behind the dense pass, at float32 350 and 538 with five, 341 and 527 with six,
-// 346 and 584 with seven, 430 and 620 with eight; in bf16 190 and 343 with six, 185 and 328 with seven,
-// 208 and 319 with eight.
-template <typename T> constexpr int kLogprobGroups = sizeof(T) == 2 ? 5 : 4;
-template <typename T> constexpr int kDistillGroups = sizeof(T) == 2 ? 7 : 6;
+// The LDS for a backward of `own` bytes of its own: what leaves room for n workgroups on a CU (the
+// middle of it) where rows of float32 take a workgroup a chunk and its threads four pieces. Eight fit,
+// but then the loads and stores of so many chunks of 13 to 16 KB meet in HBM: the log-probabilities' at
+// 8192 x 32000 and 8192 x 50001 take 338 and 521 us with four, 398 and 607 with five, 417 and 602 with
+// eight; the distillation's, whose workgroups last longer behind the dense pass, 350 and 538 with five,
+// 341 and 527 with six, 430 and 620 with eight. Smaller chunks want all eight (65536 x 5000: the
+// distillation's 630 us with six, 488 with eight), and so do bf16's, half the bytes: 5 to 8% are won
+// at some lengths (16384 x 32000) and lost at others (40000 x 10000).
+constexpr int kLogprobGroups = 4, kDistillGroups = 6;
+template <typename G, typename T, typename P>
+static int bwd_lds(const P& p, int n, int own) {
+  const bool heavy = G::NT == 256 && sizeof(T) == 4 && p.chunk > 3 * G::NT * Piece<T>::N;
+  return heavy ? 80 * 1024 / n + 80 * 1024 / (n + 1) - own : 0;
+}
 // f(group): the threads to a row
 template <typename F>
 static void with_group(int nt, F&& f) {
@@ -1493,7 +1496,7 @@ static void launch_logprob_bwd(LogprobParams& p, hipStream_t s) {
   set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
-    const int lds = NT == 256 ? lds_for(kLogprobGroups<T>, 8 * (kTopMax + 1)) : 0;
+    const int lds = bwd_lds<decltype(g), T>(p, kLogprobGroups, 8 * (kTopMax + 1));
     launch_kernel(logprob_bwd_kernel<NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s, lds);
   });
 }
@@ -1503,7 +1506,7 @@ static void launch_distill_bwd(DistillParams& p, hipStream_t s) {
   set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
-    const int lds = NT == 256 ? lds_for(kDistillGroups<T>, 8 * (kTeacherMax + 1)) : 0;
+    const int lds = bwd_lds<decltype(g), T>(p, kDistillGroups, 8 * (kTeacherMax + 1));
     launch_kernel(distill_bwd_kernel<DUAL, NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s, lds);
   });
 }
