@@ -1437,11 +1437,13 @@ static void launch_kernel(void (*f)(P), int64_t blocks, const P& p, hipStream_t 
 // middle of it) where rows of float32 take a workgroup a chunk and its threads four pieces. Eight fit,
 // but then the loads and stores of so many chunks of 13 to 16 KB meet in HBM: the log-probabilities' at
 // 8192 x 32000 and 8192 x 50001 take 338 and 521 us with four, 398 and 607 with five, 417 and 602 with
-// eight; the distillation's, whose workgroups last longer behind the dense pass, 350 and 538 with five,
-// 341 and 527 with six, 430 and 620 with eight. Smaller chunks want all eight (65536 x 5000: the
-// distillation's 630 us with six, 488 with eight), and so do bf16's, half the bytes: 5 to 8% are won
-// at some lengths (16384 x 32000) and lost at others (40000 x 10000).
-constexpr int kLogprobGroups = 4, kDistillGroups = 6;
+// eight. The distillation's workgroups last longer behind the dense pass, the more so with more teacher
+// tokens: with 16 they take 341 and 525 with six, 345 and 578 with seven, 416 and 620 with eight, with 32
+// 365 and 556, 355 and 543, 425 and 629, with 64 402 and 622, 377 and 578, 442 and 636. Smaller chunks
+// want all eight (65536 x 5000: the distillation's 630 us with six, 488 with eight), and so do bf16's,
+// half the bytes: 5 to 8% are won at some lengths (16384 x 32000) and lost at others (40000 x 10000).
+constexpr int kLogprobGroups = 4;
+static int distill_groups(int k) { return k <= 16 ? 6 : 7; }
 template <typename G, typename T, typename P>
 static int bwd_lds(const P& p, int n, int own) {
   const bool heavy = G::NT == 256 && sizeof(T) == 4 && p.chunk > 3 * G::NT * Piece<T>::N;
@@ -1506,7 +1508,7 @@ static void launch_distill_bwd(DistillParams& p, hipStream_t s) {
   set_chunks<T>(p, nt);
   with_group(nt, [&](auto g) {
     constexpr int NT = decltype(g)::NT, ROWS = decltype(g)::ROWS;
-    const int lds = bwd_lds<decltype(g), T>(p, kDistillGroups, 8 * (kTeacherMax + 1));
+    const int lds = bwd_lds<decltype(g), T>(p, distill_groups(p.k), 8 * (kTeacherMax + 1));
     launch_kernel(distill_bwd_kernel<DUAL, NT, T>, (p.rows * p.chunks + ROWS - 1) / ROWS, p, s, lds);
   });
 }
