@@ -22,11 +22,11 @@
 // Rows may start at any element: 16-byte accesses need no alignment on gfx950.
 //
 // Measured (us; TB/s of logits read and gradients written): log-probability and entropy of 8192 x
-// 32000 float32, a tenth of it padding, forward 166 (5.7), backward 345 (5.8); distillation of 8192 x
-// 50001 float32 with 32 teacher tokens and the cross-entropy, forward 253 (5.8), backward 515 (6.1);
-// of 2048 x 65536 bf16, 58 (4.6) and 106 (5.1): there the exponentials take as long as the bytes. A
-// large copy moves 5.0 TB/s. 32768 x 256 float32, 16 teacher tokens: 11.3 and 18.2, what is done once
-// a row (sums over lanes, logarithms, the entries) taking half of it.
+// 32000 float32, a tenth of it padding, forward 166 (5.7), backward 312 (6.4); distillation of 8192 x
+// 50001 float32 with 32 teacher tokens and the cross-entropy, forward 253 (5.8), backward 497 (6.3);
+// of 2048 x 65536 bf16, 53 (5.0) and 86 (6.3). A large copy moves 5.0 TB/s. 32768 x 256 float32, 16
+// teacher tokens: 9.6 and 18.2, what is done once a row (sums over lanes, logarithms, the entries)
+// taking half of it.
 #include <algorithm>
 #include <type_traits>
 
@@ -40,10 +40,10 @@ constexpr int kTopMax = 64;        // alternatives of a row
 constexpr int kTeacherMax = 256;   // teacher tokens of a row
 // The threads to a row, by measurement (us, forward / backward of the distillation with 16 teacher
 // tokens and a target, float32): many short rows go to 16 lanes each, as what is done once a row
-// then costs a quarter (20971 x 400: 9.9 / 20 against 21 / 23 by a wave, 8192 x 1000: 8.9 / 17
-// against 10.5 / 16.5; but 2048 x 1000: 5.1 / 7.1 against 4.4 / 6.6); rows up to 1024, and many up to
-// 4096, to a wave (2048 x 1000: 4.4 / 6.6 against 8.7 / 8.1 by a workgroup, 4096 x 2000: 8.8 / 16
-// against 15.6 / 16; but 512 x 4000: 5.2 / 6.0 against 4.9 / 6.0); the rest to a workgroup.
+// then costs a quarter (20971 x 400: 10.1 / 19.4 against 18.1 / 20.5 by a wave, 8192 x 1000: 8.7 / 16.6
+// against 9.8 / 15.4; but 2048 x 1000: 5.3 / 6.5 against 4.6 / 5.8); rows up to 1024, and many up to
+// 4096, to a wave (2048 x 1000: 4.6 / 5.8 against 6.2 / 9.7 by a workgroup, 4096 x 2000: 8.8 / 14.5
+// against 12.5 / 14.9; but 512 x 4000: 5.4 / 5.8 against 4.7 / 5.8); the rest to a workgroup.
 constexpr int kPartVocab = 1024, kPartRows = 4096, kWaveVocab = 4096, kWaveRows = 1024;
 constexpr int kWaveHeld = 1024;     // one batch of a wave holds the row: it goes to one whatever the rows
 constexpr int kPartTop = 24, kPartLanes = 8;        // alternatives that 16 lanes pick, of rows up to kPartPick long
@@ -544,8 +544,8 @@ __device__ __forceinline__ void values_out(const T* __restrict__ x, int n, int k
 // out(rank, value, index) for the k largest of n logits (k <= n, no NaN, no +inf, the largest
 // `top`), equal ones by index. By a workgroup: a bound that k of the threads' maxima reach is reached
 // by at least k logits, and by hardly more; those are collected from the few batches that hold them
-// and ranked against each other. 999 rows of 50001 bf16 take 21 us, with 1, 20 and 64 alternatives
-// 25, 26 and 31 (27, 43 and 53 with the exact k-th maximum, found bit by bit, and each thread reading
+// and ranked against each other. 999 rows of 50001 bf16 take 20 us, with 1, 20 and 64 alternatives
+// 24, 25 and 28 (27, 43 and 53 with the exact k-th maximum, found bit by bit, and each thread reading
 // its own batches; 5 ms by rounds of arg-max for 64).
 template <typename G, int U, typename T, typename OUT>
 __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, float top, const Best& best,
@@ -578,9 +578,9 @@ __device__ __forceinline__ void pick(const T* __restrict__ x, int n, int k, floa
 
 // The same by a wave that holds the whole row, one batch and a rest. The bound is on the lanes'
 // maxima for few alternatives (one value a lane to count), on the logits themselves for more, of
-// which the lanes' maxima would let most of the row through. 8192 x 512 float32 takes 3.8 us, with 1,
-// 20 and 64 alternatives 9.0, 11.9 and 23; listed by ballots logit for logit 20 took 12.5, with an
-// atomic for each logit and the row read again 14.8.
+// which the lanes' maxima would let most of the row through. 8192 x 512 float32 takes 3.7 us, with 1,
+// 20 and 64 alternatives 7.4, 9.3 and 19. (When 20 took 11.9 so, listing by ballots logit for logit took
+// 12.5, and an atomic for each logit with the row read again 14.8.)
 template <typename G, int U, typename T, typename OUT>
 __device__ __forceinline__ void pick_held(const T* __restrict__ x, const float* v, int n, int k, float top,
                                           PickSpace<1>& sp, OUT&& out) {
@@ -634,9 +634,9 @@ __device__ __forceinline__ void pick_held(const T* __restrict__ x, const float* 
 // comparing each with the others, beyond kPartLanes alternatives on two maxima of each (of 16 values
 // a k-th near the last lets most of the row through); the logits that reach it in a list, ranked. One,
 // and a list too long or a bound of -inf (ties, masked rows, fewer maxima than alternatives), go by
-// rounds of (largest value, lowest index). 32768 x 256 float32 takes 7 us, with 1, 5, 8, 14, 20 and 24
-// alternatives 9.6, 11.5, 12.6, 15.6, 19.5 and 24.8; by rounds 5 and 8 took 15 and 18.7, on one maximum
-// of each lane 14 took 22, and by a wave 20 and 24 took 29 and 30 (in bf16 42 and 46, here 18.6 and 24).
+// rounds of (largest value, lowest index). 32768 x 256 float32 takes 6 us, with 1, 5, 8, 14, 20 and 24
+// alternatives 8.5, 10.7, 11.8, 14.8, 18.7 and 22.7 (in bf16 20 and 24 take 17.4 and 22.5); by rounds 5
+// and 8 took 15 and 18.7, on one maximum of each lane 14 took 22, and by a wave 25 take 27 (bf16 31).
 struct PartSpace {
   static constexpr int CAP = 96;
   uint64_t list[CAP + 5];   // four zeros behind it; odd: the groups use different banks
@@ -924,11 +924,11 @@ __global__ void __launch_bounds__(kRowThreads) logprob_join_kernel(const Logprob
 }
 
 // ---- gradients ---------------------------------------------------------------------------------
-// The dense part: f(x) for every logit of lo .. hi - 1, at most kBwdPieces pieces a thread. Four, for
-// both types: at float32 logits of 8192 x 32000 the log-probabilities' backward takes 346 us with 4,
-// 357 with 6 and 396 with 8 (registers cost waves); at bf16 ones of 8192 x 50001 it takes 328 with 4,
-// 376 with 2 (too few loads in flight), 334 with 6 and 383 with 8.
-template <typename T> constexpr int kBwdPieces = 4;
+// The dense part: f(x) for every logit of lo .. hi - 1, at most kBwdPieces pieces a thread. At 8192 x
+// 50001 the log-probabilities' backward takes 525 us in float32 (585 with two, 621 with three) and 298 in
+// bf16 (272 and 291), the distillation's 527 (541 and 610) and 314 (323 and 311); at 65536 x 1000 float32,
+// by 16 lanes, the latter takes 120 (176 and 144).
+constexpr int kBwdPieces = 4;
 // P pieces a thread, without a branch between them: past the last piece a thread takes that one again,
 // and writes what its owner writes. (A wait behind a branch is for everything, stores too: one for each
 // piece would wait for the piece before to reach memory.)
@@ -951,7 +951,7 @@ __device__ __forceinline__ void chunk_map(const T* __restrict__ x, T* __restrict
                                           F&& f) {
   constexpr int N = Piece<T>::N;
   const int n = hi - lo, full = n / N;
-  static_assert(kBwdPieces<T> == 4);
+  static_assert(kBwdPieces == 4);   // the cases below
   if (full > 3 * G::NT) pieces_map<G, 4>(x + lo, dx + lo, full, f);
   else if (full > 2 * G::NT) pieces_map<G, 3>(x + lo, dx + lo, full, f);
   else if (full > G::NT) pieces_map<G, 2>(x + lo, dx + lo, full, f);
@@ -1347,11 +1347,11 @@ static int row_threads(int64_t rows, int vocab, bool part) {
 }
 // The backward's equal chunks of a row, at most kBwdPieces pieces to a thread, whole 16-byte pieces.
 // A last chunk of what full ones leave would idle most of its threads: 16384 x 10000 in bf16, which is
-// one full chunk and a fifth of one, took 189 us so and takes 145 as two equal ones.
+// one full chunk and a fifth of one, took 189 us so and 145 as two equal ones (115 by now).
 template <typename T, typename P>
 static void set_chunks(P& p, int nt) {
   constexpr int N = Piece<T>::N;
-  const int most = nt * kBwdPieces<T> * N;
+  const int most = nt * kBwdPieces * N;
   p.chunks = (p.vocab + most - 1) / most;
   p.chunk = ((p.vocab + p.chunks - 1) / p.chunks + N - 1) / N * N;
 }
