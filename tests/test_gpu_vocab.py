@@ -462,6 +462,31 @@ def test_offsets_past_31_bits(m3, dev):
     assert torch.equal(dx[-8:], K.distill_backward(last, ids[-8:], u[-8:], t[-8:], stats[-8:], g[-8:], g[-8:], 2.0))
 
 
+def test_more_rows_than_one_grid_axis(m3, dev):
+    """Rows past the workgroups of a grid's first axis (2^27 rows by 16 lanes): the last ones as if
+    they were alone."""
+    K, rows, last = m3.kernels, (1 << 27) + 37, 8192
+    x = torch.randn(rows, 2, device=dev, dtype=torch.bfloat16)
+    t = torch.randint(0, 2, (rows,), device=dev)
+    ids = torch.randint(0, 2, (rows, 1), device=dev, dtype=torch.int32)
+    u = torch.randn(rows, 1, device=dev)
+    for part in (slice(rows - last, None), slice(0, last), slice((1 << 27) - last, 1 << 27)):
+        got = [a[part] for a in K.logprob_forward(x, t, top=1)]
+        want = K.logprob_forward(x[part], t[part], top=1)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    kd, nll, kstats = K.distill_forward(x, ids, u, t, 2.0)
+    stats = K.logprob_forward(x, t)[4]
+    ones = torch.ones(rows, device=dev)
+    dx = K.logprob_backward(x, t, stats, None, ones, ones)
+    dk = K.distill_backward(x, ids, u, t, kstats, ones, ones, 2.0)
+    for part in (slice(rows - last, None), slice(0, last)):
+        one = ones[part]
+        want = K.distill_forward(x[part], ids[part], u[part], t[part], 2.0)
+        assert torch.equal(kd[part], want[0]) and torch.equal(nll[part], want[1])
+        assert torch.equal(dk[part], K.distill_backward(x[part], ids[part], u[part], t[part], want[2], one, one, 2.0))
+        assert torch.equal(dx[part], K.logprob_backward(x[part], t[part], stats[part], None, one, one))
+
+
 def test_gradients_match_differences(m3, dev):
     """Central differences of float64-accumulated sums of the kernels' own outputs: a step h leaves
     h^2 of the third derivative and 2^-24 |f| / h of rounding."""
