@@ -44,7 +44,7 @@ constexpr int kSortOne = 4096;        // tokens that one workgroup sorts alone, 
 constexpr int kSortRounds = kSortOne / kSortThreads;
 constexpr int kSortBlocks = 64;       // workgroups of a larger sort, at most
 // Waves of run_sum that make its pieces longer: longer pieces leave fewer partials, shorter ones more
-// waves. The whole gradient at 32768 x 768 (3072 waves of 32 rows) 39 us so, 45 and 56 with pieces of
+// waves. The whole gradient at 32768 x 768 in pieces of 32 rows took 39 us, 45 and 56 with pieces of
 // 16 and 8; at 16384 x 1024 (2048 waves) 65 against 68 and 78.
 constexpr int64_t kRunWaves = 2048;
 
