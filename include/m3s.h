@@ -635,8 +635,9 @@ typedef struct m3s_embed_args {
   void* workspace;       /* backward scratch, 16-byte aligned */
   int64_t workspace_bytes; /* its size, at least m3s_embed_bwd_workspace_bytes() */
 } m3s_embed_args;
-/* The sorted ids and positions, digit counts and float32 partial sums; 0 for up to 1024
- * tokens, which need none (workspace may be NULL then). -1 on bad dimensions. No counterpart in the reference. */
+/* The sorted ids and positions, digit counts and float32 partial sums; 0 where none are
+ * needed, for up to 1024 tokens of a table of up to 2^26 entries (workspace may be NULL then).
+ * -1 on bad dimensions. No counterpart in the reference. */
 int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t width);
 int32_t m3s_embed_fwd(const m3s_embed_args* args, void* stream);
 int32_t m3s_embed_bwd(const m3s_embed_args* args, void* stream);

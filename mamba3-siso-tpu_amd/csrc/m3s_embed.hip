@@ -466,8 +466,11 @@ __global__ void __launch_bounds__(256) finish_kernel(const uint32_t* __restrict_
 // against 9.7 at 64 tokens and 6.7 against 11.4 at 1024; 1024 of 50001 ids, D 1024, 29.9 against 34.6
 // (7.0 TB/s). What it is slower at is a single id on all of the tokens, whose rows one workgroup of
 // each slice then adds: 16.6 against 10.6 at 512, 29.6 against 12.3 at 1024. There it ends: at 2048
-// Zipf's ids would gain a sixth, and the single id lose 50 us.
+// Zipf's ids would gain a sixth, and the single id lose 50 us. It ends too at tables that no cache
+// holds, where rows off a cache line's border are written as parts of lines (105209 x 851 float32: 94
+// against 72 us sorted; in bf16, half of it, 29 against 32).
 constexpr int kGatherTokens = 1024, kGatherRounds = kGatherTokens / 256;
+constexpr int64_t kGatherTable = 1 << 26;   // entries
 constexpr int kGatherRows = 1024;   // rows of a workgroup's, at most
 constexpr int kAlone = 16;          // tokens of a row that one wave adds alone: two rounds of loads
 
@@ -592,9 +595,9 @@ struct EmbedSpace {
   int run;                                      // sorted rows to a piece
 };
 
-static EmbedSpace embed_space(int64_t n, int64_t D) {   // for the wider of the two types, float32
+static EmbedSpace embed_space(int64_t n, int64_t vocab, int64_t D) {   // for the wider of the two types, float32
   EmbedSpace s = {};
-  if (n <= kGatherTokens) return s;   // no sort
+  if (n <= kGatherTokens && vocab * D <= kGatherTable) return s;   // no sort
   int64_t at = 0;
   const auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -651,7 +654,7 @@ static void launch_embed_bwd(const m3s_embed_args* a, hipStream_t s) {
   const ID* ids = static_cast<const ID*>(a->ids);
   const T* dy = static_cast<const T*>(a->dy);
   T* dtable = static_cast<T*>(a->dtable);
-  const EmbedSpace sp = embed_space(n, a->width);
+  const EmbedSpace sp = embed_space(n, a->vocab, a->width);
   if (sp.total == 0) {
     int lg = 0;   // 1024 workgroups to a slice, four to a CU: more would each read the ids again
     while (lg < 10 && (1 << lg) < a->vocab) ++lg;
@@ -677,8 +680,10 @@ static void launch_embed_bwd(const m3s_embed_args* a, hipStream_t s) {
     c.nrest = share + 1 == shares ? (int)((bytes - pieces * 16) / 2) : 0;
     return c;
   };
-  const auto cleaners = [&](const Clear& c) {   // workgroups: 8 pieces to a thread, or more
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(1024, (c.hi - c.lo) / (8 * kSortThreads)));
+  // Workgroups: 8 pieces to a thread, or more. 131072 x 1535 float32 takes 153 us with up to 8192 of them,
+  // 193 with 1024.
+  const auto cleaners = [&](const Clear& c) {
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(8192, (c.hi - c.lo) / (8 * kSortThreads)));
   };
   int last = 0;
   if (n <= kSortOne) {
@@ -749,7 +754,7 @@ static int32_t check_embed(const m3s_embed_args* a, const char* who, bool bwd) {
   M3S_REQUIRE(a->dtable && (a->tokens == 0 || (a->ids && a->dy)), "%s: NULL pointer", who);
   M3S_REQUIRE((uintptr_t)a->dy % es == 0, "%s: misaligned rows", who);
   M3S_REQUIRE(aligned16(a->workspace) && aligned16(a->dtable), "%s: dtable and workspace must be 16-byte aligned", who);
-  const int64_t need = embed_space(a->tokens, a->width).total;   // none for few tokens
+  const int64_t need = embed_space(a->tokens, a->vocab, a->width).total;   // none for few tokens
   M3S_REQUIRE(need == 0 || a->workspace, "%s: NULL pointer", who);
   M3S_REQUIRE(a->workspace_bytes >= need, "%s: workspace of %lld bytes, needs %lld", who,
               (long long)a->workspace_bytes, (long long)need);
@@ -762,7 +767,7 @@ using namespace m3s;
 
 extern "C" int64_t m3s_embed_bwd_workspace_bytes(int64_t tokens, int32_t vocab, int32_t width) {
   if (!embed_sizes_ok(tokens, vocab, width)) return -1;
-  return embed_space(tokens, width).total;
+  return embed_space(tokens, vocab, width).total;
 }
 
 extern "C" int32_t m3s_embed_fwd(const m3s_embed_args* a, void* stream) {

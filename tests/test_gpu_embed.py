@@ -112,6 +112,14 @@ def test_few_tokens(m3, dev, dtype, vocab, d):
             check_grad(got, holes, dy, 0.5, pad)
 
 
+def test_few_tokens_of_a_large_table(m3, dev):
+    """Past 2^26 entries few tokens are sorted too."""
+    gen = torch.Generator().manual_seed(5)
+    vocab, d = 70001, 961
+    tokens, dy = skewed(vocab, (900,), gen), torch.randn(900, d, generator=gen)
+    check_grad(m3.kernels.embedding_backward(tokens.to(dev), dy.to(dev), vocab, 0.5), tokens, dy, 0.5, None)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_padding_and_ids_outside_the_table(m3, dev, dtype):
     """The padding id's row is looked up and gets zeros back; an id outside the table gives NaN and

@@ -63,6 +63,8 @@ def test_embed_abi_refuses_bad_structs(m3):
         assert h.m3s_embed_bwd_workspace_bytes(*sizes) == -1
     assert h.m3s_embed_bwd_workspace_bytes(1024, 10, 4) == 0   # few tokens are not sorted
     assert h.m3s_embed_bwd_workspace_bytes(1025, 10, 4) > 0
+    assert h.m3s_embed_bwd_workspace_bytes(1024, 1 << 20, 64) == 0
+    assert h.m3s_embed_bwd_workspace_bytes(1024, 1 << 20, 65) > 0
 
 
 def test_structs_match_the_header(m3, tmp_path):
