@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in ``include/m3s.h`` (``csrc/libm3s.so``).
+"""ctypes binding of the C ABI in ``include/m3s.h`` (``csrc/libm3s.so``), and the autograd nodes
+in C++ that call the same library (``csrc/m3s_nodes.so``).
 
 The structs below mirror the header field for field; `m3s_abi_version` and the
 ``struct_size`` field of each args struct guard against a stale library.
@@ -8,12 +9,14 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import importlib.util
 import os
 
 import torch
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "csrc", "libm3s.so")
+NODES_PATH = os.path.join(HERE, "csrc", "m3s_nodes.so")
 ABI_VERSION = 10
 
 DTYPE_F32 = 0
@@ -377,6 +380,31 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         fn.argtypes = [C.POINTER(DistillArgs), vp]
     _lib = lib
     return lib
+
+
+_nodes = None
+
+
+def nodes(path: str = NODES_PATH):
+    """The module of the nodes in C++, bound to the library of `load`. Raises if it is missing or was
+    built against another torch."""
+    global _nodes
+    if _nodes is not None:
+        return _nodes
+    lib = load()
+    if not os.path.exists(path):
+        raise RuntimeError(f"{path} is missing: build it with `python __graft_entry__.py build`")
+    spec = importlib.util.spec_from_file_location("m3s_nodes", path)
+    try:
+        mod = importlib.util.module_from_spec(spec)
+    except ImportError as e:
+        raise RuntimeError(f"{path} does not load with torch {torch.__version__}; rebuild it ({e})") from e
+    if mod.torch_version != torch.__version__.split("+")[0]:
+        raise RuntimeError(f"{path} was built for torch {mod.torch_version}, not {torch.__version__}; rebuild it")
+    mod.bind(*(C.cast(fn, vp).value for fn in (lib.m3s_embed_fwd, lib.m3s_embed_bwd,
+                                               lib.m3s_embed_bwd_workspace_bytes, lib.m3s_last_error)))
+    _nodes = mod
+    return mod
 
 
 def check(rc: int, what: str) -> None:

@@ -1408,8 +1408,11 @@ class Call(NamedTuple):
         return type(self.args).from_buffer_copy(self.args)
 
 
-def embedding_call(table: Tensor, tokens: Tensor, scale: float, padding_idx: int = -1):
-    """`embedding_forward` with its `Call` and the dense tokens that the call read."""
+def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
+    """``scale * table[tokens]`` (one ``m3s_embed_fwd`` launch; the lookup of
+    ``model.py:194-232``): ``table`` (V, D) float32 or bf16 with any row stride, ``tokens`` int32
+    or int64 of any shape. The result is in the table's dtype, the product formed in float32. An
+    id outside [0, V) gives a row of NaN (no host synchronisation checks it)."""
     if table.dim() != 2:
         raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
     v, d = table.shape
@@ -1419,37 +1422,12 @@ def embedding_call(table: Tensor, tokens: Tensor, scale: float, padding_idx: int
     if col != 1 and d > 1:
         table = table.contiguous()
         row = d
-    if not tokens.is_contiguous():
-        tokens = tokens.contiguous()
+    tokens = tokens.contiguous()
     y = empty(*tokens.shape, d, device=dev, dtype=table.dtype)
-    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, v, d, scale, tokens.numel(), padding_idx,
+    a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, v, d, scale, tokens.numel(), -1,
                        tokens.data_ptr(), table.data_ptr(), row, y.data_ptr())
     _lib.launch(_lib.load().m3s_embed_fwd, a, dev, "m3s_embed_fwd")
-    return y, tokens, Call(a, dev, (a.ids,), tokens.stride())
-
-
-def embedding_forward(table: Tensor, tokens: Tensor, scale: float = 1.0) -> Tensor:
-    """``scale * table[tokens]`` (one ``m3s_embed_fwd`` launch; the lookup of
-    ``model.py:194-232``): ``table`` (V, D) float32 or bf16 with any row stride, ``tokens`` int32
-    or int64 of any shape. The result is in the table's dtype, the product formed in float32. An
-    id outside [0, V) gives a row of NaN (no host synchronisation checks it)."""
-    return embedding_call(table, tokens, scale)[0]
-
-
-def embedding_call_backward(a: "_lib.EmbedArgs", dev: torch.device, dy: Tensor) -> Tensor:
-    """`embedding_backward` by a copy of the forward's struct (`Call.again`)."""
-    dy = _row_grad(dy)
-    v, d, n = a.vocab, a.width, a.tokens
-    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", n, v, d)
-    if nbytes < 0:
-        raise ValueError(f"embedding: bad sizes (tokens {n}, vocab {v}, width {d})")
-    dtable = empty(v, d, device=dev, dtype=dy.dtype)
-    a.dy, a.dtable = dy.data_ptr(), dtable.data_ptr()
-    if nbytes:
-        ws = empty(nbytes, device=dev, dtype=torch.uint8)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
-    _lib.launch(_lib.load().m3s_embed_bwd, a, dev, "m3s_embed_bwd")
-    return dtable
+    return y
 
 
 def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.0,
@@ -1465,9 +1443,18 @@ def embedding_backward(tokens: Tensor, dy: Tensor, vocab: int, scale: float = 1.
     d, pad = dy.shape[-1], -1 if padding_idx is None else embedding_padding(padding_idx, vocab)
     id_bytes, code = _embed_checks(tokens, vocab, d), _lib.dtype_code(dy.dtype)
     dev = _device_of(tokens, dy)
-    tokens = tokens.contiguous()
+    tokens, dy = tokens.contiguous(), dy.contiguous()
+    nbytes = _lib.scratch_bytes("m3s_embed_bwd_workspace_bytes", tokens.numel(), vocab, d)
+    if nbytes < 0:
+        raise ValueError(f"embedding: bad sizes (tokens {tokens.numel()}, vocab {vocab}, width {d})")
+    dtable = empty(vocab, d, device=dev, dtype=dy.dtype)
     a = _lib.EmbedArgs(_EMBED_SIZE, code, id_bytes, vocab, d, scale, tokens.numel(), pad, tokens.data_ptr())
-    return embedding_call_backward(a, dev, dy)
+    a.dy, a.dtable = dy.data_ptr(), dtable.data_ptr()
+    if nbytes:
+        ws = empty(nbytes, device=dev, dtype=torch.uint8)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _lib.launch(_lib.load().m3s_embed_bwd, a, dev, "m3s_embed_bwd")
+    return dtable
 
 
 def embedding_padding(padding_idx: int, vocab: int) -> int:

@@ -27,6 +27,7 @@ from typing import Any, NamedTuple, Optional
 import torch
 import torch.nn.functional as F
 
+from . import _lib
 from . import kernels as K
 from . import layer as LY
 from . import layout as L
@@ -327,12 +328,14 @@ def _embed(table: Tensor, tokens: Tensor) -> Tensor:
     """``table[tokens]`` through `tokens.embed_tokens`, whose gradient sums each id's rows in
     parallel pieces in a fixed order. What that does not take (other dtypes, a forward-mode
     tangent, a trace) goes to ``F.embedding``."""
+    if table.is_cuda:   # at once: the checks below cost an eager one-token step as much as the launch
+        y = _lib.nodes().embed(table, tokens, 1.0, -1, K.POISON_OUTPUTS)
+        if y is not None:
+            return y
     if (table.is_cuda and tokens.device == table.device and table.dim() == 2 and table.numel()
             and (table.dtype == torch.float32 or table.dtype == torch.bfloat16)
             and tokens.dtype in K.ID_BYTES and not torch.jit.is_tracing() and not LY.has_tangent(table)):
-        if torch.is_grad_enabled() and table.requires_grad:
-            return TK.embed_tokens(table, tokens)
-        return K.embedding_forward(table, tokens)
+        return TK.embed_tokens(table, tokens)
     return F.embedding(tokens, table)
 
 

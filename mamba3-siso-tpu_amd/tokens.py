@@ -3,7 +3,7 @@ turns tokens into rows, and what is read off the logits (`token_logprobs`, `dist
 
 Each is one autograd node over the HIP kernels of ``csrc/m3s_embed.hip`` and
 ``csrc/m3s_vocab.hip``, or a plain launch where no gradient is taken. The nodes have no
-forward-mode rule and are differentiable once.
+forward-mode rule and are differentiable once. The lookup's is in C++ (``csrc/m3s_nodes.cpp``).
 """
 
 from __future__ import annotations
@@ -13,6 +13,7 @@ from typing import NamedTuple, Optional
 import torch
 from torch.autograd.function import once_differentiable
 
+from . import _lib
 from . import kernels as K
 from . import layer as LY
 
@@ -30,24 +31,22 @@ def _needs_node(*tensors) -> bool:
 
 
 class _EmbedFn(torch.autograd.Function):
-    """`kernels.embedding_forward` / `kernels.embedding_backward` as one node."""
+    """`kernels.embedding_forward` / `kernels.embedding_backward` as a node in Python, for what the
+    one in C++ does not take: strided ids or columns, a trace, and a tangent, which it refuses."""
 
     @staticmethod
     def forward(ctx, table, tokens, scale, padding_idx):
-        y, tokens, ctx.call = K.embedding_call(table, tokens, scale, padding_idx)
+        tokens = tokens.contiguous()
+        y = K.embedding_forward(table, tokens, scale)
         ctx.save_for_backward(tokens)
+        ctx.call = table.shape[0], scale, padding_idx if padding_idx >= 0 else None
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         (tokens,) = ctx.saved_tensors
-        a = ctx.call.again((tokens,))
-        if a is None:
-            a = ctx.call.args
-            return K.embedding_backward(tokens, dy, a.vocab, a.scale,
-                                        a.padding_idx if a.padding_idx >= 0 else None), None, None, None
-        return K.embedding_call_backward(a, ctx.call.device, dy), None, None, None
+        return K.embedding_backward(tokens, dy, *ctx.call), None, None, None
 
 
 def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
@@ -61,6 +60,9 @@ def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
     if table.dim() != 2:
         raise ValueError(f"embedding: the table must be (V, D), got {tuple(table.shape)}")
     pad = -1 if padding_idx is None else K.embedding_padding(int(padding_idx), table.shape[0])
+    y = _lib.nodes().embed(table, tokens, scale, pad, K.POISON_OUTPUTS)
+    if y is not None:
+        return y
     if _needs_node(table):
         return _EmbedFn.apply(table, tokens, float(scale), pad)
     return K.embedding_forward(table, tokens, scale)

@@ -258,3 +258,121 @@ def test_model_lookup_keeps_what_it_took(m3, dev):
         assert (fwad.unpack_dual(m3.model._embed(dual, tokens)).tangent == 1).all()
         with pytest.raises((NotImplementedError, RuntimeError)):
             m3.embed_tokens(dual, tokens)
+
+
+def test_lookup_node_is_in_cpp(m3, dev):
+    """A small training step's embedding is the host's to pay for: the node of ordinary operands runs
+    without the interpreter, through the entry point and through the model, in any shape and type."""
+    python_node = torch.autograd.function.BackwardCFunction
+    for dtype in (torch.float32, torch.bfloat16):
+        for ids in (torch.int32, torch.int64):
+            w = torch.randn(300, 24, device=dev).to(dtype).requires_grad_(True)
+            tokens = torch.randint(0, 300, (4, 9), device=dev, dtype=ids)
+            for y in (m3.embed_tokens(w, tokens), m3.embed_tokens(w[:, 3:19], tokens[0]), m3.model._embed(w, tokens)):
+                assert y.requires_grad and not isinstance(y.grad_fn, python_node)
+            with torch.no_grad():
+                assert not m3.embed_tokens(w, tokens).requires_grad
+    strided = m3.embed_tokens(w.t(), tokens.t() % 24)   # copied first, by the node in Python
+    assert isinstance(strided.grad_fn, python_node)
+    assert torch.equal(strided, w.t()[tokens.t() % 24])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n", [0, 1, 40, 3000, 30000])
+def test_node_gradients_are_the_bare_calls(m3, dev, dtype, n):
+    """Through the graph and by `kernels.embedding_backward`: the same bits, with a cotangent that is
+    dense, broadcast, strided or absent, twice from one graph, and into slices of a wider table."""
+    gen = torch.Generator().manual_seed(n)
+    K, vocab, d = m3.kernels, 200, 40
+    w = torch.randn(vocab, d, generator=gen).to(dtype).to(dev).requires_grad_(True)
+    tokens = skewed(vocab, (n,), gen).to(dev)
+    dys = [torch.randn(n, d, generator=gen).to(dtype).to(dev), torch.ones(1, 1, dtype=dtype, device=dev).expand(n, d),
+           torch.randn(d, n, generator=gen).to(dtype).to(dev).t()]
+    y = m3.embed_tokens(w, tokens, scale=1.5, padding_idx=-1)
+    assert torch.equal(y, K.embedding_forward(w.detach(), tokens, 1.5))
+    for dy in dys:
+        (dw,) = torch.autograd.grad(y, w, dy, retain_graph=True)
+        assert torch.equal(dw, K.embedding_backward(tokens, dy, vocab, 1.5, vocab - 1))
+    y.backward(dys[0])
+    assert torch.equal(w.grad, K.embedding_backward(tokens, dys[0], vocab, 1.5, vocab - 1))
+    with pytest.raises(RuntimeError, match="second time"):
+        y.backward(dys[0])
+    part = m3.embed_tokens(w[:, 8:24], tokens)
+    (dw,) = torch.autograd.grad(part, w, dys[0][:, :16])
+    assert torch.equal(dw[:, 8:24], K.embedding_backward(tokens, dys[0][:, :16], vocab))
+    assert not dw[:, :8].any() and not dw[:, 24:].any()
+
+
+def test_node_refusals_and_saved_tokens(m3, dev):
+    """No second derivative, no use of ids that changed in between, and ids that a hook kept elsewhere."""
+    gen = torch.Generator().manual_seed(1)
+    w = torch.randn(50, 8, generator=gen).to(dev).requires_grad_(True)
+    tokens = skewed(50, (30,), gen).to(dev)
+    dy = torch.randn(30, 8, generator=gen).to(dev).requires_grad_(True)
+    (dw,) = torch.autograd.grad(m3.embed_tokens(w, tokens), w, dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiate twice"):
+        torch.autograd.grad(dw.sum(), dy)
+    want = m3.kernels.embedding_backward(tokens, dy.detach(), 50)
+    assert torch.equal(dw, want)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.repeat(2).to(dev)[::2][:30]):
+        y = m3.embed_tokens(w, torch.arange(30, device=dev))   # comes back strided, other ids
+    (got,) = torch.autograd.grad(y, w, dy.detach())
+    assert torch.equal(got, m3.kernels.embedding_backward(torch.arange(30).repeat(2)[::2][:30].to(dev), dy.detach(), 50))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:7]):
+        y = m3.embed_tokens(w, tokens)
+    with pytest.raises(ValueError, match="another kind"):
+        torch.autograd.grad(y, w, dy.detach())
+    y = m3.embed_tokens(w, tokens)
+    tokens.add_(0)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        torch.autograd.grad(y, w, dy.detach())
+
+
+def test_captured_training_pass_replays_on_new_inputs(m3, dev):
+    """Lookup and gradient through autograd inside a recorded graph, replayed on changed tables, ids and
+    cotangents, every replay against the bare calls."""
+    gen = torch.Generator().manual_seed(16)
+    vocab, d, K = 300, 64, m3.kernels
+    for n in (50, 6000):
+        table = torch.zeros(vocab, d, device=dev)
+        tokens = torch.zeros(n, dtype=torch.int64, device=dev)
+        dy = torch.zeros(n, d, device=dev)
+
+        def step():
+            w = table.detach().requires_grad_(True)   # a leaf of its own: no eager graph shares it
+            y = m3.embed_tokens(w, tokens, scale=2.0, padding_idx=3)
+            return y.detach(), torch.autograd.grad(y, w, dy)[0]
+
+        side = torch.cuda.Stream(dev)
+        with torch.cuda.stream(side):
+            step()
+        side.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for _ in range(3):
+            table.copy_(torch.randn(vocab, d, generator=gen))
+            tokens.copy_(skewed(vocab, (n,), gen))
+            dy.copy_(torch.randn(n, d, generator=gen))
+            graph.replay()
+            assert torch.equal(out[0], K.embedding_forward(table, tokens, 2.0))
+            assert torch.equal(out[1], K.embedding_backward(tokens, dy, vocab, 2.0, padding_idx=3))
+            torch.cuda.synchronize()
+
+
+def test_node_runs_on_the_streams_of_its_forward(m3, dev):
+    """Two training passes on streams of their own at once, backward called from the default stream."""
+    gen = torch.Generator().manual_seed(19)
+    ws = [torch.randn(400, 32, generator=gen).to(dev).requires_grad_(True) for _ in range(2)]
+    ids = [skewed(400, (5000,), gen).to(dev) for _ in range(2)]
+    dy = torch.randn(5000, 32, generator=gen).to(dev)
+    want = [m3.kernels.embedding_backward(t, dy, 400) for t in ids]
+    torch.cuda.synchronize()
+    ys = []
+    for w, t in zip(ws, ids):
+        with torch.cuda.stream(torch.cuda.Stream(dev)):
+            ys.append(m3.embed_tokens(w, t))
+    torch.cuda.synchronize()
+    got = [torch.autograd.grad(y, w, dy)[0] for y, w in zip(ys, ws)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, x) for g, x in zip(got, want))
