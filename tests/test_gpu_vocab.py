@@ -738,3 +738,31 @@ def test_model_scores_and_distillation_step(m3, dev):
         assert abs(only.item() - part.item()) <= 1e-5 * abs(part.item())
     with pytest.raises(ValueError, match="vocabulary"):
         TR.make_distill_step(cfg, opt, teacher, M.LMConfig(vocab_size=41, n_layers=1, siso=siso))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,vocab", [(300, 32000), (1100, 4000)])
+def test_small_terms_beside_a_likely_token(m3, dev, dtype, rows, vocab):
+    """A row of one logit 0 and the rest at -16.75: their terms e^-16.75 = 0.89 eps (eps = 2^-24) are
+    below half of a step of 1, so a running sum that starts with the likely token takes none of them,
+    and the row's sum is short of one for each that the token's thread meets (124 of 32000, 61 of
+    4000: 110 and 54 eps). Summed batch by batch, the 15 terms beside the likely one are lost at most, 13.4
+    eps; each of the sums that are added to it, of up to 7 batches, 4 pieces and a rest, and the 8 joins
+    across lanes and waves, round by at most half a step of a number below 2, one eps each: 34 eps. The
+    terms' own errors (exp2's, their argument's and their sums', under 100 eps of the 0.0017 that they sum
+    to), the logarithm of 1 + 0.0017 and the result's roundings are under one eps together. log s
+    is off by no more than s: 35 eps."""
+    term = math.exp(-16.75)
+    x = torch.full((rows, vocab), -16.75).to(dtype)
+    x[:, 0] = 0.0
+    targets = torch.zeros(rows, dtype=torch.int64)
+    want = -math.log1p((vocab - 1) * term)
+    xd, t = x.to(dev), targets.to(dev)
+    ids = torch.zeros(rows, 1, dtype=torch.int64, device=dev)
+    u = torch.zeros(rows, 1, device=dev)
+    K = m3.kernels
+    calls = {"logp": K.logprob_forward(xd, t)[0], "top": K.logprob_forward(xd, t, top=2)[2][:, 0],
+             "nll": -K.distill_forward(xd, ids, u, t)[1], "kd": -K.distill_forward(xd, ids, u)[0],
+             "nll beside another temperature": -K.distill_forward(xd, ids, u, t, 1.5)[1]}
+    for what, got in calls.items():
+        assert (got.double() - want).abs().max().item() <= 35 * EPS, what
