@@ -143,8 +143,9 @@ bool takes(const Tensor& table, const Tensor& tokens) {
   if (!plain(table) || !plain(tokens) || tokens.device() != table.device() || table.dim() != 2) return false;
   const int64_t v = table.size(0), d = table.size(1);
   const auto type = table.scalar_type();
-  return v > 0 && v < INT32_MAX && d > 0 && d < INT32_MAX && (table.stride(1) == 1 || d == 1) &&
-         (type == at::kFloat || type == at::kBFloat16) && ids_type(tokens.scalar_type()) && tokens.is_contiguous();
+  return v > 0 && v < INT32_MAX && d > 0 && d < 1 << 22 && tokens.numel() < INT32_MAX - 63 &&
+         (table.stride(1) == 1 || d == 1) && (type == at::kFloat || type == at::kBFloat16) &&
+         ids_type(tokens.scalar_type()) && tokens.is_contiguous();
 }
 
 // embed(table, tokens, scale, padding id or -1, poison): the looked up rows, or None.

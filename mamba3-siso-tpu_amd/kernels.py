@@ -1369,6 +1369,11 @@ ID_BYTES = {torch.int32: 4, torch.int64: 8}
 _EMBED_SIZE = ctypes.sizeof(_lib.EmbedArgs)
 
 
+def embedding_fits(vocab: int, width: int, tokens: int) -> bool:
+    """Whether sizes are within the lookup's limits (the args struct holds the first two in 32 bits)."""
+    return vocab < (1 << 31) - 1 and width < 1 << 22 and tokens < (1 << 31) - 64
+
+
 def _embed_checks(tokens: Tensor, vocab: int, width: int) -> int:
     """The bytes of an id; the checks that the lookup and its backward share."""
     id_bytes = ID_BYTES.get(tokens.dtype)
@@ -1376,6 +1381,8 @@ def _embed_checks(tokens: Tensor, vocab: int, width: int) -> int:
         raise ValueError(f"embedding: tokens must be int32 or int64, got {tokens.dtype}")
     if vocab < 1 or width < 1:
         raise ValueError(f"embedding: the table must not be empty, got {(vocab, width)}")
+    if not embedding_fits(vocab, width, tokens.numel()):
+        raise ValueError(f"embedding: too large (tokens {tokens.numel()}, vocab {vocab}, width {width})")
     return id_bytes
 
 
@@ -1475,6 +1482,9 @@ def _logit_rows(logits: Tensor, what: str):
     dim = logits.dim()
     if dim == 0 or logits.shape[-1] == 0:
         raise ValueError(f"{what}: logits must be (..., V) with V >= 1, got {tuple(logits.shape)}")
+    # the args struct holds the sizes in 32 bits
+    if logits.numel() >= 1 << 30 and (logits.shape[-1] >= 1 << 30 or logits.numel() // logits.shape[-1] >= 1 << 31):
+        raise ValueError(f"{what}: logits must be fewer than 2^31 rows of fewer than 2^30, got {tuple(logits.shape)}")
     if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
     if dim > 3:

@@ -326,15 +326,16 @@ def _norm(x: Tensor, gain: Tensor, eps: float, dt: torch.dtype) -> Tensor:
 
 def _embed(table: Tensor, tokens: Tensor) -> Tensor:
     """``table[tokens]`` through `tokens.embed_tokens`, whose gradient sums each id's rows in
-    parallel pieces in a fixed order. What that does not take (other dtypes, a forward-mode
-    tangent, a trace) goes to ``F.embedding``."""
+    parallel pieces in a fixed order. What that does not take (other dtypes, sizes past
+    its limits, a forward-mode tangent, a trace) goes to ``F.embedding``."""
     if table.is_cuda:   # at once: the checks below cost an eager one-token step as much as the launch
         y = _lib.nodes().embed(table, tokens, 1.0, -1, K.POISON_OUTPUTS)
         if y is not None:
             return y
     if (table.is_cuda and tokens.device == table.device and table.dim() == 2 and table.numel()
             and (table.dtype == torch.float32 or table.dtype == torch.bfloat16)
-            and tokens.dtype in K.ID_BYTES and not torch.jit.is_tracing() and not LY.has_tangent(table)):
+            and tokens.dtype in K.ID_BYTES and not torch.jit.is_tracing() and not LY.has_tangent(table)
+            and K.embedding_fits(*table.shape, tokens.numel())):
         return TK.embed_tokens(table, tokens)
     return F.embedding(tokens, table)
 

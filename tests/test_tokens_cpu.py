@@ -172,3 +172,25 @@ def test_vocab_abi_refuses_bad_structs(m3):
         for bad in common + extra:
             assert entry(ctypes.byref(args(cls, **bad)), None) == lib.ERR_INVALID, (cls, bad)
         assert entry(ctypes.byref(args(cls, batch=0)), None) == lib.OK   # nothing to launch
+
+
+def test_sizes_past_32_bits_are_refused(m3):
+    """The args structs hold rows, vocabularies and widths in 32 bits: what is larger must not reach
+    them cut short (2^32 + 5 ids would become 5)."""
+    one, t = torch.zeros(1, 1), torch.zeros(3, dtype=torch.int64)
+    K = m3.kernels
+    for shape in ((2 ** 32 + 5, 1), (2 ** 31 - 1, 1), (1, 2 ** 32 + 4), (1, 2 ** 22)):
+        with pytest.raises(ValueError, match="too large"):
+            m3.embed_tokens(one.expand(shape), t)
+        with pytest.raises(ValueError, match="too large"):
+            K.embedding_backward(t, one[0].expand(3, shape[1]), shape[0])
+    with pytest.raises(ValueError, match="too large"):
+        m3.embed_tokens(torch.zeros(5, 4), t[:1].expand(2 ** 31))
+    assert K.embedding_fits(2 ** 31 - 2, 2 ** 22 - 1, 2 ** 31 - 65)
+    for shape in ((2 ** 32 + 3, 1), (2 ** 32, 3, 1), (3, 2 ** 32, 1), (2 ** 16, 2 ** 16, 4), (2 ** 31, 2), (1, 2 ** 32 + 8),
+                  (2, 2 ** 30)):
+        x = one.view(-1).expand(shape)
+        with pytest.raises(ValueError, match="fewer than 2\\^31"):
+            m3.token_logprobs(x, t)
+        with pytest.raises(ValueError, match="fewer than 2\\^31"):
+            m3.distill_loss(x, t[:, None], torch.zeros(3, 1))
