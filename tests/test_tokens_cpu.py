@@ -194,3 +194,27 @@ def test_sizes_past_32_bits_are_refused(m3):
             m3.token_logprobs(x, t)
         with pytest.raises(ValueError, match="fewer than 2\\^31"):
             m3.distill_loss(x, t[:, None], torch.zeros(3, 1))
+
+
+def test_node_module_is_checked_at_load(m3, tmp_path, monkeypatch):
+    """A missing module of nodes and one of another torch raise; its calls refuse other arguments."""
+    from mamba3_siso_tpu_amd import _lib as lib
+
+    mod = lib.nodes()
+    assert mod is lib.nodes() and mod.torch_version == torch.__version__.split("+")[0]
+    for call in (lambda: mod.embed(torch.zeros(2, 2)), lambda: mod.bind(1)):
+        with pytest.raises(TypeError):
+            call()
+    # what is not the node's: tensors on the CPU, and no tensors at all
+    assert mod.embed(torch.zeros(2, 2), torch.zeros(1, dtype=torch.int64), 1.0, -1, False) is None
+    assert mod.embed(None, [1], 1.0, -1, False) is None
+    monkeypatch.setattr(lib, "_nodes", None)
+    with pytest.raises(RuntimeError, match="missing"):
+        lib.nodes(str(tmp_path / "m3s_nodes.so"))
+    broken = tmp_path / "m3s_nodes.so"
+    broken.write_bytes(b"not a library")
+    with pytest.raises(RuntimeError, match="rebuild"):
+        lib.nodes(str(broken))
+    monkeypatch.setattr(torch, "__version__", "1.0.0+other")
+    with pytest.raises(RuntimeError, match="rebuild"):
+        lib.nodes()
