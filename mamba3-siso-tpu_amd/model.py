@@ -387,8 +387,9 @@ def lm_distill_loss(params: LMParams, xs: Tensor, ys: Tensor, teacher_ids: Tenso
                     teacher_logits: Tensor, cfg: LMConfig, temperature: float = 1.0,
                     hard_weight: float = 0.0, ignore_index: int = -100) -> Tensor:
     """Mean of ``(1 - hard_weight) kd + hard_weight nll`` (`tokens.distill_loss` of `lm_forward`'s
-    logits) over the positions whose ``ys`` is not ``ignore_index``: `lm_loss` with a teacher's best
-    tokens ``teacher_ids`` / ``teacher_logits`` (B, L, K) beside the text."""
+    logits) over the positions whose ``ys`` is not ``ignore_index`` (0, with a gradient of zeros, where
+    there are none): `lm_loss` with a teacher's best tokens ``teacher_ids`` / ``teacher_logits``
+    (B, L, K) beside the text."""
     live = ys != ignore_index
     ids = teacher_ids.masked_fill(~live.unsqueeze(-1), -1)
     # a part of weight 0 is left out, not multiplied: it may be infinite
@@ -397,7 +398,7 @@ def lm_distill_loss(params: LMParams, xs: Tensor, ys: Tensor, teacher_ids: Tenso
     total = out.nll.sum() * hard_weight if hard_weight != 0.0 else 0.0
     if hard_weight != 1.0:
         total = out.kd.sum() * (1.0 - hard_weight) + total
-    return total / live.sum()
+    return total / live.sum().clamp(min=1)
 
 
 def zero_states(cfg: LMConfig, batch: int, dtype=torch.float32, device=None) -> list:

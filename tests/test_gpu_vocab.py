@@ -766,3 +766,25 @@ def test_small_terms_beside_a_likely_token(m3, dev, dtype, rows, vocab):
              "nll beside another temperature": -K.distill_forward(xd, ids, u, t, 1.5)[1]}
     for what, got in calls.items():
         assert (got.double() - want).abs().max().item() <= 35 * EPS, what
+
+
+@pytest.mark.parametrize("weight", [0.0, 0.3, 1.0])
+def test_distillation_of_padding_alone(m3, dev, weight):
+    """A batch in which every position is padding has nothing to learn: a loss of 0 and gradients of
+    zeros, and a step leaves finite parameters."""
+    M, TR = m3.model, m3.train
+    siso = m3.SISOConfig(d_model=64, d_state=16, headdim=16, expand=1, chunk=64, policy_name="f32")
+    cfg = M.LMConfig(vocab_size=40, n_layers=1, siso=siso)
+    params = TR.train_params(M.init_lm(cfg, 1, device=dev))
+    gen = torch.Generator().manual_seed(3)
+    xs = torch.randint(0, 40, (2, 64), generator=gen).to(dev)
+    ys = torch.full((2, 64), -100, device=dev)
+    ids, u = torch.zeros(2, 64, 4, dtype=torch.int64, device=dev), torch.randn(2, 64, 4, generator=gen).to(dev)
+    loss = M.lm_distill_loss(params, xs, ys, ids, u, cfg, 2.0, weight)
+    assert loss.item() == 0.0
+    for g in torch.autograd.grad(loss, M.lm_leaves(params)):
+        assert not g.any()
+    opt = TR.make_optimizer(params, lr=1e-3, warmup=1, steps=10)
+    step = TR.make_distill_step(cfg, opt, M.init_lm(cfg, 2, device=dev), cfg, k=4, hard_weight=weight)
+    got, _, _ = step(params, opt, xs, ys)
+    assert got.item() == 0.0 and all(p.isfinite().all() for p in M.lm_leaves(params))
