@@ -207,11 +207,14 @@ def make_distill_step(cfg: M.LMConfig, opt: AdamW, teacher: M.LMParams, teacher_
                       k: int = 32, temperature: float = 2.0, hard_weight: float = 0.5,
                       ignore_index: int = -100):
     """`make_step` with a teacher: each step scores the batch with the ``teacher`` model (no
-    gradient), keeps its ``k`` best tokens at each position and trains on `model.lm_distill_loss`.
-    Targets equal to ``ignore_index`` are padding. The two models share a vocabulary."""
+    gradient), keeps its ``k`` (1 to 64) best tokens at each position, or the whole vocabulary if that
+    is smaller, and trains on `model.lm_distill_loss`. Targets equal to ``ignore_index`` are padding.
+    The two models share a vocabulary."""
     if teacher_cfg.vocab_size != cfg.vocab_size:
         raise ValueError(f"make_distill_step: the teacher's vocabulary of {teacher_cfg.vocab_size} is not "
                          f"the student's of {cfg.vocab_size}")
+    if not 1 <= min(k, cfg.vocab_size) <= K.TOP_MAX:
+        raise ValueError(f"make_distill_step: k must be in [1, {K.TOP_MAX}], got {k}")
     k = min(k, cfg.vocab_size)
 
     def step(params: M.LMParams, opt_state: AdamW, xs: Tensor, ys: Tensor):

@@ -218,3 +218,14 @@ def test_node_module_is_checked_at_load(m3, tmp_path, monkeypatch):
     monkeypatch.setattr(torch, "__version__", "1.0.0+other")
     with pytest.raises(RuntimeError, match="rebuild"):
         lib.nodes()
+
+
+def test_distill_step_refuses_k_when_it_is_built(m3):
+    """The teacher's pass leaves at most 64 tokens: another k is refused before the teacher has run."""
+    cfg = m3.model.LMConfig(vocab_size=100, n_layers=1, siso=m3.SISOConfig(d_model=64, d_state=16, headdim=16))
+    small = m3.model.LMConfig(vocab_size=40, n_layers=1, siso=cfg.siso)
+    for k in (0, -1, 65, 100, 1000):
+        with pytest.raises(ValueError, match="k must be in"):
+            m3.train.make_distill_step(cfg, None, None, cfg, k=k)
+    for k, c in ((1, cfg), (64, cfg), (100, small)):
+        assert callable(m3.train.make_distill_step(c, None, None, c, k=k))
