@@ -376,3 +376,21 @@ def test_node_runs_on_the_streams_of_its_forward(m3, dev):
     got = [torch.autograd.grad(y, w, dy)[0] for y, w in zip(ys, ws)]
     torch.cuda.synchronize()
     assert all(torch.equal(g, x) for g, x in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,vocab,d", [(22003, 256, 768), (33000, 256, 1030), (70001, 300, 20), (40000, 1000, 12),
+                                       (14001, 256, 700), (9000, 300007, 8), (5000, 1 << 18, 5), (66000, 262143, 9)])
+def test_gradient_of_training_batches(m3, dev, dtype, n, vocab, d):
+    """Long batches: pieces of 32 and of 16 sorted rows (65536 and 32768 rows times column tiles of 256
+    on) in one and in several tiles, ids in every piece and in hundreds of them, and sorts of two and three
+    passes by several workgroups."""
+    gen = torch.Generator().manual_seed(n)
+    dy = torch.randn(n, d, generator=gen).to(dtype)
+    dyd = dy.to(dev)
+    one = torch.full((n,), vocab - 2)
+    one[::7001] = 1
+    for tokens, pad in ((skewed(vocab, (n,), gen), None), (one, None), (skewed(vocab, (n,), gen), 0)):
+        got = m3.kernels.embedding_backward(tokens.to(dev), dyd, vocab, 0.5, pad)
+        check_grad(got, tokens, dy, 0.5, pad)
+        assert torch.equal(got, m3.kernels.embedding_backward(tokens.to(dev).int(), dyd, vocab, 0.5, pad))
