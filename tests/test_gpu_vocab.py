@@ -788,3 +788,23 @@ def test_distillation_of_padding_alone(m3, dev, weight):
     step = TR.make_distill_step(cfg, opt, M.init_lm(cfg, 2, device=dev), cfg, k=4, hard_weight=weight)
     got, _, _ = step(params, opt, xs, ys)
     assert got.item() == 0.0 and all(p.isfinite().all() for p in M.lm_leaves(params))
+
+
+def test_alternatives_past_31_bits(m3, dev):
+    """The alternatives of the last rows of logits with more than 2^31 entries: their ids equal those of the
+    rows on their own, and everything else is the formulas'."""
+    gen = torch.Generator().manual_seed(13)
+    rows, v, temp = 68000, 32000, 1.5
+    x = torch.zeros(rows, v, device=dev, dtype=torch.bfloat16)
+    last = make_logits((8, v), torch.bfloat16, gen)
+    x[-8:] = last.to(dev)
+    t = torch.full((rows,), -100, device=dev)
+    t[-8:] = torch.randint(0, v, (8,), generator=gen).to(dev)
+    logp, h, top_lp, ids, _, _ = logprob_ref(last, t[-8:].cpu(), 20, temp)
+    _, tol_lp, tol_h = bounds(last.double(), temp)
+    out = m3.kernels.logprob_forward(x, t, 20, temp)
+    assert torch.equal(out[3][-8:].cpu(), ids) and (out[3][:-8] == -1).all()
+    assert torch.equal(out[3][-8:], m3.kernels.logprob_forward(last.to(dev), t[-8:], 20, temp)[3])
+    same(out[0][-8:], logp, tol_lp, "logp")
+    same(out[1][-8:], h, tol_h, "entropy")
+    same(out[2][-8:], top_lp, tol_lp[:, None], "top_logp")
