@@ -11,7 +11,7 @@
 // by id, stably, and each id's rows stand together in position order:
 //
 //   1. least-significant-digit radix sort of (id, position), at most 9 bits a pass: one pass for
-//      bytes, two up to 2^18 ids. Ranks within a wave come from ballots (lanes with the same digit
+//      bytes, two for fewer than 2^18 ids. Ranks within a wave come from ballots (lanes with the same digit
 //      find each other bit by bit), across waves and workgroups from digit counts, so the order
 //      is that of the positions whatever runs first. Up to 4096 tokens one workgroup sorts in LDS.
 //      The sort waits more than it works and fills few CUs: workgroups beside it clear the table.
@@ -98,6 +98,12 @@ __device__ __forceinline__ void st_cols(T* p, cols<W> v) {
 }
 
 // ---- lookup -----------------------------------------------------------------------------
+// Two forms, by measurement (us; in brackets torch's embedding): 2^lg lanes to a row, whose loads go four at a time, for
+// rows below 16 KB (32768 x 768: float32 17.7, bf16 10.8 [16.8, 11.6]; 16384 x 2048 bf16 12.9, in the output's order
+// 14.1); the output's order for longer rows, where a wave's next loads would wait for its stores (8192 x 8192:
+// float32 45.8, bf16 24.3 [46.2, 25.0], by lanes 54.9 and 27.3; 8192 x 4096 float32 24.4 [24.9], 26.7), and for rows
+// narrower than a piece (4000000 x 1: float32 10.9, bf16 10.0, 12.6 and 13.1).
+//
 // 2^lg lanes to a row. An id outside the table reads nothing and gives a row of NaN.
 template <int W, typename T, typename ID>
 __global__ void __launch_bounds__(256) embed_fwd_kernel(const T* __restrict__ table, int64_t ld,
@@ -126,6 +132,41 @@ __global__ void __launch_bounds__(256) embed_fwd_kernel(const T* __restrict__ ta
     for (; c < D; c += step) {
       const int cc = min(c, D - W);
       st_cols<W>(out + cc, ld_cols<W>(row + cc) * scale);
+    }
+  }
+}
+
+// A workgroup writes 256 U pieces of W columns in the output's order. `per` pieces to a row, and a piece's row by a
+// reciprocal of that (i < 2^11 by per <= 2^10: the product is off by i / 2^32, less than 1 / per) or, of longer
+// rows, by one comparison.
+constexpr int kLookupPieces = 2;
+template <int W, typename T, typename ID>
+__global__ void __launch_bounds__(256) embed_order_kernel(const T* __restrict__ table, int64_t ld,
+                                                          const ID* __restrict__ ids,
+                                                          T* __restrict__ y, int64_t n, int vocab,
+                                                          int D, float scale, int per, uint32_t inv) {
+  constexpr int U = kLookupPieces, SPAN = 256 * U;
+  const int64_t all = n * per;
+  for (int64_t first = (int64_t)blockIdx.x * SPAN; first < all; first += (int64_t)gridDim.x * SPAN) {
+    const int64_t t0 = first >> 32 ? first / per : (uint32_t)first / (uint32_t)per;   // the 64-bit division is long
+    const uint32_t p0 = (uint32_t)(first - t0 * per);
+    cols<W> v[U];
+    int64_t at[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t i = p0 + u * 256 + threadIdx.x;
+      const uint32_t r = per > 1024 ? (uint32_t)(i >= (uint32_t)per) : per == 1 ? i : __umulhi(i, inv);
+      const int64_t t = min(t0 + r, n - 1);
+      const int c = min(W * (int)(i - r * (uint32_t)per), D - W);
+      const int64_t id = (int64_t)ids[t];
+      const bool ok = id >= 0 && id < vocab;
+      v[u] = ld_cols<W>(table + (ok ? id : 0) * ld + c);   // of no id row 0, dropped
+      v[u] = ok ? v[u] * scale : cols<W>(__builtin_nanf(""));
+      at[u] = t0 + r < n ? t * D + c : -1;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (at[u] >= 0) st_cols<W>(y + at[u], v[u]);
     }
   }
 }
@@ -625,12 +666,30 @@ constexpr int64_t kGridMax = 1 << 20;   // workgroups of a launch: the kernels s
 
 template <int W, typename T, typename ID>
 static void launch_embed_fwd(const m3s_embed_args* a, hipStream_t s) {
-  int lg = 0;
-  while (lg < 6 && (W << lg) < a->width) ++lg;   // lanes to a row, up to a wave
-  const int64_t blocks = std::min(kGridMax, (a->tokens + (256 >> lg) - 1) / (256 >> lg));
-  hipLaunchKernelGGL((embed_fwd_kernel<W, T, ID>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T*>(a->table), a->table_stride,
-                     static_cast<const ID*>(a->ids), static_cast<T*>(a->y), a->tokens, a->vocab,
-                     a->width, a->scale, lg);
+  const int per = (a->width + W - 1) / W;
+  const T* table = static_cast<const T*>(a->table);
+  const ID* ids = static_cast<const ID*>(a->ids);
+  T* y = static_cast<T*>(a->y);
+  if (W == 1 || per >= 1024) {
+    const uint32_t inv = per > 1 ? (uint32_t)((1ull << 32) / per + 1) : 0;
+    const int64_t span = 256 * kLookupPieces, blocks = std::min(kGridMax, (a->tokens * per + span - 1) / span);
+    hipLaunchKernelGGL((embed_order_kernel<W, T, ID>), dim3((unsigned)blocks), dim3(256), 0, s, table, a->table_stride,
+                       ids, y, a->tokens, a->vocab, a->width, a->scale, per, inv);
+    return;
+  }
+  if constexpr (W > 1) {
+    // Lanes to a row: a wave, or as many as idle an eighth of the row's pieces less at its end (32768 rows of 768 bf16,
+    // 96 pieces: 12.9 -> 10.8 us by 32 lanes; of 515, 65 pieces: 13.3 -> 10.4 by 16)
+    int lg = 0;
+    while (lg < 6 && (1 << lg) < per) ++lg;
+    const auto idle = [&](int l) { return ((per + (1 << l) - 1) >> l << l) - per; };
+    for (int l = 5; lg > 4 && l >= 4; --l) {
+      if (l < lg && 8 * (idle(lg) - idle(l)) > per) lg = l;
+    }
+    const int64_t blocks = std::min(kGridMax, (a->tokens + (256 >> lg) - 1) / (256 >> lg));
+    hipLaunchKernelGGL((embed_fwd_kernel<W, T, ID>), dim3((unsigned)blocks), dim3(256), 0, s, table, a->table_stride, ids,
+                       y, a->tokens, a->vocab, a->width, a->scale, lg);
+  }
 }
 
 template <int RUN, int W, typename T>

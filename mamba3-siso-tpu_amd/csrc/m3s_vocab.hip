@@ -746,7 +746,7 @@ struct LogprobParams {
   float* part;       // a split row's pieces: (rows, split, 3) sums, (rows, split, top) values and ids
   int64_t ignore, rows;
   int seqlen, vocab, top, chunks, chunk, split, share;   // chunk, share: logits to one of chunks, to a piece
-  float temp, inv_t, c;
+  float inv_t, c;
 };
 
 struct LogprobParts {
@@ -1402,7 +1402,6 @@ static LogprobParams logprob_params(const m3s_logprob_args* a) {
   p.vocab = a->vocab;
   p.top = a->top;
   p.part = static_cast<float*>(a->workspace);
-  p.temp = a->temperature;
   p.inv_t = (float)(1.0 / a->temperature);
   p.c = (float)(1.4426950408889634 / a->temperature);
   return p;

@@ -394,3 +394,23 @@ def test_gradient_of_training_batches(m3, dev, dtype, n, vocab, d):
         got = m3.kernels.embedding_backward(tokens.to(dev), dyd, vocab, 0.5, pad)
         check_grad(got, tokens, dy, 0.5, pad)
         assert torch.equal(got, m3.kernels.embedding_backward(tokens.to(dev).int(), dyd, vocab, 0.5, pad))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [1, 2, 3, 5, 7, 8, 65, 129, 515, 768, 1100, 4092, 4095, 4096, 4097, 8191, 8192, 8195, 40003])
+def test_lookup_of_every_row_form(m3, dev, dtype, d):
+    """Rows narrower than 16 bytes, of lanes that divide them evenly or not, and of 16 KB and more, dense
+    and as slices of wider ones; ids outside the table among them. A product in float32, rounded once:
+    the same bits as torch's."""
+    gen = torch.Generator().manual_seed(d)
+    wide = torch.randn(37, d + 5, generator=gen).to(dtype).to(dev)
+    for n in (1, 2, 700, 1031):
+        tokens = torch.randint(0, 37, (n,), generator=gen)
+        tokens[3::50] = torch.tensor([-1, 37, 1 << 40])[torch.arange(len(tokens[3::50])) % 3]
+        tokens = tokens.to(dev)
+        bad = (tokens < 0) | (tokens >= 37)
+        for table in (wide[:, :d].contiguous(), wide[:, 3:3 + d]):
+            for scale in (1.0, 22.7):
+                y = m3.embed_tokens(table, tokens, scale=scale)
+                want = (table[tokens.clamp(0, 36)].float() * scale).to(dtype)
+                assert torch.equal(y[~bad], want[~bad]) and y[bad].isnan().all()
