@@ -739,10 +739,10 @@ static void launch_embed_bwd(const m3s_embed_args* a, hipStream_t s) {
     c.nrest = share + 1 == shares ? (int)((bytes - pieces * 16) / 2) : 0;
     return c;
   };
-  // Workgroups: 8 pieces to a thread, or more. 131072 x 1535 float32 takes 153 us with up to 8192 of them,
-  // 193 with 1024.
+  // Workgroups: a piece to a thread, and no loop (the gradient of one token of 131072 x 1536 float32 takes 135 us
+  // so, 144 with 8 pieces or more to a thread of up to 8192; of 100 tokens of 256000 x 2048 341 and 391).
   const auto cleaners = [&](const Clear& c) {
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(8192, (c.hi - c.lo) / (8 * kSortThreads)));
+    return (unsigned)std::max<int64_t>(1, std::min<int64_t>(kGridMax, (c.hi - c.lo + kSortThreads - 1) / kSortThreads));
   };
   int last = 0;
   if (n <= kSortOne) {
