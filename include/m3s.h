@@ -614,7 +614,7 @@ int32_t m3s_gemv_fused(const m3s_gemv_fused_args* args, void* stream);
 
 /* The LM's embedding: y[t] = scale table[ids[t]] (the lookup of model.py:194-232, with a
  * scale), and its gradient dtable[v] = scale sum of dy[t] over the t with ids[t] = v, summed in
- * float32 in position order and rounded once (bit-reproducible). Rows of ids that do not occur,
+ * float32 in a fixed order and rounded once (bit-reproducible). Rows of ids that do not occur,
  * and of padding_idx, are zeros. An id outside [0, vocab) gives a row of NaN in y and adds to no
  * row. y, dy and dtable are dense, y and dy aligned to one element, dtable to 16 bytes;
  * vocab < 2^31 - 1, width < 2^22, tokens < 2^31 - 64. */

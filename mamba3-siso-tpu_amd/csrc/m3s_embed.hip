@@ -26,10 +26,10 @@
 // table once (a row that occurs twice): bound by HBM from a few MB on, by the launches below that.
 //
 // Measured: 32768 byte tokens (Zipf), D 768, float32: lookup 17.9 us (5.6 TB/s of output), gradient
-// 33 us, of which run_sum 18 (5.6 TB/s of dy), the sort 8 and finish 6. 16384 tokens of 50001, D 1024:
-// gradient 61 us, of which clearing 205 MB beside the four sort launches takes 36 (5.7 TB/s) and
-// run_sum 20 to 25; cleared by a pass of its own behind the sort it took 96 in all. 777 tokens of
-// 32003, D 515, bf16: 12.3 us in one launch (2.7 TB/s, the table's 33 MB), 16.4 sorted.
+// 34 us, of which run_sum 19 (5.3 TB/s of dy), the sort 9 and finish 6. 16384 tokens of 50001, D 1024:
+// gradient 66 us, of which clearing 205 MB beside the four sort launches takes 38 (5.4 TB/s) and
+// run_sum 25; cleared by a pass of its own behind the sort it took 96 in all. 777 tokens of
+// 32003, D 515, bf16: 13.2 us in one launch (2.5 TB/s, the table's 33 MB), 16.4 sorted.
 #include <algorithm>
 
 #include "m3s_common.h"

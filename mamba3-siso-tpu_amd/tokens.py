@@ -54,7 +54,7 @@ def embed_tokens(table: Tensor, tokens: Tensor, scale: float = 1.0,
     """``scale * table[tokens]``, differentiable in ``table`` (V, D) float32 or bf16; ``tokens``
     int32 or int64 of any shape, on the table's device.
 
-    The gradient is dense, summed in float32 in position order and so bit-reproducible.
+    The gradient is dense, summed in float32 in a fixed order and so bit-reproducible.
     ``padding_idx`` names an id (negative: from the end) whose row is looked up but gets no
     gradient. An id outside [0, V) gives a row of NaN, and no gradient."""
     if table.dim() != 2:
