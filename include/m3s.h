@@ -716,6 +716,80 @@ int64_t m3s_distill_workspace_bytes(int64_t rows, int32_t vocab);
 int32_t m3s_distill_fwd(const m3s_distill_args* args, void* stream);
 int32_t m3s_distill_bwd(const m3s_distill_args* args, void* stream);
 
+/* Rows in 8 bits, for products on the matrix cores' block-scaled form; no counterpart in the
+ * reference. e4m3 values in blocks of 32 along a row, each with a scale 2^e, e the smallest integer
+ * >= -126 with the block's largest finite magnitude times 2^-e at most 448; a value is rounded to
+ * nearest (ties to even), and an entry that is not finite becomes NaN. values is (rows, kp) bytes,
+ * kp the width rounded up to 128 and zeros behind the width; scales (kp / 128, rows, 4) bytes of
+ * e + 127. values 16-byte aligned. */
+#define M3S_DTYPE_ROWS8 2              /* of m3s_matmul8_args.x_dtype alone */
+#define M3S_ROWS8_MAX 16777215         /* rows: 2^24 - 1 */
+#define M3S_ROWS8_WIDTH_MAX 1048576    /* width: 2^20; with a norm 16384 */
+#define M3S_MATMUL8_FLOAT_ROWS 16
+
+/* Rows to 8 bits. With a gain the rows are first normalised, as m3s_rms_fwd does, and with `add`
+ * the residual is added before that: s = x + add in x_dtype goes to `sum`, and the rows are those of
+ * s / sqrt(mean(s^2) + eps) gain in float32. Rows may start at any element. */
+typedef struct m3s_rows8_args {
+  int32_t struct_size;  /* sizeof(m3s_rows8_args) */
+  int32_t x_dtype;      /* M3S_DTYPE_* of x and sum */
+  int32_t width;
+  float eps;
+  int64_t rows;
+  const void* x;        /* (rows, width), ldx elements from row to row */
+  int64_t ldx;
+  const void* add;      /* (rows, width) bf16, or NULL */
+  int64_t ldadd;
+  const float* gain;    /* (width), or NULL: no norm */
+  void* sum;            /* out (rows, width) dense, iff add */
+  void* values;         /* out (rows, kp) */
+  void* scales;         /* out (kp / 128, rows, 4) */
+} m3s_rows8_args;
+int32_t m3s_rows8(const m3s_rows8_args* args, void* stream);
+
+/* The values that rows in 8 bits stand for, dense. */
+typedef struct m3s_rows8_values_args {
+  int32_t struct_size;  /* sizeof(m3s_rows8_values_args) */
+  int32_t y_dtype;      /* M3S_DTYPE_* of y (bf16 holds every value exactly) */
+  int32_t width;
+  int64_t rows;
+  const void* values;
+  const void* scales;
+  void* y;              /* out (rows, width) */
+} m3s_rows8_values_args;
+int32_t m3s_rows8_values(const m3s_rows8_values_args* args, void* stream);
+
+/* The projections of the LM (layer.py:233, 256; model.py:125-140, 231) on 8-bit rows and weights:
+ * y (rows, n) bf16 = act(x w + bias) + residual, dense. Gated: w has 2 n columns, value | gate, and
+ * value silu(gate) goes out as rows in 8 bits. x in 8 bits, or up to M3S_MATMUL8_FLOAT_ROWS rows in
+ * bf16 or float32, rounded to 8 bits on the way.
+ * w is packed: for every 16-row tile of its outputs and every 128 k, two planes (k 0-63, 64-127) of
+ * 64 lanes' 16 bytes, lane 16 g + r holding row r's k 16 g .. 16 g + 15 of the plane; w_scales
+ * (kp / 128, packed rows, 4). Packed row 64 q + 16 t + 4 g + i is output 64 q + 32 (t >> 1) + 8 g +
+ * 4 (t & 1) + i, n rounded up to 64 of them; gated, it is output 32 q + 8 g + 4 (t & 1) + i of value
+ * (t < 2) or gate, with n rounded up to 128. Rows behind n are zeros. */
+enum { M3S_ACT_NONE = 0, M3S_ACT_SILU = 1, M3S_ACT_GELU = 2, M3S_ACT_RELU = 3 };
+typedef struct m3s_matmul8_args {
+  int32_t struct_size;  /* sizeof(m3s_matmul8_args) */
+  int32_t x_dtype;      /* M3S_DTYPE_ROWS8, or of float rows */
+  int32_t k, n;
+  int32_t gated;
+  int32_t activation;   /* M3S_ACT_*: gelu is the one with erf; none with a gate */
+  int64_t rows;
+  const void* x;        /* (rows, kp) values, or (rows, k) with ldx elements from row to row */
+  int64_t ldx;          /* float rows */
+  const void* x_scales;
+  const void* w;
+  const void* w_scales;
+  const float* bias;    /* (n), gated (2 n), or NULL */
+  const void* residual; /* (rows, n) bf16, or NULL; not with a gate */
+  int64_t ldres;
+  void* y;              /* out (rows, n) bf16, or NULL with a gate */
+  void* y_values;       /* gated: out (rows, n rounded up to 128) */
+  void* y_scales;
+} m3s_matmul8_args;
+int32_t m3s_matmul8(const m3s_matmul8_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -256,6 +256,34 @@ class DistillArgs(C.Structure):
     ]
 
 
+class Rows8Args(C.Structure):
+    _fields_ = [
+        ("struct_size", i32), ("x_dtype", i32), ("width", i32), ("eps", C.c_float), ("rows", i64),
+        ("x", vp), ("ldx", i64), ("add", vp), ("ldadd", i64), ("gain", vp), ("sum", vp),
+        ("values", vp), ("scales", vp),
+    ]
+
+
+class Rows8ValuesArgs(C.Structure):
+    _fields_ = [
+        ("struct_size", i32), ("y_dtype", i32), ("width", i32), ("rows", i64), ("values", vp),
+        ("scales", vp), ("y", vp),
+    ]
+
+
+class Matmul8Args(C.Structure):
+    _fields_ = [
+        ("struct_size", i32), ("x_dtype", i32), ("k", i32), ("n", i32), ("gated", i32),
+        ("activation", i32), ("rows", i64), ("x", vp), ("ldx", i64), ("x_scales", vp), ("w", vp),
+        ("w_scales", vp), ("bias", vp), ("residual", vp), ("ldres", i64), ("y", vp),
+        ("y_values", vp), ("y_scales", vp),
+    ]
+
+
+#: ``M3S_DTYPE_ROWS8``, and the limits of the rows in 8 bits (``M3S_ROWS8_*``, ``M3S_MATMUL8_*``)
+DTYPE_ROWS8 = 2
+ROWS8_MAX, ROWS8_WIDTH_MAX, ROWS8_NORM_MAX, MATMUL8_FLOAT_ROWS = (1 << 24) - 1, 1 << 20, 16384, 16
+
 #: ``M3S_GEMV_*``
 GEMV_NORM, GEMV_GATE, GEMV_HEAD = 1, 2, 3
 
@@ -271,7 +299,8 @@ EXPORTS = ("m3s_abi_version", "m3s_last_error", "m3s_supported", "m3s_fwd_raw_su
            "m3s_norm_bwd_noalloc", "m3s_adamw", "m3s_wgrad", "m3s_wgrad_workspace_bytes", "m3s_gemv",
            "m3s_gemv_fused", "m3s_embed_bwd_workspace_bytes", "m3s_embed_fwd", "m3s_embed_bwd",
            "m3s_logprob_fwd", "m3s_logprob_bwd", "m3s_distill_fwd", "m3s_distill_bwd",
-           "m3s_logprob_workspace_bytes", "m3s_distill_workspace_bytes")
+           "m3s_logprob_workspace_bytes", "m3s_distill_workspace_bytes", "m3s_rows8", "m3s_rows8_values",
+           "m3s_matmul8")
 
 _lib = None
 
@@ -378,6 +407,10 @@ def load(path: str = LIB_PATH) -> C.CDLL:
     for fn in (lib.m3s_distill_fwd, lib.m3s_distill_bwd):
         fn.restype = i32
         fn.argtypes = [C.POINTER(DistillArgs), vp]
+    for fn, args in ((lib.m3s_rows8, Rows8Args), (lib.m3s_rows8_values, Rows8ValuesArgs),
+                     (lib.m3s_matmul8, Matmul8Args)):
+        fn.restype = i32
+        fn.argtypes = [C.POINTER(args), vp]
     _lib = lib
     return lib
 

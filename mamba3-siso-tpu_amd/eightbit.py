@@ -1,0 +1,312 @@
+"""The language model's rows, weights and products in 8 bits, for serving.
+
+Rows and weights are e4m3 values in blocks of 32 along the axis that a product sums over, each block
+with a power of two as its scale: the smallest one (from 2^-126 on) by which the block's largest
+magnitude is at most 448, e4m3's largest value (`Rows8`). The matrix cores multiply this form at twice
+the rate of bf16, and a weight takes half the memory and half the traffic.
+
+* `quantize8`  -- rows to 8 bits;
+* `rms_norm8`  -- the residual's addition and the block norm, its rows in 8 bits;
+* `pack8`      -- a projection's weight, rounded and laid out once;
+* `matmul8`    -- rows times a packed weight, with bias, activation and residual;
+* `swiglu8`    -- the gated MLP's first product and its gate, the rows out in 8 bits.
+
+Each is one launch of ``csrc/m3s_rows8.hip`` or ``csrc/m3s_matmul8.hip`` (`matmul8` and `swiglu8` of
+more than 16 float rows two). They take no gradient and refuse operands that need one.
+`model.eight_bit_params` makes a model of them.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+from . import kernels as K
+from . import layer as LY
+
+Tensor = torch.Tensor
+
+#: Values that share a scale, and the width that rows are padded to (the K of one matrix instruction).
+BLOCK, STEP = 32, 128
+ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+class Rows8(NamedTuple):
+    """Rows in 8 bits: ``values`` (rows, kp) float8_e4m3fn, kp the ``width`` rounded up to 128 (zeros
+    behind the width); ``scales`` (kp / 128, rows, 4) float8_e8m0fnu, the scales of a row's four
+    blocks of each 128; ``lead``, the shape of the leading axes, whose product is ``rows``."""
+
+    values: Tensor
+    scales: Tensor
+    width: int
+    lead: tuple
+
+    @property
+    def shape(self) -> tuple:
+        return (*self.lead, self.width)
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+        """The values that the 8 bits stand for, (..., width) in bf16 (exact) or float32."""
+        rows = _check_rows8(self, "dequantize")
+        y = K.empty(*self.lead, self.width, device=self.values.device, dtype=dtype)
+        a = _lib.Rows8ValuesArgs(ctypes.sizeof(_lib.Rows8ValuesArgs), _lib.dtype_code(dtype), self.width,
+                                 rows, self.values.data_ptr(), self.scales.data_ptr(), y.data_ptr())
+        _lib.launch(_lib.load().m3s_rows8_values, a, self.values.device, "m3s_rows8_values")
+        return y
+
+
+class Weight8(NamedTuple):
+    """A projection's weight (k, n) packed for the products (`pack8`): ``values``
+    (tiles, steps, 2, 64, 16) float8_e4m3fn and ``scales`` (steps, 16 tiles, 4) float8_e8m0fnu.
+    ``gated``: its columns are value | gate, n of each."""
+
+    values: Tensor
+    scales: Tensor
+    k: int
+    n: int
+    gated: bool
+
+    @property
+    def shape(self) -> tuple:
+        return (self.k, 2 * self.n if self.gated else self.n)
+
+    @property
+    def device(self) -> torch.device:
+        return self.values.device
+
+
+def _padded(n: int, to: int) -> int:
+    return (n + to - 1) // to * to
+
+
+def _refuse_gradient(what: str, *tensors) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: 8-bit operators take no gradient (detach the operands, or call "
+                                 "under torch.no_grad)")
+    if torch.jit.is_tracing() or LY.has_tangent(*tensors):
+        raise ValueError(f"{what}: 8-bit operators take no forward-mode tangent and no trace")
+
+
+def _check_rows8(x: Rows8, what: str) -> int:
+    rows, kp = 1, _padded(x.width, STEP)
+    for n in x.lead:
+        rows *= n
+    if (tuple(x.values.shape) != (rows, kp) or x.values.dtype != torch.float8_e4m3fn
+            or tuple(x.scales.shape) != (kp // STEP, rows, 4) or x.scales.dtype != torch.float8_e8m0fnu
+            or not x.values.is_contiguous() or not x.scales.is_contiguous()):
+        raise ValueError(f"{what}: rows must be dense Rows8 of {rows} x {x.width}")
+    return rows
+
+
+def _new_rows8(lead: tuple, rows: int, width: int, dev) -> Rows8:
+    kp = _padded(width, STEP)
+    return Rows8(K.empty(rows, kp, device=dev, dtype=torch.float8_e4m3fn),
+                 K.empty(kp // STEP, rows, 4, device=dev, dtype=torch.float8_e8m0fnu), width, lead)
+
+
+def _row_view(x: Tensor) -> Tensor:
+    """``x`` (..., width) as (rows, width) with any row stride and unit column stride; a copy where the
+    leading axes do not run as one."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.numel() else x.new_empty(_count(x.shape[:-1]), x.shape[-1])
+    if (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+        x = x.contiguous()
+    return x
+
+
+def _count(shape) -> int:
+    n = 1
+    for s in shape:
+        n *= s
+    return n
+
+
+def _row_stride(x: Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _check_sizes(what: str, rows: int, width: int, most: int = _lib.ROWS8_WIDTH_MAX) -> None:
+    if not 1 <= width <= most or rows > _lib.ROWS8_MAX:
+        raise ValueError(f"{what}: {rows} rows of {width} (at most {_lib.ROWS8_MAX} of 1 to {most})")
+
+
+def _check_float_rows(x: Tensor, what: str) -> None:
+    if x.dtype not in _FLOATS:
+        raise ValueError(f"{what}: rows must be float32 or bf16, got {x.dtype}")
+    if x.dim() < 1:
+        raise ValueError(f"{what}: rows must have an axis, got a scalar")
+
+
+def quantize8(x: Tensor) -> Rows8:
+    """``x`` (..., width) float32 or bf16 as `Rows8`: each value rounded to the nearest e4m3 of its
+    block's scale, ties to even. An entry that is not finite becomes NaN and leaves the scale of its
+    block to the others. Rows may have any stride between them."""
+    _check_float_rows(x, "quantize8")
+    dev = K._device_of(x)
+    _refuse_gradient("quantize8", x)
+    lead, width = tuple(x.shape[:-1]), x.shape[-1]
+    rows = _count(lead)
+    _check_sizes("quantize8", rows, width)
+    x = _row_view(x)
+    out = _new_rows8(lead, rows, width, dev)
+    a = _lib.Rows8Args(ctypes.sizeof(_lib.Rows8Args), _lib.dtype_code(x.dtype), width, 0.0, rows,
+                       x.data_ptr(), _row_stride(x), None, 0, None, None, out.values.data_ptr(),
+                       out.scales.data_ptr())
+    _lib.launch(_lib.load().m3s_rows8, a, dev, "m3s_rows8")
+    return out
+
+
+def rms_norm8(x: Tensor, gain: Tensor, eps: float, add: Optional[Tensor] = None):
+    """``(s, rows)``: ``s = x + add``, the residual stream ``x`` (..., width) float32 or bf16 after a
+    block whose bf16 output is ``add`` (``x`` itself without one), and ``s / sqrt(mean(s^2) + eps) *
+    gain`` in 8 bits, with float32 statistics and no rounding before the one to 8 bits. ``s`` is in the
+    stream's type. The width is at most 16384."""
+    _check_float_rows(x, "rms_norm8")
+    lead, width = tuple(x.shape[:-1]), x.shape[-1]
+    rows = _count(lead)
+    _check_sizes("rms_norm8", rows, width, _lib.ROWS8_NORM_MAX)
+    if tuple(gain.shape) != (width,):
+        raise ValueError(f"rms_norm8: gain must be ({width},), got {tuple(gain.shape)}")
+    if add is not None and (add.dtype != torch.bfloat16 or add.shape != x.shape):
+        raise ValueError(f"rms_norm8: add must be bf16 {tuple(x.shape)}, got {add.dtype} {tuple(add.shape)}")
+    dev = K._device_of(x, gain, add)
+    _refuse_gradient("rms_norm8", x, gain, add)
+    gain = gain.detach()
+    if gain.dtype != torch.float32 or not gain.is_contiguous():
+        gain = gain.float().contiguous()
+    xr = _row_view(x)
+    out = _new_rows8(lead, rows, width, dev)
+    a = _lib.Rows8Args(ctypes.sizeof(_lib.Rows8Args), _lib.dtype_code(x.dtype), width, eps, rows,
+                       xr.data_ptr(), _row_stride(xr), None, 0, gain.data_ptr(), None,
+                       out.values.data_ptr(), out.scales.data_ptr())
+    s = x
+    if add is not None:
+        add = _row_view(add)
+        s = K.empty(x.shape, device=dev, dtype=x.dtype)
+        a.add, a.ldadd, a.sum = add.data_ptr(), _row_stride(add), s.data_ptr()
+    _lib.launch(_lib.load().m3s_rows8, a, dev, "m3s_rows8")
+    return s, out
+
+
+def _packed_rows(n: int, gated: bool) -> Tensor:
+    """Which column of the weight each packed row holds, -1 behind the last. Four 16-row tiles t are a
+    group: row 4 g + i of tile t is output 64 q + 32 (t >> 1) + 8 g + 4 (t & 1) + i of group q, so that
+    a lane of the products has 8 neighbouring outputs; gated, the first two tiles are value's
+    outputs 32 q + ... and the others gate's."""
+    groups = _padded(n, 128) // 32 if gated else _padded(n, 64) // 64
+    q, t, g, i = torch.meshgrid(torch.arange(groups), torch.arange(4), torch.arange(4), torch.arange(4),
+                                indexing="ij")
+    j = 8 * g + 4 * (t & 1) + i
+    if gated:
+        out = 32 * q + j
+        col = torch.where(out < n, out + n * (t >> 1), -1)
+    else:
+        out = 64 * q + 32 * (t >> 1) + j
+        col = torch.where(out < n, out, -1)
+    return col.reshape(-1)
+
+
+def pack8(w: Tensor, gated: bool = False) -> Weight8:
+    """The weight ``w`` (k, n) float32 or bf16 of a projection ``x @ w``, rounded to 8 bits in blocks
+    along k (as `quantize8` rounds its columns) and laid out for `matmul8`; with ``gated`` its columns
+    are value | gate and it goes to `swiglu8`. Done once, when a model is loaded."""
+    if w.dim() != 2 or w.dtype not in _FLOATS:
+        raise ValueError(f"pack8: the weight must be (k, n) float32 or bf16, got {w.dtype} {tuple(w.shape)}")
+    k, n = w.shape
+    if gated and n % 2:
+        raise ValueError(f"pack8: a gated weight has value and gate columns, got {n}")
+    n = n // 2 if gated else n
+    for size in (k, n):
+        if not 1 <= size <= _lib.ROWS8_WIDTH_MAX:
+            raise ValueError(f"pack8: a weight of {tuple(w.shape)} (each axis 1 to {_lib.ROWS8_WIDTH_MAX})")
+    K._device_of(w)
+    w = w.detach()
+    col = _packed_rows(n, gated).to(w.device)
+    rows = w.t().index_select(0, col.clamp(min=0)).masked_fill_((col < 0).unsqueeze(1), 0.0)
+    q = quantize8(rows)
+    steps = q.scales.shape[0]
+    # (tile, row, step, plane, lane group, byte) -> (tile, step, plane, lane = group and row, byte)
+    v = q.values.view(torch.uint8).view(-1, 16, steps, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous()
+    return Weight8(v.view(-1, steps, 2, 64, 16).view(torch.float8_e4m3fn), q.scales, k, n, gated)
+
+
+def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
+    """The args struct of a product with its rows, weight and bias filled in, and what it keeps alive."""
+    if not isinstance(w, Weight8):
+        raise ValueError(f"{what}: the weight must be a Weight8 (pack8)")
+    is8 = isinstance(x, Rows8)
+    if not is8:
+        _check_float_rows(x, what)
+    lead, width = tuple(x.shape[:-1]), x.shape[-1]
+    if width != w.k:
+        raise ValueError(f"{what}: rows of {width} for a weight of {w.shape}")
+    dev = K._device_of(x.values if is8 else x, w.values, w.scales, bias)
+    _refuse_gradient(what, None if is8 else x, bias)
+    columns = w.shape[1]
+    if bias is not None:
+        if tuple(bias.shape) != (columns,):
+            raise ValueError(f"{what}: bias must be ({columns},), got {tuple(bias.shape)}")
+        bias = bias.detach()
+        if bias.dtype != torch.float32 or not bias.is_contiguous():
+            bias = bias.float().contiguous()
+    rows = _count(lead)
+    _check_sizes(what, rows, width)
+    if not is8 and rows > _lib.MATMUL8_FLOAT_ROWS:
+        x, is8 = quantize8(x), True
+    a = _lib.Matmul8Args()
+    a.struct_size = ctypes.sizeof(_lib.Matmul8Args)
+    a.k, a.n, a.gated, a.rows = w.k, w.n, int(w.gated), rows
+    if is8:
+        _check_rows8(x, what)
+        a.x_dtype, a.x, a.x_scales = _lib.DTYPE_ROWS8, x.values.data_ptr(), x.scales.data_ptr()
+    else:
+        x = _row_view(x)
+        a.x_dtype, a.x, a.ldx = _lib.dtype_code(x.dtype), x.data_ptr(), _row_stride(x)
+    a.w, a.w_scales, a.bias = w.values.data_ptr(), w.scales.data_ptr(), _lib.ptr(bias)
+    return a, dev, lead, rows, (x, bias)
+
+
+def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[str] = None,
+            residual: Optional[Tensor] = None) -> Tensor:
+    """``act(x @ w + bias) + residual`` in bf16, (..., n): ``x`` (..., k) is `Rows8`, or float32 or bf16
+    rows, which are rounded to 8 bits first (`quantize8`; up to 16 rows in the same launch); ``bias``
+    (n,) float32 or bf16; ``activation`` None, "silu", "gelu" (with erf) or "relu"; ``residual``
+    (..., n) bf16, such as a bf16 model's stream. All but the operands in 8 bits is float32 up to the
+    one rounding of the result. A row with a NaN or an infinity comes out NaN."""
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"matmul8: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    a, dev, lead, rows, keep = _operands(x, w, bias, "matmul8")
+    if w.gated:
+        raise ValueError("matmul8: a gated weight goes to swiglu8")
+    a.activation = ACTIVATIONS[activation]
+    if residual is not None:
+        if residual.dtype != torch.bfloat16 or tuple(residual.shape) != (*lead, w.n):
+            raise ValueError(f"matmul8: residual must be bf16 {(*lead, w.n)}, got {residual.dtype} "
+                             f"{tuple(residual.shape)}")
+        K._device_of(w.values, residual)
+        _refuse_gradient("matmul8", residual)
+        residual = _row_view(residual)
+        a.residual, a.ldres = residual.data_ptr(), _row_stride(residual)
+    y = K.empty(*lead, w.n, device=dev, dtype=torch.bfloat16)
+    a.y = y.data_ptr()
+    _lib.launch(_lib.load().m3s_matmul8, a, dev, "m3s_matmul8")
+    return y
+
+
+def swiglu8(x, w: Weight8, bias: Optional[Tensor] = None) -> Rows8:
+    """``value * silu(gate)`` of ``value | gate = x @ w + bias`` in 8 bits (..., n), in float32 up to that
+    rounding: the gated MLP's first product on a weight packed with ``gated=True``. ``x`` and ``bias``
+    (2 n,) as in `matmul8`."""
+    a, dev, lead, rows, keep = _operands(x, w, bias, "swiglu8")
+    if not w.gated:
+        raise ValueError("swiglu8: the weight must be packed with gated=True")
+    out = _new_rows8(lead, rows, w.n, dev)
+    a.y_values, a.y_scales = out.values.data_ptr(), out.scales.data_ptr()
+    _lib.launch(_lib.load().m3s_matmul8, a, dev, "m3s_matmul8")
+    return out
