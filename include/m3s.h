@@ -760,7 +760,7 @@ typedef struct m3s_rows8_values_args {
 int32_t m3s_rows8_values(const m3s_rows8_values_args* args, void* stream);
 
 /* The projections of the LM (layer.py:233, 256; model.py:125-140, 231) on 8-bit rows and weights:
- * y (rows, n) bf16 = act(x w + bias) + residual, dense. Gated: w has 2 n columns, value | gate, and
+ * y (rows, n) bf16 = act(x w + bias) + residual. Gated: w has 2 n columns, value | gate, and
  * value silu(gate) goes out as rows in 8 bits. x in 8 bits, or up to M3S_MATMUL8_FLOAT_ROWS rows in
  * bf16 or float32, rounded to 8 bits on the way.
  * w is packed: for every 16-row tile of its outputs and every 128 k, two planes (k 0-63, 64-127) of
@@ -785,6 +785,7 @@ typedef struct m3s_matmul8_args {
   const void* residual; /* (rows, n) bf16, or NULL; not with a gate */
   int64_t ldres;
   void* y;              /* out (rows, n) bf16, or NULL with a gate */
+  int64_t ldy;          /* elements from one row of y to the next, at least n */
   void* y_values;       /* gated: out (rows, n rounded up to 128) */
   void* y_scales;
 } m3s_matmul8_args;

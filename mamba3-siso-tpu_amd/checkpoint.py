@@ -36,6 +36,7 @@ _NP_FLOAT = {torch.float32: np.float32, torch.float64: np.float64, torch.float16
 def _named_leaves(params: M.LMParams) -> list:
     """``(name, tensor)`` for every present leaf, in tree order (``checkpoint.py:44-66``
     names: attribute names and list indices joined by dots)."""
+    M.refuse_packed(params)
     out = [("embed", params.embed)]
     for i, b in enumerate(params.blocks):
         out.append((f"blocks.{i}.norm_gain", b.norm_gain))

@@ -306,6 +306,9 @@ def lm_state_dict(params, cfg) -> dict:
     """`model.LMParams` -> a released-format state dict of float32 numpy arrays; the
     inverse of `load_lm_state_dict`. With a tied head ``lm_head.weight`` is the
     embedding, as upstream stores one shared tensor under both names."""
+    from .model import refuse_packed
+
+    refuse_packed(params)
     sd: dict = {}
     for path, key, tr in _model_leaves(cfg):
         arr = _f32(_get_path_indexed(params, path))

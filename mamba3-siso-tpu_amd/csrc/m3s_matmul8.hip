@@ -43,7 +43,7 @@ struct M8Params {
   bf16* y;
   uint8_t* yv;             // gated: (M, op) values and (op / 128, M, 4) scales
   uint8_t* ys;
-  int64_t M, ldx, ldr;
+  int64_t M, ldx, ldr, ldy;
   int K, KB, N, NP, act, vec;   // N: outputs (half the weight's columns with a gate); NP: packed rows
   int tiles_m, tiles_n;
 };
@@ -66,7 +66,7 @@ __device__ __forceinline__ uint32_t max_lanes16(uint32_t u) {   // over the four
 // 8 neighbouring outputs n .. n + 7 of row m
 __device__ __forceinline__ void finish8(const M8Params& p, int64_t m, int n, float (&v)[8]) {
   if (n >= p.N) return;
-  const bool whole = p.vec & 1;   // N % 8 == 0 and every pointer and stride allows 16 bytes
+  const bool whole = (p.vec & 1) && n + 8 <= p.N;   // pointers and strides allow 16 bytes
   if (p.bias) {
     if (whole) {
       const f32x4 a = *reinterpret_cast<const f32x4*>(p.bias + n), b = *reinterpret_cast<const f32x4*>(p.bias + n + 4);
@@ -94,7 +94,7 @@ __device__ __forceinline__ void finish8(const M8Params& p, int64_t m, int n, flo
         if (n + i < p.N) v[i] += (float)rr[i];
     }
   }
-  bf16* yr = p.y + m * p.N + n;
+  bf16* yr = p.y + m * p.ldy + n;
   if (whole) {
     bf16x8 o;
 #pragma unroll
@@ -434,18 +434,19 @@ extern "C" int32_t m3s_matmul8(const m3s_matmul8_args* a, void* stream) {
               "m3s_matmul8: 8-bit values must be 16-byte aligned");
   M3S_REQUIRE(!floats || a->ldx >= a->k, "m3s_matmul8: ldx is too short");
   M3S_REQUIRE(!a->residual || a->ldres >= a->n, "m3s_matmul8: ldres is too short");
+  M3S_REQUIRE(a->gated || a->ldy >= a->n, "m3s_matmul8: ldy is too short");
   M8Params p{};
   p.x = a->x; p.xs = static_cast<const uint8_t*>(a->x_scales);
   p.w = static_cast<const uint8_t*>(a->w); p.ws = static_cast<const uint8_t*>(a->w_scales);
   p.bias = a->bias; p.residual = static_cast<const bf16*>(a->residual); p.y = static_cast<bf16*>(a->y);
   p.yv = static_cast<uint8_t*>(a->y_values); p.ys = static_cast<uint8_t*>(a->y_scales);
-  p.M = a->rows; p.ldx = a->ldx; p.ldr = a->ldres;
+  p.M = a->rows; p.ldx = a->ldx; p.ldr = a->ldres; p.ldy = a->ldy;
   p.K = a->k; p.KB = (int)(padded8(a->k) / kStep8); p.N = a->n; p.act = a->activation;
   p.NP = (int)(a->gated ? 2 * padded8(a->n) : ((int64_t)a->n + 63) / 64 * 64);
   // scales are read through 32-bit offsets, and a launch holds at most 2^31 workgroups' tiles
   M3S_REQUIRE((int64_t)p.KB * p.M * 4 < (1ll << 31) && (int64_t)p.KB * p.NP * 4 < (1ll << 31),
               "m3s_matmul8: an operand's scales span 2 GiB or more");
-  const bool whole = p.N % 8 == 0 && aligned16(p.y) && (!p.bias || aligned16(p.bias)) &&
+  const bool whole = p.ldy % 8 == 0 && aligned16(p.y) && (!p.bias || aligned16(p.bias)) &&
                      (!p.residual || (aligned16(p.residual) && p.ldr % 8 == 0));
   const int xs = a->x_dtype == M3S_DTYPE_F32 ? 4 : 2;
   const bool xvec = floats && p.K % 8 == 0 && aligned16(p.x) && p.ldx % (16 / xs) == 0;

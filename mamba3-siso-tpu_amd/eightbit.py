@@ -25,7 +25,6 @@ import torch
 
 from . import _lib
 from . import kernels as K
-from . import layer as LY
 
 Tensor = torch.Tensor
 
@@ -81,16 +80,6 @@ class Weight8(NamedTuple):
 
 def _padded(n: int, to: int) -> int:
     return (n + to - 1) // to * to
-
-
-def _refuse_gradient(what: str, *tensors) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise ValueError(f"{what}: 8-bit operators take no gradient (detach the operands, or call "
-                                 "under torch.no_grad)")
-    if torch.jit.is_tracing() or LY.has_tangent(*tensors):
-        raise ValueError(f"{what}: 8-bit operators take no forward-mode tangent and no trace")
 
 
 def _check_rows8(x: Rows8, what: str) -> int:
@@ -149,7 +138,7 @@ def quantize8(x: Tensor) -> Rows8:
     block to the others. Rows may have any stride between them."""
     _check_float_rows(x, "quantize8")
     dev = K._device_of(x)
-    _refuse_gradient("quantize8", x)
+    K.refuse_gradient("quantize8", x)
     lead, width = tuple(x.shape[:-1]), x.shape[-1]
     rows = _count(lead)
     _check_sizes("quantize8", rows, width)
@@ -176,7 +165,7 @@ def rms_norm8(x: Tensor, gain: Tensor, eps: float, add: Optional[Tensor] = None)
     if add is not None and (add.dtype != torch.bfloat16 or add.shape != x.shape):
         raise ValueError(f"rms_norm8: add must be bf16 {tuple(x.shape)}, got {add.dtype} {tuple(add.shape)}")
     dev = K._device_of(x, gain, add)
-    _refuse_gradient("rms_norm8", x, gain, add)
+    K.refuse_gradient("rms_norm8", x, gain, add)
     gain = gain.detach()
     if gain.dtype != torch.float32 or not gain.is_contiguous():
         gain = gain.float().contiguous()
@@ -247,7 +236,7 @@ def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
     if width != w.k:
         raise ValueError(f"{what}: rows of {width} for a weight of {w.shape}")
     dev = K._device_of(x.values if is8 else x, w.values, w.scales, bias)
-    _refuse_gradient(what, None if is8 else x, bias)
+    K.refuse_gradient(what, None if is8 else x, bias)
     columns = w.shape[1]
     if bias is not None:
         if tuple(bias.shape) != (columns,):
@@ -290,11 +279,23 @@ def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[s
             raise ValueError(f"matmul8: residual must be bf16 {(*lead, w.n)}, got {residual.dtype} "
                              f"{tuple(residual.shape)}")
         K._device_of(w.values, residual)
-        _refuse_gradient("matmul8", residual)
+        K.refuse_gradient("matmul8", residual)
         residual = _row_view(residual)
         a.residual, a.ldres = residual.data_ptr(), _row_stride(residual)
     y = K.empty(*lead, w.n, device=dev, dtype=torch.bfloat16)
-    a.y = y.data_ptr()
+    a.y, a.ldy = y.data_ptr(), w.n
+    _lib.launch(_lib.load().m3s_matmul8, a, dev, "m3s_matmul8")
+    return y
+
+
+def matmul8_into(x, w: Weight8, stride: int) -> Tensor:
+    """`matmul8` without an epilogue into rows of ``stride`` (at least n) elements: a dense
+    (rows, stride) buffer whose first n columns are the product and whose others nothing writes."""
+    a, dev, _, rows, keep = _operands(x, w, None, "matmul8")
+    if w.gated or stride < w.n:
+        raise ValueError(f"matmul8: rows of {stride} for a product of {w.shape}")
+    y = K.empty(rows, stride, device=dev, dtype=torch.bfloat16)
+    a.y, a.ldy = y.data_ptr(), stride
     _lib.launch(_lib.load().m3s_matmul8, a, dev, "m3s_matmul8")
     return y
 

@@ -18,6 +18,7 @@ import math
 from typing import Any, NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as fwd_ad
 
 from . import _lib
 from . import layout as LY
@@ -108,6 +109,25 @@ def _device_of(*ts) -> torch.device:
         elif t.device != dev:
             raise ValueError(f"tensors on different devices: {dev} and {t.device}")
     return dev
+
+
+def has_tangent(*tensors) -> bool:
+    """Whether one of ``tensors`` (None passed over) carries a forward-mode tangent
+    (``torch.no_grad`` does not switch that mode off). Launches outside an autograd node would
+    drop it without a word; the nodes have no forward-mode rule and refuse it."""
+    return fwd_ad._current_level >= 0 and any(
+        t is not None and fwd_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
+def refuse_gradient(what: str, *tensors) -> None:
+    """``ValueError`` where autograd of either mode would follow a call that has no rule for it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{what}: 8-bit operators take no gradient (detach the operands, or call "
+                                 "under torch.no_grad)")
+    if torch.jit.is_tracing() or has_tangent(*tensors):
+        raise ValueError(f"{what}: 8-bit operators take no forward-mode tangent and no trace")
 
 
 def _f32c(t: Optional[Tensor]) -> Optional[Tensor]:

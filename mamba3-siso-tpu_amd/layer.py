@@ -35,12 +35,13 @@ import math
 from typing import Any, NamedTuple, Optional
 
 import torch
-import torch.autograd.forward_ad as fwd_ad
 import torch.nn.functional as F
 
+from . import eightbit as E8
 from . import kernels as K
 from . import layout as LY
 from . import scan_prep as SP
+from .kernels import has_tangent
 from .scan_prep import SISOState, heavy_tail
 from .siso import siso_segment
 
@@ -240,6 +241,19 @@ def weight_grad(a: Tensor, b: Tensor) -> Tensor:
     return torch.bmm(a3.transpose(1, 2), b3, out_dtype=torch.float32).sum(0)
 
 
+def _raw_scan(proj: Tensor, cfg: SISOConfig, bias: Tensor, b_norm_weight: Tensor, c_norm_weight: Tensor,
+              b_bias: Tensor, c_bias: Tensor, d_skip: Optional[Tensor]):
+    """The layer between its projections in raw mode (no gradient, no carried state): ``proj``
+    (B, L, d_in_proj) with any row stride -> `kernels.siso_forward_raw`'s outputs."""
+    z, x, b, c, dt_raw, a_raw, trap_raw, angles = split_in_proj(proj, cfg)
+    tile = LY.kernel_chunk(cfg.policy_name, cfg.chunk, cfg.d_state, cfg.headdim)
+    (k, q), _, angs = K.bcnorm_forward([b, c], [b_norm_weight, c_norm_weight], cfg.norm_eps,
+                                       theta=(angles, dt_raw, bias, tile))
+    return K.siso_forward_raw(q, k, x.permute(0, 2, 1, 3), dt_raw, a_raw, trap_raw, angs, bias, c_bias,
+                              b_bias, d_skip=d_skip, z=z.permute(0, 2, 1, 3), a_floor=cfg.a_floor,
+                              chunk=cfg.chunk, dtype_policy=cfg.policy_name)
+
+
 class _LayerFn(torch.autograd.Function):
     """``layer.py:201-262`` with state=None as one autograd node (see the module notes).
     Outputs: out (B, L, d_model), final ssm, final k, final v, final phi."""
@@ -273,14 +287,7 @@ class _LayerFn(torch.autograd.Function):
                and K.raw_forward_ok(cfg.policy_name, cfg.chunk, cfg.d_state, cfg.headdim,
                                     cfg.n_angles, seqlen, cfg.nheads))
         if raw:
-            tile = LY.kernel_chunk(cfg.policy_name, cfg.chunk, cfg.d_state, cfg.headdim)
-            (k, q), (rk, rq), angs = K.bcnorm_forward(
-                [b, c], [b_norm_weight, c_norm_weight], cfg.norm_eps,
-                theta=(angles, dt_raw, bias, tile))
-            outs = K.siso_forward_raw(q, k, x.permute(0, 2, 1, 3), dt_raw, a_raw, trap_raw, angs,
-                                      bias, c_bias, b_bias, d_skip=d_skip,
-                                      z=z.permute(0, 2, 1, 3), a_floor=cfg.a_floor,
-                                      chunk=cfg.chunk, dtype_policy=cfg.policy_name)
+            outs = _raw_scan(proj[..., :d], cfg, bias, b_norm_weight, c_norm_weight, b_bias, c_bias, d_skip)
             phi_final = outs[4]
         else:
             (k, q), (rk, rq) = K.bcnorm_forward([b, c], [b_norm_weight, c_norm_weight],
@@ -362,14 +369,6 @@ class _LayerFn(torch.autograd.Function):
                 None)
 
 
-def has_tangent(*tensors) -> bool:
-    """Whether one of ``tensors`` (None passed over) carries a forward-mode tangent
-    (``torch.no_grad`` does not switch that mode off). Launches outside an autograd node would
-    drop it without a word; the nodes have no forward-mode rule and refuse it."""
-    return fwd_ad._current_level >= 0 and any(
-        t is not None and fwd_ad.unpack_dual(t).tangent is not None for t in tensors)
-
-
 def _segment_fused_ok(params: SISOParams, u: Tensor, cfg: SISOConfig, state) -> bool:
     """Whether a segment with a carried state runs as `_segment_forward`: no gradient is taken,
     `_fused_ok` holds, the projection's own rows are 16-byte aligned, and the carry and the
@@ -399,19 +398,75 @@ def _segment_forward(params: SISOParams, u: Tensor, cfg: SISOConfig, state: SISO
     batch, seqlen, dm = u.shape
     m = batch * seqlen
     proj = (u.reshape(m, dm) @ params.in_proj.to(u.dtype)).view(batch, seqlen, cfg.d_in_proj)
+    y, state = _segment_scan(params, proj, cfg, state)
+    y2 = y.permute(0, 2, 1, 3).reshape(m, cfg.d_inner)
+    out = (y2 @ params.out_proj.to(u.dtype)).view(batch, seqlen, params.out_proj.shape[1])
+    return out, state
+
+
+def _segment_scan(params: SISOParams, proj: Tensor, cfg: SISOConfig, state: Optional[SISOState]):
+    """`_segment_forward` between the projections: ``(y (B, H, L, P), SISOState)``; ``state`` None
+    starts from zeros."""
     z, x, b, c, dt_raw, a_raw, trap_raw, angles = split_in_proj(proj, cfg)
     (k, q), _ = K.bcnorm_forward([b, c], [params.b_norm_weight, params.c_norm_weight], cfg.norm_eps)
     adt, gamma, scale, lam, dt, phi, phi_final = SP.prep_forward_launch(
         dt_raw, a_raw, trap_raw, angles, params.dt_bias.float().contiguous(),
-        state.phi.float().contiguous(), cfg.a_floor)
+        None if state is None else state.phi.float().contiguous(), cfg.a_floor)
+    seeds = {} if state is None else dict(seed_ssm=state.ssm, seed_k=state.k, seed_v=state.v,
+                                          seed_coef=dt[:, :, 0] * (1.0 - lam[:, :, 0]))
     y, fs, fk, fv = K.siso_forward(
         q, k, x.permute(0, 2, 1, 3), adt, gamma, scale, phi, params.c_bias, params.b_bias,
-        d_skip=params.d_skip, z=z.permute(0, 2, 1, 3), seed_ssm=state.ssm, seed_k=state.k,
-        seed_v=state.v, seed_coef=dt[:, :, 0] * (1.0 - lam[:, :, 0]), chunk=cfg.chunk,
+        d_skip=params.d_skip, z=z.permute(0, 2, 1, 3), **seeds, chunk=cfg.chunk,
         dtype_policy=cfg.policy_name)
-    y2 = y.permute(0, 2, 1, 3).reshape(m, cfg.d_inner)
-    out = (y2 @ params.out_proj.to(u.dtype)).view(batch, seqlen, params.out_proj.shape[1])
-    return out, SISOState(ssm=fs, k=fk, v=fv, phi=phi_final)
+    return y, SISOState(ssm=fs, k=fk, v=fv, phi=phi_final)
+
+
+def is_eight_bit(params: SISOParams) -> bool:
+    """Whether the layer's projections are packed in 8 bits (`eightbit.pack8`)."""
+    return isinstance(params.in_proj, E8.Weight8)
+
+
+def _check_eight(params: SISOParams, cfg: SISOConfig) -> None:
+    if (not isinstance(params.out_proj, E8.Weight8) or not is_eight_bit(params)
+            or params.in_proj.shape != (cfg.d_model, cfg.d_in_proj)
+            or params.out_proj.shape != (cfg.d_inner, cfg.d_model)):
+        raise ValueError(f"in_proj and out_proj must both be packed, {(cfg.d_model, cfg.d_in_proj)} and "
+                         f"{(cfg.d_inner, cfg.d_model)}")
+    if LY.policy(cfg.policy_name).matmul != torch.bfloat16:
+        raise ValueError(f"projections in 8 bits run under the bf16 policy, not {cfg.policy_name}")
+    K.refuse_gradient("a layer in 8 bits", *(t for t in params if isinstance(t, Tensor)))
+
+
+def _layer_eight(params: SISOParams, u, cfg: SISOConfig, state: Optional[SISOState],
+                 residual: Optional[Tensor] = None):
+    """`mamba3_siso_layer` with both projections in 8 bits: ``u`` (B, L, d_model) is `eightbit.Rows8`,
+    or rows that are rounded here. Scan, norms and carried state are those of the bf16 layer.
+    ``residual`` (bf16) is added to the output."""
+    _check_eight(params, cfg)
+    if len(u.shape) != 3:
+        raise ValueError(f"u must be (B, L, d_model), got {tuple(u.shape)}")
+    batch, seqlen = u.shape[:2]
+    d, vec = cfg.d_in_proj, 8
+    if cfg.headdim % vec or cfg.d_state % vec or cfg.d_state // vec > 64:
+        raise ValueError(f"no layer in 8 bits for headdim {cfg.headdim}, d_state {cfg.d_state}")
+    if state is not None:
+        K.refuse_gradient("a layer in 8 bits", *state)
+        b, h, n = batch, cfg.nheads, cfg.d_state
+        shapes = ((b, h, cfg.headdim, n), (b, h, n), (b, h, cfg.headdim), (b, h, cfg.n_angles))
+        if any(tuple(t.shape) != s or t.device != params.in_proj.device for t, s in zip(state, shapes)):
+            raise ValueError(f"state must be {shapes} on the layer's device")
+    # rows on 16-byte boundaries, as the scan reads its slices in place
+    proj = E8.matmul8_into(u, params.in_proj, (d + vec - 1) // vec * vec).view(batch, seqlen, -1)[..., :d]
+    bias = params.dt_bias.float().contiguous()
+    if state is None and K.raw_forward_ok(cfg.policy_name, cfg.chunk, cfg.d_state, cfg.headdim,
+                                          cfg.n_angles, seqlen, cfg.nheads):
+        y, fs, fk, fv, phi = _raw_scan(proj, cfg, bias, params.b_norm_weight, params.c_norm_weight,
+                                       params.b_bias, params.c_bias, params.d_skip)
+        st = SISOState(ssm=fs, k=fk, v=fv, phi=phi)
+    else:
+        y, st = _segment_scan(params, proj, cfg, state)
+    y2 = y.permute(0, 2, 1, 3).reshape(batch, seqlen, cfg.d_inner)
+    return E8.matmul8(y2, params.out_proj, residual=residual), st
 
 
 def mamba3_siso_layer(params: SISOParams, u: Tensor, cfg: SISOConfig,
@@ -428,8 +483,13 @@ def mamba3_siso_layer(params: SISOParams, u: Tensor, cfg: SISOConfig,
     (``None`` or True) the whole preprocess then runs inside the BCNorm and scan launches
     (`kernels.siso_forward_raw`) where a raw-mode kernel exists for the shape. With
     gradients ``None`` (the default) materialises phi, whose backward scan is faster, and
-    True keeps it compact. False always materialises phi and the row scalars first."""
+    True keeps it compact. False always materialises phi and the row scalars first.
+
+    With projections packed in 8 bits (`eightbit.pack8`; serving, no gradient) ``u`` may be
+    `eightbit.Rows8` and ``out`` is bf16."""
     cfg.require_kernels()
+    if is_eight_bit(params):
+        return _layer_eight(params, u, cfg, state)
     if _fused_ok(u, cfg, state):
         out, fs, fk, fv, phi_final = _LayerFn.apply(
             u, params.in_proj, params.out_proj, params.dt_bias, params.b_norm_weight,
@@ -461,14 +521,24 @@ def _decode_fused_ok(u: Tensor, cfg: SISOConfig) -> bool:
 
 
 def mamba3_siso_decode_step(params: SISOParams, u: Tensor, cfg: SISOConfig,
-                            state: SISOState):
+                            state: SISOState, residual: Optional[Tensor] = None):
     """One token through the layer (``model.py:266-289`` without block norm/residual):
     ``u`` ``(B, d_model)`` -> ``(out (B, d_model), next_state)``. The state is updated in
     place by the decode kernel (the reference donates it). When ``u`` is in the policy's
     operand dtype, everything between the two projections (BCNorm, dt / lambda / a, the
-    state update and readout) is one ``m3s_decode_layer`` launch on the projection rows."""
+    state update and readout) is one ``m3s_decode_layer`` launch on the projection rows.
+    With projections in 8 bits ``u`` may be `eightbit.Rows8`, and a bf16 ``residual`` is added to
+    the output."""
     cfg.require_kernels()
-    proj = K.matmul(u, params.in_proj.to(u.dtype))
+    eight = is_eight_bit(params)
+    if eight:
+        _check_eight(params, cfg)
+        K.refuse_gradient("a layer in 8 bits", *state)
+        proj = u = E8.matmul8(u, params.in_proj)
+    elif residual is not None:
+        raise ValueError("a residual goes with projections in 8 bits")
+    else:
+        proj = K.matmul(u, params.in_proj.to(u.dtype))
     if _decode_fused_ok(u, cfg):
         y, st = K.decode_layer_step(
             proj, state, nheads=cfg.nheads, headdim=cfg.headdim, state_dim=cfg.d_state,
@@ -486,5 +556,7 @@ def mamba3_siso_decode_step(params: SISOParams, u: Tensor, cfg: SISOConfig,
         y, st = K.decode_step(c, b, x[:, 0], a * dt, dt, lam, angles[:, 0], params.c_bias,
                               params.b_bias, state, d_skip=params.d_skip, z=z[:, 0],
                               dtype_policy=cfg.policy_name)
-    out = K.matmul(y.reshape(u.shape[0], cfg.d_inner).to(u.dtype), params.out_proj.to(u.dtype))
-    return out, st
+    y = y.reshape(u.shape[0], cfg.d_inner).to(u.dtype)
+    if eight:
+        return E8.matmul8(y, params.out_proj, residual=residual), st
+    return K.matmul(y, params.out_proj.to(u.dtype)), st

@@ -28,6 +28,7 @@ import torch
 import torch.nn.functional as F
 
 from . import _lib
+from . import eightbit as E8
 from . import kernels as K
 from . import layer as LY
 from . import layout as L
@@ -197,8 +198,16 @@ def lm_template(cfg: LMConfig) -> LMParams:
                     None if cfg.tie_head else e(d, cfg.vocab_size))
 
 
+def refuse_packed(params: LMParams) -> None:
+    """Packed weights are no tensors of the model's shapes: they are not cast, moved, trained or stored."""
+    if _is_eight_bit(params):
+        raise ValueError("weights in 8 bits are for serving: cast, move, train or store the weights they "
+                         "were packed from")
+
+
 def lm_map(fn, params: LMParams) -> LMParams:
     """Apply ``fn`` to every tensor of the tree, keeping its structure (``None`` stays)."""
+    refuse_packed(params)
     f = lambda t: None if t is None else fn(t)  # noqa: E731
     blocks = [BlockParams(f(b.norm_gain), LY.SISOParams(*(f(t) for t in b.siso)),
                           f(b.mlp_norm_gain),
@@ -214,6 +223,7 @@ def lm_to(params: LMParams, device=None, dtype=None) -> LMParams:
 def lm_leaves(params: LMParams) -> list:
     """The tree's tensors in a fixed order (embed, per block: norm, the eight SISO fields,
     MLP norm, fc1, fc2; final norm, head), ``None`` entries skipped."""
+    refuse_packed(params)
     out = [params.embed]
     for b in params.blocks:
         out.append(b.norm_gain)
@@ -231,7 +241,9 @@ def decode_params(params: LMParams, cfg: LMConfig) -> LMParams:
     once to the policy's operand dtype. Every product casts them to that dtype anyway, so
     results are bit-identical; a per-token step then reads half the weight bytes and
     launches no casts. The embedding (which sets the residual stream's dtype), the head
-    and the vectors are unchanged."""
+    and the vectors are unchanged, and so are weights in 8 bits (`eight_bit_params`)."""
+    if _is_eight_bit(params):
+        return params
     dt = _mm_dtype(cfg)
     blocks = [b._replace(siso=b.siso._replace(in_proj=b.siso.in_proj.detach().to(dt),
                                               out_proj=b.siso.out_proj.detach().to(dt)),
@@ -239,6 +251,33 @@ def decode_params(params: LMParams, cfg: LMConfig) -> LMParams:
                                                                   b.mlp.fc2.detach().to(dt)))
               for b in params.blocks]
     return params._replace(blocks=blocks)
+
+
+def eight_bit_params(params: LMParams, cfg: LMConfig) -> LMParams:
+    """``params`` on the device with each block's projection matrices (in_proj, out_proj, fc1, fc2) packed
+    in 8 bits (`eightbit.pack8`), for serving: `lm_forward`, `lm_decode_step`, `train.DecodeGraph` and
+    `train.generate` take the result and run every projection on the matrix cores' 8-bit form, its rows
+    rounded on the way (the block norms and the MLP's gate leave them in 8 bits). Half the bf16
+    weights' memory and traffic. Embedding, head, norms, scan and states stay as they are. Needs the
+    bf16 policy; no gradient."""
+    if _mm_dtype(cfg) != torch.bfloat16:
+        raise ValueError(f"weights in 8 bits run under the bf16 policy, not {cfg.siso.policy_name}")
+    blocks = [b._replace(siso=b.siso._replace(in_proj=E8.pack8(b.siso.in_proj),
+                                              out_proj=E8.pack8(b.siso.out_proj)),
+                         mlp=None if b.mlp is None else MLPParams(E8.pack8(b.mlp.fc1, gated=True),
+                                                                  E8.pack8(b.mlp.fc2)))
+              for b in params.blocks]
+    return LMParams(params.embed.detach(), [_detach_block(b) for b in blocks], params.final_norm.detach(),
+                    None if params.head is None else params.head.detach())
+
+
+def _detach_block(b: BlockParams) -> BlockParams:
+    f = lambda t: t.detach() if isinstance(t, Tensor) else t  # noqa: E731
+    return BlockParams(f(b.norm_gain), LY.SISOParams(*(f(t) for t in b.siso)), f(b.mlp_norm_gain), b.mlp)
+
+
+def _is_eight_bit(params: LMParams) -> bool:
+    return bool(params.blocks) and LY.is_eight_bit(params.blocks[0].siso)
 
 
 def _head(params: LMParams, cfg: LMConfig) -> Tensor:
@@ -348,6 +387,11 @@ def lm_forward(params: LMParams, tokens: Tensor, cfg: LMConfig, interpret: Any =
     returned as well: ``(logits, states)`` -- the segmented prefill of generation.
     ``interpret`` and ``device_kind`` are accepted for signature compatibility."""
     dt = _mm_dtype(cfg)
+    if _is_eight_bit(params):
+        layer = lambda p, h, i, r: LY._layer_eight(  # noqa: E731
+            p, h, cfg.siso, None if states is None else states[i], r)
+        logits, new_states = _forward_eight(params, tokens, cfg, layer)
+        return (logits, new_states) if states is not None else logits
     x = _embed(params.embed, tokens)
     new_states = []
     eps = cfg.siso.norm_eps
@@ -366,6 +410,29 @@ def lm_forward(params: LMParams, tokens: Tensor, cfg: LMConfig, interpret: Any =
         x, h = _add_norm(x, y, nxt, eps, dt)
     logits = _head_logits(h, params, cfg) if blocks else _logits(x, params, cfg)
     return (logits, new_states) if states is not None else logits
+
+
+def _forward_eight(params: LMParams, tokens: Tensor, cfg: LMConfig, layer):
+    """Logits and states of a model in 8 bits; ``layer(siso params, rows, index, residual)`` is the mixer
+    of a prompt or of one token. A bf16 stream takes each block's output in the product's epilogue; a
+    float32 stream (float32 embeddings) in the norm after it."""
+    cfg.siso.require_kernels()
+    x = _embed(params.embed, tokens)
+    K.refuse_gradient("a model in 8 bits", x)
+    eps, wide, states, y = cfg.siso.norm_eps, x.dtype != torch.bfloat16, [], None
+
+    for i, b in enumerate(params.blocks):
+        x, h = E8.rms_norm8(x, b.norm_gain, eps, add=y)
+        out, st = layer(b.siso, h, i, None if wide else x)
+        states.append(st)
+        y, x = (out, x) if wide else (None, out)
+        if b.mlp is not None:
+            x, h = E8.rms_norm8(x, b.mlp_norm_gain, eps, add=y)
+            out = E8.matmul8(E8.swiglu8(h, b.mlp.fc1), b.mlp.fc2, residual=None if wide else x)
+            y, x = (out, x) if wide else (None, out)
+    dt = _mm_dtype(cfg)
+    h = _norm(x, params.final_norm, eps, dt) if y is None else _add_norm(x, y, params.final_norm, eps, dt)[1]
+    return _head_logits(h, params, cfg), states
 
 
 def lm_loss(params: LMParams, xs: Tensor, ys: Tensor, cfg: LMConfig) -> Tensor:
@@ -487,6 +554,9 @@ def lm_decode_step(params: LMParams, token: Tensor, states: list, cfg: LMConfig,
     dt = _mm_dtype(cfg)
     c = cfg.siso
     eps = c.norm_eps
+    if _is_eight_bit(params):
+        return _forward_eight(params, token, cfg, lambda p, h, i, r: LY.mamba3_siso_decode_step(
+            p, h, c, states[i], residual=r))
     x = _embed(params.embed, token)
     if token.dim() == 1 and _decode_fused_ok(params, x, cfg):
         return _decode_step_fused(params, x, states, cfg)

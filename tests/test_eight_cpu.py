@@ -102,7 +102,9 @@ def test_matmul8_arguments_are_checked_without_a_launch(lib):
     a.w, a.gated, a.y_values, a.y_scales, a.y = 0x3000, 0, None, None, 0x5000
     a.residual, a.ldres = 0x7000, 47
     refused(lib, h.m3s_matmul8, a, b"ldres")
-    a.residual, a.x_dtype, a.ldx = None, lib.DTYPE_F32, 63
+    a.residual, a.ldy = None, 47
+    refused(lib, h.m3s_matmul8, a, b"ldy")
+    a.ldy, a.x_dtype, a.ldx = 48, lib.DTYPE_F32, 63
     a.rows = 4
     refused(lib, h.m3s_matmul8, a, b"ldx")
     # steps x rows x 4 bytes of scales behind 32-bit offsets
@@ -142,3 +144,10 @@ def test_nothing_runs_on_the_cpu(T):
 def test_exports(m3):
     for name in ("Rows8", "Weight8", "quantize8", "rms_norm8", "pack8", "matmul8", "swiglu8"):
         assert getattr(m3, name) is getattr(m3.eightbit, name)
+
+
+def test_raw_mode_is_not_for_sub_heads(m3):
+    """A head width without a scan kernel of its own runs as sub-heads, which have no raw mode."""
+    for chunk, n, p in ((64, 64, 128), (128, 128, 128)):
+        assert m3.layout.kernel_headdim("bf16", chunk, n, p) == 64
+        assert not m3.kernels.raw_forward_ok("bf16", chunk, n, p, n // 4, 128, 2)
