@@ -720,8 +720,8 @@ int32_t m3s_distill_bwd(const m3s_distill_args* args, void* stream);
  * reference. e4m3 values in blocks of 32 along a row, each with a scale 2^e, e the smallest integer
  * >= -126 with the block's largest finite magnitude times 2^-e at most 448; a value is rounded to
  * nearest (ties to even), and an entry that is not finite becomes NaN. values is (rows, kp) bytes,
- * kp the width rounded up to 128 and zeros behind the width; scales (kp / 128, rows, 4) bytes of
- * e + 127. values 16-byte aligned. */
+ * kp the width rounded up to 128 and zeros behind the width; scales (kp / 32, mp) bytes of
+ * e + 127, mp the rows rounded up to 16. values 16-byte aligned, scales 4-byte. */
 #define M3S_DTYPE_ROWS8 2              /* of m3s_matmul8_args.x_dtype alone */
 #define M3S_ROWS8_MAX 16777215         /* rows: 2^24 - 1 */
 #define M3S_ROWS8_WIDTH_MAX 1048576    /* width: 2^20; with a norm 16384 */
@@ -743,7 +743,7 @@ typedef struct m3s_rows8_args {
   const float* gain;    /* (width), or NULL: no norm */
   void* sum;            /* out (rows, width) dense, iff add */
   void* values;         /* out (rows, kp) */
-  void* scales;         /* out (kp / 128, rows, 4) */
+  void* scales;         /* out (kp / 32, mp) */
 } m3s_rows8_args;
 int32_t m3s_rows8(const m3s_rows8_args* args, void* stream);
 
@@ -764,8 +764,9 @@ int32_t m3s_rows8_values(const m3s_rows8_values_args* args, void* stream);
  * value silu(gate) goes out as rows in 8 bits. x in 8 bits, or up to M3S_MATMUL8_FLOAT_ROWS rows in
  * bf16 or float32, rounded to 8 bits on the way.
  * w is packed: for every 16-row tile of its outputs and every 128 k, two planes (k 0-63, 64-127) of
- * 64 lanes' 16 bytes, lane 16 g + r holding row r's k 16 g .. 16 g + 15 of the plane; w_scales
- * (kp / 128, packed rows, 4). Packed row 64 q + 16 t + 4 g + i is output 64 q + 32 (t >> 1) + 8 g +
+ * 64 lanes' 16 bytes, lane 16 g + r holding row r's k 16 g .. 16 g + 15 of the plane; w_scales a
+ * dword for every 128 k, group of four tiles and lane 16 g + r: the tiles' scales of row r's block g.
+ * Packed row 64 q + 16 t + 4 g + i is output 64 q + 32 (t >> 1) + 8 g +
  * 4 (t & 1) + i, n rounded up to 64 of them; gated, it is output 32 q + 8 g + 4 (t & 1) + i of value
  * (t < 2) or gate, with n rounded up to 128. Rows behind n are zeros. */
 enum { M3S_ACT_NONE = 0, M3S_ACT_SILU = 1, M3S_ACT_GELU = 2, M3S_ACT_RELU = 3 };

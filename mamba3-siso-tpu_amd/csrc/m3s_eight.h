@@ -11,9 +11,9 @@
 // NaN, as they would be in floating point, and its block's other values keep their scale.
 //
 // Layout: values (rows, kp) bytes with kp the width rounded up to 128 (zeros behind the width), the
-// K of one matrix instruction, and scales (kp / 128, rows, 4) bytes: the four scales that one row
-// brings to one instruction lie together, and the rows of a 16-row tile behind each other, so a
-// wave's scales are one 64-byte piece.
+// K of one matrix instruction, and scales (kp / 32, mp) bytes with mp the rows rounded up to 16: a
+// block's scales of four rows are one dword, which the products' lanes read at once and pick
+// their byte of by the instruction's own selector. Nothing writes the scales behind the last row.
 #pragma once
 
 #include "m3s_common.h"
@@ -23,6 +23,7 @@ namespace m3s {
 constexpr int kBlock8 = 32;    // values to a scale
 constexpr int kStep8 = 128;    // K of one v_mfma_scale_f32_16x16x128_f8f6f4
 
+__host__ __device__ inline int64_t padded16(int64_t rows) { return (rows + 15) & ~(int64_t)15; }
 inline int64_t padded8(int64_t width) { return (width + kStep8 - 1) / kStep8 * kStep8; }
 
 typedef int i32x2_ __attribute__((ext_vector_type(2)));

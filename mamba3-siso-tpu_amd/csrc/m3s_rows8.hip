@@ -27,7 +27,7 @@ struct R8Params {
   void* sum;
   uint8_t* values;
   uint8_t* scales;
-  int64_t M, ldx, lda;
+  int64_t M, mp, ldx, lda;
   int D, kp;
   float eps;
 };
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kR8Threads) rows8_kernel(const R8Params p) {
                       pack4(v[k][4], v[k][5], v[k][6], v[k][7], down)};
     *reinterpret_cast<i32x2_*>(p.values + r * p.kp + c) = q;
     if ((lane & 3) == 0)
-      p.scales[((int64_t)(c / kStep8) * p.M + r) * 4 + (c % kStep8) / kBlock8] = (uint8_t)byte;
+      p.scales[(int64_t)(c / kBlock8) * p.mp + r] = (uint8_t)byte;
   }
 }
 
@@ -172,7 +172,7 @@ __global__ void __launch_bounds__(kR8Threads) rows8_values_kernel(const uint8_t*
   const int c = 8 * (threadIdx.x & 63) + (int)blockIdx.y * kR8Pass;
   if (r >= M || c >= D) return;
   const i32x2_ q = *reinterpret_cast<const i32x2_*>(values + r * kp + c);
-  const float up = scale_up(scales[((int64_t)(c / kStep8) * M + r) * 4 + (c % kStep8) / kBlock8]);
+  const float up = scale_up(scales[(int64_t)(c / kBlock8) * padded16(M) + r]);
   float v[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -237,7 +237,7 @@ extern "C" int32_t m3s_rows8(const m3s_rows8_args* a, void* stream) {
   M3S_REQUIRE(a->ldx >= a->width && (!a->add || a->ldadd >= a->width), "m3s_rows8: a row stride is too short");
   M3S_REQUIRE((uintptr_t)a->values % 16 == 0, "m3s_rows8: values must be 16-byte aligned");
   R8Params p{a->x, a->add, a->gain, a->sum, static_cast<uint8_t*>(a->values),
-             static_cast<uint8_t*>(a->scales), a->rows, a->ldx, a->ldadd, a->width,
+             static_cast<uint8_t*>(a->scales), a->rows, padded16(a->rows), a->ldx, a->ldadd, a->width,
              (int)padded8(a->width), a->eps};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!a->gain) dispatch_rows8<false, false>(a, p, s);

@@ -36,8 +36,9 @@ _FLOATS = (torch.float32, torch.bfloat16)
 
 class Rows8(NamedTuple):
     """Rows in 8 bits: ``values`` (rows, kp) float8_e4m3fn, kp the ``width`` rounded up to 128 (zeros
-    behind the width); ``scales`` (kp / 128, rows, 4) float8_e8m0fnu, the scales of a row's four
-    blocks of each 128; ``lead``, the shape of the leading axes, whose product is ``rows``."""
+    behind the width); ``scales`` (kp / 32, mp) float8_e8m0fnu, a column for each row, mp the rows
+    rounded up to 16 (nothing behind the last row is written or used); ``lead``, the shape of the
+    leading axes, whose product is ``rows``."""
 
     values: Tensor
     scales: Tensor
@@ -60,7 +61,7 @@ class Rows8(NamedTuple):
 
 class Weight8(NamedTuple):
     """A projection's weight (k, n) packed for the products (`pack8`): ``values``
-    (tiles, steps, 2, 64, 16) float8_e4m3fn and ``scales`` (steps, 16 tiles, 4) float8_e8m0fnu.
+    (tiles, steps, 2, 64, 16) float8_e4m3fn and ``scales`` (steps, tiles / 4, 64, 4) float8_e8m0fnu.
     ``gated``: its columns are value | gate, n of each."""
 
     values: Tensor
@@ -87,7 +88,7 @@ def _check_rows8(x: Rows8, what: str) -> int:
     for n in x.lead:
         rows *= n
     if (tuple(x.values.shape) != (rows, kp) or x.values.dtype != torch.float8_e4m3fn
-            or tuple(x.scales.shape) != (kp // STEP, rows, 4) or x.scales.dtype != torch.float8_e8m0fnu
+            or tuple(x.scales.shape) != (kp // BLOCK, _padded(rows, 16)) or x.scales.dtype != torch.float8_e8m0fnu
             or not x.values.is_contiguous() or not x.scales.is_contiguous()):
         raise ValueError(f"{what}: rows must be dense Rows8 of {rows} x {x.width}")
     return rows
@@ -96,7 +97,7 @@ def _check_rows8(x: Rows8, what: str) -> int:
 def _new_rows8(lead: tuple, rows: int, width: int, dev) -> Rows8:
     kp = _padded(width, STEP)
     return Rows8(K.empty(rows, kp, device=dev, dtype=torch.float8_e4m3fn),
-                 K.empty(kp // STEP, rows, 4, device=dev, dtype=torch.float8_e8m0fnu), width, lead)
+                 K.empty(kp // BLOCK, _padded(rows, 16), device=dev, dtype=torch.float8_e8m0fnu), width, lead)
 
 
 def _row_view(x: Tensor) -> Tensor:
@@ -219,10 +220,13 @@ def pack8(w: Tensor, gated: bool = False) -> Weight8:
     col = _packed_rows(n, gated).to(w.device)
     rows = w.t().index_select(0, col.clamp(min=0)).masked_fill_((col < 0).unsqueeze(1), 0.0)
     q = quantize8(rows)
-    steps = q.scales.shape[0]
+    steps = q.values.shape[1] // STEP
     # (tile, row, step, plane, lane group, byte) -> (tile, step, plane, lane = group and row, byte)
     v = q.values.view(torch.uint8).view(-1, 16, steps, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous()
-    return Weight8(v.view(-1, steps, 2, 64, 16).view(torch.float8_e4m3fn), q.scales, k, n, gated)
+    # (step, lane group, group of tiles, tile, row) -> (step, group of tiles, lane, tile)
+    c = q.scales.view(torch.uint8).view(steps, 4, -1, 4, 16).permute(0, 2, 1, 4, 3).contiguous()
+    return Weight8(v.view(-1, steps, 2, 64, 16).view(torch.float8_e4m3fn),
+                   c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, gated)
 
 
 def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
