@@ -35,17 +35,14 @@ constexpr uint32_t kInfBits = 0x7f800000u;
 __device__ __forceinline__ uint32_t abs_bits(float v) {
   return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu;
 }
-// The larger magnitude as integers: a finite float's bits order like its magnitude, and an
-// infinity or NaN comes out >= kInfBits.
+// The largest magnitude's bits, which order as the magnitudes do; NaN is passed over, an infinity
+// comes out as kInfBits.
 template <int N>
 __device__ __forceinline__ uint32_t max_bits(const float (&v)[N]) {
-  uint32_t u = 0;
+  float u = 0.f;
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const uint32_t b = abs_bits(v[i]);
-    u = u > b ? u : b;
-  }
-  return u;
+  for (int i = 0; i < N; ++i) u = __builtin_fmaxf(u, __builtin_fabsf(v[i]));
+  return __builtin_bit_cast(uint32_t, u);
 }
 // ... of the finite entries alone
 template <int N>

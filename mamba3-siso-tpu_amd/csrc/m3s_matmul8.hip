@@ -24,6 +24,7 @@
 // 4 (t & 1) + i, which leaves a lane 8 neighbouring outputs (16 bytes of bf16) in two tiles, and four
 // lanes the 32 of a block. With a gate, tiles 0 and 1 hold value's outputs 32 grp + 8 g + 4 t + i and
 // tiles 2 and 3 gate's, so a lane has both.
+#include <algorithm>
 #include <type_traits>
 
 #include "m3s_eight.h"
@@ -48,7 +49,11 @@ struct M8Params {
   int tiles_m, tiles_n;
 };
 
-__device__ __forceinline__ float silu8(float v) { return v / (1.f + __expf(-v)); }
+// v / (1 + e^-v) by the hardware's exponential and reciprocal, an ulp each (a division in full is some
+// ten instructions of the gate's epilogue). e^-v past float32 is an infinity, and the result -0.
+__device__ __forceinline__ float silu8(float v) {
+  return v * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-kLog2e * v));
+}
 __device__ __forceinline__ float act8(float v, int act) {
   if (act == kActSilu) return silu8(v);
   if (act == kActGelu) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
@@ -161,16 +166,11 @@ template <int SA, int SB>
 __device__ __forceinline__ void mma8(f32x4& acc, i32x8_ a, int sa, i32x8_ b, int sb) {
   acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc, 0, 0, SA, sa, SB, sb);
 }
-// a row of products: tile t of the weight (its byte of sa) with the TM row tiles
-template <int T, int TM>
-__device__ __forceinline__ void mma8_rows(f32x4 (&acc)[TM], i32x8_ a, int sa, const i32x8_ (&b)[TM],
-                                          const int (&sb)[(TM + 3) / 4]) {
-#pragma unroll
-  for (int q = 0; q < (TM + 3) / 4; ++q) {
-    mma8<T, 0>(acc[4 * q], a, sa, b[4 * q], sb[q]);
-    if constexpr (TM > 1) mma8<T, 1>(acc[4 * q + 1], a, sa, b[4 * q + 1], sb[q]);
-    if constexpr (TM > 2) mma8<T, 2>(acc[4 * q + 2], a, sa, b[4 * q + 2], sb[q]);
-    if constexpr (TM > 3) mma8<T, 3>(acc[4 * q + 3], a, sa, b[4 * q + 3], sb[q]);
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F f) {
+  if constexpr (N > 0) {
+    static_for<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
   }
 }
 
@@ -301,155 +301,140 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
 }
 
 // ---- many rows --------------------------------------------------------------------------
-// A workgroup of WN x WM waves takes 16 TN WN outputs (packed rows) and 16 TM WM rows, a wave TN x TM
-// tiles of them in accumulators. Each step's operands go to LDS by direct loads, as the lanes will
-// read them: a plane of 16 bytes a lane, so neither the loads nor the reads meet a bank twice. Two
-// stages: the loads of the next step, and its scales, are in flight under this one's products. Row
-// tile j of four holds rows 4 r + j, so that a lane's four scales are one dword.
-template <int WN, int WM, int TN, int TM, bool GATED>
-__global__ void __launch_bounds__(64 * WN * WM) matmul8_kernel(const M8Params p) {
-  constexpr int NW = WN * WM, NTL = TN * WN, MTL = TM * WM;
-  constexpr int LN = NTL / NW, LM = MTL / NW;    // tiles a wave loads
-  static_assert(NTL % NW == 0 && MTL % NW == 0 && TN % 4 == 0 && TM % 4 == 0, "whole tiles to a wave");
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2][(NTL + MTL) * 2048];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int r = lane & 15, g = lane >> 4;
-  // the tiles that one XCD works on at a time share rows: its workgroups walk the outputs first
-  const int nb = p.tiles_m * p.tiles_n, per = (nb + 7) >> 3, bid = blockIdx.x;
-  const int lin = (bid & 7) * per + (bid >> 3);
-  if (lin >= nb) return;
-  const int tn = lin % p.tiles_n, tm = lin / p.tiles_n;
-  const int ntiles = p.NP / 16, tile0 = tn * NTL;
-  const int64_t m0 = (int64_t)tm * (16 * MTL);
-  const int64_t kp = (int64_t)p.KB * kStep8;
-  const uint32_t wstep = (uint32_t)p.KB * 2048;
-  const __amdgpu_buffer_rsrc_t rw = make_rsrc(p.w + (int64_t)tile0 * wstep, 0xfffffff0u);
-  const __amdgpu_buffer_rsrc_t rx = make_rsrc(static_cast<const uint8_t*>(p.x) + m0 * kp, 0xfffffff0u);
-  const __amdgpu_buffer_rsrc_t rws = make_rsrc(p.ws, (uint32_t)((int64_t)p.KB * p.NP * 4));
-  const __amdgpu_buffer_rsrc_t rxs = make_rsrc(p.xs, (uint32_t)((int64_t)p.KB * p.mp * 4));
-  // a tile behind the last, and a row behind the last, reads the last one instead; neither is stored
-  uint32_t ow[LN], ox[LM];
-#pragma unroll
-  for (int i = 0; i < LN; ++i) ow[i] = (uint32_t)min(wave * LN + i, ntiles - 1 - tile0) * wstep + 16 * lane;
-#pragma unroll
-  for (int i = 0; i < LM; ++i) {
-    const int t = wave * LM + i;
-    const int64_t row = min((int64_t)(64 * (t >> 2) + 4 * r + (t & 3)), p.M - 1 - m0);
-    ox[i] = (uint32_t)(row * kp) + 16 * g;
-  }
-  auto load = [&](int buf, int kb) {
-#pragma unroll
-    for (int i = 0; i < LN; ++i) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        buf_load_lds16(rw, lds[buf] + (wave * LN + i) * 2048 + 1024 * h, ow[i] + 1024 * h, (uint32_t)kb * 2048);
-    }
-#pragma unroll
-    for (int i = 0; i < LM; ++i) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        buf_load_lds16(rx, lds[buf] + (NTL + wave * LM + i) * 2048 + 1024 * h, ox[i] + 64 * h, (uint32_t)kb * kStep8);
-    }
-  };
-  const int wn = wave % WN, wm = wave / WN;
-  const uint32_t osw = (uint32_t)(16 * (tile0 + wn * TN)) * 4 + 4 * lane;
-  const uint32_t osx = (uint32_t)((int64_t)g * p.mp + m0 + 16 * wm * TM + 4 * r);
-  auto scales = [&](int kb, int (&sw)[TN / 4], int (&sx)[TM / 4]) {
-#pragma unroll
-    for (int t = 0; t < TN / 4; ++t)
-      sw[t] = __builtin_amdgcn_raw_buffer_load_b32(rws, osw + 256 * t, (uint32_t)kb * (uint32_t)p.NP * 4, 0);
-#pragma unroll
-    for (int j = 0; j < TM / 4; ++j)
-      sx[j] = __builtin_amdgcn_raw_buffer_load_b32(rxs, osx + 64 * j, (uint32_t)((int64_t)kb * p.mp * 4), 0);
-  };
-  f32x4 acc[TN][TM];
-#pragma unroll
-  for (int t = 0; t < TN; ++t) {
-#pragma unroll
-    for (int j = 0; j < TM; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  int sw[TN / 4], sx[TM / 4], sw1[TN / 4], sx1[TM / 4];
-  load(0, 0);
-  scales(0, sw1, sx1);
-  for (int kb = 0; kb < p.KB; ++kb) {
-    vm_wait_all();
-    __syncthreads();   // this step's stage is whole, and every wave has read the other one
-#pragma unroll
-    for (int t = 0; t < TN / 4; ++t) sw[t] = sw1[t];
-#pragma unroll
-    for (int j = 0; j < TM / 4; ++j) sx[j] = sx1[j];
-    if (kb + 1 < p.KB) {
-      load((kb + 1) & 1, kb + 1);
-      scales(kb + 1, sw1, sx1);
-    }
-    const uint8_t* s = lds[kb & 1] + 16 * lane;
-    auto frag = [&](int tile) {
-      const uint8_t* q = s + tile * 2048;
-      return join8(*reinterpret_cast<const i32x4_*>(q), *reinterpret_cast<const i32x4_*>(q + 1024));
-    };
-    i32x8_ b[TM];
-#pragma unroll
-    for (int j = 0; j < TM; ++j) b[j] = frag(NTL + wm * TM + j);
-#pragma unroll
-    for (int q = 0; q < TN / 4; ++q) {
-      mma8_rows<0, TM>(acc[4 * q], frag(wn * TN + 4 * q), sw[q], b, sx);
-      mma8_rows<1, TM>(acc[4 * q + 1], frag(wn * TN + 4 * q + 1), sw[q], b, sx);
-      mma8_rows<2, TM>(acc[4 * q + 2], frag(wn * TN + 4 * q + 2), sw[q], b, sx);
-      mma8_rows<3, TM>(acc[4 * q + 3], frag(wn * TN + 4 * q + 3), sw[q], b, sx);
-    }
-  }
-  const int grp0 = (tile0 + wn * TN) / 4;
-  const int64_t mw = m0 + 16 * wm * TM + 4 * r;
-  // straight from the accumulators where every output of the tile is whole and goes out as it is
-  if (GATED || ((p.vec & 1) && p.act == kActNone && 16 * (tile0 + NTL) <= p.N)) {
+// v_mfma_scale_f32_32x32x64_f8f6f4: a 32-row tile of the weight is two packed tiles, and 64 k one of
+// their planes. Lane l (c = l & 31, h = l >> 5) gives row c's k 16 h .. and 32 + 16 h .., and its
+// scale of the 32 k of half h. A workgroup of four waves takes 32 TN WN outputs (packed rows) and
+// 32 TM WM rows. Each step of 64 k goes to LDS by direct loads as the lanes will read it, in planes of
+// 16 bytes a lane, two steps ahead of its products in a ring of three stages; the scales go to
+// registers. Two workgroups share a CU, so that one's loads, outputs and gates run under the
+// other's products: with one of 256 x 256 outputs there they stood in line (16384 x 1024 x 4480:
+// 104 us, of them 31 for the outputs and some 25 until a tile's first products).
+// Row tile j holds rows TM c + j of the wave's, so that a lane's scales of a step lie together.
+constexpr int kStage8 = 64;    // k of a stage
+constexpr int kBand = 16;
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+// A wave's accumulators: group q's tile T and row tile j; element 4 u + e of lane (c, h) is row
+// TM c + j and output 64 q + 32 T + 16 (u & 1) + 8 h + 4 (u >> 1) + e (gated: 32 q + ... of value or gate).
+template <int TN, int TM, bool GATED>
+__device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&acc)[TN][TM], int grp0,
+                                            int64_t row0, bool plain, int lane, float* sh) {
+  const int c = lane & 31, h = lane >> 5;
+  if constexpr (GATED) {
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
-      const int64_t m = mw + 64 * (j >> 2) + (j & 3);
-      if (m >= p.M) continue;
+      const int64_t m = row0 + TM * c + j;
 #pragma unroll
-      for (int q = 0; q < TN / 4; ++q) {
-        if (!GATED || grp0 + q < p.NP / 64) {
-          const f32x4 v[4] = {acc[4 * q][j], acc[4 * q + 1][j], acc[4 * q + 2][j], acc[4 * q + 3][j]};
-          finish_group<GATED, true>(p, m, grp0 + q, lane, v);
+      for (int q = 0; q < TN / 2; ++q) {
+        const int grp = grp0 + q;
+        if (m < p.M && grp < p.NP / 64) {   // both lanes of a row
+          float v[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {   // i: 8 outputs from 8 h, then 8 from 16 + 8 h
+            const int e = 8 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
+            float a = acc[2 * q][j][e], b = acc[2 * q + 1][j][e];
+            if (p.bias) {
+              const int n = min(32 * grp + 16 * (i >> 3) + 8 * h + (i & 7), p.N - 1);
+              a += p.bias[n];
+              b += p.bias[p.N + n];
+            }
+            v[i] = a * silu8(b);
+          }
+          if (32 * grp + 32 > p.N) {   // zeros behind the width
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (32 * grp + 16 * (i >> 3) + 8 * h + (i & 7) >= p.N) v[i] = 0.f;
+          }
+          uint32_t u = max_bits(v), o = (uint32_t)__shfl_xor((int)u, 32, 64);
+          u = u > o ? u : o;
+          if (u >= kInfBits) {
+            u = max_bits_finite(v);
+            o = (uint32_t)__shfl_xor((int)u, 32, 64);
+            u = u > o ? u : o;
+          }
+          const int byte = scale_byte(u);
+          const float down = scale_down(byte);
+          uint8_t* out = p.yv + m * ((int64_t)(p.NP / 256) * kStep8) + 32 * grp + 8 * h;
+          *reinterpret_cast<i32x2_*>(out) = i32x2_{pack4(v[0], v[1], v[2], v[3], down), pack4(v[4], v[5], v[6], v[7], down)};
+          *reinterpret_cast<i32x2_*>(out + 16) =
+              i32x2_{pack4(v[8], v[9], v[10], v[11], down), pack4(v[12], v[13], v[14], v[15], down)};
+          if (h == 0) p.ys[(int64_t)grp * p.mp + m] = (uint8_t)byte;
         }
       }
     }
-    return;
-  }
-  // else 16 rows at a time through the wave's share of LDS, so that odd widths and the activations are
-  // one loop each, and not unrolled over every accumulator
-  if constexpr (!GATED) {
-    constexpr int LD = 16 * TN + 4;
-    static_assert(16 * LD * 4 <= (int)sizeof(lds) / NW, "a wave's 16 rows fit its share");
-    __syncthreads();   // the last step's reads
-    float* sh = reinterpret_cast<float*>(&lds[0][0]) + wave * (sizeof(lds) / NW / 4);
+  } else if (plain) {
+    // No activation or residual: rounded to bf16 in the accumulators' order, turned in LDS, and out as
+    // whole 16-byte pieces of rows, 64 TN bytes of a row behind each other. From the accumulators alone
+    // a store's lanes hold 32 bytes of each of 32 rows (16384 x 1024 x 4480: 103 us, so 87).
+    constexpr int W = 32 * TN, LD = W + 8, PR = W / 8, RI = 64 / PR;   // pieces a row, rows at once
+    bf16* sb = reinterpret_cast<bf16*>(sh);
+    const int n0 = 64 * grp0, piece = lane % PR, n = n0 + 8 * piece;
+#pragma unroll
+    for (int j = 0; j < TM; ++j) {
+#pragma unroll
+      for (int t = 0; t < TN; ++t) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int at = 32 * t + 16 * k + 8 * h;
+          float v[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] = acc[t][j][8 * (i >> 2) + 4 * k + (i & 3)];
+          if (p.bias && n0 + at < p.N) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(p.bias + n0 + at);
+            const f32x4 d = *reinterpret_cast<const f32x4*>(p.bias + n0 + at + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] += a[i]; v[4 + i] += d[i]; }
+          }
+          bf16x8 o;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = (bf16)v[i];
+          *reinterpret_cast<bf16x8*>(sb + c * LD + at) = o;
+        }
+      }
+      wave_sync();
+      const int64_t mj = row0 + j + (int64_t)TM * (lane / PR);
+      bf16* yr = p.y + mj * p.ldy + n;
+#pragma unroll
+      for (int i = 0; i < 32 / RI; ++i) {
+        const bf16x8 o = *reinterpret_cast<const bf16x8*>(sb + (i * RI + lane / PR) * LD + 8 * piece);
+        if (mj + TM * RI * i < p.M && n < p.N) *reinterpret_cast<bf16x8*>(yr + (int64_t)(TM * RI * i) * p.ldy) = o;
+      }
+      wave_sync();
+    }
+  } else {
+    // 32 rows at a time through the wave's share of LDS, so that odd widths and the activations are one
+    // loop each, and not unrolled over every accumulator
+    constexpr int W = 32 * TN, LD = W + 4;
     const int n0 = 64 * grp0;
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
 #pragma unroll
-      for (int t = 0; t < TN; ++t)
-        *reinterpret_cast<f32x4*>(sh + r * LD + 64 * (t >> 2) + 32 * ((t >> 1) & 1) + 8 * g + 4 * (t & 1)) = acc[t][j];
+      for (int t = 0; t < TN; ++t) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          *reinterpret_cast<f32x4*>(sh + c * LD + 32 * t + 16 * (u & 1) + 8 * h + 4 * (u >> 1)) =
+              f32x4{acc[t][j][4 * u], acc[t][j][4 * u + 1], acc[t][j][4 * u + 2], acc[t][j][4 * u + 3]};
+      }
       wave_sync();
-      const int64_t mj = m0 + 16 * wm * TM + 64 * (j >> 2) + (j & 3);
+      const int64_t mj = row0 + j;
       if (p.vec & 1) {
 #pragma unroll 1
-        for (int e = lane; e < 16 * 2 * TN; e += 64) {
-          const int row = e / (2 * TN), c = 8 * (e % (2 * TN));
-          if (mj + 4 * row < p.M) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(sh + row * LD + c);
-            const f32x4 d = *reinterpret_cast<const f32x4*>(sh + row * LD + c + 4);
+        for (int e = lane; e < 32 * (W / 8); e += 64) {
+          const int row = e / (W / 8), n = 8 * (e % (W / 8));
+          if (mj + TM * row < p.M) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(sh + row * LD + n);
+            const f32x4 d = *reinterpret_cast<const f32x4*>(sh + row * LD + n + 4);
             float v[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
-            finish8<false>(p, mj + 4 * row, n0 + c, v);
+            finish8<false>(p, mj + TM * row, n0 + n, v);
           }
         }
       } else {
 #pragma unroll 1
-        for (int e = lane; e < 16 * 16 * TN; e += 64) {
-          const int row = e / (16 * TN), c = e % (16 * TN);
-          const int64_t m = mj + 4 * row;
-          const int n = n0 + c;
+        for (int e = lane; e < 32 * W; e += 64) {
+          const int row = e / W, n = n0 + e % W;
+          const int64_t m = mj + TM * row;
           if (m < p.M && n < p.N) {
-            float v = sh[row * LD + c];
+            float v = sh[row * LD + e % W];
             if (p.bias) v += p.bias[n];
             v = act8(v, p.act);
             if (p.residual) v += (float)p.residual[m * p.ldr + n];
@@ -462,6 +447,137 @@ __global__ void __launch_bounds__(64 * WN * WM) matmul8_kernel(const M8Params p)
   }
 }
 
+template <int WN, int WM, int TN, int TM, bool GATED>
+__global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params p) {
+  constexpr int NW = WN * WM, NTL = 2 * TN * WN, MTL = 2 * TM * WM;   // 16-row tiles
+  constexpr int LN = NTL / NW, LM = MTL / NW;    // tiles whose plane a wave loads
+  constexpr int kOps = LN + LM + TN / 2 + 1;     // vector memory operations of a step's loads
+  static_assert(NTL % NW == 0 && MTL % NW == 0 && TN % 2 == 0 && (TM == 1 || TM == 2 || TM == 4), "tiles");
+  constexpr int kStageBytes = (NTL + MTL) * 1024, kShare = 32 * (32 * TN + 4) * 4;
+  constexpr int kLds = 3 * kStageBytes > NW * kShare || GATED ? 3 * kStageBytes : NW * kShare;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // One XCD's workgroups take consecutive tiles, kBand row tiles high and walked along the outputs:
+  // the 64 at work at a time read some 16 strips of rows and 4 of the weight through their L2, where
+  // one row tile's would read as many strips of the weight as there are workgroups (8192^3, 256 x 256
+  // outputs to a workgroup: 540 us, with bands 447).
+  const int nb = p.tiles_m * p.tiles_n, per = (nb + 7) >> 3, bid = blockIdx.x;
+  const int lin = (bid & 7) * per + (bid >> 3);
+  if (lin >= nb) return;
+  const int band = lin / (kBand * p.tiles_n), high = min(kBand, p.tiles_m - band * kBand);
+  const int at = lin - band * kBand * p.tiles_n;
+  const int ntiles = p.NP / 16, tile0 = at / high * NTL;
+  const int64_t m0 = (int64_t)(band * kBand + at % high) * (16 * MTL);
+  const int64_t kp = (int64_t)p.KB * kStep8;
+  const uint32_t wstep = (uint32_t)p.KB * 2048;
+  const uint8_t* wbase = p.w + (int64_t)tile0 * wstep;
+  const uint8_t* xbase = static_cast<const uint8_t*>(p.x) + m0 * kp;
+  const int S = 2 * p.KB;
+  const int wn = wave % WN, wm = wave / WN, c = lane & 31, h = lane >> 5;
+  // A tile behind the last, and a row behind the last, reads the last one instead; neither is stored.
+  // Tile t's row r is row TM c + j of its wave's 32 TM, with 32 j + c = 16 (t % (2 TM)) + r.
+  uint32_t ow[LN], ox[LM];
+#pragma unroll
+  for (int i = 0; i < LN; ++i) ow[i] = (uint32_t)min(wave * LN + i, ntiles - 1 - tile0) * wstep + 16 * lane;
+#pragma unroll
+  for (int i = 0; i < LM; ++i) {
+    const int t = wave * LM + i, tw = t % (2 * TM);
+    const int64_t row = min((int64_t)(32 * TM * (t / (2 * TM)) + TM * (16 * (tw & 1) + (lane & 15)) + (tw >> 1)),
+                            p.M - 1 - m0);
+    ox[i] = (uint32_t)(row * kp) + 16 * (lane >> 4);
+  }
+  // behind the last step the loads go through empty descriptors and touch no memory
+  auto load = [&](int stage, int s) {
+    s = __builtin_amdgcn_readfirstlane(s);
+    const uint32_t bytes = s < S ? 0xfffffff0u : 0u;
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(wbase, bytes), rx = make_rsrc(xbase, bytes);
+    uint8_t* to = lds + stage * kStageBytes;
+#pragma unroll
+    for (int i = 0; i < LN; ++i) buf_load_lds16(rw, to + (wave * LN + i) * 1024, ow[i], (uint32_t)s * 1024);
+#pragma unroll
+    for (int i = 0; i < LM; ++i) buf_load_lds16(rx, to + (NTL + wave * LM + i) * 1024, ox[i], (uint32_t)s * kStage8);
+  };
+  // group q's dword holds its four 16-row tiles' scales of a row; bit 4 of the lane picks the tile of a pair
+  const uint32_t osw = (uint32_t)(16 * tile0 + 32 * TN * wn) * 4 + 4 * (16 * h + (lane & 15));
+  const uint32_t osx = (uint32_t)((int64_t)h * p.mp + m0 + 32 * TM * wm + (TM * c & ~3));
+  auto scales = [&](int s, int (&sw)[TN / 2], int& sx) {
+    s = __builtin_amdgcn_readfirstlane(s);
+    const __amdgpu_buffer_rsrc_t rws = make_rsrc(p.ws, s < S ? (uint32_t)((int64_t)p.KB * p.NP * 4) : 0u);
+    const __amdgpu_buffer_rsrc_t rxs = make_rsrc(p.xs, s < S ? (uint32_t)((int64_t)p.KB * p.mp * 4) : 0u);
+#pragma unroll
+    for (int q = 0; q < TN / 2; ++q)
+      sw[q] = __builtin_amdgcn_raw_buffer_load_b32(rws, osw + 256 * q, (uint32_t)(s >> 1) * (uint32_t)p.NP * 4 + (s & 1) * 128, 0);
+    sx = __builtin_amdgcn_raw_buffer_load_b32(rxs, osx, (uint32_t)((int64_t)s * 2 * p.mp), 0);
+  };
+  f32x16 acc[TN][TM];
+#pragma unroll
+  for (int t = 0; t < TN; ++t) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) acc[t][j] = f32x16{};
+  }
+  int sw[3][TN / 2], sx[3];
+  // half h's k of tile pair T: lane group 2 half + h of plane, rows c of both tiles
+  const int lread = (c >> 4) * 1024 + h * 256 + (c & 15) * 16;
+  auto step = [&](auto rc, int s) {
+    constexpr int R = decltype(rc)::value;
+    // this step's loads are done when only the next one's are under way; every wave has read the stage
+    // that the loads of the step after that fill
+    vm_wait_keep<kOps>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    load((R + 2) % 3, s + 2);
+    const uint8_t* at = lds + R * kStageBytes + lread;
+    auto frag = [&](int tile) {
+      return join8(*reinterpret_cast<const i32x4_*>(at + tile * 2048),
+                   *reinterpret_cast<const i32x4_*>(at + tile * 2048 + 512));
+    };
+    i32x8_ b[TM];
+#pragma unroll
+    for (int j = 0; j < TM; ++j) b[j] = frag(NTL / 2 + wm * TM + j);
+    const int by = 8 * (c >> 4), sr = (int)((uint32_t)sx[R] >> (8 * (TM * c & 3)));
+#pragma unroll
+    for (int q = 0; q < TN / 2; ++q) {
+      const int s4 = (int)((uint32_t)sw[R][q] >> by);
+      const i32x8_ a0 = frag(wn * TN + 2 * q), a1 = frag(wn * TN + 2 * q + 1);
+      static_for<TM>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        acc[2 * q][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, b[j], acc[2 * q][j], 0, 0, 0, s4, j, sr);
+      });
+      static_for<TM>([&](auto jc) {
+        constexpr int j = decltype(jc)::value;
+        acc[2 * q + 1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, b[j], acc[2 * q + 1][j], 0, 0, 2, s4, j, sr);
+      });
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    scales(s + 3, sw[R], sx[R]);
+    asm volatile("" ::: "memory");
+  };
+  const std::integral_constant<int, 0> r0;
+  const std::integral_constant<int, 1> r1;
+  const std::integral_constant<int, 2> r2;
+  // in this order: a step counts the operations behind its own loads
+  scales(0, sw[0], sx[0]);
+  load(0, 0);
+  __builtin_amdgcn_sched_barrier(0);
+  scales(1, sw[1], sx[1]);
+  load(1, 1);
+  scales(2, sw[2], sx[2]);
+  __builtin_amdgcn_sched_barrier(0);
+  for (int s = 0;; s += 3) {
+    step(r0, s);
+    if (s + 1 >= S) break;
+    step(r1, s + 1);
+    if (s + 2 >= S) break;
+    step(r2, s + 2);
+    if (s + 3 >= S) break;
+  }
+  vm_wait_all();   // no load may reach LDS behind the workgroup's end
+  const bool plain = (p.vec & 1) && p.act == kActNone && !p.residual && p.N % 8 == 0;
+  if (!GATED) __syncthreads();
+  finish_tile<TN, TM, GATED>(p, acc, (tile0 + 2 * TN * wn) / 4, m0 + 32 * TM * wm, plain, lane,
+                             reinterpret_cast<float*>(lds) + wave * (kShare / 4));
+}
+
 template <int MT, int XK, bool GATED>
 static void launch_few(const M8Params& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.NP / 64), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
@@ -470,8 +586,8 @@ static void launch_few(const M8Params& p, hipStream_t s) {
 
 template <int WN, int WM, int TN, int TM, bool GATED>
 static void launch_many(M8Params p, hipStream_t s) {
-  p.tiles_n = (p.NP / 16 + TN * WN - 1) / (TN * WN);
-  p.tiles_m = (int)((p.M + 16 * TM * WM - 1) / (16 * TM * WM));
+  p.tiles_n = (p.NP + 32 * TN * WN - 1) / (32 * TN * WN);
+  p.tiles_m = (int)((p.M + 32 * TM * WM - 1) / (32 * TM * WM));
   const int64_t nb = (int64_t)p.tiles_m * p.tiles_n;
   const unsigned grid = (unsigned)(((nb + 7) >> 3) * 8);
   hipLaunchKernelGGL((matmul8_kernel<WN, WM, TN, TM, GATED>), dim3(grid), dim3(64 * WN * WM), 0, s, p);
@@ -483,7 +599,7 @@ static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED>(p, s);
   if (p.M <= 16) return launch_few<1, kRows8, GATED>(p, s);
   if (p.M <= 256) return launch_few<2, kRows8, GATED>(p, s);
-  launch_many<2, 4, 8, 4, GATED>(p, s);
+  launch_many<4, 1, 2, 4, GATED>(p, s);
 }
 
 }  // namespace m3s
