@@ -436,6 +436,7 @@ def nodes(path: str = NODES_PATH):
         raise RuntimeError(f"{path} was built for torch {mod.torch_version}, not {torch.__version__}; rebuild it")
     mod.bind(*(C.cast(fn, vp).value for fn in (lib.m3s_embed_fwd, lib.m3s_embed_bwd,
                                                lib.m3s_embed_bwd_workspace_bytes, lib.m3s_last_error)))
+    mod.bind8(*(C.cast(fn, vp).value for fn in (lib.m3s_rows8, lib.m3s_rows8_values, lib.m3s_matmul8)))
     _nodes = mod
     return mod
 

@@ -7,9 +7,13 @@
 // lookup alone, without a gradient, 7.5 and 4.7. What is left is the engine's hand-over to its thread
 // and back.
 //
+// The operators in 8 bits (eightbit.py) are here for the same reason, without a gradient: rows of a token
+// take the device 2 to 6 us and took the host 8 to 12 in Python (a product of 256 float rows, two
+// launches, 17).
+//
 // This module holds no mathematics and no launch of its own: the package's binding (_lib.py) hands it
-// the loaded library's entry points. embed() takes dense tensors of the kernels' types and answers None
-// for everything else, which the package then handles, or refuses, in Python.
+// the loaded library's entry points. Each function takes dense tensors of the kernels' types and answers
+// None for everything else, which the package then handles, or refuses, in Python.
 #include <Python.h>
 
 #include <mutex>
@@ -40,6 +44,9 @@ struct Entries {   // of the loaded library, by bind()
   decltype(&m3s_embed_bwd) bwd;
   decltype(&m3s_embed_bwd_workspace_bytes) bwd_bytes;
   decltype(&m3s_last_error) error;
+  decltype(&m3s_rows8) rows8;   // by bind8()
+  decltype(&m3s_rows8_values) values8;
+  decltype(&m3s_matmul8) matmul8;
 } lib = {};
 
 // The exception types of the Python binding's check().
@@ -190,6 +197,306 @@ PyObject* embed(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- 8 bits -------------------------------------------------------------------------------------
+
+constexpr int64_t kNormMax8 = 16384;   // the widest row that m3s_rows8 normalises
+
+int64_t padded(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+bool float_type(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16; }
+int32_t code(at::ScalarType t) { return t == at::kBFloat16 ? M3S_DTYPE_BF16 : M3S_DTYPE_F32; }
+
+// A tensor that the argument is, or null: plain, on `device` if that is given, and without a gradient to take.
+const Tensor* given(PyObject* o, const at::Device* device) {
+  if (!THPVariable_Check(o)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(o);
+  if (!t.defined() || !plain(t) || (device && t.device() != *device) ||
+      (at::GradMode::is_enabled() && t.requires_grad()))
+    return nullptr;
+  return &t;
+}
+
+// Rows of `t` (..., width) that run as one matrix of unit column stride: their count and stride.
+bool row_matrix(const Tensor& t, int64_t& rows, int64_t& stride) {
+  if (t.dim() < 1) return false;
+  const int64_t width = t.size(-1);
+  if (width < 1 || width > M3S_ROWS8_WIDTH_MAX) return false;
+  rows = t.numel() / width;
+  stride = width;
+  if (rows < 1 || rows > M3S_ROWS8_MAX) return false;
+  if (t.is_contiguous()) return true;
+  if (t.dim() != 2 || (width > 1 && t.stride(1) != 1) || (rows > 1 && t.stride(0) < width)) return false;
+  if (rows > 1) stride = t.stride(0);
+  return true;
+}
+
+struct Rows {   // rows in 8 bits
+  Tensor values, scales;
+  int64_t rows = 0, width = 0;
+};
+
+Rows fresh_rows(int64_t rows, int64_t width, at::Device device, bool poison) {
+  const int64_t kp = padded(width, 128);
+  return {fresh({rows, kp}, at::kFloat8_e4m3fn, device, poison),
+          fresh({kp / 32, padded(rows, 16)}, at::kFloat8_e8m0fnu, device, poison), rows, width};
+}
+
+m3s_rows8_args rows8_args(const Tensor& x, int64_t stride, const Rows& out) {
+  m3s_rows8_args a = {};
+  a.struct_size = sizeof(a);
+  a.x_dtype = code(x.scalar_type());
+  a.width = (int32_t)out.width;
+  a.rows = out.rows;
+  a.x = x.data_ptr();
+  a.ldx = stride;
+  a.values = out.values.data_ptr();
+  a.scales = out.scales.data_ptr();
+  return a;
+}
+
+// The fields of a Rows8 (values, scales, width, lead) with the leading sizes of `shape`.
+PyObject* wrap_rows(Rows& r, at::IntArrayRef lead) {
+  PyObject* sizes = PyTuple_New((Py_ssize_t)lead.size());
+  if (!sizes) return nullptr;
+  for (size_t i = 0; i < lead.size(); ++i) PyTuple_SET_ITEM(sizes, i, PyLong_FromLongLong(lead[i]));
+  return Py_BuildValue("(NNLN)", THPVariable_Wrap(std::move(r.values)), THPVariable_Wrap(std::move(r.scales)),
+                       (long long)r.width, sizes);
+}
+
+// A Rows8 as the argument holds it.
+bool unwrap_rows(PyObject* o, Rows& r, at::DimVector& lead) {
+  if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
+  const Tensor* values = given(PyTuple_GET_ITEM(o, 0), nullptr);
+  if (!values) return false;
+  const at::Device device = values->device();
+  const Tensor* scales = given(PyTuple_GET_ITEM(o, 1), &device);
+  PyObject *width = PyTuple_GET_ITEM(o, 2), *sizes = PyTuple_GET_ITEM(o, 3);
+  if (!scales || !PyLong_Check(width) || !PyTuple_Check(sizes)) return false;
+  r.width = PyLong_AsLongLong(width);
+  r.rows = 1;
+  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes); ++i) {
+    PyObject* n = PyTuple_GET_ITEM(sizes, i);
+    if (!PyLong_Check(n)) return false;
+    const int64_t size = PyLong_AsLongLong(n);
+    if (size < 1 || size > M3S_ROWS8_MAX) return false;   // no rows: Python's
+    lead.push_back(size);
+    r.rows *= size;
+    if (r.rows > M3S_ROWS8_MAX) return false;
+  }
+  if (r.width < 1 || r.width > M3S_ROWS8_WIDTH_MAX) return false;
+  const int64_t kp = padded(r.width, 128);
+  if (values->scalar_type() != at::kFloat8_e4m3fn || scales->scalar_type() != at::kFloat8_e8m0fnu ||
+      values->sizes() != at::IntArrayRef({r.rows, kp}) ||
+      scales->sizes() != at::IntArrayRef({kp / 32, padded(r.rows, 16)}) || !values->is_contiguous() ||
+      !scales->is_contiguous())
+    return false;
+  r.values = *values;
+  r.scales = *scales;
+  return true;
+}
+
+// rows8(x, gain or None, eps, add or None, poison): ((values, scales, width, lead), sum or None), or None.
+PyObject* rows8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 5) {
+    PyErr_SetString(PyExc_TypeError, "rows8 takes rows, a gain, an epsilon, rows to add and a truth value");
+    return nullptr;
+  }
+  TORCH_CHECK(lib.rows8, "rows8: the library's entry points are not bound");
+  const double eps = PyFloat_AsDouble(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  const Tensor* x = given(args[0], nullptr);
+  int64_t rows = 0, stride = 0, add_rows = 0, add_stride = 0;
+  if (!x || torch::jit::tracer::isTracing() || !float_type(x->scalar_type()) || !row_matrix(*x, rows, stride))
+    Py_RETURN_NONE;
+  const at::Device device = x->device();
+  const int64_t width = x->size(-1);
+  const Tensor *gain = nullptr, *add = nullptr;
+  if (args[1] != Py_None) {
+    gain = given(args[1], &device);
+    if (!gain || gain->scalar_type() != at::kFloat || gain->dim() != 1 || gain->size(0) != width ||
+        !gain->is_contiguous() || width > kNormMax8)
+      Py_RETURN_NONE;
+  }
+  if (args[3] != Py_None) {
+    add = given(args[3], &device);
+    if (!add || !gain || add->scalar_type() != at::kBFloat16 || add->sizes() != x->sizes() ||
+        !row_matrix(*add, add_rows, add_stride))
+      Py_RETURN_NONE;
+  }
+  const c10::DeviceGuard guard(device);
+  const bool poison = args[4] == Py_True;
+  Rows out = fresh_rows(rows, width, device, poison);
+  m3s_rows8_args a = rows8_args(*x, stride, out);
+  a.eps = (float)eps;
+  Tensor sum;
+  if (gain) a.gain = static_cast<const float*>(gain->data_ptr());
+  if (add) {
+    sum = fresh(x->sizes(), x->scalar_type(), device, poison);
+    a.add = add->data_ptr();
+    a.ldadd = add_stride;
+    a.sum = sum.data_ptr();
+  }
+  check(lib.rows8(&a, stream_of(device)), "m3s_rows8");
+  PyObject* r = wrap_rows(out, x->sizes().slice(0, x->dim() - 1));
+  if (!r) return nullptr;
+  if (add) return Py_BuildValue("(NN)", r, THPVariable_Wrap(std::move(sum)));
+  return Py_BuildValue("(NO)", r, Py_None);
+  END_HANDLE_TH_ERRORS
+}
+
+// rows8_values(rows, bf16 (else float32), poison): the values that a Rows8 stands for, or None.
+PyObject* rows8_values(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 3) {
+    PyErr_SetString(PyExc_TypeError, "rows8_values takes rows and two truth values");
+    return nullptr;
+  }
+  TORCH_CHECK(lib.values8, "rows8_values: the library's entry points are not bound");
+  Rows r;
+  at::DimVector sizes;
+  if (torch::jit::tracer::isTracing() || !unwrap_rows(args[0], r, sizes)) Py_RETURN_NONE;
+  const at::Device device = r.values.device();
+  const c10::DeviceGuard guard(device);
+  sizes.push_back(r.width);
+  const at::ScalarType type = args[1] == Py_True ? at::kBFloat16 : at::kFloat;
+  Tensor y = fresh(sizes, type, device, args[2] == Py_True);
+  m3s_rows8_values_args a = {};
+  a.struct_size = sizeof(a);
+  a.y_dtype = code(type);
+  a.width = (int32_t)r.width;
+  a.rows = r.rows;
+  a.values = r.values.data_ptr();
+  a.scales = r.scales.data_ptr();
+  a.y = y.data_ptr();
+  check(lib.values8(&a, stream_of(device)), "m3s_rows8_values");
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// matmul8(rows, weight, gated, activation, bias or None, residual or None, poison): the product, gated a
+// Rows8's fields, or None. `rows` is a tensor or a Rows8, `weight` a Weight8.
+PyObject* matmul8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 7) {
+    PyErr_SetString(PyExc_TypeError,
+                    "matmul8 takes rows, a weight, a truth value, an activation, a bias, a residual and a truth value");
+    return nullptr;
+  }
+  TORCH_CHECK(lib.matmul8 && lib.rows8, "matmul8: the library's entry points are not bound");
+  const int64_t activation = PyLong_AsLongLong(args[3]);
+  if (PyErr_Occurred()) return nullptr;
+  PyObject* wt = args[1];
+  const bool gated = args[2] == Py_True;
+  if (torch::jit::tracer::isTracing() || !PyTuple_Check(wt) || PyTuple_GET_SIZE(wt) != 5 ||
+      PyTuple_GET_ITEM(wt, 4) != (gated ? Py_True : Py_False) || !PyLong_Check(PyTuple_GET_ITEM(wt, 2)) ||
+      !PyLong_Check(PyTuple_GET_ITEM(wt, 3)))
+    Py_RETURN_NONE;
+  const Tensor* wv = given(PyTuple_GET_ITEM(wt, 0), nullptr);
+  if (!wv) Py_RETURN_NONE;
+  const at::Device device = wv->device();
+  const Tensor* wsc = given(PyTuple_GET_ITEM(wt, 1), &device);
+  const int64_t k = PyLong_AsLongLong(PyTuple_GET_ITEM(wt, 2)), n = PyLong_AsLongLong(PyTuple_GET_ITEM(wt, 3));
+  if (!wsc || k < 1 || k > M3S_ROWS8_WIDTH_MAX || n < 1 || n > M3S_ROWS8_WIDTH_MAX) Py_RETURN_NONE;
+  const int64_t tiles = (gated ? 2 * padded(n, 128) : padded(n, 64)) / 16, steps = padded(k, 128) / 128;
+  if (wv->sizes() != at::IntArrayRef({tiles, steps, 2, 64, 16}) || wv->scalar_type() != at::kFloat8_e4m3fn ||
+      wsc->sizes() != at::IntArrayRef({steps, tiles / 4, 64, 4}) || wsc->scalar_type() != at::kFloat8_e8m0fnu ||
+      !wv->is_contiguous() || !wsc->is_contiguous())
+    Py_RETURN_NONE;
+  m3s_matmul8_args a = {};
+  a.struct_size = sizeof(a);
+  a.k = (int32_t)k;
+  a.n = (int32_t)n;
+  a.gated = gated;
+  a.activation = (int32_t)activation;
+  a.w = wv->data_ptr();
+  a.w_scales = wsc->data_ptr();
+  Rows r;
+  at::DimVector lead;
+  const Tensor* x = nullptr;
+  int64_t stride = 0;
+  if (THPVariable_Check(args[0])) {
+    x = given(args[0], &device);
+    if (!x || !float_type(x->scalar_type()) || !row_matrix(*x, r.rows, stride)) Py_RETURN_NONE;
+    r.width = x->size(-1);
+    lead.append(x->sizes().begin(), x->sizes().end() - 1);
+  } else if (!unwrap_rows(args[0], r, lead) || r.values.device() != device) {
+    Py_RETURN_NONE;
+  }
+  if (r.width != k) Py_RETURN_NONE;
+  at::DimVector sizes = lead;
+  sizes.push_back(n);
+  if (args[4] != Py_None) {
+    const Tensor* bias = given(args[4], &device);
+    if (!bias || bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != (gated ? 2 * n : n) ||
+        !bias->is_contiguous())
+      Py_RETURN_NONE;
+    a.bias = static_cast<const float*>(bias->data_ptr());
+  }
+  if (args[5] != Py_None) {
+    const Tensor* res = given(args[5], &device);
+    int64_t rows = 0;
+    if (!res || gated || res->scalar_type() != at::kBFloat16 || res->sizes() != at::IntArrayRef(sizes) ||
+        !row_matrix(*res, rows, a.ldres))
+      Py_RETURN_NONE;
+    a.residual = res->data_ptr();
+  }
+  const c10::DeviceGuard guard(device);
+  const bool poison = args[6] == Py_True;
+  void* stream = stream_of(device);
+  if (x && r.rows > M3S_MATMUL8_FLOAT_ROWS) {
+    r = fresh_rows(r.rows, r.width, device, poison);
+    m3s_rows8_args q = rows8_args(*x, stride, r);
+    check(lib.rows8(&q, stream), "m3s_rows8");
+    x = nullptr;
+  }
+  a.rows = r.rows;
+  if (x) {
+    a.x_dtype = code(x->scalar_type());
+    a.x = x->data_ptr();
+    a.ldx = stride;
+  } else {
+    a.x_dtype = M3S_DTYPE_ROWS8;
+    a.x = r.values.data_ptr();
+    a.x_scales = r.scales.data_ptr();
+  }
+  if (gated) {
+    Rows out = fresh_rows(r.rows, n, device, poison);
+    a.y_values = out.values.data_ptr();
+    a.y_scales = out.scales.data_ptr();
+    check(lib.matmul8(&a, stream), "m3s_matmul8");
+    return wrap_rows(out, lead);
+  }
+  Tensor y = fresh(sizes, at::kBFloat16, device, poison);
+  a.y = y.data_ptr();
+  a.ldy = n;
+  check(lib.matmul8(&a, stream), "m3s_matmul8");
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+bool addresses(PyObject* const* args, Py_ssize_t nargs, void** at, Py_ssize_t count) {
+  if (nargs != count) {
+    PyErr_Format(PyExc_TypeError, "takes %zd addresses", count);
+    return false;
+  }
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    at[i] = PyLong_AsVoidPtr(args[i]);
+    if (PyErr_Occurred()) return false;
+  }
+  return true;
+}
+
+// bind8(m3s_rows8, m3s_rows8_values, m3s_matmul8): addresses.
+PyObject* bind8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  void* at[3];
+  if (!addresses(args, nargs, at, 3)) return nullptr;
+  lib.rows8 = reinterpret_cast<decltype(lib.rows8)>(at[0]);
+  lib.values8 = reinterpret_cast<decltype(lib.values8)>(at[1]);
+  lib.matmul8 = reinterpret_cast<decltype(lib.matmul8)>(at[2]);
+  Py_RETURN_NONE;
+}
+
 // bind(m3s_embed_fwd, m3s_embed_bwd, m3s_embed_bwd_workspace_bytes, m3s_last_error): addresses.
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   void* at[4];
@@ -210,6 +517,10 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
 
 PyMethodDef methods[] = {
     {"embed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(embed)), METH_FASTCALL, nullptr},
+    {"rows8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rows8)), METH_FASTCALL, nullptr},
+    {"rows8_values", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(rows8_values)), METH_FASTCALL, nullptr},
+    {"matmul8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(matmul8)), METH_FASTCALL, nullptr},
+    {"bind8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind8)), METH_FASTCALL, nullptr},
     {"bind", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(bind)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "m3s_nodes", nullptr, -1, methods};

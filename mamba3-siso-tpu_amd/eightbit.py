@@ -12,7 +12,8 @@ the rate of bf16, and a weight takes half the memory and half the traffic.
 * `swiglu8`    -- the gated MLP's first product and its gate, the rows out in 8 bits.
 
 Each is one launch of ``csrc/m3s_rows8.hip`` or ``csrc/m3s_matmul8.hip`` (`matmul8` and `swiglu8` of
-more than 16 float rows two). They take no gradient and refuse operands that need one.
+more than 16 float rows two), called from C++ (``csrc/m3s_nodes.cpp``) for dense operands of the kernels'
+types and from here for others. They take no gradient and refuse operands that need one.
 `model.eight_bit_params` makes a model of them.
 """
 
@@ -51,6 +52,10 @@ class Rows8(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tensor:
         """The values that the 8 bits stand for, (..., width) in bf16 (exact) or float32."""
+        if dtype in _FLOATS:
+            y = _lib.nodes().rows8_values(self, dtype is torch.bfloat16, K.POISON_OUTPUTS)
+            if y is not None:
+                return y
         rows = _check_rows8(self, "dequantize")
         y = K.empty(*self.lead, self.width, device=self.values.device, dtype=dtype)
         a = _lib.Rows8ValuesArgs(ctypes.sizeof(_lib.Rows8ValuesArgs), _lib.dtype_code(dtype), self.width,
@@ -137,6 +142,9 @@ def quantize8(x: Tensor) -> Rows8:
     """``x`` (..., width) float32 or bf16 as `Rows8`: each value rounded to the nearest e4m3 of its
     block's scale, ties to even. An entry that is not finite becomes NaN and leaves the scale of its
     block to the others. Rows may have any stride between them."""
+    done = _lib.nodes().rows8(x, None, 0.0, None, K.POISON_OUTPUTS)
+    if done is not None:
+        return Rows8._make(done[0])
     _check_float_rows(x, "quantize8")
     dev = K._device_of(x)
     K.refuse_gradient("quantize8", x)
@@ -157,6 +165,9 @@ def rms_norm8(x: Tensor, gain: Tensor, eps: float, add: Optional[Tensor] = None)
     block whose bf16 output is ``add`` (``x`` itself without one), and ``s / sqrt(mean(s^2) + eps) *
     gain`` in 8 bits, with float32 statistics and no rounding before the one to 8 bits. ``s`` is in the
     stream's type. The width is at most 16384."""
+    done = _lib.nodes().rows8(x, gain, eps, add, K.POISON_OUTPUTS)
+    if done is not None:
+        return x if add is None else done[1], Rows8._make(done[0])
     _check_float_rows(x, "rms_norm8")
     lead, width = tuple(x.shape[:-1]), x.shape[-1]
     rows = _count(lead)
@@ -226,7 +237,7 @@ def pack8(w: Tensor, gated: bool = False) -> Weight8:
     # (step, lane group, group of tiles, tile, row) -> (step, group of tiles, lane, tile)
     c = q.scales.view(torch.uint8).view(steps, 4, -1, 4, 16).permute(0, 2, 1, 4, 3).contiguous()
     return Weight8(v.view(-1, steps, 2, 64, 16).view(torch.float8_e4m3fn),
-                   c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, gated)
+                   c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, bool(gated))
 
 
 def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
@@ -274,6 +285,9 @@ def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[s
     one rounding of the result. A row with a NaN or an infinity comes out NaN."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"matmul8: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    y = _lib.nodes().matmul8(x, w, False, ACTIVATIONS[activation], bias, residual, K.POISON_OUTPUTS)
+    if y is not None:
+        return y
     a, dev, lead, rows, keep = _operands(x, w, bias, "matmul8")
     if w.gated:
         raise ValueError("matmul8: a gated weight goes to swiglu8")
@@ -308,6 +322,9 @@ def swiglu8(x, w: Weight8, bias: Optional[Tensor] = None) -> Rows8:
     """``value * silu(gate)`` of ``value | gate = x @ w + bias`` in 8 bits (..., n), in float32 up to that
     rounding: the gated MLP's first product on a weight packed with ``gated=True``. ``x`` and ``bias``
     (2 n,) as in `matmul8`."""
+    done = _lib.nodes().matmul8(x, w, True, 0, bias, None, K.POISON_OUTPUTS)
+    if done is not None:
+        return Rows8._make(done)
     a, dev, lead, rows, keep = _operands(x, w, bias, "swiglu8")
     if not w.gated:
         raise ValueError("swiglu8: the weight must be packed with gated=True")
