@@ -363,9 +363,53 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
       }
     }
   } else if (plain) {
-    // No activation or residual: rounded to bf16 in the accumulators' order, turned in LDS, and out as
-    // whole 16-byte pieces of rows, 64 TN bytes of a row behind each other. From the accumulators alone
-    // a store's lanes hold 32 bytes of each of 32 rows (16384 x 1024 x 4480: 103 us, so 87).
+    // No activation: turned in LDS, and out as whole 16-byte pieces of rows, 64 TN bytes of a row behind
+    // each other. From the accumulators alone a store's lanes hold 32 bytes of each of 32 rows
+    // (16384 x 1024 x 4480: 103 us, so 87). Without a residual LDS holds the outputs' own bf16; with one
+    // float32, as the sum is rounded once, and the residual's rows are read under the turn.
+    if (p.residual) {
+      constexpr int W = 32 * TN, LD = W + 4, PR = W / 8, RI = 64 / PR;
+      const int n0 = 64 * grp0, piece = lane % PR, n = n0 + 8 * piece;
+      float bias[8] = {};
+      if (p.bias && n < p.N) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p.bias + n), d = *reinterpret_cast<const f32x4*>(p.bias + n + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { bias[i] = a[i]; bias[4 + i] = d[i]; }
+      }
+#pragma unroll
+      for (int j = 0; j < TM; ++j) {
+        const int64_t mj = row0 + j + (int64_t)TM * (lane / PR);
+        bf16x8 res[32 / RI];
+#pragma unroll
+        for (int i = 0; i < 32 / RI; ++i) {
+          const int64_t m = mj + TM * RI * i;
+          res[i] = m < p.M && n < p.N ? *reinterpret_cast<const bf16x8*>(p.residual + m * p.ldr + n) : bf16x8{};
+        }
+#pragma unroll
+        for (int t = 0; t < TN; ++t) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<f32x4*>(sh + c * LD + 32 * t + 16 * (u & 1) + 8 * h + 4 * (u >> 1)) =
+                f32x4{acc[t][j][4 * u], acc[t][j][4 * u + 1], acc[t][j][4 * u + 2], acc[t][j][4 * u + 3]};
+        }
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 32 / RI; ++i) {
+          const int64_t m = mj + TM * RI * i;
+          const float* from = sh + (i * RI + lane / PR) * LD + 8 * piece;
+          const f32x4 a = *reinterpret_cast<const f32x4*>(from), d = *reinterpret_cast<const f32x4*>(from + 4);
+          bf16x8 o;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            o[e] = (bf16)(a[e] + bias[e] + (float)res[i][e]);
+            o[4 + e] = (bf16)(d[e] + bias[4 + e] + (float)res[i][4 + e]);
+          }
+          if (m < p.M && n < p.N) *reinterpret_cast<bf16x8*>(p.y + m * p.ldy + n) = o;
+        }
+        wave_sync();
+      }
+      return;
+    }
     constexpr int W = 32 * TN, LD = W + 8, PR = W / 8, RI = 64 / PR;   // pieces a row, rows at once
     bf16* sb = reinterpret_cast<bf16*>(sh);
     const int n0 = 64 * grp0, piece = lane % PR, n = n0 + 8 * piece;
@@ -572,7 +616,7 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
     if (s + 3 >= S) break;
   }
   vm_wait_all();   // no load may reach LDS behind the workgroup's end
-  const bool plain = (p.vec & 1) && p.act == kActNone && !p.residual && p.N % 8 == 0;
+  const bool plain = (p.vec & 1) && p.act == kActNone && p.N % 8 == 0;
   if (!GATED) __syncthreads();
   finish_tile<TN, TM, GATED>(p, acc, (tile0 + 2 * TN * wn) / 4, m0 + 32 * TM * wm, plain, lane,
                              reinterpret_cast<float*>(lds) + wave * (kShare / 4));
@@ -597,9 +641,17 @@ template <bool GATED>
 static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED>(p, s);
   if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED>(p, s);
-  if (p.M <= 16) return launch_few<1, kRows8, GATED>(p, s);
-  if (p.M <= 256) return launch_few<2, kRows8, GATED>(p, s);
-  launch_many<4, 1, 2, 4, GATED>(p, s);
+  // By the workgroups that each form makes, of 256 CUs. Few rows go to the streaming form, 16 and 32 rows
+  // to a workgroup, as long as a CU has one, or two, of them; then come tiles of 128 x 64, 256 x 64 and
+  // 256 x 128 outputs x rows, each while the CUs have one of them. us of (16, 32 rows, the three tiles):
+  // 64 x 1024 x 4480 4.5, 4.4, 6.0, 7.7, 10.6; 256 rows 8.6, 7.9, 6.3, 8.0, 11; 1024 rows 25, 19, 13.2, 12.8, 12.2;
+  // 256 x 4096 x 4096 17, 14, 16, 21, 31; 1024 rows 62, 48, 28, 27, 35; 2048 rows 121, 91, 56, 45, 39.
+  const int64_t g64 = p.NP / 64, g128 = (p.NP + 127) / 128, g256 = (p.NP + 255) / 256, r64 = (p.M + 63) / 64;
+  if (g64 * ((p.M + 15) / 16) <= 256) launch_few<1, kRows8, GATED>(p, s);
+  else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED>(p, s);
+  else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED>(p, s);
+  else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED>(p, s);
+  else launch_many<4, 1, 2, 4, GATED>(p, s);
 }
 
 }  // namespace m3s
