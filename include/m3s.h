@@ -719,9 +719,12 @@ int32_t m3s_distill_bwd(const m3s_distill_args* args, void* stream);
 /* Rows in 8 bits, for products on the matrix cores' block-scaled form; no counterpart in the
  * reference. e4m3 values in blocks of 32 along a row, each with a scale 2^e, e the smallest integer
  * >= -126 with the block's largest finite magnitude times 2^-e at most 448; a value is rounded to
- * nearest (ties to even), and an entry that is not finite becomes NaN. values is (rows, kp) bytes,
- * kp the width rounded up to 128 and zeros behind the width; scales (kp / 32, mp) bytes of
- * e + 127, mp the rows rounded up to 16. values 16-byte aligned, scales 4-byte. */
+ * nearest (ties to even), and an entry that is not finite becomes NaN. values holds a tile of 2048
+ * bytes for every 16 rows and every 128 k, row tiles outermost (kp the width rounded up to 128, zeros
+ * behind the width): two planes (k 0-63, 64-127) of 64 lanes' 16 bytes, lane 16 g + r holding row r's
+ * k 16 g .. 16 g + 15 of the plane. scales is (kp / 32, mp) bytes of e + 127, mp the rows rounded up to
+ * 128; of 128 rows, row 32 j + c's is the 4 c + j-th. Rows behind the last may hold anything. values 16-byte
+ * aligned, scales 4-byte. */
 #define M3S_DTYPE_ROWS8 2              /* of m3s_matmul8_args.x_dtype alone */
 #define M3S_ROWS8_MAX 16777215         /* rows: 2^24 - 1 */
 #define M3S_ROWS8_WIDTH_MAX 1048576    /* width: 2^20; with a norm 16384 */
@@ -742,7 +745,7 @@ typedef struct m3s_rows8_args {
   int64_t ldadd;
   const float* gain;    /* (width), or NULL: no norm */
   void* sum;            /* out (rows, width) dense, iff add */
-  void* values;         /* out (rows, kp) */
+  void* values;         /* out, packed */
   void* scales;         /* out (kp / 32, mp) */
 } m3s_rows8_args;
 int32_t m3s_rows8(const m3s_rows8_args* args, void* stream);
@@ -763,9 +766,8 @@ int32_t m3s_rows8_values(const m3s_rows8_values_args* args, void* stream);
  * y (rows, n) bf16 = act(x w + bias) + residual. Gated: w has 2 n columns, value | gate, and
  * value silu(gate) goes out as rows in 8 bits. x in 8 bits, or up to M3S_MATMUL8_FLOAT_ROWS rows in
  * bf16 or float32, rounded to 8 bits on the way.
- * w is packed: for every 16-row tile of its outputs and every 128 k, two planes (k 0-63, 64-127) of
- * 64 lanes' 16 bytes, lane 16 g + r holding row r's k 16 g .. 16 g + 15 of the plane; w_scales a
- * dword for every 128 k, group of four tiles and lane 16 g + r: the tiles' scales of row r's block g.
+ * w is packed as rows are, each of its outputs a row; w_scales a dword for every 128 k, group of four
+ * 16-row tiles and lane 16 g + r: the tiles' scales of row r's block g.
  * Packed row 64 q + 16 t + 4 g + i is output 64 q + 32 (t >> 1) + 8 g +
  * 4 (t & 1) + i, n rounded up to 64 of them; gated, it is output 32 q + 8 g + 4 (t & 1) + i of value
  * (t < 2) or gate, with n rounded up to 128. Rows behind n are zeros. */
@@ -777,7 +779,7 @@ typedef struct m3s_matmul8_args {
   int32_t gated;
   int32_t activation;   /* M3S_ACT_*: gelu is the one with erf; none with a gate */
   int64_t rows;
-  const void* x;        /* (rows, kp) values, or (rows, k) with ldx elements from row to row */
+  const void* x;        /* packed values, or (rows, k) with ldx elements from row to row */
   int64_t ldx;          /* float rows */
   const void* x_scales;
   const void* w;
@@ -787,7 +789,7 @@ typedef struct m3s_matmul8_args {
   int64_t ldres;
   void* y;              /* out (rows, n) bf16, or NULL with a gate */
   int64_t ldy;          /* elements from one row of y to the next, at least n */
-  void* y_values;       /* gated: out (rows, n rounded up to 128) */
+  void* y_values;       /* gated: out, packed */
   void* y_scales;
 } m3s_matmul8_args;
 int32_t m3s_matmul8(const m3s_matmul8_args* args, void* stream);

@@ -10,10 +10,13 @@
 // non-finite entry becomes e4m3's NaN and does not count for the maximum: its row's products are
 // NaN, as they would be in floating point, and its block's other values keep their scale.
 //
-// Layout: values (rows, kp) bytes with kp the width rounded up to 128 (zeros behind the width), the
-// K of one matrix instruction, and scales (kp / 32, mp) bytes with mp the rows rounded up to 16: a
-// block's scales of four rows are one dword, which the products' lanes read at once and pick
-// their byte of by the instruction's own selector. Nothing writes the scales behind the last row.
+// Layout, of rows and of packed weights alike: 16 rows and 128 k are a tile of 2048 bytes, two planes of
+// 64 k, in each 16 bytes for every one of 64 lanes: lane 16 g + r holds row r's k 16 g .. 16 g + 15. A
+// wave's load is 1 KB in one piece; from rows that lie one behind the other it takes 64 bytes of each of
+// 16, twice the lines for the address unit, which bounded the products (8192^3: 429 us, so 392). Scales
+// are (kp / 32, mp) bytes, mp the rows rounded up to 128: of 128 rows, row 32 j + c's byte is the 4 c + j-th, so
+// that a lane's four row tiles are one dword, of which the instruction's own selector picks a byte.
+// Nothing is written for rows behind the last, or read from there into a result.
 #pragma once
 
 #include "m3s_common.h"
@@ -23,8 +26,16 @@ namespace m3s {
 constexpr int kBlock8 = 32;    // values to a scale
 constexpr int kStep8 = 128;    // K of one v_mfma_scale_f32_16x16x128_f8f6f4
 
-__host__ __device__ inline int64_t padded16(int64_t rows) { return (rows + 15) & ~(int64_t)15; }
+__host__ __device__ inline int64_t padded_rows(int64_t rows) { return (rows + 127) & ~(int64_t)127; }
 inline int64_t padded8(int64_t width) { return (width + kStep8 - 1) / kStep8 * kStep8; }
+
+// Where row r's scales stand in a block's, and the byte of its k (a multiple of 8: 8 bytes lie together)
+__device__ __forceinline__ int64_t scale_at(int64_t r) {
+  return (r & ~(int64_t)127) + 4 * (r & 31) + ((r >> 5) & 3);
+}
+__device__ __forceinline__ int64_t value_at(int64_t r, int k, int steps) {
+  return ((r >> 4) * steps + (k >> 7)) * 2048 + ((k >> 6) & 1) * 1024 + (((k >> 4) & 3) * 16 + (r & 15)) * 16 + (k & 15);
+}
 
 typedef int i32x2_ __attribute__((ext_vector_type(2)));
 typedef int i32x4_ __attribute__((ext_vector_type(4)));

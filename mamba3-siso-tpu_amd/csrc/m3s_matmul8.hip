@@ -18,8 +18,7 @@
 // leave in bf16 or 8 bits. The float32 route, e4m3 widened to bf16 and multiplied at half the rate,
 // would sum in full and round its operands no better.
 //
-// Weights are packed once (eightbit.pack8): 16-row tiles of 2048 bytes a step, as two planes of 16
-// bytes a lane, so that a wave's load is 1 KB in one piece, straight to registers or LDS. Four
+// Weights are packed once (eightbit.pack8) in the rows' own tiles, their outputs being the rows. Four
 // tiles are a group of 64 outputs: tile t, row 4 g + i is output 64 grp + 32 (t >> 1) + 8 g +
 // 4 (t & 1) + i, which leaves a lane 8 neighbouring outputs (16 bytes of bf16) in two tiles, and four
 // lanes the 32 of a block. With a gate, tiles 0 and 1 hold value's outputs 32 grp + 8 g + 4 t + i and
@@ -35,14 +34,14 @@ namespace m3s {
 enum Act8 { kActNone = M3S_ACT_NONE, kActSilu = M3S_ACT_SILU, kActGelu = M3S_ACT_GELU, kActRelu = M3S_ACT_RELU };
 
 struct M8Params {
-  const void* x;           // (M, kp) e4m3, or (M, K) bf16 / float32 for few rows
+  const void* x;           // packed tiles, or (M, K) bf16 / float32 for few rows
   const uint8_t* xs;       // (4 KB, mp)
-  const uint8_t* w;        // [n tile][step][2][lane][16]
+  const uint8_t* w;        // packed tiles
   const uint8_t* ws;       // [step][group of four tiles][lane][4]
   const float* bias;
   const bf16* residual;
   bf16* y;
-  uint8_t* yv;             // gated: (M, op) values and (op / 32, mp) scales
+  uint8_t* yv;             // gated: packed values and (4 steps, mp) scales
   uint8_t* ys;
   int64_t M, mp, ldx, ldr, ldy;
   int K, KB, N, NP, act, vec;   // N: outputs (half the weight's columns with a gate); NP: packed rows
@@ -144,10 +143,9 @@ __device__ __forceinline__ void finish_group(const M8Params& p, int64_t m, int g
     if (u >= kInfBits) u = max_lanes16(max_bits_finite(v));
     const int byte = scale_byte(u);
     const float down = scale_down(byte);
-    const int64_t op = (int64_t)(p.NP / 256) * kStep8;
-    *reinterpret_cast<i32x2_*>(p.yv + m * op + j) =
+    *reinterpret_cast<i32x2_*>(p.yv + value_at(m, j, p.NP / 256)) =
         i32x2_{pack4(v[0], v[1], v[2], v[3], down), pack4(v[4], v[5], v[6], v[7], down)};
-    if (g == 0) p.ys[(int64_t)grp * p.mp + m] = (uint8_t)byte;
+    if (g == 0) p.ys[(int64_t)grp * p.mp + scale_at(m)] = (uint8_t)byte;
   }
 }
 
@@ -187,10 +185,11 @@ __device__ __forceinline__ void rows_operand(const M8Params& p, int64_t m0, int 
   const int r = lane & 15, g = lane >> 4;
   const int64_t m = m0 + r;
   if constexpr (XK == kRows8) {
-    const int64_t mc = m < p.M ? m : p.M - 1;
-    const uint8_t* xr = static_cast<const uint8_t*>(p.x) + mc * ((int64_t)p.KB * kStep8) + kb * kStep8 + 16 * g;
-    b = join8(*reinterpret_cast<const i32x4_*>(xr), *reinterpret_cast<const i32x4_*>(xr + 64));
-    sb = p.xs[((int64_t)kb * 4 + g) * p.mp + mc];
+    // rows behind the last give nothing but their own products, which are not stored
+    const int64_t tile = min(m0, p.M - 1) >> 4;
+    const uint8_t* xr = static_cast<const uint8_t*>(p.x) + (tile * p.KB + kb) * 2048 + 16 * lane;
+    b = join8(*reinterpret_cast<const i32x4_*>(xr), *reinterpret_cast<const i32x4_*>(xr + 1024));
+    sb = p.xs[((int64_t)kb * 4 + g) * p.mp + scale_at(m)];
   } else {
     using TX = std::conditional_t<XK == kRowsBf16, bf16, float>;
     int q[8], byte[2];
@@ -309,13 +308,11 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
 // registers. Two workgroups share a CU, so that one's loads, outputs and gates run under the
 // other's products: with one of 256 x 256 outputs there they stood in line (16384 x 1024 x 4480:
 // 104 us, of them 31 for the outputs and some 25 until a tile's first products).
-// Row tile j holds rows TM c + j of the wave's, so that a lane's scales of a step lie together.
-constexpr int kStage8 = 64;    // k of a stage
 constexpr int kBand = 16;
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // A wave's accumulators: group q's tile T and row tile j; element 4 u + e of lane (c, h) is row
-// TM c + j and output 64 q + 32 T + 16 (u & 1) + 8 h + 4 (u >> 1) + e (gated: 32 q + ... of value or gate).
+// 32 j + c and output 64 q + 32 T + 16 (u & 1) + 8 h + 4 (u >> 1) + e (gated: 32 q + ... of value or gate).
 template <int TN, int TM, bool GATED>
 __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&acc)[TN][TM], int grp0,
                                             int64_t row0, bool plain, int lane, float* sh) {
@@ -323,7 +320,7 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
   if constexpr (GATED) {
 #pragma unroll
     for (int j = 0; j < TM; ++j) {
-      const int64_t m = row0 + TM * c + j;
+      const int64_t m = row0 + 32 * j + c;
 #pragma unroll
       for (int q = 0; q < TN / 2; ++q) {
         const int grp = grp0 + q;
@@ -354,11 +351,11 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
           }
           const int byte = scale_byte(u);
           const float down = scale_down(byte);
-          uint8_t* out = p.yv + m * ((int64_t)(p.NP / 256) * kStep8) + 32 * grp + 8 * h;
+          uint8_t* out = p.yv + value_at(m, 32 * grp + 8 * h, p.NP / 256);
           *reinterpret_cast<i32x2_*>(out) = i32x2_{pack4(v[0], v[1], v[2], v[3], down), pack4(v[4], v[5], v[6], v[7], down)};
-          *reinterpret_cast<i32x2_*>(out + 16) =
+          *reinterpret_cast<i32x2_*>(out + 256) =   // 16 k on
               i32x2_{pack4(v[8], v[9], v[10], v[11], down), pack4(v[12], v[13], v[14], v[15], down)};
-          if (h == 0) p.ys[(int64_t)grp * p.mp + m] = (uint8_t)byte;
+          if (h == 0) p.ys[(int64_t)grp * p.mp + scale_at(m)] = (uint8_t)byte;
         }
       }
     }
@@ -378,11 +375,11 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
       }
 #pragma unroll
       for (int j = 0; j < TM; ++j) {
-        const int64_t mj = row0 + j + (int64_t)TM * (lane / PR);
+        const int64_t mj = row0 + 32 * j + lane / PR;
         bf16x8 res[32 / RI];
 #pragma unroll
         for (int i = 0; i < 32 / RI; ++i) {
-          const int64_t m = mj + TM * RI * i;
+          const int64_t m = mj + RI * i;
           res[i] = m < p.M && n < p.N ? *reinterpret_cast<const bf16x8*>(p.residual + m * p.ldr + n) : bf16x8{};
         }
 #pragma unroll
@@ -395,7 +392,7 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
         wave_sync();
 #pragma unroll
         for (int i = 0; i < 32 / RI; ++i) {
-          const int64_t m = mj + TM * RI * i;
+          const int64_t m = mj + RI * i;
           const float* from = sh + (i * RI + lane / PR) * LD + 8 * piece;
           const f32x4 a = *reinterpret_cast<const f32x4*>(from), d = *reinterpret_cast<const f32x4*>(from + 4);
           bf16x8 o;
@@ -436,12 +433,12 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
         }
       }
       wave_sync();
-      const int64_t mj = row0 + j + (int64_t)TM * (lane / PR);
+      const int64_t mj = row0 + 32 * j + lane / PR;
       bf16* yr = p.y + mj * p.ldy + n;
 #pragma unroll
       for (int i = 0; i < 32 / RI; ++i) {
         const bf16x8 o = *reinterpret_cast<const bf16x8*>(sb + (i * RI + lane / PR) * LD + 8 * piece);
-        if (mj + TM * RI * i < p.M && n < p.N) *reinterpret_cast<bf16x8*>(yr + (int64_t)(TM * RI * i) * p.ldy) = o;
+        if (mj + RI * i < p.M && n < p.N) *reinterpret_cast<bf16x8*>(yr + (int64_t)(RI * i) * p.ldy) = o;
       }
       wave_sync();
     }
@@ -460,23 +457,23 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
               f32x4{acc[t][j][4 * u], acc[t][j][4 * u + 1], acc[t][j][4 * u + 2], acc[t][j][4 * u + 3]};
       }
       wave_sync();
-      const int64_t mj = row0 + j;
+      const int64_t mj = row0 + 32 * j;
       if (p.vec & 1) {
 #pragma unroll 1
         for (int e = lane; e < 32 * (W / 8); e += 64) {
           const int row = e / (W / 8), n = 8 * (e % (W / 8));
-          if (mj + TM * row < p.M) {
+          if (mj + row < p.M) {
             const f32x4 a = *reinterpret_cast<const f32x4*>(sh + row * LD + n);
             const f32x4 d = *reinterpret_cast<const f32x4*>(sh + row * LD + n + 4);
             float v[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
-            finish8<false>(p, mj + TM * row, n0 + n, v);
+            finish8<false>(p, mj + row, n0 + n, v);
           }
         }
       } else {
 #pragma unroll 1
         for (int e = lane; e < 32 * W; e += 64) {
           const int row = e / W, n = n0 + e % W;
-          const int64_t m = mj + TM * row;
+          const int64_t m = mj + row;
           if (m < p.M && n < p.N) {
             float v = sh[row * LD + e % W];
             if (p.bias) v += p.bias[n];
@@ -512,24 +509,18 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
   const int at = lin - band * kBand * p.tiles_n;
   const int ntiles = p.NP / 16, tile0 = at / high * NTL;
   const int64_t m0 = (int64_t)(band * kBand + at % high) * (16 * MTL);
-  const int64_t kp = (int64_t)p.KB * kStep8;
   const uint32_t wstep = (uint32_t)p.KB * 2048;
   const uint8_t* wbase = p.w + (int64_t)tile0 * wstep;
-  const uint8_t* xbase = static_cast<const uint8_t*>(p.x) + m0 * kp;
+  const uint8_t* xbase = static_cast<const uint8_t*>(p.x) + (m0 >> 4) * wstep;
   const int S = 2 * p.KB;
   const int wn = wave % WN, wm = wave / WN, c = lane & 31, h = lane >> 5;
-  // A tile behind the last, and a row behind the last, reads the last one instead; neither is stored.
-  // Tile t's row r is row TM c + j of its wave's 32 TM, with 32 j + c = 16 (t % (2 TM)) + r.
+  const int rtiles = (int)min((p.M - m0 + 15) >> 4, (int64_t)MTL);
+  // a tile behind the last reads the last one instead, and is not stored
   uint32_t ow[LN], ox[LM];
 #pragma unroll
   for (int i = 0; i < LN; ++i) ow[i] = (uint32_t)min(wave * LN + i, ntiles - 1 - tile0) * wstep + 16 * lane;
 #pragma unroll
-  for (int i = 0; i < LM; ++i) {
-    const int t = wave * LM + i, tw = t % (2 * TM);
-    const int64_t row = min((int64_t)(32 * TM * (t / (2 * TM)) + TM * (16 * (tw & 1) + (lane & 15)) + (tw >> 1)),
-                            p.M - 1 - m0);
-    ox[i] = (uint32_t)(row * kp) + 16 * (lane >> 4);
-  }
+  for (int i = 0; i < LM; ++i) ox[i] = (uint32_t)min(wave * LM + i, rtiles - 1) * wstep + 16 * lane;
   // behind the last step the loads go through empty descriptors and touch no memory
   auto load = [&](int stage, int s) {
     s = __builtin_amdgcn_readfirstlane(s);
@@ -539,11 +530,12 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
 #pragma unroll
     for (int i = 0; i < LN; ++i) buf_load_lds16(rw, to + (wave * LN + i) * 1024, ow[i], (uint32_t)s * 1024);
 #pragma unroll
-    for (int i = 0; i < LM; ++i) buf_load_lds16(rx, to + (NTL + wave * LM + i) * 1024, ox[i], (uint32_t)s * kStage8);
+    for (int i = 0; i < LM; ++i) buf_load_lds16(rx, to + (NTL + wave * LM + i) * 1024, ox[i], (uint32_t)s * 1024);
   };
   // group q's dword holds its four 16-row tiles' scales of a row; bit 4 of the lane picks the tile of a pair
   const uint32_t osw = (uint32_t)(16 * tile0 + 32 * TN * wn) * 4 + 4 * (16 * h + (lane & 15));
-  const uint32_t osx = (uint32_t)((int64_t)h * p.mp + m0 + 32 * TM * wm + (TM * c & ~3));
+  const int64_t mw = m0 + 32 * TM * wm;   // the wave's rows
+  const uint32_t osx = (uint32_t)((int64_t)h * p.mp + (mw & ~(int64_t)127) + 4 * c);
   auto scales = [&](int s, int (&sw)[TN / 2], int& sx) {
     s = __builtin_amdgcn_readfirstlane(s);
     const __amdgpu_buffer_rsrc_t rws = make_rsrc(p.ws, s < S ? (uint32_t)((int64_t)p.KB * p.NP * 4) : 0u);
@@ -578,7 +570,7 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
     i32x8_ b[TM];
 #pragma unroll
     for (int j = 0; j < TM; ++j) b[j] = frag(NTL / 2 + wm * TM + j);
-    const int by = 8 * (c >> 4), sr = (int)((uint32_t)sx[R] >> (8 * (TM * c & 3)));
+    const int by = 8 * (c >> 4), sr = (int)((uint32_t)sx[R] >> (8 * ((int)(mw >> 5) & 3)));
 #pragma unroll
     for (int q = 0; q < TN / 2; ++q) {
       const int s4 = (int)((uint32_t)sw[R][q] >> by);
@@ -622,6 +614,375 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
                              reinterpret_cast<float*>(lds) + wave * (kShare / 4));
 }
 
+// ---- more rows than the CUs hold at once ------------------------------------------------------
+// One workgroup of eight waves on each CU, 256 outputs x 256 rows at a time, a wave 64 x 128 of them; it
+// stays for its share of the tiles. Its loads run three steps of 64 k ahead of the products through a ring
+// of three stages, and on into the next tile while this one's outputs leave; a step's operands are
+// read into registers under the products of the step before, so that a barrier a step costs the matrix
+// units nothing but the waves' differences. Scales come to LDS as the operands do.
+constexpr int kBigWaves = 8, kBigSide = 256;
+constexpr int kBigOps = 5;                       // loads of a step: two tiles of either operand, and scales
+constexpr int kBigScales = 32 * 1024;            // in a stage, behind the 32 planes: weight 1 KB, rows 512 B,
+constexpr int kBigStage = kBigScales + 2048;     // and as much that nothing reads
+constexpr int kBigTurn = 32 * (64 + 8) * 2;      // a wave's 32 rows of 64 bf16
+constexpr int kCus = 256;
+
+template <int n>
+__device__ __forceinline__ void vm_wait_to() {   // vmcnt(n), n < 64
+  __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | (n >> 4) << 14);
+}
+
+struct BigTile {
+  int tile0;      // first packed tile of 16
+  int64_t m0;     // first row
+};
+
+__device__ __forceinline__ BigTile big_tile(const M8Params& p, int lin) {
+  constexpr int kHigh = 8;
+  const int band = lin / (kHigh * p.tiles_n), high = min(kHigh, p.tiles_m - band * kHigh);
+  const int at = lin - band * kHigh * p.tiles_n;
+  return {__builtin_amdgcn_readfirstlane(at / high) * (kBigSide / 16),
+          (int64_t)__builtin_amdgcn_readfirstlane(band * kHigh + at % high) * kBigSide};
+}
+
+// A wave's 64 x 128 accumulators: tiles T = 0, 1 of its group and row tiles j; element 4 u + e of lane (c, h) is
+// row row0 + 32 j + c and output 64 grp + 32 T + 16 (u & 1) + 8 h + 4 (u >> 1) + e.
+__device__ __forceinline__ void finish_big(const M8Params& p, const f32x16 (&acc)[2][4], int grp, int64_t row0,
+                                           int lane, uint8_t* turn) {
+  constexpr int LD = 64 + 8;
+  bf16* sb = reinterpret_cast<bf16*>(turn);
+  const int c = lane & 31, h = lane >> 5, piece = lane & 7, rl = lane >> 3;
+  const int n0 = 64 * grp, n = n0 + 8 * piece;
+  if ((p.vec & 1) && p.act == kActNone && p.N % 8 == 0) {
+    if (n0 >= p.N) return;
+    const bool whole = row0 + 128 <= p.M && n0 + 64 <= p.N;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t mj = row0 + 32 * j + rl;
+      if (p.residual) {   // its rows turned into the accumulators' order
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int64_t m = mj + 8 * i;
+          *reinterpret_cast<bf16x8*>(sb + (8 * i + rl) * LD + 8 * piece) =
+              m < p.M && n < p.N ? *reinterpret_cast<const bf16x8*>(p.residual + m * p.ldr + n) : bf16x8{};
+        }
+        wave_sync();
+      }
+      bf16x8 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {   // outputs 32 T + 16 k + 8 h .., i = 2 T + k
+        const int at = 16 * i + 8 * h;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = acc[i >> 1][j][8 * (e >> 2) + 4 * (i & 1) + (e & 3)];
+        if (p.bias && n0 + at < p.N) {
+          const f32x4 a = *reinterpret_cast<const f32x4*>(p.bias + n0 + at);
+          const f32x4 d = *reinterpret_cast<const f32x4*>(p.bias + n0 + at + 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) { v[e] += a[e]; v[4 + e] += d[e]; }
+        }
+        if (p.residual) {
+          const bf16x8 r = *reinterpret_cast<const bf16x8*>(sb + c * LD + at);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += (float)r[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[i][e] = (bf16)v[e];
+      }
+      if (p.residual) wave_sync();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16x8*>(sb + c * LD + 16 * i + 8 * h) = o[i];
+      wave_sync();
+      bf16* yr = p.y + mj * p.ldy + n;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const bf16x8*>(sb + (8 * i + rl) * LD + 8 * piece);
+      if (whole) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16x8*>(yr + (int64_t)(8 * i) * p.ldy) = o[i];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (mj + 8 * i < p.M && n < p.N) *reinterpret_cast<bf16x8*>(yr + (int64_t)(8 * i) * p.ldy) = o[i];
+      }
+      wave_sync();
+    }
+    return;
+  }
+  // odd widths and activations: 16 rows at a time in float32, one loop each
+  constexpr int LF = 64 + 4;
+  static_assert(16 * LF * 4 <= kBigTurn, "16 rows of float32 fit");
+  float* sf = reinterpret_cast<float*>(turn);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if ((c >> 4) == half) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            *reinterpret_cast<f32x4*>(sf + (c & 15) * LF + 32 * t + 16 * (u & 1) + 8 * h + 4 * (u >> 1)) =
+                f32x4{acc[t][j][4 * u], acc[t][j][4 * u + 1], acc[t][j][4 * u + 2], acc[t][j][4 * u + 3]};
+        }
+      }
+      wave_sync();
+      const int64_t mj = row0 + 32 * j + 16 * half;
+      if (p.vec & 1) {
+#pragma unroll 1
+        for (int e = rl; e < 16; e += 8) {
+          if (mj + e < p.M) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(sf + e * LF + 8 * piece);
+            const f32x4 d = *reinterpret_cast<const f32x4*>(sf + e * LF + 8 * piece + 4);
+            float v[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
+            finish8<false>(p, mj + e, n, v);
+          }
+        }
+      } else {
+#pragma unroll 1
+        for (int e = 0; e < 16; ++e) {
+          const int64_t m = mj + e;
+          if (m < p.M && n0 + lane < p.N) {
+            float v = sf[e * LF + lane];
+            if (p.bias) v += p.bias[n0 + lane];
+            v = act8(v, p.act);
+            if (p.residual) v += (float)p.residual[m * p.ldr + n0 + lane];
+            p.y[m * p.ldy + n0 + lane] = (bf16)v;
+          }
+        }
+      }
+      wave_sync();
+    }
+  }
+}
+
+// The same of a gate: tile 0 is value's, tile 1 gate's 32 outputs of block grp.
+__device__ __forceinline__ void finish_big_gate(const M8Params& p, const f32x16 (&acc)[2][4], int grp, int64_t row0,
+                                                int lane) {
+  const int c = lane & 31, h = lane >> 5;
+  if (grp >= p.NP / 64 || row0 >= p.M) return;
+  uint8_t* out = p.yv + value_at(row0 + c, 32 * grp + 8 * h, p.NP / 256);
+  uint32_t bytes = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {   // i: 8 outputs from 8 h, then 8 from 16 + 8 h
+      const int e = 8 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
+      float a = acc[0][j][e], b = acc[1][j][e];
+      if (p.bias) {
+        const int n = min(32 * grp + 16 * (i >> 3) + 8 * h + (i & 7), p.N - 1);
+        a += p.bias[n];
+        b += p.bias[p.N + n];
+      }
+      v[i] = a * silu8(b);
+    }
+    if (32 * grp + 32 > p.N) {   // zeros behind the width
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (32 * grp + 16 * (i >> 3) + 8 * h + (i & 7) >= p.N) v[i] = 0.f;
+    }
+    uint32_t u = max_bits(v), o = (uint32_t)__shfl_xor((int)u, 32, 64);
+    u = u > o ? u : o;
+    if (u >= kInfBits) {   // both lanes of a row
+      u = max_bits_finite(v);
+      o = (uint32_t)__shfl_xor((int)u, 32, 64);
+      u = u > o ? u : o;
+    }
+    const int byte = scale_byte(u);
+    const float down = scale_down(byte);
+    bytes |= (uint32_t)byte << (8 * j);
+    // the row tile's two tiles of 16, 256 bytes in a piece
+    if (row0 + 32 * j + c < p.M) {
+      uint8_t* to = out + (int64_t)j * 2 * (p.NP / 256) * 2048;
+      *reinterpret_cast<i32x2_*>(to) = i32x2_{pack4(v[0], v[1], v[2], v[3], down), pack4(v[4], v[5], v[6], v[7], down)};
+      *reinterpret_cast<i32x2_*>(to + 256) =   // 16 k on
+          i32x2_{pack4(v[8], v[9], v[10], v[11], down), pack4(v[12], v[13], v[14], v[15], down)};
+    }
+  }
+  // four rows' scales in one dword; those of rows behind the last are anything
+  if (h == 0) *reinterpret_cast<uint32_t*>(p.ys + (int64_t)grp * p.mp + row0 + 4 * c) = bytes;
+}
+
+template <bool GATED>
+__global__ void __launch_bounds__(64 * kBigWaves) matmul8_big_kernel(const M8Params p) {
+  __shared__ __attribute__((aligned(16))) uint8_t lds[3 * kBigStage + (GATED ? 0 : kBigWaves * kBigTurn)];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wave & 3, wm = wave >> 2, c = lane & 31, h = lane >> 5;
+  // An XCD's workgroups take consecutive tiles, eight row tiles high and walked along the outputs: the 32
+  // at work at a time read some 8 strips of rows and 4 of the weight through their L2.
+  const int nb = p.tiles_m * p.tiles_n, per = (nb + 7) >> 3, stride = (int)(gridDim.x >> 3);
+  const int first = (blockIdx.x & 7) * per, last = min(first + per, nb);
+  int lin = first + (int)(blockIdx.x >> 3);
+  if (lin >= last) return;
+  const int S = 2 * p.KB, ntiles = p.NP / 16;
+  const uint32_t wstep = (uint32_t)p.KB * 2048;
+  // waves 0 to 3 load the weight's scales (a dword a lane for 128 k), the others the rows' (for 32 k each)
+  const bool of_w = wave < 4;
+  const uint8_t* sbase = of_w ? p.ws : p.xs;
+  const uint32_t sbytes = of_w ? (uint32_t)((int64_t)p.KB * p.NP * 4) : (uint32_t)((int64_t)p.KB * p.mp * 4);
+  const uint32_t sshift = of_w ? 1 : 0, sstep = of_w ? (uint32_t)p.NP * 4 : (uint32_t)p.mp * 2;
+  // where a tile's loads start
+  struct Place {
+    const uint8_t *w, *x;
+    uint32_t ow[2], ox[2], os;
+  };
+  auto place = [&](int at) {
+    const BigTile t = big_tile(p, min(at, last - 1));
+    Place q;
+    q.w = p.w + (int64_t)t.tile0 * wstep;
+    q.x = static_cast<const uint8_t*>(p.x) + (t.m0 >> 4) * wstep;
+    const int rtiles = (int)min((p.M - t.m0 + 15) >> 4, (int64_t)16);
+    // a tile behind the last reads the last one instead, and is not stored
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      q.ow[i] = (uint32_t)min(2 * wave + i, ntiles - 1 - t.tile0) * wstep + 16 * lane;
+      q.ox[i] = (uint32_t)min(2 * wave + i, rtiles - 1) * wstep + 16 * lane;
+    }
+    q.os = of_w ? (uint32_t)(t.tile0 / 4 + wave) * 256 + 4 * lane
+                : (uint32_t)((int64_t)(wave & 1) * p.mp + t.m0 + 4 * lane);
+    return q;
+  };
+  // the step of the loads, three ahead of the products', and whether there is one
+  int ls = 0;
+  bool on = true;
+  Place at = place(lin);
+  auto load = [&](int stage) {
+    const uint32_t bytes = on ? 0xfffffff0u : 0u;
+    const __amdgpu_buffer_rsrc_t rw = make_rsrc(at.w, bytes), rx = make_rsrc(at.x, bytes);
+    const __amdgpu_buffer_rsrc_t rs = make_rsrc(sbase, on ? sbytes : 0u);
+    uint8_t* to = lds + stage;
+    const uint32_t s = __builtin_amdgcn_readfirstlane(ls);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) buf_load_lds16(rw, to + (2 * wave + i) * 1024, at.ow[i], s * 1024);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) buf_load_lds16(rx, to + (16 + 2 * wave + i) * 1024, at.ox[i], s * 1024);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        rs, (__attribute__((address_space(3))) void*)(to + kBigScales + 256 * wave), 4, at.os,
+        __builtin_amdgcn_readfirstlane((s >> sshift) * sstep), 0, 0);
+    ++ls;
+  };
+  struct Operands {
+    i32x8_ a[2], b[4];
+    int sw, sx;
+  };
+  const int lread = (c >> 4) * 1024 + h * 256 + (c & 15) * 16;
+  auto read = [&](int stage, int odd, Operands& o) {
+    const uint8_t* at = lds + stage;
+    auto frag = [&](int tile) {
+      return join8(*reinterpret_cast<const i32x4_*>(at + lread + tile * 2048),
+                   *reinterpret_cast<const i32x4_*>(at + lread + tile * 2048 + 512));
+    };
+    const int* sc = reinterpret_cast<const int*>(at + kBigScales);
+    o.sw = sc[64 * wn + 32 * odd + 16 * h + (c & 15)];
+    o.sx = sc[256 + 64 * h + 32 * wm + c];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) o.a[t] = frag(2 * wn + t);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o.b[j] = frag(8 + 4 * wm + j);
+  };
+  f32x16 acc[2][4];
+  auto products = [&](const Operands& o) {
+    const int s4 = (int)((uint32_t)o.sw >> (8 * (c >> 4)));
+    static_for<4>([&](auto jc) {
+      constexpr int j = decltype(jc)::value;
+      acc[0][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.a[0], o.b[j], acc[0][j], 0, 0, 0, s4, j, o.sx);
+      acc[1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.a[1], o.b[j], acc[1][j], 0, 0, 2, s4, j, o.sx);
+    });
+  };
+  int stage = 0;
+  // Before a step the stage that it reads ahead from is whole: only the loads of the step after that are
+  // still under way. Every wave has read the stage that is filled next.
+  auto open = [&](auto waits) {
+    if constexpr (decltype(waits)::value) __builtin_amdgcn_s_waitcnt(0x0070 | kBigOps);   // vmcnt(kBigOps), lgkmcnt(0)
+    else __builtin_amdgcn_s_waitcnt(0xc07f);                                               // lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // Products first, reads and then loads between them: every wave issues its loads behind the same
+  // barrier, and products that stood behind them would wait for the address unit (8192^3: 459 us, so 428).
+  auto interleave = [&]() {
+    auto group = [&](auto reads, auto loads) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
+      if constexpr (decltype(reads)::value > 0) __builtin_amdgcn_sched_group_barrier(0x100, decltype(reads)::value, 0);
+      if constexpr (decltype(loads)::value > 0) __builtin_amdgcn_sched_group_barrier(0x010, decltype(loads)::value, 0);
+    };
+    const std::integral_constant<int, 0> n0;
+    const std::integral_constant<int, 1> n1;
+    const std::integral_constant<int, 2> n2;
+    const std::integral_constant<int, 4> n4;
+    group(n4, n0);
+    group(n4, n0);
+    group(n4, n0);
+    group(n2, n1);
+    group(n0, n1);
+    group(n0, n1);
+    group(n0, n2);
+    group(n0, n0);
+  };
+  Operands even, odd;
+  Place then;
+  bool again;
+  // Two steps; nothing branches in them (the compiler would move the products past it).
+  auto pair = [&](auto waits) {
+    open(waits);
+    const int filled = stage;
+    stage = stage == 2 * kBigStage ? 0 : stage + kBigStage;
+    read(stage, 1, odd);
+    load(filled);
+    products(even);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+    const bool turn = ls == S;   // after an odd number of loads: S is even, and three were made before
+    ls = turn ? 0 : ls;
+    on = turn ? again : on;
+    at.w = turn ? then.w : at.w;
+    at.x = turn ? then.x : at.x;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      at.ow[i] = turn ? then.ow[i] : at.ow[i];
+      at.ox[i] = turn ? then.ox[i] : at.ox[i];
+    }
+    at.os = turn ? then.os : at.os;
+    open(waits);
+    const int freed = stage;
+    stage = stage == 2 * kBigStage ? 0 : stage + kBigStage;
+    read(stage, 0, even);
+    load(freed);
+    products(odd);
+    interleave();
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  load(0);
+  load(kBigStage);
+  load(2 * kBigStage);
+  vm_wait_all();
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  read(0, 0, even);
+  while (true) {
+    const BigTile t = big_tile(p, lin);
+    then = place(lin + stride);   // where the loads go on behind this tile
+    again = lin + stride < last;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[k][j] = f32x16{};
+    }
+    // The three steps that are loaded need no wait, and one here would be for the outputs of the tile
+    // before, which left behind those loads.
+    pair(std::false_type{});
+    for (int s = 2; s < S; s += 2) pair(std::true_type{});
+    vm_wait_all();   // the next tile's first three steps, before outputs stand behind them
+    const int grp = t.tile0 / 4 + wn;
+    const int64_t row0 = t.m0 + 128 * wm;
+    if constexpr (GATED) finish_big_gate(p, acc, grp, row0, lane);
+    else finish_big(p, acc, grp, row0, lane, lds + 3 * kBigStage + wave * kBigTurn);
+    lin += stride;
+    if (!again) break;
+  }
+  vm_wait_all();   // no load may reach LDS behind the workgroup's end
+}
+
 template <int MT, int XK, bool GATED>
 static void launch_few(const M8Params& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.NP / 64), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
@@ -638,6 +999,13 @@ static void launch_many(M8Params p, hipStream_t s) {
 }
 
 template <bool GATED>
+static void launch_big(M8Params p, hipStream_t s) {
+  p.tiles_n = (p.NP + kBigSide - 1) / kBigSide;
+  p.tiles_m = (int)((p.M + kBigSide - 1) / kBigSide);
+  hipLaunchKernelGGL((matmul8_big_kernel<GATED>), dim3(kCus), dim3(64 * kBigWaves), 0, s, p);
+}
+
+template <bool GATED>
 static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED>(p, s);
   if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED>(p, s);
@@ -651,6 +1019,7 @@ static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED>(p, s);
   else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED>(p, s);
   else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED>(p, s);
+  else if (p.KB >= 2) launch_big<GATED>(p, s);   // its loads are three steps ahead, half a tile at least
   else launch_many<4, 1, 2, 4, GATED>(p, s);
 }
 
@@ -691,7 +1060,7 @@ extern "C" int32_t m3s_matmul8(const m3s_matmul8_args* a, void* stream) {
   p.w = static_cast<const uint8_t*>(a->w); p.ws = static_cast<const uint8_t*>(a->w_scales);
   p.bias = a->bias; p.residual = static_cast<const bf16*>(a->residual); p.y = static_cast<bf16*>(a->y);
   p.yv = static_cast<uint8_t*>(a->y_values); p.ys = static_cast<uint8_t*>(a->y_scales);
-  p.M = a->rows; p.mp = padded16(a->rows); p.ldx = a->ldx; p.ldr = a->ldres; p.ldy = a->ldy;
+  p.M = a->rows; p.mp = padded_rows(a->rows); p.ldx = a->ldx; p.ldr = a->ldres; p.ldy = a->ldy;
   p.K = a->k; p.KB = (int)(padded8(a->k) / kStep8); p.N = a->n; p.act = a->activation;
   p.NP = (int)(a->gated ? 2 * padded8(a->n) : ((int64_t)a->n + 63) / 64 * 64);
   // scales are read through 32-bit offsets, and a launch holds at most 2^31 workgroups' tiles

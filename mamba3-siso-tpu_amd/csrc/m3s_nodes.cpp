@@ -236,9 +236,9 @@ struct Rows {   // rows in 8 bits
 };
 
 Rows fresh_rows(int64_t rows, int64_t width, at::Device device, bool poison) {
-  const int64_t kp = padded(width, 128);
-  return {fresh({rows, kp}, at::kFloat8_e4m3fn, device, poison),
-          fresh({kp / 32, padded(rows, 16)}, at::kFloat8_e8m0fnu, device, poison), rows, width};
+  const int64_t steps = padded(width, 128) / 128;
+  return {fresh({padded(rows, 16) / 16, steps, 2, 64, 16}, at::kFloat8_e4m3fn, device, poison),
+          fresh({4 * steps, padded(rows, 128)}, at::kFloat8_e8m0fnu, device, poison), rows, width};
 }
 
 m3s_rows8_args rows8_args(const Tensor& x, int64_t stride, const Rows& out) {
@@ -284,10 +284,10 @@ bool unwrap_rows(PyObject* o, Rows& r, at::DimVector& lead) {
     if (r.rows > M3S_ROWS8_MAX) return false;
   }
   if (r.width < 1 || r.width > M3S_ROWS8_WIDTH_MAX) return false;
-  const int64_t kp = padded(r.width, 128);
+  const int64_t steps = padded(r.width, 128) / 128;
   if (values->scalar_type() != at::kFloat8_e4m3fn || scales->scalar_type() != at::kFloat8_e8m0fnu ||
-      values->sizes() != at::IntArrayRef({r.rows, kp}) ||
-      scales->sizes() != at::IntArrayRef({kp / 32, padded(r.rows, 16)}) || !values->is_contiguous() ||
+      values->sizes() != at::IntArrayRef({padded(r.rows, 16) / 16, steps, 2, 64, 16}) ||
+      scales->sizes() != at::IntArrayRef({4 * steps, padded(r.rows, 128)}) || !values->is_contiguous() ||
       !scales->is_contiguous())
     return false;
   r.values = *values;

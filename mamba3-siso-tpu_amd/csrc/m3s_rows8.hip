@@ -8,17 +8,17 @@
 //
 // HBM-bound: x and add in, s and the rows out, each once. A lane holds 8 neighbouring columns (one
 // or two 16-byte loads, one 8-byte store), so a block's 32 are four lanes of a quad and its maximum
-// is two DPP steps. A row stays in registers between its sum of squares and its rounding.
+// is two DPP steps. A row stays in registers between its sum of squares and its rounding. A
+// workgroup of 16 waves takes the 16 rows of a tile, so that their 16-byte pieces meet in one L2.
 #include "m3s_eight.h"
 #include "m3s_internal.h"
 
 namespace m3s {
 
-constexpr int kR8Threads = 256;
-constexpr int kR8Waves = kR8Threads / 64;
+constexpr int kR8Waves = 16;
+constexpr int kR8Threads = 64 * kR8Waves;
 constexpr int kR8Pass = 64 * 8;                 // columns a wave takes at once
-constexpr int kR8MaxPieces = 8;
-constexpr int kR8MaxWidth = kR8Waves * kR8Pass * kR8MaxPieces;   // 16384, of a norm
+constexpr int kR8MaxWidth = kR8Waves * kR8Pass * 2;   // 16384, of a norm
 
 struct R8Params {
   const void* x;
@@ -28,7 +28,7 @@ struct R8Params {
   uint8_t* values;
   uint8_t* scales;
   int64_t M, mp, ldx, lda;
-  int D, kp;
+  int D, kp, steps;
   float eps;
 };
 
@@ -81,84 +81,81 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t u) {
   return u > o ? u : o;
 }
 
-// RW waves to a row (1 or 4), NP pieces of 8 columns to a lane; without a norm a workgroup's waves
-// take pieces of the flat (row, column) order instead, and NP is 1.
+// RW waves to a row (1, 4 or 16), NP pieces of 8 columns to a lane; without a norm RW is 1 and the
+// grid's second axis takes the columns.
 template <typename TX, bool NORM, bool ADD, bool VEC, int RW, int NP>
 __global__ void __launch_bounds__(kR8Threads) rows8_kernel(const R8Params p) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t r;
-  int c0;
-  if constexpr (RW == 1) {
-    r = (int64_t)blockIdx.x * kR8Waves + wave;
-    c0 = 8 * lane + (NORM ? 0 : (int)blockIdx.y * kR8Pass * NP);
-    if (r >= p.M) return;   // whole waves; no barrier below in this form
-  } else {
-    r = blockIdx.x;
-    c0 = 8 * threadIdx.x;
-  }
   constexpr int STEP = kR8Pass * RW;
-  const TX* xr = static_cast<const TX*>(p.x) + r * p.ldx;
-  float v[NP][8];
+  const int c0 = 8 * lane + kR8Pass * (wave % RW) + (NORM ? 0 : (int)blockIdx.y * kR8Pass * NP);
+#pragma unroll 1
+  for (int it = 0; it < RW; ++it) {
+    const int64_t r = (int64_t)blockIdx.x * 16 + it * (kR8Waves / RW) + wave / RW;
+    if (RW == 1 && r >= p.M) return;   // whole waves; no barrier below in this form
+    const int D = r < p.M ? p.D : 0;
+    const TX* xr = static_cast<const TX*>(p.x) + r * p.ldx;
+    float v[NP][8];
 #pragma unroll
-  for (int k = 0; k < NP; ++k) load8<TX, VEC>(xr + c0 + k * STEP, p.D - c0 - k * STEP, v[k]);
-  if constexpr (ADD) {
-    const bf16* ar = static_cast<const bf16*>(p.add) + r * p.lda;
-    TX* sr = static_cast<TX*>(p.sum) + r * p.D;
+    for (int k = 0; k < NP; ++k) load8<TX, VEC>(xr + c0 + k * STEP, D - c0 - k * STEP, v[k]);
+    if constexpr (ADD) {
+      const bf16* ar = static_cast<const bf16*>(p.add) + r * p.lda;
+      TX* sr = static_cast<TX*>(p.sum) + r * p.D;
 #pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      float d[8];
-      load8<bf16, VEC>(ar + c0 + k * STEP, p.D - c0 - k * STEP, d);
+      for (int k = 0; k < NP; ++k) {
+        float d[8];
+        load8<bf16, VEC>(ar + c0 + k * STEP, D - c0 - k * STEP, d);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = (float)(TX)(v[k][i] + d[i]);
+        for (int i = 0; i < 8; ++i) v[k][i] = (float)(TX)(v[k][i] + d[i]);
+      }
+#pragma unroll
+      for (int k = 0; k < NP; ++k) store8<TX, VEC>(sr + c0 + k * STEP, D - c0 - k * STEP, v[k]);
     }
-#pragma unroll
-    for (int k = 0; k < NP; ++k) store8<TX, VEC>(sr + c0 + k * STEP, p.D - c0 - k * STEP, v[k]);
-  }
-  if constexpr (NORM) {
-    float ss = 0.f;
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ss += v[k][i] * v[k][i];
-    }
-    ss = wave_total(ss);
-    if constexpr (RW > 1) {
-      __shared__ float part[RW];
-      if (lane == 0) part[wave] = ss;
-      __syncthreads();
-      ss = part[0];
-#pragma unroll
-      for (int w = 1; w < RW; ++w) ss += part[w];
-    }
-    const float rs = 1.f / sqrtf(ss / (float)p.D + p.eps);
-#pragma unroll
-    for (int k = 0; k < NP; ++k) {
-      float g[8];
-      load8<float, VEC>(p.gain + c0 + k * STEP, p.D - c0 - k * STEP, g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * rs * g[i];
-    }
-  }
-  // a column behind the width is a zero, whatever the row's statistics are (zero times the inverse
-  // of a NaN is not)
-#pragma unroll
-  for (int k = 0; k < NP; ++k) {
-    const int c = c0 + k * STEP;
-    if (c >= p.kp) continue;   // whole quads: kp is a multiple of 128
     if constexpr (NORM) {
+      float ss = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (c + i >= p.D) v[k][i] = 0.f;
+      for (int k = 0; k < NP; ++k) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ss += v[k][i] * v[k][i];
+      }
+      ss = wave_total(ss);
+      if constexpr (RW > 1) {
+        __shared__ float part[2][kR8Waves];   // by turns: one barrier a row
+        if (lane == 0) part[it & 1][wave] = ss;
+        __syncthreads();
+        ss = 0.f;
+#pragma unroll
+        for (int w = 0; w < RW; ++w) ss += part[it & 1][wave / RW * RW + w];
+      }
+      const float rs = 1.f / sqrtf(ss / (float)p.D + p.eps);
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        float g[8];
+        load8<float, VEC>(p.gain + c0 + k * STEP, p.D - c0 - k * STEP, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * rs * g[i];
+      }
     }
-    uint32_t u = quad_max(max_bits(v[k]));
-    if (u >= kInfBits) u = quad_max(max_bits_finite(v[k]));   // a quad takes this together
-    const int byte = scale_byte(u);
-    const float down = scale_down(byte);
-    const i32x2_ q = {pack4(v[k][0], v[k][1], v[k][2], v[k][3], down),
-                      pack4(v[k][4], v[k][5], v[k][6], v[k][7], down)};
-    *reinterpret_cast<i32x2_*>(p.values + r * p.kp + c) = q;
-    if ((lane & 3) == 0)
-      p.scales[(int64_t)(c / kBlock8) * p.mp + r] = (uint8_t)byte;
+    if (r >= p.M) continue;
+    // a column behind the width is a zero, whatever the row's statistics are (zero times the inverse
+    // of a NaN is not)
+#pragma unroll
+    for (int k = 0; k < NP; ++k) {
+      const int c = c0 + k * STEP;
+      if (c >= p.kp) continue;   // whole quads: kp is a multiple of 128
+      if constexpr (NORM) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (c + i >= p.D) v[k][i] = 0.f;
+      }
+      uint32_t u = quad_max(max_bits(v[k]));
+      if (u >= kInfBits) u = quad_max(max_bits_finite(v[k]));   // a quad takes this together
+      const int byte = scale_byte(u);
+      const float down = scale_down(byte);
+      const i32x2_ q = {pack4(v[k][0], v[k][1], v[k][2], v[k][3], down),
+                        pack4(v[k][4], v[k][5], v[k][6], v[k][7], down)};
+      *reinterpret_cast<i32x2_*>(p.values + value_at(r, c, p.steps)) = q;
+      if ((lane & 3) == 0) p.scales[(int64_t)(c / kBlock8) * p.mp + scale_at(r)] = (uint8_t)byte;
+    }
   }
 }
 
@@ -167,12 +164,12 @@ template <typename TY, bool VEC>
 __global__ void __launch_bounds__(kR8Threads) rows8_values_kernel(const uint8_t* __restrict__ values,
                                                                   const uint8_t* __restrict__ scales,
                                                                   TY* __restrict__ y, int64_t M, int D,
-                                                                  int kp) {
+                                                                  int steps) {
   const int64_t r = (int64_t)blockIdx.x * kR8Waves + (threadIdx.x >> 6);
   const int c = 8 * (threadIdx.x & 63) + (int)blockIdx.y * kR8Pass;
   if (r >= M || c >= D) return;
-  const i32x2_ q = *reinterpret_cast<const i32x2_*>(values + r * kp + c);
-  const float up = scale_up(scales[(int64_t)(c / kBlock8) * padded16(M) + r]);
+  const i32x2_ q = *reinterpret_cast<const i32x2_*>(values + value_at(r, c, steps));
+  const float up = scale_up(scales[(int64_t)(c / kBlock8) * padded_rows(M) + scale_at(r)]);
   float v[8];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
@@ -186,19 +183,20 @@ __global__ void __launch_bounds__(kR8Threads) rows8_values_kernel(const uint8_t*
 
 template <typename TX, bool NORM, bool ADD, bool VEC>
 static void launch_rows8(const R8Params& p, hipStream_t s) {
-  const unsigned by_wave = (unsigned)((p.M + kR8Waves - 1) / kR8Waves);
-#define M3S_R8(RW, NP, GRID) \
-  hipLaunchKernelGGL((rows8_kernel<TX, NORM, ADD, VEC, RW, NP>), GRID, dim3(kR8Threads), 0, s, p)
+  const unsigned tiles = (unsigned)((p.M + 15) / 16);
+  const unsigned few = 64 * (unsigned)(p.M < 16 ? p.M : 16);   // a wave to a row, and none for rows that are not there
+#define M3S_R8(RW, NP, GRID, THREADS) \
+  hipLaunchKernelGGL((rows8_kernel<TX, NORM, ADD, VEC, RW, NP>), GRID, dim3(THREADS), 0, s, p)
   if constexpr (!NORM) {
-    M3S_R8(1, 1, dim3(by_wave, (unsigned)((p.kp + kR8Pass - 1) / kR8Pass)));
+    M3S_R8(1, 1, dim3(tiles, (unsigned)((p.kp + kR8Pass - 1) / kR8Pass)), few);
   } else {
     const int pieces = (p.kp + kR8Pass - 1) / kR8Pass;
-    if (pieces <= 1) M3S_R8(1, 1, dim3(by_wave));
-    else if (pieces <= 2) M3S_R8(1, 2, dim3(by_wave));
-    else if (pieces <= 4) M3S_R8(1, 4, dim3(by_wave));
-    else if (pieces <= 8) M3S_R8(4, 2, dim3((unsigned)p.M));
-    else if (pieces <= 16) M3S_R8(4, 4, dim3((unsigned)p.M));
-    else M3S_R8(4, 8, dim3((unsigned)p.M));
+    if (pieces <= 1) M3S_R8(1, 1, dim3(tiles), few);
+    else if (pieces <= 2) M3S_R8(1, 2, dim3(tiles), few);
+    else if (pieces <= 4) M3S_R8(1, 4, dim3(tiles), few);
+    else if (pieces <= 8) M3S_R8(4, 2, dim3(tiles), kR8Threads);
+    else if (pieces <= 16) M3S_R8(16, 1, dim3(tiles), kR8Threads);
+    else M3S_R8(16, 2, dim3(tiles), kR8Threads);
   }
 #undef M3S_R8
 }
@@ -237,8 +235,8 @@ extern "C" int32_t m3s_rows8(const m3s_rows8_args* a, void* stream) {
   M3S_REQUIRE(a->ldx >= a->width && (!a->add || a->ldadd >= a->width), "m3s_rows8: a row stride is too short");
   M3S_REQUIRE((uintptr_t)a->values % 16 == 0, "m3s_rows8: values must be 16-byte aligned");
   R8Params p{a->x, a->add, a->gain, a->sum, static_cast<uint8_t*>(a->values),
-             static_cast<uint8_t*>(a->scales), a->rows, padded16(a->rows), a->ldx, a->ldadd, a->width,
-             (int)padded8(a->width), a->eps};
+             static_cast<uint8_t*>(a->scales), a->rows, padded_rows(a->rows), a->ldx, a->ldadd, a->width,
+             (int)padded8(a->width), (int)(padded8(a->width) / kStep8), a->eps};
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (!a->gain) dispatch_rows8<false, false>(a, p, s);
   else if (!a->add) dispatch_rows8<true, false>(a, p, s);
@@ -266,7 +264,7 @@ extern "C" int32_t m3s_rows8_values(const m3s_rows8_values_args* a, void* stream
   const bool vec = a->width % 8 == 0 && (uintptr_t)a->y % 16 == 0;
 #define M3S_R8V(TY, VEC)                                                                          \
   hipLaunchKernelGGL((rows8_values_kernel<TY, VEC>), grid, dim3(kR8Threads), 0, s, v, c,          \
-                     static_cast<TY*>(a->y), a->rows, a->width, kp)
+                     static_cast<TY*>(a->y), a->rows, a->width, kp / kStep8)
   if (a->y_dtype == M3S_DTYPE_BF16) {
     if (vec) M3S_R8V(bf16, true);
     else M3S_R8V(bf16, false);

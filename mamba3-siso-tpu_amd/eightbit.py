@@ -29,17 +29,18 @@ from . import kernels as K
 
 Tensor = torch.Tensor
 
-#: Values that share a scale, and the width that rows are padded to (the K of one matrix instruction).
-BLOCK, STEP = 32, 128
+#: The width that rows are padded to.
+STEP = 128
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "relu": 3}
 _FLOATS = (torch.float32, torch.bfloat16)
 
 
 class Rows8(NamedTuple):
-    """Rows in 8 bits: ``values`` (rows, kp) float8_e4m3fn, kp the ``width`` rounded up to 128 (zeros
-    behind the width); ``scales`` (kp / 32, mp) float8_e8m0fnu, a column for each row, mp the rows
-    rounded up to 16 (nothing behind the last row is written or used); ``lead``, the shape of the
-    leading axes, whose product is ``rows``."""
+    """Rows in 8 bits, as the products read them: ``values`` (tiles, steps, 2, 64, 16) float8_e4m3fn, a tile
+    for 16 rows and a step for 128 of the ``width`` (zeros behind it), whose lane 16 g + r holds 16 values
+    of row r; ``scales`` (4 steps, mp) float8_e8m0fnu, the blocks' scales of each row, mp the rows rounded
+    up to 128 (``csrc/m3s_eight.h`` has the order of both; rows behind the last may hold anything);
+    ``lead``, the shape of the leading axes, whose product is the number of rows."""
 
     values: Tensor
     scales: Tensor
@@ -66,7 +67,7 @@ class Rows8(NamedTuple):
 
 class Weight8(NamedTuple):
     """A projection's weight (k, n) packed for the products (`pack8`): ``values``
-    (tiles, steps, 2, 64, 16) float8_e4m3fn and ``scales`` (steps, tiles / 4, 64, 4) float8_e8m0fnu.
+    (tiles, steps, 2, 64, 16) float8_e4m3fn, as of `Rows8` with the outputs for rows, and ``scales`` (steps, tiles / 4, 64, 4) float8_e8m0fnu.
     ``gated``: its columns are value | gate, n of each."""
 
     values: Tensor
@@ -89,20 +90,23 @@ def _padded(n: int, to: int) -> int:
 
 
 def _check_rows8(x: Rows8, what: str) -> int:
-    rows, kp = 1, _padded(x.width, STEP)
-    for n in x.lead:
-        rows *= n
-    if (tuple(x.values.shape) != (rows, kp) or x.values.dtype != torch.float8_e4m3fn
-            or tuple(x.scales.shape) != (kp // BLOCK, _padded(rows, 16)) or x.scales.dtype != torch.float8_e8m0fnu
+    rows = _count(x.lead)
+    if (tuple(x.values.shape), tuple(x.scales.shape)) != _shapes(rows, x.width) or (
+            x.values.dtype != torch.float8_e4m3fn or x.scales.dtype != torch.float8_e8m0fnu
             or not x.values.is_contiguous() or not x.scales.is_contiguous()):
         raise ValueError(f"{what}: rows must be dense Rows8 of {rows} x {x.width}")
     return rows
 
 
+def _shapes(rows: int, width: int) -> tuple:
+    steps = _padded(width, STEP) // STEP
+    return (_padded(rows, 16) // 16, steps, 2, 64, 16), (4 * steps, _padded(rows, 128))
+
+
 def _new_rows8(lead: tuple, rows: int, width: int, dev) -> Rows8:
-    kp = _padded(width, STEP)
-    return Rows8(K.empty(rows, kp, device=dev, dtype=torch.float8_e4m3fn),
-                 K.empty(kp // BLOCK, _padded(rows, 16), device=dev, dtype=torch.float8_e8m0fnu), width, lead)
+    values, scales = _shapes(rows, width)
+    return Rows8(K.empty(*values, device=dev, dtype=torch.float8_e4m3fn),
+                 K.empty(*scales, device=dev, dtype=torch.float8_e8m0fnu), width, lead)
 
 
 def _row_view(x: Tensor) -> Tensor:
@@ -231,13 +235,11 @@ def pack8(w: Tensor, gated: bool = False) -> Weight8:
     col = _packed_rows(n, gated).to(w.device)
     rows = w.t().index_select(0, col.clamp(min=0)).masked_fill_((col < 0).unsqueeze(1), 0.0)
     q = quantize8(rows)
-    steps = q.values.shape[1] // STEP
-    # (tile, row, step, plane, lane group, byte) -> (tile, step, plane, lane = group and row, byte)
-    v = q.values.view(torch.uint8).view(-1, 16, steps, 2, 4, 16).permute(0, 2, 3, 4, 1, 5).contiguous()
+    steps, at = q.values.shape[1], torch.arange(len(col), device=w.device)
+    c = q.scales.view(torch.uint8).index_select(1, (at & ~127) + 4 * (at & 31) + (at >> 5 & 3))
     # (step, lane group, group of tiles, tile, row) -> (step, group of tiles, lane, tile)
-    c = q.scales.view(torch.uint8).view(steps, 4, -1, 4, 16).permute(0, 2, 1, 4, 3).contiguous()
-    return Weight8(v.view(-1, steps, 2, 64, 16).view(torch.float8_e4m3fn),
-                   c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, bool(gated))
+    c = c.view(steps, 4, -1, 4, 16).permute(0, 2, 1, 4, 3).contiguous()
+    return Weight8(q.values, c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, bool(gated))
 
 
 def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):

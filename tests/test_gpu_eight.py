@@ -58,6 +58,16 @@ def half_step(x, slack):
     return torch.maximum(x.abs() * HALF8, s * 2.0 ** -10)
 
 
+def unpacked(q):
+    """The 8-bit values (rows, kp) and the scales (rows, kp / 32) of a Rows8, taken out of their tiles."""
+    rows = math.prod(q.lead)
+    v = q.values.view(torch.uint8).cpu()     # tile, step, plane, lane group g, row, byte
+    v = v.view(len(v), -1, 2, 4, 16, 16).permute(0, 4, 1, 2, 3, 5).reshape(16 * len(v), -1)[:rows]
+    r = torch.arange(rows)
+    s = q.scales.view(torch.uint8).cpu()[:, (r & ~127) + 4 * (r & 31) + (r >> 5 & 3)].t()
+    return v.contiguous().view(torch.float8_e4m3fn), s.contiguous().view(torch.float8_e8m0fnu)
+
+
 def acts(gen, rows, k, dtype):
     x = torch.randn(rows, k, generator=gen, dtype=F64)
     x = x * torch.where(torch.rand(k, generator=gen) < 0.02, 12.0, 1.0)
@@ -92,13 +102,13 @@ def test_quantize(T, rows, width, dtype):
     x = acts(gen, rows, width, dtype)
     x = x * torch.exp2(torch.randint(-30, 30, (rows, 1), generator=gen).double()).to(dtype)
     q = T.quantize8(x.cuda())
-    assert q.shape == (rows, width) and q.values.shape[1] % 128 == 0
+    assert q.shape == (rows, width)
     same(q.dequantize(), round8(x.double()), "bf16")
     same(q.dequantize(F32), round8(x.double()), "f32")
-    assert not bool(q.values.view(torch.uint8)[:, width:].any())
-    # the scales are the definition's, and the types are torch's own
-    up = q.scales.float()[:, :rows].t().repeat_interleave(32, 1)
-    same((q.values.float() * up)[:, :width], round8(x.double()), "by torch")
+    # the tiles hold the definition's values and scales in torch's own types, and zeros behind the width
+    v, s = unpacked(q)
+    assert not bool(v.view(torch.uint8)[:, width:].any())
+    same((v.float() * s.float().repeat_interleave(32, 1))[:, :width], round8(x.double()), "by torch")
 
 
 def test_quantize_special(T):
@@ -152,7 +162,7 @@ def test_norm_special(T):
     d = q.dequantize(F32).cpu()
     assert bool(torch.isnan(d[1]).all()) and bool(torch.isnan(d[2, 129])) and not bool(d[2, :129].any())
     assert not bool(d[3].any()) and bool(torch.isfinite(d[[0, 4, 5]]).all())
-    assert not bool(q.values.view(torch.uint8)[:, 130:].any())      # zeros behind the width, NaN rows too
+    assert not bool(unpacked(q)[0].view(torch.uint8)[:, 130:].any())      # zeros behind the width, NaN rows too
     same(s, x.double())
 
 
@@ -167,7 +177,7 @@ def test_strided_rows(T):
         s0, a = T.rms_norm8(view, gain, 1e-5, add=view)
         s1, b = T.rms_norm8(dense, gain, 1e-5, add=dense)
         same(s0, s1.double().cpu())
-        assert torch.equal(a.values.view(torch.uint8), b.values.view(torch.uint8))
+        assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(unpacked(a), unpacked(b)))
 
 
 def sum_error(x, w):
@@ -221,6 +231,60 @@ def test_matmul(T, rows, k, n):
         bounded(T.matmul8(x.cuda(), w8, bias=bias.cuda(), activation=act, residual=res.cuda()), full, e, str(act))
 
 
+# every form of the product: 128 x 64, 256 x 64 and 256 x 128 outputs x rows, and 256 x 256 with long sums
+LARGE = [(600, 300, 1027), (1100, 520, 2000), (900, 260, 4488), (2500, 130, 1544), (4200, 1024, 1031), (3333, 640, 2304),
+         (2304, 3200, 2310), (4111, 3080, 1288), (9000, 100, 600)]
+
+
+def large_bound(xr, wr):
+    """`sum_error` with every magnitude of the 8 in place of the largest one's seven."""
+    return (xr.abs() @ wr.abs()) * (7 * 2.0 ** -13 + (xr.shape[1] / 8 + 8) * 2.0 ** -24)
+
+
+@pytest.mark.parametrize("rows,k,n", LARGE)
+def test_matmul_large(T, rows, k, n):
+    gen = torch.Generator().manual_seed(rows + k + n)
+    x, w = acts(gen, rows, k, BF16).cuda(), weight(gen, k, n).cuda()
+    w8 = T.pack8(w)
+    xr, wr = round8(x.double()), rounded_weight(w)
+    want, err = xr @ wr, large_bound(xr, wr)
+    got = T.matmul8(x, w8)
+    bounded(got, want.cpu(), (err + want.abs() * HALF16 * 1.01).cpu(), "plain")
+    # a few rows by themselves take another form, whose sums have the same cuts and another order
+    pick = [0, 1, rows // 2, rows - 1]
+    near = T.matmul8(x[pick].contiguous(), w8).double()
+    assert bool(((got[pick].double() - near).abs() <= near.abs() * 2 * HALF16 + err[pick] * 2 ** -6).all())
+    bias, res = torch.randn(n, generator=gen).cuda(), acts(gen, rows, n, BF16).cuda()
+    for b, act, r in ((bias, None, None), (None, None, res), (bias, None, res), (bias, "gelu", res), (None, "silu", None)):
+        full = act_of(act)(want + (0 if b is None else b.double())) + (0 if r is None else r.double())
+        e = 1.13 * err + 2.0 ** -19 * (want.abs() + bias.double().abs() + res.double().abs()) + full.abs() * HALF16 * 1.01
+        bounded(T.matmul8(x, w8, bias=b, activation=act, residual=r), full.cpu(), e.cpu(), f"{b is None} {act} {r is None}")
+
+
+@pytest.mark.parametrize("rows,k,n", [(600, 300, 500), (1100, 520, 1000), (2500, 130, 772), (4200, 260, 700), (3000, 1500, 1153)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_swiglu_large(T, rows, k, n, biased):
+    gen = torch.Generator().manual_seed(rows + k + n)
+    x, w = acts(gen, rows, k, BF16).cuda(), weight(gen, k, 2 * n).cuda()
+    bias = torch.randn(2 * n, generator=gen).cuda() if biased else None
+    got = T.swiglu8(x, T.pack8(w, gated=True), bias)
+    assert not bool(unpacked(got)[0].view(torch.uint8)[:, n:].any())
+    xr, wr = round8(x.double()), rounded_weight(w)
+    h, cuts = xr @ wr, large_bound(xr, wr)
+    if biased:
+        h = h + bias.double()
+    v, g = h[:, :n], h[:, n:]
+    silu = g * torch.sigmoid(g)
+    want = v * silu
+    err = cuts[:, :n] * (silu.abs() + 1.1 * cuts[:, n:]) + 1.1 * v.abs() * cuts[:, n:] + 2.0 ** -19 * v.abs() * (silu.abs() + g.abs())
+    top = torch.nn.functional.pad(want.abs() + err, (0, -n % 32)).unflatten(-1, (-1, 32)).amax(-1)
+    scale = scales_of(top.repeat_interleave(32, -1))[:, :n]
+    half = torch.maximum((want.abs() + err) * HALF8, scale * 2.0 ** -10)
+    bounded(got.dequantize(F32), want.cpu(), (half + err * 1.01 + 1e-30).cpu(), "gate")
+    few = T.swiglu8(x[-40:].contiguous(), T.pack8(w, gated=True), bias).dequantize(F32)
+    assert float((few - got.dequantize(F32)[-40:]).norm() / few.norm()) < 0.01
+
+
 @pytest.mark.parametrize("rows,k,n", [(1, 64, 1), (1, 768, 96), (3, 515, 33), (16, 128, 128), (40, 260, 130),
                                       (256, 512, 320), (300, 1024, 129), (513, 384, 515)])
 @pytest.mark.parametrize("biased", [False, True])
@@ -231,10 +295,9 @@ def test_swiglu(T, rows, k, n, biased):
     w8 = T.pack8(w.cuda(), gated=True)
     assert w8.shape == (k, 2 * n)
     got = T.swiglu8(x.cuda(), w8, None if bias is None else bias.cuda())
-    assert got.shape == (rows, n) and not bool(got.values.view(torch.uint8)[:, n:].any())
+    assert got.shape == (rows, n) and not bool(unpacked(got)[0].view(torch.uint8)[:, n:].any())
     again = T.swiglu8(T.quantize8(x.cuda()), w8, None if bias is None else bias.cuda())
-    assert torch.equal(got.values.view(torch.uint8), again.values.view(torch.uint8))
-    assert torch.equal(got.scales.view(torch.uint8)[:, :rows], again.scales.view(torch.uint8)[:, :rows])
+    assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(unpacked(got), unpacked(again)))
     xr, wr = round8(x.double()), rounded_weight(w)
     h, cuts = xr @ wr, sum_error(xr, wr)
     if biased:
@@ -304,7 +367,7 @@ def test_empty_and_shapes(T):
 
 def test_rows_past_32_bits(T):
     """More than 2^32 bytes of 8-bit rows: the last rows of the product, and of the rounding."""
-    rows, k = (1 << 22) + 300, 1024
+    rows, k = (1 << 22) + 300, 1024     # tiles of the 256 x 128 form
     gen = torch.Generator().manual_seed(1)
     w8 = T.pack8(weight(gen, k, 40).cuda())
     x = torch.zeros(rows, k, device="cuda", dtype=BF16)
@@ -372,7 +435,8 @@ def test_refusals(T):
             (lambda: T.rms_norm8(torch.zeros(1, 16385, device="cuda"), torch.ones(16385, device="cuda"), 1e-5), "16384"),
             (lambda: T.quantize8(torch.zeros(2, 0, device="cuda")), "rows of 0"),
             (lambda: T.pack8(torch.zeros(8, 7, device="cuda"), gated=True), "value and gate"),
-            (lambda: T.quantize8(x)._replace(width=129).dequantize(), "Rows8")):
+            (lambda: T.quantize8(x)._replace(width=129).dequantize(), "Rows8"),
+            (lambda: T.matmul8(T.quantize8(x)._replace(lead=(17,)), w8), "Rows8")):
         with pytest.raises(ValueError, match=what):
             bad()
     with torch.no_grad():
