@@ -23,7 +23,6 @@
 // 4 (t & 1) + i, which leaves a lane 8 neighbouring outputs (16 bytes of bf16) in two tiles, and four
 // lanes the 32 of a block. With a gate, tiles 0 and 1 hold value's outputs 32 grp + 8 g + 4 t + i and
 // tiles 2 and 3 gate's, so a lane has both.
-#include <algorithm>
 #include <type_traits>
 
 #include "m3s_eight.h"
@@ -561,28 +560,33 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
     vm_wait_keep<kOps>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    load((R + 2) % 3, s + 2);
     const uint8_t* at = lds + R * kStageBytes + lread;
     auto frag = [&](int tile) {
       return join8(*reinterpret_cast<const i32x4_*>(at + tile * 2048),
                    *reinterpret_cast<const i32x4_*>(at + tile * 2048 + 512));
     };
-    i32x8_ b[TM];
+    i32x8_ a[TN], b[TM];
+#pragma unroll
+    for (int t = 0; t < TN; ++t) a[t] = frag(wn * TN + t);
 #pragma unroll
     for (int j = 0; j < TM; ++j) b[j] = frag(NTL / 2 + wm * TM + j);
+    __builtin_amdgcn_sched_barrier(0);
+    load((R + 2) % 3, s + 2);
     const int by = 8 * (c >> 4), sr = (int)((uint32_t)sx[R] >> (8 * ((int)(mw >> 5) & 3)));
 #pragma unroll
     for (int q = 0; q < TN / 2; ++q) {
       const int s4 = (int)((uint32_t)sw[R][q] >> by);
-      const i32x8_ a0 = frag(wn * TN + 2 * q), a1 = frag(wn * TN + 2 * q + 1);
       static_for<TM>([&](auto jc) {
         constexpr int j = decltype(jc)::value;
-        acc[2 * q][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a0, b[j], acc[2 * q][j], 0, 0, 0, s4, j, sr);
+        acc[2 * q][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[2 * q], b[j], acc[2 * q][j], 0, 0, 0, s4, j, sr);
+        acc[2 * q + 1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[2 * q + 1], b[j], acc[2 * q + 1][j], 0, 0, 2, s4, j, sr);
       });
-      static_for<TM>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        acc[2 * q + 1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a1, b[j], acc[2 * q + 1][j], 0, 0, 2, s4, j, sr);
-      });
+    }
+    // the loads between the products, and not before the first of them
+#pragma unroll
+    for (int i = 0; i < TN * TM; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x010, (LN + LM + TN * TM - 1) / (TN * TM), 0);
     }
     __builtin_amdgcn_sched_barrier(0);
     scales(s + 3, sw[R], sx[R]);
@@ -599,388 +603,19 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
   load(1, 1);
   scales(2, sw[2], sx[2]);
   __builtin_amdgcn_sched_barrier(0);
-  for (int s = 0;; s += 3) {
+  int s = 0;
+  for (; s + 3 <= S; s += 3) {   // no way out in the middle: the compiler would wait for scales just asked for
     step(r0, s);
-    if (s + 1 >= S) break;
     step(r1, s + 1);
-    if (s + 2 >= S) break;
     step(r2, s + 2);
-    if (s + 3 >= S) break;
   }
+  if (s < S) step(r0, s);
+  if (s + 1 < S) step(r1, s + 1);
   vm_wait_all();   // no load may reach LDS behind the workgroup's end
   const bool plain = (p.vec & 1) && p.act == kActNone && p.N % 8 == 0;
   if (!GATED) __syncthreads();
   finish_tile<TN, TM, GATED>(p, acc, (tile0 + 2 * TN * wn) / 4, m0 + 32 * TM * wm, plain, lane,
                              reinterpret_cast<float*>(lds) + wave * (kShare / 4));
-}
-
-// ---- more rows than the CUs hold at once ------------------------------------------------------
-// One workgroup of eight waves on each CU, 256 outputs x 256 rows at a time, a wave 64 x 128 of them; it
-// stays for its share of the tiles. Its loads run three steps of 64 k ahead of the products through a ring
-// of three stages, and on into the next tile while this one's outputs leave; a step's operands are
-// read into registers under the products of the step before, so that a barrier a step costs the matrix
-// units nothing but the waves' differences. Scales come to LDS as the operands do.
-constexpr int kBigWaves = 8, kBigSide = 256;
-constexpr int kBigOps = 5;                       // loads of a step: two tiles of either operand, and scales
-constexpr int kBigScales = 32 * 1024;            // in a stage, behind the 32 planes: weight 1 KB, rows 512 B,
-constexpr int kBigStage = kBigScales + 2048;     // and as much that nothing reads
-constexpr int kBigTurn = 32 * (64 + 8) * 2;      // a wave's 32 rows of 64 bf16
-constexpr int kCus = 256;
-
-template <int n>
-__device__ __forceinline__ void vm_wait_to() {   // vmcnt(n), n < 64
-  __builtin_amdgcn_s_waitcnt(0x0F70 | (n & 15) | (n >> 4) << 14);
-}
-
-struct BigTile {
-  int tile0;      // first packed tile of 16
-  int64_t m0;     // first row
-};
-
-__device__ __forceinline__ BigTile big_tile(const M8Params& p, int lin) {
-  constexpr int kHigh = 8;
-  const int band = lin / (kHigh * p.tiles_n), high = min(kHigh, p.tiles_m - band * kHigh);
-  const int at = lin - band * kHigh * p.tiles_n;
-  return {__builtin_amdgcn_readfirstlane(at / high) * (kBigSide / 16),
-          (int64_t)__builtin_amdgcn_readfirstlane(band * kHigh + at % high) * kBigSide};
-}
-
-// A wave's 64 x 128 accumulators: tiles T = 0, 1 of its group and row tiles j; element 4 u + e of lane (c, h) is
-// row row0 + 32 j + c and output 64 grp + 32 T + 16 (u & 1) + 8 h + 4 (u >> 1) + e.
-__device__ __forceinline__ void finish_big(const M8Params& p, const f32x16 (&acc)[2][4], int grp, int64_t row0,
-                                           int lane, uint8_t* turn) {
-  constexpr int LD = 64 + 8;
-  bf16* sb = reinterpret_cast<bf16*>(turn);
-  const int c = lane & 31, h = lane >> 5, piece = lane & 7, rl = lane >> 3;
-  const int n0 = 64 * grp, n = n0 + 8 * piece;
-  if ((p.vec & 1) && p.act == kActNone && p.N % 8 == 0) {
-    if (n0 >= p.N) return;
-    const bool whole = row0 + 128 <= p.M && n0 + 64 <= p.N;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t mj = row0 + 32 * j + rl;
-      if (p.residual) {   // its rows turned into the accumulators' order
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int64_t m = mj + 8 * i;
-          *reinterpret_cast<bf16x8*>(sb + (8 * i + rl) * LD + 8 * piece) =
-              m < p.M && n < p.N ? *reinterpret_cast<const bf16x8*>(p.residual + m * p.ldr + n) : bf16x8{};
-        }
-        wave_sync();
-      }
-      bf16x8 o[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {   // outputs 32 T + 16 k + 8 h .., i = 2 T + k
-        const int at = 16 * i + 8 * h;
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = acc[i >> 1][j][8 * (e >> 2) + 4 * (i & 1) + (e & 3)];
-        if (p.bias && n0 + at < p.N) {
-          const f32x4 a = *reinterpret_cast<const f32x4*>(p.bias + n0 + at);
-          const f32x4 d = *reinterpret_cast<const f32x4*>(p.bias + n0 + at + 4);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) { v[e] += a[e]; v[4 + e] += d[e]; }
-        }
-        if (p.residual) {
-          const bf16x8 r = *reinterpret_cast<const bf16x8*>(sb + c * LD + at);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += (float)r[e];
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[i][e] = (bf16)v[e];
-      }
-      if (p.residual) wave_sync();
-#pragma unroll
-      for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16x8*>(sb + c * LD + 16 * i + 8 * h) = o[i];
-      wave_sync();
-      bf16* yr = p.y + mj * p.ldy + n;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = *reinterpret_cast<const bf16x8*>(sb + (8 * i + rl) * LD + 8 * piece);
-      if (whole) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *reinterpret_cast<bf16x8*>(yr + (int64_t)(8 * i) * p.ldy) = o[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (mj + 8 * i < p.M && n < p.N) *reinterpret_cast<bf16x8*>(yr + (int64_t)(8 * i) * p.ldy) = o[i];
-      }
-      wave_sync();
-    }
-    return;
-  }
-  // odd widths and activations: 16 rows at a time in float32, one loop each
-  constexpr int LF = 64 + 4;
-  static_assert(16 * LF * 4 <= kBigTurn, "16 rows of float32 fit");
-  float* sf = reinterpret_cast<float*>(turn);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if ((c >> 4) == half) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-#pragma unroll
-          for (int u = 0; u < 4; ++u)
-            *reinterpret_cast<f32x4*>(sf + (c & 15) * LF + 32 * t + 16 * (u & 1) + 8 * h + 4 * (u >> 1)) =
-                f32x4{acc[t][j][4 * u], acc[t][j][4 * u + 1], acc[t][j][4 * u + 2], acc[t][j][4 * u + 3]};
-        }
-      }
-      wave_sync();
-      const int64_t mj = row0 + 32 * j + 16 * half;
-      if (p.vec & 1) {
-#pragma unroll 1
-        for (int e = rl; e < 16; e += 8) {
-          if (mj + e < p.M) {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(sf + e * LF + 8 * piece);
-            const f32x4 d = *reinterpret_cast<const f32x4*>(sf + e * LF + 8 * piece + 4);
-            float v[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
-            finish8<false>(p, mj + e, n, v);
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int e = 0; e < 16; ++e) {
-          const int64_t m = mj + e;
-          if (m < p.M && n0 + lane < p.N) {
-            float v = sf[e * LF + lane];
-            if (p.bias) v += p.bias[n0 + lane];
-            v = act8(v, p.act);
-            if (p.residual) v += (float)p.residual[m * p.ldr + n0 + lane];
-            p.y[m * p.ldy + n0 + lane] = (bf16)v;
-          }
-        }
-      }
-      wave_sync();
-    }
-  }
-}
-
-// The same of a gate: tile 0 is value's, tile 1 gate's 32 outputs of block grp.
-__device__ __forceinline__ void finish_big_gate(const M8Params& p, const f32x16 (&acc)[2][4], int grp, int64_t row0,
-                                                int lane) {
-  const int c = lane & 31, h = lane >> 5;
-  if (grp >= p.NP / 64 || row0 >= p.M) return;
-  uint8_t* out = p.yv + value_at(row0 + c, 32 * grp + 8 * h, p.NP / 256);
-  uint32_t bytes = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float v[16];
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {   // i: 8 outputs from 8 h, then 8 from 16 + 8 h
-      const int e = 8 * ((i >> 2) & 1) + 4 * (i >> 3) + (i & 3);
-      float a = acc[0][j][e], b = acc[1][j][e];
-      if (p.bias) {
-        const int n = min(32 * grp + 16 * (i >> 3) + 8 * h + (i & 7), p.N - 1);
-        a += p.bias[n];
-        b += p.bias[p.N + n];
-      }
-      v[i] = a * silu8(b);
-    }
-    if (32 * grp + 32 > p.N) {   // zeros behind the width
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (32 * grp + 16 * (i >> 3) + 8 * h + (i & 7) >= p.N) v[i] = 0.f;
-    }
-    uint32_t u = max_bits(v), o = (uint32_t)__shfl_xor((int)u, 32, 64);
-    u = u > o ? u : o;
-    if (u >= kInfBits) {   // both lanes of a row
-      u = max_bits_finite(v);
-      o = (uint32_t)__shfl_xor((int)u, 32, 64);
-      u = u > o ? u : o;
-    }
-    const int byte = scale_byte(u);
-    const float down = scale_down(byte);
-    bytes |= (uint32_t)byte << (8 * j);
-    // the row tile's two tiles of 16, 256 bytes in a piece
-    if (row0 + 32 * j + c < p.M) {
-      uint8_t* to = out + (int64_t)j * 2 * (p.NP / 256) * 2048;
-      *reinterpret_cast<i32x2_*>(to) = i32x2_{pack4(v[0], v[1], v[2], v[3], down), pack4(v[4], v[5], v[6], v[7], down)};
-      *reinterpret_cast<i32x2_*>(to + 256) =   // 16 k on
-          i32x2_{pack4(v[8], v[9], v[10], v[11], down), pack4(v[12], v[13], v[14], v[15], down)};
-    }
-  }
-  // four rows' scales in one dword; those of rows behind the last are anything
-  if (h == 0) *reinterpret_cast<uint32_t*>(p.ys + (int64_t)grp * p.mp + row0 + 4 * c) = bytes;
-}
-
-template <bool GATED>
-__global__ void __launch_bounds__(64 * kBigWaves) matmul8_big_kernel(const M8Params p) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[3 * kBigStage + (GATED ? 0 : kBigWaves * kBigTurn)];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wn = wave & 3, wm = wave >> 2, c = lane & 31, h = lane >> 5;
-  // An XCD's workgroups take consecutive tiles, eight row tiles high and walked along the outputs: the 32
-  // at work at a time read some 8 strips of rows and 4 of the weight through their L2.
-  const int nb = p.tiles_m * p.tiles_n, per = (nb + 7) >> 3, stride = (int)(gridDim.x >> 3);
-  const int first = (blockIdx.x & 7) * per, last = min(first + per, nb);
-  int lin = first + (int)(blockIdx.x >> 3);
-  if (lin >= last) return;
-  const int S = 2 * p.KB, ntiles = p.NP / 16;
-  const uint32_t wstep = (uint32_t)p.KB * 2048;
-  // waves 0 to 3 load the weight's scales (a dword a lane for 128 k), the others the rows' (for 32 k each)
-  const bool of_w = wave < 4;
-  const uint8_t* sbase = of_w ? p.ws : p.xs;
-  const uint32_t sbytes = of_w ? (uint32_t)((int64_t)p.KB * p.NP * 4) : (uint32_t)((int64_t)p.KB * p.mp * 4);
-  const uint32_t sshift = of_w ? 1 : 0, sstep = of_w ? (uint32_t)p.NP * 4 : (uint32_t)p.mp * 2;
-  // where a tile's loads start
-  struct Place {
-    const uint8_t *w, *x;
-    uint32_t ow[2], ox[2], os;
-  };
-  auto place = [&](int at) {
-    const BigTile t = big_tile(p, min(at, last - 1));
-    Place q;
-    q.w = p.w + (int64_t)t.tile0 * wstep;
-    q.x = static_cast<const uint8_t*>(p.x) + (t.m0 >> 4) * wstep;
-    const int rtiles = (int)min((p.M - t.m0 + 15) >> 4, (int64_t)16);
-    // a tile behind the last reads the last one instead, and is not stored
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      q.ow[i] = (uint32_t)min(2 * wave + i, ntiles - 1 - t.tile0) * wstep + 16 * lane;
-      q.ox[i] = (uint32_t)min(2 * wave + i, rtiles - 1) * wstep + 16 * lane;
-    }
-    q.os = of_w ? (uint32_t)(t.tile0 / 4 + wave) * 256 + 4 * lane
-                : (uint32_t)((int64_t)(wave & 1) * p.mp + t.m0 + 4 * lane);
-    return q;
-  };
-  // the step of the loads, three ahead of the products', and whether there is one
-  int ls = 0;
-  bool on = true;
-  Place at = place(lin);
-  auto load = [&](int stage) {
-    const uint32_t bytes = on ? 0xfffffff0u : 0u;
-    const __amdgpu_buffer_rsrc_t rw = make_rsrc(at.w, bytes), rx = make_rsrc(at.x, bytes);
-    const __amdgpu_buffer_rsrc_t rs = make_rsrc(sbase, on ? sbytes : 0u);
-    uint8_t* to = lds + stage;
-    const uint32_t s = __builtin_amdgcn_readfirstlane(ls);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) buf_load_lds16(rw, to + (2 * wave + i) * 1024, at.ow[i], s * 1024);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) buf_load_lds16(rx, to + (16 + 2 * wave + i) * 1024, at.ox[i], s * 1024);
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        rs, (__attribute__((address_space(3))) void*)(to + kBigScales + 256 * wave), 4, at.os,
-        __builtin_amdgcn_readfirstlane((s >> sshift) * sstep), 0, 0);
-    ++ls;
-  };
-  struct Operands {
-    i32x8_ a[2], b[4];
-    int sw, sx;
-  };
-  const int lread = (c >> 4) * 1024 + h * 256 + (c & 15) * 16;
-  auto read = [&](int stage, int odd, Operands& o) {
-    const uint8_t* at = lds + stage;
-    auto frag = [&](int tile) {
-      return join8(*reinterpret_cast<const i32x4_*>(at + lread + tile * 2048),
-                   *reinterpret_cast<const i32x4_*>(at + lread + tile * 2048 + 512));
-    };
-    const int* sc = reinterpret_cast<const int*>(at + kBigScales);
-    o.sw = sc[64 * wn + 32 * odd + 16 * h + (c & 15)];
-    o.sx = sc[256 + 64 * h + 32 * wm + c];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) o.a[t] = frag(2 * wn + t);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o.b[j] = frag(8 + 4 * wm + j);
-  };
-  f32x16 acc[2][4];
-  auto products = [&](const Operands& o) {
-    const int s4 = (int)((uint32_t)o.sw >> (8 * (c >> 4)));
-    static_for<4>([&](auto jc) {
-      constexpr int j = decltype(jc)::value;
-      acc[0][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.a[0], o.b[j], acc[0][j], 0, 0, 0, s4, j, o.sx);
-      acc[1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(o.a[1], o.b[j], acc[1][j], 0, 0, 2, s4, j, o.sx);
-    });
-  };
-  int stage = 0;
-  // Before a step the stage that it reads ahead from is whole: only the loads of the step after that are
-  // still under way. Every wave has read the stage that is filled next.
-  auto open = [&](auto waits) {
-    if constexpr (decltype(waits)::value) __builtin_amdgcn_s_waitcnt(0x0070 | kBigOps);   // vmcnt(kBigOps), lgkmcnt(0)
-    else __builtin_amdgcn_s_waitcnt(0xc07f);                                               // lgkmcnt(0)
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  // Products first, reads and then loads between them: every wave issues its loads behind the same
-  // barrier, and products that stood behind them would wait for the address unit (8192^3: 459 us, so 428).
-  auto interleave = [&]() {
-    auto group = [&](auto reads, auto loads) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);   // a product
-      if constexpr (decltype(reads)::value > 0) __builtin_amdgcn_sched_group_barrier(0x100, decltype(reads)::value, 0);
-      if constexpr (decltype(loads)::value > 0) __builtin_amdgcn_sched_group_barrier(0x010, decltype(loads)::value, 0);
-    };
-    const std::integral_constant<int, 0> n0;
-    const std::integral_constant<int, 1> n1;
-    const std::integral_constant<int, 2> n2;
-    const std::integral_constant<int, 4> n4;
-    group(n4, n0);
-    group(n4, n0);
-    group(n4, n0);
-    group(n2, n1);
-    group(n0, n1);
-    group(n0, n1);
-    group(n0, n2);
-    group(n0, n0);
-  };
-  Operands even, odd;
-  Place then;
-  bool again;
-  // Two steps; nothing branches in them (the compiler would move the products past it).
-  auto pair = [&](auto waits) {
-    open(waits);
-    const int filled = stage;
-    stage = stage == 2 * kBigStage ? 0 : stage + kBigStage;
-    read(stage, 1, odd);
-    load(filled);
-    products(even);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-    const bool turn = ls == S;   // after an odd number of loads: S is even, and three were made before
-    ls = turn ? 0 : ls;
-    on = turn ? again : on;
-    at.w = turn ? then.w : at.w;
-    at.x = turn ? then.x : at.x;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      at.ow[i] = turn ? then.ow[i] : at.ow[i];
-      at.ox[i] = turn ? then.ox[i] : at.ox[i];
-    }
-    at.os = turn ? then.os : at.os;
-    open(waits);
-    const int freed = stage;
-    stage = stage == 2 * kBigStage ? 0 : stage + kBigStage;
-    read(stage, 0, even);
-    load(freed);
-    products(odd);
-    interleave();
-    __builtin_amdgcn_sched_barrier(0);
-  };
-  load(0);
-  load(kBigStage);
-  load(2 * kBigStage);
-  vm_wait_all();
-  __builtin_amdgcn_s_barrier();
-  asm volatile("" ::: "memory");
-  read(0, 0, even);
-  while (true) {
-    const BigTile t = big_tile(p, lin);
-    then = place(lin + stride);   // where the loads go on behind this tile
-    again = lin + stride < last;
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[k][j] = f32x16{};
-    }
-    // The three steps that are loaded need no wait, and one here would be for the outputs of the tile
-    // before, which left behind those loads.
-    pair(std::false_type{});
-    for (int s = 2; s < S; s += 2) pair(std::true_type{});
-    vm_wait_all();   // the next tile's first three steps, before outputs stand behind them
-    const int grp = t.tile0 / 4 + wn;
-    const int64_t row0 = t.m0 + 128 * wm;
-    if constexpr (GATED) finish_big_gate(p, acc, grp, row0, lane);
-    else finish_big(p, acc, grp, row0, lane, lds + 3 * kBigStage + wave * kBigTurn);
-    lin += stride;
-    if (!again) break;
-  }
-  vm_wait_all();   // no load may reach LDS behind the workgroup's end
 }
 
 template <int MT, int XK, bool GATED>
@@ -999,13 +634,6 @@ static void launch_many(M8Params p, hipStream_t s) {
 }
 
 template <bool GATED>
-static void launch_big(M8Params p, hipStream_t s) {
-  p.tiles_n = (p.NP + kBigSide - 1) / kBigSide;
-  p.tiles_m = (int)((p.M + kBigSide - 1) / kBigSide);
-  hipLaunchKernelGGL((matmul8_big_kernel<GATED>), dim3(kCus), dim3(64 * kBigWaves), 0, s, p);
-}
-
-template <bool GATED>
 static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED>(p, s);
   if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED>(p, s);
@@ -1019,7 +647,6 @@ static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED>(p, s);
   else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED>(p, s);
   else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED>(p, s);
-  else if (p.KB >= 2) launch_big<GATED>(p, s);   // its loads are three steps ahead, half a tile at least
   else launch_many<4, 1, 2, 4, GATED>(p, s);
 }
 
