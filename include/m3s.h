@@ -743,7 +743,7 @@ typedef struct m3s_rows8_args {
   int64_t ldx;
   const void* add;      /* (rows, width) bf16, or NULL */
   int64_t ldadd;
-  const float* gain;    /* (width), or NULL: no norm */
+  const float* gain;    /* (width), 16-byte aligned, or NULL: no norm */
   void* sum;            /* out (rows, width) dense, iff add */
   void* values;         /* out, packed */
   void* scales;         /* out (kp / 32, mp) */

@@ -315,7 +315,7 @@ PyObject* rows8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (args[1] != Py_None) {
     gain = given(args[1], &device);
     if (!gain || gain->scalar_type() != at::kFloat || gain->dim() != 1 || gain->size(0) != width ||
-        !gain->is_contiguous() || width > kNormMax8)
+        !gain->is_contiguous() || width > kNormMax8 || reinterpret_cast<uintptr_t>(gain->data_ptr()) % 16)
       Py_RETURN_NONE;
   }
   if (args[3] != Py_None) {

@@ -81,34 +81,72 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t u) {
   return u > o ? u : o;
 }
 
-// RW waves to a row (1, 4 or 16), NP pieces of 8 columns to a lane; without a norm RW is 1 and the
-// grid's second axis takes the columns.
-template <typename TX, bool NORM, bool ADD, bool VEC, int RW, int NP>
+// RW waves to a row (1, 4, 8 or 16), NP pieces of 8 columns to a lane, W columns together; without a norm RW is 1
+// and the grid's second axis takes the columns. TURN: the tile's bytes and scales meet in LDS and go out in
+// whole pieces; else (rows past 8192 columns) a lane's 8 bytes go where they belong (16384 x 2048 bf16: 30 us
+// so, 24 turned). Rows that do not keep 16-byte boundaries are read a column to a lane, and each lane's 8
+// columns come from LDS.
+template <typename TX, bool NORM, bool ADD, bool VEC, int RW, int NP, bool TURN>
 __global__ void __launch_bounds__(kR8Threads) rows8_kernel(const R8Params p) {
+  constexpr int STEP = kR8Pass * RW, W = STEP * NP, LD = W + 16;
+  __shared__ __attribute__((aligned(16))) uint8_t turn[TURN ? 16 * LD : 16];
+  __shared__ uint8_t turn_scales[TURN ? W / 2 : 1];   // [block][row]
+  __shared__ __attribute__((aligned(16))) float cols[VEC ? 4 : kR8Waves * kR8Pass];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  constexpr int STEP = kR8Pass * RW;
-  const int c0 = 8 * lane + kR8Pass * (wave % RW) + (NORM ? 0 : (int)blockIdx.y * kR8Pass * NP);
+  const int w0 = NORM ? 0 : (int)blockIdx.y * W, c0 = w0 + 8 * lane + kR8Pass * (wave % RW);
+  const int64_t r0 = (int64_t)blockIdx.x * 16;
 #pragma unroll 1
   for (int it = 0; it < RW; ++it) {
-    const int64_t r = (int64_t)blockIdx.x * 16 + it * (kR8Waves / RW) + wave / RW;
-    if (RW == 1 && r >= p.M) return;   // whole waves; no barrier below in this form
+    const int rt = it * (kR8Waves / RW) + wave / RW;   // row of the tile
+    const int64_t r = r0 + rt;
     const int D = r < p.M ? p.D : 0;
     const TX* xr = static_cast<const TX*>(p.x) + r * p.ldx;
+    const bf16* ar = ADD ? static_cast<const bf16*>(p.add) + r * p.lda : nullptr;
+    TX* sr = ADD ? static_cast<TX*>(p.sum) + r * p.D : nullptr;
     float v[NP][8];
+    if constexpr (VEC) {
 #pragma unroll
-    for (int k = 0; k < NP; ++k) load8<TX, VEC>(xr + c0 + k * STEP, D - c0 - k * STEP, v[k]);
-    if constexpr (ADD) {
-      const bf16* ar = static_cast<const bf16*>(p.add) + r * p.lda;
-      TX* sr = static_cast<TX*>(p.sum) + r * p.D;
+      for (int k = 0; k < NP; ++k) load8<TX, true>(xr + c0 + k * STEP, D - c0 - k * STEP, v[k]);
+      if constexpr (ADD) {
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+          float d[8];
+          load8<bf16, true>(ar + c0 + k * STEP, D - c0 - k * STEP, d);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[k][i] = (float)(TX)(v[k][i] + d[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < NP; ++k) store8<TX, true>(sr + c0 + k * STEP, D - c0 - k * STEP, v[k]);
+      }
+    } else {
+      float* mine = cols + wave * kR8Pass;
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
-        float d[8];
-        load8<bf16, VEC>(ar + c0 + k * STEP, D - c0 - k * STEP, d);
+        const int c = c0 - 8 * lane + k * STEP + lane;
+        float t[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[k][i] = (float)(TX)(v[k][i] + d[i]);
+        for (int i = 0; i < 8; ++i) t[i] = c + 64 * i < D ? (float)xr[c + 64 * i] : 0.f;
+        if constexpr (ADD) {
+          float d[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] = c + 64 * i < D ? (float)ar[c + 64 * i] : 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const TX sum = (TX)(t[i] + d[i]);
+            t[i] = (float)sum;
+            if (c + 64 * i < D) sr[c + 64 * i] = sum;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) mine[lane + 64 * i] = t[i];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const f32x4 a = *reinterpret_cast<const f32x4*>(mine + 8 * lane), b = *reinterpret_cast<const f32x4*>(mine + 8 * lane + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[k][i] = a[i]; v[k][4 + i] = b[i]; }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
-#pragma unroll
-      for (int k = 0; k < NP; ++k) store8<TX, VEC>(sr + c0 + k * STEP, D - c0 - k * STEP, v[k]);
     }
     if constexpr (NORM) {
       float ss = 0.f;
@@ -130,18 +168,19 @@ __global__ void __launch_bounds__(kR8Threads) rows8_kernel(const R8Params p) {
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
         float g[8];
-        load8<float, VEC>(p.gain + c0 + k * STEP, p.D - c0 - k * STEP, g);
+        const int c = c0 + k * STEP;
+        if (VEC || c + 8 <= p.D) load8<float, true>(p.gain + c, p.D - c, g);   // gain is on its boundary
+        else load8<float, false>(p.gain + c, p.D - c, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[k][i] = v[k][i] * rs * g[i];
       }
     }
-    if (r >= p.M) continue;
     // a column behind the width is a zero, whatever the row's statistics are (zero times the inverse
     // of a NaN is not)
 #pragma unroll
     for (int k = 0; k < NP; ++k) {
       const int c = c0 + k * STEP;
-      if (c >= p.kp) continue;   // whole quads: kp is a multiple of 128
+      if (c >= p.kp || r >= p.M) continue;   // whole quads: kp is a multiple of 128
       if constexpr (NORM) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -153,8 +192,30 @@ __global__ void __launch_bounds__(kR8Threads) rows8_kernel(const R8Params p) {
       const float down = scale_down(byte);
       const i32x2_ q = {pack4(v[k][0], v[k][1], v[k][2], v[k][3], down),
                         pack4(v[k][4], v[k][5], v[k][6], v[k][7], down)};
-      *reinterpret_cast<i32x2_*>(p.values + value_at(r, c, p.steps)) = q;
-      if ((lane & 3) == 0) p.scales[(int64_t)(c / kBlock8) * p.mp + scale_at(r)] = (uint8_t)byte;
+      if constexpr (TURN) {
+        *reinterpret_cast<i32x2_*>(turn + rt * LD + c - w0) = q;
+        if ((lane & 3) == 0) turn_scales[(c - w0) / 2 + rt] = (uint8_t)byte;
+      } else {
+        *reinterpret_cast<i32x2_*>(p.values + value_at(r, c, p.steps)) = q;
+        if ((lane & 3) == 0) p.scales[(int64_t)(c / kBlock8) * p.mp + scale_at(r)] = (uint8_t)byte;
+      }
+    }
+  }
+  if constexpr (TURN) {
+    __syncthreads();
+    const int n = min(W, p.kp - w0);   // the window's columns, and its tile's pieces of 16 bytes
+    const int rows = (int)min(p.M - r0, (int64_t)16);
+    uint8_t* out = p.values + (int64_t)blockIdx.x * p.steps * 2048 + w0 * 16;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+      const int row = i & 15;
+      if (row < rows)
+        *reinterpret_cast<i32x4_*>(out + 16 * i) =
+            *reinterpret_cast<const i32x4_*>(turn + row * LD + (i >> 7) * 128 + ((i >> 4) & 7) * 16);
+    }
+    for (int i = threadIdx.x; i < n / 2; i += blockDim.x) {
+      const int row = i & 15;
+      if (row < rows)
+        p.scales[(int64_t)(w0 / kBlock8 + (i >> 4)) * p.mp + scale_at(r0 + row)] = turn_scales[i];
     }
   }
 }
@@ -165,38 +226,60 @@ __global__ void __launch_bounds__(kR8Threads) rows8_values_kernel(const uint8_t*
                                                                   const uint8_t* __restrict__ scales,
                                                                   TY* __restrict__ y, int64_t M, int D,
                                                                   int steps) {
+  __shared__ __attribute__((aligned(16))) float cols[VEC ? 4 : kR8Waves * kR8Pass];   // a row's, to leave a column a lane
   const int64_t r = (int64_t)blockIdx.x * kR8Waves + (threadIdx.x >> 6);
-  const int c = 8 * (threadIdx.x & 63) + (int)blockIdx.y * kR8Pass;
-  if (r >= M || c >= D) return;
-  const i32x2_ q = *reinterpret_cast<const i32x2_*>(values + value_at(r, c, steps));
-  const float up = scale_up(scales[(int64_t)(c / kBlock8) * padded_rows(M) + scale_at(r)]);
-  float v[8];
+  const int lane = threadIdx.x & 63, w0 = (int)blockIdx.y * kR8Pass, c = 8 * lane + w0;
+  if (r >= M) return;   // whole waves
+  float v[8] = {};
+  if (c < D) {
+    const i32x2_ q = *reinterpret_cast<const i32x2_*>(values + value_at(r, c, steps));
+    const float up = scale_up(scales[(int64_t)(c / kBlock8) * padded_rows(M) + scale_at(r)]);
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[h], false);
-    const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[h], true);
-    v[4 * h] = lo[0] * up; v[4 * h + 1] = lo[1] * up;
-    v[4 * h + 2] = hi[0] * up; v[4 * h + 3] = hi[1] * up;
+    for (int h = 0; h < 2; ++h) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(q[h], false);
+      const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(q[h], true);
+      v[4 * h] = lo[0] * up; v[4 * h + 1] = lo[1] * up;
+      v[4 * h + 2] = hi[0] * up; v[4 * h + 3] = hi[1] * up;
+    }
   }
-  store8<TY, VEC>(y + r * D + c, D - c, v);
+  if constexpr (VEC) {
+    store8<TY, true>(y + r * D + c, D - c, v);
+  } else {
+    float* mine = cols + (threadIdx.x >> 6) * kR8Pass;
+    *reinterpret_cast<f32x4*>(mine + 8 * lane) = f32x4{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4*>(mine + 8 * lane + 4) = f32x4{v[4], v[5], v[6], v[7]};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = w0 + lane + 64 * i;
+      if (at < D) y[r * D + at] = (TY)mine[lane + 64 * i];
+    }
+  }
 }
 
 template <typename TX, bool NORM, bool ADD, bool VEC>
 static void launch_rows8(const R8Params& p, hipStream_t s) {
   const unsigned tiles = (unsigned)((p.M + 15) / 16);
   const unsigned few = 64 * (unsigned)(p.M < 16 ? p.M : 16);   // a wave to a row, and none for rows that are not there
-#define M3S_R8(RW, NP, GRID, THREADS) \
-  hipLaunchKernelGGL((rows8_kernel<TX, NORM, ADD, VEC, RW, NP>), GRID, dim3(THREADS), 0, s, p)
+#define M3S_R8(RW, NP, TURN, GRID, THREADS) \
+  hipLaunchKernelGGL((rows8_kernel<TX, NORM, ADD, VEC, RW, NP, TURN>), GRID, dim3(THREADS), 0, s, p)
+  // Fewer rows than a tile has nothing to turn (1 x 768: 3.4 us, so 2.1). Several waves to a row leave each fewer
+  // registers, and a CU two workgroups (16384 x 2048 bf16: one wave a row 34 us, four 29).
   if constexpr (!NORM) {
-    M3S_R8(1, 1, dim3(tiles, (unsigned)((p.kp + kR8Pass - 1) / kR8Pass)), few);
+    const dim3 grid(tiles, (unsigned)((p.kp + 2 * kR8Pass - 1) / (2 * kR8Pass)));
+    if (p.M < 16) M3S_R8(1, 2, false, grid, few);
+    else if (p.kp <= kR8Pass) M3S_R8(1, 1, true, grid, few);
+    else M3S_R8(1, 2, true, grid, few);
   } else {
     const int pieces = (p.kp + kR8Pass - 1) / kR8Pass;
-    if (pieces <= 1) M3S_R8(1, 1, dim3(tiles), few);
-    else if (pieces <= 2) M3S_R8(1, 2, dim3(tiles), few);
-    else if (pieces <= 4) M3S_R8(1, 4, dim3(tiles), few);
-    else if (pieces <= 8) M3S_R8(4, 2, dim3(tiles), kR8Threads);
-    else if (pieces <= 16) M3S_R8(16, 1, dim3(tiles), kR8Threads);
-    else M3S_R8(16, 2, dim3(tiles), kR8Threads);
+    if (p.M < 16 && pieces <= 2) M3S_R8(1, 2, false, dim3(tiles), few);
+    else if (pieces <= 1) M3S_R8(1, 1, true, dim3(tiles), few);
+    else if (pieces <= 2) M3S_R8(1, 2, true, dim3(tiles), few);
+    else if (pieces <= 4) M3S_R8(4, 1, true, dim3(tiles), kR8Threads);
+    else if (pieces <= 8) M3S_R8(8, 1, true, dim3(tiles), kR8Threads);
+    else if (pieces <= 16) M3S_R8(16, 1, VEC, dim3(tiles), kR8Threads);   // LDS holds no columns besides
+    else M3S_R8(16, 2, false, dim3(tiles), kR8Threads);
   }
 #undef M3S_R8
 }
@@ -206,8 +289,7 @@ static void dispatch_rows8(const m3s_rows8_args* a, const R8Params& p, hipStream
   const int xs = a->x_dtype == M3S_DTYPE_BF16 ? 2 : 4;
   // 8 columns at once where rows and pointers keep them on their boundary
   const bool vec = p.D % 8 == 0 && p.ldx % 8 == 0 && (uintptr_t)p.x % 16 == 0 &&
-                   (!ADD || (p.lda % 8 == 0 && (uintptr_t)p.add % 16 == 0 && (uintptr_t)p.sum % 16 == 0)) &&
-                   (!NORM || (uintptr_t)p.gain % 16 == 0);
+                   (!ADD || (p.lda % 8 == 0 && (uintptr_t)p.add % 16 == 0 && (uintptr_t)p.sum % 16 == 0));
   if (xs == 2) vec ? launch_rows8<bf16, NORM, ADD, true>(p, s) : launch_rows8<bf16, NORM, ADD, false>(p, s);
   else vec ? launch_rows8<float, NORM, ADD, true>(p, s) : launch_rows8<float, NORM, ADD, false>(p, s);
 }
@@ -233,7 +315,8 @@ extern "C" int32_t m3s_rows8(const m3s_rows8_args* a, void* stream) {
   M3S_REQUIRE((a->add == nullptr) == (a->sum == nullptr) && (!a->add || a->gain),
               "m3s_rows8: give both add and sum, with a gain, or neither");
   M3S_REQUIRE(a->ldx >= a->width && (!a->add || a->ldadd >= a->width), "m3s_rows8: a row stride is too short");
-  M3S_REQUIRE((uintptr_t)a->values % 16 == 0, "m3s_rows8: values must be 16-byte aligned");
+  M3S_REQUIRE((uintptr_t)a->values % 16 == 0 && (uintptr_t)a->gain % 16 == 0,
+              "m3s_rows8: values and gain must be 16-byte aligned");
   R8Params p{a->x, a->add, a->gain, a->sum, static_cast<uint8_t*>(a->values),
              static_cast<uint8_t*>(a->scales), a->rows, padded_rows(a->rows), a->ldx, a->ldadd, a->width,
              (int)padded8(a->width), (int)(padded8(a->width) / kStep8), a->eps};

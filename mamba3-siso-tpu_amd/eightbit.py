@@ -185,6 +185,8 @@ def rms_norm8(x: Tensor, gain: Tensor, eps: float, add: Optional[Tensor] = None)
     gain = gain.detach()
     if gain.dtype != torch.float32 or not gain.is_contiguous():
         gain = gain.float().contiguous()
+    if gain.data_ptr() % 16:
+        gain = gain.clone()
     xr = _row_view(x)
     out = _new_rows8(lead, rows, width, dev)
     a = _lib.Rows8Args(ctypes.sizeof(_lib.Rows8Args), _lib.dtype_code(x.dtype), width, eps, rows,

@@ -191,6 +191,15 @@ def sum_error(x, w):
     return cuts * 7 * 2.0 ** -13 + (x.abs() @ w.abs()) * (k / 8 + 8) * 2.0 ** -24
 
 
+def test_gain_off_its_boundary(T):
+    gen = torch.Generator().manual_seed(6)
+    x, gain = acts(gen, 20, 200, F32).cuda(), torch.randn(201, generator=gen).cuda()
+    for g in (gain[1:], gain[:200].double().float(), gain[:200].to(BF16), torch.stack([gain[1:], gain[1:]], 1)[:, 0]):
+        dense = g.float().contiguous().clone()
+        a, b = T.rms_norm8(x, g, 1e-5)[1], T.rms_norm8(x, dense, 1e-5)[1]
+        same(a.dequantize(), b.dequantize().double().cpu())
+
+
 def weight(gen, k, n, dtype=BF16):
     return (torch.randn(k, n, generator=gen, dtype=F64) / math.sqrt(k)).to(dtype)
 
