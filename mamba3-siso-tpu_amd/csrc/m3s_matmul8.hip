@@ -244,6 +244,22 @@ __device__ __forceinline__ void rows_operand(const M8Params& p, int64_t m0, int 
   }
 }
 
+// the scale of each plane's 16 bytes, from the lane that holds its block's
+__device__ __forceinline__ int plane_scale(int s, int lane, int h) {
+  return __shfl(s, (lane & 15) + 16 * (2 * h + (lane >> 5)), 64);
+}
+// bytes 8 i .. 8 i + 7 of an operand, in bfloat16 with their scale 2^(byte - 127): exact, but that 256 2^120
+// and up (float32's last values, 3.4e38) is an infinity, as it is where the rows are read back
+__device__ __forceinline__ bf16x8 widen8(i32x8_ v, int i, int byte) {
+  typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+  const float s = __int_as_float((byte & 255) << 23);
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * i], s, false);
+  const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * i], s, true);
+  const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * i + 1], s, false);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[2 * i + 1], s, true);
+  return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 template <int MT, int XK, bool GATED>
 __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Params p) {
   constexpr int NT = 4;
@@ -267,15 +283,32 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
       const uint8_t* q = wt + ((int64_t)t * p.KB + kb) * 2048;
       a[t] = join8(*reinterpret_cast<const i32x4_*>(q), *reinterpret_cast<const i32x4_*>(q + 1024));
     }
+    i32x8_ b[MT];
+    int sb[MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      i32x8_ b;
-      int sb;
-      rows_operand<XK>(p, m0 + 16 * j, kb, lane, b, sb);
-      mma8<0, 0>(acc[j][0], a[0], sa, b, sb);
-      mma8<1, 0>(acc[j][1], a[1], sa, b, sb);
-      mma8<2, 0>(acc[j][2], a[2], sa, b, sb);
-      mma8<3, 0>(acc[j][3], a[3], sa, b, sb);
+    for (int j = 0; j < MT; ++j) rows_operand<XK>(p, m0 + 16 * j, kb, lane, b[j], sb[j]);
+    if constexpr (GATED) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {   // a plane's halves, each 8 k of a lane
+        const int sw = plane_scale(sa, lane, i >> 1);
+        bf16x8 w[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) w[t] = widen8(a[t], i, sw >> (8 * t));
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          const bf16x8 x = widen8(b[j], i, plane_scale(sb[j], lane, i >> 1));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) acc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t], x, acc[j][t], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        mma8<0, 0>(acc[j][0], a[0], sa, b[j], sb[j]);
+        mma8<1, 0>(acc[j][1], a[1], sa, b[j], sb[j]);
+        mma8<2, 0>(acc[j][2], a[2], sa, b[j], sb[j]);
+        mma8<3, 0>(acc[j][3], a[3], sa, b[j], sb[j]);
+      }
     }
   }
 #pragma unroll

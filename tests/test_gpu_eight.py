@@ -180,6 +180,39 @@ def test_strided_rows(T):
         assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(unpacked(a), unpacked(b)))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,width", [(20, 520), (17, 1100), (40, 2052), (18, 4100), (3, 5001), (33, 8192), (2, 9001), (17, 12288)])
+def test_rows_of_every_form(T, rows, width, dtype):
+    """One to sixteen waves to a row, whole tiles and a part of one, pieces of 16 bytes and odd widths."""
+    gen = torch.Generator().manual_seed(rows + width)
+    x, a = acts(gen, rows, width, dtype), acts(gen, rows, width, BF16)
+    gain = (1 + 0.2 * torch.randn(width, generator=gen, dtype=F64)).float()
+    q = T.quantize8(x.cuda())
+    same(q.dequantize(F32), round8(x.double()), "quantize")
+    same(q.dequantize(BF16), round8(x.double()), "quantize, bf16")
+    s, n8 = T.rms_norm8(x.cuda(), gain.cuda(), 1e-5, add=a.cuda())
+    h = (x.double() + a.double()).to(F32).to(dtype).double()
+    same(s, h, "sum")
+    n = h / torch.sqrt(h.square().mean(-1, keepdim=True) + 1e-5) * gain.double()
+    slack = (width / 2 + 6) * 2.0 ** -24
+    bounded(n8.dequantize(F32), n, half_step(n, slack) + n.abs() * slack * 1.1, "rows")
+    assert not bool(unpacked(n8)[0].view(torch.uint8)[:, width:].any())
+
+
+@pytest.mark.parametrize("rows", [3, 40, 700])
+def test_products_of_views(T, rows):
+    """Rows, bias and residual off their boundaries and apart, against dense copies of them."""
+    gen = torch.Generator().manual_seed(rows)
+    base = acts(gen, rows, 1200, BF16).cuda()
+    w8 = T.pack8(weight(gen, 515, 264).cuda())
+    bias = torch.randn(265, generator=gen).cuda()[1:]
+    for x in (base[:, 1:516], base[:, 8:523], base.t().contiguous().t()[:, :515]):
+        for r in (base[:, 700:964], base[:, 703:967], base.t().contiguous().t()[:, 600:864], base[:1, :264].expand(rows, 264)):
+            a = T.matmul8(x, w8, bias=bias, residual=r)
+            b = T.matmul8(x.contiguous(), w8, bias=bias.clone(), residual=r.contiguous())
+            same(a, b.double().cpu())
+
+
 def sum_error(x, w):
     """The bound on the instruction's cuts for float64 rows (M, K) and weight (K, N), and float32's sums."""
     m, k = x.shape
@@ -321,6 +354,33 @@ def test_swiglu(T, rows, k, n, biased):
     scale = scales_of(top.repeat_interleave(32, -1))[:, :n]
     half = torch.maximum((want.abs() + err) * HALF8, scale * 2.0 ** -10)
     bounded(got.dequantize(F32), want, half + err, "gate")
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 1024, 2816), (1, 2048, 700), (5, 515, 330), (16, 768, 704), (40, 1000, 320), (100, 256, 96)])
+@pytest.mark.parametrize("factor", [1.0, 2.0 ** 90])
+def test_swiglu_of_few_rows_is_float32s(T, rows, k, n, factor):
+    """A few rows' sums have float32's error alone, so that hardly a value falls to its neighbour."""
+    gen = torch.Generator().manual_seed(rows + k + n)
+    x, w = acts(gen, rows, k, F32) * factor, weight(gen, k, 2 * n, F32) / factor
+    w8 = T.pack8(w.cuda(), gated=True)
+    got = T.swiglu8(T.quantize8(x.cuda()), w8).dequantize(F32).double().cpu()
+    xr, wr = round8(x.double()), rounded_weight(w)
+    h, e = xr @ wr, xr.abs() @ wr.abs() * (k / 8 + 16) * 2.0 ** -24
+    v, g = h[:, :n], h[:, n:]
+    silu = g * torch.sigmoid(g)
+    want = v * silu
+    # silu and the product in float32: the exponential's argument is off by |g| 2^-24, five roundings more
+    err = 1.01 * (e[:, :n] * (silu.abs() + 1.1 * e[:, n:]) + 1.1 * v.abs() * e[:, n:] + want.abs() * (g.abs() + 8) * 2.0 ** -23) + 1e-30
+    lo, hi = round8(want - err), round8(want + err)
+    sure = (lo == hi) & (scales_of(want.abs() + err) == scales_of((want.abs() - err).clamp(min=0.0)))
+    # How many of the values the bound leaves to compare says nothing of the kernel: at 1024 normal products
+    # e is 144 2^-24 650 / 32 = 1.7e-4, of each factor, where their sizes are about 1; borders lie 2^-3 apart
+    # at most, so an even value is within 2 (2 1.7e-4) 8 = 0.6 % of one, and the tenth whose factor is under
+    # a tenth in size ten times as often or more: some 5 % in all.
+    assert float(sure.double().mean()) > 0.85
+    same(got[sure], lo[sure], "far from a border")
+    # the others fall to one of the two sides (a scale's own border moves no value by more)
+    assert bool(((got - want).abs() <= half_step(want, 0.0) * 2 + err).all())
 
 
 def test_block_of_a_model(T):
