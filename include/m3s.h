@@ -728,7 +728,7 @@ int32_t m3s_distill_bwd(const m3s_distill_args* args, void* stream);
 #define M3S_DTYPE_ROWS8 2              /* of m3s_matmul8_args.x_dtype alone */
 #define M3S_ROWS8_MAX 16777215         /* rows: 2^24 - 1 */
 #define M3S_ROWS8_WIDTH_MAX 1048576    /* width: 2^20; with a norm 16384 */
-#define M3S_MATMUL8_FLOAT_ROWS 16
+#define M3S_MATMUL8_FLOAT_ROWS 256     /* rows of floats that m3s_matmul8 rounds itself */
 
 /* Rows to 8 bits. With a gain the rows are first normalised, as m3s_rms_fwd does, and with `add`
  * the residual is added before that: s = x + add in x_dtype goes to `sum`, and the rows are those of

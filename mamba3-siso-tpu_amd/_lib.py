@@ -282,7 +282,7 @@ class Matmul8Args(C.Structure):
 
 #: ``M3S_DTYPE_ROWS8``, and the limits of the rows in 8 bits (``M3S_ROWS8_*``, ``M3S_MATMUL8_*``)
 DTYPE_ROWS8 = 2
-ROWS8_MAX, ROWS8_WIDTH_MAX, ROWS8_NORM_MAX, MATMUL8_FLOAT_ROWS = (1 << 24) - 1, 1 << 20, 16384, 16
+ROWS8_MAX, ROWS8_WIDTH_MAX, ROWS8_NORM_MAX, MATMUL8_FLOAT_ROWS = (1 << 24) - 1, 1 << 20, 16384, 256
 
 #: ``M3S_GEMV_*``
 GEMV_NORM, GEMV_GATE, GEMV_HEAD = 1, 2, 3

@@ -12,7 +12,7 @@ the rate of bf16, and a weight takes half the memory and half the traffic.
 * `swiglu8`    -- the gated MLP's first product and its gate, the rows out in 8 bits.
 
 Each is one launch of ``csrc/m3s_rows8.hip`` or ``csrc/m3s_matmul8.hip`` (`matmul8` and `swiglu8` of
-more than 16 float rows two), called from C++ (``csrc/m3s_nodes.cpp``) for dense operands of the kernels'
+more than a few float rows two), called from C++ (``csrc/m3s_nodes.cpp``) for dense operands of the kernels'
 types and from here for others. They take no gradient and refuse operands that need one.
 `model.eight_bit_params` makes a model of them.
 """
@@ -244,6 +244,17 @@ def pack8(w: Tensor, gated: bool = False) -> Weight8:
     return Weight8(q.values, c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, bool(gated))
 
 
+def _in_one_launch(x: Tensor, rows: int, w: Weight8) -> bool:
+    """Whether a product rounds its float rows itself. Each of its workgroups (64 outputs, 16 rows) then
+    rounds all that it reads, which saves a launch as long as the CUs have one each and a row is short.
+    us in two launches and in one: 16 x 1024 x 4480 bf16 6.1, 4.5; 96 rows (420 workgroups) 7.0, 6.3 and 128
+    rows 7.8, 10.8; 96 x 2048 x 1024 bf16 7.2, 5.9, float32 7.2, 7.3; 16 x 4096 x 2048 bf16 8.5, 8.7, float32
+    8.5, 11.5; 1 x 8192 x 4096 bf16 12.2, 17.1; 1 x 1024 x 32000 (500 workgroups) 7.6, 9.7. The same rule
+    stands in ``csrc/m3s_nodes.cpp``."""
+    return (rows <= _lib.MATMUL8_FLOAT_ROWS and w.values.shape[0] // 4 * ((rows + 15) // 16) <= 256
+            and x.shape[-1] * x.element_size() <= 8192)
+
+
 def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
     """The args struct of a product with its rows, weight and bias filled in, and what it keeps alive."""
     if not isinstance(w, Weight8):
@@ -265,7 +276,7 @@ def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
             bias = bias.float().contiguous()
     rows = _count(lead)
     _check_sizes(what, rows, width)
-    if not is8 and rows > _lib.MATMUL8_FLOAT_ROWS:
+    if not is8 and not _in_one_launch(x, rows, w):
         x, is8 = quantize8(x), True
     a = _lib.Matmul8Args()
     a.struct_size = ctypes.sizeof(_lib.Matmul8Args)
@@ -283,7 +294,7 @@ def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
 def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[str] = None,
             residual: Optional[Tensor] = None) -> Tensor:
     """``act(x @ w + bias) + residual`` in bf16, (..., n): ``x`` (..., k) is `Rows8`, or float32 or bf16
-    rows, which are rounded to 8 bits first (`quantize8`; up to 16 rows in the same launch); ``bias``
+    rows, which are rounded to 8 bits first (`quantize8`; a few rows in the same launch); ``bias``
     (n,) float32 or bf16; ``activation`` None, "silu", "gelu" (with erf) or "relu"; ``residual``
     (..., n) bf16, such as a bf16 model's stream. All but the operands in 8 bits is float32 up to the
     one rounding of the result. A row with a NaN or an infinity comes out NaN."""
