@@ -341,6 +341,20 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
 // other's products: with one of 256 x 256 outputs there they stood in line (16384 x 1024 x 4480:
 // 104 us, of them 31 for the outputs and some 25 until a tile's first products).
 constexpr int kBand = 16;
+// Outputs past the L2s (8 of 4 MB) go by them: kept there they push out the operands, and are gone when
+// they are read again. (us, 16384 x 1024 x 4480 over rotating buffers 106, so 75; 8192 rows 50, 41; a
+// model's forward of 16384 tokens, d_model 2048, 3500, 3430; d_model 1024, which reads 147 MB back at once,
+// 1715, 1724.)
+constexpr int64_t kPastCache = 32 << 20;
+__device__ __forceinline__ void store_once(const M8Params& p, bf16* to, bf16x8 o) {
+  if (p.vec & 4) {
+    asm volatile("" ::: "memory");   // else the two stores become a plain one
+    __builtin_nontemporal_store(o, reinterpret_cast<bf16x8*>(to));
+    asm volatile("" ::: "memory");
+  } else {
+    *reinterpret_cast<bf16x8*>(to) = o;
+  }
+}
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // A wave's accumulators: group q's tile T and row tile j; element 4 u + e of lane (c, h) is row
@@ -433,7 +447,7 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
             o[e] = (bf16)(a[e] + bias[e] + (float)res[i][e]);
             o[4 + e] = (bf16)(d[e] + bias[4 + e] + (float)res[i][4 + e]);
           }
-          if (m < p.M && n < p.N) *reinterpret_cast<bf16x8*>(p.y + m * p.ldy + n) = o;
+          if (m < p.M && n < p.N) store_once(p, p.y + m * p.ldy + n, o);
         }
         wave_sync();
       }
@@ -470,7 +484,7 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
 #pragma unroll
       for (int i = 0; i < 32 / RI; ++i) {
         const bf16x8 o = *reinterpret_cast<const bf16x8*>(sb + (i * RI + lane / PR) * LD + 8 * piece);
-        if (mj + RI * i < p.M && n < p.N) *reinterpret_cast<bf16x8*>(yr + (int64_t)(RI * i) * p.ldy) = o;
+        if (mj + RI * i < p.M && n < p.N) store_once(p, yr + (int64_t)(RI * i) * p.ldy, o);
       }
       wave_sync();
     }
@@ -730,7 +744,7 @@ extern "C" int32_t m3s_matmul8(const m3s_matmul8_args* a, void* stream) {
                      (!p.residual || (aligned16(p.residual) && p.ldr % 8 == 0));
   const int xs = a->x_dtype == M3S_DTYPE_F32 ? 4 : 2;
   const bool xvec = floats && p.K % 8 == 0 && aligned16(p.x) && p.ldx % (16 / xs) == 0;
-  p.vec = (whole ? 1 : 0) | (xvec ? 2 : 0);
+  p.vec = (whole ? 1 : 0) | (xvec ? 2 : 0) | (a->rows * (int64_t)a->n * 2 > kPastCache ? 4 : 0);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a->gated) dispatch8<true>(p, a->x_dtype, s);
   else dispatch8<false>(p, a->x_dtype, s);
