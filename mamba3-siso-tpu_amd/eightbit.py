@@ -58,6 +58,7 @@ class Rows8(NamedTuple):
             if y is not None:
                 return y
         rows = _check_rows8(self, "dequantize")
+        K._device_of(self.values, self.scales)
         y = K.empty(*self.lead, self.width, device=self.values.device, dtype=dtype)
         a = _lib.Rows8ValuesArgs(ctypes.sizeof(_lib.Rows8ValuesArgs), _lib.dtype_code(dtype), self.width,
                                  rows, self.values.data_ptr(), self.scales.data_ptr(), y.data_ptr())
@@ -96,6 +97,15 @@ def _check_rows8(x: Rows8, what: str) -> int:
             or not x.values.is_contiguous() or not x.scales.is_contiguous()):
         raise ValueError(f"{what}: rows must be dense Rows8 of {rows} x {x.width}")
     return rows
+
+
+def _check_weight8(w: Weight8, what: str) -> None:
+    tiles = _padded(w.n, 128) // 8 if w.gated else _padded(w.n, 64) // 16
+    steps = _padded(w.k, STEP) // STEP
+    if (tuple(w.values.shape) != (tiles, steps, 2, 64, 16) or tuple(w.scales.shape) != (steps, tiles // 4, 64, 4)
+            or w.values.dtype != torch.float8_e4m3fn or w.scales.dtype != torch.float8_e8m0fnu
+            or not w.values.is_contiguous() or not w.scales.is_contiguous()):
+        raise ValueError(f"{what}: the weight must be a dense Weight8 of {w.shape} (pack8)")
 
 
 def _shapes(rows: int, width: int) -> tuple:
@@ -265,7 +275,8 @@ def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
     lead, width = tuple(x.shape[:-1]), x.shape[-1]
     if width != w.k:
         raise ValueError(f"{what}: rows of {width} for a weight of {w.shape}")
-    dev = K._device_of(x.values if is8 else x, w.values, w.scales, bias)
+    _check_weight8(w, what)
+    dev = K._device_of(*((x.values, x.scales) if is8 else (x,)), w.values, w.scales, bias)
     K.refuse_gradient(what, None if is8 else x, bias)
     columns = w.shape[1]
     if bias is not None:

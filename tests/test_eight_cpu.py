@@ -141,6 +141,34 @@ def test_nothing_runs_on_the_cpu(T):
         T.pack8(torch.randn(4, 4, 4))
 
 
+def test_operands_that_are_not_what_they_say(T):
+    """Rows and weights put together or cut by hand are refused by their shapes, before a launch could
+    read past them."""
+    f8, e8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+    x = torch.randn(3, 200)
+    w = T.Weight8(torch.zeros(4, 2, 2, 64, 16, dtype=f8), torch.zeros(2, 1, 64, 4, dtype=torch.uint8).view(e8), 200, 64, False)
+    g = T.Weight8(torch.zeros(16, 2, 2, 64, 16, dtype=f8), torch.zeros(2, 4, 64, 4, dtype=torch.uint8).view(e8), 200, 128, True)
+    r = T.Rows8(torch.zeros(1, 2, 2, 64, 16, dtype=f8), torch.zeros(8, 128, dtype=torch.uint8).view(e8), 200, (3,))
+    for good, call in ((w, T.matmul8), (g, T.swiglu8)):
+        with pytest.raises(ValueError, match="ROCm device"):
+            call(x, good)
+        for bad in (good._replace(n=good.n + 65), good._replace(values=good.values[:, :1]), good._replace(gated=not good.gated),
+                    good._replace(scales=good.scales[:1]), good._replace(values=good.values.view(torch.uint8)),
+                    good._replace(values=good.values.transpose(0, 1).contiguous().transpose(0, 1)),
+                    good._replace(scales=good.scales.view(torch.uint8))):
+            with pytest.raises(ValueError, match="dense Weight8"):
+                call(x, bad)
+        with pytest.raises(ValueError, match="rows of 200"):
+            call(x, good._replace(k=300))
+        with pytest.raises(ValueError, match="ROCm device"):
+            call(r, good)
+    with pytest.raises(ValueError, match="ROCm device"):
+        r.dequantize()
+    for bad in (r._replace(lead=(17,)), r._replace(width=257), r._replace(scales=r.scales[:4]), r._replace(values=r.values.view(torch.uint8))):
+        with pytest.raises(ValueError, match="dense Rows8"):
+            bad.dequantize()
+
+
 def test_exports(m3):
     for name in ("Rows8", "Weight8", "quantize8", "rms_norm8", "pack8", "matmul8", "swiglu8"):
         assert getattr(m3, name) is getattr(m3.eightbit, name)
