@@ -263,6 +263,13 @@ PyObject* wrap_rows(Rows& r, at::IntArrayRef lead) {
                        (long long)r.width, sizes);
 }
 
+// An int's value, -1 past 64 bits (Python refuses it).
+int64_t whole_number(PyObject* o) {
+  const int64_t n = PyLong_AsLongLong(o);
+  if (n == -1) PyErr_Clear();
+  return n;
+}
+
 // A Rows8 as the argument holds it.
 bool unwrap_rows(PyObject* o, Rows& r, at::DimVector& lead) {
   if (!PyTuple_Check(o) || PyTuple_GET_SIZE(o) != 4) return false;
@@ -272,12 +279,12 @@ bool unwrap_rows(PyObject* o, Rows& r, at::DimVector& lead) {
   const Tensor* scales = given(PyTuple_GET_ITEM(o, 1), &device);
   PyObject *width = PyTuple_GET_ITEM(o, 2), *sizes = PyTuple_GET_ITEM(o, 3);
   if (!scales || !PyLong_Check(width) || !PyTuple_Check(sizes)) return false;
-  r.width = PyLong_AsLongLong(width);
+  r.width = whole_number(width);
   r.rows = 1;
   for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(sizes); ++i) {
     PyObject* n = PyTuple_GET_ITEM(sizes, i);
     if (!PyLong_Check(n)) return false;
-    const int64_t size = PyLong_AsLongLong(n);
+    const int64_t size = whole_number(n);
     if (size < 1 || size > M3S_ROWS8_MAX) return false;   // no rows: Python's
     lead.push_back(size);
     r.rows *= size;
@@ -396,7 +403,7 @@ PyObject* matmul8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (!wv) Py_RETURN_NONE;
   const at::Device device = wv->device();
   const Tensor* wsc = given(PyTuple_GET_ITEM(wt, 1), &device);
-  const int64_t k = PyLong_AsLongLong(PyTuple_GET_ITEM(wt, 2)), n = PyLong_AsLongLong(PyTuple_GET_ITEM(wt, 3));
+  const int64_t k = whole_number(PyTuple_GET_ITEM(wt, 2)), n = whole_number(PyTuple_GET_ITEM(wt, 3));
   if (!wsc || k < 1 || k > M3S_ROWS8_WIDTH_MAX || n < 1 || n > M3S_ROWS8_WIDTH_MAX) Py_RETURN_NONE;
   const int64_t tiles = (gated ? 2 * padded(n, 128) : padded(n, 64)) / 16, steps = padded(k, 128) / 128;
   if (wv->sizes() != at::IntArrayRef({tiles, steps, 2, 64, 16}) || wv->scalar_type() != at::kFloat8_e4m3fn ||

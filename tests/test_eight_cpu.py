@@ -152,7 +152,7 @@ def test_operands_that_are_not_what_they_say(T):
     for good, call in ((w, T.matmul8), (g, T.swiglu8)):
         with pytest.raises(ValueError, match="ROCm device"):
             call(x, good)
-        for bad in (good._replace(n=good.n + 65), good._replace(values=good.values[:, :1]), good._replace(gated=not good.gated),
+        for bad in (good._replace(n=good.n + 65), good._replace(n=1 << 70), good._replace(values=good.values[:, :1]), good._replace(gated=not good.gated),
                     good._replace(scales=good.scales[:1]), good._replace(values=good.values.view(torch.uint8)),
                     good._replace(values=good.values.transpose(0, 1).contiguous().transpose(0, 1)),
                     good._replace(scales=good.scales.view(torch.uint8))):
