@@ -178,51 +178,69 @@ __device__ __forceinline__ void static_for(F f) {
 constexpr int kFewWaves = 8;
 enum Rows8Kind { kRows8 = 0, kRowsBf16 = 1, kRowsF32 = 2 };
 
-// lane's operand and scale of rows m .. m + 15, step kb
+// A lane's share of rows m0 .. m0 + 15 of a step as memory holds it, so that nothing waits for its loads
+// where they are issued: 8 bits and a scale, or floats in 16-byte pieces. Rows behind the last read the
+// last one and give nothing but their own products, which are not stored.
 template <int XK>
-__device__ __forceinline__ void rows_operand(const M8Params& p, int64_t m0, int kb, int lane, i32x8_& b, int& sb) {
+struct RowsRaw {
+  i32x4_ v[XK == kRowsF32 ? 8 : 4];
+};
+template <>
+struct RowsRaw<kRows8> {
+  i32x8_ b;
+  int sb;
+};
+
+template <int XK>
+__device__ __forceinline__ void load_rows(const M8Params& p, int64_t m0, int kb, int lane, RowsRaw<XK>& x) {
   const int r = lane & 15, g = lane >> 4;
-  const int64_t m = m0 + r;
   if constexpr (XK == kRows8) {
-    // rows behind the last give nothing but their own products, which are not stored
     const int64_t tile = min(m0, p.M - 1) >> 4;
     const uint8_t* xr = static_cast<const uint8_t*>(p.x) + (tile * p.KB + kb) * 2048 + 16 * lane;
-    b = join8(*reinterpret_cast<const i32x4_*>(xr), *reinterpret_cast<const i32x4_*>(xr + 1024));
-    sb = p.xs[((int64_t)kb * 4 + g) * p.mp + scale_at(m)];
+    x.b = join8(*reinterpret_cast<const i32x4_*>(xr), *reinterpret_cast<const i32x4_*>(xr + 1024));
+    x.sb = p.xs[((int64_t)kb * 4 + g) * p.mp + scale_at(m0 + r)];
   } else {
     using TX = std::conditional_t<XK == kRowsBf16, bf16, float>;
+    constexpr int E = 16 / sizeof(TX);   // a piece's
+    const TX* xr = static_cast<const TX*>(p.x) + min(m0 + r, p.M - 1) * p.ldx;
+    const int c0 = kb * kStep8 + 16 * g;
+    if (p.vec & 2) {   // whole pieces; K % 8 == 0
+#pragma unroll
+      for (int i = 0; i < 32 / E; ++i) {
+        const int c = c0 + 64 * (i / (16 / E)) + E * (i % (16 / E));
+        x.v[i] = *reinterpret_cast<const i32x4_*>(xr + min(c, p.K - E));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32 / E; ++i) {
+        const int c = c0 + 64 * (i / (16 / E)) + E * (i % (16 / E));
+        TX t[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) t[e] = xr[min(c + e, p.K - 1)];
+        x.v[i] = __builtin_bit_cast(i32x4_, t);
+      }
+    }
+  }
+}
+
+// lane's operand and scale of them; `left` columns lie before the width's end
+template <int XK>
+__device__ __forceinline__ void rows_operand(const RowsRaw<XK>& x, int left, int lane, i32x8_& b, int& sb) {
+  if constexpr (XK == kRows8) {
+    b = x.b;
+    sb = x.sb;
+  } else {
+    const int r = lane & 15, g = lane >> 4;
     int q[8], byte[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int c = kb * kStep8 + 64 * h + 16 * g;
       float v[16];
-      if (m < p.M) {
-        const TX* xr = static_cast<const TX*>(p.x) + m * p.ldx + c;
-        if (p.vec & 2) {   // whole pieces of 16 bytes; K % 8 == 0
 #pragma unroll
-          for (int e = 0; e < 16; e += 8) {
-            if (c + e < p.K) {
-              if constexpr (XK == kRowsBf16) {
-                const bf16x8 t = *reinterpret_cast<const bf16x8*>(xr + e);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) v[e + i] = (float)t[i];
-              } else {
-                const f32x4 t = *reinterpret_cast<const f32x4*>(xr + e), s = *reinterpret_cast<const f32x4*>(xr + e + 4);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) { v[e + i] = t[i]; v[e + 4 + i] = s[i]; }
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[e + i] = 0.f;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) v[i] = c + i < p.K ? (float)xr[i] : 0.f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = 0.f;
+      for (int e = 0; e < 16; ++e) {
+        float f;
+        if constexpr (XK == kRowsF32) f = __builtin_bit_cast(f32x4, x.v[4 * h + e / 4])[e % 4];
+        else f = (float)__builtin_bit_cast(bf16x8, x.v[2 * h + e / 8])[e % 8];
+        v[e] = 64 * h + 16 * g + e < left ? f : 0.f;
       }
       uint32_t u = max_bits(v), o = (uint32_t)__shfl_xor((int)u, 16, 64);
       u = u > o ? u : o;
@@ -276,6 +294,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
   const uint8_t* wt = p.w + (int64_t)tile0 * p.KB * 2048 + 16 * lane;
   const uint8_t* st = p.ws + 64 * tile0 + 4 * lane;
   for (int kb = wave; kb < p.KB; kb += kFewWaves) {
+    RowsRaw<XK> x[MT];
+    // float rows are asked for before the weight, and rounded while it is on its way
+    if constexpr (XK != kRows8) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) load_rows<XK>(p, m0 + 16 * j, kb, lane, x[j]);
+    }
     i32x8_ a[NT];
     const int sa = *reinterpret_cast<const int*>(st + (int64_t)kb * p.NP * 4);
 #pragma unroll
@@ -283,10 +307,14 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
       const uint8_t* q = wt + ((int64_t)t * p.KB + kb) * 2048;
       a[t] = join8(*reinterpret_cast<const i32x4_*>(q), *reinterpret_cast<const i32x4_*>(q + 1024));
     }
+    if constexpr (XK == kRows8) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) load_rows<XK>(p, m0 + 16 * j, kb, lane, x[j]);
+    }
     i32x8_ b[MT];
     int sb[MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) rows_operand<XK>(p, m0 + 16 * j, kb, lane, b[j], sb[j]);
+    for (int j = 0; j < MT; ++j) rows_operand<XK>(x[j], p.K - kb * kStep8, lane, b[j], sb[j]);
     if constexpr (GATED) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // a plane's halves, each 8 k of a lane
@@ -296,9 +324,9 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
         for (int t = 0; t < NT; ++t) w[t] = widen8(a[t], i, sw >> (8 * t));
 #pragma unroll
         for (int j = 0; j < MT; ++j) {
-          const bf16x8 x = widen8(b[j], i, plane_scale(sb[j], lane, i >> 1));
+          const bf16x8 v = widen8(b[j], i, plane_scale(sb[j], lane, i >> 1));
 #pragma unroll
-          for (int t = 0; t < NT; ++t) acc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t], x, acc[j][t], 0, 0, 0);
+          for (int t = 0; t < NT; ++t) acc[j][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[t], v, acc[j][t], 0, 0, 0);
         }
       }
     } else {
