@@ -719,12 +719,14 @@ static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED>(p, s);
   if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED>(p, s);
   // By the workgroups that each form makes, of 256 CUs. Few rows go to the streaming form, 16 and 32 rows
-  // to a workgroup, as long as a CU has one, or two, of them; then come tiles of 128 x 64, 256 x 64 and
-  // 256 x 128 outputs x rows, each while the CUs have one of them. us of (16, 32 rows, the three tiles):
-  // 64 x 1024 x 4480 4.5, 4.4, 6.0, 7.7, 10.6; 256 rows 8.6, 7.9, 6.3, 8.0, 11; 1024 rows 25, 19, 13.2, 12.8, 12.2;
-  // 256 x 4096 x 4096 17, 14, 16, 21, 31; 1024 rows 62, 48, 28, 27, 35; 2048 rows 121, 91, 56, 45, 39.
+  // to a workgroup, as long as a CU has one, or two, of them, and up to 16 rows at any width (half of a tile
+  // of 32 would be empty: 16 x 2048 x 32000 11.6 and 11.8 us, the gate of 16 x 2048 x 16384 12.2 and 13.6);
+  // then come tiles of 128 x 64, 256 x 64 and 256 x 128 outputs x rows, each while the CUs have one of them.
+  // us of (16, 32 rows, the three tiles): 64 x 1024 x 4480 4.5, 4.4, 6.0, 7.7, 10.6; 256 rows 8.6, 7.9, 6.3,
+  // 8.0, 11; 1024 rows 25, 19, 13.2, 12.8, 12.2; 256 x 4096 x 4096 17, 14, 16, 21, 31; 1024 rows 62, 48, 28,
+  // 27, 35; 2048 rows 121, 91, 56, 45, 39.
   const int64_t g64 = p.NP / 64, g128 = (p.NP + 127) / 128, g256 = (p.NP + 255) / 256, r64 = (p.M + 63) / 64;
-  if (g64 * ((p.M + 15) / 16) <= 256) launch_few<1, kRows8, GATED>(p, s);
+  if (p.M <= 16 || g64 * ((p.M + 15) / 16) <= 256) launch_few<1, kRows8, GATED>(p, s);
   else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED>(p, s);
   else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED>(p, s);
   else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED>(p, s);

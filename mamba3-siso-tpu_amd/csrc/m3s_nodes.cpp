@@ -452,8 +452,8 @@ PyObject* matmul8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const bool poison = args[6] == Py_True;
   void* stream = stream_of(device);
   // one launch or two for float rows: eightbit._in_one_launch, with what both measured
-  if (x && (r.rows > M3S_MATMUL8_FLOAT_ROWS || tiles / 4 * ((r.rows + 15) / 16) > 256 ||
-            k * (int64_t)x->element_size() > 8192)) {
+  if (x && (r.rows > M3S_MATMUL8_FLOAT_ROWS || k * (int64_t)x->element_size() > 8192 ||
+            (r.rows * (int64_t)x->element_size() > 32 && tiles / 4 * ((r.rows + 15) / 16) > 256))) {
     r = fresh_rows(r.rows, r.width, device, poison);
     m3s_rows8_args q = rows8_args(*x, stride, r);
     check(lib.rows8(&q, stream), "m3s_rows8");

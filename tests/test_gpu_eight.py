@@ -510,3 +510,21 @@ def test_refusals(T):
             bad()
     with torch.no_grad():
         T.matmul8(x.clone().requires_grad_(), w8)
+
+
+@pytest.mark.parametrize("rows", [1, 8, 9, 16, 17])
+def test_few_rows_of_wide_products(T, rows):
+    """More workgroups than CUs: rounded in the launch or before it, a row has the same bits and the same sums."""
+    k, n = 200, 17000
+    gen = torch.Generator().manual_seed(rows)
+    x, w = acts(gen, rows, k, BF16), weight(gen, k, n)
+    xr, wr = round8(x.double()), rounded_weight(w)
+    want, w8 = xr @ wr, T.pack8(w.cuda())
+    err = (xr.abs() @ wr.abs()) * (7 * 2.0 ** -13 + (k / 8 + 8) * 2.0 ** -24) + want.abs() * HALF16 * 1.01
+    got = T.matmul8(T.quantize8(x.cuda()), w8)
+    bounded(got, want, err, "Rows8")
+    gate = T.pack8(torch.cat([w, w.flip(1)], 1).cuda(), gated=True)
+    g8 = unpacked(T.swiglu8(T.quantize8(x.cuda()), gate))
+    for f in (x.cuda(), x.float().cuda(), x.cuda().t().contiguous().t()):
+        same(T.matmul8(f, w8), got.double().cpu(), "floats")
+        assert all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(unpacked(T.swiglu8(f, gate)), g8))
