@@ -27,6 +27,7 @@
 
 #include "m3s_eight.h"
 #include "m3s_internal.h"
+#include "m3s_tiles8.h"
 
 namespace m3s {
 
@@ -601,29 +602,34 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
   for (int i = 0; i < LN; ++i) ow[i] = (uint32_t)min(wave * LN + i, ntiles - 1 - tile0) * wstep + 16 * lane;
 #pragma unroll
   for (int i = 0; i < LM; ++i) ox[i] = (uint32_t)min(wave * LM + i, rtiles - 1) * wstep + 16 * lane;
-  // behind the last step the loads go through empty descriptors and touch no memory
+  // Behind the last step the loads go through empty descriptors, at offsets that lie in the operands
+  // whatever the range check makes of a uniform one, and touch no memory.
   auto load = [&](int stage, int s) {
     s = __builtin_amdgcn_readfirstlane(s);
-    const uint32_t bytes = s < S ? 0xfffffff0u : 0u;
+    const uint32_t bytes = s < S ? 0xfffffff0u : 0u, from = (uint32_t)step_within(s, S) * 1024;
     const __amdgpu_buffer_rsrc_t rw = make_rsrc(wbase, bytes), rx = make_rsrc(xbase, bytes);
     uint8_t* to = lds + stage * kStageBytes;
 #pragma unroll
-    for (int i = 0; i < LN; ++i) buf_load_lds16(rw, to + (wave * LN + i) * 1024, ow[i], (uint32_t)s * 1024);
+    for (int i = 0; i < LN; ++i) buf_load_lds16(rw, to + (wave * LN + i) * 1024, ow[i], from);
 #pragma unroll
-    for (int i = 0; i < LM; ++i) buf_load_lds16(rx, to + (NTL + wave * LM + i) * 1024, ox[i], (uint32_t)s * 1024);
+    for (int i = 0; i < LM; ++i) buf_load_lds16(rx, to + (NTL + wave * LM + i) * 1024, ox[i], from);
   };
   // group q's dword holds its four 16-row tiles' scales of a row; bit 4 of the lane picks the tile of a pair
-  const uint32_t osw = (uint32_t)(16 * tile0 + 32 * TN * wn) * 4 + 4 * (16 * h + (lane & 15));
+  const int grp0 = tile0 / 4 + TN / 2 * wn;
+  uint32_t osw[TN / 2];
+#pragma unroll
+  for (int q = 0; q < TN / 2; ++q) osw[q] = weight_scale_at(grp0 + q, p.NP / 64, 16 * h + (lane & 15));
   const int64_t mw = m0 + 32 * TM * wm;   // the wave's rows
   const uint32_t osx = (uint32_t)((int64_t)h * p.mp + (mw & ~(int64_t)127) + 4 * c);
   auto scales = [&](int s, int (&sw)[TN / 2], int& sx) {
     s = __builtin_amdgcn_readfirstlane(s);
+    const int at = step_within(s, S);
     const __amdgpu_buffer_rsrc_t rws = make_rsrc(p.ws, s < S ? (uint32_t)((int64_t)p.KB * p.NP * 4) : 0u);
     const __amdgpu_buffer_rsrc_t rxs = make_rsrc(p.xs, s < S ? (uint32_t)((int64_t)p.KB * p.mp * 4) : 0u);
 #pragma unroll
     for (int q = 0; q < TN / 2; ++q)
-      sw[q] = __builtin_amdgcn_raw_buffer_load_b32(rws, osw + 256 * q, (uint32_t)(s >> 1) * (uint32_t)p.NP * 4 + (s & 1) * 128, 0);
-    sx = __builtin_amdgcn_raw_buffer_load_b32(rxs, osx, (uint32_t)((int64_t)s * 2 * p.mp), 0);
+      sw[q] = __builtin_amdgcn_raw_buffer_load_b32(rws, osw[q], weight_scale_step(at, p.NP), 0);
+    sx = __builtin_amdgcn_raw_buffer_load_b32(rxs, osx, (uint32_t)((int64_t)at * 2 * p.mp), 0);
   };
   f32x16 acc[TN][TM];
 #pragma unroll

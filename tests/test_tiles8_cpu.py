@@ -1,0 +1,46 @@
+"""The index rules of the tiled products in 8 bits (``csrc/m3s_tiles8.h``), compiled for the host and held
+to the sizes of what they point into: a value that the kernel reads and throws away shows in no result."""
+
+import os
+import subprocess
+import sys
+
+import pytest
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mamba3-siso-tpu_amd", "csrc")
+
+
+def run(tmp_path, body):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text('#include <stdio.h>\n#include "m3s_tiles8.h"\nusing namespace m3s;\nint main() {\n' + body + "\n}\n")
+    subprocess.run([os.environ.get("CXX", "g++"), "-O1", "-std=c++17", "-Wall", "-Werror", "-I", CSRC, str(src), "-o", str(exe)],
+                   check=True, stdout=sys.stderr)
+    return subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+
+
+@pytest.mark.parametrize("tile_groups", [2, 4])
+def test_scales_of_a_weight_are_read_within_it(tmp_path, tile_groups):
+    """Every group of a tile of outputs, the last one's groups behind the weight too, every lane and every
+    step that is asked for, three behind the last."""
+    out = run(tmp_path, f"""
+  long bad = 0, calls = 0;
+  for (int np = 64; np <= 2048; np += 64)
+    for (int kb = 1; kb <= 5; ++kb) {{
+      const long bytes = (long)kb * np * 4;
+      const int groups = np / 64;
+      for (int g0 = 0; g0 < groups; g0 += {tile_groups})
+        for (int q = 0; q < {tile_groups}; ++q)
+          for (int entry = 0; entry < 32; ++entry)
+            for (int s = 0; s < 2 * kb + 3; ++s) {{
+              const int at = step_within(s, 2 * kb);
+              const long byte = (long)weight_scale_at(g0 + q, groups, entry) + weight_scale_step(at, np);
+              bad += at < 0 || at >= 2 * kb || byte < 0 || byte + 4 > bytes;
+              // a group of the weight has its own scales: dword (step of 128, group, lane 16 g + r)
+              const int g = 2 * (s & 1) + entry / 16;
+              if (s < 2 * kb && g0 + q < groups) bad += byte != (((long)(s / 2) * groups + g0 + q) * 64 + 16 * g + entry % 16) * 4;
+              ++calls;
+            }}
+    }}
+  printf("%ld %ld\\n", bad, calls);""")
+    bad, calls = map(int, out.split())
+    assert bad == 0 and calls > 100000
