@@ -640,11 +640,15 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
   int sw[3][TN / 2], sx[3];
   // half h's k of tile pair T: lane group 2 half + h of plane, rows c of both tiles
   const int lread = (c >> 4) * 1024 + h * 256 + (c & 15) * 16;
-  auto step = [&](auto rc, int s) {
+  auto step = [&](auto rc, auto behind, int s) {
     constexpr int R = decltype(rc)::value;
-    // this step's loads are done when only the next one's are under way; every wave has read the stage
-    // that the loads of the step after that fill
-    vm_wait_keep<kOps>();
+    // This step's loads are done when only the next one's are under way; every wave has read the stage
+    // that the loads of the step after that fill. The count holds where each step of the loop before it
+    // asked for its kOps, which the loop's carried registers keep alive; the last steps, behind the loop,
+    // ask for nothing more and wait for all.
+    constexpr bool kLast = decltype(behind)::value;
+    if constexpr (kLast) vm_wait_all();
+    else vm_wait_keep<kOps>();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     const uint8_t* at = lds + R * kStageBytes + lread;
@@ -658,7 +662,7 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
 #pragma unroll
     for (int j = 0; j < TM; ++j) b[j] = frag(NTL / 2 + wm * TM + j);
     __builtin_amdgcn_sched_barrier(0);
-    load((R + 2) % 3, s + 2);
+    if constexpr (!kLast) load((R + 2) % 3, s + 2);
     const int by = 8 * (c >> 4), sr = (int)((uint32_t)sx[R] >> (8 * ((int)(mw >> 5) & 3)));
 #pragma unroll
     for (int q = 0; q < TN / 2; ++q) {
@@ -676,7 +680,7 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
       __builtin_amdgcn_sched_group_barrier(0x010, (LN + LM + TN * TM - 1) / (TN * TM), 0);
     }
     __builtin_amdgcn_sched_barrier(0);
-    scales(s + 3, sw[R], sx[R]);
+    if constexpr (!kLast) scales(s + 3, sw[R], sx[R]);
     asm volatile("" ::: "memory");
   };
   const std::integral_constant<int, 0> r0;
@@ -692,12 +696,12 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
   __builtin_amdgcn_sched_barrier(0);
   int s = 0;
   for (; s + 3 <= S; s += 3) {   // no way out in the middle: the compiler would wait for scales just asked for
-    step(r0, s);
-    step(r1, s + 1);
-    step(r2, s + 2);
+    step(r0, std::false_type{}, s);
+    step(r1, std::false_type{}, s + 1);
+    step(r2, std::false_type{}, s + 2);
   }
-  if (s < S) step(r0, s);
-  if (s + 1 < S) step(r1, s + 1);
+  if (s < S) step(r0, std::true_type{}, s);
+  if (s + 1 < S) step(r1, std::true_type{}, s + 1);
   vm_wait_all();   // no load may reach LDS behind the workgroup's end
   const bool plain = (p.vec & 1) && p.act == kActNone && p.N % 8 == 0;
   if (!GATED) __syncthreads();
