@@ -274,7 +274,7 @@ class Rows8ValuesArgs(C.Structure):
 class Matmul8Args(C.Structure):
     _fields_ = [
         ("struct_size", i32), ("x_dtype", i32), ("k", i32), ("n", i32), ("gated", i32),
-        ("activation", i32), ("rows", i64), ("x", vp), ("ldx", i64), ("x_scales", vp), ("w", vp),
+        ("activation", i32), ("short_sums", i32), ("rows", i64), ("x", vp), ("ldx", i64), ("x_scales", vp), ("w", vp),
         ("w_scales", vp), ("bias", vp), ("residual", vp), ("ldres", i64), ("y", vp),
         ("ldy", i64), ("y_values", vp), ("y_scales", vp),
     ]

@@ -7,16 +7,18 @@
 // They stand for the projections of the LM (layer.py:233, 256; model.py:125-140, 231) on weights in
 // 8 bits.
 //
-// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 128 k at twice bf16's rate and applies a scale for
-// every 32 of them on the way. Its A operand is the weight and its B operand the rows, so a lane's
-// four accumulators are four neighbouring outputs of one row. Lane l (r = l & 15, g = l >> 4) gives
-// row r's k 16 g .. 16 g + 15 and 64 + 16 g .. of the 128, and the scale of its k 32 g .. 32 g + 31.
-// Its sums are short of float32's: of each 8 neighbouring products it cuts what is below 2^-13 of the
-// largest one's power of two, and adds the rest to the float32 accumulator (found with pairs of
-// products; groups of 8 do not touch each other). A product of N(0, 1) rows is 1.3e-5 off for any
-// K from 1024 to 16384, a 150th of a bf16 rounding and a thousandth of e4m3's: that is why products
-// leave in bf16 or 8 bits. The float32 route, e4m3 widened to bf16 and multiplied at half the rate,
-// would sum in full and round its operands no better.
+// Rows are the B operand and the weight A, so a lane's accumulators are neighbouring outputs of one row.
+// There are two ways to a sum, chosen by whoever packs the weight:
+//
+// Float32 (the default): e4m3 values and their scales widen to bf16, which holds them (widen8), and
+// v_mfma_f32_*_bf16 multiplies them: 4e-8 of a product of N(0, 1) rows, as float32 in any order.
+//
+// Short: v_mfma_scale_f32_*_f8f6f4 multiplies the 8 bits themselves, at twice bf16's rate, and applies a
+// scale for every 32 of them on the way. Of each 8 neighbouring products it cuts what is below 2^-13 of the
+// largest one's power of two, and adds the rest to the float32 accumulator (found with pairs of products;
+// groups of 8 do not touch each other). A product of N(0, 1) rows is 1.3e-5 off for any K from 1024 to
+// 16384; where large products cancel, small ones beside them are gone. What layouts and stores measure
+// below was measured with short sums, where it weighs most.
 //
 // Weights are packed once (eightbit.pack8) in the rows' own tiles, their outputs being the rows. Four
 // tiles are a group of 64 outputs: tile t, row 4 g + i is output 64 grp + 32 (t >> 1) + 8 g +
@@ -173,8 +175,10 @@ __device__ __forceinline__ void static_for(F f) {
 }
 
 // ---- few rows ---------------------------------------------------------------------------
-// The weight is the traffic. A workgroup takes a group of 64 outputs and 16 MT rows; its eight waves take the steps of K in turn, each loading its tiles straight to
-// registers, and their sums meet in LDS in wave order (deterministic). Float rows are rounded to 8
+// The weight is the traffic. A workgroup takes a group of 64 outputs and 16 MT rows; its eight waves take the steps of
+// K in turn, each loading its tiles straight to registers, and their sums meet in LDS in wave order
+// (deterministic). The loads hide what float32 sums take more than short ones (1 x 1024 x 4480 3.6 us, short 3.4;
+// 64 rows 4.4 and 4.0). Float rows are rounded to 8
 // bits on the way in: a block is two lanes' half rows.
 constexpr int kFewWaves = 8;
 enum Rows8Kind { kRows8 = 0, kRowsBf16 = 1, kRowsF32 = 2 };
@@ -267,8 +271,9 @@ __device__ __forceinline__ void rows_operand(const RowsRaw<XK>& x, int left, int
 __device__ __forceinline__ int plane_scale(int s, int lane, int h) {
   return __shfl(s, (lane & 15) + 16 * (2 * h + (lane >> 5)), 64);
 }
-// bytes 8 i .. 8 i + 7 of an operand, in bfloat16 with their scale 2^(byte - 127): exact, but that 256 2^120
-// and up (float32's last values, 3.4e38) is an infinity, as it is where the rows are read back
+// Bytes 8 i .. 8 i + 7 of an operand, in bfloat16 with their scale 2^(byte - 127): exact from 2^-126 to below
+// 2^128. 256 2^120 (float32's last values, 3.4e38) is an infinity, as it is where the rows are read back, and of
+// values of a block of the least scale, below 2^-126, the bits under 2^-133 are lost.
 __device__ __forceinline__ bf16x8 widen8(i32x8_ v, int i, int byte) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   const float s = __int_as_float((byte & 255) << 23);
@@ -279,7 +284,7 @@ __device__ __forceinline__ bf16x8 widen8(i32x8_ v, int i, int byte) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-template <int MT, int XK, bool GATED>
+template <int MT, int XK, bool GATED, bool SHORT>
 __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Params p) {
   constexpr int NT = 4;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -316,7 +321,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
     int sb[MT];
 #pragma unroll
     for (int j = 0; j < MT; ++j) rows_operand<XK>(x[j], p.K - kb * kStep8, lane, b[j], sb[j]);
-    if constexpr (GATED) {
+    if constexpr (!SHORT) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {   // a plane's halves, each 8 k of a lane
         const int sw = plane_scale(sa, lane, i >> 1);
@@ -361,9 +366,12 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
 }
 
 // ---- many rows --------------------------------------------------------------------------
-// v_mfma_scale_f32_32x32x64_f8f6f4: a 32-row tile of the weight is two packed tiles, and 64 k one of
-// their planes. Lane l (c = l & 31, h = l >> 5) gives row c's k 16 h .. and 32 + 16 h .., and its
-// scale of the 32 k of half h. A workgroup of four waves takes 32 TN WN outputs (packed rows) and
+// Tiles of 32 x 32: 32 rows of the weight are two packed tiles, and a step of 64 k one of their planes, of
+// which lane l (c = l & 31, h = l >> 5) has row c's k 16 h .. and 32 + 16 h ... Four
+// v_mfma_f32_32x32x16_bf16 take 8 k of either half each, with the scales of both blocks of row c; one
+// v_mfma_scale_f32_32x32x64_f8f6f4 (short sums) takes all 64, with the scale of block h. Three widenings of
+// two values to a product lie under it (8192^3: 775 us, 1.42 PFLOP/s, the library's in bf16 1.27; short sums
+// 392). A workgroup of four waves takes 32 TN WN outputs (packed rows) and
 // 32 TM WM rows. Each step of 64 k goes to LDS by direct loads as the lanes will read it, in planes of
 // 16 bytes a lane, two steps ahead of its products in a ring of three stages; the scales go to
 // registers. Two workgroups share a CU, so that one's loads, outputs and gates run under the
@@ -569,11 +577,12 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
   }
 }
 
-template <int WN, int WM, int TN, int TM, bool GATED>
+template <int WN, int WM, int TN, int TM, bool GATED, bool SHORT>
 __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params p) {
   constexpr int NW = WN * WM, NTL = 2 * TN * WN, MTL = 2 * TM * WM;   // 16-row tiles
   constexpr int LN = NTL / NW, LM = MTL / NW;    // tiles whose plane a wave loads
-  constexpr int kOps = LN + LM + TN / 2 + 1;     // vector memory operations of a step's loads
+  constexpr int NS = SHORT ? 1 : 2;              // scales of a lane's row: its half's block, or both blocks
+  constexpr int kOps = LN + LM + NS * (TN / 2 + 1);   // vector memory operations of a step's loads
   static_assert(NTL % NW == 0 && MTL % NW == 0 && TN % 2 == 0 && (TM == 1 || TM == 2 || TM == 4), "tiles");
   constexpr int kStageBytes = (NTL + MTL) * 1024, kShare = 32 * (32 * TN + 4) * 4;
   constexpr int kLds = 3 * kStageBytes > NW * kShare || GATED ? 3 * kStageBytes : NW * kShare;
@@ -618,18 +627,21 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
   const int grp0 = tile0 / 4 + TN / 2 * wn;
   uint32_t osw[TN / 2];
 #pragma unroll
-  for (int q = 0; q < TN / 2; ++q) osw[q] = weight_scale_at(grp0 + q, p.NP / 64, 16 * h + (lane & 15));
+  for (int q = 0; q < TN / 2; ++q) osw[q] = weight_scale_at(grp0 + q, p.NP / 64, (SHORT ? 16 * h : 0) + (lane & 15));
   const int64_t mw = m0 + 32 * TM * wm;   // the wave's rows
-  const uint32_t osx = (uint32_t)((int64_t)h * p.mp + (mw & ~(int64_t)127) + 4 * c);
-  auto scales = [&](int s, int (&sw)[TN / 2], int& sx) {
+  const uint32_t osx = (uint32_t)((SHORT ? (int64_t)h * p.mp : 0) + (mw & ~(int64_t)127) + 4 * c);
+  auto scales = [&](int s, int (&sw)[TN / 2][NS], int (&sx)[NS]) {
     s = __builtin_amdgcn_readfirstlane(s);
     const int at = step_within(s, S);
     const __amdgpu_buffer_rsrc_t rws = make_rsrc(p.ws, s < S ? (uint32_t)((int64_t)p.KB * p.NP * 4) : 0u);
     const __amdgpu_buffer_rsrc_t rxs = make_rsrc(p.xs, s < S ? (uint32_t)((int64_t)p.KB * p.mp * 4) : 0u);
 #pragma unroll
-    for (int q = 0; q < TN / 2; ++q)
-      sw[q] = __builtin_amdgcn_raw_buffer_load_b32(rws, osw[q], weight_scale_step(at, p.NP), 0);
-    sx = __builtin_amdgcn_raw_buffer_load_b32(rxs, osx, (uint32_t)((int64_t)at * 2 * p.mp), 0);
+    for (int e = 0; e < NS; ++e) {
+#pragma unroll
+      for (int q = 0; q < TN / 2; ++q)
+        sw[q][e] = __builtin_amdgcn_raw_buffer_load_b32(rws, osw[q], weight_scale_step(at, p.NP) + 64 * e, 0);
+      sx[e] = __builtin_amdgcn_raw_buffer_load_b32(rxs, osx, (uint32_t)((int64_t)(2 * at + e) * p.mp), 0);
+    }
   };
   f32x16 acc[TN][TM];
 #pragma unroll
@@ -637,7 +649,7 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
 #pragma unroll
     for (int j = 0; j < TM; ++j) acc[t][j] = f32x16{};
   }
-  int sw[3][TN / 2], sx[3];
+  int sw[3][TN / 2][NS], sx[3][NS];
   // half h's k of tile pair T: lane group 2 half + h of plane, rows c of both tiles
   const int lread = (c >> 4) * 1024 + h * 256 + (c & 15) * 16;
   auto step = [&](auto rc, auto behind, int s) {
@@ -663,21 +675,37 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
     for (int j = 0; j < TM; ++j) b[j] = frag(NTL / 2 + wm * TM + j);
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!kLast) load((R + 2) % 3, s + 2);
-    const int by = 8 * (c >> 4), sr = (int)((uint32_t)sx[R] >> (8 * ((int)(mw >> 5) & 3)));
+    const int by = 8 * (c >> 4), bx = 8 * ((int)(mw >> 5) & 3);
+    if constexpr (SHORT) {
+      const int sr = (int)((uint32_t)sx[R][0] >> bx);
 #pragma unroll
-    for (int q = 0; q < TN / 2; ++q) {
-      const int s4 = (int)((uint32_t)sw[R][q] >> by);
-      static_for<TM>([&](auto jc) {
-        constexpr int j = decltype(jc)::value;
-        acc[2 * q][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[2 * q], b[j], acc[2 * q][j], 0, 0, 0, s4, j, sr);
-        acc[2 * q + 1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[2 * q + 1], b[j], acc[2 * q + 1][j], 0, 0, 2, s4, j, sr);
-      });
-    }
-    // the loads between the products, and not before the first of them
+      for (int q = 0; q < TN / 2; ++q) {
+        const int s4 = (int)((uint32_t)sw[R][q][0] >> by);
+        static_for<TM>([&](auto jc) {
+          constexpr int j = decltype(jc)::value;
+          acc[2 * q][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[2 * q], b[j], acc[2 * q][j], 0, 0, 0, s4, j, sr);
+          acc[2 * q + 1][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[2 * q + 1], b[j], acc[2 * q + 1][j], 0, 0, 2, s4, j, sr);
+        });
+      }
+      // the loads between the products, and not before the first of them
 #pragma unroll
-    for (int i = 0; i < TN * TM; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-      __builtin_amdgcn_sched_group_barrier(0x010, (LN + LM + TN * TM - 1) / (TN * TM), 0);
+      for (int i = 0; i < TN * TM; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x010, (LN + LM + TN * TM - 1) / (TN * TM), 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {   // 8 k of either half, of block i >> 1
+        bf16x8 wa[TN];
+#pragma unroll
+        for (int t = 0; t < TN; ++t) wa[t] = widen8(a[t], i, sw[R][t / 2][i >> 1] >> (by + 16 * (t & 1)));
+#pragma unroll
+        for (int j = 0; j < TM; ++j) {
+          const bf16x8 xb = widen8(b[j], i, sx[R][i >> 1] >> (bx + 8 * j));
+#pragma unroll
+          for (int t = 0; t < TN; ++t) acc[t][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wa[t], xb, acc[t][j], 0, 0, 0);
+        }
+      }
     }
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (!kLast) scales(s + 3, sw[R], sx[R]);
@@ -709,38 +737,40 @@ __global__ void __launch_bounds__(64 * WN * WM, 2) matmul8_kernel(const M8Params
                              reinterpret_cast<float*>(lds) + wave * (kShare / 4));
 }
 
-template <int MT, int XK, bool GATED>
+template <int MT, int XK, bool GATED, bool SHORT>
 static void launch_few(const M8Params& p, hipStream_t s) {
   const dim3 grid((unsigned)(p.NP / 64), (unsigned)((p.M + 16 * MT - 1) / (16 * MT)));
-  hipLaunchKernelGGL((matmul8_few_kernel<MT, XK, GATED>), grid, dim3(64 * kFewWaves), 0, s, p);
+  hipLaunchKernelGGL((matmul8_few_kernel<MT, XK, GATED, SHORT>), grid, dim3(64 * kFewWaves), 0, s, p);
 }
 
-template <int WN, int WM, int TN, int TM, bool GATED>
+template <int WN, int WM, int TN, int TM, bool GATED, bool SHORT>
 static void launch_many(M8Params p, hipStream_t s) {
   p.tiles_n = (p.NP + 32 * TN * WN - 1) / (32 * TN * WN);
   p.tiles_m = (int)((p.M + 32 * TM * WM - 1) / (32 * TM * WM));
   const int64_t nb = (int64_t)p.tiles_m * p.tiles_n;
   const unsigned grid = (unsigned)(((nb + 7) >> 3) * 8);
-  hipLaunchKernelGGL((matmul8_kernel<WN, WM, TN, TM, GATED>), dim3(grid), dim3(64 * WN * WM), 0, s, p);
+  hipLaunchKernelGGL((matmul8_kernel<WN, WM, TN, TM, GATED, SHORT>), dim3(grid), dim3(64 * WN * WM), 0, s, p);
 }
 
-template <bool GATED>
+template <bool GATED, bool SHORT>
 static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
-  if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED>(p, s);
-  if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED>(p, s);
+  if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED, SHORT>(p, s);
+  if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED, SHORT>(p, s);
   // By the workgroups that each form makes, of 256 CUs. Few rows go to the streaming form, 16 and 32 rows
   // to a workgroup, as long as a CU has one, or two, of them, and up to 16 rows at any width (half of a tile
   // of 32 would be empty: 16 x 2048 x 32000 11.6 and 11.8 us, the gate of 16 x 2048 x 16384 12.2 and 13.6);
   // then come tiles of 128 x 64, 256 x 64 and 256 x 128 outputs x rows, each while the CUs have one of them.
-  // us of (16, 32 rows, the three tiles): 64 x 1024 x 4480 4.5, 4.4, 6.0, 7.7, 10.6; 256 rows 8.6, 7.9, 6.3,
-  // 8.0, 11; 1024 rows 25, 19, 13.2, 12.8, 12.2; 256 x 4096 x 4096 17, 14, 16, 21, 31; 1024 rows 62, 48, 28,
-  // 27, 35; 2048 rows 121, 91, 56, 45, 39.
+  // us of (16, 32 rows, the three tiles), weights in cache: 64 x 1024 x 4480 4.8, 4.4, 8.5, 11.3, 16.3; 256 rows
+  // 9.3, 8.9, 8.9, 11.7, 16.7; 768 rows 20.6, 17.5, 11.3, 12.5, 17.4; 4096 rows 39.5, 41.8, 40.6 (tiles);
+  // 256 x 4096 x 4096 17.5, 14.0, 26, 35, 53; 1024 rows -, 47, 37, 39, 54; 4096 rows 129, 116, 104 (tiles). The
+  // same borders do for short sums: 64 x 1024 x 4480 4.4, 4.0, 5.4, 6.7, 9.3; 256 rows 8.2, 7.3, 5.6, 7.0, 9.8; 768
+  // rows 18.1, 14.1, 8.1, 7.8, 10.5; 4096 rows 25, 25, 23.6 (tiles).
   const int64_t g64 = p.NP / 64, g128 = (p.NP + 127) / 128, g256 = (p.NP + 255) / 256, r64 = (p.M + 63) / 64;
-  if (p.M <= 16 || g64 * ((p.M + 15) / 16) <= 256) launch_few<1, kRows8, GATED>(p, s);
-  else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED>(p, s);
-  else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED>(p, s);
-  else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED>(p, s);
-  else launch_many<4, 1, 2, 4, GATED>(p, s);
+  if (p.M <= 16 || g64 * ((p.M + 15) / 16) <= 256) launch_few<1, kRows8, GATED, SHORT>(p, s);
+  else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED, SHORT>(p, s);
+  else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED, SHORT>(p, s);
+  else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED, SHORT>(p, s);
+  else launch_many<4, 1, 2, 4, GATED, SHORT>(p, s);
 }
 
 }  // namespace m3s
@@ -792,7 +822,7 @@ extern "C" int32_t m3s_matmul8(const m3s_matmul8_args* a, void* stream) {
   const bool xvec = floats && p.K % 8 == 0 && aligned16(p.x) && p.ldx % (16 / xs) == 0;
   p.vec = (whole ? 1 : 0) | (xvec ? 2 : 0) | (a->rows * (int64_t)a->n * 2 > kPastCache ? 4 : 0);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a->gated) dispatch8<true>(p, a->x_dtype, s);
-  else dispatch8<false>(p, a->x_dtype, s);
+  if (a->gated) a->short_sums ? dispatch8<true, true>(p, a->x_dtype, s) : dispatch8<true, false>(p, a->x_dtype, s);
+  else a->short_sums ? dispatch8<false, true>(p, a->x_dtype, s) : dispatch8<false, false>(p, a->x_dtype, s);
   return launch_status("m3s_matmul8");
 }

@@ -395,8 +395,9 @@ PyObject* matmul8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   if (PyErr_Occurred()) return nullptr;
   PyObject* wt = args[1];
   const bool gated = args[2] == Py_True;
-  if (torch::jit::tracer::isTracing() || !PyTuple_Check(wt) || PyTuple_GET_SIZE(wt) != 5 ||
-      PyTuple_GET_ITEM(wt, 4) != (gated ? Py_True : Py_False) || !PyLong_Check(PyTuple_GET_ITEM(wt, 2)) ||
+  if (torch::jit::tracer::isTracing() || !PyTuple_Check(wt) || PyTuple_GET_SIZE(wt) != 6 ||
+      PyTuple_GET_ITEM(wt, 4) != (gated ? Py_True : Py_False) || !PyBool_Check(PyTuple_GET_ITEM(wt, 5)) ||
+      !PyLong_Check(PyTuple_GET_ITEM(wt, 2)) ||
       !PyLong_Check(PyTuple_GET_ITEM(wt, 3)))
     Py_RETURN_NONE;
   const Tensor* wv = given(PyTuple_GET_ITEM(wt, 0), nullptr);
@@ -416,6 +417,7 @@ PyObject* matmul8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   a.n = (int32_t)n;
   a.gated = gated;
   a.activation = (int32_t)activation;
+  a.short_sums = PyTuple_GET_ITEM(wt, 5) == Py_True;
   a.w = wv->data_ptr();
   a.w_scales = wsc->data_ptr();
   Rows r;

@@ -2,8 +2,9 @@
 
 Rows and weights are e4m3 values in blocks of 32 along the axis that a product sums over, each block
 with a power of two as its scale: the smallest one (from 2^-126 on) by which the block's largest
-magnitude is at most 448, e4m3's largest value (`Rows8`). The matrix cores multiply this form at twice
-the rate of bf16, and a weight takes half the memory and half the traffic.
+magnitude is at most 448, e4m3's largest value (`Rows8`). A weight takes half the memory of bf16 and half
+the traffic. Products sum in float32; a weight packed with ``short_sums`` is multiplied by the matrix cores'
+own 8-bit form, at twice the rate of bf16 and with sums of fewer bits (`pack8`).
 
 * `quantize8`  -- rows to 8 bits;
 * `rms_norm8`  -- the residual's addition and the block norm, its rows in 8 bits;
@@ -69,13 +70,14 @@ class Rows8(NamedTuple):
 class Weight8(NamedTuple):
     """A projection's weight (k, n) packed for the products (`pack8`): ``values``
     (tiles, steps, 2, 64, 16) float8_e4m3fn, as of `Rows8` with the outputs for rows, and ``scales`` (steps, tiles / 4, 64, 4) float8_e8m0fnu.
-    ``gated``: its columns are value | gate, n of each."""
+    ``gated``: its columns are value | gate, n of each. ``short_sums``: how its products sum."""
 
     values: Tensor
     scales: Tensor
     k: int
     n: int
     gated: bool
+    short_sums: bool = False
 
     @property
     def shape(self) -> tuple:
@@ -229,10 +231,15 @@ def _packed_rows(n: int, gated: bool) -> Tensor:
     return col.reshape(-1)
 
 
-def pack8(w: Tensor, gated: bool = False) -> Weight8:
+def pack8(w: Tensor, gated: bool = False, short_sums: bool = False) -> Weight8:
     """The weight ``w`` (k, n) float32 or bf16 of a projection ``x @ w``, rounded to 8 bits in blocks
     along k (as `quantize8` rounds its columns) and laid out for `matmul8`; with ``gated`` its columns
-    are value | gate and it goes to `swiglu8`. Done once, when a model is loaded."""
+    are value | gate and it goes to `swiglu8`. Done once, when a model is loaded.
+
+    Products with it sum in float32 (the operands widened to bf16, which holds them). With ``short_sums``
+    the matrix cores multiply the 8 bits themselves, at twice that rate, and cut each of 8 neighbouring
+    products at 2^-13 of the power of two of the largest of them: 1.3e-5 of a sum over normal values, and
+    more of one whose large products cancel."""
     if w.dim() != 2 or w.dtype not in _FLOATS:
         raise ValueError(f"pack8: the weight must be (k, n) float32 or bf16, got {w.dtype} {tuple(w.shape)}")
     k, n = w.shape
@@ -251,7 +258,8 @@ def pack8(w: Tensor, gated: bool = False) -> Weight8:
     c = q.scales.view(torch.uint8).index_select(1, (at & ~127) + 4 * (at & 31) + (at >> 5 & 3))
     # (step, lane group, group of tiles, tile, row) -> (step, group of tiles, lane, tile)
     c = c.view(steps, 4, -1, 4, 16).permute(0, 2, 1, 4, 3).contiguous()
-    return Weight8(q.values, c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, bool(gated))
+    return Weight8(q.values, c.view(steps, -1, 64, 4).view(torch.float8_e8m0fnu), k, n, bool(gated),
+                   bool(short_sums))
 
 
 def _in_one_launch(x: Tensor, rows: int, w: Weight8) -> bool:
@@ -293,7 +301,7 @@ def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
         x, is8 = quantize8(x), True
     a = _lib.Matmul8Args()
     a.struct_size = ctypes.sizeof(_lib.Matmul8Args)
-    a.k, a.n, a.gated, a.rows = w.k, w.n, int(w.gated), rows
+    a.k, a.n, a.gated, a.short_sums, a.rows = w.k, w.n, int(w.gated), int(w.short_sums), rows
     if is8:
         _check_rows8(x, what)
         a.x_dtype, a.x, a.x_scales = _lib.DTYPE_ROWS8, x.values.data_ptr(), x.scales.data_ptr()
@@ -310,7 +318,7 @@ def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[s
     rows, which are rounded to 8 bits first (`quantize8`; a few rows in the same launch); ``bias``
     (n,) float32 or bf16; ``activation`` None, "silu", "gelu" (with erf) or "relu"; ``residual``
     (..., n) bf16, such as a bf16 model's stream. All but the operands in 8 bits is float32 up to the
-    one rounding of the result. A row with a NaN or an infinity comes out NaN."""
+    one rounding of the result, but for the sums of a weight packed with ``short_sums``. A row with a NaN or an infinity comes out NaN."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"matmul8: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     y = _lib.nodes().matmul8(x, w, False, ACTIVATIONS[activation], bias, residual, K.POISON_OUTPUTS)
@@ -348,8 +356,8 @@ def matmul8_into(x, w: Weight8, stride: int) -> Tensor:
 
 def swiglu8(x, w: Weight8, bias: Optional[Tensor] = None) -> Rows8:
     """``value * silu(gate)`` of ``value | gate = x @ w + bias`` in 8 bits (..., n), in float32 up to that
-    rounding: the gated MLP's first product on a weight packed with ``gated=True``. ``x`` and ``bias``
-    (2 n,) as in `matmul8`."""
+    rounding (but for the sums of a weight packed with ``short_sums``): the gated MLP's first product on a
+    weight packed with ``gated=True``. ``x`` and ``bias`` (2 n,) as in `matmul8`."""
     done = _lib.nodes().matmul8(x, w, True, 0, bias, None, K.POISON_OUTPUTS)
     if done is not None:
         return Rows8._make(done)

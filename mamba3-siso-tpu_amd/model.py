@@ -21,6 +21,7 @@ when no state is carried); per-token decode goes through the one-launch
 from __future__ import annotations
 
 import dataclasses
+import functools
 import math
 from typing import Any, NamedTuple, Optional
 
@@ -253,19 +254,19 @@ def decode_params(params: LMParams, cfg: LMConfig) -> LMParams:
     return params._replace(blocks=blocks)
 
 
-def eight_bit_params(params: LMParams, cfg: LMConfig) -> LMParams:
+def eight_bit_params(params: LMParams, cfg: LMConfig, short_sums: bool = False) -> LMParams:
     """``params`` on the device with each block's projection matrices (in_proj, out_proj, fc1, fc2) packed
     in 8 bits (`eightbit.pack8`), for serving: `lm_forward`, `lm_decode_step`, `train.DecodeGraph` and
-    `train.generate` take the result and run every projection on the matrix cores' 8-bit form, its rows
+    `train.generate` take the result and run every projection on rows and weights in 8 bits, the rows
     rounded on the way (the block norms and the MLP's gate leave them in 8 bits). Half the bf16
-    weights' memory and traffic. Embedding, head, norms, scan and states stay as they are. Needs the
-    bf16 policy; no gradient."""
+    weights' memory and traffic. Sums are float32's; ``short_sums`` doubles the products' rate over a
+    prompt with sums of fewer bits (`eightbit.pack8`). Embedding, head, norms, scan and states stay as
+    they are. Needs the bf16 policy; no gradient."""
     if _mm_dtype(cfg) != torch.bfloat16:
         raise ValueError(f"weights in 8 bits run under the bf16 policy, not {cfg.siso.policy_name}")
-    blocks = [b._replace(siso=b.siso._replace(in_proj=E8.pack8(b.siso.in_proj),
-                                              out_proj=E8.pack8(b.siso.out_proj)),
-                         mlp=None if b.mlp is None else MLPParams(E8.pack8(b.mlp.fc1, gated=True),
-                                                                  E8.pack8(b.mlp.fc2)))
+    pack = functools.partial(E8.pack8, short_sums=short_sums)
+    blocks = [b._replace(siso=b.siso._replace(in_proj=pack(b.siso.in_proj), out_proj=pack(b.siso.out_proj)),
+                         mlp=None if b.mlp is None else MLPParams(pack(b.mlp.fc1, gated=True), pack(b.mlp.fc2)))
               for b in params.blocks]
     return LMParams(params.embed.detach(), [_detach_block(b) for b in blocks], params.final_norm.detach(),
                     None if params.head is None else params.head.detach())
