@@ -432,6 +432,16 @@ def _check_eight(params: SISOParams, cfg: SISOConfig) -> None:
             or params.out_proj.shape != (cfg.d_inner, cfg.d_model)):
         raise ValueError(f"in_proj and out_proj must both be packed, {(cfg.d_model, cfg.d_in_proj)} and "
                          f"{(cfg.d_inner, cfg.d_model)}")
+    # these go to the kernels by address
+    h, n, dev = cfg.nheads, cfg.d_state, params.in_proj.device
+    for name, shape in (("dt_bias", (h,)), ("b_norm_weight", (n,)), ("c_norm_weight", (n,)),
+                        ("b_bias", (h, n)), ("c_bias", (h, n)), ("d_skip", (h,))):
+        t = getattr(params, name)
+        if t is None and name == "d_skip":
+            continue
+        if not isinstance(t, Tensor) or tuple(t.shape) != shape or t.device != dev:
+            raise ValueError(f"{name} must be {shape} on the layer's device {dev}, got "
+                             f"{(tuple(t.shape), t.device) if isinstance(t, Tensor) else t}")
     if LY.policy(cfg.policy_name).matmul != torch.bfloat16:
         raise ValueError(f"projections in 8 bits run under the bf16 policy, not {cfg.policy_name}")
     K.refuse_gradient("a layer in 8 bits", *(t for t in params if isinstance(t, Tensor)))
