@@ -60,6 +60,7 @@ class Rows8(NamedTuple):
                 return y
         rows = _check_rows8(self, "dequantize")
         K._device_of(self.values, self.scales)
+        K.refuse_gradient("dequantize", self.values, self.scales)
         y = K.empty(*self.lead, self.width, device=self.values.device, dtype=dtype)
         a = _lib.Rows8ValuesArgs(ctypes.sizeof(_lib.Rows8ValuesArgs), _lib.dtype_code(dtype), self.width,
                                  rows, self.values.data_ptr(), self.scales.data_ptr(), y.data_ptr())
