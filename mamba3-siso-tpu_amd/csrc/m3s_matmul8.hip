@@ -69,11 +69,10 @@ __device__ __forceinline__ uint32_t max_lanes16(uint32_t u) {   // over the four
   return u > o ? u : o;
 }
 
-// 8 neighbouring outputs n .. n + 7 of row m. PLAIN: all there, 16 bytes at once, no activation.
-template <bool PLAIN>
+// 8 neighbouring outputs n .. n + 7 of row m.
 __device__ __forceinline__ void finish8(const M8Params& p, int64_t m, int n, float (&v)[8]) {
-  if (!PLAIN && n >= p.N) return;
-  const bool whole = PLAIN || ((p.vec & 1) && n + 8 <= p.N);   // pointers and strides allow 16 bytes
+  if (n >= p.N) return;
+  const bool whole = (p.vec & 1) && n + 8 <= p.N;   // pointers and strides allow 16 bytes
   if (p.bias) {
     if (whole) {
       const f32x4 a = *reinterpret_cast<const f32x4*>(p.bias + n), b = *reinterpret_cast<const f32x4*>(p.bias + n + 4);
@@ -85,7 +84,7 @@ __device__ __forceinline__ void finish8(const M8Params& p, int64_t m, int n, flo
         if (n + i < p.N) v[i] += p.bias[n + i];
     }
   }
-  if (!PLAIN && p.act != kActNone) {
+  if (p.act != kActNone) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = act8(v[i], p.act);
   }
@@ -116,7 +115,7 @@ __device__ __forceinline__ void finish8(const M8Params& p, int64_t m, int n, flo
 
 // A group's four accumulator tiles of row m. The gate's block of 32 outputs is the row's four lanes;
 // outputs behind N are zeros (the packed weight has zero rows there), up to the rows' padded width.
-template <bool GATED, bool PLAIN>
+template <bool GATED>
 __device__ __forceinline__ void finish_group(const M8Params& p, int64_t m, int grp, int lane,
                                              const f32x4 (&acc)[4]) {
   const int g = lane >> 4;
@@ -126,7 +125,7 @@ __device__ __forceinline__ void finish_group(const M8Params& p, int64_t m, int g
       float v[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) { v[i] = acc[2 * h][i]; v[4 + i] = acc[2 * h + 1][i]; }
-      finish8<PLAIN>(p, m, 64 * grp + 32 * h + 8 * g, v);
+      finish8(p, m, 64 * grp + 32 * h + 8 * g, v);
     }
   } else {
     const int j = 32 * grp + 8 * g;
@@ -361,7 +360,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
       for (int w = 1; w < kFewWaves; ++w) v[t] += part[w][j][t][lane];
     }
     if (m >= p.M) continue;
-    finish_group<GATED, false>(p, m, tile0 / 4, lane, v);
+    finish_group<GATED>(p, m, tile0 / 4, lane, v);
   }
 }
 
@@ -555,7 +554,7 @@ __device__ __forceinline__ void finish_tile(const M8Params& p, const f32x16 (&ac
             const f32x4 a = *reinterpret_cast<const f32x4*>(sh + row * LD + n);
             const f32x4 d = *reinterpret_cast<const f32x4*>(sh + row * LD + n + 4);
             float v[8] = {a[0], a[1], a[2], a[3], d[0], d[1], d[2], d[3]};
-            finish8<false>(p, mj + row, n0 + n, v);
+            finish8(p, mj + row, n0 + n, v);
           }
         }
       } else {
