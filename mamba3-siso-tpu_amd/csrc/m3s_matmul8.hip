@@ -755,21 +755,13 @@ template <bool GATED, bool SHORT>
 static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
   if (x_dtype == M3S_DTYPE_BF16) return launch_few<1, kRowsBf16, GATED, SHORT>(p, s);
   if (x_dtype == M3S_DTYPE_F32) return launch_few<1, kRowsF32, GATED, SHORT>(p, s);
-  // By the workgroups that each form makes, of 256 CUs. Few rows go to the streaming form, 16 and 32 rows
-  // to a workgroup, as long as a CU has one, or two, of them, and up to 16 rows at any width (half of a tile
-  // of 32 would be empty: 16 x 2048 x 32000 11.6 and 11.8 us, the gate of 16 x 2048 x 16384 12.2 and 13.6);
-  // then come tiles of 128 x 64, 256 x 64 and 256 x 128 outputs x rows, each while the CUs have one of them.
-  // us of (16, 32 rows, the three tiles), weights in cache: 64 x 1024 x 4480 4.8, 4.4, 8.5, 11.3, 16.3; 256 rows
-  // 9.3, 8.9, 8.9, 11.7, 16.7; 768 rows 20.6, 17.5, 11.3, 12.5, 17.4; 4096 rows 39.5, 41.8, 40.6 (tiles);
-  // 256 x 4096 x 4096 17.5, 14.0, 26, 35, 53; 1024 rows -, 47, 37, 39, 54; 4096 rows 129, 116, 104 (tiles). The
-  // same borders do for short sums: 64 x 1024 x 4480 4.4, 4.0, 5.4, 6.7, 9.3; 256 rows 8.2, 7.3, 5.6, 7.0, 9.8; 768
-  // rows 18.1, 14.1, 8.1, 7.8, 10.5; 4096 rows 25, 25, 23.6 (tiles).
-  const int64_t g64 = p.NP / 64, g128 = (p.NP + 127) / 128, g256 = (p.NP + 255) / 256, r64 = (p.M + 63) / 64;
-  if (p.M <= 16 || g64 * ((p.M + 15) / 16) <= 256) launch_few<1, kRows8, GATED, SHORT>(p, s);
-  else if (g64 * ((p.M + 31) / 32) <= 512) launch_few<2, kRows8, GATED, SHORT>(p, s);
-  else if (g128 * r64 <= 256) launch_many<2, 2, 2, 1, GATED, SHORT>(p, s);
-  else if (g256 * r64 <= 256) launch_many<4, 1, 2, 2, GATED, SHORT>(p, s);
-  else launch_many<4, 1, 2, 4, GATED, SHORT>(p, s);
+  switch (form8(p.M, p.NP)) {
+    case kFew16: return launch_few<1, kRows8, GATED, SHORT>(p, s);
+    case kFew32: return launch_few<2, kRows8, GATED, SHORT>(p, s);
+    case kTiles64: return launch_many<2, 2, 2, 1, GATED, SHORT>(p, s);
+    case kTiles64Wide: return launch_many<4, 1, 2, 2, GATED, SHORT>(p, s);
+    case kTiles128: return launch_many<4, 1, 2, 4, GATED, SHORT>(p, s);
+  }
 }
 
 }  // namespace m3s

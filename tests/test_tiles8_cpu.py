@@ -44,3 +44,18 @@ def test_scales_of_a_weight_are_read_within_it(tmp_path, tile_groups):
   printf("%ld %ld\\n", bad, calls);""")
     bad, calls = map(int, out.split())
     assert bad == 0 and calls > 100000
+
+
+def test_every_form_has_its_sizes(tmp_path):
+    """The sizes that the GPU's tests take for a form take it, each form with whole pieces and an odd width."""
+    import test_gpu_eight_forms as forms
+
+    names = ["few16", "few32", "tiles64", "tiles64wide", "tiles128"]
+    cases = [(f, r, -(-n // 64) * 64, n) for f, r, k, n in forms.each(forms.FORMS)]
+    gated = [(f, r, -(-n // 128) * 256, n) for f, r, k, n in forms.each(forms.GATED_FORMS)]
+    out = run(tmp_path, "".join(f'printf("%d ", (int)form8({r}, {np}));' for _, r, np, _ in cases + gated) + 'puts("");')
+    assert [names[int(i)] for i in out.split()] == [c[0] for c in cases + gated]
+    for some in (cases, gated):
+        for f in names:
+            widths = [n for name, _, _, n in some if name == f]
+            assert any(n % 2 for n in widths) and any(n % 8 == 0 for n in widths), f
