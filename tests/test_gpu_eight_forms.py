@@ -91,3 +91,20 @@ def test_gates_of_every_form(T, form, rows, k, n, biased, short):
     top = torch.nn.functional.pad(want.abs() + err, (0, -n % 32)).unflatten(-1, (-1, 32)).amax(-1)
     half = torch.maximum((want.abs() + err) * HALF8, scales_of(top.repeat_interleave(32, -1))[:, :n] * 2.0 ** -10)
     bounded(got.dequantize(F32), want.cpu(), (half + err * 1.01 + 1e-30).cpu(), "gate")
+
+
+@pytest.mark.parametrize("short", [False, True])
+def test_outputs_past_the_caches(T, short):
+    """Over 32 MB of output, which goes by the L2s: every row, without a residual and with one."""
+    rows, k, n = 16400, 128, 1096
+    assert rows * n * 2 > 32 << 20
+    gen = torch.Generator().manual_seed(7)
+    x, w = acts(gen, rows, k, BF16).cuda(), weight(gen, k, n).cuda()
+    w8, q = T.pack8(w, short_sums=short), T.quantize8(x)
+    xr, wr = round8(x.double()), rounded_weight(w)
+    want, err = xr @ wr, (large_bound if short else float32_bound)(xr, wr)
+    bias, res = torch.randn(n, generator=gen).cuda(), acts(gen, rows, n, BF16).cuda()
+    for b, r in ((None, None), (bias, None), (None, res), (bias, res)):
+        full = want + (0 if b is None else b.double()) + (0 if r is None else r.double())
+        e = err + 2.0 ** -22 * (bias.double().abs() + res.double().abs()) + full.abs() * HALF16 * 1.01
+        bounded(T.matmul8(q, w8, bias=b, residual=r), full.cpu(), e.cpu(), f"{b is None} {r is None}")
