@@ -796,6 +796,9 @@ typedef struct m3s_matmul8_args {
   void* y_scales;
 } m3s_matmul8_args;
 int32_t m3s_matmul8(const m3s_matmul8_args* args, void* stream);
+/* 1 where float rows are best given to m3s_matmul8 as they are, 0 where m3s_rows8 should round them first
+ * (or must, or the sizes are none). */
+int32_t m3s_matmul8_takes_floats(int64_t rows, int32_t k, int32_t n, int32_t gated, int32_t x_dtype);
 
 #ifdef __cplusplus
 }

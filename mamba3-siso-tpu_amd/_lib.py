@@ -300,7 +300,7 @@ EXPORTS = ("m3s_abi_version", "m3s_last_error", "m3s_supported", "m3s_fwd_raw_su
            "m3s_gemv_fused", "m3s_embed_bwd_workspace_bytes", "m3s_embed_fwd", "m3s_embed_bwd",
            "m3s_logprob_fwd", "m3s_logprob_bwd", "m3s_distill_fwd", "m3s_distill_bwd",
            "m3s_logprob_workspace_bytes", "m3s_distill_workspace_bytes", "m3s_rows8", "m3s_rows8_values",
-           "m3s_matmul8")
+           "m3s_matmul8", "m3s_matmul8_takes_floats")
 
 _lib = None
 
@@ -411,6 +411,8 @@ def load(path: str = LIB_PATH) -> C.CDLL:
                      (lib.m3s_matmul8, Matmul8Args)):
         fn.restype = i32
         fn.argtypes = [C.POINTER(args), vp]
+    lib.m3s_matmul8_takes_floats.restype = i32
+    lib.m3s_matmul8_takes_floats.argtypes = [i64, i32, i32, i32, i32]
     _lib = lib
     return lib
 
@@ -436,7 +438,8 @@ def nodes(path: str = NODES_PATH):
         raise RuntimeError(f"{path} was built for torch {mod.torch_version}, not {torch.__version__}; rebuild it")
     mod.bind(*(C.cast(fn, vp).value for fn in (lib.m3s_embed_fwd, lib.m3s_embed_bwd,
                                                lib.m3s_embed_bwd_workspace_bytes, lib.m3s_last_error)))
-    mod.bind8(*(C.cast(fn, vp).value for fn in (lib.m3s_rows8, lib.m3s_rows8_values, lib.m3s_matmul8)))
+    mod.bind8(*(C.cast(fn, vp).value for fn in (lib.m3s_rows8, lib.m3s_rows8_values, lib.m3s_matmul8,
+                                                lib.m3s_matmul8_takes_floats)))
     _nodes = mod
     return mod
 

@@ -768,6 +768,16 @@ static void dispatch8(const M8Params& p, int x_dtype, hipStream_t s) {
 
 using namespace m3s;
 
+static int packed_outputs(int32_t n, bool gated) {
+  return (int)(gated ? 2 * padded8(n) : ((int64_t)n + 63) / 64 * 64);
+}
+
+extern "C" int32_t m3s_matmul8_takes_floats(int64_t rows, int32_t k, int32_t n, int32_t gated, int32_t x_dtype) {
+  if (rows < 0 || k < 1 || k > M3S_ROWS8_WIDTH_MAX || n < 1 || n > M3S_ROWS8_WIDTH_MAX) return 0;
+  if (x_dtype != M3S_DTYPE_BF16 && x_dtype != M3S_DTYPE_F32) return 0;
+  return rounds_in_launch(rows, packed_outputs(n, gated != 0), k, x_dtype == M3S_DTYPE_F32 ? 4 : 2);
+}
+
 extern "C" int32_t m3s_matmul8(const m3s_matmul8_args* a, void* stream) {
   clear_error();
   M3S_REQUIRE(a != nullptr, "m3s_matmul8: args is NULL");
@@ -803,7 +813,7 @@ extern "C" int32_t m3s_matmul8(const m3s_matmul8_args* a, void* stream) {
   p.yv = static_cast<uint8_t*>(a->y_values); p.ys = static_cast<uint8_t*>(a->y_scales);
   p.M = a->rows; p.mp = padded_rows(a->rows); p.ldx = a->ldx; p.ldr = a->ldres; p.ldy = a->ldy;
   p.K = a->k; p.KB = (int)(padded8(a->k) / kStep8); p.N = a->n; p.act = a->activation;
-  p.NP = (int)(a->gated ? 2 * padded8(a->n) : ((int64_t)a->n + 63) / 64 * 64);
+  p.NP = packed_outputs(a->n, a->gated != 0);
   // scales are read through 32-bit offsets, and a launch holds at most 2^31 workgroups' tiles
   M3S_REQUIRE((int64_t)p.KB * p.mp * 4 < (1ll << 31) && (int64_t)p.KB * p.NP * 4 < (1ll << 31),
               "m3s_matmul8: an operand's scales span 2 GiB or more");

@@ -47,6 +47,7 @@ struct Entries {   // of the loaded library, by bind()
   decltype(&m3s_rows8) rows8;   // by bind8()
   decltype(&m3s_rows8_values) values8;
   decltype(&m3s_matmul8) matmul8;
+  decltype(&m3s_matmul8_takes_floats) takes_floats;
 } lib = {};
 
 // The exception types of the Python binding's check().
@@ -453,9 +454,7 @@ PyObject* matmul8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   const c10::DeviceGuard guard(device);
   const bool poison = args[6] == Py_True;
   void* stream = stream_of(device);
-  // one launch or two for float rows: eightbit._in_one_launch, with what both measured
-  if (x && (r.rows > M3S_MATMUL8_FLOAT_ROWS || k * (int64_t)x->element_size() > 8192 ||
-            (r.rows * (int64_t)x->element_size() > 32 && tiles / 4 * ((r.rows + 15) / 16) > 256))) {
+  if (x && !lib.takes_floats(r.rows, a.k, a.n, gated, code(x->scalar_type()))) {
     r = fresh_rows(r.rows, r.width, device, poison);
     m3s_rows8_args q = rows8_args(*x, stride, r);
     check(lib.rows8(&q, stream), "m3s_rows8");
@@ -498,13 +497,14 @@ bool addresses(PyObject* const* args, Py_ssize_t nargs, void** at, Py_ssize_t co
   return true;
 }
 
-// bind8(m3s_rows8, m3s_rows8_values, m3s_matmul8): addresses.
+// bind8(m3s_rows8, m3s_rows8_values, m3s_matmul8, m3s_matmul8_takes_floats): addresses.
 PyObject* bind8(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
-  void* at[3];
-  if (!addresses(args, nargs, at, 3)) return nullptr;
+  void* at[4];
+  if (!addresses(args, nargs, at, 4)) return nullptr;
   lib.rows8 = reinterpret_cast<decltype(lib.rows8)>(at[0]);
   lib.values8 = reinterpret_cast<decltype(lib.values8)>(at[1]);
   lib.matmul8 = reinterpret_cast<decltype(lib.matmul8)>(at[2]);
+  lib.takes_floats = reinterpret_cast<decltype(lib.takes_floats)>(at[3]);
   Py_RETURN_NONE;
 }
 

@@ -4,6 +4,8 @@
 
 #include <stdint.h>
 
+#include "../../include/m3s.h"
+
 #ifdef __HIPCC__
 #define M3S_BOTH __host__ __device__ __forceinline__
 #else
@@ -33,6 +35,20 @@ M3S_BOTH Form8 form8(int64_t rows, int64_t np) {
   if (g128 * r64 <= 256) return kTiles64;
   if (g256 * r64 <= 256) return kTiles64Wide;
   return kTiles128;
+}
+
+// Whether a product rounds its float rows (k of `size` bytes) itself. Each of its workgroups, 64 outputs and 16
+// rows, then rounds all that it reads, which saves a launch as long as a CU rounds little: the rows' bytes times
+// the workgroups that a CU takes in turn. Up to 16 rows of bf16 or 8 of float32, whose weight is read once all the
+// same, it pays up to 8 KB a row at any width. us in one launch and in two, weights in cache: bf16 16 x 1024 x
+// 4480 5.0, 6.6; 112 rows (two turns) 6.8, 9.3; 160 (three) 9.1, 9.7; 192 (four) 10.9, 9.8; 48 x 2048 x 4480 (one)
+// 7.5, 8.9; 96 rows (two) 10.8, 10.1; 16 x 2048 x 32000 13.6, 16.2; 1 x 4096 x 8192 10.2, 9.4 (short sums 8.2,
+// 9.4), 64 rows 17.4, 12.6. float32: 48 x 1024 x 4480 5.8, 6.8; 64 rows (two) 8.1, 7.3; 8 x 2048 x 32000 13.9, 15.3;
+// 1 x 2048 x 1024 6.2, 6.8; 16 rows 8.8, 7.4.
+M3S_BOTH bool rounds_in_launch(int64_t rows, int64_t np, int64_t k, int size) {
+  if (rows > M3S_MATMUL8_FLOAT_ROWS) return false;
+  const int64_t turns = (np / 64 * ((rows + 15) / 16) + 255) / 256;
+  return turns * k * size <= 6144 || (rows * size <= 32 && k * size <= 8192);
 }
 
 // A step of 64 k that lies in the operands: loads are asked for up to three steps behind the last of S,

@@ -263,19 +263,6 @@ def pack8(w: Tensor, gated: bool = False, short_sums: bool = False) -> Weight8:
                    bool(short_sums))
 
 
-def _in_one_launch(x: Tensor, rows: int, w: Weight8) -> bool:
-    """Whether a product rounds its float rows itself. Each of its workgroups (64 outputs, 16 rows) then
-    rounds all that it reads, which saves a launch as long as a row is short and the CUs have a workgroup
-    each. Behind that many, it pays for one tile's rows in bf16, or half as many in float32, whose weight
-    is read once all the same. us in two launches and in one, bf16: 16 x 1024 x 4480 6.1, 4.3; 96 x 2048 x
-    1024 7.1, 5.7; 16 x 4096 x 2048 8.5, 8.4; 1 x 8192 x 4096 12.2, 12.1; of more than 256 workgroups 16 x
-    2048 x 32000 15.1, 12.6, 32 x 2048 x 8832 7.6, 10.7, 48 x 4096 x 8192 11.2, 15.0 (112 x 1024 x 4480 7.5,
-    5.7, left out). float32: 1 x 2048 x 1024 6.3, 5.3; 8 x 2048 x 32000 14.3, 13.0, 16 rows 14.9, 16.1. The
-    same rule stands in ``csrc/m3s_nodes.cpp``."""
-    return (rows <= _lib.MATMUL8_FLOAT_ROWS and x.shape[-1] * x.element_size() <= 8192
-            and (rows * x.element_size() <= 32 or w.values.shape[0] // 4 * ((rows + 15) // 16) <= 256))
-
-
 def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
     """The args struct of a product with its rows, weight and bias filled in, and what it keeps alive."""
     if not isinstance(w, Weight8):
@@ -298,7 +285,7 @@ def _operands(x, w: Weight8, bias: Optional[Tensor], what: str):
             bias = bias.float().contiguous()
     rows = _count(lead)
     _check_sizes(what, rows, width)
-    if not is8 and not _in_one_launch(x, rows, w):
+    if not is8 and not _lib.load().m3s_matmul8_takes_floats(rows, w.k, w.n, int(w.gated), _lib.dtype_code(x.dtype)):
         x, is8 = quantize8(x), True
     a = _lib.Matmul8Args()
     a.struct_size = ctypes.sizeof(_lib.Matmul8Args)

@@ -59,3 +59,18 @@ def test_every_form_has_its_sizes(tmp_path):
         for f in names:
             widths = [n for name, _, _, n in some if name == f]
             assert any(n % 2 for n in widths) and any(n % 8 == 0 for n in widths), f
+
+
+def test_one_rule_for_rows_rounded_in_the_launch():
+    """The library's own answer, which both callers take: turns of workgroups on 256 CUs times a row's bytes."""
+    from mamba3_siso_tpu_amd import _lib
+
+    takes, bf16, f32 = _lib.load().m3s_matmul8_takes_floats, _lib.DTYPE_BF16, _lib.DTYPE_F32
+    for rows, k, n, gated, dtype, want in (
+            (1, 1024, 4480, 0, bf16, 1), (112, 1024, 4480, 0, bf16, 1), (160, 1024, 4480, 0, bf16, 1), (192, 1024, 4480, 0, bf16, 0),
+            (80, 1024, 2816, 1, bf16, 1), (48, 2048, 4480, 0, bf16, 1), (96, 2048, 4480, 0, bf16, 0), (16, 2048, 32000, 0, bf16, 1),
+            (17, 2048, 32000, 0, bf16, 0), (16, 4096, 2048, 0, bf16, 1), (17, 4096, 2048, 0, bf16, 0), (16, 4097, 2048, 0, bf16, 0),
+            (48, 1024, 4480, 0, f32, 1), (64, 1024, 4480, 0, f32, 0), (8, 2048, 1024, 0, f32, 1), (9, 2048, 1024, 0, f32, 0),
+            (256, 200, 1000, 0, bf16, 1), (257, 200, 1000, 0, bf16, 0), (0, 64, 64, 0, bf16, 1), (-1, 64, 64, 0, bf16, 0),
+            (4, 0, 64, 0, bf16, 0), (4, 64, 0, 0, bf16, 0), (4, (1 << 20) + 1, 64, 0, bf16, 0), (4, 64, 64, 0, _lib.DTYPE_ROWS8, 0)):
+        assert takes(rows, k, n, gated, dtype) == want, (rows, k, n, gated, dtype)
