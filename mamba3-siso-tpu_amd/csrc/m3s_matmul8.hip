@@ -57,7 +57,8 @@ __device__ __forceinline__ float silu8(float v) {
 }
 __device__ __forceinline__ float act8(float v, int act) {
   if (act == kActSilu) return silu8(v);
-  if (act == kActGelu) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
+  // 1 + erf as erfc, which keeps its bits where the two cancel (at -5 the sum has four left)
+  if (act == kActGelu) return 0.5f * v * erfcf(v * -0.70710678118654752f);
   if (act == kActRelu) return v > 0.f ? v : (v == v ? 0.f : v);
   return v;
 }
