@@ -753,7 +753,7 @@ int32_t m3s_rows8(const m3s_rows8_args* args, void* stream);
 /* The values that rows in 8 bits stand for, dense. */
 typedef struct m3s_rows8_values_args {
   int32_t struct_size;  /* sizeof(m3s_rows8_values_args) */
-  int32_t y_dtype;      /* M3S_DTYPE_* of y (bf16 holds every value exactly) */
+  int32_t y_dtype;      /* M3S_DTYPE_* of y: exact, but that 2^128 is an infinity, and below 2^-130 bf16 rounds */
   int32_t width;
   int64_t rows;
   const void* values;

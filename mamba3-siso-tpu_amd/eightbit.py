@@ -53,7 +53,9 @@ class Rows8(NamedTuple):
         return (*self.lead, self.width)
 
     def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> Tensor:
-        """The values that the 8 bits stand for, (..., width) in bf16 (exact) or float32."""
+        """The values that the 8 bits stand for, (..., width) in float32 or bf16. Both hold them exactly, but for
+        float32's last values, which 8 bits hold as 2^128 (an infinity in either), and, in bf16, values of
+        a block of the least scale below 2^-130, which it may round (its steps are 2^-133)."""
         if dtype in _FLOATS:
             y = _lib.nodes().rows8_values(self, dtype is torch.bfloat16, K.POISON_OUTPUTS)
             if y is not None:
@@ -306,7 +308,8 @@ def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[s
     rows, which are rounded to 8 bits first (`quantize8`; a few rows in the same launch); ``bias``
     (n,) float32 or bf16; ``activation`` None, "silu", "gelu" (with erf) or "relu"; ``residual``
     (..., n) bf16, such as a bf16 model's stream. All but the operands in 8 bits is float32 up to the
-    one rounding of the result, but for the sums of a weight packed with ``short_sums``. A row with a NaN or an infinity comes out NaN."""
+    one rounding of the result, but for the sums of a weight packed with ``short_sums``. A row with a NaN or an infinity comes out NaN, and
+    one with a value that 8 bits hold as 2^128 may come out infinite or NaN."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"matmul8: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     y = _lib.nodes().matmul8(x, w, False, ACTIVATIONS[activation], bias, residual, K.POISON_OUTPUTS)
