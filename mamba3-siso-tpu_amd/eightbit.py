@@ -308,8 +308,8 @@ def matmul8(x, w: Weight8, bias: Optional[Tensor] = None, activation: Optional[s
     rows, which are rounded to 8 bits first (`quantize8`; a few rows in the same launch); ``bias``
     (n,) float32 or bf16; ``activation`` None, "silu", "gelu" (with erf) or "relu"; ``residual``
     (..., n) bf16, such as a bf16 model's stream. All but the operands in 8 bits is float32 up to the
-    one rounding of the result, but for the sums of a weight packed with ``short_sums``. A row with a NaN or an infinity comes out NaN, and
-    one with a value that 8 bits hold as 2^128 may come out infinite or NaN."""
+    one rounding of the result, but for the sums of a weight packed with ``short_sums``. A row with a NaN or
+    an infinity comes out NaN, and one with a value that 8 bits hold as 2^128 may come out infinite or NaN."""
     if activation not in ACTIVATIONS:
         raise ValueError(f"matmul8: activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
     y = _lib.nodes().matmul8(x, w, False, ACTIVATIONS[activation], bias, residual, K.POISON_OUTPUTS)

@@ -456,6 +456,8 @@ def _layer_eight(params: SISOParams, u, cfg: SISOConfig, state: Optional[SISOSta
     if len(u.shape) != 3:
         raise ValueError(f"u must be (B, L, d_model), got {tuple(u.shape)}")
     batch, seqlen = u.shape[:2]
+    if batch < 1 or seqlen < 1:
+        raise ValueError(f"u must hold a token at least, got {tuple(u.shape)}")
     d, vec = cfg.d_in_proj, 8
     if cfg.headdim % vec or cfg.d_state % vec or cfg.d_state // vec > 64:
         raise ValueError(f"no layer in 8 bits for headdim {cfg.headdim}, d_state {cfg.d_state}")

@@ -46,3 +46,11 @@ def test_vectors_that_are_missing(m3, layer):
     for call in calls(m3, cfg, p._replace(d_skip=None)):
         with pytest.raises(ValueError, match="ROCm device"):
             call()
+
+
+@pytest.mark.parametrize("shape", [(0, 64), (2, 0)])
+def test_no_tokens(m3, layer, shape):
+    """As the layer in bf16, a ValueError of its own."""
+    cfg, p = layer
+    with pytest.raises(ValueError, match="a token at least"):
+        m3.mamba3_siso_layer(p, torch.zeros(*shape, cfg.d_model, dtype=torch.bfloat16), cfg)
