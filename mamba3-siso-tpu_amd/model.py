@@ -200,9 +200,10 @@ def lm_template(cfg: LMConfig) -> LMParams:
 
 
 def refuse_packed(params: LMParams) -> None:
-    """Packed weights are no tensors of the model's shapes: they are not cast, moved, trained or stored."""
+    """Packed weights are no tensors of the model's shapes: they are not cast, moved, packed again, trained
+    or stored."""
     if _is_eight_bit(params):
-        raise ValueError("weights in 8 bits are for serving: cast, move, train or store the weights they "
+        raise ValueError("weights in 8 bits are for serving: cast, move, pack, train or store the weights they "
                          "were packed from")
 
 
@@ -262,6 +263,7 @@ def eight_bit_params(params: LMParams, cfg: LMConfig, short_sums: bool = False) 
     weights' memory and traffic. Sums are float32's; ``short_sums`` doubles the products' rate over a
     prompt with sums of fewer bits (`eightbit.pack8`). Embedding, head, norms, scan and states stay as
     they are. Needs the bf16 policy; no gradient."""
+    refuse_packed(params)
     if _mm_dtype(cfg) != torch.bfloat16:
         raise ValueError(f"weights in 8 bits run under the bf16 policy, not {cfg.siso.policy_name}")
     pack = functools.partial(E8.pack8, short_sums=short_sums)

@@ -54,3 +54,14 @@ def test_no_tokens(m3, layer, shape):
     cfg, p = layer
     with pytest.raises(ValueError, match="a token at least"):
         m3.mamba3_siso_layer(p, torch.zeros(*shape, cfg.d_model, dtype=torch.bfloat16), cfg)
+
+
+def test_packed_weights_are_not_packed_again(m3, layer):
+    cfg, p = layer
+    M = m3.model
+    lm = M.LMConfig(vocab_size=7, n_layers=1, siso=cfg)
+    params = M.init_lm(lm, 0)
+    params = params._replace(blocks=[b._replace(siso=p) for b in params.blocks])
+    for short in (False, True):
+        with pytest.raises(ValueError, match="for serving"):
+            M.eight_bit_params(params, lm, short_sums=short)
