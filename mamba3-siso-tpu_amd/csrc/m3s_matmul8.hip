@@ -370,7 +370,7 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
 // which lane l (c = l & 31, h = l >> 5) has row c's k 16 h .. and 32 + 16 h ... Four
 // v_mfma_f32_32x32x16_bf16 take 8 k of either half each, with the scales of both blocks of row c; one
 // v_mfma_scale_f32_32x32x64_f8f6f4 (short sums) takes all 64, with the scale of block h. Three widenings of
-// two values to a product lie under it (8192^3: 775 us, 1.42 PFLOP/s, the library's in bf16 1.27; short sums
+// two values to a product lie under it (8192^3: 763 us, 1.44 PFLOP/s, the library's in bf16 1.27; short sums
 // 392). A workgroup of four waves takes 32 TN WN outputs (packed rows) and
 // 32 TM WM rows. Each step of 64 k goes to LDS by direct loads as the lanes will read it, in planes of
 // 16 bytes a lane, two steps ahead of its products in a ring of three stages; the scales go to
@@ -379,9 +379,10 @@ __global__ void __launch_bounds__(64 * kFewWaves) matmul8_few_kernel(const M8Par
 // 104 us, of them 31 for the outputs and some 25 until a tile's first products).
 constexpr int kBand = 16;
 // Outputs past the L2s (8 of 4 MB) go by them: kept there they push out the operands, and are gone when
-// they are read again. (us, 16384 x 1024 x 4480 over rotating buffers 106, so 75; 8192 rows 50, 41; a
-// model's forward of 16384 tokens, d_model 2048, 3500, 3430; d_model 1024, which reads 147 MB back at once,
-// 1715, 1724.)
+// they are read again. (us with short sums, 16384 x 1024 x 4480 over rotating buffers 106, so 75; 8192 rows 50, 41;
+// a model's forward of 16384 tokens, d_model 2048, 3500, 3430; d_model 1024, which reads 147 MB back at once,
+// 1715, 1724. With float32 sums, whose products take as long as the outputs, either way is the same within
+// 2%: 8192 rows 73, 71; 32768 x 2048 x 1024 with a residual 123, 123.)
 constexpr int64_t kPastCache = 32 << 20;
 __device__ __forceinline__ void store_once(const M8Params& p, bf16* to, bf16x8 o) {
   if (p.vec & 4) {

@@ -20,14 +20,12 @@ enum Form8 { kFew16, kFew32, kTiles64, kTiles64Wide, kTiles128 };
 
 // The form of rows in 8 bits by np packed outputs, by the workgroups that each makes, of 256 CUs. Few rows go to
 // the streaming form, 16 and 32 rows to a workgroup, as long as a CU has one, or two, of them, and up to 16 rows
-// at any width (half of a tile of 32 would be empty: 16 x 2048 x 32000 12.4 and 13.8 us, the gate
-// of 16 x 2048 x 16384 13.2 and 13.9); then come the tiles, each while the CUs have
-// one of them.
-// us of the five, weights in cache: 64 x 1024 x 4480 4.8, 4.4, 8.5, 11.3, 16.3; 256 rows
-// 9.3, 8.9, 8.9, 11.7, 16.7; 768 rows 20.6, 17.5, 11.3, 12.5, 17.4; 4096 rows 39.5, 41.8, 40.6 (tiles);
-// 256 x 4096 x 4096 17.5, 14.0, 26, 35, 53; 1024 rows -, 47, 37, 39, 54; 4096 rows 129, 116, 104 (tiles). The
-// same borders do for short sums: 64 x 1024 x 4480 4.4, 4.0, 5.4, 6.7, 9.3; 256 rows 8.2, 7.3, 5.6, 7.0, 9.8; 768
-// rows 18.1, 14.1, 8.1, 7.8, 10.5; 4096 rows 25, 25, 23.6 (tiles).
+// at any width (half of a tile of 32 would be empty: 16 x 2048 x 32000 12.4 and 13.8 us, the gate of 16 x 2048 x
+// 16384 13.2 and 13.9); then come the tiles, each while the CUs have one of them. us of the five, weights in
+// cache: 64 x 1024 x 4480 4.8, 4.4, 8.5, 11.3, 16.3; 256 rows 9.3, 8.9, 8.9, 11.7, 16.7; 768 rows 20.6, 17.5, 11.3,
+// 12.5, 17.4; 4096 rows 39.5, 41.8, 40.6 (tiles); 256 x 4096 x 4096 17.5, 14.0, 26, 35, 53; 1024 rows -, 47, 37, 39,
+// 54; 4096 rows 129, 116, 104 (tiles). The same borders do for short sums: 64 x 1024 x 4480 4.4, 4.0, 5.4, 6.7,
+// 9.3; 256 rows 8.2, 7.3, 5.6, 7.0, 9.8; 768 rows 18.1, 14.1, 8.1, 7.8, 10.5; 4096 rows 25, 25, 23.6 (tiles).
 M3S_BOTH Form8 form8(int64_t rows, int64_t np) {
   const int64_t g64 = np / 64, g128 = (np + 127) / 128, g256 = (np + 255) / 256, r64 = (rows + 63) / 64;
   if (rows <= 16 || g64 * ((rows + 15) / 16) <= 256) return kFew16;
@@ -55,9 +53,9 @@ M3S_BOTH bool rounds_in_launch(int64_t rows, int64_t np, int64_t k, int size) {
 // and go nowhere then.
 M3S_BOTH int step_within(int s, int S) { return s < S ? s : 0; }
 
-// The weight's scales are a dword for every step of 128 k, group of 64 packed outputs and lane. The byte of
-// a group's dword in a step for a lane that takes entry 16 g + r (g < 2: the blocks of a step of 64 k); a group behind the last of `groups` reads the
-// last one instead, as its tiles do, and is not stored.
+// The weight's scales are a dword for every step of 128 k, group of 64 packed outputs and lane. The byte of a
+// group's dword in a step for a lane that takes entry 16 g + r (g < 2: the blocks of a step of 64 k); a group
+// behind the last of `groups` reads the last one instead, as its tiles do, and is not stored.
 M3S_BOTH uint32_t weight_scale_at(int group, int groups, int entry) {
   return (uint32_t)(group < groups ? group : groups - 1) * 256 + 4 * entry;
 }

@@ -58,12 +58,13 @@ def test_products_sum_in_float32(T, rows, k, n):
 
 
 @pytest.mark.parametrize("rows,k,n", [(3, 333, 130), (40, 333, 130), (700, 333, 1100)])
-@pytest.mark.parametrize("e", [-118, 118])
-def test_float32_sums_over_the_scales(T, rows, k, n, e):
-    """Rows near either end of float32 beside weights near the other one: bf16 holds both."""
+@pytest.mark.parametrize("e,f", [(-118, 118), (118, -118), (-130, 118)])
+def test_float32_sums_over_the_scales(T, rows, k, n, e, f):
+    """Rows near either end of float32 beside weights near the other one: bf16 holds both, below its normal
+    values (from 2^-126) too."""
     x, w = whole_numbers(rows, k, n)
-    got = T.matmul8((x * 2.0 ** e).float().cuda(), T.pack8((w * 2.0 ** -e).float().cuda()))
-    same(got, (x @ w).to(BF16).double())
+    got = T.matmul8((x * 2.0 ** e).float().cuda(), T.pack8((w * 2.0 ** f).float().cuda()))
+    same(got, (x @ w).to(BF16).double() * 2.0 ** (e + f))
 
 
 GATES = [(1, 2048, 5632), (7, 515, 330), (40, 1000, 320), (300, 300, 2048), (450, 260, 1155), (1100, 520, 1000),
